@@ -1,0 +1,542 @@
+// Log-probabilities of given tokens with their rank, the entropy of the
+// distribution and its largest entries (sm_100a).
+//
+// For a row of logits x, temperature T and a token t, with y = x / T:
+//   logprob = y_t - log sum_j exp(y_j)
+//   entropy = -sum_j p_j log p_j = log z - (sum_j (y_j - m) exp(y_j - m)) / z,
+//             z = sum_j exp(y_j - m), m = max y: both terms are >= 0, nothing
+//             cancels
+//   rank    = 1 + #{j : x_j > x_t} + #{j < t : x_j = x_t}
+//   top n   = the n first entries by (x falling, id rising)
+// A NaN counts as the largest value, -0 equals +0.  The sampling kernels of
+// the verify round give a token and its probability after top-k / top-p; a
+// caller that ranks samples needs the untruncated log-probabilities.
+//
+// One pass over the logits.  A row is cut into parts of up to LP_UNITS 16-byte
+// units per thread, held in registers: a part's loads are all in flight at
+// once and its elements are looked at twice (maximum, then sums) without a
+// second read.  logp_part_kernel leaves per part the partial sums in base 2
+// relative to the part's maximum, the count of elements ahead of the token,
+// and the part's top n as sorted 64-bit keys (value key, complement of the
+// id); logp_rows_kernel (a programmatic dependent launch) joins a row's parts
+// in part order.  No atomics reach a result: the list below is filled in any
+// order and then ranked by unique keys.
+//
+// Top n of a part without comparing every element: with M_w the thread maxima
+// of warp w, T = max(max_w (n-th largest of M_w), min_w (ceil(n/8)-th largest
+// of M_w)) has at least n elements at or above it, and few more; only threads
+// whose maximum reaches T look through their registers again.
+#include <cuda_runtime.h>
+#include <math_constants.h>
+
+#include <algorithm>
+#include <cfloat>
+
+#include "sd_common.cuh"
+
+namespace sd {
+
+constexpr int LP_THREADS = 256;
+constexpr int LP_WARPS = LP_THREADS / 32;
+constexpr int LP_UNITS = 16;                    // 16-byte units per thread and part
+constexpr int LP_LIST = 4096;                   // >= SD_TOPN_MAX * 8 * LP_UNITS, >= parts * n
+static_assert(LP_LIST >= SD_TOPN_MAX * 8 * LP_UNITS, "a part's list holds every flagged element");
+static_assert(SD_LOGPROBS_MAX_V / (4 * LP_UNITS * LP_THREADS) + 2 <= LP_LIST / SD_TOPN_MAX,
+              "a row's lists fit the join's list");
+static_assert(SD_TOPN_MAX <= 32, "the n-th largest thread maximum of one warp");
+constexpr int LP_ROW_THREADS = 128;
+
+struct LpPart {
+  float m, s, e;                                // max (logit units), sum 2^d, sum d 2^d
+  int ahead;                                    // elements at or ahead of the token
+};
+
+struct LpParams {
+  const void* x;
+  int64_t bs, ps;
+  const int64_t* ids;
+  int64_t ids_bs;
+  int B, L, V, top, parts, dtype;
+  float temperature, c;                         // c = log2(e) / temperature
+  float* logprob;
+  int64_t* rank;
+  float* entropy;
+  int64_t* top_ids;
+  float* top_lp;
+  LpPart* part;
+  unsigned long long* keys;                     // [rows][parts][top]
+};
+
+__device__ __forceinline__ float lp_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 32-bit order key: NaN (either sign) largest, -0 = +0; 0 is no value's key.
+__device__ __forceinline__ uint32_t lp_key(float f) {
+  return f != f ? 0xFFFFFFFFu : fkey(f);
+}
+// An exponent held at or above -256, where 2^x is 0: an element far below the
+// maximum (-inf, or a mask of the type's lowest value) then adds 0 * -256 to
+// the entropy sum, not 0 * -inf.  A NaN stays.
+__device__ __forceinline__ float lp_hold(float x) { return x < -256.f ? -256.f : x; }
+__device__ __forceinline__ float lp_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+}
+
+// A 16-byte unit of the logits' type: E elements.
+template <typename T> struct Unit;
+template <> struct Unit<__nv_bfloat16> {
+  static constexpr int E = 8;
+  __device__ static float get(const uint4& u, int e) {
+    const uint32_t w = e < 2 ? u.x : e < 4 ? u.y : e < 6 ? u.z : u.w;
+    return __uint_as_float((e & 1) ? (w & 0xFFFF0000u) : (w << 16));
+  }
+  __device__ static uint32_t bits(const __nv_bfloat16* p) {
+    return *reinterpret_cast<const unsigned short*>(p);
+  }
+  static constexpr uint32_t NEG_INF = 0xFF80u;
+};
+template <> struct Unit<__half> {
+  static constexpr int E = 8;
+  __device__ static float get(const uint4& u, int e) {
+    const uint32_t w = e < 2 ? u.x : e < 4 ? u.y : e < 6 ? u.z : u.w;
+    return __half2float(__ushort_as_half((unsigned short)((e & 1) ? (w >> 16) : (w & 0xFFFFu))));
+  }
+  __device__ static uint32_t bits(const __half* p) {
+    return *reinterpret_cast<const unsigned short*>(p);
+  }
+  static constexpr uint32_t NEG_INF = 0xFC00u;
+};
+template <> struct Unit<float> {
+  static constexpr int E = 4;
+  __device__ static float get(const uint4& u, int e) {
+    return __uint_as_float(e == 0 ? u.x : e == 1 ? u.y : e == 2 ? u.z : u.w);
+  }
+  __device__ static uint32_t bits(const float* p) { return __float_as_uint(*p); }
+  static constexpr uint32_t NEG_INF = 0xFF800000u;
+};
+
+// Elements [i0, i0 + E) of a row of V elements; those outside [0, V) are -inf.
+// Whole units are one 16-byte load (the unit grid is the row's 16-byte grid).
+template <typename T>
+__device__ __forceinline__ uint4 load_unit(const T* row, int i0, int V) {
+  constexpr int E = Unit<T>::E;
+  if (i0 >= 0 && i0 + E <= V) return __ldcs(reinterpret_cast<const uint4*>(row + i0));
+  uint32_t w[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (E == 4) {
+      const int i = i0 + q;
+      w[q] = (i >= 0 && i < V) ? Unit<T>::bits(row + i) : Unit<T>::NEG_INF;
+    } else {
+      const int i = i0 + 2 * q;
+      const uint32_t lo = (i >= 0 && i < V) ? Unit<T>::bits(row + i) : Unit<T>::NEG_INF;
+      const uint32_t hi = (i + 1 >= 0 && i + 1 < V) ? Unit<T>::bits(row + i + 1) : Unit<T>::NEG_INF;
+      w[q] = lo | (hi << 16);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The n largest of the cnt unique keys in `list` (shared memory), in falling
+// order, to out[0..n): all threads of the block call it.  cnt <= LP_LIST;
+// slots past cnt keys are 0.  A long list is first cut to its n largest by
+// finding the n-th key bit by bit.
+template <int THREADS>
+__device__ void sort_top(unsigned long long* list, int cnt, int n, unsigned long long* out,
+                         int* counter) {
+  const int t = threadIdx.x;
+  if (cnt > 2 * THREADS) {
+    unsigned long long nth = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const unsigned long long cand = nth | (1ULL << bit);
+      int c = 0;
+      for (int i0 = 0; i0 < cnt; i0 += THREADS)
+        c += __syncthreads_count(i0 + t < cnt && list[i0 + t] >= cand);
+      if (c >= n) nth = cand;
+    }
+    // the n keys >= nth move to the front, a block of THREADS at a time
+    int kept = 0;
+    for (int i0 = 0; i0 < cnt; i0 += THREADS) {
+      const unsigned long long k = i0 + t < cnt ? list[i0 + t] : 0ULL;
+      __syncthreads();                               // everybody has read its key
+      if (t == 0) *counter = kept;
+      __syncthreads();
+      if (k >= nth && k != 0ULL) list[atomicAdd(counter, 1)] = k;   // at most i0 + THREADS so far
+      __syncthreads();
+      kept = *counter;
+    }
+    cnt = kept;
+    __syncthreads();
+  }
+  for (int i = t; i < cnt; i += THREADS) {
+    const unsigned long long k = list[i];
+    int r = 0;
+    for (int j = 0; j < cnt; ++j) r += list[j] > k;
+    if (r < n) out[r] = k;
+  }
+  for (int i = cnt + t; i < n; i += THREADS) out[i] = 0ULL;
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(LP_THREADS, 2) logp_part_kernel(const LpParams P) {
+  constexpr int E = Unit<T>::E;
+  extern __shared__ __align__(16) unsigned char lp_smem[];
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(lp_smem);   // TOP only
+  __shared__ float red_m[LP_WARPS], red_s[LP_WARPS], red_e[LP_WARPS];
+  __shared__ int red_c[LP_WARPS];
+  __shared__ uint32_t kth[LP_WARPS], jth[LP_WARPS];
+  __shared__ unsigned long long uth[LP_WARPS];
+  __shared__ int n_list, counter;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+  const int64_t item = blockIdx.x;
+  const int64_t r = item / P.parts;
+  const int part = (int)(item % P.parts);
+  const int64_t rb = r / P.L, rl = r % P.L;
+  const T* row = reinterpret_cast<const T*>(P.x) + rb * P.bs + rl * P.ps;
+  const int V = P.V;
+  // the row's 16-byte grid: unit u holds elements [u * E - head, ...)
+  const int head = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+  const int units = (int)(((int64_t)V + head + E - 1) / E);
+  const int per = (units + P.parts - 1) / P.parts;   // <= LP_THREADS * LP_UNITS
+  const int u0 = min(part * per, units), u1 = min(u0 + per, units);
+  if (t == 0) n_list = 0;
+
+  const int64_t tok = P.ids[rb * P.ids_bs + rl];
+  const bool have = tok >= 0 && tok < V;
+  uint4 d[LP_UNITS];
+#pragma unroll
+  for (int i = 0; i < LP_UNITS; ++i) {
+    const int u = u0 + i * LP_THREADS + t;
+    if (u < u1) {
+      d[i] = load_unit<T>(row, u * E - head, V);
+    } else {
+      constexpr uint32_t ni = E == 4 ? Unit<T>::NEG_INF : Unit<T>::NEG_INF * 0x10001u;
+      d[i] = make_uint4(ni, ni, ni, ni);
+    }
+  }
+  const float xt = have ? load_logit(P.x, P.dtype, rb * P.bs + rl * P.ps + tok) : 0.f;
+  // thread maximum; a NaN wins
+  float m = -CUDART_INF_F;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < LP_UNITS; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float v = Unit<T>::get(d[i], e);
+      m = fmaxf(m, v);
+      nan |= v != v;
+    }
+  // sums in base 2 relative to the thread's maximum
+  const float m0 = m == -CUDART_INF_F ? 0.f : m;
+  float s = 0.f, es = 0.f;
+  int ahead = 0;
+  const uint32_t kt = lp_key(xt);
+#pragma unroll
+  for (int i = 0; i < LP_UNITS; ++i) {
+    const int u = u0 + i * LP_THREADS + t;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float v = Unit<T>::get(d[i], e);
+      const float dd = lp_hold((v - m0) * P.c);
+      const float p = lp_ex2(dd);
+      s += p;
+      es = fmaf(dd, p, es);
+    }
+    if (u < u1) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int idx = u * E - head + e;
+        const uint32_t k = lp_key(Unit<T>::get(d[i], e));
+        ahead += (idx >= 0 && idx < V) && (k > kt || (k == kt && idx <= tok));
+      }
+    }
+  }
+  // join over the block: the maxima first, then the sums at the block's maximum
+  float bm = warp_max(m);
+  if (lane == 0) red_m[w] = bm;
+  if (TOP) {
+    // this warp's sorted thread maxima (bitonic over lanes, falling)
+    uint32_t k = nan ? 0xFFFFFFFFu : lp_key(m);
+    if (u0 + t >= u1) k = 0u;                        // no unit at all
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+      for (int st = size >> 1; st > 0; st >>= 1) {
+        const uint32_t o = __shfl_xor_sync(0xffffffffu, k, st);
+        const bool up = ((lane & size) == 0) == ((lane & st) == 0);
+        k = up ? max(k, o) : min(k, o);
+      }
+    const int j = (P.top + LP_WARPS - 1) / LP_WARPS;
+    if (lane == P.top - 1) kth[w] = k;
+    if (lane == j - 1) jth[w] = k;
+  }
+  __syncthreads();
+  bm = red_m[0];
+#pragma unroll
+  for (int q = 1; q < LP_WARPS; ++q) bm = fmaxf(bm, red_m[q]);
+  const float dm = lp_hold((m - bm) * P.c), f = lp_ex2(dm);
+  float s2 = f * s, es2 = f * fmaf(dm, s, es);
+  if (m == -CUDART_INF_F) s2 = es2 = 0.f;            // nothing above -inf
+  if (nan) s2 = CUDART_NAN_F;
+  s2 = warp_sum(s2);
+  es2 = warp_sum(es2);
+  ahead = warp_sum(ahead);
+  if (lane == 0) {
+    red_s[w] = s2;
+    red_e[w] = es2;
+    red_c[w] = ahead;
+  }
+  if (TOP) {
+    uint32_t T1 = 0, T2 = 0xFFFFFFFFu;
+#pragma unroll
+    for (int q = 0; q < LP_WARPS; ++q) {
+      T1 = max(T1, kth[q]);
+      T2 = min(T2, jth[q]);
+    }
+    const uint32_t thr = max(max(T1, T2), 1u);
+    const uint32_t km = nan ? 0xFFFFFFFFu : lp_key(m);
+    if (km >= thr && u0 + t < u1) {
+#pragma unroll
+      for (int i = 0; i < LP_UNITS; ++i) {
+        const int u = u0 + i * LP_THREADS + t;
+        if (u < u1) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const int idx = u * E - head + e;
+            const uint32_t k = lp_key(Unit<T>::get(d[i], e));
+            if (k >= thr && idx >= 0 && idx < V) {
+              const int at = atomicAdd(&n_list, 1);
+              if (at < LP_LIST)
+                list[at] = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)idx;
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+    int cnt = n_list;
+    if (cnt > LP_LIST) {
+      // Many elements equal the threshold (flat logits).  Again with the keys
+      // (value, first unit that reaches it) of the threads: unique, so at
+      // most n threads reach the n-th of them, with E * LP_UNITS elements each.
+      unsigned long long uk = 0ULL;
+#pragma unroll
+      for (int i = 0; i < LP_UNITS; ++i) {
+        const int u = u0 + i * LP_THREADS + t;
+        if (u < u1) {
+          uint32_t k = 0;
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const int idx = u * E - head + e;
+            if (idx >= 0 && idx < V) k = max(k, lp_key(Unit<T>::get(d[i], e)));
+          }
+          const unsigned long long q = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)u;
+          uk = q > uk ? q : uk;
+        }
+      }
+      __syncthreads();
+      list[t] = uk;
+      if (t == 0) n_list = 0;
+      __syncthreads();
+      int ahead_of = 0;
+      for (int q = 0; q < LP_THREADS; ++q) ahead_of += list[q] > uk;
+      if (ahead_of == P.top - 1 && uk != 0ULL) uth[0] = uk;   // exactly one such thread, or fewer keys
+      if (t == 0) counter = 0;
+      __syncthreads();
+      if (uk != 0ULL) atomicAdd(&counter, 1);
+      __syncthreads();
+      const unsigned long long ut = counter >= P.top ? uth[0] : 1ULL;
+      __syncthreads();
+      if (uk >= ut) {
+#pragma unroll
+        for (int i = 0; i < LP_UNITS; ++i) {
+          const int u = u0 + i * LP_THREADS + t;
+          if (u < u1) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const int idx = u * E - head + e;
+              const uint32_t k = lp_key(Unit<T>::get(d[i], e));
+              const unsigned long long q = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)u;
+              if (idx >= 0 && idx < V && q >= ut) {
+                const int at = atomicAdd(&n_list, 1);
+                if (at < LP_LIST)
+                  list[at] = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)idx;
+              }
+            }
+          }
+        }
+      }
+      __syncthreads();
+      cnt = min(n_list, LP_LIST);
+      __syncthreads();
+    }
+    sort_top<LP_THREADS>(list, cnt, P.top, P.keys + item * P.top, &counter);
+  } else {
+    __syncthreads();
+  }
+  if (t == 0) {
+    LpPart o;
+    o.m = bm;
+    o.s = 0.f;
+    o.e = 0.f;
+    o.ahead = 0;
+#pragma unroll
+    for (int q = 0; q < LP_WARPS; ++q) {
+      o.s += red_s[q];
+      o.e += red_e[q];
+      o.ahead += red_c[q];
+    }
+    P.part[item] = o;
+  }
+}
+
+// One CTA per row: the parts' sums at the row's maximum, the token, the
+// entropy, and the row's top n from the parts' lists.
+__global__ void __launch_bounds__(LP_ROW_THREADS) logp_rows_kernel(const LpParams P) {
+  extern __shared__ __align__(16) unsigned char lp_smem[];
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(lp_smem);   // [parts * top]
+  __shared__ float sh_m, sh_lz;
+  __shared__ int counter;
+  __shared__ unsigned long long best[SD_TOPN_MAX];
+  const int t = threadIdx.x;
+  const int64_t r = blockIdx.x, rb = r / P.L, rl = r % P.L;
+  const int64_t tok = P.ids[rb * P.ids_bs + rl];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const LpPart* part = P.part + r * P.parts;
+  if (t < 32) {
+    float m = -CUDART_INF_F;
+    for (int i = t; i < P.parts; i += 32) m = fmaxf(m, part[i].m);
+    m = warp_max(m);
+    float s = 0.f, e = 0.f;
+    int ahead = 0;
+    for (int i = t; i < P.parts; i += 32) {
+      const LpPart q = part[i];
+      ahead += q.ahead;
+      if (q.m == -CUDART_INF_F && q.s == q.s) continue;          // nothing finite, no NaN
+      const float dm = lp_hold((q.m - m) * P.c), f = lp_ex2(dm);
+      s = fmaf(f, q.s, s);
+      e = fmaf(f, fmaf(dm, q.s, q.e), e);
+    }
+    s = warp_sum(s);
+    e = warp_sum(e);
+    ahead = warp_sum(ahead);
+    if (t == 0) {
+      const float lz = logf(s);
+      sh_m = m;
+      sh_lz = lz;
+      const bool none = !(m > -CUDART_INF_F);                    // every entry is -inf
+      const bool have = tok >= 0 && tok < P.V;
+      P.entropy[r] = none || m == CUDART_INF_F ? CUDART_NAN_F
+                                               : lz - 0.69314718055994531f * (e / s);
+      P.rank[r] = have ? (int64_t)ahead : 0;
+      float lp = CUDART_NAN_F;
+      if (have && !none)
+        lp = __fdiv_rn(load_logit(P.x, P.dtype, rb * P.bs + rl * P.ps + tok) - m, P.temperature) - lz;
+      P.logprob[r] = lp;
+    }
+  }
+  __syncthreads();
+  if (P.top == 0) return;
+  const unsigned long long* keys = P.keys + r * P.parts * P.top;
+  const int all = P.parts * P.top;
+  for (int i = t; i < all; i += LP_ROW_THREADS) list[i] = keys[i];
+  __syncthreads();
+  sort_top<LP_ROW_THREADS>(list, all, P.top, best, &counter);
+  __syncthreads();
+  if (t < P.top) {
+    const unsigned long long k = best[t];
+    const float v = lp_value((uint32_t)(k >> 32));
+    P.top_ids[r * P.top + t] = (int64_t)(uint32_t)~(uint32_t)k;
+    P.top_lp[r * P.top + t] = __fdiv_rn(v - sh_m, P.temperature) - sh_lz;
+  }
+}
+
+static int lp_parts(int64_t rows, int V, int dtype) {
+  const int E = dtype == SD_DTYPE_F32 ? 4 : 8;
+  // a row that starts off the 16-byte grid covers one unit more
+  const int64_t units = ((int64_t)V + 2 * E - 2) / E;
+  const int64_t least = (units + LP_THREADS * LP_UNITS - 1) / (LP_THREADS * LP_UNITS);
+  const int64_t most = std::min<int64_t>((units + LP_THREADS - 1) / LP_THREADS, 64);
+  // few rows: parts of fewer units, so that two CTAs land on every SM
+  const int64_t fill = (2 * 148 + rows - 1) / rows;
+  return (int)std::max(least, std::min(most, fill));
+}
+
+template <typename T>
+static int launch_logprobs(const LpParams& P, cudaStream_t st) {
+  const int64_t rows = (int64_t)P.B * P.L;
+  const dim3 grid((unsigned)(rows * P.parts));
+  if (P.top > 0)
+    logp_part_kernel<T, true><<<grid, LP_THREADS, LP_LIST * sizeof(unsigned long long), st>>>(P);
+  else
+    logp_part_kernel<T, false><<<grid, LP_THREADS, 0, st>>>(P);
+  if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows);
+  cfg.blockDim = dim3(LP_ROW_THREADS);
+  cfg.dynamicSmemBytes = (size_t)P.parts * P.top * sizeof(unsigned long long);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, logp_rows_kernel, P) != cudaSuccess) return SD_ELAUNCH;
+  return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
+}
+
+}  // namespace sd
+
+using namespace sd;
+
+extern "C" {
+
+size_t sd_token_logprobs_workspace_bytes(int B, int L, int V, int dtype, int top_n) {
+  if (B <= 0 || L <= 0 || V <= 0 || V > SD_LOGPROBS_MAX_V || top_n < 0 || top_n > SD_TOPN_MAX)
+    return 0;
+  const int64_t rows = (int64_t)B * L;
+  const size_t items = (size_t)rows * lp_parts(rows, V, dtype);
+  return items * (sizeof(LpPart) + (size_t)top_n * sizeof(unsigned long long));
+}
+
+int sd_token_logprobs(const void* logits, int64_t bs, int64_t ps, int dtype, const int64_t* ids,
+                      int64_t ids_bs, int B, int L, int V, float temperature, int top_n,
+                      float* logprob, int64_t* rank, float* entropy, int64_t* top_ids,
+                      float* top_logprobs, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+  if (B < 0 || L < 0) return SD_EINVAL;
+  if (B == 0 || L == 0) return SD_OK;
+  if (!logits || !ids || !logprob || !rank || !entropy || V <= 0) return SD_EINVAL;
+  if (dtype != SD_DTYPE_F32 && dtype != SD_DTYPE_F16 && dtype != SD_DTYPE_BF16) return SD_EINVAL;
+  if (!(temperature > 0.f) || temperature > FLT_MAX) return SD_EINVAL;
+  if (top_n < 0 || top_n > V || (top_n > 0 && (!top_ids || !top_logprobs))) return SD_EINVAL;
+  const int64_t rows = (int64_t)B * L;
+  if (V > SD_LOGPROBS_MAX_V || top_n > SD_TOPN_MAX) return SD_ENOTSUP;
+  const int parts = lp_parts(rows, V, dtype);
+  if (rows * parts > 0x7FFFFFFF) return SD_ENOTSUP;
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == SD_DTYPE_F32 ? 4 : 2)) return SD_EINVAL;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+      workspace_bytes < sd_token_logprobs_workspace_bytes(B, L, V, dtype, top_n))
+    return SD_ENOSPC;
+  LpParams P;
+  P.x = logits; P.bs = bs; P.ps = ps; P.dtype = dtype;
+  P.ids = ids; P.ids_bs = ids_bs;
+  P.B = B; P.L = L; P.V = V; P.top = top_n; P.parts = parts;
+  P.temperature = temperature;
+  P.c = (float)(1.4426950408889634 / (double)temperature);
+  P.logprob = logprob; P.rank = rank; P.entropy = entropy;
+  P.top_ids = top_ids; P.top_lp = top_logprobs;
+  // keys first: both arrays then sit on their own alignment
+  P.keys = reinterpret_cast<unsigned long long*>(workspace);
+  P.part = reinterpret_cast<LpPart*>(P.keys + (size_t)rows * parts * top_n);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == SD_DTYPE_BF16) return launch_logprobs<__nv_bfloat16>(P, st);
+  if (dtype == SD_DTYPE_F16) return launch_logprobs<__half>(P, st);
+  return launch_logprobs<float>(P, st);
+}
+
+}  // extern "C"

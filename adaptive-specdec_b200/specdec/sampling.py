@@ -7,7 +7,11 @@ meaning and output dtypes, plus the two fused entry points the engine uses:
 * ``verify_sample`` -- one launch sequence for engine.py:282-303: to_probs on
   the k+1 target and k draft vectors, the accept test, and the residual or
   bonus draw;
-* ``draft_sample``  -- one draft step, engine.py:250-251 and :256.
+* ``draft_sample``  -- one draft step, engine.py:250-251 and :256;
+
+and ``token_logprobs`` (no counterpart in the reference): log-probability, rank
+and entropy for given tokens, with the largest alternatives, for callers that
+rank several samples of one prompt.
 
 Draws are inverse-CDF with uniforms: either passed in (``u=...``) or drawn
 from ``generator`` on the device.  Given the same uniforms, results match the
@@ -17,12 +21,18 @@ Tie rule at the top-p boundary: among equal probabilities, lower vocabulary
 index first (the reference's ``torch.sort`` is unstable, so any order is a
 valid reading of it; this one is deterministic).
 """
+from typing import NamedTuple, Optional
+
 import torch
 
 from specdec import _lib as L
 
 __all__ = ["to_probs", "sample_from_probs", "residual_probs", "gather_prob",
-           "verify_sample", "verify_sample_probs", "draft_sample"]
+           "verify_sample", "verify_sample_probs", "draft_sample", "TokenLogprobs",
+           "token_logprobs"]
+
+TOP_N_MAX = 32             # SD_TOPN_MAX
+LOGPROBS_MAX_V = 1 << 20   # SD_LOGPROBS_MAX_V
 
 
 def _knobs(temperature, top_p, top_k):
@@ -238,3 +248,71 @@ def draft_sample(logits, u, temperature=1.0, top_p=1.0, top_k=0):
                                     L.ptr(x), L.ptr(qx), L.ptr(ws), ws.numel(),
                                     L.stream_ptr(x2.device)), "draft_sample")
     return x, qx
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` returns (shapes: those of ``ids``; top_* have one
+    more dimension of top_n entries and are None without alternatives)."""
+    logprob: torch.Tensor                   # float32
+    rank: torch.Tensor                      # int64, 1 = the largest logit
+    entropy: torch.Tensor                   # float32, natural log
+    top_ids: Optional[torch.Tensor]         # int64
+    top_logprobs: Optional[torch.Tensor]    # float32
+
+
+def token_logprobs(logits, ids, temperature=1.0, top_n=0):
+    """Log-probabilities of ``ids`` under softmax(logits / temperature).
+
+    logits [..., V] (bf16 / fp16 / fp32, vocabulary contiguous, other strides
+    free up to three dimensions), ids [...] integer.  Per position: the
+    token's log-probability, its rank by (logit falling, id rising; 1 = first),
+    the entropy of the distribution, and with ``top_n`` > 0 the first top_n ids
+    in that order with their log-probabilities.  No top-p / top-k applies.  An
+    id outside [0, V) (padding) gets logprob NaN and rank 0.  A row with a NaN or
+    a +inf, or with nothing above -inf, has NaN log-probabilities and entropy.
+    One pass over the logits (sd_token_logprobs), no host synchronisation.
+    """
+    L.require_cuda(logits, ids)
+    if logits.dim() < 1 or tuple(ids.shape) != tuple(logits.shape[:-1]):
+        raise L.SpecdecError(f"token_logprobs needs one id per row: logits {tuple(logits.shape)}, "
+                             f"ids {tuple(ids.shape)}")
+    if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+        raise L.SpecdecError(f"ids must be integers, got {ids.dtype}")
+    if ids.device != logits.device:
+        raise L.SpecdecError("logits and ids must be on one device")
+    code = L.dtype_code(logits.dtype)
+    V = logits.shape[-1]
+    n = int(top_n)
+    if not 0 <= n <= min(V, TOP_N_MAX):
+        raise L.SpecdecError(f"top_n must be between 0 and min(V, {TOP_N_MAX}), got {n}")
+    if not 1 <= V <= LOGPROBS_MAX_V:
+        raise L.SpecdecError(f"the vocabulary must have 1 to {LOGPROBS_MAX_V} entries, got {V}")
+    T = float(temperature)
+    if not 0.0 < T < float("inf"):
+        raise L.SpecdecError(f"temperature must be positive and finite, got {temperature}")
+    x = logits if V == 1 else _vocab_rows(logits, "logits")
+    x = x.reshape(-1, V) if x.dim() > 3 else x.reshape(1, V) if x.dim() == 1 else x
+    x = x.unsqueeze(1) if x.dim() == 2 else x
+    if x.stride(-1) != 1:
+        x = x.contiguous()
+    B, Lr = x.shape[0], x.shape[1]
+    tok = ids.long().reshape(B, Lr)
+    if tok.stride(-1) != 1:
+        tok = tok.contiguous()
+    dev, shape = x.device, tuple(ids.shape)
+    logprob = torch.empty(shape, dtype=torch.float32, device=dev)
+    rank = torch.empty(shape, dtype=torch.long, device=dev)
+    entropy = torch.empty(shape, dtype=torch.float32, device=dev)
+    top_ids = torch.empty(shape + (n,), dtype=torch.long, device=dev) if n else None
+    top_lp = torch.empty(shape + (n,), dtype=torch.float32, device=dev) if n else None
+    lib = L.lib()
+    with torch.cuda.device(dev):
+        # a fresh buffer per call: calls on several streams and calls captured
+        # into different graphs never share one
+        ws = torch.empty(lib.sd_token_logprobs_workspace_bytes(B, Lr, V, code, n),
+                         dtype=torch.uint8, device=dev)
+        L.check(lib.sd_token_logprobs(L.ptr(x), x.stride(0), x.stride(1), code, L.ptr(tok),
+                                      tok.stride(0), B, Lr, V, T, n, L.ptr(logprob), L.ptr(rank),
+                                      L.ptr(entropy), L.ptr(top_ids), L.ptr(top_lp), L.ptr(ws),
+                                      ws.numel(), L.stream_ptr(dev)), "token_logprobs")
+    return TokenLogprobs(logprob, rank, entropy, top_ids, top_lp)

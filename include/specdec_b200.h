@@ -173,6 +173,31 @@ int sd_sample_from_probs(const float* probs, int n_rows, int V, const float* u,
 int sd_gather_prob(const float* probs, int n_rows, int V, const int64_t* ids, float* out,
                    void* stream);
 
+/*
+ * No counterpart in the reference (added entry point): the log-probabilities
+ * of given tokens under softmax(logits / temperature) over the whole
+ * vocabulary (no top-p / top-k), as a caller that ranks several samples of a
+ * prompt needs beside the verify round's tokens.  Per row [b, l]:
+ *   logprob[b, l] = x_t / T - log sum_j exp(x_j / T),   t = ids[b, l]
+ *   rank[b, l]    = 1 + #{j : x_j > x_t} + #{j < t : x_j = x_t}
+ *   entropy[b, l] = -sum_j p_j log p_j  (natural log)
+ *   top_ids / top_logprobs[b, l, 0..top_n): the first entries by (logit
+ *                   falling, id rising), top_n <= min(V, SD_TOPN_MAX)
+ * logits [B, L, V] of `dtype` (element strides (bs, ps, 1)), ids [B, L] int64
+ * (row stride ids_bs); outputs contiguous.  An id outside [0, V) (a padding
+ * position) gets logprob NaN and rank 0; its row's other outputs are as for
+ * any id.  -inf entries have probability 0.  A row with a NaN or a +inf, or
+ * with nothing above -inf, has NaN log-probabilities and entropy (as the
+ * formula); its rank and top_ids still follow the logits, NaN first.
+ */
+#define SD_TOPN_MAX 32
+#define SD_LOGPROBS_MAX_V (1 << 20)
+size_t sd_token_logprobs_workspace_bytes(int B, int L, int V, int dtype, int top_n);
+int sd_token_logprobs(const void* logits, int64_t bs, int64_t ps, int dtype, const int64_t* ids,
+                      int64_t ids_bs, int B, int L, int V, float temperature, int top_n,
+                      float* logprob, int64_t* rank, float* entropy, int64_t* top_ids,
+                      float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- ragged KV cache (reference specdec/kvcache.py) --------------------- */
 
 /*
