@@ -39,6 +39,10 @@ _SIGNATURES = {
     "sd_token_logprobs_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32], _sz),
     "sd_token_logprobs": ([_vp, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _f32, _i32, _vp,
                            _vp, _vp, _vp, _vp, _vp, _sz, _vp], _i32),
+    "sd_pages_workspace_bytes": ([_i32], _sz),
+    "sd_pages_reserve": ([_vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _i64,
+                          _vp, _vp, _vp, _sz, _vp], _i32),
+    "sd_pages_trim": ([_vp, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp], _i32),
     "sd_kv_lengths_update": ([_vp, _vp, _i64, _i32, _i32, _i64, _vp, _vp], _i32),
     "sd_qkv_norm_rope_append": ([_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _f32, _vp, _vp, _i64,
                                  _i64, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _i32,

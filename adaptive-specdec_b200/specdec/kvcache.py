@@ -28,7 +28,10 @@ indistinguishable from one that only ever processed the accepted prefix.
 ``PagedRaggedCache`` keeps the same interface over pages of PAGE tokens
 drawn from one pool per layer, so that memory follows each row's own length
 rather than the widest row's (the reference pads every row to the capacity,
-kvcache.py:98-116).
+kvcache.py:98-116).  Its page bookkeeping runs on the host (``PageTable``) or, with
+``device_pages=True``, on the device (``DevicePageTable``): pages then follow the
+device lengths without a host copy of them, and ``fork`` makes several rows of
+one prompt that share its pages.
 """
 import numpy as np
 import torch
@@ -36,7 +39,7 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 
 from specdec import _lib as L
 
-__all__ = ["RaggedCache", "PagedRaggedCache", "PAGE"]
+__all__ = ["RaggedCache", "PagedRaggedCache", "DevicePageTable", "PAGE"]
 
 PAGE = 128            # tokens per page (SD_KV_PAGE): one K/V tile of the verify attention
 
@@ -422,6 +425,138 @@ class PageTable:
         for b in range(self.B):
             o = int(self.owned[b])
             assert (self.bt[b, :o] >= 0).all() and (self.bt[b, :o] != self.sink).all()
+
+
+class DevicePageTable:
+    """Page bookkeeping on the device: PageTable's page order, by device lengths.
+
+    ``block_table`` [B, W] int32 (-1 = none), ``owned`` [B] pages of each row,
+    ``shared`` [B] leading pages that the row reads but does not give back,
+    ``free`` [n_pages] a stack of ``n_free`` [1] free pages, ``err`` [1] sticky
+    error bits.  ``reserve`` and ``trim`` are stream ordered, never
+    synchronise the host and can be captured into CUDA graphs; a call that
+    cannot serve every row changes nothing and sets bits of ``err``
+    (``check_errors``).  The stack starts with page 0 on top; the last page is
+    kept out of it as the sink of right-padded prefills (``sink``).
+    """
+
+    ERRORS = {1: "a row's length left [0, capacity]", 2: "a slot was written without a page",
+              4: "page pool exhausted", 8: "more new tokens than max_tokens"}
+
+    def __init__(self, batch_size, pages_per_row, n_pages, device, err=None, stack=None):
+        B, W, n = int(batch_size), int(pages_per_row), int(n_pages)
+        if n < 2:
+            raise L.SpecdecError("a page pool needs at least two pages (one is the sink)")
+        if B < 1 or W < 1:
+            raise L.SpecdecError("a page table needs at least one row and one page per row")
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise L.SpecdecError("DevicePageTable keeps its state on the GPU (no CPU fallback)")
+        if stack is None:
+            free = torch.arange(n - 2, -2, -1, dtype=torch.int32, device=dev)
+            n_free = torch.full((1,), n - 1, dtype=torch.int32, device=dev)
+        else:
+            free, n_free = stack                   # another table's: one pool for both
+        self._bind(torch.full((B, W), -1, dtype=torch.int32, device=dev),
+                   torch.zeros(B, dtype=torch.int32, device=dev),
+                   torch.zeros(B, dtype=torch.int32, device=dev), free, n_free,
+                   torch.zeros(1, dtype=torch.int32, device=dev) if err is None else err)
+
+    def _bind(self, block_table, owned, shared, free, n_free, err):
+        self.block_table, self.owned, self.shared = block_table, owned, shared
+        self.free, self.n_free, self.err = free, n_free, err
+        self.B, self.W = block_table.shape
+        self.n_pages = free.numel()
+        self.sink = self.n_pages - 1
+        self.device = block_table.device
+
+    @classmethod
+    def over(cls, block_table, owned, shared, free, n_free, err):
+        """A table over state that the caller holds (no copies)."""
+        if block_table.dim() != 2 or block_table.stride(1) != 1:
+            raise L.SpecdecError("block_table must be [B, W] with contiguous rows")
+        B = block_table.shape[0]
+        for name, t, n in (("block_table", block_table, None), ("owned", owned, B),
+                           ("shared", shared, B), ("free", free, None), ("n_free", n_free, 1),
+                           ("err", err, 1)):
+            if t.dtype != torch.int32 or not t.is_cuda or t.device != block_table.device:
+                raise L.SpecdecError(f"{name} must be int32 on one CUDA device")
+            if t is not block_table and not t.is_contiguous():
+                raise L.SpecdecError(f"{name} must be contiguous")
+            if n is not None and t.numel() != n:
+                raise L.SpecdecError(f"{name} must have {n} entries, got {t.numel()}")
+        if B == 0 or block_table.shape[1] == 0 or free.numel() == 0:
+            raise L.SpecdecError("a page table needs at least one row, one page per row and a pool")
+        self = cls.__new__(cls)
+        self._bind(block_table, owned, shared, free, n_free, err)
+        return self
+
+    def _rows(self, t, name):
+        if t.device != self.device or t.numel() != self.B or t.is_floating_point():
+            raise L.SpecdecError(f"{name} must be an integer [B] tensor on {self.device}")
+        return t if t.dtype == torch.long and t.is_contiguous() else t.long().contiguous()
+
+    def reserve(self, lengths, new, max_tokens=None):
+        """Pages for ``new`` more tokens of every row past ``lengths`` [B].
+
+        ``new`` is one int for all rows or an integer [B] tensor; with a tensor
+        ``max_tokens`` bounds their sum (the size of ``slots``).  Returns
+        (slots [max_tokens] int64, starts [B + 1] int32): token i of row b goes
+        to pool slot slots[starts[b] + i] = page * PAGE + offset; slots behind
+        the last token are -1.
+        """
+        lens = self._rows(lengths, "lengths")
+        if torch.is_tensor(new):
+            if max_tokens is None:
+                raise L.SpecdecError("max_tokens is needed with per-row token counts")
+            add, each, total = self._rows(new, "new"), 0, int(max_tokens)
+        else:
+            add, each = None, int(new)
+            if each < 0:
+                raise L.SpecdecError(f"new tokens must not be negative, got {each}")
+            total = self.B * each if max_tokens is None else int(max_tokens)
+        if total < 0:
+            raise L.SpecdecError(f"max_tokens must not be negative, got {total}")
+        lib = L.lib()
+        with torch.cuda.device(self.device):
+            slots = torch.empty(total, dtype=torch.long, device=self.device)
+            starts = torch.empty(self.B + 1, dtype=torch.int32, device=self.device)
+            ws = torch.empty(lib.sd_pages_workspace_bytes(self.B), dtype=torch.uint8,
+                             device=self.device)
+            L.check(lib.sd_pages_reserve(
+                L.ptr(self.block_table), self.block_table.stride(0), self.W, L.ptr(self.owned),
+                L.ptr(self.free), self.n_pages, L.ptr(self.n_free), L.ptr(lens), L.ptr(add), each,
+                self.B, L.ptr(slots), total, L.ptr(starts), L.ptr(self.err), L.ptr(ws), ws.numel(),
+                L.stream_ptr(self.device)), "pages_reserve")
+        return slots, starts
+
+    def trim(self, lengths):
+        """Give back every row's pages past its ``lengths`` [B] tokens (never
+        its shared ones); a trim after a reserve restores the stack."""
+        lens = self._rows(lengths, "lengths")
+        with torch.cuda.device(self.device):
+            L.check(L.lib().sd_pages_trim(
+                L.ptr(self.block_table), self.block_table.stride(0), self.W, L.ptr(self.owned),
+                L.ptr(self.shared), L.ptr(self.free), self.n_pages, L.ptr(self.n_free),
+                L.ptr(lens), self.B, L.ptr(self.err), L.stream_ptr(self.device)), "pages_trim")
+
+    def reset(self):
+        """Every page back on the stack, page 0 on top (of this table's pool)."""
+        self.block_table.fill_(-1)
+        self.owned.zero_()
+        self.shared.zero_()
+        n = self.n_pages
+        self.free.copy_(torch.arange(n - 2, -2, -1, dtype=torch.int32, device=self.device))
+        self.n_free.fill_(n - 1)
+        self.err.zero_()
+
+    def check_errors(self):
+        """Raise if a call could not be done (syncs once)."""
+        e = int(self.err.item())
+        if e:
+            self.err.zero_()
+            raise RuntimeError("DevicePageTable: " + "; ".join(
+                text for bit, text in self.ERRORS.items() if e & bit))
 
 
 class PagedRaggedCache(RaggedCache):

@@ -240,6 +240,45 @@ int sd_kv_append_paged(void* kpool, void* vpool, const void* new_k, const void* 
                        int q, int dtype, int* err, void* stream);
 
 /*
+ * No counterpart in the reference (added entry points): the page table of a
+ * paged cache kept on the device, so that pages follow the device lengths
+ * without a host copy of them (and inside a captured graph).  State, all on
+ * the device and owned by the caller: block_table [B, W] (rows bt_stride
+ * apart, -1 = no page), owned [B] (pages of each row, shared ones included),
+ * shared [B] (leading pages that the row does not give back: a prompt's pages
+ * read by several rows), the stack free_stack [n_pages] with *n_free entries.
+ *
+ * sd_pages_reserve gives row b the pages for lengths[b] + new tokens
+ * (new_tokens[b], or new_each for every row when new_tokens is NULL): the
+ * o-th missing page over all rows, row by row, is the o-th from the top of
+ * the stack.  It writes starts [B + 1] (exclusive prefix of the new token
+ * counts) and slots [max_tokens]: token i of row b gets
+ *   slots[starts[b] + i] = page * SD_KV_PAGE + offset
+ * of cache position lengths[b] + i; slots behind the last token are -1.
+ * Rows keep the pages they have: nothing is given back.
+ *
+ * sd_pages_trim gives back every row's pages past max(ceil(lengths[b] /
+ * SD_KV_PAGE), shared[b]), so that a trim after a reserve restores the stack.
+ *
+ * A call that cannot serve every row changes nothing and sets bits of *err:
+ * CAPACITY (a row past W pages, a negative length or count), EXHAUSTED (too
+ * few free pages), SLOTS (more new tokens than max_tokens); starts is still
+ * written and every slot is -1.  Calls on one table are stream ordered.
+ */
+#define SD_PAGES_ERR_CAPACITY 1
+#define SD_PAGES_ERR_EXHAUSTED 4
+#define SD_PAGES_ERR_SLOTS 8
+size_t sd_pages_workspace_bytes(int B);
+int sd_pages_reserve(int32_t* block_table, int bt_stride, int W, int32_t* owned,
+                     const int32_t* free_stack, int n_pages, int32_t* n_free,
+                     const int64_t* lengths, const int64_t* new_tokens, int64_t new_each, int B,
+                     int64_t* slots, int64_t max_tokens, int32_t* starts, int* err,
+                     void* workspace, size_t workspace_bytes, void* stream);
+int sd_pages_trim(int32_t* block_table, int bt_stride, int W, int32_t* owned,
+                  const int32_t* shared, int32_t* free_stack, int n_pages, int32_t* n_free,
+                  const int64_t* lengths, int B, int* err, void* stream);
+
+/*
  * The fused step between an attention layer's QKV projections and its
  * attention, for bf16 Qwen3 / Llama-style layers: per row b, position
  * l < L and head, the head's RMSNorm on q and k (weights q_norm_w / k_norm_w
