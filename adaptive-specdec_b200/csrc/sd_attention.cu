@@ -22,7 +22,8 @@
 #include <atomic>
 #include <cstdlib>
 
-#include "specdec_b200.h"
+#include "sd_attn.cuh"
+#include "sd_tcgen05.cuh"
 
 namespace sd {
 
@@ -41,47 +42,6 @@ template <typename T> __device__ __forceinline__ T from_f(float x);
 template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) {
   return __float2bfloat16(x);
-}
-
-struct AttnParams {
-  const void* q; int64_t qbs, qhs, qqs;
-  const void* k; const void* v;
-  const int64_t* lengths; const int64_t* valid;
-  int B, Hq, Hkv, D, C, qlen, group, R, nsplit, nrc;
-  float scale;
-  void* out; int64_t obs, oqs, ohs;
-  float* part_acc;   // [B, Hkv, nsplit, R, D]
-  float* part_ml;    // [B, Hkv, nsplit, R, 2]
-  int* split_done;   // [B, Hkv] pieces finished (tensor-core path; zeroed per call)
-  int* rowpre;       // [B + 1] exclusive prefix of 64-key tiles per row (tensor-core path)
-  int* rowkmax;      // [B] live-key bound of each row (tensor-core path)
-  int npiece;        // partial slots per (row, kv head) on the tensor-core path
-  int out_vec4;      // out is 8-byte aligned and its strides are multiples of 4 elements
-  int tile_keys;     // keys per tile of the tensor-core schedule (plan kernel)
-  int seg_ovh;       // schedule cost of a (row, kv head) beyond its tiles, in tiles
-  int* status;       // sticky: bit 0 = a bounded wait of the tcgen05 kernel gave up
-  // paged caches: k / v are pools [npages, Hkv, SD_KV_PAGE, D] and row b's key
-  // s sits in page bt[b * bt_stride + s / SD_KV_PAGE]; bt == nullptr: the
-  // contiguous [B, Hkv, C, D] layout
-  const int32_t* bt;
-  int bt_stride, npages;
-};
-
-// Offset, in rows of D elements, of key s of row b and kv head h.  A page
-// index outside the pool reads page 0 (the caller's block table is wrong, but
-// nothing is read out of bounds).
-__device__ __forceinline__ int64_t kv_row(const AttnParams& P, int b, int h, int s) {
-  if (P.bt == nullptr) return ((int64_t)b * P.Hkv + h) * P.C + s;
-  int pg = __ldg(P.bt + (int64_t)b * P.bt_stride + (s / SD_KV_PAGE));
-  if ((unsigned)pg >= (unsigned)P.npages) pg = 0;
-  return ((int64_t)pg * P.Hkv + h) * SD_KV_PAGE + (s % SD_KV_PAGE);
-}
-
-__device__ __forceinline__ int row_limit(const AttnParams& P, int b, int j) {
-  int64_t lim = P.lengths[b] + j + 1;
-  if (P.valid && P.valid[b] < lim) lim = P.valid[b];
-  if (lim > P.C) lim = P.C;
-  return lim > 0 ? (int)lim : 0;
 }
 
 template <typename T>
@@ -260,9 +220,6 @@ struct MmaSmem {
 __device__ __forceinline__ uint32_t sw_off(int r, int c) {
   return (uint32_t)(r * (MT_D * 2) + ((c ^ (r & 7)) << 4));
 }
-__device__ __forceinline__ uint32_t smem_addr(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
                :: "r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
@@ -298,16 +255,6 @@ __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uin
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Merge with every load issued up front (128 threads; `scratch` holds
 // 2 * R * np floats of shared memory): (max, sum) of every (row, piece) in
 // one pass, per-row weights in shared memory, then each thread (head-dim
@@ -756,14 +703,14 @@ constexpr int TC_N = 32;                 // query rows per kv head (padded)
 constexpr int TC_NST = 3;                // K/V ring stages
 constexpr int TC_THREADS = 192;
 constexpr int TC_MIN_SHARE = SPLIT_KEYS / TC_KEYS;
+static_assert(TC_MIN_SHARE == ATTN_MIN_SHARE, "the join knows the schedule");
 constexpr float TC_HEADROOM = 8.f;
 // Schedule cost of starting a (row, kv head) segment, in tiles: its Q,
 // first-tile max, epilogue and barriers take about as long as this many
 // tiles, so CTAs that cover many short rows get fewer tiles.  The schedule
 // lays these virtual tiles in front of each (row, kv head)'s real ones.
-constexpr int TC_OVH = 6;
+constexpr int TC_OVH = ATTN_SEG_OVH;
 constexpr uint32_t TC_TMEM_COLS = 128;   // S0, S1, O0, O1 (32 columns each)
-constexpr long long TC_WAIT = 1LL << 31; // cycles (~1 s) before a wait gives up
 
 struct TcSmem {
   alignas(1024) unsigned char k[TC_NST][2][TC_KEYS * 128];   // [stage][64-col box][128 rows x 128 B]
@@ -784,99 +731,6 @@ struct TcSmem {
 };
 static_assert(sizeof(TcSmem) + 1024 <= 227 * 1024, "tcgen05 attention shared memory");
 
-__device__ __forceinline__ uint32_t tc_sw128(int row, int col) {  // element offset in a 64-col box
-  return (uint32_t)(row * 128 + ((((col >> 3) ^ (row & 7))) << 4) + (col & 7) * 2);
-}
-__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo, uint32_t sbo,
-                                            uint32_t layout) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) |
-         ((uint64_t)((sbo >> 4) & 0x3FFF) << 32) | ((uint64_t)1 << 46) |
-         ((uint64_t)(layout & 7) << 61);
-}
-// kind::f16 instruction descriptor: bf16 A and B, f32 D, M x N, majors
-__host__ __device__ constexpr uint32_t tc_idesc(int M, int N, int a_mn, int b_mn) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, int acc) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-               :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(acc) : "memory");
-}
-__device__ __forceinline__ void tc_commit(unsigned long long* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-               :: "r"(smem_addr(bar)) : "memory");
-}
-__device__ __forceinline__ void tc_bar_init(unsigned long long* bar, int count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(smem_addr(bar)), "r"(count)
-               : "memory");
-}
-__device__ __forceinline__ void tc_arrive(unsigned long long* bar) {
-  asm volatile("{\n .reg .b64 st;\n mbarrier.arrive.shared::cta.b64 st, [%0];\n}"
-               :: "r"(smem_addr(bar)) : "memory");
-}
-__device__ __forceinline__ void tc_expect_tx(unsigned long long* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-               :: "r"(smem_addr(bar)), "r"(bytes) : "memory");
-}
-// Has the phase of parity `par` completed?  (non-blocking)
-__device__ __forceinline__ bool tc_test(unsigned long long* bar, uint32_t par) {
-  uint32_t done;
-  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-               " selp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(smem_addr(bar)), "r"(par)
-               : "memory");
-  return done != 0;
-}
-// Bounded wait for the phase of parity `par`; false (and the CTA's abort
-// flag set) on expiry or when another thread already gave up.
-__device__ __forceinline__ bool tc_wait(unsigned long long* bar, uint32_t par, int* abort_) {
-  const long long t0 = clock64();
-  while (true) {
-    uint32_t done;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-                 " selp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(smem_addr(bar)), "r"(par)
-                 : "memory");
-    if (done) return true;
-    if (*reinterpret_cast<volatile int*>(abort_) || clock64() - t0 > TC_WAIT) {
-      *reinterpret_cast<volatile int*>(abort_) = 1;
-      return false;
-    }
-  }
-}
-__device__ __forceinline__ void tc_tma_2d(void* dst, const void* tmap, int x, int y,
-                                          unsigned long long* bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-               " [%0], [%1, {%2, %3}], [%4];"
-               :: "r"(smem_addr(dst)), "l"(tmap), "r"(x), "r"(y), "r"(smem_addr(bar))
-               : "memory");
-}
-#define TC_LD32(r, addr)                                                                        \
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,"    \
-               "%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"  \
-               "%30,%31}, [%32];"                                                               \
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),        \
-                 "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),     \
-                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), \
-                 "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), \
-                 "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), \
-                 "=r"(r[30]), "=r"(r[31])                                                      \
-               : "r"(addr) : "memory")
-#define TC_ST32(addr, r)                                                                        \
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,"  \
-               "%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"  \
-               "%30,%31,%32};"                                                                  \
-               :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), \
-                 "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),\
-                 "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),       \
-                 "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),       \
-                 "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),       \
-                 "r"(r[31]) : "memory")
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
 // barrier of the four softmax warps
 __device__ __forceinline__ void tc_sbar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ bool tc_sbar_or(bool p) {
@@ -900,13 +754,15 @@ __device__ __forceinline__ void tc_seg_init(TcSeg& g, const AttnParams& P, int b
   g.tt = t0;
   g.t1 = t1;
 }
+template <bool PFX>
 __device__ __forceinline__ void tc_seg_bounds(TcSeg& g, const AttnParams& P) {
   g.ncost = min(g.tb - g.off, g.t1 - g.tt);
   const int r0 = max(g.off, TC_OVH) - TC_OVH;          // real tiles: units past the virtual ones
   const int r1 = g.off + g.ncost - TC_OVH;
   g.nseg = max(r1 - r0, 0);
-  g.s0 = r0 * TC_KEYS;
-  g.s1 = min(P.rowkmax[g.b], r1 * TC_KEYS);
+  const int k0 = PFX ? P.rowstart[g.b] : 0;            // keys before it belong to the shared prefix
+  g.s0 = k0 + r0 * TC_KEYS;
+  g.s1 = min(P.rowkmax[g.b], k0 + r1 * TC_KEYS);
 }
 // advance past the current segment; false when the run is over
 __device__ __forceinline__ bool tc_seg_next(TcSeg& g, const AttnParams& P) {
@@ -921,16 +777,21 @@ __device__ __forceinline__ bool tc_seg_next(TcSeg& g, const AttnParams& P) {
   return true;
 }
 // the current or next segment that holds real tiles; false when none is left
+template <bool PFX>
 __device__ __forceinline__ bool tc_seg_real(TcSeg& g, const AttnParams& P) {
-  tc_seg_bounds(g, P);
+  tc_seg_bounds<PFX>(g, P);
   while (g.nseg == 0) {
     if (!tc_seg_next(g, P)) return false;
-    tc_seg_bounds(g, P);
+    tc_seg_bounds<PFX>(g, P);
   }
   return true;
 }
 
-template <int NTG>                                    // 8-row groups of real query rows
+// PFX: the rows' own keys behind a shared prefix (sd_prefix.cu).  Segments
+// start at P.rowstart[b], gridDim.y chunks of P.qc queries take their turn,
+// and every piece leaves its partial, base-2 maximum, in slot
+// (chunk, row * Hkv + head + CTA) for the join over prefix and row.
+template <int NTG, bool PFX>                          // NTG: 8-row groups of real query rows
 __global__ void __launch_bounds__(TC_THREADS, 1)
 attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap tmk,
                const __grid_constant__ CUtensorMap tmv) {
@@ -939,7 +800,8 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
   const uint32_t pad = (1024u - (smem_addr(tc_raw) & 1023u)) & 1023u;  // swizzle atoms: 1024 B
   TcSmem& S = *reinterpret_cast<TcSmem*>(tc_raw + pad);
   const int t = threadIdx.x, w = t >> 5, lane = t & 31;
-  const int R = P.R, Hkv = P.Hkv;
+  const int j0 = PFX ? (int)blockIdx.y * P.qc : 0;
+  const int R = PFX ? min(P.qc, P.qlen - j0) * P.group : P.R, Hkv = P.Hkv;
   const int total = P.rowpre[P.B] * Hkv;
   const int share = max(TC_MIN_SHARE, (total + (int)gridDim.x - 1) / (int)gridDim.x);
   const int t0 = (int)blockIdx.x * share;
@@ -982,7 +844,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
       uint32_t gi = 0;
       bool ok = true;
       do {
-        tc_seg_bounds(g, P);
+        tc_seg_bounds<PFX>(g, P);
         const int row0 = P.bt ? 0 : (g.b * Hkv + g.h) * P.C + g.s0;
         for (int i = 0; i < g.nseg && ok; ++i, ++gi) {
           const int st = (int)(gi % TC_NST);
@@ -1018,15 +880,15 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
       uint32_t ntot = 0;                               // real tiles of the run
       {
         TcSeg gw = g;
-        bool more = tc_seg_real(gw, P);
+        bool more = tc_seg_real<PFX>(gw, P);
         while (more) {
           ntot += (uint32_t)gw.nseg;
-          more = tc_seg_next(gw, P) && tc_seg_real(gw, P);
+          more = tc_seg_next(gw, P) && tc_seg_real<PFX>(gw, P);
         }
       }
       TcSeg ga = g, gc = g;
-      tc_seg_real(ga, P);
-      tc_seg_real(gc, P);
+      tc_seg_real<PFX>(ga, P);
+      tc_seg_real<PFX>(gc, P);
       int ia = 0, ic = 0;
       uint32_t a = 0, c = 0, sa = 0, sc = 0;             // tiles and segments of the two heads
       long long idle0 = clock64();
@@ -1055,7 +917,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
             if (++ia == ga.nseg) {
               ia = 0;
               ++sa;
-              if (tc_seg_next(ga, P)) tc_seg_real(ga, P);
+              if (tc_seg_next(ga, P)) tc_seg_real<PFX>(ga, P);
             }
             progressed = true;
           }
@@ -1075,7 +937,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
             if (++ic == gc.nseg) {
               ic = 0;
               ++sc;
-              if (tc_seg_next(gc, P)) tc_seg_real(gc, P);
+              if (tc_seg_next(gc, P)) tc_seg_real<PFX>(gc, P);
             }
             progressed = true;
           }
@@ -1111,7 +973,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
         const int r = i >> 4, c = i & 15;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (r < R) {
-          const int j = r / P.group, hq = qh * P.group + r % P.group;
+          const int j = j0 + r / P.group, hq = qh * P.group + r % P.group;
           v = *reinterpret_cast<const uint4*>(Qg + qb * P.qbs + hq * P.qhs + j * P.qqs + 8 * c);
         }
         *reinterpret_cast<uint4*>(S.q[qs & 1u][c >> 3] + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
@@ -1121,7 +983,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
     };
     uint32_t gi = 0, seg = 0;
     bool run = true;
-    bool more = tc_seg_real(g, P);
+    bool more = tc_seg_real<PFX>(g, P);
     if (more) write_q(g.b, g.h, 0u);
     while (more) {
       const int b = g.b, h = g.h;
@@ -1136,7 +998,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
       const int64_t capb = min(P.valid ? __ldg(P.valid + b) : (int64_t)P.C, (int64_t)P.C);
 #pragma unroll
       for (int r = 0; r < RN; ++r) {
-        const int64_t lj = min(lenb + r / P.group + 1, capb);
+        const int64_t lj = min(lenb + j0 + r / P.group + 1, capb);
         lim[r] = r < R ? (int)min(max(lj, (int64_t)0), (int64_t)g.s1) : 0;
         if (r < R) lim_min = min(lim_min, lim[r]);
         m[r] = -INFINITY;
@@ -1237,7 +1099,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
           // segment's GEMM1s) finished before this tile's S arrived, and the
           // global loads overlap this segment's tiles
           TcSeg gn = g;
-          if (tc_seg_next(gn, P) && tc_seg_real(gn, P)) write_q(gn.b, gn.h, seg + 1u);
+          if (tc_seg_next(gn, P) && tc_seg_real<PFX>(gn, P)) write_q(gn.b, gn.h, seg + 1u);
         }
       }
       if (!run) break;
@@ -1258,6 +1120,24 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
       }
       tc_sbar();
       const int bh = b * Hkv + h;
+      if (PFX) {
+        const int64_t base =
+            (((int64_t)blockIdx.y * P.slots + bh + blockIdx.x) * (P.qc * P.group)) * MT_D;
+#pragma unroll
+        for (int r = 0; r < RN; ++r) {
+          if (r >= R) continue;
+          const float L = (S.red[0][r] + S.red[1][r]) + (S.red[2][r] + S.red[3][r]);
+          P.part_acc[base + r * MT_D + t] = __uint_as_float(o[r]);
+          if (t == 0) {
+            P.part_ml[base / MT_D * 2 + 2 * r] = m[r];
+            P.part_ml[base / MT_D * 2 + 2 * r + 1] = L;
+          }
+        }
+        tc_sbar();                                     // S.red is reused next segment
+        ++seg;
+        more = tc_seg_next(g, P) && tc_seg_real<PFX>(g, P);
+        continue;
+      }
       const int Tb = P.rowpre[b] * Hkv + h * g.tb;     // first tile of this (row, kv head)
       const int cfirst = (Tb + TC_OVH) / share;         // CTAs holding its real tiles
       const int npieces = (Tb + g.tb - 1) / share - cfirst + 1;
@@ -1295,7 +1175,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
       }
       tc_sbar();                                       // S.red and S.last reused next segment
       ++seg;
-      more = tc_seg_next(g, P) && tc_seg_real(g, P);
+      more = tc_seg_next(g, P) && tc_seg_real<PFX>(g, P);
     }
   }
   // ---------------- teardown: TMEM back once every role is done with it
@@ -1356,7 +1236,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
 
 // 2D map over a [B, Hkv, C, 128] bf16 cache viewed as [B * Hkv * C, 128]:
 // boxes of 128 rows x 64 columns (128 B), 128-byte swizzle, zero fill
-static bool cache_map(CUtensorMap* map, const void* base, int64_t rows) {
+bool cache_map(CUtensorMap* map, const void* base, int64_t rows) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
   if (enc == nullptr) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)MT_D, (cuuint64_t)rows};
@@ -1369,17 +1249,19 @@ static bool cache_map(CUtensorMap* map, const void* base, int64_t rows) {
          CUDA_SUCCESS;
 }
 
-template <int NTG>
+template <int NTG, bool PFX>
 static int launch_tc_ntg(const AttnParams& P, const CUtensorMap& mk, const CUtensorMap& mv,
                          int nsm, cudaStream_t st) {
   const int sm = (int)sizeof(TcSmem) + 1024;         // + room to align to 1024 B
-  if (cudaFuncSetAttribute(attn_tc_kernel<NTG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  if (cudaFuncSetAttribute(attn_tc_kernel<NTG, PFX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            sm) != cudaSuccess)
     return SD_ELAUNCH;
-  attn_tc_kernel<NTG><<<nsm, TC_THREADS, sm, st>>>(P, mk, mv);
+  const dim3 grid((unsigned)nsm, PFX ? (unsigned)((P.qlen + P.qc - 1) / P.qc) : 1u);
+  attn_tc_kernel<NTG, PFX><<<grid, TC_THREADS, sm, st>>>(P, mk, mv);
   return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
 }
 
+template <bool PFX>
 static int launch_tc(const AttnParams& P, cudaStream_t st) {
   const int64_t rows = P.bt ? (int64_t)P.npages * P.Hkv * SD_KV_PAGE : (int64_t)P.B * P.Hkv * P.C;
   if (rows >= (int64_t)1 << 31) return SD_ENOTSUP;
@@ -1389,13 +1271,16 @@ static int launch_tc(const AttnParams& P, cudaStream_t st) {
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return SD_ELAUNCH;
-  switch ((P.R + 7) / 8) {
-    case 1: return launch_tc_ntg<1>(P, mk, mv, nsm, st);
-    case 2: return launch_tc_ntg<2>(P, mk, mv, nsm, st);
-    case 3: return launch_tc_ntg<3>(P, mk, mv, nsm, st);
-    default: return launch_tc_ntg<4>(P, mk, mv, nsm, st);
+  if (PFX) nsm = P.ncta;
+  switch (((PFX ? P.qc * P.group : P.R) + 7) / 8) {
+    case 1: return launch_tc_ntg<1, PFX>(P, mk, mv, nsm, st);
+    case 2: return launch_tc_ntg<2, PFX>(P, mk, mv, nsm, st);
+    case 3: return launch_tc_ntg<3, PFX>(P, mk, mv, nsm, st);
+    default: return launch_tc_ntg<4, PFX>(P, mk, mv, nsm, st);
   }
 }
+
+int launch_suffix(const AttnParams& P, cudaStream_t st) { return launch_tc<true>(P, st); }
 
 // Which kernel takes the tensor-core shapes: tcgen05 (default) or the
 // mma.sync kernel (SD_ATTN_KERNEL=mma, kept for comparison).
@@ -1473,7 +1358,7 @@ static int verify_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, con
     P.seg_ovh = TC_OVH;
     attn_plan_kernel<<<1, 1024, 0, st>>>(P);
     if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
-    return launch_tc(P, st);
+    return launch_tc<false>(P, st);
   }
   if (mma_ok) {
     P.nrc = 1;

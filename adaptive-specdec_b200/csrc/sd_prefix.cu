@@ -1,0 +1,760 @@
+// Attention over a paged cache whose rows share a prefix (sm_100a).
+//
+// The rows of a group (samples of one prompt, requests under one system
+// prompt) hold the same pages in front: block_table[b, 0..pages_g) is equal
+// for every row b of group g.  With the softmax split over two key ranges,
+//   out = (2^(m1 - m) O1 + 2^(m2 - m) O2) / (2^(m1 - m) l1 + 2^(m2 - m) l2),
+//   m = max(m1, m2), (m_i, l_i, O_i) the running maximum (base 2), sum and
+//   unnormalised output over range i,
+// the shared range is computed for all query rows of a group at once and each
+// row's own range by itself:
+//   prefix_plan_kernel  lays out the work of both from the device lengths;
+//   prefix_tc_kernel    the shared pages, query rows of the whole group on
+//                       the M side of tcgen05.mma: K and V are read once per
+//                       256 query rows instead of once per row;
+//   attn_tc_kernel      (sd_attention.cu, PFX) the rows' own pages;
+//   prefix_join_kernel  merges the partials, in piece order, into the output.
+// A row whose first query does not see the whole shared range (an empty or a
+// padding row, a short cap) takes no part in it: its own range starts at 0, so
+// the shared range needs no mask and no row meets another row's masked keys.
+#include <math_constants.h>
+
+#include <algorithm>
+
+#include "sd_attn.cuh"
+#include "sd_common.cuh"
+#include "sd_tcgen05.cuh"
+
+namespace sd {
+
+constexpr int PX_D = 128;
+constexpr int PX_ROWS = 256;                 // query rows per item: two tiles of 128
+constexpr int PX_SLOTS = 4;                  // 32 KB K / V tiles in flight
+constexpr int PX_THREADS = 320;              // warps 0-3, 4-7: softmax of tile 0, 1; 8 TMA; 9 MMA
+constexpr int PX_CTAS = 148;                 // one CTA per SM
+constexpr int PX_OVH = 2;                    // schedule cost of an item beyond its pages, in pages
+constexpr int PX_MIN_SHARE = 4;              // fewest schedule units per CTA
+constexpr float PX_HEADROOM = 8.f;           // lazy-rescale headroom of the running max (base 2)
+constexpr int PX_JOIN_THREADS = 256;
+
+struct PrefixParams {
+  AttnParams A;
+  const int32_t* starts;                     // [G + 1] first row of each group
+  const int32_t* pages;                      // [G] shared pages of each group
+  int G, max_items;
+  // workspace
+  int* g_unit;                               // [G + 1] exclusive prefix of schedule units
+  int* g_item;                               // [G + 1] exclusive prefix of items
+  int* g_row0;                               // [G]
+  int* g_rows;                               // [G]
+  int* g_pages;                              // [G] 0: the group shares nothing
+  int* rowgroup;                             // [B] the row's group, -1: it takes no part
+  float* pacc;                               // [slot][PX_ROWS][D]
+  float* pml;                                // [slot][PX_ROWS][2]
+};
+
+// The items of a group: (kv head, 256 query rows), kv head outer.
+__device__ __forceinline__ int px_pairs(const PrefixParams& P, int g) {
+  return (P.g_rows[g] * P.A.R + PX_ROWS - 1) / PX_ROWS;
+}
+__device__ __forceinline__ int px_share(int total) {
+  return max(PX_MIN_SHARE, (total + PX_CTAS - 1) / PX_CTAS);
+}
+
+__global__ void __launch_bounds__(1024) prefix_plan_kernel(const PrefixParams P) {
+  __shared__ long long red[33];
+  __shared__ int redi[33];
+  const AttnParams& A = P.A;
+  const int t = threadIdx.x;
+  if (t == 0) *A.status = 0;
+  const int W = A.bt_stride;
+  long long items0 = 0, units0 = 0;
+  for (int g0 = 0; g0 < P.G; g0 += 1024) {
+    const int g = g0 + t;
+    long long items = 0, units = 0;
+    if (g < P.G) {
+      const int s0 = min(max(P.starts[g], 0), A.B), s1 = min(max(P.starts[g + 1], s0), A.B);
+      const int rows = s1 - s0;
+      const int pg = rows < 2 ? 0 : min(max(P.pages[g], 0), W);   // one row shares with nobody
+      if (pg > 0) {
+        items = (long long)A.Hkv * (((long long)rows * A.R + PX_ROWS - 1) / PX_ROWS);
+        units = items * (pg + PX_OVH);
+      }
+      P.g_row0[g] = s0;
+      P.g_rows[g] = rows;
+      P.g_pages[g] = pg;
+    }
+    long long si, su;
+    const long long xi = block_excl_scan<long long>(items, red, &si);
+    __syncthreads();
+    const long long xu = block_excl_scan<long long>(units, red, &su);
+    if (g < P.G) {
+      P.g_item[g] = (int)(items0 + xi);
+      P.g_unit[g] = (int)(units0 + xu);
+    }
+    items0 += si;
+    units0 += su;
+    __syncthreads();
+  }
+  // groups that overlap could ask for more items than the workspace holds:
+  // then nothing is shared
+  const bool share = items0 <= P.max_items && units0 <= 0x7FFFFFFF;
+  if (t == 0) {
+    P.g_item[P.G] = share ? (int)items0 : 0;
+    P.g_unit[P.G] = share ? (int)units0 : 0;
+  }
+  __syncthreads();
+  int carry = 0;
+  for (int b0 = 0; b0 < A.B; b0 += 1024) {
+    const int b = b0 + t;
+    int tiles = 0;
+    if (b < A.B) {
+      int lo = 0, hi = P.G;                          // the last group that starts at or before b
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (P.starts[mid] <= b) lo = mid + 1; else hi = mid;
+      }
+      const int g = lo - 1;
+      int start = 0;
+      if (share && g >= 0 && b < P.g_row0[g] + P.g_rows[g] && b >= P.g_row0[g]) {
+        const int keys = P.g_pages[g] * SD_KV_PAGE;
+        if (row_limit(A, b, 0) >= keys) start = keys;
+      }
+      P.rowgroup[b] = start > 0 ? g : -1;
+      const int km = row_limit(A, b, A.qlen - 1);
+      const_cast<int*>(A.rowstart)[b] = start;
+      A.rowkmax[b] = km;
+      tiles = (max(km - start, 0) + SD_KV_PAGE - 1) / SD_KV_PAGE;
+      if (tiles > 0) tiles += ATTN_SEG_OVH;
+    }
+    int sum;
+    const int ex = block_excl_scan<int>(tiles, redi, &sum);
+    if (b < A.B) A.rowpre[b] = carry + ex;
+    carry += sum;
+    __syncthreads();
+  }
+  if (t == 0) A.rowpre[A.B] = carry;
+}
+
+// A CTA's run of schedule units as segments of items, walked identically by
+// every role.
+struct PxSeg {
+  int g, h, p, np, tb, off, tt, t1, ncost, j0, j1;   // pages [j0, j1) of the segment
+  bool dup;                                          // one tile of rows: both halves work on it
+};
+__device__ __forceinline__ void px_item(PxSeg& s, const PrefixParams& P) {
+  s.dup = P.g_rows[s.g] * P.A.R - s.p * PX_ROWS <= PX_ROWS / 2;
+}
+__device__ __forceinline__ void px_bounds(PxSeg& s) {
+  s.ncost = min(s.tb - s.off, s.t1 - s.tt);
+  s.j0 = max(s.off, PX_OVH) - PX_OVH;
+  s.j1 = max(s.off + s.ncost - PX_OVH, s.j0);
+}
+__device__ __forceinline__ void px_init(PxSeg& s, const PrefixParams& P, int g, int t0, int t1) {
+  s.g = g;
+  s.np = px_pairs(P, g);
+  s.tb = P.g_pages[g] + PX_OVH;
+  const int u = t0 - P.g_unit[g], it = u / s.tb;
+  s.off = u % s.tb;
+  s.h = it / s.np;
+  s.p = it % s.np;
+  s.tt = t0;
+  s.t1 = t1;
+  px_item(s, P);
+  px_bounds(s);
+}
+__device__ __forceinline__ bool px_next(PxSeg& s, const PrefixParams& P) {
+  s.tt += s.ncost;
+  if (s.tt >= s.t1) return false;
+  s.off = 0;
+  if (++s.p == s.np) {
+    s.p = 0;
+    if (++s.h == P.A.Hkv) {
+      s.h = 0;
+      do { ++s.g; } while (P.g_pages[s.g] == 0);     // units remain, so a sharing group follows
+      s.np = px_pairs(P, s.g);
+      s.tb = P.g_pages[s.g] + PX_OVH;
+    }
+  }
+  px_item(s, P);
+  px_bounds(s);
+  return true;
+}
+// Pages of a segment that tile x works on: all, or every second one.
+__device__ __forceinline__ int px_tasks(const PxSeg& s, int x) {
+  const int n = s.j1 - s.j0;
+  return s.dup ? (n + 1 - x) / 2 : n;
+}
+// The current or next segment with work for tile x; false when none is left.
+__device__ __forceinline__ bool px_work(PxSeg& s, const PrefixParams& P, int x) {
+  while (px_tasks(s, x) == 0)
+    if (!px_next(s, P)) return false;
+  return true;
+}
+
+struct PxSmem {
+  alignas(1024) unsigned char q[2][2][128 * 128];            // [tile][64-col box][128 rows x 128 B]
+  alignas(1024) unsigned char kv[PX_SLOTS][2][128 * 128];    // [slot][64-col box][128 keys x 128 B]
+  alignas(8) unsigned long long full[PX_SLOTS], empty[PX_SLOTS];
+  alignas(8) unsigned long long qfull[2], sfull[2], pfull[2], oready[2], fin;
+  uint32_t tmem;
+  int seg_g;
+  int abort_;
+};
+static_assert(sizeof(PxSmem) + 1024 <= 227 * 1024, "prefix attention shared memory");
+
+__device__ __forceinline__ void px_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, int acc) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+               :: "r"(d), "r"(a), "l"(b), "r"(id), "r"(acc) : "memory");
+}
+
+// What one tile's issue state walks: its segments, the page of the segment,
+// and the page's number in the CTA's run (the ring position).
+struct PxIssue {
+  PxSeg s;
+  int i;                                             // page of the segment (0-based)
+  uint32_t q;                                        // ring number of the segment's first page
+  uint32_t n, segs;                                  // tasks issued, segments with work before
+  bool more;
+};
+__device__ __forceinline__ void px_issue_seg(PxIssue& c, const PrefixParams& P, int x) {
+  // skip segments without work for this tile, counting their pages
+  while (px_tasks(c.s, x) == 0) {
+    c.q += (uint32_t)(c.s.j1 - c.s.j0);
+    if (!px_next(c.s, P)) {
+      c.more = false;
+      return;
+    }
+  }
+  c.i = c.s.dup ? x : 0;
+}
+__device__ __forceinline__ void px_issue_next(PxIssue& c, const PrefixParams& P, int x) {
+  c.i += c.s.dup ? 2 : 1;
+  ++c.n;
+  if (c.i < c.s.j1 - c.s.j0) return;
+  c.q += (uint32_t)(c.s.j1 - c.s.j0);
+  ++c.segs;
+  if (!px_next(c.s, P)) {
+    c.more = false;
+    return;
+  }
+  px_issue_seg(c, P, x);
+}
+
+// Persistent, stream-K: the (item, page) units lie end to end and each CTA
+// takes one contiguous run.  Per page and tile of 128 query rows:
+//   S[128 rows, 128 keys] = Q . K^T      (tcgen05.mma, operands in shared memory)
+//   thread t of the tile's four softmax warps owns row t (TMEM lane t): its
+//   128 scores in registers, a lazy reference maximum (moved when a score
+//   passes it by PX_HEADROOM), p = 2^(s - m) as bf16 back into the TMEM columns
+//   of S
+//   O[128 rows, 128 d] += P . V          (tcgen05.mma, A in TMEM)
+// TMEM: S0, S1, O0, O1 (128 columns each: all 512).  While one tile's softmax
+// runs, the tensor core works on the other tile.  P overwrites S, so S of a
+// tile's next page is issued behind P . V of this one; both run in issue order.
+// Two waits bound a tile: its scores (sfull) and, before O is touched, its
+// last P . V (oready).
+__global__ void __launch_bounds__(PX_THREADS, 1)
+prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CUtensorMap tmk,
+                 const __grid_constant__ CUtensorMap tmv) {
+  extern __shared__ __align__(1024) unsigned char px_raw[];
+  const uint32_t pad = (1024u - (smem_addr(px_raw) & 1023u)) & 1023u;   // swizzle atoms: 1024 B
+  PxSmem& S = *reinterpret_cast<PxSmem*>(px_raw + pad);
+  const AttnParams& A = P.A;
+  const int t = threadIdx.x, w = t >> 5, lane = t & 31;
+  const int total = P.g_unit[P.G];
+  const int share = px_share(total);
+  const int t0 = (int)blockIdx.x * share;
+  if (t0 >= total) return;                           // no work for this CTA (uniform)
+  const int t1 = min(total, t0 + share);
+  for (int g = t; g < P.G; g += PX_THREADS)
+    if (P.g_unit[g] <= t0 && t0 < P.g_unit[g + 1]) S.seg_g = g;
+  if (t == 0) {
+    for (int i = 0; i < PX_SLOTS; ++i) {
+      tc_bar_init(&S.full[i], 1);
+      tc_bar_init(&S.empty[i], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      tc_bar_init(&S.qfull[x], 128);
+      tc_bar_init(&S.sfull[x], 1);
+      tc_bar_init(&S.pfull[x], 128);
+      tc_bar_init(&S.oready[x], 1);
+    }
+    tc_bar_init(&S.fin, 1);
+    S.abort_ = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (w == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_addr(&S.tmem)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = S.tmem;
+  PxSeg seg;
+  px_init(seg, P, S.seg_g, t0, t1);
+
+  if (w == 8) {
+    // ---------------- TMA producer: K then V of each page, PX_SLOTS tiles ahead
+    if (lane == 0) {
+      uint32_t idx = 0;
+      bool ok = true;
+      do {
+        const int32_t* bt = A.bt + (int64_t)P.g_row0[seg.g] * A.bt_stride;
+        for (int j = seg.j0; j < seg.j1 && ok; ++j) {
+          int pg = __ldg(bt + j);
+          if ((unsigned)pg >= (unsigned)A.npages) pg = 0;    // a wrong table reads page 0
+          const int y = (int)(((int64_t)pg * A.Hkv + seg.h) * SD_KV_PAGE);
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv, ++idx) {
+            const int sl = (int)(idx % PX_SLOTS);
+            if (idx >= (uint32_t)PX_SLOTS)
+              ok = tc_wait(&S.empty[sl], ((idx / PX_SLOTS) - 1) & 1u, &S.abort_);
+            if (!ok) break;
+            tc_expect_tx(&S.full[sl], 2u * 128u * 128u);
+            const void* tm_ = kv ? (const void*)&tmv : (const void*)&tmk;
+            tc_tma_2d(S.kv[sl][0], tm_, 0, y, &S.full[sl]);
+            tc_tma_2d(S.kv[sl][1], tm_, 64, y, &S.full[sl]);
+          }
+        }
+      } while (ok && px_next(seg, P));
+      if (!ok) {
+        // let the copies already issued land before the CTA leaves
+        for (uint32_t q = idx > (uint32_t)PX_SLOTS ? idx - PX_SLOTS : 0u; q < idx; ++q) {
+          int dummy = 0;
+          tc_wait(&S.full[q % PX_SLOTS], (q / PX_SLOTS) & 1u, &dummy);
+        }
+      }
+    }
+  } else if (w == 9) {
+    // ---------------- MMA issuer: per tile an S queue and a P . V queue, polled
+    if (lane == 0) {
+      constexpr uint32_t ID1 = tc_idesc(128, 128, 0, 0);     // S = Q . K^T
+      constexpr uint32_t ID2 = tc_idesc(128, 128, 0, 1);     // O += P . V (V [key][d]: N-major)
+      PxIssue cs[2], cp[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        cs[x].s = seg;
+        cs[x].q = cs[x].n = cs[x].segs = 0;
+        cs[x].more = true;
+        px_issue_seg(cs[x], P, x);
+        cp[x] = cs[x];
+      }
+      uint32_t seen = 0;                             // tiles read by one of two users, by slot
+      long long idle0 = clock64();
+      while (cp[0].more || cp[1].more) {
+        bool progressed = false;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (cp[x].more && cp[x].n < cs[x].n) {
+            const uint32_t idx = 2u * (cp[x].q + (uint32_t)cp[x].i) + 1u, sl = idx % PX_SLOTS;
+            if (tc_test(&S.pfull[x], cp[x].n & 1u) && tc_test(&S.full[sl], (idx / PX_SLOTS) & 1u)) {
+              tc_fence_after();
+              const uint32_t va = smem_addr(S.kv[sl][0]);
+              const bool first = cp[x].i == (cp[x].s.dup ? x : 0);
+#pragma unroll
+              for (int ks = 0; ks < 8; ++ks)
+                px_mma_ts(tm + 256u + 128u * x, tm + 128u * x + 8u * ks,
+                          tc_desc(va + ks * 2048, 16384, 1024, 2), ID2, (!first || ks > 0) ? 1 : 0);
+              tc_commit(&S.oready[x]);
+              if (cp[x].s.dup || (seen >> sl & 1u)) {
+                seen &= ~(1u << sl);
+                tc_commit(&S.empty[sl]);
+              } else {
+                seen |= 1u << sl;
+              }
+              px_issue_next(cp[x], P, x);
+              progressed = true;
+            }
+          }
+          if (cs[x].more && cs[x].n == cp[x].n) {
+            const uint32_t idx = 2u * (cs[x].q + (uint32_t)cs[x].i), sl = idx % PX_SLOTS;
+            const bool first = cs[x].i == (cs[x].s.dup ? x : 0);
+            if (tc_test(&S.full[sl], (idx / PX_SLOTS) & 1u) &&
+                (!first || tc_test(&S.qfull[x], cs[x].segs & 1u))) {
+              tc_fence_after();
+              const uint32_t k0 = smem_addr(S.kv[sl][0]), k1 = smem_addr(S.kv[sl][1]);
+              const uint32_t q0 = smem_addr(S.q[x][0]), q1 = smem_addr(S.q[x][1]);
+#pragma unroll
+              for (int ks = 0; ks < 8; ++ks) {
+                const uint32_t ko = (uint32_t)(ks & 3) * 32u;
+                tc_mma(tm + 128u * x, tc_desc((ks < 4 ? q0 : q1) + ko, 16, 1024, 2),
+                       tc_desc((ks < 4 ? k0 : k1) + ko, 16, 1024, 2), ID1, ks > 0 ? 1 : 0);
+              }
+              tc_commit(&S.sfull[x]);
+              if (cs[x].s.dup || (seen >> sl & 1u)) {
+                seen &= ~(1u << sl);
+                tc_commit(&S.empty[sl]);
+              } else {
+                seen |= 1u << sl;
+              }
+              px_issue_next(cs[x], P, x);
+              progressed = true;
+            }
+          }
+        }
+        if (progressed) {
+          idle0 = clock64();
+        } else if (*reinterpret_cast<volatile int*>(&S.abort_) || clock64() - idle0 > TC_WAIT) {
+          *reinterpret_cast<volatile int*>(&S.abort_) = 1;
+          break;
+        }
+      }
+      // every MMA this thread issued has finished before the CTA leaves
+      tc_commit(&S.fin);
+      int dummy = 0;
+      tc_wait(&S.fin, 0u, &dummy);
+    }
+  } else {
+    // ---------------- softmax warps of tile x: thread r owns query row r
+    const int x = w >> 2, r = t & 127;
+    const uint32_t lrow = (uint32_t)(32 * (w & 3)) << 16;
+    const uint32_t scol = tm + lrow + 128u * x, ocol = scol + 256u;
+    const float sl2 = A.scale * 1.4426950408889634f;
+    const __nv_bfloat16* Qg = reinterpret_cast<const __nv_bfloat16*>(A.q);
+    uint32_t n = 0;                                  // tasks done
+    bool more = true;
+    while (more) {
+      const int tasks = px_tasks(seg, x);
+      const int rows = P.g_rows[seg.g] * A.R;
+      const int base = seg.p * PX_ROWS + (seg.dup ? 0 : 128 * x);
+      float m = -CUDART_INF_F, l = 0.f;
+      bool ok = true;
+      if (tasks > 0) {
+        // Q of the tile's rows (b, query, head of the group) into the swizzled
+        // K-major tile; rows past the group's are 0.  The last segment's S
+        // reads of this buffer ended before its last P . V was waited for.
+        for (int i = r; i < 128 * 16; i += 128) {
+          const int rr = i >> 4, c = i & 15, f = base + rr;
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (f < rows) {
+            const int bl = f / A.R, f2 = f - bl * A.R, j = f2 / A.group;
+            const int hq = seg.h * A.group + f2 - j * A.group;
+            v = *reinterpret_cast<const uint4*>(Qg + (int64_t)(P.g_row0[seg.g] + bl) * A.qbs +
+                                                hq * A.qhs + j * A.qqs + 8 * c);
+          }
+          *reinterpret_cast<uint4*>(S.q[x][c >> 3] + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc_arrive(&S.qfull[x]);
+      }
+      for (int i = 0; i < tasks; ++i, ++n) {
+        ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[x], n & 1u, &S.abort_));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[128];
+        TC_LD32((s + 0), scol);
+        TC_LD32((s + 32), scol + 32u);
+        TC_LD32((s + 64), scol + 64u);
+        TC_LD32((s + 96), scol + 96u);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+        for (int e = 0; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+        const bool move = mt > m + PX_HEADROOM;
+        if (__any_sync(0xffffffffu, move)) {
+          const float mn = move ? mt : m;
+          const float alpha = move ? (m == -CUDART_INF_F ? 0.f : ex2f(m - mn)) : 1.f;
+          m = mn;
+          l *= alpha;
+          if (i > 0) {
+            // O holds this segment's earlier pages: the last P . V into it first
+            ok = __all_sync(0xffffffffu, tc_wait(&S.oready[x], (n - 1) & 1u, &S.abort_));
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+              uint32_t o[32];
+              TC_LD32(o, ocol + 32u * q);
+              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              TC_ST32(ocol + 32u * q, o);
+            }
+          }
+        }
+        const float mc = fmaxf(m, -1e30f);           // 2^(-inf - mc) = 0
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float a = ex2f(fmaf(__uint_as_float(s[64 * hf + 2 * e]), sl2, -mc));
+            const float b = ex2f(fmaf(__uint_as_float(s[64 * hf + 2 * e + 1]), sl2, -mc));
+            ls[e & 3] += a + b;
+            pk[e] = pack_bf16(a, b);
+          }
+          TC_ST32(scol + 32u * hf, pk);
+        }
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
+        tc_arrive(&S.pfull[x]);
+      }
+      if (!ok) break;
+      if (seg.j1 > seg.j0) {
+        // ---- the segment's partial: slot (item + CTA) of the workspace
+        const int64_t slot = (int64_t)P.g_item[seg.g] + seg.h * seg.np + seg.p + blockIdx.x;
+        const int64_t at = slot * PX_ROWS + 128 * x + r;
+        if (tasks > 0) {
+          ok = __all_sync(0xffffffffu, tc_wait(&S.oready[x], (n - 1) & 1u, &S.abort_));
+          if (!ok) break;
+          tc_fence_after();
+          float4* dst = reinterpret_cast<float4*>(P.pacc + at * PX_D);
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            uint32_t o[32];
+            TC_LD32(o, ocol + 32u * q);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (base + r < rows) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                dst[8 * q + e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                             __uint_as_float(o[4 * e + 2]),
+                                             __uint_as_float(o[4 * e + 3]));
+            }
+          }
+          tc_fence_before();
+        }
+        P.pml[at * 2] = m;
+        P.pml[at * 2 + 1] = l;
+      }
+      more = px_next(seg, P);
+    }
+  }
+  // ---------------- teardown: TMEM back once every role is done with it
+  tc_fence_before();
+  __syncthreads();
+  if (w == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
+                 :: "r"(tm), "r"(512u) : "memory");
+  }
+  if (t == 0 && S.abort_) atomicOr(A.status, 1);
+}
+
+// A warp per (row, query, head): the pieces of the shared range and of the
+// row's own range, in piece order.
+__global__ void __launch_bounds__(PX_JOIN_THREADS) prefix_join_kernel(const PrefixParams P) {
+  const AttnParams& A = P.A;
+  const int lane = threadIdx.x & 31;
+  const int64_t wid = (int64_t)blockIdx.x * (PX_JOIN_THREADS / 32) + (threadIdx.x >> 5);
+  if (wid >= (int64_t)A.B * A.qlen * A.Hq) return;
+  const int hq = (int)(wid % A.Hq);
+  const int j = (int)(wid / A.Hq % A.qlen);
+  const int b = (int)(wid / A.Hq / A.qlen);
+  const int h = hq / A.group, gq = hq - h * A.group;
+  // pieces [0, n1): the shared range, two per CTA where both halves worked on
+  // the rows; [n1, n1 + n2): the row's own range
+  int n1 = 0, n2 = 0;
+  int64_t at1 = 0, at2 = 0;                          // row of the first piece's partial
+  int dup = 0;
+  const int g = P.rowgroup[b];
+  if (g >= 0) {
+    const int rows = P.g_rows[g] * A.R, np = (rows + PX_ROWS - 1) / PX_ROWS;
+    const int f = ((b - P.g_row0[g]) * A.qlen + j) * A.group + gq, p = f / PX_ROWS;
+    const int tb = P.g_pages[g] + PX_OVH, it = h * np + p;
+    const int u = P.g_unit[g] + it * tb, share = px_share(P.g_unit[P.G]);
+    const int c0 = (u + PX_OVH) / share, c1 = (u + tb - 1) / share;
+    dup = rows - p * PX_ROWS <= PX_ROWS / 2;
+    n1 = (c1 - c0 + 1) << dup;
+    at1 = ((int64_t)P.g_item[g] + it + c0) * PX_ROWS + f % PX_ROWS;
+  }
+  const int tb = A.rowpre[b + 1] - A.rowpre[b];
+  const int RC = A.qc * A.group;
+  if (tb > 0) {
+    const int total = A.rowpre[A.B] * A.Hkv;
+    const int share = max(ATTN_MIN_SHARE, (total + A.ncta - 1) / A.ncta);
+    const int u = A.rowpre[b] * A.Hkv + h * tb;
+    const int c0 = (u + ATTN_SEG_OVH) / share, c1 = (u + tb - 1) / share;
+    n2 = c1 - c0 + 1;
+    at2 = ((int64_t)(j / A.qc) * A.slots + b * A.Hkv + h + c0) * RC + (j % A.qc) * A.group + gq;
+  }
+  const int np = n1 + n2;
+  auto row_of = [&](int i) -> int64_t {
+    return i < n1 ? at1 + (int64_t)(i >> dup) * PX_ROWS + (dup & i) * (PX_ROWS / 2)
+                  : at2 + (int64_t)(i - n1) * RC;
+  };
+  float m = -CUDART_INF_F, l = 0.f;                  // per lane, then over the warp
+  bool nan = false;                                  // a NaN score leaves no maximum, but its sum
+  for (int i = lane; i < np; i += 32) {
+    const float* ml = (i < n1 ? P.pml : A.part_ml) + row_of(i) * 2;
+    const float mi = __ldcg(ml), li = __ldcg(ml + 1);
+    nan |= li != li;
+    if (mi != -CUDART_INF_F) {
+      const float mn = fmaxf(m, mi);
+      l = (m == -CUDART_INF_F ? 0.f : l * ex2f(m - mn)) + li * ex2f(mi - mn);
+      m = mn;
+    }
+  }
+  const float gm = warp_max(m);
+  const float L = warp_sum(m == -CUDART_INF_F ? 0.f : l * ex2f(m - gm));
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < np; i0 += 32) {
+    const int i = i0 + lane;
+    float f = 0.f;
+    if (i < np) {
+      const float mi = __ldcg((i < n1 ? P.pml : A.part_ml) + row_of(i) * 2);
+      f = mi == -CUDART_INF_F ? 0.f : ex2f(mi - gm);
+    }
+    const int cnt = min(32, np - i0);
+    for (int q = 0; q < cnt; ++q) {
+      const float fq = __shfl_sync(0xffffffffu, f, q);
+      if (fq == 0.f) continue;                       // nothing there (maybe never written)
+      const int k = i0 + q;
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(
+                                  (k < n1 ? P.pacc : A.part_acc) + row_of(k) * PX_D) + lane);
+      a.x = fmaf(fq, v.x, a.x); a.y = fmaf(fq, v.y, a.y);
+      a.z = fmaf(fq, v.z, a.z); a.w = fmaf(fq, v.w, a.w);
+    }
+  }
+  // a wait that gave up somewhere leaves partials unwritten: say so in the output
+  nan = __any_sync(0xffffffffu, nan);
+  const float il = nan || *A.status ? CUDART_NAN_F : L == 0.f ? 0.f : 1.f / L;
+  const __nv_bfloat162 y0 = __floats2bfloat162_rn(a.x * il, a.y * il);
+  const __nv_bfloat162 y1 = __floats2bfloat162_rn(a.z * il, a.w * il);
+  __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(A.out) + b * A.obs + j * A.oqs + hq * A.ohs +
+                       4 * lane;
+  if (A.out_vec4) {
+    uint2 pk;
+    pk.x = *reinterpret_cast<const uint32_t*>(&y0);
+    pk.y = *reinterpret_cast<const uint32_t*>(&y1);
+    *reinterpret_cast<uint2*>(dst) = pk;
+  } else {
+    dst[0] = y0.x; dst[1] = y0.y; dst[2] = y1.x; dst[3] = y1.y;
+  }
+}
+
+// The shapes of the tensor-core path; every other shape reads each row's pages
+// by itself (its kernels are bound by their arithmetic, not by the bytes that
+// sharing saves).
+static bool px_fast(int dtype, int D, int group) {
+  return dtype == SD_DTYPE_BF16 && D == PX_D && group <= 32;
+}
+
+struct PxLayout {
+  size_t ints, acc, ml, sacc, sml, bytes;
+  int max_items, qc, chunks, slots;
+};
+static PxLayout px_layout(int B, int G, int Hq, int Hkv, int qlen) {
+  PxLayout L;
+  const int group = Hq / Hkv, R = qlen * group;
+  L.max_items = (int)std::min<int64_t>((int64_t)Hkv * ((int64_t)B * R / PX_ROWS + G), 1 << 28);
+  L.qc = std::min(qlen, 32 / group);
+  L.chunks = (qlen + L.qc - 1) / L.qc;
+  L.slots = B * Hkv + PX_CTAS;
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  const size_t n1 = (size_t)(L.max_items + PX_CTAS) * PX_ROWS;
+  const size_t n2 = (size_t)L.chunks * L.slots * L.qc * group;
+  size_t o = up((5 * (size_t)G + 2 + 4 * (size_t)B + 2) * sizeof(int));
+  L.ints = 0;
+  L.acc = o; o = up(o + n1 * PX_D * sizeof(float));
+  L.ml = o; o = up(o + n1 * 2 * sizeof(float));
+  L.sacc = o; o = up(o + n2 * PX_D * sizeof(float));
+  L.sml = o; o = up(o + n2 * 2 * sizeof(float));
+  L.bytes = o;
+  return L;
+}
+
+}  // namespace sd
+
+using namespace sd;
+
+extern "C" {
+
+size_t sd_prefix_attn_workspace_bytes(int B, int G, int Hq, int Hkv, int D, int W, int qlen,
+                                      int dtype) {
+  if (B <= 0 || G < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || W <= 0 || qlen <= 0) return 0;
+  if ((int64_t)W * SD_KV_PAGE > 0x7FFFFFFF) return 0;
+  if (!px_fast(dtype, D, Hq / Hkv))
+    return sd_verify_attn_workspace_bytes(B, Hq, Hkv, D, W * SD_KV_PAGE, qlen);
+  return px_layout(B, G, Hq, Hkv, qlen).bytes;
+}
+
+int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const void* kpool,
+                   const void* vpool, const int32_t* block_table, int bt_stride, int npages,
+                   const int64_t* lengths, const int64_t* valid, const int32_t* group_starts,
+                   const int32_t* prefix_pages, int G, int B, int Hq, int Hkv, int D, int qlen,
+                   float scale, void* out, int64_t obs, int64_t oqs, int64_t ohs, int dtype,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  if (B < 0 || G < 0 || qlen < 0) return SD_EINVAL;
+  if (B == 0 || qlen == 0) return SD_OK;
+  if (!q || !kpool || !vpool || !block_table || !lengths || !out) return SD_EINVAL;
+  if (G > 0 && (!group_starts || !prefix_pages)) return SD_EINVAL;
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || bt_stride <= 0 || npages <= 0) return SD_EINVAL;
+  if (!(scale > 0.f) || scale > 3e38f) return SD_EINVAL;
+  if (dtype != SD_DTYPE_BF16 && dtype != SD_DTYPE_F32) return SD_ENOTSUP;
+  if ((int64_t)bt_stride * SD_KV_PAGE > 0x7FFFFFFF) return SD_ENOTSUP;
+  const int group = Hq / Hkv;
+  if (!px_fast(dtype, D, group))
+    return sd_verify_attn_paged(q, qbs, qhs, qqs, kpool, vpool, block_table, bt_stride, npages,
+                                lengths, valid, B, Hq, Hkv, D, qlen, scale, out, obs, oqs, ohs,
+                                dtype, workspace, workspace_bytes, stream);
+  // 16-byte loads of q rows and TMA boxes of the pools
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || qbs % 8 || qhs % 8 || qqs % 8 ||
+      (reinterpret_cast<uintptr_t>(kpool) & 15) || (reinterpret_cast<uintptr_t>(vpool) & 15))
+    return SD_EINVAL;
+  const int64_t rows = (int64_t)npages * Hkv * SD_KV_PAGE;
+  if (rows >= (int64_t)1 << 31) return SD_ENOTSUP;
+  // the schedules count units in 32 bits
+  const int64_t R = (int64_t)qlen * group;
+  if (R * B > 0x7FFFFFFF || (int64_t)B * Hkv * (bt_stride + ATTN_SEG_OVH) > 0x7FFFFFFF ||
+      (int64_t)Hkv * (B * R / PX_ROWS + G) * (bt_stride + PX_OVH) > 0x7FFFFFFF)
+    return SD_ENOTSUP;
+  const PxLayout L = px_layout(B, G, Hq, Hkv, qlen);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < L.bytes)
+    return SD_ENOSPC;
+  char* ws = reinterpret_cast<char*>(workspace);
+  PrefixParams P = {};
+  AttnParams& A = P.A;
+  A.q = q; A.qbs = qbs; A.qhs = qhs; A.qqs = qqs;
+  A.k = kpool; A.v = vpool; A.lengths = lengths; A.valid = valid;
+  A.B = B; A.Hq = Hq; A.Hkv = Hkv; A.D = D; A.C = bt_stride * SD_KV_PAGE; A.qlen = qlen;
+  A.group = group; A.R = (int)R; A.scale = scale;
+  A.out = out; A.obs = obs; A.oqs = oqs; A.ohs = ohs;
+  A.out_vec4 = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && obs % 4 == 0 && oqs % 4 == 0 &&
+               ohs % 4 == 0;
+  A.bt = block_table; A.bt_stride = bt_stride; A.npages = npages;
+  A.tile_keys = SD_KV_PAGE; A.seg_ovh = ATTN_SEG_OVH;
+  A.qc = L.qc; A.slots = L.slots; A.ncta = PX_CTAS;
+  P.starts = group_starts; P.pages = prefix_pages; P.G = G; P.max_items = L.max_items;
+  int* in = reinterpret_cast<int*>(ws + L.ints);
+  P.g_unit = in; in += G + 1;
+  P.g_item = in; in += G + 1;
+  P.g_row0 = in; in += G;
+  P.g_rows = in; in += G;
+  P.g_pages = in; in += G;
+  P.rowgroup = in; in += B;
+  A.rowstart = in; in += B;
+  A.rowkmax = in; in += B;
+  A.rowpre = in; in += B + 1;
+  A.status = in;
+  P.pacc = reinterpret_cast<float*>(ws + L.acc);
+  P.pml = reinterpret_cast<float*>(ws + L.ml);
+  A.part_acc = reinterpret_cast<float*>(ws + L.sacc);
+  A.part_ml = reinterpret_cast<float*>(ws + L.sml);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  CUtensorMap mk, mv;
+  if (!cache_map(&mk, kpool, rows) || !cache_map(&mv, vpool, rows)) return SD_ENOTSUP;
+  const int sm = (int)sizeof(PxSmem) + 1024;         // + room to align to 1024 B
+  if (cudaFuncSetAttribute(prefix_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) !=
+      cudaSuccess)
+    return SD_ELAUNCH;
+  prefix_plan_kernel<<<1, 1024, 0, st>>>(P);
+  if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
+  if (G > 0) {
+    prefix_tc_kernel<<<PX_CTAS, PX_THREADS, sm, st>>>(P, mk, mv);
+    if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
+  }
+  if (int rc = launch_suffix(A, st)) return rc;
+  const int64_t warps = (int64_t)B * qlen * Hq, per = PX_JOIN_THREADS / 32;
+  prefix_join_kernel<<<(unsigned)((warps + per - 1) / per), PX_JOIN_THREADS, 0, st>>>(P);
+  return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
+}
+
+}  // extern "C"

@@ -62,6 +62,10 @@ _SIGNATURES = {
     "sd_verify_attn": ([_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
                         _i32, _f32, _vp, _i64, _i64, _i64, _i32, _vp, _sz, _vp], _i32),
     "sd_verify_attn_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32], _sz),
+    "sd_prefix_attn_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32], _sz),
+    "sd_prefix_attn": ([_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32,
+                        _i32, _i32, _i32, _i32, _i32, _f32, _vp, _i64, _i64, _i64, _i32, _vp, _sz,
+                        _vp], _i32),
     "sd_shard_workspace_bytes": ([_i32, _i32, _i32], _sz),
     "sd_shard_send_bytes": ([_i32, _i32, _i32, _i32, _i32], _sz),
     "sd_shard_phase": ([_vp, _i32, _vp, _vp, _vp], _i32),

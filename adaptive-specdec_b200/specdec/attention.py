@@ -5,7 +5,8 @@ attention where query j of row b reads cache slots s <= lengths[b] + j (and
 s < valid[b] in a right-padded prefill).  It replaces the reference's HF SDPA
 over ``_RaggedLayer.update``'s max-width view plus the additive mask
 (specdec/kvcache.py:61-74 and :138-162, called at specdec/engine.py:274): each
-row reads only its own live keys.
+row reads only its own live keys.  ``prefix_attention`` is the same over a paged
+cache whose rows share their first pages (sd_prefix_attn).
 
 ``register()`` installs it as the transformers attention implementation
 "specdec_b200" (with a mask function that builds no mask); a model loaded with
@@ -101,6 +102,80 @@ def _verify_attention_paged(q, kpool, vpool, lengths, valid, scale, out, bt):
             W, npages, L.ptr(lens), L.ptr(val), B, Hq, Hkv, D, qlen, sc, L.ptr(out), out.stride(0),
             out.stride(1), out.stride(2), _ATTN_DTYPES[q.dtype], L.ptr(ws), ws.numel(),
             L.stream_ptr(q.device)), "verify_attn_paged")
+    return out
+
+
+def prefix_attention(q, k_pool, v_pool, lengths, block_table, group_starts, prefix_pages,
+                     valid=None, scale=None, out=None):
+    """``verify_attention`` over a paged cache whose rows share pages in front.
+
+    q [B, Hq, qlen, D], pools [n_pages, Hkv, PAGE, D], ``lengths`` [B] and
+    ``block_table`` [B, W] int32 as in ``verify_attention`` -> out [B, qlen, Hq,
+    D].  Group g is the rows ``group_starts[g]`` .. ``group_starts[g + 1]`` (int32
+    [G + 1] on the device, rising) whose first ``prefix_pages[g]`` (int32 [G])
+    table entries are equal: samples of one prompt, requests under one system
+    prompt.  Their keys are read once for the group instead of once per row.
+    The result is ``verify_attention``'s but for the order of the float32 sums.
+    Both group arrays live on the device, so a captured call follows them.
+    bf16 heads of 128 share; other shapes are computed row by row.
+    """
+    from specdec.kvcache import PAGE
+    L.require_cuda(q, k_pool, v_pool, lengths, block_table, group_starts, prefix_pages, valid, out)
+    if q.dim() != 4 or k_pool.dim() != 4:
+        raise L.SpecdecError("prefix_attention needs q [B, Hq, qlen, D] and pools "
+                             "[n_pages, Hkv, PAGE, D]")
+    if q.dtype not in _ATTN_DTYPES or k_pool.dtype != q.dtype or v_pool.dtype != q.dtype:
+        raise L.SpecdecError(f"prefix_attention supports bf16 / fp32, got {q.dtype}")
+    B, Hq, qlen, D = q.shape
+    npages, Hkv, page, Dk = k_pool.shape
+    if page != PAGE or Dk != D or v_pool.shape != k_pool.shape or not (
+            k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise L.SpecdecError("paged caches must be contiguous [n_pages, Hkv, PAGE, D] pools")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B \
+            or not block_table.is_contiguous():
+        raise L.SpecdecError("block_table must be a contiguous [B, W] int32 tensor")
+    G = prefix_pages.numel()
+    if group_starts.dtype != torch.int32 or prefix_pages.dtype != torch.int32 or \
+            group_starts.numel() != G + 1 or not (group_starts.is_contiguous()
+                                                  and prefix_pages.is_contiguous()):
+        raise L.SpecdecError("group_starts [G + 1] and prefix_pages [G] must be contiguous int32")
+    if lengths.numel() != B or (valid is not None and valid.numel() != B):
+        raise L.SpecdecError(f"lengths and valid need one entry per row ({B})")
+    dev = q.device
+    for t in (k_pool, v_pool, lengths, block_table, group_starts, prefix_pages, valid, out):
+        if t is not None and t.device != dev:
+            raise L.SpecdecError("prefix_attention needs every tensor on one device")
+    sc = float(scale) if scale is not None else D ** -0.5
+    if not 0.0 < sc < 3e38:
+        raise L.SpecdecError(f"scale must be positive and finite, got {scale}")
+    if out is None:
+        out = torch.empty(B, qlen, Hq, D, dtype=q.dtype, device=dev)
+    elif out.shape != (B, qlen, Hq, D) or out.dtype != q.dtype or (D > 1 and out.stride(3) != 1):
+        raise L.SpecdecError(f"out must be {(B, qlen, Hq, D)} of {q.dtype}, contiguous along D")
+    if B == 0 or qlen == 0:
+        return out
+    if q.stride(-1) != 1 or (q.dtype == torch.bfloat16 and D == 128 and (
+            q.data_ptr() % 16 or any(q.stride(i) % 8 for i in range(3)))):
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+    lens = lengths if lengths.dtype == torch.long and lengths.is_contiguous() \
+        else lengths.long().contiguous()
+    val = None if valid is None else valid.long().contiguous()
+    W = block_table.shape[1]
+    lib = L.lib()
+    with torch.cuda.device(dev):
+        # a fresh buffer per call: calls on several streams and calls captured
+        # into different graphs never share one
+        ws = torch.empty(lib.sd_prefix_attn_workspace_bytes(B, G, Hq, Hkv, D, W, qlen,
+                                                            _ATTN_DTYPES[q.dtype]),
+                         dtype=torch.uint8, device=dev)
+        L.check(lib.sd_prefix_attn(
+            L.ptr(q), q.stride(0), q.stride(1), q.stride(2), L.ptr(k_pool), L.ptr(v_pool),
+            L.ptr(block_table), W, npages, L.ptr(lens), L.ptr(val), L.ptr(group_starts),
+            L.ptr(prefix_pages), G, B, Hq, Hkv, D, qlen, sc, L.ptr(out), out.stride(0),
+            out.stride(1), out.stride(2), _ATTN_DTYPES[q.dtype], L.ptr(ws), ws.numel(),
+            L.stream_ptr(dev)), "prefix_attn")
     return out
 
 

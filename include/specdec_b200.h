@@ -374,6 +374,33 @@ int sd_verify_attn_paged(const void* q, int64_t qbs, int64_t qhs, int64_t qqs,
                          size_t workspace_bytes, void* stream);
 
 /*
+ * sd_verify_attn_paged for rows that share pages in front (no counterpart in
+ * the reference): the samples of one prompt, requests under one system
+ * prompt.  Group g holds rows group_starts[g] .. group_starts[g + 1) (int32
+ * [G + 1], rising) whose first prefix_pages[g] (int32 [G]) block-table entries
+ * are equal; the keys of those pages are read once for the whole group, at
+ * the entries of its first row.  Rows of no group share nothing.  Same masking
+ * as sd_verify_attn_paged, and the same result but for the order of the
+ * float32 sums; query rows without a visible key give 0.  A row whose first
+ * query does not see the whole shared range (a short length or cap) is
+ * computed from its own table alone.  Both arrays are device memory, so a
+ * captured call follows them.
+ * bf16 with D = 128 and Hq / Hkv <= 32 shares (q, kpool and vpool 16-byte
+ * aligned, q strides multiples of 8); other shapes of sd_verify_attn_paged
+ * are computed row by row.  scale > 0.  The workspace must be 256-byte aligned
+ * and, as a call writes all it reads, needs no initialisation.  If a bounded
+ * wait inside the kernels gives up, the output is NaN.
+ */
+size_t sd_prefix_attn_workspace_bytes(int B, int G, int Hq, int Hkv, int D, int W, int qlen,
+                                      int dtype);
+int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const void* kpool,
+                   const void* vpool, const int32_t* block_table, int bt_stride, int npages,
+                   const int64_t* lengths, const int64_t* valid, const int32_t* group_starts,
+                   const int32_t* prefix_pages, int G, int B, int Hq, int Hkv, int D, int qlen,
+                   float scale, void* out, int64_t obs, int64_t oqs, int64_t ohs, int dtype,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Vocabulary-sharded verify round: the SPMD form of sd_verify_sample for a
  * vocab-parallel LM head.  Rank r holds columns [v_start[r], v_start[r+1]) of
  * every target and draft logits vector; every rank ends with the n_acc and y
