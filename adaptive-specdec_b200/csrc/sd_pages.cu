@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(PT_THREADS) pages_reserve_plan_kernel(const Pa
   if (t == 0) P.starts[P.B] = (int32_t)tokens;
   int why = bad;
   if (!why && pages > had_free) why = SD_PAGES_ERR_EXHAUSTED;
-  if (!why && tokens > P.max_tokens) why = SD_PAGES_ERR_SLOTS;
+  if (!why && P.slots && tokens > P.max_tokens) why = SD_PAGES_ERR_SLOTS;
   __syncthreads();                                   // everybody has read n_free
   if (t == 0) {
     P.plan[2 * P.B] = had_free;
@@ -138,6 +138,7 @@ __global__ void __launch_bounds__(PF_THREADS) pages_reserve_fill_kernel(const Pa
     const int need = (int)((len + n + SD_KV_PAGE - 1) / SD_KV_PAGE);
     for (int p = had + lane; p < need; p += 32) row[p] = P.free_stack[top - (pre + p - had)];
   }
+  if (!P.slots) return;
   const int i1 = min(n, (run + 1) * P.run);
   for (int i = run * P.run + lane; i < i1; i += 32) {
     const int64_t pos = len + i;
@@ -228,11 +229,11 @@ int sd_pages_reserve(int32_t* block_table, int bt_stride, int W, int32_t* owned,
   P.bt = block_table; P.bt_stride = bt_stride; P.W = W; P.n_pages = n_pages; P.B = B;
   P.owned = owned; P.free_stack = const_cast<int32_t*>(free_stack); P.n_free = n_free;
   P.lengths = lengths; P.add = new_tokens; P.add_all = new_each;
-  P.slots = slots; P.max_tokens = max_tokens; P.starts = starts; P.err = err;
+  P.slots = slots; P.max_tokens = slots ? max_tokens : 0; P.starts = starts; P.err = err;
   P.plan = reinterpret_cast<int*>(workspace);
   if (int rc = pages_check(P)) return rc;
   if (B == 0) return SD_OK;
-  if (!starts || max_tokens < 0 || (max_tokens > 0 && !slots)) return SD_EINVAL;
+  if (!starts || max_tokens < 0) return SD_EINVAL;
   if (!new_tokens && new_each < 0) return SD_EINVAL;
   if (max_tokens > 0x7FFFFFFF) return SD_ENOTSUP;
   // starts is int32, and the scan packs the token count in 32 bits
@@ -242,13 +243,12 @@ int sd_pages_reserve(int32_t* block_table, int bt_stride, int W, int32_t* owned,
     return SD_ENOSPC;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int64_t most = std::min<int64_t>(
-      std::min<int64_t>(max_tokens, (int64_t)W * SD_KV_PAGE), new_tokens ? max_tokens : new_each);
+      std::min<int64_t>(P.max_tokens, (int64_t)W * SD_KV_PAGE), new_tokens ? P.max_tokens : new_each);
   P.run = 512;
   while ((most + P.run - 1) / P.run * B > 65536) P.run *= 2;
   P.runs = (int)std::max<int64_t>(1, (most + P.run - 1) / P.run);
-  // with one number for all rows every slot belongs to a row; else some warps
-  // for the slots behind the last token
-  const int64_t tail = (max_tokens + 4095) / 4096;
+  // some warps for the slots behind the last token
+  const int64_t tail = (P.max_tokens + 4095) / 4096;
   const int64_t warps = (int64_t)B * P.runs + std::min<int64_t>(std::max<int64_t>(tail, 1), 1024);
   pages_reserve_plan_kernel<<<1, PT_THREADS, 0, st>>>(P);
   if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;

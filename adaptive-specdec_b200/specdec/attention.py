@@ -208,8 +208,12 @@ def hf_attention(module, query, key, value, attention_mask, dropout=0.0, scaling
             out = torch.nn.functional.scaled_dot_product_attention(
                 query, ks, vs, is_causal=True, scale=scaling, enable_gqa=True)
             return out.transpose(1, 2), None
+        bt, prefix = getattr(cache, "block_table", None), getattr(cache, "prefix", None)
+        if prefix is not None:                      # a forked cache: rows share their prompt's pages
+            return prefix_attention(query, key, value, cache.lengths, bt, *prefix,
+                                    valid=cache.valid, scale=scaling), None
         out = verify_attention(query, key, value, cache.lengths, valid=cache.valid, scale=scaling,
-                               block_table=getattr(cache, "block_table", None))
+                               block_table=bt)
         return out, None
     # a forward without a RaggedCache: causal self-attention over the given
     # K/V, i.e. the same kernel with every row starting at length 0

@@ -32,6 +32,13 @@ Draws use uniforms from the round's torch.Generator, so runs are reproducible
 for a seed; the random stream differs from the reference's multinomial calls,
 so agreement with the reference is distributional (gate G1) and exact for
 greedy decoding (gate G2).
+
+Beyond the reference, ``generate(n=...)`` draws several samples per prompt: each
+prompt is prefilled once, its full cache pages are shared by its n rows (a
+forked PagedRaggedCache with its page table on the device) and read once per
+group by the verify attention; ``logprobs=...`` reports the target model's
+log-probability of every emitted token (and alternatives), which is what ranks
+the samples.
 """
 import time
 from dataclasses import dataclass, field
@@ -40,7 +47,7 @@ import torch
 
 from specdec import attention as A
 from specdec.kvcache import PAGE, PagedRaggedCache, RaggedCache
-from specdec.sampling import draft_sample, to_probs, verify_sample
+from specdec.sampling import TOP_N_MAX, draft_sample, to_probs, token_logprobs, verify_sample
 
 __all__ = ["SamplingConfig", "RunStats", "SpecDecodeEngine"]
 
@@ -72,6 +79,11 @@ class RunStats:
     accepted_at: list = field(default_factory=list)
     k_history: list = field(default_factory=list)
     accept_history: list = field(default_factory=list)
+    # with generate(logprobs=...), per row and emitted token: the target's
+    # log-probability (temperature 1, no top-p / top-k) and the alternatives
+    # [(id, log-probability), ...]
+    logprobs: list = field(default_factory=list)
+    top_logprobs: list = field(default_factory=list)
 
     def _grow(self, n):
         while len(self.offered_at) < n:
@@ -255,8 +267,19 @@ class SpecDecodeEngine:
         return ids
 
     # ---- plumbing ----------------------------------------------------------
-    def _mk_cache(self, model, batch, plen=None, max_new=0, k_max=16):
+    def _mk_cache(self, model, batch, plen=None, max_new=0, k_max=16, n=1):
         n_layers = model.config.num_hidden_layers
+        if n > 1:
+            # one row per prompt now, n after the fork: the prompt's pages once,
+            # a copy of its last page and the new tokens' pages per sample
+            n_pages = self.kv_pages
+            if n_pages is None:
+                pl = plen.to("cpu", torch.long)
+                grow = 2 * int(max_new) + 2 * (int(k_max) + 1)
+                own = ((pl % PAGE + grow).clamp(max=self.capacity) + PAGE - 1) // PAGE
+                n_pages = int(((pl + PAGE - 1) // PAGE).sum()) + n * int(own.sum()) + 1
+            return PagedRaggedCache(n_layers, batch, self.capacity, self.device, attn_impl=A.IMPL,
+                                    n_pages=n_pages, device_pages=True)
         if not self.paged_kv:
             return RaggedCache(n_layers, batch, self.capacity, self.device, attn_impl=A.IMPL)
         n_pages = self.kv_pages
@@ -308,6 +331,16 @@ class SpecDecodeEngine:
         cache.set_lengths(plen)
         return logits
 
+    @staticmethod
+    def _logprob_lists(logits, ids, top_n):
+        """(log-probabilities, [(id, log-probability), ...]) of ids [B, L] as lists."""
+        r = token_logprobs(logits, ids, top_n=int(top_n))
+        if not top_n:
+            return r.logprob.tolist(), None
+        top = [[list(zip(i, p)) for i, p in zip(ib, pb)]
+               for ib, pb in zip(r.top_ids.tolist(), r.top_logprobs.tolist())]
+        return r.logprob.tolist(), top
+
     def _sync_phase(self):
         if self.time_phases:
             torch.cuda.synchronize(self.device)
@@ -315,11 +348,20 @@ class SpecDecodeEngine:
     # ---- main loop ---------------------------------------------------------
     @torch.inference_mode()
     def generate(self, input_ids, plen, max_new_tokens, sampling=None, controller=None,
-                 seed=None, k_fixed=None):
+                 seed=None, k_fixed=None, n=1, logprobs=None):
         """input_ids [B, P] right-padded, plen [B] real prompt lengths.
+
+        ``n`` samples per prompt (rows of one prompt side by side: B * n lists);
+        ``logprobs`` (0 or more alternatives, None: off) fills the stats'
+        ``logprobs`` and ``top_logprobs`` per row and emitted token.
 
         Returns (list of generated id lists, RunStats).
         """
+        n = int(n)
+        if n < 1:
+            raise ValueError(f"n must be at least 1, got {n}")
+        if logprobs is not None and not 0 <= int(logprobs) <= min(TOP_N_MAX, self.vocab_size):
+            raise ValueError(f"logprobs must be None or between 0 and {TOP_N_MAX}, got {logprobs}")
         sp = sampling or SamplingConfig()
         T, tp, tk = sp.temperature, sp.top_p, sp.top_k
         dev = self.device
@@ -329,10 +371,11 @@ class SpecDecodeEngine:
         input_ids = input_ids.to(dev)
         plen = plen.to(dev)
         k_cap = int(k_fixed) if k_fixed is not None else int(getattr(controller, "k_max", 16))
-        tcache = self._mk_cache(self.target, B, plen, max_new_tokens, k_cap)
-        dcache = self._mk_cache(self.draft, B, plen, max_new_tokens, k_cap)
-        paged = self.paged_kv
-        st = RunStats(batch=B)
+        tcache = self._mk_cache(self.target, B, plen, max_new_tokens, k_cap, n)
+        dcache = self._mk_cache(self.draft, B, plen, max_new_tokens, k_cap, n)
+        paged = self.paged_kv and n == 1
+        device_pages = n > 1
+        st = RunStats(batch=B * n)
         t0 = time.perf_counter()
 
         with self._range("prefill"):
@@ -340,12 +383,20 @@ class SpecDecodeEngine:
             self._prefill(self.draft, dcache, input_ids, plen)
             st.target_forwards += 1
             st.draft_forwards += 1
+            if n > 1:
+                tcache, dcache = tcache.fork([n] * B), dcache.fork([n] * B)
+                tlog = tlog.repeat_interleave(n, 0)
+                B = B * n
 
         pending, _ = draft_sample(tlog, torch.rand(B, generator=gen, device=dev), T, tp, tk)
         pend_l = pending.tolist()
         out = [[int(pend_l[b])] for b in range(B)]
         done_l = [int(pend_l[b]) in self.eos_ids for b in range(B)]
         st.emitted += B
+        if logprobs is not None:
+            lp, top = self._logprob_lists(tlog.unsqueeze(1), pending.view(B, 1), logprobs)
+            st.logprobs = [list(r) for r in lp]
+            st.top_logprobs = [list(r) for r in top] if logprobs else []
         drf_buf = None
         graphs = None
         K_BUF = 8
@@ -368,6 +419,11 @@ class SpecDecodeEngine:
             if paged:
                 # pages for this round's k + 1 tokens per cache, from the
                 # lengths read back at the end of the last round (no sync)
+                dcache.reserve(k + 1)
+                tcache.reserve(k + 1)
+            elif device_pages:
+                # the same from the device lengths; a pool that ran out shows in
+                # the error flags read with the round's tokens
                 dcache.reserve(k + 1)
                 tcache.reserve(k + 1)
             conf = torch.ones(B, device=dev)
@@ -445,7 +501,20 @@ class SpecDecodeEngine:
                 cols = [n_acc.view(B, 1), y.view(B, 1), xs]
                 if paged:
                     cols += [tcache.lengths.view(B, 1), dcache.lengths.view(B, 1)]
+                if device_pages:
+                    cols += [(tcache._err | dcache._err).long().expand(B).view(B, 1)]
                 host = torch.cat(cols, dim=1).tolist()
+                if device_pages and host[0][-1]:
+                    tcache.check_errors()
+                    dcache.check_errors()
+                if logprobs is not None:
+                    # token i of a row under the logits before it: the accepted
+                    # drafts, then y; -1 past that
+                    at = torch.arange(k_eff + 1, device=dev).view(1, -1)
+                    emitted = torch.where(at < n_acc.view(B, 1),
+                                          torch.cat([xs, y.view(B, 1)], dim=1),
+                                          torch.where(at == n_acc.view(B, 1), y.view(B, 1), -1))
+                    lp, top = self._logprob_lists(vlog, emitted, logprobs)
                 if paged:
                     tcache.set_host_lengths([r[-2] for r in host])
                     dcache.set_host_lengths([r[-1] for r in host])
@@ -465,6 +534,10 @@ class SpecDecodeEngine:
                     tok = row[2 + j]
                     out[b].append(tok)
                     st.emitted += 1
+                    if logprobs is not None:
+                        st.logprobs[b].append(lp[b][j])
+                        if logprobs:
+                            st.top_logprobs[b].append(top[b][j])
                     if tok in self.eos_ids or len(out[b]) >= max_new_tokens:
                         done_l[b] = True
                         break
@@ -472,6 +545,10 @@ class SpecDecodeEngine:
                     continue
                 out[b].append(row[1])
                 st.emitted += 1
+                if logprobs is not None:
+                    st.logprobs[b].append(lp[b][n_acc_l[b]])
+                    if logprobs:
+                        st.top_logprobs[b].append(top[b][n_acc_l[b]])
                 if row[1] in self.eos_ids or len(out[b]) >= max_new_tokens:
                     done_l[b] = True
             pending = y
@@ -486,8 +563,12 @@ class SpecDecodeEngine:
 
     # ---- baseline ----------------------------------------------------------
     @torch.inference_mode()
-    def generate_autoregressive(self, input_ids, plen, max_new_tokens, sampling=None, seed=None):
-        """Target-only decoding through the same cache, attention and sampling kernels."""
+    def generate_autoregressive(self, input_ids, plen, max_new_tokens, sampling=None, seed=None,
+                                logprobs=None):
+        """Target-only decoding through the same cache, attention and sampling kernels
+        (``logprobs`` as in ``generate``)."""
+        if logprobs is not None and not 0 <= int(logprobs) <= min(TOP_N_MAX, self.vocab_size):
+            raise ValueError(f"logprobs must be None or between 0 and {TOP_N_MAX}, got {logprobs}")
         sp = sampling or SamplingConfig()
         T, tp, tk = sp.temperature, sp.top_p, sp.top_k
         dev = self.device
@@ -505,6 +586,10 @@ class SpecDecodeEngine:
         out = [[int(nl[b])] for b in range(B)]
         done_l = [int(nl[b]) in self.eos_ids for b in range(B)]
         st.emitted += B
+        if logprobs is not None:
+            lp, top = self._logprob_lists(logits.unsqueeze(1), nxt.view(B, 1), logprobs)
+            st.logprobs = [list(r) for r in lp]
+            st.top_logprobs = [list(r) for r in top] if logprobs else []
         while not all(done_l):
             if isinstance(cache, PagedRaggedCache):
                 cache.reserve(1)
@@ -514,11 +599,17 @@ class SpecDecodeEngine:
             st.target_forwards += 1
             nxt, _ = draft_sample(logits, torch.rand(B, generator=gen, device=dev), T, tp, tk)
             nl = nxt.tolist()
+            if logprobs is not None:
+                lp, top = self._logprob_lists(logits.unsqueeze(1), nxt.view(B, 1), logprobs)
             for b in range(B):
                 if done_l[b]:
                     continue
                 out[b].append(nl[b])
                 st.emitted += 1
+                if logprobs is not None:
+                    st.logprobs[b].append(lp[b][0])
+                    if logprobs:
+                        st.top_logprobs[b].append(top[b][0])
                 if nl[b] in self.eos_ids or len(out[b]) >= max_new_tokens:
                     done_l[b] = True
         st.t_total = time.perf_counter() - t0

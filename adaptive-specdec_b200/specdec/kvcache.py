@@ -496,16 +496,19 @@ class DevicePageTable:
             raise L.SpecdecError(f"{name} must be an integer [B] tensor on {self.device}")
         return t if t.dtype == torch.long and t.is_contiguous() else t.long().contiguous()
 
-    def reserve(self, lengths, new, max_tokens=None):
+    def reserve(self, lengths, new, max_tokens=None, slot_map=True):
         """Pages for ``new`` more tokens of every row past ``lengths`` [B].
 
         ``new`` is one int for all rows or an integer [B] tensor; with a tensor
         ``max_tokens`` bounds their sum (the size of ``slots``).  Returns
         (slots [max_tokens] int64, starts [B + 1] int32): token i of row b goes
         to pool slot slots[starts[b] + i] = page * PAGE + offset; slots behind
-        the last token are -1.
+        the last token are -1.  ``slot_map=False`` leaves the map out: (None,
+        starts).
         """
         lens = self._rows(lengths, "lengths")
+        if not slot_map:
+            max_tokens = 0
         if torch.is_tensor(new):
             if max_tokens is None:
                 raise L.SpecdecError("max_tokens is needed with per-row token counts")
@@ -519,7 +522,9 @@ class DevicePageTable:
             raise L.SpecdecError(f"max_tokens must not be negative, got {total}")
         lib = L.lib()
         with torch.cuda.device(self.device):
-            slots = torch.empty(total, dtype=torch.long, device=self.device)
+            # (an empty map still has an address: NULL means no map)
+            slots = torch.empty(max(total, 1), dtype=torch.long, device=self.device) \
+                if slot_map else None
             starts = torch.empty(self.B + 1, dtype=torch.int32, device=self.device)
             ws = torch.empty(lib.sd_pages_workspace_bytes(self.B), dtype=torch.uint8,
                              device=self.device)
@@ -528,7 +533,7 @@ class DevicePageTable:
                 L.ptr(self.free), self.n_pages, L.ptr(self.n_free), L.ptr(lens), L.ptr(add), each,
                 self.B, L.ptr(slots), total, L.ptr(starts), L.ptr(self.err), L.ptr(ws), ws.numel(),
                 L.stream_ptr(self.device)), "pages_reserve")
-        return slots, starts
+        return (slots[:total] if slot_map and total == 0 else slots), starts
 
     def trim(self, lengths):
         """Give back every row's pages past its ``lengths`` [B] tokens (never
@@ -573,6 +578,12 @@ class PagedRaggedCache(RaggedCache):
     grows back into them); ``release(rows)`` and ``reset()`` return them.
     A slot written without a page sets the device error flag (bit 1).
 
+    With ``device_pages`` the bookkeeping is a DevicePageTable: ``reserve``
+    follows the device lengths with no host copy of them, a pool that runs out
+    sets the error flag instead of raising, and ``fork`` makes several rows
+    of each prompt that share its pages.  ``prefix`` (group starts, shared
+    pages) then tells the attention which rows share what.
+
     Only the kernel attention path (attn_impl "specdec_b200") reads paged
     layers.
     """
@@ -580,13 +591,20 @@ class PagedRaggedCache(RaggedCache):
     _layer_cls = _PagedLayer
 
     def __init__(self, n_layers, batch_size, capacity, device, attn_impl="specdec_b200",
-                 n_pages=None):
+                 n_pages=None, device_pages=False, _stack=None):
         if attn_impl != "specdec_b200":
             raise L.SpecdecError("PagedRaggedCache is read by the specdec_b200 attention only")
         self.pages_per_row = -(-int(capacity) // PAGE)
         super().__init__(n_layers, batch_size, self.pages_per_row * PAGE, device, attn_impl)
         self.n_pages = int(n_pages) if n_pages is not None else \
             self.batch_size * self.pages_per_row + 1
+        self.device_pages = bool(device_pages)
+        self.prefix = None
+        if self.device_pages:
+            self.pages = DevicePageTable(self.batch_size, self.pages_per_row, self.n_pages,
+                                         self.device, err=self._err, stack=_stack)
+            self.block_table = self.pages.block_table
+            return
         self.pages = PageTable(self.batch_size, self.pages_per_row, self.n_pages)
         self.block_table = torch.full((self.batch_size, self.pages_per_row), -1,
                                       dtype=torch.int32, device=self.device)
@@ -594,43 +612,126 @@ class PagedRaggedCache(RaggedCache):
     # ---- pages -------------------------------------------------------------
     @property
     def free_pages(self):
-        return len(self.pages.free)
+        return int(self.pages.n_free) if self.device_pages else len(self.pages.free)
 
     def _push(self, changed=True):
         if changed:
             self.block_table.copy_(torch.from_numpy(self.pages.bt))
 
+    def _columns(self):
+        return torch.arange(self.pages_per_row, device=self.device).view(1, -1)
+
     def reserve(self, q):
         """Pages for the next q tokens of every row (call before the forward)."""
+        if self.device_pages:
+            self.pages.reserve(self.lengths, int(q), slot_map=False)
+            return
         self._push(self.pages.reserve(self._mirror().numpy(), q))
 
     def reserve_prefill(self, P, plen):
         """Pages for a right-padded prefill of P tokens with prompt lengths
         plen (real pages for each row's prompt, the sink for its padding)."""
+        if self.device_pages:
+            pl = torch.as_tensor(plen).to(self.device, torch.long).reshape(-1).clamp(max=int(P))
+            self.pages.reserve(self.lengths, pl, slot_map=False)
+            top = (self.lengths + int(P) + PAGE - 1) // PAGE
+            pad = (self._columns() < top.view(-1, 1)) & (self.block_table < 0)
+            self.block_table.masked_fill_(pad, self.pages.sink)
+            return
         pl = torch.as_tensor(plen).to("cpu", torch.long).reshape(-1).numpy()
         self._push(self.pages.reserve_prefill(self._mirror().numpy(), P, pl))
 
     def release(self, rows):
-        """Return the pages of the given rows to the pool (their lengths go to 0)."""
+        """Return the pages of the given rows to the pool (their lengths go to 0).
+        Shared pages of a forked row stay with the rows that still read them."""
         rows = [int(r) for r in rows]
+        if self.device_pages:
+            at = torch.tensor(rows, dtype=torch.long, device=self.device)
+            keep = self.pages.owned.long() * PAGE
+            keep[at] = 0
+            self.pages.trim(keep)
+            self.lengths[at] = 0
+            self.block_table[at] = -1
+            self.pages.owned[at] = 0
+            self.pages.shared[at] = 0
+            if self._host_valid:
+                self._host[rows] = 0
+            return
         h = self._mirror().clone()
         h[rows] = 0
         self.pages.release(rows)
         self.set_lengths(h)
         self._push()
 
+    def fork(self, counts):
+        """counts[b] rows for each row b, which share the full pages of row b;
+        its last, partly filled page is copied to each.  Returns the new cache
+        (rows of one source row side by side) over the same pools; this cache
+        is left empty and must not be used further.  The shared pages go back
+        with the new cache's ``reset``.  Synchronises once (error check)."""
+        if not self.device_pages:
+            raise L.SpecdecError("fork needs device_pages=True")
+        counts = [int(c) for c in counts]
+        if len(counts) != self.batch_size or min(counts) < 1:
+            raise L.SpecdecError(f"fork needs one positive count per row ({self.batch_size})")
+        host = self._mirror().clone()
+        src = torch.repeat_interleave(torch.arange(self.batch_size), torch.tensor(counts))
+        new = PagedRaggedCache(len(self.layers), len(src), self.capacity, self.device,
+                               n_pages=self.n_pages, device_pages=True,
+                               _stack=(self.pages.free, self.pages.n_free))
+        lens, full = host[src], host[src] // PAGE
+        srcd, fulld = src.to(self.device), full.to(self.device)
+        table = torch.where(new._columns() < fulld.view(-1, 1), self.block_table[srcd], -1)
+        new.block_table.copy_(table)
+        new.pages.owned.copy_(fulld)
+        new.pages.shared.copy_(fulld)
+        new.set_lengths(lens)
+        new.pages.reserve(new.lengths, 0, slot_map=False)
+        new.check_errors()
+        part = torch.nonzero(lens % PAGE).view(-1).to(self.device)
+        old_page = self.block_table[srcd[part], fulld[part]].long()
+        new_page = new.block_table[part, fulld[part]].long()
+        for a, b in zip(self.layers, new.layers):
+            if not a.is_initialized:
+                continue
+            for pool in (a.keys, a.values):
+                pool[new_page] = pool[old_page]
+            b.dtype, b.device, b.is_initialized = a.dtype, a.device, True
+            b.keys, b.values = a.keys[:], a.values[:]
+            b.keys._sd_cache = b.values._sd_cache = new
+        # the copies are taken: the partly filled source pages go back
+        self.pages.shared.copy_(host // PAGE)
+        self.pages.trim(self.lengths // PAGE * PAGE)
+        self.block_table.fill_(-1)
+        self.pages.owned.zero_()
+        self.pages.shared.zero_()
+        self.set_lengths(torch.zeros(self.batch_size, dtype=torch.long))
+        starts = torch.tensor([0] + counts).cumsum(0)
+        new.prefix = (starts.to(self.device, torch.int32),
+                      (host // PAGE).to(self.device, torch.int32))
+        return new
+
     def set_lengths(self, lengths):
         super().set_lengths(lengths)
+        if self.device_pages:
+            self.block_table.masked_fill_(self.block_table == self.pages.sink, -1)
+            return
         self._push(self.pages.unsink())
 
     def reset(self):
         super().reset()
+        self.prefix = None
+        if self.device_pages:
+            self.pages.reset()
+            return
         self._push(self.pages.reset())
 
     def check_errors(self):
         e = int(self._err.item())
         if e:
             self._err.zero_()
+            if e & 4:
+                raise L.SpecdecError("KV page pool exhausted")
             if e & 2:
                 raise RuntimeError("PagedRaggedCache: a slot was written without a page "
                                    "(reserve() before the forward)")

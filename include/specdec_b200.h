@@ -255,6 +255,7 @@ int sd_kv_append_paged(void* kpool, void* vpool, const void* new_k, const void* 
  * counts) and slots [max_tokens]: token i of row b gets
  *   slots[starts[b] + i] = page * SD_KV_PAGE + offset
  * of cache position lengths[b] + i; slots behind the last token are -1.
+ * With slots NULL there is no slot map and max_tokens does not count.
  * Rows keep the pages they have: nothing is given back.
  *
  * sd_pages_trim gives back every row's pages past max(ceil(lengths[b] /

@@ -225,6 +225,17 @@ def test_nothing_to_reserve_and_more_room_than_tokens():
 
 
 @gpu
+def test_reserve_without_a_slot_map():
+    a, b = DevicePageTable(5, 6, 40, DEV), DevicePageTable(5, 6, 40, DEV)
+    new = _lens([0, 5, 600, 128, 1])
+    slots, starts = a.reserve(_lens([0] * 5), new, slot_map=False)
+    want, want_starts = b.reserve(_lens([0] * 5), new, max_tokens=800)
+    assert slots is None and torch.equal(starts, want_starts)
+    assert torch.equal(a.block_table, b.block_table) and torch.equal(a.n_free, b.n_free)
+    assert int(a.err) == 0
+
+
+@gpu
 def test_refusals():
     t = DevicePageTable(3, 4, 20, DEV)
     with pytest.raises(L.SpecdecError):
@@ -265,7 +276,7 @@ def test_arguments_are_checked_before_any_launch():
     assert reserve(B=0) == 0
     assert reserve(B=-1) == -22 and reserve(bt=n) == -22 and reserve(lens=n) == -22
     assert reserve(W=0) == -22 and reserve(stride=3) == -22 and reserve(pages=0) == -22
-    assert reserve(slots=n) == -22 and reserve(room=-1) == -22 and reserve(each=-1) == -22
+    assert reserve(room=-1) == -22 and reserve(each=-1) == -22
     assert reserve(W=1 << 25, stride=1 << 25) == -95
     assert reserve(B=1 << 20, W=1 << 10, stride=1 << 10, nws=1 << 30) == -95
     assert reserve(ws=n) == -28 and reserve(nws=16) == -28

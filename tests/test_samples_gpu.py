@@ -1,0 +1,261 @@
+"""Several samples per prompt: the device page table, the forked cache, the
+shared-prefix attention and the token log-probabilities together.
+
+Cache comparisons are exact.  fp32 tiny models attend row by row on the CUDA
+cores whether rows share or not, so their greedy tokens are equal, too.  The
+log-probability comparisons are between two fp32 forwards of the same 2-layer
+model (other batch sizes, or the engine's and a plain teacher-forced one): float32 rounding through
+about 10 dependent matrix products of widths up to 64 and logits of order 1 is
+within 10 * 64 * 2^-24 * 4 = 1.6e-4 of scale; 1e-3 is asserted.
+"""
+import copy
+
+import pytest
+import torch
+from transformers import Qwen3Config, Qwen3ForCausalLM
+
+from specdec import _lib as L
+from specdec import attention as A
+from specdec.engine import SamplingConfig, SpecDecodeEngine
+from specdec.kvcache import PAGE, DevicePageTable, PagedRaggedCache, PageTable
+from tests.tiny_models import VOCAB, TinyTok, tiny_pair_noisy
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+
+
+def _filled(lens, n_pages, H=2, D=128, layers=2, seed=0):
+    """A device-paged cache with `lens` random tokens per row."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    B, P = len(lens), max(lens)
+    c = PagedRaggedCache(layers, B, 1024, DEV, n_pages=n_pages, device_pages=True)
+    c.reserve_prefill(P, torch.tensor(lens))
+    kv = [(torch.randn(B, H, P, D, generator=g, device=DEV).bfloat16(),
+           torch.randn(B, H, P, D, generator=g, device=DEV).bfloat16()) for _ in range(layers)]
+    for lay, (k, v) in zip(c.layers, kv):
+        lay.update(k, v)
+    c.set_lengths(torch.tensor(lens))
+    c.check_errors()
+    return c, kv
+
+
+def test_device_pages_prefill_like_the_host_tables():
+    lens = [5, 300, 128, 257]
+    c, kv = _filled(lens, 40)
+    h = PagedRaggedCache(2, 4, 1024, DEV, n_pages=40)
+    h.reserve_prefill(300, torch.tensor(lens))
+    for lay, (k, v) in zip(h.layers, kv):
+        lay.update(k, v)
+    h.set_lengths(torch.tensor(lens))
+    assert torch.equal(c.block_table, h.block_table)
+    for a, b in zip(c.layers, h.layers):
+        assert torch.equal(a.keys[:39], b.keys[:39]) and torch.equal(a.values[:39], b.values[:39])
+    for _ in range(30):
+        for x in (c, h):
+            x.reserve(9)
+            x.layers[0].update(kv[0][0][:, :, :9], kv[0][1][:, :, :9])
+            x.advance(9)
+        assert torch.equal(c.block_table, h.block_table)
+    c.check_errors()
+    assert c.free_pages == h.free_pages
+    c.release([1, 3])
+    h.release([1, 3])
+    assert c.free_pages == h.free_pages and c.lengths.tolist() == h.lengths.tolist()
+    c.reset()
+    assert c.free_pages == 39 and bool((c.block_table == -1).all())
+
+
+def test_fork_shares_full_pages_and_copies_the_last():
+    lens = [5, 300, 128, 257]
+    c, kv = _filled(lens, 60)
+    want = [[A.gather_pages(p, c.block_table, 512).clone() for p in (l.keys, l.values)]
+            for l in c.layers]
+    old = c.block_table.clone()
+    free = c.free_pages
+    f = c.fork([3, 1, 2, 4])
+    src = [0] * 3 + [1] + [2] * 2 + [3] * 4
+    assert f.lengths.tolist() == [lens[s] for s in src]
+    assert f.prefix[0].tolist() == [0, 3, 4, 6, 10] and f.prefix[1].tolist() == [0, 2, 1, 2]
+    for l, w in zip(f.layers, want):
+        for pool, ww in zip((l.keys, l.values), w):
+            got = A.gather_pages(pool, f.block_table, 512)
+            for b, s in enumerate(src):
+                assert torch.equal(got[b, :, :lens[s]], ww[s, :, :lens[s]])
+    bt = f.block_table.tolist()
+    for b, s in enumerate(src):
+        full = lens[s] // PAGE
+        assert bt[b][:full] == old[s, :full].tolist()
+    private = [p for b, s in enumerate(src) for p in bt[b][lens[s] // PAGE:] if p >= 0]
+    assert len(set(private)) == len(private) == 3 + 1 + 4      # rows of 5, 300 and 257 tokens
+    assert f.free_pages == free + 3 - 8                        # three copied-from pages came back
+    assert bool((c.block_table == -1).all()) and c.lengths.tolist() == [0] * 4
+    # a row's own tokens do not reach its neighbours
+    f.reserve(7)
+    k = torch.randn(10, 2, 7, 128, device=DEV).bfloat16()
+    f.layers[0].update(k, k)
+    f.advance(7)
+    f.check_errors()
+    got = A.gather_pages(f.layers[0].keys, f.block_table, 512)
+    for b, s in enumerate(src):
+        assert torch.equal(got[b, :, :lens[s]], want[0][0][s, :, :lens[s]])
+        assert torch.equal(got[b, :, lens[s]:lens[s] + 7], k[b])
+    f.release([0, 9])
+    assert f.pages.owned[[0, 9]].tolist() == [0, 0] and f.lengths[[0, 9]].tolist() == [0, 0]
+    f.reset()
+    assert f.free_pages == 59
+
+
+def test_forked_rows_attend_like_unforked_ones():
+    """The shared-prefix attention on a fork against the plain one on the same table."""
+    c, _ = _filled([260, 5, 700], 80, H=2)
+    f = c.fork([6, 3, 8])
+    f.reserve(4)
+    k = torch.randn(17, 2, 4, 128, device=DEV).bfloat16()
+    f.layers[0].update(k, k)
+    q = torch.randn(17, 8, 4, 128, device=DEV).bfloat16()
+    got = A.prefix_attention(q, f.layers[0].keys, f.layers[0].values, f.lengths, f.block_table,
+                             *f.prefix).float()
+    want = A.verify_attention(q, f.layers[0].keys, f.layers[0].values, f.lengths,
+                              block_table=f.block_table).float()
+    mag = A.verify_attention(q, f.layers[0].keys, f.layers[0].values.abs(), f.lengths,
+                             block_table=f.block_table).float()
+    # weights and results are rounded to bf16 on both sides: 4 * 2^-8 of sum w |v|
+    assert bool(((got - want).abs() <= 2.0 ** -6 * mag * 1.02).all())
+
+
+def test_fork_refusals():
+    c, _ = _filled([5, 300], 8)                                # 4 pages used, 3 left
+    with pytest.raises(L.SpecdecError):
+        c.fork([1])
+    with pytest.raises(L.SpecdecError):
+        c.fork([1, 0])
+    bt, free = c.block_table.clone(), c.free_pages
+    with pytest.raises(L.SpecdecError):
+        c.fork([2, 2])                                         # four private pages wanted
+    assert torch.equal(c.block_table, bt) and c.free_pages == free
+    f = c.fork([1, 2])
+    assert f.lengths.tolist() == [5, 300, 300]
+    h = PagedRaggedCache(1, 2, 256, DEV)
+    with pytest.raises(L.SpecdecError):
+        h.fork([1, 1])
+
+
+@pytest.fixture(scope="module")
+def engine():
+    target, draft = tiny_pair_noisy(noise=4.0)
+    return SpecDecodeEngine(target, draft, TinyTok(), device=DEV, capacity=512)
+
+
+def _prompts(P=150):
+    torch.manual_seed(0)
+    return torch.randint(0, VOCAB, (3, P)), torch.tensor([P, 7, P - 20])
+
+
+@pytest.mark.parametrize("k", [1, 4])
+def test_greedy_samples_equal_the_single_one(engine, k):
+    ids, plen = _prompts()
+    sp = SamplingConfig(temperature=0.0)
+    one, st1 = engine.generate(ids, plen, 40, sampling=sp, k_fixed=k, logprobs=2)
+    out, st = engine.generate(ids, plen, 40, sampling=sp, k_fixed=k, n=3, logprobs=2)
+    assert len(out) == 9 and st.batch == 9
+    for b in range(9):
+        m = min(len(out[b]), len(one[b // 3]))
+        assert m >= 40 and out[b][:40] == one[b // 3][:40]
+        # the projections' GEMMs run on 9 rows here and on 3 there, in another
+        # order of float32 sums: two forwards of the module's bound (sorted
+        # alternatives move by no more than their values)
+        for x, y in zip(st.logprobs[b][:40], st1.logprobs[b // 3][:40]):
+            assert abs(x - y) < 1e-3
+        for x, y in zip(st.top_logprobs[b][:40], st1.top_logprobs[b // 3][:40]):
+            assert all(abs(p - q) < 1e-3 for (_, p), (_, q) in zip(x, y))
+
+
+def _teacher_logprobs(model, prompt, tokens):
+    """log softmax of a plain forward at the tokens' positions (eager attention)."""
+    m = copy.deepcopy(model)
+    from specdec import fused_attention as FA
+    from specdec import fused_layers as FL
+    FA.uninstall(m)
+    FL.uninstall(m)
+    m.set_attn_implementation("eager")
+    seq = torch.tensor([prompt + tokens], device=DEV)
+    with torch.no_grad():
+        lp = torch.log_softmax(m(input_ids=seq).logits[0].double(), -1)
+    at = torch.arange(len(prompt) - 1, len(prompt) + len(tokens) - 1, device=DEV)
+    return lp[at]
+
+
+@pytest.mark.parametrize("T", [0.0, 1.0])
+def test_logprobs_of_the_emitted_tokens(engine, T):
+    ids, plen = _prompts(40)
+    out, st = engine.generate(ids, plen, 30, sampling=SamplingConfig(temperature=T, top_p=0.9),
+                              k_fixed=3, n=2, seed=5, logprobs=3)
+    for b, toks in enumerate(out):
+        assert len(st.logprobs[b]) == len(toks) == len(st.top_logprobs[b])
+        prompt = ids[b // 2, :int(plen[b // 2])].tolist()
+        lp = _teacher_logprobs(engine.target, prompt, toks)
+        want = lp[torch.arange(len(toks)), torch.tensor(toks, device=DEV)]
+        got = torch.tensor(st.logprobs[b], device=DEV).double()
+        assert bool(((got - want).abs() < 1e-3).all())
+        for alts, row in zip(st.top_logprobs[b], lp):
+            assert len(alts) == 3 and all(abs(p - float(row[i])) < 1e-3 for i, p in alts)
+            assert alts[0][1] >= alts[1][1] >= alts[2][1]
+    if T == 0.0:
+        assert all(a[0][0] == t for b in range(6) for a, t in zip(st.top_logprobs[b], out[b]))
+
+
+def test_samples_differ_and_repeat_for_a_seed(engine):
+    ids, plen = _prompts(30)
+    sp = SamplingConfig(temperature=1.0)
+    a, _ = engine.generate(ids, plen, 24, sampling=sp, k_fixed=3, n=4, seed=11)
+    b, _ = engine.generate(ids, plen, 24, sampling=sp, k_fixed=3, n=4, seed=11)
+    assert a == b
+    assert len({tuple(x) for x in a[:4]}) > 1
+    ar, st = engine.generate_autoregressive(ids, plen, 8, sampling=SamplingConfig(), logprobs=0)
+    assert [len(x) for x in st.logprobs] == [len(x) for x in ar] and st.top_logprobs == []
+
+
+def _bf16_pair():
+    cfg = Qwen3Config(vocab_size=VOCAB, hidden_size=64, intermediate_size=128, num_hidden_layers=2,
+                      num_attention_heads=4, num_key_value_heads=2, head_dim=128,
+                      max_position_embeddings=1024, tie_word_embeddings=True)
+    torch.manual_seed(3)
+    target = Qwen3ForCausalLM(cfg).eval().to(torch.bfloat16).to(DEV)
+    return target, copy.deepcopy(target)
+
+
+def test_bf16_samples_share_their_prompt():
+    """Heads of 128 in bf16 take the shared path (fused layers, CUDA graphs): the
+    draft equals the target, so nearly every draft is accepted, and every
+    log-probability is the one of its own sequence."""
+    target, draft = _bf16_pair()
+    eng = SpecDecodeEngine(target, draft, TinyTok(), device=DEV, capacity=1024)
+    torch.manual_seed(1)
+    ids = torch.randint(0, VOCAB, (2, 400))
+    plen = torch.tensor([400, 290])
+    out, st = eng.generate(ids, plen, 60, sampling=SamplingConfig(temperature=1.0), k_fixed=4, n=8,
+                           seed=2, logprobs=1)
+    assert len(out) == 16 and all(len(x) >= 60 for x in out)
+    assert st.acceptance_rate > 0.9
+    for b in (0, 7, 8, 15):
+        prompt = ids[b // 8, :int(plen[b // 8])].tolist()
+        lp = _teacher_logprobs(eng.target, prompt, out[b])
+        want = lp[torch.arange(len(out[b])), torch.tensor(out[b], device=DEV)]
+        got = torch.tensor(st.logprobs[b], device=DEV).double()
+        # bf16 logits of order 1 (2^-8 each), activations rounded a dozen times
+        assert bool(((got - want).abs() < 0.1).all())
+
+
+def test_a_pool_that_runs_out_raises(engine):
+    ids, plen = _prompts(30)
+    small = SpecDecodeEngine(engine.target, engine.draft, TinyTok(), device=DEV, capacity=512,
+                             kv_pages=3 + 6 + 1)
+    with pytest.raises(L.SpecdecError):
+        small.generate(ids, plen, 200, sampling=SamplingConfig(), k_fixed=3, n=2)
+
+
+def test_bad_arguments(engine):
+    ids, plen = _prompts(10)
+    for bad in (dict(n=0), dict(logprobs=-1), dict(logprobs=VOCAB + 1)):
+        with pytest.raises(ValueError):
+            engine.generate(ids, plen, 4, **bad)
