@@ -3,7 +3,9 @@
 The library is loaded lazily on first use.  There is no fallback: without the
 built library, or with CPU tensors, every entry point raises.
 """
+import contextlib
 import ctypes
+import functools
 import pathlib
 import threading
 
@@ -142,6 +144,33 @@ def ptr(t):
 
 def stream_ptr(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context in which ``device`` is the current one (nothing to do when it is:
+    torch.cuda.device costs more than a small kernel's launch)."""
+    if torch.cuda.current_device() == device.index:
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
+
+
+def stream_of(device):
+    """The current stream's handle on ``device``, as an int."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def address(t):
+    """data_ptr of a tensor or None, as ctypes takes it for a void* argument."""
+    return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=4096)
+def workspace_bytes(name, *args):
+    """The library's answer to a workspace-size query, remembered."""
+    return getattr(lib(), name)(*args)
 
 
 def dtype_code(dt):

@@ -19,6 +19,7 @@ from specdec import _lib as L
 
 IMPL = "specdec_b200"
 PREFILL_SDPA_MIN = 64          # prefills longer than this (fresh cache) use torch SDPA
+SD_PAGE = 128                  # SD_KV_PAGE (kvcache.PAGE)
 _ATTN_DTYPES = {torch.bfloat16: 2, torch.float32: 0}
 
 
@@ -119,16 +120,21 @@ def prefix_attention(q, k_pool, v_pool, lengths, block_table, group_starts, pref
     Both group arrays live on the device, so a captured call follows them.
     bf16 heads of 128 share; other shapes are computed row by row.
     """
-    from specdec.kvcache import PAGE
-    L.require_cuda(q, k_pool, v_pool, lengths, block_table, group_starts, prefix_pages, valid, out)
+    dev = q.device
+    if dev.type != "cuda":
+        L.require_cuda(q)
+    for t in (k_pool, v_pool, lengths, block_table, group_starts, prefix_pages, valid, out):
+        if t is not None and t.device != dev:
+            raise L.SpecdecError("prefix_attention needs every tensor on one CUDA device")
     if q.dim() != 4 or k_pool.dim() != 4:
         raise L.SpecdecError("prefix_attention needs q [B, Hq, qlen, D] and pools "
                              "[n_pages, Hkv, PAGE, D]")
-    if q.dtype not in _ATTN_DTYPES or k_pool.dtype != q.dtype or v_pool.dtype != q.dtype:
-        raise L.SpecdecError(f"prefix_attention supports bf16 / fp32, got {q.dtype}")
+    dt = q.dtype
+    if dt not in _ATTN_DTYPES or k_pool.dtype != dt or v_pool.dtype != dt:
+        raise L.SpecdecError(f"prefix_attention supports bf16 / fp32, got {dt}")
     B, Hq, qlen, D = q.shape
     npages, Hkv, page, Dk = k_pool.shape
-    if page != PAGE or Dk != D or v_pool.shape != k_pool.shape or not (
+    if page != SD_PAGE or Dk != D or v_pool.shape != k_pool.shape or not (
             k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise L.SpecdecError("paged caches must be contiguous [n_pages, Hkv, PAGE, D] pools")
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B \
@@ -141,41 +147,39 @@ def prefix_attention(q, k_pool, v_pool, lengths, block_table, group_starts, pref
         raise L.SpecdecError("group_starts [G + 1] and prefix_pages [G] must be contiguous int32")
     if lengths.numel() != B or (valid is not None and valid.numel() != B):
         raise L.SpecdecError(f"lengths and valid need one entry per row ({B})")
-    dev = q.device
-    for t in (k_pool, v_pool, lengths, block_table, group_starts, prefix_pages, valid, out):
-        if t is not None and t.device != dev:
-            raise L.SpecdecError("prefix_attention needs every tensor on one device")
     sc = float(scale) if scale is not None else D ** -0.5
     if not 0.0 < sc < 3e38:
         raise L.SpecdecError(f"scale must be positive and finite, got {scale}")
-    if out is None:
-        out = torch.empty(B, qlen, Hq, D, dtype=q.dtype, device=dev)
-    elif out.shape != (B, qlen, Hq, D) or out.dtype != q.dtype or (D > 1 and out.stride(3) != 1):
-        raise L.SpecdecError(f"out must be {(B, qlen, Hq, D)} of {q.dtype}, contiguous along D")
-    if B == 0 or qlen == 0:
-        return out
-    if q.stride(-1) != 1 or (q.dtype == torch.bfloat16 and D == 128 and (
-            q.data_ptr() % 16 or any(q.stride(i) % 8 for i in range(3)))):
+    if out is not None and (out.shape != (B, qlen, Hq, D) or out.dtype != dt
+                            or (D > 1 and out.stride(3) != 1)):
+        raise L.SpecdecError(f"out must be {(B, qlen, Hq, D)} of {dt}, contiguous along D")
+    qb, qh, ql, qd = q.stride()
+    if qd != 1 or (dt == torch.bfloat16 and D == 128 and (
+            q.data_ptr() % 16 or qb % 8 or qh % 8 or ql % 8)):
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-    lens = lengths if lengths.dtype == torch.long and lengths.is_contiguous() \
-        else lengths.long().contiguous()
-    val = None if valid is None else valid.long().contiguous()
-    W = block_table.shape[1]
-    lib = L.lib()
-    with torch.cuda.device(dev):
+        qb, qh, ql, qd = q.stride()
+    if lengths.dtype != torch.long or not lengths.is_contiguous():
+        lengths = lengths.long().contiguous()
+    if valid is not None and (valid.dtype != torch.long or not valid.is_contiguous()):
+        valid = valid.long().contiguous()
+    W, code = block_table.shape[1], _ATTN_DTYPES[dt]
+    with L.on_device(dev):
+        if out is None:
+            out = torch.empty((B, qlen, Hq, D), dtype=dt, device=dev)
+        if B == 0 or qlen == 0:
+            return out
         # a fresh buffer per call: calls on several streams and calls captured
         # into different graphs never share one
-        ws = torch.empty(lib.sd_prefix_attn_workspace_bytes(B, G, Hq, Hkv, D, W, qlen,
-                                                            _ATTN_DTYPES[q.dtype]),
-                         dtype=torch.uint8, device=dev)
-        L.check(lib.sd_prefix_attn(
-            L.ptr(q), q.stride(0), q.stride(1), q.stride(2), L.ptr(k_pool), L.ptr(v_pool),
-            L.ptr(block_table), W, npages, L.ptr(lens), L.ptr(val), L.ptr(group_starts),
-            L.ptr(prefix_pages), G, B, Hq, Hkv, D, qlen, sc, L.ptr(out), out.stride(0),
-            out.stride(1), out.stride(2), _ATTN_DTYPES[q.dtype], L.ptr(ws), ws.numel(),
-            L.stream_ptr(dev)), "prefix_attn")
+        nws = L.workspace_bytes("sd_prefix_attn_workspace_bytes", B, G, Hq, Hkv, D, W, qlen, code)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        ob, ol, oh, _ = out.stride()
+        L.check(L.lib().sd_prefix_attn(
+            q.data_ptr(), qb, qh, ql, k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
+            W, npages, lengths.data_ptr(), L.address(valid), group_starts.data_ptr(),
+            prefix_pages.data_ptr(), G, B, Hq, Hkv, D, qlen, sc, out.data_ptr(), ob, ol, oh, code,
+            ws.data_ptr(), nws, L.stream_of(dev)), "prefix_attn")
     return out
 
 

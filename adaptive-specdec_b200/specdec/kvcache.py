@@ -473,18 +473,19 @@ class DevicePageTable:
     @classmethod
     def over(cls, block_table, owned, shared, free, n_free, err):
         """A table over state that the caller holds (no copies)."""
+        dev = block_table.device
+        if dev.type != "cuda":
+            raise L.SpecdecError("DevicePageTable keeps its state on the GPU (no CPU fallback)")
+        for t in (block_table, owned, shared, free, n_free, err):
+            if t.dtype != torch.int32 or t.device != dev:
+                raise L.SpecdecError("a page table's state is int32 on one CUDA device")
+            if t is not block_table and not t.is_contiguous():
+                raise L.SpecdecError("owned, shared, free, n_free and err must be contiguous")
         if block_table.dim() != 2 or block_table.stride(1) != 1:
             raise L.SpecdecError("block_table must be [B, W] with contiguous rows")
         B = block_table.shape[0]
-        for name, t, n in (("block_table", block_table, None), ("owned", owned, B),
-                           ("shared", shared, B), ("free", free, None), ("n_free", n_free, 1),
-                           ("err", err, 1)):
-            if t.dtype != torch.int32 or not t.is_cuda or t.device != block_table.device:
-                raise L.SpecdecError(f"{name} must be int32 on one CUDA device")
-            if t is not block_table and not t.is_contiguous():
-                raise L.SpecdecError(f"{name} must be contiguous")
-            if n is not None and t.numel() != n:
-                raise L.SpecdecError(f"{name} must have {n} entries, got {t.numel()}")
+        if owned.numel() != B or shared.numel() != B or n_free.numel() != 1 or err.numel() != 1:
+            raise L.SpecdecError(f"owned and shared need {B} entries, n_free and err one")
         if B == 0 or block_table.shape[1] == 0 or free.numel() == 0:
             raise L.SpecdecError("a page table needs at least one row, one page per row and a pool")
         self = cls.__new__(cls)
@@ -520,30 +521,32 @@ class DevicePageTable:
             total = self.B * each if max_tokens is None else int(max_tokens)
         if total < 0:
             raise L.SpecdecError(f"max_tokens must not be negative, got {total}")
-        lib = L.lib()
-        with torch.cuda.device(self.device):
+        dev = self.device
+        with L.on_device(dev):
             # (an empty map still has an address: NULL means no map)
-            slots = torch.empty(max(total, 1), dtype=torch.long, device=self.device) \
+            slots = torch.empty(max(total, 1), dtype=torch.long, device=dev) \
                 if slot_map else None
-            starts = torch.empty(self.B + 1, dtype=torch.int32, device=self.device)
-            ws = torch.empty(lib.sd_pages_workspace_bytes(self.B), dtype=torch.uint8,
-                             device=self.device)
-            L.check(lib.sd_pages_reserve(
-                L.ptr(self.block_table), self.block_table.stride(0), self.W, L.ptr(self.owned),
-                L.ptr(self.free), self.n_pages, L.ptr(self.n_free), L.ptr(lens), L.ptr(add), each,
-                self.B, L.ptr(slots), total, L.ptr(starts), L.ptr(self.err), L.ptr(ws), ws.numel(),
-                L.stream_ptr(self.device)), "pages_reserve")
+            starts = torch.empty(self.B + 1, dtype=torch.int32, device=dev)
+            nws = L.workspace_bytes("sd_pages_workspace_bytes", self.B)
+            ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+            L.check(L.lib().sd_pages_reserve(
+                self.block_table.data_ptr(), self.block_table.stride(0), self.W,
+                self.owned.data_ptr(), self.free.data_ptr(), self.n_pages, self.n_free.data_ptr(),
+                lens.data_ptr(), L.address(add), each, self.B, L.address(slots), total,
+                starts.data_ptr(), self.err.data_ptr(), ws.data_ptr(), nws, L.stream_of(dev)),
+                "pages_reserve")
         return (slots[:total] if slot_map and total == 0 else slots), starts
 
     def trim(self, lengths):
         """Give back every row's pages past its ``lengths`` [B] tokens (never
         its shared ones); a trim after a reserve restores the stack."""
         lens = self._rows(lengths, "lengths")
-        with torch.cuda.device(self.device):
+        with L.on_device(self.device):
             L.check(L.lib().sd_pages_trim(
-                L.ptr(self.block_table), self.block_table.stride(0), self.W, L.ptr(self.owned),
-                L.ptr(self.shared), L.ptr(self.free), self.n_pages, L.ptr(self.n_free),
-                L.ptr(lens), self.B, L.ptr(self.err), L.stream_ptr(self.device)), "pages_trim")
+                self.block_table.data_ptr(), self.block_table.stride(0), self.W,
+                self.owned.data_ptr(), self.shared.data_ptr(), self.free.data_ptr(), self.n_pages,
+                self.n_free.data_ptr(), lens.data_ptr(), self.B, self.err.data_ptr(),
+                L.stream_of(self.device)), "pages_trim")
 
     def reset(self):
         """Every page back on the stack, page 0 on top (of this table's pool)."""

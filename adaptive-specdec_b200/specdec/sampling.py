@@ -272,47 +272,56 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
     a +inf, or with nothing above -inf, has NaN log-probabilities and entropy.
     One pass over the logits (sd_token_logprobs), no host synchronisation.
     """
-    L.require_cuda(logits, ids)
-    if logits.dim() < 1 or tuple(ids.shape) != tuple(logits.shape[:-1]):
-        raise L.SpecdecError(f"token_logprobs needs one id per row: logits {tuple(logits.shape)}, "
-                             f"ids {tuple(ids.shape)}")
-    if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
-        raise L.SpecdecError(f"ids must be integers, got {ids.dtype}")
-    if ids.device != logits.device:
+    dev, shape, V = logits.device, ids.shape, logits.shape[-1] if logits.dim() else 0
+    if dev.type != "cuda" or ids.device != dev:
+        L.require_cuda(logits, ids)
         raise L.SpecdecError("logits and ids must be on one device")
+    if logits.dim() < 1 or shape != logits.shape[:-1]:
+        raise L.SpecdecError(f"token_logprobs needs one id per row: logits {tuple(logits.shape)}, "
+                             f"ids {tuple(shape)}")
+    if ids.dtype != torch.long:
+        if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+            raise L.SpecdecError(f"ids must be integers, got {ids.dtype}")
+        ids = ids.long()
     code = L.dtype_code(logits.dtype)
-    V = logits.shape[-1]
-    n = int(top_n)
-    if not 0 <= n <= min(V, TOP_N_MAX):
-        raise L.SpecdecError(f"top_n must be between 0 and min(V, {TOP_N_MAX}), got {n}")
+    n, T = int(top_n), float(temperature)
     if not 1 <= V <= LOGPROBS_MAX_V:
         raise L.SpecdecError(f"the vocabulary must have 1 to {LOGPROBS_MAX_V} entries, got {V}")
-    T = float(temperature)
+    if not 0 <= n <= min(V, TOP_N_MAX):
+        raise L.SpecdecError(f"top_n must be between 0 and min(V, {TOP_N_MAX}), got {n}")
     if not 0.0 < T < float("inf"):
         raise L.SpecdecError(f"temperature must be positive and finite, got {temperature}")
-    x = logits if V == 1 else _vocab_rows(logits, "logits")
-    x = x.reshape(-1, V) if x.dim() > 3 else x.reshape(1, V) if x.dim() == 1 else x
-    x = x.unsqueeze(1) if x.dim() == 2 else x
-    if x.stride(-1) != 1:
-        x = x.contiguous()
-    B, Lr = x.shape[0], x.shape[1]
-    tok = ids.long().reshape(B, Lr)
-    if tok.stride(-1) != 1:
-        tok = tok.contiguous()
-    dev, shape = x.device, tuple(ids.shape)
-    logprob = torch.empty(shape, dtype=torch.float32, device=dev)
-    rank = torch.empty(shape, dtype=torch.long, device=dev)
-    entropy = torch.empty(shape, dtype=torch.float32, device=dev)
-    top_ids = torch.empty(shape + (n,), dtype=torch.long, device=dev) if n else None
-    top_lp = torch.empty(shape + (n,), dtype=torch.float32, device=dev) if n else None
-    lib = L.lib()
-    with torch.cuda.device(dev):
+    # rows (b, l) with strides (bs, ps), their ids with stride ids_bs over b
+    dims = logits.dim()
+    if V == 1:
+        logits = logits.contiguous()
+    x = _vocab_rows(logits, "logits")
+    if dims == 2:
+        B, Lr, bs, ps = shape[0], 1, x.stride(0), 0
+        ids_bs = ids.stride(0)
+    elif dims == 3:
+        B, Lr, bs, ps = shape[0], shape[1], x.stride(0), x.stride(1)
+        if ids.stride(1) != 1 and Lr > 1:
+            ids = ids.contiguous()
+        ids_bs = ids.stride(0)
+    else:
+        x = x.reshape(-1, V)
+        if x.stride(1) != 1:                       # what reshape makes of a single row or entry
+            x = x.contiguous()
+        ids = ids.reshape(-1)
+        B, Lr, bs, ps, ids_bs = x.shape[0], 1, x.stride(0), 0, ids.stride(0)
+    with L.on_device(dev):
+        logprob = torch.empty(shape, dtype=torch.float32, device=dev)
+        rank = torch.empty(shape, dtype=torch.long, device=dev)
+        entropy = torch.empty(shape, dtype=torch.float32, device=dev)
+        top_ids = torch.empty(shape + (n,), dtype=torch.long, device=dev) if n else None
+        top_lp = torch.empty(shape + (n,), dtype=torch.float32, device=dev) if n else None
         # a fresh buffer per call: calls on several streams and calls captured
         # into different graphs never share one
-        ws = torch.empty(lib.sd_token_logprobs_workspace_bytes(B, Lr, V, code, n),
-                         dtype=torch.uint8, device=dev)
-        L.check(lib.sd_token_logprobs(L.ptr(x), x.stride(0), x.stride(1), code, L.ptr(tok),
-                                      tok.stride(0), B, Lr, V, T, n, L.ptr(logprob), L.ptr(rank),
-                                      L.ptr(entropy), L.ptr(top_ids), L.ptr(top_lp), L.ptr(ws),
-                                      ws.numel(), L.stream_ptr(dev)), "token_logprobs")
+        nws = L.workspace_bytes("sd_token_logprobs_workspace_bytes", B, Lr, V, code, n)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        L.check(L.lib().sd_token_logprobs(
+            x.data_ptr(), bs, ps, code, ids.data_ptr(), ids_bs, B, Lr, V, T, n, logprob.data_ptr(),
+            rank.data_ptr(), entropy.data_ptr(), L.address(top_ids), L.address(top_lp),
+            ws.data_ptr(), nws, L.stream_of(dev)), "token_logprobs")
     return TokenLogprobs(logprob, rank, entropy, top_ids, top_lp)
