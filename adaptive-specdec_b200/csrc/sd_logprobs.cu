@@ -39,8 +39,9 @@ namespace sd {
 constexpr int LP_THREADS = 256;
 constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_UNITS = 16;                    // 16-byte units per thread and part
-constexpr int LP_LIST = 4096;                   // >= SD_TOPN_MAX * 8 * LP_UNITS, >= parts * n
-static_assert(LP_LIST >= SD_TOPN_MAX * 8 * LP_UNITS, "a part's list holds every flagged element");
+constexpr int LP_CTAS = 2;                      // per SM
+constexpr int LP_LIST = 4096 + 32;              // a part's flagged elements; a row's parts * n
+static_assert(LP_LIST >= SD_TOPN_MAX * 8 * LP_UNITS + 14, "a part's list holds every flagged element");
 static_assert(SD_LOGPROBS_MAX_V / (4 * LP_UNITS * LP_THREADS) + 2 <= LP_LIST / SD_TOPN_MAX,
               "a row's lists fit the join's list");
 static_assert(SD_TOPN_MAX <= 32, "the n-th largest thread maximum of one warp");
@@ -85,59 +86,101 @@ __device__ __forceinline__ float lp_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
-// A 16-byte unit of the logits' type: E elements.
-template <typename T> struct Unit;
-template <> struct Unit<__nv_bfloat16> {
-  static constexpr int E = 8;
-  __device__ static float get(const uint4& u, int e) {
-    const uint32_t w = e < 2 ? u.x : e < 4 ? u.y : e < 6 ? u.z : u.w;
-    return __uint_as_float((e & 1) ? (w & 0xFFFF0000u) : (w << 16));
+// What the kernel does on a 32-bit word of the logits' type (two 16-bit
+// elements or one float): maximum with NaN winning, elements, and counting the
+// elements that are not below a threshold (a NaN is not) with packed compares
+// and adds; a thread counts at most 8 * LP_UNITS / 2 = 64 per half, which bf16
+// holds exactly (up to 256).
+template <typename T> struct Word;
+template <> struct Word<__nv_bfloat16> {
+  static constexpr int N = 2;
+  static constexpr uint32_t NEG_INF = 0xFF80FF80u;
+  __device__ static __nv_bfloat162 v(uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+  __device__ static uint32_t w(__nv_bfloat162 v) { return *reinterpret_cast<uint32_t*>(&v); }
+  __device__ static uint32_t vmax(uint32_t a, uint32_t b) { return w(__hmax2_nan(v(a), v(b))); }
+  __device__ static float get(uint32_t x, int e) {
+    return __uint_as_float(e ? (x & 0xFFFF0000u) : (x << 16));
   }
-  __device__ static uint32_t bits(const __nv_bfloat16* p) {
-    return *reinterpret_cast<const unsigned short*>(p);
+  __device__ static uint32_t count(uint32_t c, uint32_t x, uint32_t thr) {
+    return w(__hadd2(v(c), __hgeu2(v(x), v(thr))));
   }
-  static constexpr uint32_t NEG_INF = 0xFF80u;
+  __device__ static int total(uint32_t c) { return (int)(get(c, 0) + get(c, 1)); }
+  __device__ static bool any(uint32_t x, uint32_t thr) { return w(__hgeu2(v(x), v(thr))) != 0u; }
+  // both halves the element's bits; the next larger value of a finite one
+  __device__ static uint32_t splat(float f) { return (__float_as_uint(f) >> 16) * 0x10001u; }
+  __device__ static uint32_t above(float f) {
+    const uint32_t b = __float_as_uint(f) >> 16;
+    return (f == 0.f ? 1u : (b & 0x8000u) ? b - 1u : b + 1u) * 0x10001u;
+  }
 };
-template <> struct Unit<__half> {
-  static constexpr int E = 8;
-  __device__ static float get(const uint4& u, int e) {
-    const uint32_t w = e < 2 ? u.x : e < 4 ? u.y : e < 6 ? u.z : u.w;
-    return __half2float(__ushort_as_half((unsigned short)((e & 1) ? (w >> 16) : (w & 0xFFFFu))));
+template <> struct Word<__half> {
+  static constexpr int N = 2;
+  static constexpr uint32_t NEG_INF = 0xFC00FC00u;
+  __device__ static __half2 v(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
+  __device__ static uint32_t w(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+  __device__ static uint32_t vmax(uint32_t a, uint32_t b) { return w(__hmax2_nan(v(a), v(b))); }
+  __device__ static float get(uint32_t x, int e) {
+    return e ? __high2float(v(x)) : __low2float(v(x));
   }
-  __device__ static uint32_t bits(const __half* p) {
-    return *reinterpret_cast<const unsigned short*>(p);
+  __device__ static uint32_t count(uint32_t c, uint32_t x, uint32_t thr) {
+    return w(__hadd2(v(c), __hgeu2(v(x), v(thr))));
   }
-  static constexpr uint32_t NEG_INF = 0xFC00u;
+  __device__ static int total(uint32_t c) { return (int)(get(c, 0) + get(c, 1)); }
+  __device__ static bool any(uint32_t x, uint32_t thr) { return w(__hgeu2(v(x), v(thr))) != 0u; }
+  __device__ static uint32_t bits(float f) { return __half_as_ushort(__float2half_rn(f)); }
+  __device__ static uint32_t splat(float f) { return bits(f) * 0x10001u; }
+  __device__ static uint32_t above(float f) {
+    const uint32_t b = bits(f);
+    return (f == 0.f ? 1u : (b & 0x8000u) ? b - 1u : b + 1u) * 0x10001u;
+  }
 };
-template <> struct Unit<float> {
-  static constexpr int E = 4;
-  __device__ static float get(const uint4& u, int e) {
-    return __uint_as_float(e == 0 ? u.x : e == 1 ? u.y : e == 2 ? u.z : u.w);
-  }
-  __device__ static uint32_t bits(const float* p) { return __float_as_uint(*p); }
+template <> struct Word<float> {
+  static constexpr int N = 1;
   static constexpr uint32_t NEG_INF = 0xFF800000u;
+  __device__ static uint32_t vmax(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ static float get(uint32_t x, int) { return __uint_as_float(x); }
+  __device__ static uint32_t count(uint32_t c, uint32_t x, uint32_t thr) {
+    return c + !(__uint_as_float(x) < __uint_as_float(thr));
+  }
+  __device__ static int total(uint32_t c) { return (int)c; }
+  __device__ static bool any(uint32_t x, uint32_t thr) {
+    return !(__uint_as_float(x) < __uint_as_float(thr));
+  }
+  __device__ static uint32_t splat(float f) { return __float_as_uint(f); }
+  __device__ static uint32_t above(float f) {
+    const uint32_t b = __float_as_uint(f);
+    return f == 0.f ? 1u : (b & 0x80000000u) ? b - 1u : b + 1u;
+  }
 };
 
-// Elements [i0, i0 + E) of a row of V elements; those outside [0, V) are -inf.
-// Whole units are one 16-byte load (the unit grid is the row's 16-byte grid).
-template <typename T>
-__device__ __forceinline__ uint4 load_unit(const T* row, int i0, int V) {
-  constexpr int E = Unit<T>::E;
-  if (i0 >= 0 && i0 + E <= V) return __ldcs(reinterpret_cast<const uint4*>(row + i0));
-  uint32_t w[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (E == 4) {
-      const int i = i0 + q;
-      w[q] = (i >= 0 && i < V) ? Unit<T>::bits(row + i) : Unit<T>::NEG_INF;
-    } else {
-      const int i = i0 + 2 * q;
-      const uint32_t lo = (i >= 0 && i < V) ? Unit<T>::bits(row + i) : Unit<T>::NEG_INF;
-      const uint32_t hi = (i + 1 >= 0 && i + 1 < V) ? Unit<T>::bits(row + i + 1) : Unit<T>::NEG_INF;
-      w[q] = lo | (hi << 16);
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+// Two floats in one 64-bit register for the packed FP32 instructions.
+__device__ __forceinline__ unsigned long long pair2(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(unsigned long long p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b,
+                                                   unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
 // The n largest of the cnt unique keys in `list` (shared memory), in falling
@@ -180,88 +223,131 @@ __device__ void sort_top(unsigned long long* list, int cnt, int n, unsigned long
   for (int i = cnt + t; i < n; i += THREADS) out[i] = 0ULL;
 }
 
+// Word q of the thread's unit i.
+#define LP_WORD(i, q) (q == 0 ? d[i].x : q == 1 ? d[i].y : q == 2 ? d[i].z : d[i].w)
+
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, 2) logp_part_kernel(const LpParams P) {
-  constexpr int E = Unit<T>::E;
+__global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const LpParams P) {
+  using Wd = Word<T>;
+  constexpr int E = 4 * Wd::N;                       // elements per 16-byte unit
   extern __shared__ __align__(16) unsigned char lp_smem[];
   unsigned long long* list = reinterpret_cast<unsigned long long*>(lp_smem);   // TOP only
   __shared__ float red_m[LP_WARPS], red_s[LP_WARPS], red_e[LP_WARPS];
   __shared__ int red_c[LP_WARPS];
   __shared__ uint32_t kth[LP_WARPS], jth[LP_WARPS];
-  __shared__ unsigned long long uth[LP_WARPS];
+  __shared__ unsigned long long uth;
   __shared__ int n_list, counter;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   const int64_t item = blockIdx.x;
   const int64_t r = item / P.parts;
-  const int part = (int)(item % P.parts);
-  const int64_t rb = r / P.L, rl = r % P.L;
-  const T* row = reinterpret_cast<const T*>(P.x) + rb * P.bs + rl * P.ps;
+  const int part = (int)(item - r * P.parts);
+  const int64_t rb = r / P.L, rl = r - rb * P.L;
+  const int64_t row0 = rb * P.bs + rl * P.ps;
+  const T* row = reinterpret_cast<const T*>(P.x) + row0;
   const int V = P.V;
-  // the row's 16-byte grid: unit u holds elements [u * E - head, ...)
-  const int head = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-  const int units = (int)(((int64_t)V + head + E - 1) / E);
+  // whole 16-byte units between the row's first and last aligned address; the
+  // < 2 E elements outside them go one each to threads of part 0
+  const int h0 = min((int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)), V);
+  const int units = (V - h0) / E, tail = V - h0 - units * E;
   const int per = (units + P.parts - 1) / P.parts;   // <= LP_THREADS * LP_UNITS
   const int u0 = min(part * per, units), u1 = min(u0 + per, units);
-  if (t == 0) n_list = 0;
-
-  const int64_t tok = P.ids[rb * P.ids_bs + rl];
-  const bool have = tok >= 0 && tok < V;
+  const uint4* body = reinterpret_cast<const uint4*>(row + h0);
   uint4 d[LP_UNITS];
 #pragma unroll
   for (int i = 0; i < LP_UNITS; ++i) {
     const int u = u0 + i * LP_THREADS + t;
-    if (u < u1) {
-      d[i] = load_unit<T>(row, u * E - head, V);
-    } else {
-      constexpr uint32_t ni = E == 4 ? Unit<T>::NEG_INF : Unit<T>::NEG_INF * 0x10001u;
-      d[i] = make_uint4(ni, ni, ni, ni);
-    }
+    d[i] = u < u1 ? __ldcs(body + u) : make_uint4(Wd::NEG_INF, Wd::NEG_INF, Wd::NEG_INF, Wd::NEG_INF);
   }
-  const float xt = have ? load_logit(P.x, P.dtype, rb * P.bs + rl * P.ps + tok) : 0.f;
+  if (t == 0) n_list = 0;
+  const bool lone = part == 0 && t < h0 + tail;      // this thread's extra element
+  const int xi = t < h0 ? t : V - tail + (t - h0);
+  const float xe = lone ? load_logit(P.x, P.dtype, row0 + xi) : -CUDART_INF_F;
+  const int64_t tok = P.ids[rb * P.ids_bs + rl];
+  const bool have = tok >= 0 && tok < V;
+  const float xt = have ? load_logit(P.x, P.dtype, row0 + tok) : CUDART_INF_F;
   // thread maximum; a NaN wins
-  float m = -CUDART_INF_F;
-  bool nan = false;
+  uint32_t wm = Wd::NEG_INF;
 #pragma unroll
   for (int i = 0; i < LP_UNITS; ++i)
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float v = Unit<T>::get(d[i], e);
-      m = fmaxf(m, v);
-      nan |= v != v;
-    }
-  // sums in base 2 relative to the thread's maximum
-  const float m0 = m == -CUDART_INF_F ? 0.f : m;
-  float s = 0.f, es = 0.f;
-  int ahead = 0;
-  const uint32_t kt = lp_key(xt);
+    wm = Wd::vmax(wm, Wd::vmax(Wd::vmax(d[i].x, d[i].y), Wd::vmax(d[i].z, d[i].w)));
+  float m = Word<float>::get(Word<float>::vmax(__float_as_uint(Wd::get(wm, 0)),
+                                               __float_as_uint(Wd::get(wm, Wd::N - 1))), 0);
+  m = __uint_as_float(Word<float>::vmax(__float_as_uint(m), __float_as_uint(xe)));
+  const bool nan = m != m;
+  // sums in base 2 relative to the thread's maximum: d = (x - m) c, held at or
+  // above -256 (2^-256 is 0 here, and -inf elements add 0 * -256, not 0 * -inf)
+  const float m0 = m == -CUDART_INF_F || m == CUDART_INF_F || nan ? 0.f : m;
+  const unsigned long long nm2 = pair2(-m0, -m0), c2 = pair2(P.c, P.c);
+  unsigned long long s2 = 0ULL, e2 = 0ULL;           // (0.f, 0.f)
+  uint32_t cnt = 0u;
+  // elements at ids up to the token's count when not below it, later ones when above it:
+  // units up to the token's compare with x_t, later ones with the next larger value
+  const bool plain = have && xt > -CUDART_INF_F && xt < CUDART_INF_F;
+  const int tu = tok < h0 ? -1 : (int)((tok - h0) / E);
+  const uint32_t thr_at = Wd::splat(xt), thr_up = Wd::above(xt);
 #pragma unroll
   for (int i = 0; i < LP_UNITS; ++i) {
-    const int u = u0 + i * LP_THREADS + t;
+    const uint32_t thr = u0 + i * LP_THREADS + t <= tu ? thr_at : thr_up;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float v = Unit<T>::get(d[i], e);
-      const float dd = lp_hold((v - m0) * P.c);
-      const float p = lp_ex2(dd);
-      s += p;
-      es = fmaf(dd, p, es);
-    }
-    if (u < u1) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int idx = u * E - head + e;
-        const uint32_t k = lp_key(Unit<T>::get(d[i], e));
-        ahead += (idx >= 0 && idx < V) && (k > kt || (k == kt && idx <= tok));
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t x = LP_WORD(i, q);
+      cnt = Wd::count(cnt, x, thr);
+      unsigned long long x2;
+      if (Wd::N == 2) {
+        x2 = pair2(Wd::get(x, 0), Wd::get(x, 1));
+      } else {
+        if (q & 1) continue;
+        x2 = pair2(Wd::get(x, 0), Wd::get(LP_WORD(i, q + 1), 0));
       }
+      float a, b;
+      unpair(mul2(add2(x2, nm2), c2), a, b);
+      a = fmaxf(a, -256.f);
+      b = fmaxf(b, -256.f);
+      const unsigned long long p2 = pair2(lp_ex2(a), lp_ex2(b));
+      s2 = add2(s2, p2);
+      e2 = fma2(pair2(a, b), p2, e2);
     }
   }
+  float s, es;
+  {
+    float a, b;
+    unpair(s2, s, b);
+    unpair(e2, es, a);
+    const float dd = fmaxf((xe - m0) * P.c, -256.f), p = lp_ex2(dd);
+    s = s + b + p;
+    es = es + a + dd * p;
+  }
+  const uint32_t kt = lp_key(xt);
+  int ahead = 0;
+  if (plain) {
+    ahead = Wd::total(cnt);
+    if (tu >= u0 && tu < u1 && (tu - u0) % LP_THREADS == t) {
+      // the token's own unit: entries behind it that equal it were counted
+      for (int e = (int)((tok - h0) % E) + 1; e < E; ++e)
+        ahead -= load_logit(P.x, P.dtype, row0 + h0 + tu * E + e) == xt;
+    }
+  } else if (have) {
+    // an infinite or NaN token: by keys
+#pragma unroll 1
+    for (int u = u0 + t; u < u1; u += LP_THREADS)
+      for (int e = 0; e < E; ++e) {
+        const int idx = h0 + u * E + e;
+        const uint32_t k = lp_key(load_logit(P.x, P.dtype, row0 + idx));
+        ahead += k > kt || (k == kt && idx <= tok);
+      }
+  }
+  if (lone && have) {
+    const uint32_t k = lp_key(xe);
+    ahead += k > kt || (k == kt && xi <= tok);
+  }
   // join over the block: the maxima first, then the sums at the block's maximum
-  float bm = warp_max(m);
+  float bm = warp_max(nan ? -CUDART_INF_F : m);
   if (lane == 0) red_m[w] = bm;
+  const bool any = u0 + t < u1 || lone;              // this thread holds an element
   if (TOP) {
     // this warp's sorted thread maxima (bitonic over lanes, falling)
-    uint32_t k = nan ? 0xFFFFFFFFu : lp_key(m);
-    if (u0 + t >= u1) k = 0u;                        // no unit at all
+    uint32_t k = any ? lp_key(m) : 0u;
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -279,15 +365,15 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logp_part_kernel(const LpParams
 #pragma unroll
   for (int q = 1; q < LP_WARPS; ++q) bm = fmaxf(bm, red_m[q]);
   const float dm = lp_hold((m - bm) * P.c), f = lp_ex2(dm);
-  float s2 = f * s, es2 = f * fmaf(dm, s, es);
-  if (m == -CUDART_INF_F) s2 = es2 = 0.f;            // nothing above -inf
-  if (nan) s2 = CUDART_NAN_F;
-  s2 = warp_sum(s2);
-  es2 = warp_sum(es2);
+  float sj = f * s, ej = f * fmaf(dm, s, es);
+  if (m == -CUDART_INF_F) sj = ej = 0.f;             // nothing above -inf
+  if (nan || m == CUDART_INF_F) sj = CUDART_NAN_F;   // as the formula: inf - inf
+  sj = warp_sum(sj);
+  ej = warp_sum(ej);
   ahead = warp_sum(ahead);
   if (lane == 0) {
-    red_s[w] = s2;
-    red_e[w] = es2;
+    red_s[w] = sj;
+    red_e[w] = ej;
     red_c[w] = ahead;
   }
   if (TOP) {
@@ -298,83 +384,74 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logp_part_kernel(const LpParams
       T2 = min(T2, jth[q]);
     }
     const uint32_t thr = max(max(T1, T2), 1u);
-    const uint32_t km = nan ? 0xFFFFFFFFu : lp_key(m);
-    if (km >= thr && u0 + t < u1) {
+    auto put = [&](uint32_t k, int idx) {
+      const int at = atomicAdd(&n_list, 1);
+      if (at < LP_LIST) list[at] = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)idx;
+    };
+    if (any && lp_key(m) >= thr) {
+      const uint32_t tw = Wd::splat(lp_value(thr));
+      if (lone && lp_key(xe) >= thr) put(lp_key(xe), xi);
 #pragma unroll
       for (int i = 0; i < LP_UNITS; ++i) {
         const int u = u0 + i * LP_THREADS + t;
-        if (u < u1) {
+        if (u >= u1) break;
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const int idx = u * E - head + e;
-            const uint32_t k = lp_key(Unit<T>::get(d[i], e));
-            if (k >= thr && idx >= 0 && idx < V) {
-              const int at = atomicAdd(&n_list, 1);
-              if (at < LP_LIST)
-                list[at] = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)idx;
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t x = LP_WORD(i, q);
+          if (Wd::any(x, tw)) {
+#pragma unroll
+            for (int e = 0; e < Wd::N; ++e) {
+              const uint32_t k = lp_key(Wd::get(x, e));
+              if (k >= thr) put(k, h0 + u * E + q * Wd::N + e);
             }
           }
         }
       }
     }
     __syncthreads();
-    int cnt = n_list;
-    if (cnt > LP_LIST) {
+    int found = n_list;
+    if (found > LP_LIST) {
       // Many elements equal the threshold (flat logits).  Again with the keys
       // (value, first unit that reaches it) of the threads: unique, so at
-      // most n threads reach the n-th of them, with E * LP_UNITS elements each.
+      // most n threads reach the n-th of them, with their E * LP_UNITS
+      // elements each.  The head and tail elements join as units -1 and
+      // `units`, whose threads' own units hold other values of this key.
       unsigned long long uk = 0ULL;
-#pragma unroll
-      for (int i = 0; i < LP_UNITS; ++i) {
-        const int u = u0 + i * LP_THREADS + t;
-        if (u < u1) {
-          uint32_t k = 0;
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const int idx = u * E - head + e;
-            if (idx >= 0 && idx < V) k = max(k, lp_key(Unit<T>::get(d[i], e)));
-          }
-          const unsigned long long q = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)u;
+      auto unit_key = [&](uint32_t k, int u) {
+        return ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)(u + 1);
+      };
+#pragma unroll 1
+      for (int u = u0 + t; u < u1; u += LP_THREADS)
+        for (int e = 0; e < E; ++e) {
+          const unsigned long long q =
+              unit_key(lp_key(load_logit(P.x, P.dtype, row0 + h0 + u * E + e)), u);
           uk = q > uk ? q : uk;
         }
-      }
       __syncthreads();
       list[t] = uk;
-      if (t == 0) n_list = 0;
+      if (t == 0) n_list = counter = 0;
       __syncthreads();
-      int ahead_of = 0;
-      for (int q = 0; q < LP_THREADS; ++q) ahead_of += list[q] > uk;
-      if (ahead_of == P.top - 1 && uk != 0ULL) uth[0] = uk;   // exactly one such thread, or fewer keys
-      if (t == 0) counter = 0;
-      __syncthreads();
+      int before = 0;
+      for (int q = 0; q < LP_THREADS; ++q) before += list[q] > uk;
+      if (before == P.top - 1 && uk != 0ULL) uth = uk;       // exactly one such thread, or too few
       if (uk != 0ULL) atomicAdd(&counter, 1);
       __syncthreads();
-      const unsigned long long ut = counter >= P.top ? uth[0] : 1ULL;
+      const unsigned long long ut = counter >= P.top ? uth : 1ULL;
       __syncthreads();
+      if (lone && unit_key(lp_key(xe), xi < h0 ? -1 : units) >= ut) put(lp_key(xe), xi);
       if (uk >= ut) {
-#pragma unroll
-        for (int i = 0; i < LP_UNITS; ++i) {
-          const int u = u0 + i * LP_THREADS + t;
-          if (u < u1) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-              const int idx = u * E - head + e;
-              const uint32_t k = lp_key(Unit<T>::get(d[i], e));
-              const unsigned long long q = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)u;
-              if (idx >= 0 && idx < V && q >= ut) {
-                const int at = atomicAdd(&n_list, 1);
-                if (at < LP_LIST)
-                  list[at] = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)idx;
-              }
-            }
+#pragma unroll 1
+        for (int u = u0 + t; u < u1; u += LP_THREADS)
+          for (int e = 0; e < E; ++e) {
+            const uint32_t k = lp_key(load_logit(P.x, P.dtype, row0 + h0 + u * E + e));
+            if (unit_key(k, u) >= ut) put(k, h0 + u * E + e);
           }
-        }
       }
       __syncthreads();
-      cnt = min(n_list, LP_LIST);
+      found = min(n_list, LP_LIST);
       __syncthreads();
     }
-    sort_top<LP_THREADS>(list, cnt, P.top, P.keys + item * P.top, &counter);
+    sort_top<LP_THREADS>(list, found, P.top, P.keys + item * P.top, &counter);
   } else {
     __syncthreads();
   }
