@@ -12,20 +12,21 @@
 // the verify round give a token and its probability after top-k / top-p; a
 // caller that ranks samples needs the untruncated log-probabilities.
 //
-// One pass over the logits.  A row is cut into parts of up to LP_UNITS 16-byte
-// units per thread, held in registers: a part's loads are all in flight at
-// once and its elements are looked at twice (maximum, then sums) without a
-// second read.  logp_part_kernel leaves per part the partial sums in base 2
-// relative to the part's maximum, the count of elements ahead of the token,
-// and the part's top n as sorted 64-bit keys (value key, complement of the
-// id); logp_rows_kernel (a programmatic dependent launch) joins a row's parts
-// in part order.  No atomics reach a result: the list below is filled in any
-// order and then ranked by unique keys.
+// One pass over the logits.  A row is cut into parts; a part's CTA streams its
+// 16-byte units, LP_UNITS per thread and step with the next step's loads in
+// flight, each thread keeping its maximum, sums in base 2 against a reference
+// that moves only when a step's maximum passes it by LP_HEADROOM, and the count
+// of elements ahead of the token (packed compares and adds).
+// logp_part_kernel leaves per part the sums at the part's maximum, the count,
+// and the part's top n as sorted 64-bit keys (value key, complement of the id);
+// logp_rows_kernel (a programmatic dependent launch) joins a row's parts in part
+// order.  No atomics reach a result: the list below is filled in any order and
+// then ranked by unique keys.
 //
 // Top n of a part without comparing every element: with M_w the thread maxima
 // of warp w, T = max(max_w (n-th largest of M_w), min_w (ceil(n/8)-th largest
 // of M_w)) has at least n elements at or above it, and few more; only threads
-// whose maximum reaches T look through their registers again.
+// whose maximum reaches T look through their units again (from L2).
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
@@ -38,12 +39,13 @@ namespace sd {
 
 constexpr int LP_THREADS = 256;
 constexpr int LP_WARPS = LP_THREADS / 32;
-constexpr int LP_UNITS = 16;                    // 16-byte units per thread and part
-constexpr int LP_CTAS = 2;                      // per SM
-constexpr int LP_LIST = 4096 + 32;              // a part's flagged elements; a row's parts * n
-static_assert(LP_LIST >= SD_TOPN_MAX * 8 * LP_UNITS + 14, "a part's list holds every flagged element");
-static_assert(SD_LOGPROBS_MAX_V / (4 * LP_UNITS * LP_THREADS) + 2 <= LP_LIST / SD_TOPN_MAX,
-              "a row's lists fit the join's list");
+constexpr int LP_UNITS = 4;                     // 16-byte units per thread and step
+constexpr int LP_CTAS = 3;                      // per SM
+constexpr int LP_STEP = LP_THREADS * LP_UNITS;  // units per step of a CTA
+constexpr float LP_HEADROOM = 8.f;              // base 2
+constexpr int LP_LIST = 2048;                   // a part's flagged elements; a row's parts * n
+constexpr int LP_MAX_PARTS = 64;
+static_assert(LP_MAX_PARTS * SD_TOPN_MAX <= LP_LIST, "a row's lists fit the join's list");
 static_assert(SD_TOPN_MAX <= 32, "the n-th largest thread maximum of one warp");
 constexpr int LP_ROW_THREADS = 128;
 
@@ -89,8 +91,7 @@ __device__ __forceinline__ float lp_value(uint32_t k) {
 // What the kernel does on a 32-bit word of the logits' type (two 16-bit
 // elements or one float): maximum with NaN winning, elements, and counting the
 // elements that are not below a threshold (a NaN is not) with packed compares
-// and adds; a thread counts at most 8 * LP_UNITS / 2 = 64 per half, which bf16
-// holds exactly (up to 256).
+// and adds: 4 * LP_UNITS per half and step, which bf16 holds exactly (up to 256).
 template <typename T> struct Word;
 template <> struct Word<__nv_bfloat16> {
   static constexpr int N = 2;
@@ -104,7 +105,7 @@ template <> struct Word<__nv_bfloat16> {
   __device__ static uint32_t count(uint32_t c, uint32_t x, uint32_t thr) {
     return w(__hadd2(v(c), __hgeu2(v(x), v(thr))));
   }
-  __device__ static int total(uint32_t c) { return (int)(get(c, 0) + get(c, 1)); }
+  __device__ static float total(uint32_t c) { return get(c, 0) + get(c, 1); }
   __device__ static bool any(uint32_t x, uint32_t thr) { return w(__hgeu2(v(x), v(thr))) != 0u; }
   // both halves the element's bits; the next larger value of a finite one
   __device__ static uint32_t splat(float f) { return (__float_as_uint(f) >> 16) * 0x10001u; }
@@ -125,7 +126,7 @@ template <> struct Word<__half> {
   __device__ static uint32_t count(uint32_t c, uint32_t x, uint32_t thr) {
     return w(__hadd2(v(c), __hgeu2(v(x), v(thr))));
   }
-  __device__ static int total(uint32_t c) { return (int)(get(c, 0) + get(c, 1)); }
+  __device__ static float total(uint32_t c) { return get(c, 0) + get(c, 1); }
   __device__ static bool any(uint32_t x, uint32_t thr) { return w(__hgeu2(v(x), v(thr))) != 0u; }
   __device__ static uint32_t bits(float f) { return __half_as_ushort(__float2half_rn(f)); }
   __device__ static uint32_t splat(float f) { return bits(f) * 0x10001u; }
@@ -146,7 +147,7 @@ template <> struct Word<float> {
   __device__ static uint32_t count(uint32_t c, uint32_t x, uint32_t thr) {
     return c + !(__uint_as_float(x) < __uint_as_float(thr));
   }
-  __device__ static int total(uint32_t c) { return (int)c; }
+  __device__ static float total(uint32_t c) { return (float)(int)c; }
   __device__ static bool any(uint32_t x, uint32_t thr) {
     return !(__uint_as_float(x) < __uint_as_float(thr));
   }
@@ -223,8 +224,81 @@ __device__ void sort_top(unsigned long long* list, int cnt, int n, unsigned long
   for (int i = cnt + t; i < n; i += THREADS) out[i] = 0ULL;
 }
 
-// Word q of the thread's unit i.
-#define LP_WORD(i, q) (q == 0 ? d[i].x : q == 1 ? d[i].y : q == 2 ? d[i].z : d[i].w)
+// A thread's running state over its units.
+template <typename T>
+struct LpRun {
+  using Wd = Word<T>;
+  uint32_t wm;                                       // maximum, a NaN wins
+  float ref, nref, ahead;                            // reference of the sums and its negative
+  unsigned long long s2, e2;                         // sum 2^d, sum d 2^d, d = (x - ref) c
+  __device__ void init() {
+    wm = Wd::NEG_INF;
+    ref = nref = 0.f;
+    ahead = 0.f;
+    s2 = e2 = 0ULL;
+  }
+  // One step: units u, u + LP_THREADS, ...; `first`: the reference is set, not moved.
+  __device__ __forceinline__ void step(const uint4 (&d)[LP_UNITS], int u, bool first, float c,
+                                       unsigned long long c2, int tu, uint32_t thr_at,
+                                       uint32_t thr_up) {
+    uint32_t g = Wd::vmax(Wd::vmax(d[0].x, d[0].y), Wd::vmax(d[0].z, d[0].w));
+#pragma unroll
+    for (int i = 1; i < LP_UNITS; ++i)
+      g = Wd::vmax(g, Wd::vmax(Wd::vmax(d[i].x, d[i].y), Wd::vmax(d[i].z, d[i].w)));
+    wm = Wd::vmax(wm, g);
+    const float gm = fmaxf(Wd::get(g, 0), Wd::get(g, Wd::N - 1));
+    const float up = (gm - ref) * c;
+    if (first ? gm > -CUDART_INF_F && gm < CUDART_INF_F : up > LP_HEADROOM && gm < CUDART_INF_F) {
+      // the sums so far move to the new reference (2^-256 is 0)
+      const float dm = fmaxf(-up, -256.f), f = lp_ex2(dm);
+      const unsigned long long f2 = pair2(f, f);
+      if (!first) {
+        e2 = mul2(f2, fma2(pair2(dm, dm), s2, e2));
+        s2 = mul2(f2, s2);
+      }
+      ref = gm;
+      nref = -gm;
+    }
+    const unsigned long long nr2 = pair2(nref, nref);
+    uint32_t cnt = 0u;
+#pragma unroll
+    for (int i = 0; i < LP_UNITS; ++i) {
+      const uint32_t thr = u + i * LP_THREADS <= tu ? thr_at : thr_up;
+      const uint32_t w[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) cnt = Wd::count(cnt, w[q], thr);
+#pragma unroll
+      for (int q = 0; q < 4; q += 3 - Wd::N) {
+        const unsigned long long x2 = Wd::N == 2 ? pair2(Wd::get(w[q], 0), Wd::get(w[q], 1))
+                                                 : pair2(Wd::get(w[q], 0), Wd::get(w[q | 1], 0));
+        float a, b;
+        unpair(mul2(add2(x2, nr2), c2), a, b);
+        // -inf elements add 0 * -256, not 0 * -inf
+        a = fmaxf(a, -256.f);
+        b = fmaxf(b, -256.f);
+        const unsigned long long p2 = pair2(lp_ex2(a), lp_ex2(b));
+        s2 = add2(s2, p2);
+        e2 = fma2(pair2(a, b), p2, e2);
+      }
+    }
+    ahead += Wd::total(cnt);
+  }
+};
+
+// A step's units from p on (p: this thread's first); those past `left` units
+// of the part are -inf.
+__device__ __forceinline__ void lp_load(uint4 (&d)[LP_UNITS], const uint4* p) {
+#pragma unroll
+  for (int i = 0; i < LP_UNITS; ++i) d[i] = __ldcs(p + i * LP_THREADS);
+}
+template <typename T>
+__device__ __forceinline__ void lp_load_rest(uint4 (&d)[LP_UNITS], const uint4* p, int left) {
+#pragma unroll
+  for (int i = 0; i < LP_UNITS; ++i) {
+    constexpr uint32_t ni = Word<T>::NEG_INF;
+    d[i] = i * LP_THREADS < left ? __ldcs(p + i * LP_THREADS) : make_uint4(ni, ni, ni, ni);
+  }
+}
 
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const LpParams P) {
@@ -235,7 +309,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const Lp
   __shared__ float red_m[LP_WARPS], red_s[LP_WARPS], red_e[LP_WARPS];
   __shared__ int red_c[LP_WARPS];
   __shared__ uint32_t kth[LP_WARPS], jth[LP_WARPS];
-  __shared__ unsigned long long uth;
+  __shared__ unsigned long long red_k[LP_WARPS];
   __shared__ int n_list, counter;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
@@ -250,15 +324,16 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const Lp
   // < 2 E elements outside them go one each to threads of part 0
   const int h0 = min((int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)), V);
   const int units = (V - h0) / E, tail = V - h0 - units * E;
-  const int per = (units + P.parts - 1) / P.parts;   // <= LP_THREADS * LP_UNITS
+  const int per = (units + P.parts - 1) / P.parts;
   const int u0 = min(part * per, units), u1 = min(u0 + per, units);
   const uint4* body = reinterpret_cast<const uint4*>(row + h0);
-  uint4 d[LP_UNITS];
-#pragma unroll
-  for (int i = 0; i < LP_UNITS; ++i) {
-    const int u = u0 + i * LP_THREADS + t;
-    d[i] = u < u1 ? __ldcs(body + u) : make_uint4(Wd::NEG_INF, Wd::NEG_INF, Wd::NEG_INF, Wd::NEG_INF);
-  }
+  uint4 cur[LP_UNITS], nxt[LP_UNITS];
+  // whole steps two by two, the loads of one in flight while the other is
+  // worked on; then what is left (k whole steps, `left` units past this thread)
+  const uint4* p = body + u0 + t;
+  int k = (u1 - u0) / LP_STEP;
+  const int left = u1 - u0 - k * LP_STEP - t;
+  if (k > 0) lp_load(cur, p); else lp_load_rest<T>(cur, p, left);
   if (t == 0) n_list = 0;
   const bool lone = part == 0 && t < h0 + tail;      // this thread's extra element
   const int xi = t < h0 ? t : V - tail + (t - h0);
@@ -266,62 +341,64 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const Lp
   const int64_t tok = P.ids[rb * P.ids_bs + rl];
   const bool have = tok >= 0 && tok < V;
   const float xt = have ? load_logit(P.x, P.dtype, row0 + tok) : CUDART_INF_F;
-  // thread maximum; a NaN wins
-  uint32_t wm = Wd::NEG_INF;
-#pragma unroll
-  for (int i = 0; i < LP_UNITS; ++i)
-    wm = Wd::vmax(wm, Wd::vmax(Wd::vmax(d[i].x, d[i].y), Wd::vmax(d[i].z, d[i].w)));
-  float m = Word<float>::get(Word<float>::vmax(__float_as_uint(Wd::get(wm, 0)),
-                                               __float_as_uint(Wd::get(wm, Wd::N - 1))), 0);
-  m = __uint_as_float(Word<float>::vmax(__float_as_uint(m), __float_as_uint(xe)));
-  const bool nan = m != m;
-  // sums in base 2 relative to the thread's maximum: d = (x - m) c, held at or
-  // above -256 (2^-256 is 0 here, and -inf elements add 0 * -256, not 0 * -inf)
-  const float m0 = m == -CUDART_INF_F || m == CUDART_INF_F || nan ? 0.f : m;
-  const unsigned long long nm2 = pair2(-m0, -m0), c2 = pair2(P.c, P.c);
-  unsigned long long s2 = 0ULL, e2 = 0ULL;           // (0.f, 0.f)
-  uint32_t cnt = 0u;
-  // elements at ids up to the token's count when not below it, later ones when above it:
-  // units up to the token's compare with x_t, later ones with the next larger value
+  // elements at ids up to the token's count when not below it, later ones when
+  // above it: units up to the token's compare with x_t, later ones with the
+  // next larger value
   const bool plain = have && xt > -CUDART_INF_F && xt < CUDART_INF_F;
   const int tu = tok < h0 ? -1 : (int)((tok - h0) / E);
   const uint32_t thr_at = Wd::splat(xt), thr_up = Wd::above(xt);
-#pragma unroll
-  for (int i = 0; i < LP_UNITS; ++i) {
-    const uint32_t thr = u0 + i * LP_THREADS + t <= tu ? thr_at : thr_up;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint32_t x = LP_WORD(i, q);
-      cnt = Wd::count(cnt, x, thr);
-      unsigned long long x2;
-      if (Wd::N == 2) {
-        x2 = pair2(Wd::get(x, 0), Wd::get(x, 1));
-      } else {
-        if (q & 1) continue;
-        x2 = pair2(Wd::get(x, 0), Wd::get(LP_WORD(i, q + 1), 0));
-      }
-      float a, b;
-      unpair(mul2(add2(x2, nm2), c2), a, b);
-      a = fmaxf(a, -256.f);
-      b = fmaxf(b, -256.f);
-      const unsigned long long p2 = pair2(lp_ex2(a), lp_ex2(b));
-      s2 = add2(s2, p2);
-      e2 = fma2(pair2(a, b), p2, e2);
-    }
+  const unsigned long long c2 = pair2(P.c, P.c);
+  LpRun<T> run;
+  run.init();
+  int u = u0 + t;
+  bool first = true;
+  auto step = [&](const uint4 (&d)[LP_UNITS]) {
+    run.step(d, u, first, P.c, c2, tu, thr_at, thr_up);
+    // the reference is set by the first step that has a finite element
+    first = first && run.s2 == 0ULL;
+    u += LP_STEP;
+  };
+#pragma unroll 1
+  for (; k >= 2; k -= 2) {
+    p += LP_STEP;
+    lp_load(nxt, p);
+    step(cur);
+    p += LP_STEP;
+    if (k > 2) lp_load(cur, p); else lp_load_rest<T>(cur, p, left);
+    step(nxt);
   }
+  if (k == 1) {
+    lp_load_rest<T>(nxt, p + LP_STEP, left);
+    step(cur);
+    step(nxt);
+  } else {
+    step(cur);
+  }
+  float m = __uint_as_float(Word<float>::vmax(
+      Word<float>::vmax(__float_as_uint(Wd::get(run.wm, 0)),
+                        __float_as_uint(Wd::get(run.wm, Wd::N - 1))),
+      __float_as_uint(xe)));
+  const bool nan = m != m;
+  // the thread's sums at its own maximum, with its extra element
+  const float m0 = m == -CUDART_INF_F || m == CUDART_INF_F || nan ? 0.f : m;
   float s, es;
   {
     float a, b;
-    unpair(s2, s, b);
-    unpair(e2, es, a);
+    unpair(run.s2, s, b);
+    unpair(run.e2, es, a);
+    s += b;
+    es += a;
+    const float dm = s > 0.f ? fmaxf((run.ref - m0) * P.c, -256.f) : 0.f, f = lp_ex2(dm);
+    es = f * fmaf(dm, s, es);
+    s *= f;
     const float dd = fmaxf((xe - m0) * P.c, -256.f), p = lp_ex2(dd);
-    s = s + b + p;
-    es = es + a + dd * p;
+    s += p;
+    es = fmaf(dd, p, es);
   }
   const uint32_t kt = lp_key(xt);
   int ahead = 0;
   if (plain) {
-    ahead = Wd::total(cnt);
+    ahead = (int)run.ahead;
     if (tu >= u0 && tu < u1 && (tu - u0) % LP_THREADS == t) {
       // the token's own unit: entries behind it that equal it were counted
       for (int e = (int)((tok - h0) % E) + 1; e < E; ++e)
@@ -388,21 +465,36 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const Lp
       const int at = atomicAdd(&n_list, 1);
       if (at < LP_LIST) list[at] = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)idx;
     };
-    if (any && lp_key(m) >= thr) {
-      const uint32_t tw = Wd::splat(lp_value(thr));
-      if (lone && lp_key(xe) >= thr) put(lp_key(xe), xi);
+    // the warp looks through its flagged threads' units, four threads at a time
+    const uint32_t tw = Wd::splat(lp_value(thr));
+    if (lone && lp_key(xe) >= thr) put(lp_key(xe), xi);
+    uint32_t flagged = __ballot_sync(0xffffffffu, any && lp_key(m) >= thr);
+    while (flagged) {
+      int at[4];
 #pragma unroll
-      for (int i = 0; i < LP_UNITS; ++i) {
-        const int u = u0 + i * LP_THREADS + t;
-        if (u >= u1) break;
+      for (int i = 0; i < 4; ++i) {
+        at[i] = flagged ? u0 + 32 * w + __ffs(flagged) - 1 : u1;
+        flagged &= flagged - 1;
+      }
+#pragma unroll 1
+      for (int o = lane * LP_THREADS; u0 + 32 * w + o < u1; o += 32 * LP_THREADS) {
+        uint4 d[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t x = LP_WORD(i, q);
-          if (Wd::any(x, tw)) {
+        for (int i = 0; i < 4; ++i) {
+          constexpr uint32_t ni = Wd::NEG_INF;
+          d[i] = at[i] + o < u1 ? __ldg(body + at[i] + o) : make_uint4(ni, ni, ni, ni);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (at[i] + o >= u1) continue;
+          const uint32_t x[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (!Wd::any(x[q], tw)) continue;
 #pragma unroll
             for (int e = 0; e < Wd::N; ++e) {
-              const uint32_t k = lp_key(Wd::get(x, e));
-              if (k >= thr) put(k, h0 + u * E + q * Wd::N + e);
+              const uint32_t key = lp_key(Wd::get(x[q], e));
+              if (key >= thr) put(key, h0 + (at[i] + o) * E + q * Wd::N + e);
             }
           }
         }
@@ -411,44 +503,37 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const Lp
     __syncthreads();
     int found = n_list;
     if (found > LP_LIST) {
-      // Many elements equal the threshold (flat logits).  Again with the keys
-      // (value, first unit that reaches it) of the threads: unique, so at
-      // most n threads reach the n-th of them, with their E * LP_UNITS
-      // elements each.  The head and tail elements join as units -1 and
-      // `units`, whose threads' own units hold other values of this key.
-      unsigned long long uk = 0ULL;
-      auto unit_key = [&](uint32_t k, int u) {
-        return ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)(u + 1);
-      };
+      // More elements than the list holds reach the threshold (flat logits):
+      // the n largest keys one after the other, a pass over the part for each.
+      unsigned long long last = ~0ULL;
+      for (int n = 0; n < P.top; ++n) {
+        unsigned long long best = 0ULL;
+        auto see = [&](float x, int idx) {
+          const unsigned long long k =
+              ((unsigned long long)lp_key(x) << 32) | (uint32_t)~(uint32_t)idx;
+          if (k < last && k > best) best = k;
+        };
 #pragma unroll 1
-      for (int u = u0 + t; u < u1; u += LP_THREADS)
-        for (int e = 0; e < E; ++e) {
-          const unsigned long long q =
-              unit_key(lp_key(load_logit(P.x, P.dtype, row0 + h0 + u * E + e)), u);
-          uk = q > uk ? q : uk;
+        for (int v = u0 + t; v < u1; v += LP_THREADS) {
+          const uint4 d = __ldg(body + v);
+          const uint32_t x[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < Wd::N; ++e) see(Wd::get(x[q], e), h0 + v * E + q * Wd::N + e);
         }
-      __syncthreads();
-      list[t] = uk;
-      if (t == 0) n_list = counter = 0;
-      __syncthreads();
-      int before = 0;
-      for (int q = 0; q < LP_THREADS; ++q) before += list[q] > uk;
-      if (before == P.top - 1 && uk != 0ULL) uth = uk;       // exactly one such thread, or too few
-      if (uk != 0ULL) atomicAdd(&counter, 1);
-      __syncthreads();
-      const unsigned long long ut = counter >= P.top ? uth : 1ULL;
-      __syncthreads();
-      if (lone && unit_key(lp_key(xe), xi < h0 ? -1 : units) >= ut) put(lp_key(xe), xi);
-      if (uk >= ut) {
-#pragma unroll 1
-        for (int u = u0 + t; u < u1; u += LP_THREADS)
-          for (int e = 0; e < E; ++e) {
-            const uint32_t k = lp_key(load_logit(P.x, P.dtype, row0 + h0 + u * E + e));
-            if (unit_key(k, u) >= ut) put(k, h0 + u * E + e);
-          }
+        if (lone) see(xe, xi);
+        best = warp_max(best);
+        __syncthreads();                             // red_k of the last round has been read
+        if (lane == 0) red_k[w] = best;
+        __syncthreads();
+        best = red_k[0];
+#pragma unroll
+        for (int q = 1; q < LP_WARPS; ++q) best = red_k[q] > best ? red_k[q] : best;
+        if (t == 0) list[n] = best;
+        last = best;
       }
-      __syncthreads();
-      found = min(n_list, LP_LIST);
+      found = P.top;
       __syncthreads();
     }
     sort_top<LP_THREADS>(list, found, P.top, P.keys + item * P.top, &counter);
@@ -477,8 +562,8 @@ __global__ void __launch_bounds__(LP_ROW_THREADS) logp_rows_kernel(const LpParam
   extern __shared__ __align__(16) unsigned char lp_smem[];
   unsigned long long* list = reinterpret_cast<unsigned long long*>(lp_smem);   // [parts * top]
   __shared__ float sh_m, sh_lz;
-  __shared__ int counter;
-  __shared__ unsigned long long best[SD_TOPN_MAX];
+  __shared__ int counter, n_list;
+  __shared__ unsigned long long sh_t, best[SD_TOPN_MAX];
   const int t = threadIdx.x;
   const int64_t r = blockIdx.x, rb = r / P.L, rl = r % P.L;
   const int64_t tok = P.ids[rb * P.ids_bs + rl];
@@ -518,11 +603,34 @@ __global__ void __launch_bounds__(LP_ROW_THREADS) logp_rows_kernel(const LpParam
   }
   __syncthreads();
   if (P.top == 0) return;
+  // Each part's keys are sorted: the best part's n-th key, and the least of the
+  // parts' ceil(n / parts)-th keys, have n keys at or above them.
   const unsigned long long* keys = P.keys + r * P.parts * P.top;
-  const int all = P.parts * P.top;
-  for (int i = t; i < all; i += LP_ROW_THREADS) list[i] = keys[i];
+  const int all = P.parts * P.top, j = (P.top + P.parts - 1) / P.parts;
+  if (t < 32) {
+    unsigned long long T1 = 0ULL, T2 = ~0ULL;
+    for (int i = t; i < P.parts; i += 32) {
+      const unsigned long long a = keys[i * P.top + P.top - 1], b = keys[i * P.top + j - 1];
+      T1 = a > T1 ? a : T1;
+      T2 = b < T2 ? b : T2;
+    }
+    T1 = warp_max(T1);
+    T2 = warp_min(T2);
+    if (t == 0) {
+      sh_t = T1 > T2 ? T1 : T2;
+      n_list = 0;
+    }
+  }
   __syncthreads();
-  sort_top<LP_ROW_THREADS>(list, all, P.top, best, &counter);
+  const unsigned long long thr = sh_t > 1ULL ? sh_t : 1ULL;    // absent keys are 0
+  for (int i = t; i < all; i += LP_ROW_THREADS) {
+    const unsigned long long k = keys[i];
+    if (k >= thr) list[atomicAdd(&n_list, 1)] = k;
+  }
+  __syncthreads();
+  const int found = n_list;
+  __syncthreads();
+  sort_top<LP_ROW_THREADS>(list, found, P.top, best, &counter);
   __syncthreads();
   if (t < P.top) {
     const unsigned long long k = best[t];
@@ -532,15 +640,25 @@ __global__ void __launch_bounds__(LP_ROW_THREADS) logp_rows_kernel(const LpParam
   }
 }
 
+// Parts per row: the CTAs run in rounds of LP_CTAS per SM, a round takes a
+// part's units plus about LP_FIXED units' time for its start and its join, and
+// the fewest of round * length wins.
+constexpr int LP_FIXED = 2048;
 static int lp_parts(int64_t rows, int V, int dtype) {
   const int E = dtype == SD_DTYPE_F32 ? 4 : 8;
-  // a row that starts off the 16-byte grid covers one unit more
-  const int64_t units = ((int64_t)V + 2 * E - 2) / E;
-  const int64_t least = (units + LP_THREADS * LP_UNITS - 1) / (LP_THREADS * LP_UNITS);
-  const int64_t most = std::min<int64_t>((units + LP_THREADS - 1) / LP_THREADS, 64);
-  // few rows: parts of fewer units, so that two CTAs land on every SM
-  const int64_t fill = (2 * 148 + rows - 1) / rows;
-  return (int)std::max(least, std::min(most, fill));
+  const int64_t units = ((int64_t)V + E - 1) / E, slots = LP_CTAS * 148;
+  const int64_t most = std::min<int64_t>(std::max<int64_t>(units / LP_THREADS, 1), LP_MAX_PARTS);
+  int best = 1;
+  int64_t least = -1;
+  for (int p = 1; p <= most; ++p) {
+    const int64_t rounds = (rows * p + slots - 1) / slots;
+    const int64_t cost = rounds * ((units + p - 1) / p + LP_FIXED);
+    if (least < 0 || cost < least) {
+      least = cost;
+      best = p;
+    }
+  }
+  return best;
 }
 
 template <typename T>

@@ -1,18 +1,19 @@
 """token_logprobs against its definition in 64 bits.
 
 Tolerances, from the kernel's arithmetic.  u = 2^-24.  Every exponent is
-d = (x - m) c with |d| <= 256 and c = log2(e) / T rounded: |error of d| <=
-3 u |d|, plus 2^-22 relative for ex2.approx; the terms' weights 2^d make
-|d| 2^d <= 0.54, so each term is off by at most (3 ln2 u |d| + 2^-22) 2^d, and
-the sum z of at most 64 * 16 sequential adds per level by 2^-22 + 3 ln2 u D
-+ 140 u relative, where D = sum |d| 2^d / z (the entropy's second part in
-bits): a thread adds at most 128 terms one after another, then 5 + 8 + 7 + 7
-joining adds, each u relative of a sum of positive terms.
+d = (x - m) c held at -256 and c = log2(e) / T rounded: |error of d| <=
+3 u |d|, plus 2^-22 relative for ex2.approx; the terms' weights 2^d make the
+mean of that 3 ln2 u D, where D = sum |d| 2^d / z (the entropy's second part in
+bits).  Sums of positive terms lose u relative per add: a thread adds at most
+V / 512 + 8 terms one after another into each of two sums (a part has a step of
+1024 units of 16 bytes or more; 2 V / 512 for fp32), moves them to a larger
+reference a few times (3 u each, at most 20 here) and the joins add 5 + 8 + 7 + 7
+more: K = 150 + V / 256 covers both types.
   log z: absolute error of that relative error, plus u |log z| for logf.
   logprob = (x - m) / T - log z: u |x - m| / T + u |log z| more.
   entropy = log z + ln2 D': D' carries the same relative errors as z plus one
   product per term, twice in the quotient.
-With E(z) = 2^-22 + 150 u + 3 u D: |logprob| is within E + 3 u (|x-m|/T + |log
+With E(z) = 2^-22 + K u + 3 u D: |logprob| is within E + 3 u (|x-m|/T + |log
 z|), |entropy| within 3 E (1 + D).  Ranks and ids are exact.
 """
 import math
@@ -68,7 +69,7 @@ def _bounds(x, T):
     w = d.exp()
     z = w.sum(-1)
     D = (-d * w).sum(-1) / z / math.log(2.0)
-    return 2.0 ** -22 + 150 * U + 3 * U * D, D, z.log().abs()
+    return 2.0 ** -22 + (150 + x.shape[-1] / 256) * U + 3 * U * D, D, z.log().abs()
 
 
 def _check(x, ids, T, n):
