@@ -12,22 +12,25 @@
 // the verify round give a token and its probability after top-k / top-p; a
 // caller that ranks samples needs the untruncated log-probabilities.
 //
-// One pass over the logits.  A row is cut into parts; a part's CTA streams its
-// 16-byte units, LP_UNITS per thread and step with the next step's loads in
-// flight, each thread keeping its maximum, sums in base 2 against a reference
-// that moves only when a step's maximum passes it by LP_HEADROOM, and the count
-// of elements ahead of the token (packed compares and adds).
-// logp_part_kernel leaves per part the sums at the part's maximum, the count,
-// and the part's top n as sorted 64-bit keys (value key, complement of the id);
-// logp_rows_kernel (a programmatic dependent launch) joins a row's parts in part
-// order.  No atomics reach a result: the list below is filled in any order and
-// then ranked by unique keys.
+// One pass over the logits, one launch.  Clusters of 1, 2, 4 or 8 CTAs take
+// either a whole row per CTA or one row together, a part each: whole rows while
+// there is one for every SM, then parts, so that the SMs end together.  A CTA
+// streams its part's 16-byte
+// units, LP_UNITS per thread and step with the next step's loads in flight,
+// each thread keeping its maximum, sums in base 2 against a reference that
+// moves only when a step's maximum passes it by LP_HEADROOM, and the count of
+// elements ahead of the token (packed compares and adds).  Each CTA leaves its
+// sums at the part's maximum, its count and its top n as sorted 64-bit keys
+// (value key, complement of the id) in the shared memory of the cluster's first
+// CTA, which joins them in part order.  No atomics reach a result: the list
+// below is filled in any order and then ranked by unique keys.
 //
-// Top n of a part without comparing every element: with M_w the thread maxima
-// of warp w, T = max(max_w (n-th largest of M_w), min_w (ceil(n/8)-th largest
-// of M_w)) has at least n elements at or above it, and few more; only threads
-// whose maximum reaches T look through their units again (from L2).
+// Top n of a part without comparing every element: of the 32 maxima of 8
+// threads each, the n-th largest has at least n elements at or above it, and
+// few more; only threads whose maximum reaches it look through their units
+// again (from L2), a warp together.
 #include <cuda_runtime.h>
+#include <cooperative_groups.h>
 #include <math_constants.h>
 
 #include <algorithm>
@@ -37,17 +40,19 @@
 
 namespace sd {
 
+namespace cg = cooperative_groups;
+
 constexpr int LP_THREADS = 256;
 constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_UNITS = 4;                     // 16-byte units per thread and step
 constexpr int LP_CTAS = 3;                      // per SM
+constexpr int LP_SMS = 148;
 constexpr int LP_STEP = LP_THREADS * LP_UNITS;  // units per step of a CTA
 constexpr float LP_HEADROOM = 8.f;              // base 2
-constexpr int LP_LIST = 2048;                   // a part's flagged elements; a row's parts * n
-constexpr int LP_MAX_PARTS = 64;
-static_assert(LP_MAX_PARTS * SD_TOPN_MAX <= LP_LIST, "a row's lists fit the join's list");
-static_assert(SD_TOPN_MAX <= 32, "the n-th largest thread maximum of one warp");
-constexpr int LP_ROW_THREADS = 128;
+constexpr int LP_LIST = 2048;                   // a part's flagged elements
+constexpr int LP_MAX_PARTS = 8;                 // CTAs of a cluster
+static_assert(LP_MAX_PARTS * SD_TOPN_MAX <= LP_THREADS, "a thread per key of the join");
+static_assert(SD_TOPN_MAX <= 4 * LP_WARPS, "the n-th largest of the group maxima");
 
 struct LpPart {
   float m, s, e;                                // max (logit units), sum 2^d, sum d 2^d
@@ -59,15 +64,14 @@ struct LpParams {
   int64_t bs, ps;
   const int64_t* ids;
   int64_t ids_bs;
-  int B, L, V, top, parts, dtype;
+  int B, L, V, top, dtype;
+  int csize, whole;                             // CTAs per cluster; clusters of whole rows
   float temperature, c;                         // c = log2(e) / temperature
   float* logprob;
   int64_t* rank;
   float* entropy;
   int64_t* top_ids;
   float* top_lp;
-  LpPart* part;
-  unsigned long long* keys;                     // [rows][parts][top]
 };
 
 __device__ __forceinline__ float lp_ex2(float x) {
@@ -301,21 +305,29 @@ __device__ __forceinline__ void lp_load_rest(uint4 (&d)[LP_UNITS], const uint4* 
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const LpParams P) {
+__global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParams P) {
   using Wd = Word<T>;
   constexpr int E = 4 * Wd::N;                       // elements per 16-byte unit
   extern __shared__ __align__(16) unsigned char lp_smem[];
   unsigned long long* list = reinterpret_cast<unsigned long long*>(lp_smem);   // TOP only
   __shared__ float red_m[LP_WARPS], red_s[LP_WARPS], red_e[LP_WARPS];
   __shared__ int red_c[LP_WARPS];
-  __shared__ uint32_t kth[LP_WARPS], jth[LP_WARPS];
+  __shared__ uint32_t group_k[4 * LP_WARPS];
   __shared__ unsigned long long red_k[LP_WARPS];
   __shared__ int n_list, counter;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // of the cluster's first CTA: what every part found
+  __shared__ LpPart parts[LP_MAX_PARTS];
+  __shared__ unsigned long long part_keys[LP_MAX_PARTS * SD_TOPN_MAX];
+  __shared__ float sh_m, sh_lz;
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-  const int64_t item = blockIdx.x;
-  const int64_t r = item / P.parts;
-  const int part = (int)(item - r * P.parts);
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int cid = (int)(blockIdx.x / P.csize), crank = (int)(blockIdx.x % P.csize);
+  const bool split = cid >= P.whole && P.csize > 1;
+  const int64_t r = split ? (int64_t)P.whole * P.csize + (cid - P.whole)
+                          : (int64_t)cid * P.csize + crank;
+  const int part = split ? crank : 0, nparts = split ? P.csize : 1;
+  // the first CTA's shared memory may be written once its CTA has started
+  if (split) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int64_t rb = r / P.L, rl = r - rb * P.L;
   const int64_t row0 = rb * P.bs + rl * P.ps;
   const T* row = reinterpret_cast<const T*>(P.x) + row0;
@@ -324,7 +336,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const Lp
   // < 2 E elements outside them go one each to threads of part 0
   const int h0 = min((int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)), V);
   const int units = (V - h0) / E, tail = V - h0 - units * E;
-  const int per = (units + P.parts - 1) / P.parts;
+  const int per = (units + nparts - 1) / nparts;
   const int u0 = min(part * per, units), u1 = min(u0 + per, units);
   const uint4* body = reinterpret_cast<const uint4*>(row + h0);
   uint4 cur[LP_UNITS], nxt[LP_UNITS];
@@ -418,24 +430,17 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const Lp
     const uint32_t k = lp_key(xe);
     ahead += k > kt || (k == kt && xi <= tok);
   }
+  if (split) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   // join over the block: the maxima first, then the sums at the block's maximum
   float bm = warp_max(nan ? -CUDART_INF_F : m);
   if (lane == 0) red_m[w] = bm;
   const bool any = u0 + t < u1 || lone;              // this thread holds an element
   if (TOP) {
-    // this warp's sorted thread maxima (bitonic over lanes, falling)
+    // the maximum of 8 threads each
     uint32_t k = any ? lp_key(m) : 0u;
 #pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-      for (int st = size >> 1; st > 0; st >>= 1) {
-        const uint32_t o = __shfl_xor_sync(0xffffffffu, k, st);
-        const bool up = ((lane & size) == 0) == ((lane & st) == 0);
-        k = up ? max(k, o) : min(k, o);
-      }
-    const int j = (P.top + LP_WARPS - 1) / LP_WARPS;
-    if (lane == P.top - 1) kth[w] = k;
-    if (lane == j - 1) jth[w] = k;
+    for (int o = 4; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+    if ((lane & 7) == 0) group_k[4 * w + (lane >> 3)] = k;
   }
   __syncthreads();
   bm = red_m[0];
@@ -454,13 +459,12 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const Lp
     red_c[w] = ahead;
   }
   if (TOP) {
-    uint32_t T1 = 0, T2 = 0xFFFFFFFFu;
+    // the largest group maximum with n group maxima at or above it
+    const uint32_t mine = group_k[lane];
+    int above = 0;
 #pragma unroll
-    for (int q = 0; q < LP_WARPS; ++q) {
-      T1 = max(T1, kth[q]);
-      T2 = min(T2, jth[q]);
-    }
-    const uint32_t thr = max(max(T1, T2), 1u);
+    for (int q = 0; q < 4 * LP_WARPS; ++q) above += group_k[q] >= mine;
+    const uint32_t thr = max(__reduce_max_sync(0xffffffffu, above >= P.top ? mine : 0u), 1u);
     auto put = [&](uint32_t k, int idx) {
       const int at = atomicAdd(&n_list, 1);
       if (at < LP_LIST) list[at] = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)idx;
@@ -536,7 +540,9 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const Lp
       found = P.top;
       __syncthreads();
     }
-    sort_top<LP_THREADS>(list, found, P.top, P.keys + item * P.top, &counter);
+    sort_top<LP_THREADS>(list, found, P.top,
+                         (split ? cluster.map_shared_rank(part_keys, 0) : part_keys) + part * P.top,
+                         &counter);
   } else {
     __syncthreads();
   }
@@ -552,135 +558,88 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_part_kernel(const Lp
       o.e += red_e[q];
       o.ahead += red_c[q];
     }
-    P.part[item] = o;
+    (split ? cluster.map_shared_rank(parts, 0) : parts)[part] = o;
+  }
+  // the cluster's first CTA joins; the others leave once all have delivered
+  if (split) cluster.sync(); else __syncthreads();
+  if (part != 0) return;
+  if (t == 0) {
+    float rm = -CUDART_INF_F, rs = 0.f, re = 0.f;
+    int ra = 0;
+    for (int i = 0; i < nparts; ++i) rm = fmaxf(rm, parts[i].m);
+    for (int i = 0; i < nparts; ++i) {
+      const LpPart q = parts[i];
+      ra += q.ahead;
+      if (q.m == -CUDART_INF_F && q.s == q.s) continue;          // nothing above -inf, no NaN
+      const float dj = lp_hold((q.m - rm) * P.c), fj = lp_ex2(dj);
+      rs = fmaf(fj, q.s, rs);
+      re = fmaf(fj, fmaf(dj, q.s, q.e), re);
+    }
+    const float lz = logf(rs);
+    const bool none = !(rm > -CUDART_INF_F);                     // every entry is -inf
+    sh_m = rm;
+    sh_lz = lz;
+    P.entropy[r] = none || rm == CUDART_INF_F ? CUDART_NAN_F
+                                              : lz - 0.69314718055994531f * (re / rs);
+    P.rank[r] = have ? (int64_t)ra : 0;
+    P.logprob[r] = have && !none ? __fdiv_rn(xt - rm, P.temperature) - lz : CUDART_NAN_F;
+  }
+  if (!TOP) return;
+  __syncthreads();
+  if (t < nparts * P.top) {
+    const unsigned long long key = part_keys[t];
+    int rank = 0;
+    if (nparts == 1) {
+      rank = t;                                      // sorted already
+    } else {
+      for (int q = 0; q < nparts * P.top; ++q) rank += part_keys[q] > key;
+    }
+    if (rank < P.top) {                              // absent keys (0) rank behind the V >= n real ones
+      P.top_ids[r * P.top + rank] = (int64_t)(uint32_t)~(uint32_t)key;
+      P.top_lp[r * P.top + rank] =
+          __fdiv_rn(lp_value((uint32_t)(key >> 32)) - sh_m, P.temperature) - sh_lz;
+    }
   }
 }
 
-// One CTA per row: the parts' sums at the row's maximum, the token, the
-// entropy, and the row's top n from the parts' lists.
-__global__ void __launch_bounds__(LP_ROW_THREADS) logp_rows_kernel(const LpParams P) {
-  extern __shared__ __align__(16) unsigned char lp_smem[];
-  unsigned long long* list = reinterpret_cast<unsigned long long*>(lp_smem);   // [parts * top]
-  __shared__ float sh_m, sh_lz;
-  __shared__ int counter, n_list;
-  __shared__ unsigned long long sh_t, best[SD_TOPN_MAX];
-  const int t = threadIdx.x;
-  const int64_t r = blockIdx.x, rb = r / P.L, rl = r % P.L;
-  const int64_t tok = P.ids[rb * P.ids_bs + rl];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const LpPart* part = P.part + r * P.parts;
-  if (t < 32) {
-    float m = -CUDART_INF_F;
-    for (int i = t; i < P.parts; i += 32) m = fmaxf(m, part[i].m);
-    m = warp_max(m);
-    float s = 0.f, e = 0.f;
-    int ahead = 0;
-    for (int i = t; i < P.parts; i += 32) {
-      const LpPart q = part[i];
-      ahead += q.ahead;
-      if (q.m == -CUDART_INF_F && q.s == q.s) continue;          // nothing finite, no NaN
-      const float dm = lp_hold((q.m - m) * P.c), f = lp_ex2(dm);
-      s = fmaf(f, q.s, s);
-      e = fmaf(f, fmaf(dm, q.s, q.e), e);
-    }
-    s = warp_sum(s);
-    e = warp_sum(e);
-    ahead = warp_sum(ahead);
-    if (t == 0) {
-      const float lz = logf(s);
-      sh_m = m;
-      sh_lz = lz;
-      const bool none = !(m > -CUDART_INF_F);                    // every entry is -inf
-      const bool have = tok >= 0 && tok < P.V;
-      P.entropy[r] = none || m == CUDART_INF_F ? CUDART_NAN_F
-                                               : lz - 0.69314718055994531f * (e / s);
-      P.rank[r] = have ? (int64_t)ahead : 0;
-      float lp = CUDART_NAN_F;
-      if (have && !none)
-        lp = __fdiv_rn(load_logit(P.x, P.dtype, rb * P.bs + rl * P.ps + tok) - m, P.temperature) - lz;
-      P.logprob[r] = lp;
-    }
-  }
-  __syncthreads();
-  if (P.top == 0) return;
-  // Each part's keys are sorted: the best part's n-th key, and the least of the
-  // parts' ceil(n / parts)-th keys, have n keys at or above them.
-  const unsigned long long* keys = P.keys + r * P.parts * P.top;
-  const int all = P.parts * P.top, j = (P.top + P.parts - 1) / P.parts;
-  if (t < 32) {
-    unsigned long long T1 = 0ULL, T2 = ~0ULL;
-    for (int i = t; i < P.parts; i += 32) {
-      const unsigned long long a = keys[i * P.top + P.top - 1], b = keys[i * P.top + j - 1];
-      T1 = a > T1 ? a : T1;
-      T2 = b < T2 ? b : T2;
-    }
-    T1 = warp_max(T1);
-    T2 = warp_min(T2);
-    if (t == 0) {
-      sh_t = T1 > T2 ? T1 : T2;
-      n_list = 0;
-    }
-  }
-  __syncthreads();
-  const unsigned long long thr = sh_t > 1ULL ? sh_t : 1ULL;    // absent keys are 0
-  for (int i = t; i < all; i += LP_ROW_THREADS) {
-    const unsigned long long k = keys[i];
-    if (k >= thr) list[atomicAdd(&n_list, 1)] = k;
-  }
-  __syncthreads();
-  const int found = n_list;
-  __syncthreads();
-  sort_top<LP_ROW_THREADS>(list, found, P.top, best, &counter);
-  __syncthreads();
-  if (t < P.top) {
-    const unsigned long long k = best[t];
-    const float v = lp_value((uint32_t)(k >> 32));
-    P.top_ids[r * P.top + t] = (int64_t)(uint32_t)~(uint32_t)k;
-    P.top_lp[r * P.top + t] = __fdiv_rn(v - sh_m, P.temperature) - sh_lz;
-  }
-}
-
-// Parts per row: the CTAs run in rounds of LP_CTAS per SM, a round takes a
-// part's units plus about LP_FIXED units' time for its start and its join, and
-// the fewest of round * length wins.
-constexpr int LP_FIXED = 2048;
-static int lp_parts(int64_t rows, int V, int dtype) {
-  const int E = dtype == SD_DTYPE_F32 ? 4 : 8;
-  const int64_t units = ((int64_t)V + E - 1) / E, slots = LP_CTAS * 148;
-  const int64_t most = std::min<int64_t>(std::max<int64_t>(units / LP_THREADS, 1), LP_MAX_PARTS);
-  int best = 1;
-  int64_t least = -1;
-  for (int p = 1; p <= most; ++p) {
-    const int64_t rounds = (rows * p + slots - 1) / slots;
-    const int64_t cost = rounds * ((units + p - 1) / p + LP_FIXED);
-    if (least < 0 || cost < least) {
-      least = cost;
-      best = p;
-    }
-  }
-  return best;
+// How the rows are cut.  Up to one row per SM, every row is split, over as many
+// CTAs as fit the machine at once; beyond, whole rows while there is one for
+// every SM and the rest in halves, so that the SMs end together.  Measured
+// (bf16, V = 151936, five alternatives; us): 8 rows in 8 parts 8.0, in 4 9.8, in
+// 1 16.2; 100 rows in 4 parts 13.4, in 2 15.5, in 8 21.5; 148 rows in 2 parts
+// 15.9, in 4 21.8, in 1 18.4; 320 rows, 296 of them whole and 24 in halves 26.2,
+// all whole 31.2, all in halves 33.0.  A part has at least a unit per thread.
+struct LpPlan { int csize, whole; int64_t ctas; };
+static LpPlan lp_plan(int64_t rows, int V, int dtype) {
+  const int units = V / (dtype == SD_DTYPE_F32 ? 4 : 8);
+  LpPlan p = {2, 0, 0};
+  if (rows * 8 <= LP_SMS)
+    p.csize = 8;
+  else if (rows * 4 <= LP_SMS * LP_CTAS)
+    p.csize = 4;
+  while (p.csize > 1 && units / p.csize < LP_THREADS) p.csize /= 2;
+  const int64_t full = p.csize == 1 ? rows : rows <= LP_SMS ? 0 : rows / LP_SMS * LP_SMS;
+  p.whole = (int)(full / p.csize);
+  p.ctas = full + (rows - full) * p.csize;
+  return p;
 }
 
 template <typename T>
-static int launch_logprobs(const LpParams& P, cudaStream_t st) {
-  const int64_t rows = (int64_t)P.B * P.L;
-  const dim3 grid((unsigned)(rows * P.parts));
-  if (P.top > 0)
-    logp_part_kernel<T, true><<<grid, LP_THREADS, LP_LIST * sizeof(unsigned long long), st>>>(P);
-  else
-    logp_part_kernel<T, false><<<grid, LP_THREADS, 0, st>>>(P);
-  if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
+static int launch_logprobs(const LpParams& P, int64_t ctas, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)rows);
-  cfg.blockDim = dim3(LP_ROW_THREADS);
-  cfg.dynamicSmemBytes = (size_t)P.parts * P.top * sizeof(unsigned long long);
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(LP_THREADS);
+  cfg.dynamicSmemBytes = P.top > 0 ? LP_LIST * sizeof(unsigned long long) : 0;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)P.csize;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, logp_rows_kernel, P) != cudaSuccess) return SD_ELAUNCH;
+  const cudaError_t rc = P.top > 0 ? cudaLaunchKernelEx(&cfg, logp_kernel<T, true>, P)
+                                   : cudaLaunchKernelEx(&cfg, logp_kernel<T, false>, P);
+  if (rc != cudaSuccess) return SD_ELAUNCH;
   return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
 }
 
@@ -690,19 +649,10 @@ using namespace sd;
 
 extern "C" {
 
-size_t sd_token_logprobs_workspace_bytes(int B, int L, int V, int dtype, int top_n) {
-  if (B <= 0 || L <= 0 || V <= 0 || V > SD_LOGPROBS_MAX_V || top_n < 0 || top_n > SD_TOPN_MAX)
-    return 0;
-  const int64_t rows = (int64_t)B * L;
-  const size_t items = (size_t)rows * lp_parts(rows, V, dtype);
-  return items * (sizeof(LpPart) + (size_t)top_n * sizeof(unsigned long long));
-}
-
 int sd_token_logprobs(const void* logits, int64_t bs, int64_t ps, int dtype, const int64_t* ids,
                       int64_t ids_bs, int B, int L, int V, float temperature, int top_n,
                       float* logprob, int64_t* rank, float* entropy, int64_t* top_ids,
-                      float* top_logprobs, void* workspace, size_t workspace_bytes,
-                      void* stream) {
+                      float* top_logprobs, void* stream) {
   if (B < 0 || L < 0) return SD_EINVAL;
   if (B == 0 || L == 0) return SD_OK;
   if (!logits || !ids || !logprob || !rank || !entropy || V <= 0) return SD_EINVAL;
@@ -711,27 +661,22 @@ int sd_token_logprobs(const void* logits, int64_t bs, int64_t ps, int dtype, con
   if (top_n < 0 || top_n > V || (top_n > 0 && (!top_ids || !top_logprobs))) return SD_EINVAL;
   const int64_t rows = (int64_t)B * L;
   if (V > SD_LOGPROBS_MAX_V || top_n > SD_TOPN_MAX) return SD_ENOTSUP;
-  const int parts = lp_parts(rows, V, dtype);
-  if (rows * parts > 0x7FFFFFFF) return SD_ENOTSUP;
+  const LpPlan plan = lp_plan(rows, V, dtype);
+  if (plan.ctas > 0x7FFFFFFF) return SD_ENOTSUP;
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == SD_DTYPE_F32 ? 4 : 2)) return SD_EINVAL;
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
-      workspace_bytes < sd_token_logprobs_workspace_bytes(B, L, V, dtype, top_n))
-    return SD_ENOSPC;
   LpParams P;
   P.x = logits; P.bs = bs; P.ps = ps; P.dtype = dtype;
   P.ids = ids; P.ids_bs = ids_bs;
-  P.B = B; P.L = L; P.V = V; P.top = top_n; P.parts = parts;
+  P.B = B; P.L = L; P.V = V; P.top = top_n;
+  P.csize = plan.csize; P.whole = plan.whole;
   P.temperature = temperature;
   P.c = (float)(1.4426950408889634 / (double)temperature);
   P.logprob = logprob; P.rank = rank; P.entropy = entropy;
   P.top_ids = top_ids; P.top_lp = top_logprobs;
-  // keys first: both arrays then sit on their own alignment
-  P.keys = reinterpret_cast<unsigned long long*>(workspace);
-  P.part = reinterpret_cast<LpPart*>(P.keys + (size_t)rows * parts * top_n);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == SD_DTYPE_BF16) return launch_logprobs<__nv_bfloat16>(P, st);
-  if (dtype == SD_DTYPE_F16) return launch_logprobs<__half>(P, st);
-  return launch_logprobs<float>(P, st);
+  if (dtype == SD_DTYPE_BF16) return launch_logprobs<__nv_bfloat16>(P, plan.ctas, st);
+  if (dtype == SD_DTYPE_F16) return launch_logprobs<__half>(P, plan.ctas, st);
+  return launch_logprobs<float>(P, plan.ctas, st);
 }
 
 }  // extern "C"

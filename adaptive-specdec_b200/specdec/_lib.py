@@ -38,9 +38,8 @@ _SIGNATURES = {
     "sd_residual_probs": ([_vp, _vp, _i32, _i32, _vp, _vp], _i32),
     "sd_sample_from_probs": ([_vp, _i32, _i32, _vp, _vp, _vp], _i32),
     "sd_gather_prob": ([_vp, _i32, _i32, _vp, _vp, _vp], _i32),
-    "sd_token_logprobs_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32], _sz),
     "sd_token_logprobs": ([_vp, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _f32, _i32, _vp,
-                           _vp, _vp, _vp, _vp, _vp, _sz, _vp], _i32),
+                           _vp, _vp, _vp, _vp, _vp], _i32),
     "sd_pages_workspace_bytes": ([_i32], _sz),
     "sd_pages_reserve": ([_vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _i64,
                           _vp, _vp, _vp, _sz, _vp], _i32),

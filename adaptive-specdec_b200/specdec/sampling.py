@@ -316,12 +316,8 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
         entropy = torch.empty(shape, dtype=torch.float32, device=dev)
         top_ids = torch.empty(shape + (n,), dtype=torch.long, device=dev) if n else None
         top_lp = torch.empty(shape + (n,), dtype=torch.float32, device=dev) if n else None
-        # a fresh buffer per call: calls on several streams and calls captured
-        # into different graphs never share one
-        nws = L.workspace_bytes("sd_token_logprobs_workspace_bytes", B, Lr, V, code, n)
-        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
         L.check(L.lib().sd_token_logprobs(
             x.data_ptr(), bs, ps, code, ids.data_ptr(), ids_bs, B, Lr, V, T, n, logprob.data_ptr(),
             rank.data_ptr(), entropy.data_ptr(), L.address(top_ids), L.address(top_lp),
-            ws.data_ptr(), nws, L.stream_of(dev)), "token_logprobs")
+            L.stream_of(dev)), "token_logprobs")
     return TokenLogprobs(logprob, rank, entropy, top_ids, top_lp)

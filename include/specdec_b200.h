@@ -188,15 +188,15 @@ int sd_gather_prob(const float* probs, int n_rows, int V, const int64_t* ids, fl
  * position) gets logprob NaN and rank 0; its row's other outputs are as for
  * any id.  -inf entries have probability 0.  A row with a NaN or a +inf, or
  * with nothing above -inf, has NaN log-probabilities and entropy (as the
- * formula); its rank and top_ids still follow the logits, NaN first.
+ * formula); its rank and top_ids still follow the logits, NaN first.  Needs
+ * no workspace.
  */
 #define SD_TOPN_MAX 32
 #define SD_LOGPROBS_MAX_V (1 << 20)
-size_t sd_token_logprobs_workspace_bytes(int B, int L, int V, int dtype, int top_n);
 int sd_token_logprobs(const void* logits, int64_t bs, int64_t ps, int dtype, const int64_t* ids,
                       int64_t ids_bs, int B, int L, int V, float temperature, int top_n,
                       float* logprob, int64_t* rank, float* entropy, int64_t* top_ids,
-                      float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
+                      float* top_logprobs, void* stream);
 
 /* ---- ragged KV cache (reference specdec/kvcache.py) --------------------- */
 

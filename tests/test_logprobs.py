@@ -296,9 +296,9 @@ def test_arguments_are_checked_before_any_launch():
     lib = L.lib()
     n, d = ctypes.c_void_p(0), ctypes.c_void_p(4096)
 
-    def call(x=d, dtype=2, ids=d, B=2, Lr=3, V=100, T=1.0, top=0, out=d, tops=n, ws=d, nws=1 << 20):
+    def call(x=d, dtype=2, ids=d, B=2, Lr=3, V=100, T=1.0, top=0, out=d, tops=n):
         return lib.sd_token_logprobs(x, 0, 0, dtype, ids, 0, B, Lr, V, T, top, out, d, d, tops, tops,
-                                     ws, nws, n)
+                                     n)
     assert call(B=0) == 0 and call(Lr=0) == 0                  # nothing to do
     assert call(B=-1) == -22 and call(x=n) == -22 and call(ids=n) == -22 and call(out=n) == -22
     assert call(V=0) == -22 and call(dtype=3) == -22
@@ -308,6 +308,3 @@ def test_arguments_are_checked_before_any_launch():
     assert call(top=33, tops=d) == -95
     assert call(V=(1 << 20) + 1) == -95
     assert call(x=ctypes.c_void_p(4097)) == -22                # not aligned to its type
-    assert call(ws=n) == -28 and call(nws=16) == -28
-    assert lib.sd_token_logprobs_workspace_bytes(64, 5, 151936, 2, 5) > 0
-    assert lib.sd_token_logprobs_workspace_bytes(64, 5, 151936, 2, 33) == 0
