@@ -34,7 +34,6 @@
 #include <math_constants.h>
 
 #include <algorithm>
-#include <cfloat>
 
 #include "sd_common.cuh"
 
@@ -45,7 +44,7 @@ namespace cg = cooperative_groups;
 constexpr int LP_THREADS = 256;
 constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_UNITS = 4;                     // 16-byte units per thread and step
-constexpr int LP_CTAS = 3;                      // per SM
+constexpr int LP_CTAS = 4;                      // per SM
 constexpr int LP_SMS = 148;
 constexpr int LP_STEP = LP_THREADS * LP_UNITS;  // units per step of a CTA
 constexpr float LP_HEADROOM = 8.f;              // base 2
@@ -55,7 +54,7 @@ static_assert(LP_MAX_PARTS * SD_TOPN_MAX <= LP_THREADS, "a thread per key of the
 static_assert(SD_TOPN_MAX <= 4 * LP_WARPS, "the n-th largest of the group maxima");
 
 struct LpPart {
-  float m, s, e;                                // max (logit units), sum 2^d, sum d 2^d
+  float m, s, e;                                // max (base-2 units), sum 2^d, sum d 2^d
   int ahead;                                    // elements at or ahead of the token
 };
 
@@ -66,7 +65,7 @@ struct LpParams {
   int64_t ids_bs;
   int B, L, V, top, dtype;
   int csize, whole;                             // CTAs per cluster; clusters of whole rows
-  float temperature, c;                         // c = log2(e) / temperature
+  float c;                                      // log2(e) / temperature
   float* logprob;
   int64_t* rank;
   float* entropy;
@@ -88,6 +87,13 @@ __device__ __forceinline__ uint32_t lp_key(float f) {
 // maximum (-inf, or a mask of the type's lowest value) then adds 0 * -256 to
 // the entropy sum, not 0 * -inf.  A NaN stays.
 __device__ __forceinline__ float lp_hold(float x) { return x < -256.f ? -256.f : x; }
+// ln2 (x c - lse): a log-probability from a logit and the base-2 log of the sum.
+// In 64 bits, where x c is exact and the difference loses nothing; the rounding
+// of the sum alone may not make a probability above 1.
+__device__ __forceinline__ float lp_final(float x, float c, double lse) {
+  const double v = 0.69314718055994530942 * ((double)x * (double)c - lse);
+  return v > 0.0 ? 0.f : (float)v;
+}
 __device__ __forceinline__ float lp_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
@@ -228,42 +234,41 @@ __device__ void sort_top(unsigned long long* list, int cnt, int n, unsigned long
   for (int i = cnt + t; i < n; i += THREADS) out[i] = 0ULL;
 }
 
-// A thread's running state over its units.
+// A thread's running state over its units.  Exponents are d = fma(x, c, -R) with
+// the reference R a float in base-2 units: one rounding of d, whatever the size
+// of x c, as long as everything is measured against the same R.
 template <typename T>
 struct LpRun {
   using Wd = Word<T>;
   uint32_t wm;                                       // maximum, a NaN wins
-  float ref, nref, ahead;                            // reference of the sums and its negative
-  unsigned long long s2, e2;                         // sum 2^d, sum d 2^d, d = (x - ref) c
+  float R, ahead;
+  unsigned long long s2, e2;                         // sums of 2^d and d 2^d
   __device__ void init() {
     wm = Wd::NEG_INF;
-    ref = nref = 0.f;
-    ahead = 0.f;
+    R = ahead = 0.f;
     s2 = e2 = 0ULL;
   }
-  // One step: units u, u + LP_THREADS, ...; `first`: the reference is set, not moved.
-  __device__ __forceinline__ void step(const uint4 (&d)[LP_UNITS], int u, bool first, float c,
-                                       unsigned long long c2, int tu, uint32_t thr_at,
-                                       uint32_t thr_up) {
+  // One step: units u, u + LP_THREADS, ...
+  __device__ __forceinline__ void step(const uint4 (&d)[LP_UNITS], int u, float c, int tu,
+                                       uint32_t thr_at, uint32_t thr_up) {
     uint32_t g = Wd::vmax(Wd::vmax(d[0].x, d[0].y), Wd::vmax(d[0].z, d[0].w));
 #pragma unroll
     for (int i = 1; i < LP_UNITS; ++i)
       g = Wd::vmax(g, Wd::vmax(Wd::vmax(d[i].x, d[i].y), Wd::vmax(d[i].z, d[i].w)));
     wm = Wd::vmax(wm, g);
-    const float gm = fmaxf(Wd::get(g, 0), Wd::get(g, Wd::N - 1));
-    const float up = (gm - ref) * c;
-    if (first ? gm > -CUDART_INF_F && gm < CUDART_INF_F : up > LP_HEADROOM && gm < CUDART_INF_F) {
+    const float gs = fmaxf(Wd::get(g, 0), Wd::get(g, Wd::N - 1)) * c;
+    // nothing summed yet: any finite maximum is the reference
+    const bool first = s2 == 0ULL;
+    if (gs < CUDART_INF_F && (first ? gs > -CUDART_INF_F : gs - R > LP_HEADROOM)) {
       // the sums so far move to the new reference (2^-256 is 0)
-      const float dm = fmaxf(-up, -256.f), f = lp_ex2(dm);
+      const float dm = fmaxf(R - gs, -256.f), f = lp_ex2(dm);
       const unsigned long long f2 = pair2(f, f);
-      if (!first) {
-        e2 = mul2(f2, fma2(pair2(dm, dm), s2, e2));
-        s2 = mul2(f2, s2);
-      }
-      ref = gm;
-      nref = -gm;
+      e2 = mul2(f2, fma2(pair2(dm, dm), s2, e2));
+      s2 = mul2(f2, s2);
+      if (first) s2 = e2 = 0ULL;
+      R = gs;
     }
-    const unsigned long long nr2 = pair2(nref, nref);
+    const unsigned long long c2 = pair2(c, c), nR2 = pair2(-R, -R);
     uint32_t cnt = 0u;
 #pragma unroll
     for (int i = 0; i < LP_UNITS; ++i) {
@@ -276,7 +281,7 @@ struct LpRun {
         const unsigned long long x2 = Wd::N == 2 ? pair2(Wd::get(w[q], 0), Wd::get(w[q], 1))
                                                  : pair2(Wd::get(w[q], 0), Wd::get(w[q | 1], 0));
         float a, b;
-        unpair(mul2(add2(x2, nr2), c2), a, b);
+        unpair(fma2(x2, c2, nR2), a, b);
         // -inf elements add 0 * -256, not 0 * -inf
         a = fmaxf(a, -256.f);
         b = fmaxf(b, -256.f);
@@ -318,7 +323,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   // of the cluster's first CTA: what every part found
   __shared__ LpPart parts[LP_MAX_PARTS];
   __shared__ unsigned long long part_keys[LP_MAX_PARTS * SD_TOPN_MAX];
-  __shared__ float sh_m, sh_lz;
+  __shared__ double sh_lse;                          // log2 of the sum of all exponentials
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   const cg::cluster_group cluster = cg::this_cluster();
   const int cid = (int)(blockIdx.x / P.csize), crank = (int)(blockIdx.x % P.csize);
@@ -359,15 +364,11 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   const bool plain = have && xt > -CUDART_INF_F && xt < CUDART_INF_F;
   const int tu = tok < h0 ? -1 : (int)((tok - h0) / E);
   const uint32_t thr_at = Wd::splat(xt), thr_up = Wd::above(xt);
-  const unsigned long long c2 = pair2(P.c, P.c);
   LpRun<T> run;
   run.init();
   int u = u0 + t;
-  bool first = true;
   auto step = [&](const uint4 (&d)[LP_UNITS]) {
-    run.step(d, u, first, P.c, c2, tu, thr_at, thr_up);
-    // the reference is set by the first step that has a finite element
-    first = first && run.s2 == 0ULL;
+    run.step(d, u, P.c, tu, thr_at, thr_up);
     u += LP_STEP;
   };
 #pragma unroll 1
@@ -391,8 +392,9 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
                         __float_as_uint(Wd::get(run.wm, Wd::N - 1))),
       __float_as_uint(xe)));
   const bool nan = m != m;
-  // the thread's sums at its own maximum, with its extra element
-  const float m0 = m == -CUDART_INF_F || m == CUDART_INF_F || nan ? 0.f : m;
+  // the thread's sums at its own maximum (base-2 units), with its extra element
+  const float ms = m * P.c;
+  const float m0 = ms > -CUDART_INF_F && ms < CUDART_INF_F ? ms : 0.f;
   float s, es;
   {
     float a, b;
@@ -400,10 +402,10 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
     unpair(run.e2, es, a);
     s += b;
     es += a;
-    const float dm = s > 0.f ? fmaxf((run.ref - m0) * P.c, -256.f) : 0.f, f = lp_ex2(dm);
+    const float dm = s > 0.f ? fmaxf(run.R - m0, -256.f) : 0.f, f = lp_ex2(dm);
     es = f * fmaf(dm, s, es);
     s *= f;
-    const float dd = fmaxf((xe - m0) * P.c, -256.f), p = lp_ex2(dd);
+    const float dd = fmaxf(fmaf(xe, P.c, -m0), -256.f), p = lp_ex2(dd);
     s += p;
     es = fmaf(dd, p, es);
   }
@@ -432,7 +434,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   }
   if (split) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   // join over the block: the maxima first, then the sums at the block's maximum
-  float bm = warp_max(nan ? -CUDART_INF_F : m);
+  float bm = warp_max(nan ? -CUDART_INF_F : ms);
   if (lane == 0) red_m[w] = bm;
   const bool any = u0 + t < u1 || lone;              // this thread holds an element
   if (TOP) {
@@ -446,10 +448,10 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   bm = red_m[0];
 #pragma unroll
   for (int q = 1; q < LP_WARPS; ++q) bm = fmaxf(bm, red_m[q]);
-  const float dm = lp_hold((m - bm) * P.c), f = lp_ex2(dm);
+  const float dm = lp_hold(ms - bm), f = lp_ex2(dm);
   float sj = f * s, ej = f * fmaf(dm, s, es);
-  if (m == -CUDART_INF_F) sj = ej = 0.f;             // nothing above -inf
-  if (nan || m == CUDART_INF_F) sj = CUDART_NAN_F;   // as the formula: inf - inf
+  if (ms == -CUDART_INF_F) sj = ej = 0.f;            // nothing above -inf
+  if (nan || ms == CUDART_INF_F) sj = CUDART_NAN_F;  // as the formula: inf - inf
   sj = warp_sum(sj);
   ej = warp_sum(ej);
   ahead = warp_sum(ahead);
@@ -571,18 +573,17 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
       const LpPart q = parts[i];
       ra += q.ahead;
       if (q.m == -CUDART_INF_F && q.s == q.s) continue;          // nothing above -inf, no NaN
-      const float dj = lp_hold((q.m - rm) * P.c), fj = lp_ex2(dj);
+      const float dj = lp_hold(q.m - rm), fj = lp_ex2(dj);
       rs = fmaf(fj, q.s, rs);
       re = fmaf(fj, fmaf(dj, q.s, q.e), re);
     }
-    const float lz = logf(rs);
+    const float lz = log2f(rs);
     const bool none = !(rm > -CUDART_INF_F);                     // every entry is -inf
-    sh_m = rm;
-    sh_lz = lz;
-    P.entropy[r] = none || rm == CUDART_INF_F ? CUDART_NAN_F
-                                              : lz - 0.69314718055994531f * (re / rs);
+    sh_lse = none ? CUDART_NAN : (double)rm + (double)lz;
+    const float h = 0.69314718055994531f * (lz - re / rs);
+    P.entropy[r] = none || rm == CUDART_INF_F ? CUDART_NAN_F : h < 0.f ? 0.f : h;
     P.rank[r] = have ? (int64_t)ra : 0;
-    P.logprob[r] = have && !none ? __fdiv_rn(xt - rm, P.temperature) - lz : CUDART_NAN_F;
+    P.logprob[r] = have ? lp_final(xt, P.c, sh_lse) : CUDART_NAN_F;
   }
   if (!TOP) return;
   __syncthreads();
@@ -597,7 +598,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
     if (rank < P.top) {                              // absent keys (0) rank behind the V >= n real ones
       P.top_ids[r * P.top + rank] = (int64_t)(uint32_t)~(uint32_t)key;
       P.top_lp[r * P.top + rank] =
-          __fdiv_rn(lp_value((uint32_t)(key >> 32)) - sh_m, P.temperature) - sh_lz;
+          lp_final(lp_value((uint32_t)(key >> 32)), P.c, sh_lse);
     }
   }
 }
@@ -657,7 +658,7 @@ int sd_token_logprobs(const void* logits, int64_t bs, int64_t ps, int dtype, con
   if (B == 0 || L == 0) return SD_OK;
   if (!logits || !ids || !logprob || !rank || !entropy || V <= 0) return SD_EINVAL;
   if (dtype != SD_DTYPE_F32 && dtype != SD_DTYPE_F16 && dtype != SD_DTYPE_BF16) return SD_EINVAL;
-  if (!(temperature > 0.f) || temperature > FLT_MAX) return SD_EINVAL;
+  if (!(temperature >= 1e-6f && temperature <= 1e6f)) return SD_EINVAL;
   if (top_n < 0 || top_n > V || (top_n > 0 && (!top_ids || !top_logprobs))) return SD_EINVAL;
   const int64_t rows = (int64_t)B * L;
   if (V > SD_LOGPROBS_MAX_V || top_n > SD_TOPN_MAX) return SD_ENOTSUP;
@@ -669,7 +670,6 @@ int sd_token_logprobs(const void* logits, int64_t bs, int64_t ps, int dtype, con
   P.ids = ids; P.ids_bs = ids_bs;
   P.B = B; P.L = L; P.V = V; P.top = top_n;
   P.csize = plan.csize; P.whole = plan.whole;
-  P.temperature = temperature;
   P.c = (float)(1.4426950408889634 / (double)temperature);
   P.logprob = logprob; P.rank = rank; P.entropy = entropy;
   P.top_ids = top_ids; P.top_lp = top_logprobs;

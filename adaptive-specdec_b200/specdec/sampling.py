@@ -264,7 +264,7 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
     """Log-probabilities of ``ids`` under softmax(logits / temperature).
 
     logits [..., V] (bf16 / fp16 / fp32, vocabulary contiguous, other strides
-    free up to three dimensions), ids [...] integer.  Per position: the
+    free up to three dimensions), ids [...] integer, temperature in [1e-6, 1e6].  Per position: the
     token's log-probability, its rank by (logit falling, id rising; 1 = first),
     the entropy of the distribution, and with ``top_n`` > 0 the first top_n ids
     in that order with their log-probabilities.  No top-p / top-k applies.  An
@@ -289,8 +289,8 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
         raise L.SpecdecError(f"the vocabulary must have 1 to {LOGPROBS_MAX_V} entries, got {V}")
     if not 0 <= n <= min(V, TOP_N_MAX):
         raise L.SpecdecError(f"top_n must be between 0 and min(V, {TOP_N_MAX}), got {n}")
-    if not 0.0 < T < float("inf"):
-        raise L.SpecdecError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-6 <= T <= 1e6:
+        raise L.SpecdecError(f"temperature must be between 1e-6 and 1e6, got {temperature}")
     # rows (b, l) with strides (bs, ps), their ids with stride ids_bs over b
     dims = logits.dim()
     if V == 1:

@@ -1,8 +1,8 @@
 """token_logprobs against its definition in 64 bits.
 
 Tolerances, from the kernel's arithmetic.  u = 2^-24.  Every exponent is
-d = (x - m) c held at -256 and c = log2(e) / T rounded: |error of d| <=
-3 u |d|, plus 2^-22 relative for ex2.approx; the terms' weights 2^d make the
+d = fma(x, c, -R) held at -256 against a float reference R that cancels, and c =
+log2(e) / T rounded: |error of d| <= 3 u |d|, plus 2^-22 relative for ex2.approx; the terms' weights 2^d make the
 mean of that 3 ln2 u D, where D = sum |d| 2^d / z (the entropy's second part in
 bits).  Sums of positive terms lose u relative per add: a thread adds at most
 V / 512 + 8 terms one after another into each of two sums (a part has a step of
@@ -168,7 +168,10 @@ def test_masked_entries(dt):
     ids[0], ids[1], ids[2], ids[3], ids[4] = 3, 39999, 4, 0, 200
     got = _check(x, ids, 0.7, 32)
     assert float(got.logprob[4]) == -math.inf
-    assert float(got.logprob[3]) == 0.0 and float(got.entropy[3]) == 0.0
+    # one live entry: its exponent is fma(m, c, -R) with R = m c rounded, |m c| u at
+    # most, and the sum rounds to 1; never above 0
+    near = float(x[3, 0].abs()) / 0.7 * U
+    assert -near <= float(got.logprob[3]) <= 0.0 <= float(got.entropy[3]) <= near
 
 
 @gpu
@@ -216,6 +219,17 @@ def test_padding_ids():
     ids = torch.tensor([-1, 12000, 11999, 2 ** 40], device=DEV)
     got = _check(x, ids, 1.0, 2)
     assert got.rank.tolist()[:2] == [0, 0] and got.rank.tolist()[3] == 0
+
+
+@gpu
+@pytest.mark.parametrize("T", [1e-3, 0.05, 30.0, 1e6])
+def test_temperatures_and_offsets(T):
+    """Nearly one-hot to flat; logits far from 0 (a common offset changes nothing)."""
+    x, ids = _logits((4,), 20000, torch.float32, 11)
+    x[1] += 5000.0
+    x[2] -= 70000.0
+    _check(x, ids, T, 4)
+    _check(x, x.argmax(-1), T, 4)
 
 
 @gpu
@@ -269,7 +283,7 @@ def test_streams_and_graphs():
 def test_refusals():
     x, ids = _logits((4,), 1000, torch.bfloat16, 10)
     for bad in (dict(top_n=33), dict(top_n=-1), dict(temperature=0.0), dict(temperature=-1.0),
-                dict(temperature=math.inf), dict(temperature=math.nan)):
+                dict(temperature=1e-7), dict(temperature=1e7), dict(temperature=math.inf), dict(temperature=math.nan)):
         with pytest.raises(L.SpecdecError):
             S.token_logprobs(x, ids, **bad)
     with pytest.raises(L.SpecdecError):
