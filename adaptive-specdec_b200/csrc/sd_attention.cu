@@ -703,13 +703,12 @@ constexpr int TC_N = 32;                 // query rows per kv head (padded)
 constexpr int TC_NST = 3;                // K/V ring stages
 constexpr int TC_THREADS = 192;
 constexpr int TC_MIN_SHARE = SPLIT_KEYS / TC_KEYS;
-static_assert(TC_MIN_SHARE == ATTN_MIN_SHARE, "the join knows the schedule");
 constexpr float TC_HEADROOM = 8.f;
 // Schedule cost of starting a (row, kv head) segment, in tiles: its Q,
 // first-tile max, epilogue and barriers take about as long as this many
 // tiles, so CTAs that cover many short rows get fewer tiles.  The schedule
 // lays these virtual tiles in front of each (row, kv head)'s real ones.
-constexpr int TC_OVH = ATTN_SEG_OVH;
+constexpr int TC_OVH = 6;
 constexpr uint32_t TC_TMEM_COLS = 128;   // S0, S1, O0, O1 (32 columns each)
 
 struct TcSmem {
@@ -754,15 +753,13 @@ __device__ __forceinline__ void tc_seg_init(TcSeg& g, const AttnParams& P, int b
   g.tt = t0;
   g.t1 = t1;
 }
-template <bool PFX>
 __device__ __forceinline__ void tc_seg_bounds(TcSeg& g, const AttnParams& P) {
   g.ncost = min(g.tb - g.off, g.t1 - g.tt);
   const int r0 = max(g.off, TC_OVH) - TC_OVH;          // real tiles: units past the virtual ones
   const int r1 = g.off + g.ncost - TC_OVH;
   g.nseg = max(r1 - r0, 0);
-  const int k0 = PFX ? P.rowstart[g.b] : 0;            // keys before it belong to the shared prefix
-  g.s0 = k0 + r0 * TC_KEYS;
-  g.s1 = min(P.rowkmax[g.b], k0 + r1 * TC_KEYS);
+  g.s0 = r0 * TC_KEYS;
+  g.s1 = min(P.rowkmax[g.b], r1 * TC_KEYS);
 }
 // advance past the current segment; false when the run is over
 __device__ __forceinline__ bool tc_seg_next(TcSeg& g, const AttnParams& P) {
@@ -777,21 +774,16 @@ __device__ __forceinline__ bool tc_seg_next(TcSeg& g, const AttnParams& P) {
   return true;
 }
 // the current or next segment that holds real tiles; false when none is left
-template <bool PFX>
 __device__ __forceinline__ bool tc_seg_real(TcSeg& g, const AttnParams& P) {
-  tc_seg_bounds<PFX>(g, P);
+  tc_seg_bounds(g, P);
   while (g.nseg == 0) {
     if (!tc_seg_next(g, P)) return false;
-    tc_seg_bounds<PFX>(g, P);
+    tc_seg_bounds(g, P);
   }
   return true;
 }
 
-// PFX: the rows' own keys behind a shared prefix (sd_prefix.cu).  Segments
-// start at P.rowstart[b], gridDim.y chunks of P.qc queries take their turn,
-// and every piece leaves its partial, base-2 maximum, in slot
-// (chunk, row * Hkv + head + CTA) for the join over prefix and row.
-template <int NTG, bool PFX>                          // NTG: 8-row groups of real query rows
+template <int NTG>                                    // 8-row groups of real query rows
 __global__ void __launch_bounds__(TC_THREADS, 1)
 attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap tmk,
                const __grid_constant__ CUtensorMap tmv) {
@@ -800,8 +792,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
   const uint32_t pad = (1024u - (smem_addr(tc_raw) & 1023u)) & 1023u;  // swizzle atoms: 1024 B
   TcSmem& S = *reinterpret_cast<TcSmem*>(tc_raw + pad);
   const int t = threadIdx.x, w = t >> 5, lane = t & 31;
-  const int j0 = PFX ? (int)blockIdx.y * P.qc : 0;
-  const int R = PFX ? min(P.qc, P.qlen - j0) * P.group : P.R, Hkv = P.Hkv;
+  const int R = P.R, Hkv = P.Hkv;
   const int total = P.rowpre[P.B] * Hkv;
   const int share = max(TC_MIN_SHARE, (total + (int)gridDim.x - 1) / (int)gridDim.x);
   const int t0 = (int)blockIdx.x * share;
@@ -844,7 +835,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
       uint32_t gi = 0;
       bool ok = true;
       do {
-        tc_seg_bounds<PFX>(g, P);
+        tc_seg_bounds(g, P);
         const int row0 = P.bt ? 0 : (g.b * Hkv + g.h) * P.C + g.s0;
         for (int i = 0; i < g.nseg && ok; ++i, ++gi) {
           const int st = (int)(gi % TC_NST);
@@ -880,15 +871,15 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
       uint32_t ntot = 0;                               // real tiles of the run
       {
         TcSeg gw = g;
-        bool more = tc_seg_real<PFX>(gw, P);
+        bool more = tc_seg_real(gw, P);
         while (more) {
           ntot += (uint32_t)gw.nseg;
-          more = tc_seg_next(gw, P) && tc_seg_real<PFX>(gw, P);
+          more = tc_seg_next(gw, P) && tc_seg_real(gw, P);
         }
       }
       TcSeg ga = g, gc = g;
-      tc_seg_real<PFX>(ga, P);
-      tc_seg_real<PFX>(gc, P);
+      tc_seg_real(ga, P);
+      tc_seg_real(gc, P);
       int ia = 0, ic = 0;
       uint32_t a = 0, c = 0, sa = 0, sc = 0;             // tiles and segments of the two heads
       long long idle0 = clock64();
@@ -917,7 +908,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
             if (++ia == ga.nseg) {
               ia = 0;
               ++sa;
-              if (tc_seg_next(ga, P)) tc_seg_real<PFX>(ga, P);
+              if (tc_seg_next(ga, P)) tc_seg_real(ga, P);
             }
             progressed = true;
           }
@@ -937,7 +928,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
             if (++ic == gc.nseg) {
               ic = 0;
               ++sc;
-              if (tc_seg_next(gc, P)) tc_seg_real<PFX>(gc, P);
+              if (tc_seg_next(gc, P)) tc_seg_real(gc, P);
             }
             progressed = true;
           }
@@ -973,7 +964,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
         const int r = i >> 4, c = i & 15;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (r < R) {
-          const int j = j0 + r / P.group, hq = qh * P.group + r % P.group;
+          const int j = r / P.group, hq = qh * P.group + r % P.group;
           v = *reinterpret_cast<const uint4*>(Qg + qb * P.qbs + hq * P.qhs + j * P.qqs + 8 * c);
         }
         *reinterpret_cast<uint4*>(S.q[qs & 1u][c >> 3] + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
@@ -983,7 +974,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
     };
     uint32_t gi = 0, seg = 0;
     bool run = true;
-    bool more = tc_seg_real<PFX>(g, P);
+    bool more = tc_seg_real(g, P);
     if (more) write_q(g.b, g.h, 0u);
     while (more) {
       const int b = g.b, h = g.h;
@@ -998,7 +989,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
       const int64_t capb = min(P.valid ? __ldg(P.valid + b) : (int64_t)P.C, (int64_t)P.C);
 #pragma unroll
       for (int r = 0; r < RN; ++r) {
-        const int64_t lj = min(lenb + j0 + r / P.group + 1, capb);
+        const int64_t lj = min(lenb + r / P.group + 1, capb);
         lim[r] = r < R ? (int)min(max(lj, (int64_t)0), (int64_t)g.s1) : 0;
         if (r < R) lim_min = min(lim_min, lim[r]);
         m[r] = -INFINITY;
@@ -1099,7 +1090,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
           // segment's GEMM1s) finished before this tile's S arrived, and the
           // global loads overlap this segment's tiles
           TcSeg gn = g;
-          if (tc_seg_next(gn, P) && tc_seg_real<PFX>(gn, P)) write_q(gn.b, gn.h, seg + 1u);
+          if (tc_seg_next(gn, P) && tc_seg_real(gn, P)) write_q(gn.b, gn.h, seg + 1u);
         }
       }
       if (!run) break;
@@ -1120,24 +1111,6 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
       }
       tc_sbar();
       const int bh = b * Hkv + h;
-      if (PFX) {
-        const int64_t base =
-            (((int64_t)blockIdx.y * P.slots + bh + blockIdx.x) * (P.qc * P.group)) * MT_D;
-#pragma unroll
-        for (int r = 0; r < RN; ++r) {
-          if (r >= R) continue;
-          const float L = (S.red[0][r] + S.red[1][r]) + (S.red[2][r] + S.red[3][r]);
-          P.part_acc[base + r * MT_D + t] = __uint_as_float(o[r]);
-          if (t == 0) {
-            P.part_ml[base / MT_D * 2 + 2 * r] = m[r];
-            P.part_ml[base / MT_D * 2 + 2 * r + 1] = L;
-          }
-        }
-        tc_sbar();                                     // S.red is reused next segment
-        ++seg;
-        more = tc_seg_next(g, P) && tc_seg_real<PFX>(g, P);
-        continue;
-      }
       const int Tb = P.rowpre[b] * Hkv + h * g.tb;     // first tile of this (row, kv head)
       const int cfirst = (Tb + TC_OVH) / share;         // CTAs holding its real tiles
       const int npieces = (Tb + g.tb - 1) / share - cfirst + 1;
@@ -1175,7 +1148,7 @@ attn_tc_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUt
       }
       tc_sbar();                                       // S.red and S.last reused next segment
       ++seg;
-      more = tc_seg_next(g, P) && tc_seg_real<PFX>(g, P);
+      more = tc_seg_next(g, P) && tc_seg_real(g, P);
     }
   }
   // ---------------- teardown: TMEM back once every role is done with it
@@ -1249,19 +1222,17 @@ bool cache_map(CUtensorMap* map, const void* base, int64_t rows) {
          CUDA_SUCCESS;
 }
 
-template <int NTG, bool PFX>
+template <int NTG>
 static int launch_tc_ntg(const AttnParams& P, const CUtensorMap& mk, const CUtensorMap& mv,
                          int nsm, cudaStream_t st) {
   const int sm = (int)sizeof(TcSmem) + 1024;         // + room to align to 1024 B
-  if (cudaFuncSetAttribute(attn_tc_kernel<NTG, PFX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  if (cudaFuncSetAttribute(attn_tc_kernel<NTG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            sm) != cudaSuccess)
     return SD_ELAUNCH;
-  const dim3 grid((unsigned)nsm, PFX ? (unsigned)((P.qlen + P.qc - 1) / P.qc) : 1u);
-  attn_tc_kernel<NTG, PFX><<<grid, TC_THREADS, sm, st>>>(P, mk, mv);
+  attn_tc_kernel<NTG><<<nsm, TC_THREADS, sm, st>>>(P, mk, mv);
   return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
 }
 
-template <bool PFX>
 static int launch_tc(const AttnParams& P, cudaStream_t st) {
   const int64_t rows = P.bt ? (int64_t)P.npages * P.Hkv * SD_KV_PAGE : (int64_t)P.B * P.Hkv * P.C;
   if (rows >= (int64_t)1 << 31) return SD_ENOTSUP;
@@ -1271,16 +1242,13 @@ static int launch_tc(const AttnParams& P, cudaStream_t st) {
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return SD_ELAUNCH;
-  if (PFX) nsm = P.ncta;
-  switch (((PFX ? P.qc * P.group : P.R) + 7) / 8) {
-    case 1: return launch_tc_ntg<1, PFX>(P, mk, mv, nsm, st);
-    case 2: return launch_tc_ntg<2, PFX>(P, mk, mv, nsm, st);
-    case 3: return launch_tc_ntg<3, PFX>(P, mk, mv, nsm, st);
-    default: return launch_tc_ntg<4, PFX>(P, mk, mv, nsm, st);
+  switch ((P.R + 7) / 8) {
+    case 1: return launch_tc_ntg<1>(P, mk, mv, nsm, st);
+    case 2: return launch_tc_ntg<2>(P, mk, mv, nsm, st);
+    case 3: return launch_tc_ntg<3>(P, mk, mv, nsm, st);
+    default: return launch_tc_ntg<4>(P, mk, mv, nsm, st);
   }
 }
-
-int launch_suffix(const AttnParams& P, cudaStream_t st) { return launch_tc<true>(P, st); }
 
 // Which kernel takes the tensor-core shapes: tcgen05 (default) or the
 // mma.sync kernel (SD_ATTN_KERNEL=mma, kept for comparison).
@@ -1358,7 +1326,7 @@ static int verify_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, con
     P.seg_ovh = TC_OVH;
     attn_plan_kernel<<<1, 1024, 0, st>>>(P);
     if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
-    return launch_tc<false>(P, st);
+    return launch_tc(P, st);
   }
   if (mma_ok) {
     P.nrc = 1;

@@ -9,9 +9,6 @@
 
 namespace sd {
 
-constexpr int ATTN_SEG_OVH = 6;     // schedule cost of a (row, kv head), in tiles (tcgen05 kernel)
-constexpr int ATTN_MIN_SHARE = 8;   // fewest tiles per CTA
-
 struct AttnParams {
   const void* q; int64_t qbs, qhs, qqs;
   const void* k; const void* v;
@@ -34,11 +31,6 @@ struct AttnParams {
   // contiguous [B, Hkv, C, D] layout
   const int32_t* bt;
   int bt_stride, npages;
-  // a row's own keys behind a shared prefix (tcgen05 kernel, PFX)
-  const int* rowstart;   // [B] first own key of each row, a page bound
-  int qc;                // queries per chunk (qc * group <= 32)
-  int slots;             // partial slots per chunk: B * Hkv + ncta
-  int ncta;              // CTAs per chunk
 };
 
 // Offset, in rows of D elements, of key s of row b and kv head h.  A page
@@ -59,9 +51,7 @@ __device__ __forceinline__ int row_limit(const AttnParams& P, int b, int j) {
 }
 
 // sd_attention.cu: a 2D tensor map over a cache viewed as [rows, 128] bf16
-// (boxes of 128 rows x 64 columns, 128-byte swizzle); the tcgen05 kernel over
-// the rows' own keys.
+// (boxes of 128 rows x 64 columns, 128-byte swizzle)
 bool cache_map(CUtensorMap* map, const void* base, int64_t rows);
-int launch_suffix(const AttnParams& P, cudaStream_t st);
 
 }  // namespace sd

@@ -12,7 +12,7 @@
 //   prefix_tc_kernel    the shared pages, query rows of the whole group on
 //                       the M side of tcgen05.mma: K and V are read once per
 //                       256 query rows instead of once per row;
-//   attn_tc_kernel      (sd_attention.cu, PFX) the rows' own pages;
+//   own_tc_kernel       the rows' own pages, four rows at a time;
 //   prefix_join_kernel  merges the partials, in piece order, into the output.
 // A row whose first query does not see the whole shared range (an empty or a
 // padding row, a short cap) takes no part in it: its own range starts at 0, so
@@ -36,6 +36,10 @@ constexpr int PX_OVH = 2;                    // schedule cost of an item beyond 
 constexpr int PX_MIN_SHARE = 4;              // fewest schedule units per CTA
 constexpr float PX_HEADROOM = 8.f;           // lazy-rescale headroom of the running max (base 2)
 constexpr int PX_JOIN_THREADS = 256;
+constexpr int OW_STAGES = 3;                 // K + V tiles in flight (own ranges)
+constexpr int OW_THREADS = 192;              // warps 0-3 softmax, 4 TMA, 5 MMA
+constexpr int OW_OVH = 2;                    // schedule cost of a (row, kv head) beyond its pages
+constexpr int OW_MIN_SHARE = 4;
 
 struct PrefixParams {
   AttnParams A;
@@ -49,6 +53,9 @@ struct PrefixParams {
   int* g_rows;                               // [G]
   int* g_pages;                              // [G] 0: the group shares nothing
   int* rowgroup;                             // [B] the row's group, -1: it takes no part
+  int* rowstart;                             // [B] first key of the row's own range, a page bound
+  int qc, nq;                                // queries per chunk; lane quarters of a chunk's rows
+  int slots;                                 // partial slots of a chunk of the own ranges
   float* pacc;                               // [slot][PX_ROWS][D]
   float* pml;                                // [slot][PX_ROWS][2]
 };
@@ -59,6 +66,10 @@ __device__ __forceinline__ int px_pairs(const PrefixParams& P, int g) {
 }
 __device__ __forceinline__ int px_share(int total) {
   return max(PX_MIN_SHARE, (total + PX_CTAS - 1) / PX_CTAS);
+}
+
+__device__ __forceinline__ int ow_share(int total) {
+  return max(OW_MIN_SHARE, (total + PX_CTAS - 1) / PX_CTAS);
 }
 
 __global__ void __launch_bounds__(1024) prefix_plan_kernel(const PrefixParams P) {
@@ -122,10 +133,10 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const PrefixParams P)
       }
       P.rowgroup[b] = start > 0 ? g : -1;
       const int km = row_limit(A, b, A.qlen - 1);
-      const_cast<int*>(A.rowstart)[b] = start;
+      P.rowstart[b] = start;
       A.rowkmax[b] = km;
       tiles = (max(km - start, 0) + SD_KV_PAGE - 1) / SD_KV_PAGE;
-      if (tiles > 0) tiles += ATTN_SEG_OVH;
+      if (tiles > 0) tiles += OW_OVH;
     }
     int sum;
     const int ex = block_excl_scan<int>(tiles, redi, &sum);
@@ -202,12 +213,6 @@ struct PxSmem {
   int abort_;
 };
 static_assert(sizeof(PxSmem) + 1024 <= 227 * 1024, "prefix attention shared memory");
-
-__device__ __forceinline__ void px_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, int acc) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-               :: "r"(d), "r"(a), "l"(b), "r"(id), "r"(acc) : "memory");
-}
 
 // What one tile's issue state walks: its segments, the page of the segment,
 // and the page's number in the CTA's run (the ring position).
@@ -357,7 +362,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
               const bool first = cp[x].i == (cp[x].s.dup ? x : 0);
 #pragma unroll
               for (int ks = 0; ks < 8; ++ks)
-                px_mma_ts(tm + 256u + 128u * x, tm + 128u * x + 8u * ks,
+                tc_mma_ts(tm + 256u + 128u * x, tm + 128u * x + 8u * ks,
                           tc_desc(va + ks * 2048, 16384, 1024, 2), ID2, (!first || ks > 0) ? 1 : 0);
               tc_commit(&S.oready[x]);
               if (cp[x].s.dup || (seen >> sl & 1u)) {
@@ -427,16 +432,24 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
         // Q of the tile's rows (b, query, head of the group) into the swizzled
         // K-major tile; rows past the group's are 0.  The last segment's S
         // reads of this buffer ended before its last P . V was waited for.
-        for (int i = r; i < 128 * 16; i += 128) {
-          const int rr = i >> 4, c = i & 15, f = base + rr;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        // (all of a thread's loads go out before the first store)
+        const int c = r & 15, row0 = P.g_row0[seg.g];
+        uint4 v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int f = base + (r >> 4) + 8 * i;
+          v[i] = make_uint4(0u, 0u, 0u, 0u);
           if (f < rows) {
             const int bl = f / A.R, f2 = f - bl * A.R, j = f2 / A.group;
             const int hq = seg.h * A.group + f2 - j * A.group;
-            v = *reinterpret_cast<const uint4*>(Qg + (int64_t)(P.g_row0[seg.g] + bl) * A.qbs +
-                                                hq * A.qhs + j * A.qqs + 8 * c);
+            v[i] = __ldg(reinterpret_cast<const uint4*>(Qg + (int64_t)(row0 + bl) * A.qbs +
+                                                        hq * A.qhs + j * A.qqs + 8 * c));
           }
-          *reinterpret_cast<uint4*>(S.q[x][c >> 3] + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int rr = (r >> 4) + 8 * i;
+          *reinterpret_cast<uint4*>(S.q[x][c >> 3] + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         tc_arrive(&S.qfull[x]);
@@ -538,6 +551,417 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
   if (t == 0 && S.abort_) atomicOr(A.status, 1);
 }
 
+// ---------------------------------------------------------------------------
+// The rows' own ranges
+// ---------------------------------------------------------------------------
+// A CTA's run of (row, kv head, page) units as segments, walked identically
+// by every role (row-major, kv head inner; OW_OVH virtual units in front of
+// each (row, kv head)'s pages).
+struct OwSeg {
+  int b, h, tb, off, tt, t1, ncost, n, s0, s1;       // n pages; keys [s0, s1)
+};
+__device__ __forceinline__ void ow_bounds(OwSeg& g, const PrefixParams& P) {
+  g.ncost = min(g.tb - g.off, g.t1 - g.tt);
+  const int r0 = max(g.off, OW_OVH) - OW_OVH, r1 = g.off + g.ncost - OW_OVH;
+  g.n = max(r1 - r0, 0);
+  const int k0 = P.rowstart[g.b];
+  g.s0 = k0 + r0 * SD_KV_PAGE;
+  g.s1 = min(P.A.rowkmax[g.b], k0 + r1 * SD_KV_PAGE);
+}
+__device__ __forceinline__ bool ow_next(OwSeg& g, const PrefixParams& P) {
+  const AttnParams& A = P.A;
+  g.tt += g.ncost;
+  if (g.tt >= g.t1) return false;
+  g.off = 0;
+  if (++g.h == A.Hkv) {
+    g.h = 0;
+    do { ++g.b; } while (A.rowpre[g.b + 1] == A.rowpre[g.b]);   // units remain, so a row follows
+    g.tb = A.rowpre[g.b + 1] - A.rowpre[g.b];
+  }
+  ow_bounds(g, P);
+  return true;
+}
+// The current or next segment with pages; false when none is left.
+__device__ __forceinline__ bool ow_real(OwSeg& g, const PrefixParams& P) {
+  while (g.n == 0)
+    if (!ow_next(g, P)) return false;
+  return true;
+}
+
+struct OwSmem {
+  alignas(1024) unsigned char k[OW_STAGES][2][128 * 128];    // [stage][64-col box][128 keys x 128 B]
+  alignas(1024) unsigned char v[OW_STAGES][2][128 * 128];
+  alignas(1024) unsigned char q[2][128 * 128];               // [64-col box][128 rows x 128 B]
+  alignas(8) unsigned long long full[OW_STAGES], empty[OW_STAGES];
+  // by stream and the stream's page parity (at most two phases of each are open)
+  alignas(8) unsigned long long sfull[4][2], pfull[4][2], oready[4][2], qfull[4], fin;
+  uint32_t tmem;
+  int seg_b;
+  int abort_;
+};
+static_assert(sizeof(OwSmem) + 1024 <= 227 * 1024, "own-range attention shared memory");
+
+// Stream-K over the pages of all (row, kv head) segments.  A segment has at
+// most 128 query rows and needs 1, 2 or 4 quarters of the 128 accumulator lanes
+// (P.nq): 4 / nq segments are in work at once, each on its own quarters, its own
+// warps and, by the lane masks of tcgen05.mma, its own part of every
+// accumulator.  Per page:
+//   S[lanes, 128 keys] = Q . K^T     (all lanes multiply, the segment's are written)
+//   thread = query row = lane: scores in registers, lazy reference maximum,
+//   p = 2^(s - m) as bf16 over the columns of S
+//   O[lanes, 128 d] += P . V
+// So a segment's start and end (Q, first maximum, partial out) overlap the
+// pages of the next one, no reduction crosses a thread, and K and V are read
+// once whatever the number of query rows.  The idle lanes cost tensor time that
+// is not the bound: 1024 cycles a page against about 2800 for its 64 KB from HBM.
+// K and V of a page share a stage; slots behind a row's live keys that TMA
+// brings in are zeroed in V before P . V reads them (they may hold NaN).
+__global__ void __launch_bounds__(OW_THREADS, 1)
+own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CUtensorMap tmk,
+              const __grid_constant__ CUtensorMap tmv) {
+  extern __shared__ __align__(1024) unsigned char px_raw[];
+  const uint32_t pad = (1024u - (smem_addr(px_raw) & 1023u)) & 1023u;   // swizzle atoms: 1024 B
+  OwSmem& S = *reinterpret_cast<OwSmem*>(px_raw + pad);
+  const AttnParams& A = P.A;
+  const int t = threadIdx.x, w = t >> 5, lane = t & 31;
+  const int total = A.rowpre[A.B] * A.Hkv;
+  const int share = ow_share(total);
+  const int t0 = (int)blockIdx.x * share;
+  if (t0 >= total) return;                           // no work for this CTA (uniform)
+  const int t1 = min(total, t0 + share);
+  const int j0 = (int)blockIdx.y * P.qc;             // the chunk's first query
+  const int R = min(P.qc, A.qlen - j0) * A.group;    // its query rows per kv head
+  const int nq = P.nq, ns = 4 / nq;                  // quarters per segment, streams
+  for (int b = t; b < A.B; b += OW_THREADS)
+    if (A.rowpre[b] * A.Hkv <= t0 && t0 < A.rowpre[b + 1] * A.Hkv) S.seg_b = b;
+  if (t == 0) {
+    for (int i = 0; i < OW_STAGES; ++i) {
+      tc_bar_init(&S.full[i], 1);
+      tc_bar_init(&S.empty[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      tc_bar_init(&S.qfull[i], 32 * nq);
+      for (int p = 0; p < 2; ++p) {
+        tc_bar_init(&S.sfull[i][p], 1);
+        tc_bar_init(&S.pfull[i][p], 32 * nq);
+        tc_bar_init(&S.oready[i][p], 1);
+      }
+    }
+    tc_bar_init(&S.fin, 1);
+    S.abort_ = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (w == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_addr(&S.tmem)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = S.tmem;                        // S0, S1 (128 columns each), O (128)
+  OwSeg seg;
+  seg.b = S.seg_b;
+  seg.tb = A.rowpre[seg.b + 1] - A.rowpre[seg.b];
+  seg.h = (t0 - A.rowpre[seg.b] * A.Hkv) / seg.tb;
+  seg.off = (t0 - A.rowpre[seg.b] * A.Hkv) % seg.tb;
+  seg.tt = t0;
+  seg.t1 = t1;
+  ow_bounds(seg, P);
+  bool more = ow_real(seg, P);
+
+  if (w == 4) {
+    // ---------------- TMA producer: pages in segment order
+    if (lane == 0) {
+      uint32_t gi = 0;
+      bool ok = true;
+      while (more && ok) {
+        for (int i = 0; i < seg.n && ok; ++i, ++gi) {
+          const int st = (int)(gi % OW_STAGES);
+          if (gi >= (uint32_t)OW_STAGES)
+            ok = tc_wait(&S.empty[st], ((gi / OW_STAGES) - 1) & 1u, &S.abort_);
+          if (!ok) break;
+          const int y = (int)kv_row(A, seg.b, seg.h, seg.s0 + i * SD_KV_PAGE);
+          tc_expect_tx(&S.full[st], 4u * 128u * 128u);
+          tc_tma_2d(S.k[st][0], &tmk, 0, y, &S.full[st]);
+          tc_tma_2d(S.k[st][1], &tmk, 64, y, &S.full[st]);
+          tc_tma_2d(S.v[st][0], &tmv, 0, y, &S.full[st]);
+          tc_tma_2d(S.v[st][1], &tmv, 64, y, &S.full[st]);
+        }
+        if (ok) more = ow_next(seg, P) && ow_real(seg, P);
+      }
+      if (!ok) {
+        // let the copies already issued land before the CTA leaves
+        for (uint32_t q = gi > (uint32_t)OW_STAGES ? gi - OW_STAGES : 0u; q < gi; ++q) {
+          int dummy = 0;
+          tc_wait(&S.full[q % OW_STAGES], (q / OW_STAGES) & 1u, &dummy);
+        }
+      }
+    }
+  } else if (w == 5) {
+    // ---------------- MMA issuer: S of page a and P . V of page c, each in page
+    // order, polled together; S(a) behind P . V(a - 2), whose P it overwrites
+    if (lane == 0) {
+      constexpr uint32_t ID1 = tc_idesc(128, 128, 0, 0);     // S = Q . K^T
+      constexpr uint32_t ID2 = tc_idesc(128, 128, 0, 1);     // O += P . V (V [key][d]: N-major)
+      OwSeg sa = seg, sc = seg;
+      bool ma = more, mc = more;
+      int ia = 0, ic = 0;                            // page of the segment
+      uint32_t a = 0, c = 0, ga = 0, gc = 0;         // pages and segments issued
+      uint32_t na[4] = {0u, 0u, 0u, 0u}, nc[4] = {0u, 0u, 0u, 0u};   // pages by stream
+      auto lanes = [&](uint32_t (&off)[4], uint32_t g) {
+        const int q0 = (int)(g % ns) * nq;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) off[i] = i >= q0 && i < q0 + nq ? 0u : 0xFFFFFFFFu;
+      };
+      auto count = [&](uint32_t (&n)[4], int s, bool step) -> uint32_t {
+        uint32_t v = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i == s) {
+            v = n[i];
+            if (step) ++n[i];
+          }
+        return v;
+      };
+      long long idle0 = clock64();
+      while (mc) {
+        bool progressed = false;
+        if (ma && a < c + 2) {
+          const int st = (int)(a % OW_STAGES), s = (int)(ga % ns);
+          if (tc_test(&S.full[st], (a / OW_STAGES) & 1u) &&
+              (ia != 0 || tc_test(&S.qfull[s], (ga / ns) & 1u))) {
+            tc_fence_after();
+            uint32_t off[4];
+            lanes(off, ga);
+            const uint32_t n = count(na, s, true);
+            const uint32_t k0 = smem_addr(S.k[st][0]), k1 = smem_addr(S.k[st][1]);
+            const uint32_t q0 = smem_addr(S.q[0]), q1 = smem_addr(S.q[1]);
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+              const uint32_t ko = (uint32_t)(ks & 3) * 32u;
+              tc_mma_lanes(tm + 128u * (a & 1u), tc_desc((ks < 4 ? q0 : q1) + ko, 16, 1024, 2),
+                           tc_desc((ks < 4 ? k0 : k1) + ko, 16, 1024, 2), ID1, off, ks > 0 ? 1 : 0);
+            }
+            tc_commit(&S.sfull[s][n & 1u]);
+            ++a;
+            if (++ia == sa.n) {
+              ia = 0;
+              ++ga;
+              ma = ow_next(sa, P) && ow_real(sa, P);
+            }
+            progressed = true;
+          }
+        }
+        if (c < a) {
+          const int st = (int)(c % OW_STAGES), s = (int)(gc % ns);
+          const uint32_t n = count(nc, s, false);
+          if (tc_test(&S.pfull[s][n & 1u], (n >> 1) & 1u)) {
+            tc_fence_after();
+            uint32_t off[4];
+            lanes(off, gc);
+            count(nc, s, true);
+            const uint32_t va = smem_addr(S.v[st][0]);
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+              tc_mma_ts_lanes(tm + 256u, tm + 128u * (c & 1u) + 8u * ks,
+                              tc_desc(va + ks * 2048, 16384, 1024, 2), ID2, off,
+                              (ic > 0 || ks > 0) ? 1 : 0);
+            tc_commit(&S.empty[st]);
+            tc_commit(&S.oready[s][n & 1u]);
+            ++c;
+            if (++ic == sc.n) {
+              ic = 0;
+              ++gc;
+              mc = ow_next(sc, P) && ow_real(sc, P);
+            }
+            progressed = true;
+          }
+        }
+        if (progressed) {
+          idle0 = clock64();
+        } else if (*reinterpret_cast<volatile int*>(&S.abort_) || clock64() - idle0 > TC_WAIT) {
+          *reinterpret_cast<volatile int*>(&S.abort_) = 1;
+          break;
+        }
+      }
+      // every MMA this thread issued has finished before the CTA leaves
+      tc_commit(&S.fin);
+      int dummy = 0;
+      tc_wait(&S.fin, 0u, &dummy);
+    }
+  } else {
+    // ---------------- softmax warps: lane quarter w, query row r of the chunk
+    const int s = w / nq, r = (w % nq) * 32 + lane;
+    const uint32_t lcol = tm + ((uint32_t)(32 * w) << 16), ocol = lcol + 256u;
+    const float sl2 = A.scale * 1.4426950408889634f;
+    const __nv_bfloat16* Qg = reinterpret_cast<const __nv_bfloat16*>(A.q);
+    // Q of the warp's 32 rows into the swizzled K-major tile; rows >= R are 0
+    auto write_q = [&](int b, int h) {
+      const int c = lane & 15;
+      uint4 v[16];                                   // all loads before the first store
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int f = (w % nq) * 32 + 2 * i + (lane >> 4);
+        v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (f < R) {
+          const int j = j0 + f / A.group, hq = h * A.group + f % A.group;
+          v[i] = __ldg(reinterpret_cast<const uint4*>(Qg + (int64_t)b * A.qbs + hq * A.qhs +
+                                                      j * A.qqs + 8 * c));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int rr = 32 * w + 2 * i + (lane >> 4);
+        *reinterpret_cast<uint4*>(S.q[c >> 3] + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_arrive(&S.qfull[s]);
+    };
+    uint32_t gi = 0, n = 0;                          // pages before; the stream's pages done
+    int g = 0;                                       // segment
+    // this stream's first segment
+    auto skip = [&]() {
+      while (more && g % ns != s) {
+        gi += (uint32_t)seg.n;
+        more = ow_next(seg, P) && ow_real(seg, P);
+        ++g;
+      }
+    };
+    skip();
+    if (more) write_q(seg.b, seg.h);
+    bool ok = true;
+    while (more) {
+      const OwSeg cur = seg;
+      const uint32_t g0 = gi;
+      // the stream's next segment
+      gi += (uint32_t)seg.n;
+      more = ow_next(seg, P) && ow_real(seg, P);
+      ++g;
+      skip();
+      // the row's live keys (an idle lane sees all: its result goes nowhere)
+      int lim = 0x7FFFFFFF;
+      if (r < R) lim = row_limit(A, cur.b, j0 + r / A.group);
+      float m = -CUDART_INF_F, l = 0.f;
+      for (int i = 0; i < cur.n; ++i, ++n) {
+        ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[s][n & 1u], (n >> 1) & 1u, &S.abort_));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t scol = lcol + 128u * ((g0 + (uint32_t)i) & 1u);
+        uint32_t sc[128];
+        TC_LD32((sc + 0), scol);
+        TC_LD32((sc + 32), scol + 32u);
+        TC_LD32((sc + 64), scol + 64u);
+        TC_LD32((sc + 96), scol + 96u);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        const int key0 = cur.s0 + i * SD_KV_PAGE;
+        if (!__all_sync(0xffffffffu, key0 + SD_KV_PAGE <= lim)) {
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            if (key0 + e >= lim) sc[e] = 0xFF800000u;          // -inf
+        }
+        float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+        for (int e = 0; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(sc[e]));
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+        const bool move = mt > m + PX_HEADROOM;
+        if (__any_sync(0xffffffffu, move)) {
+          const float mn = move ? mt : m;
+          const float alpha = move ? (m == -CUDART_INF_F ? 0.f : ex2f(m - mn)) : 1.f;
+          m = mn;
+          l *= alpha;
+          if (i > 0) {
+            // O holds this segment's earlier pages: the last P . V into it first
+            ok = __all_sync(0xffffffffu,
+                            tc_wait(&S.oready[s][(n - 1) & 1u], ((n - 1) >> 1) & 1u, &S.abort_));
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+              uint32_t o[32];
+              TC_LD32(o, ocol + 32u * q);
+              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              TC_ST32(ocol + 32u * q, o);
+            }
+          }
+        }
+        const float mc = fmaxf(m, -1e30f);           // 2^(-inf - mc) = 0
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float x = ex2f(fmaf(__uint_as_float(sc[64 * hf + 2 * e]), sl2, -mc));
+            const float y = ex2f(fmaf(__uint_as_float(sc[64 * hf + 2 * e + 1]), sl2, -mc));
+            ls[e & 3] += x + y;
+            pk[e] = pack_bf16(x, y);
+          }
+          TC_ST32(scol + 32u * hf, pk);
+        }
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        if (key0 + SD_KV_PAGE > cur.s1) {
+          // past the live window the page holds other slots: zero their V
+          const int st = (int)((g0 + (uint32_t)i) % OW_STAGES);
+          for (int kr = cur.s1 - key0 + r; kr < 128; kr += 32 * nq) {
+            uint4* v0 = reinterpret_cast<uint4*>(S.v[st][0] + kr * 128);
+            uint4* v1 = reinterpret_cast<uint4*>(S.v[st][1] + kr * 128);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              v0[q] = make_uint4(0u, 0u, 0u, 0u);
+              v1[q] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
+        tc_arrive(&S.pfull[s][n & 1u]);
+        // the segment's S are all done with Q: the next segment's may come
+        if (i == cur.n - 1 && more) write_q(seg.b, seg.h);
+      }
+      if (!ok) break;
+      // ---- the segment's partial: slot (chunk, row * Hkv + head + CTA)
+      ok = __all_sync(0xffffffffu,
+                      tc_wait(&S.oready[s][(n - 1) & 1u], ((n - 1) >> 1) & 1u, &S.abort_));
+      if (!ok) break;
+      tc_fence_after();
+      const int64_t at = ((int64_t)blockIdx.y * P.slots + cur.b * A.Hkv + cur.h + blockIdx.x) *
+                             (P.qc * A.group) + r;
+      float4* dst = reinterpret_cast<float4*>(A.part_acc + at * PX_D);
+#pragma unroll 1
+      for (int q = 0; q < 4; ++q) {
+        uint32_t o[32];
+        TC_LD32(o, ocol + 32u * q);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (r < R) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            dst[8 * q + e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                         __uint_as_float(o[4 * e + 2]),
+                                         __uint_as_float(o[4 * e + 3]));
+        }
+      }
+      tc_fence_before();
+      if (r < R) {
+        A.part_ml[at * 2] = m;
+        A.part_ml[at * 2 + 1] = l;
+      }
+    }
+  }
+  // ---------------- teardown: TMEM back once every role is done with it
+  tc_fence_before();
+  __syncthreads();
+  if (w == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
+                 :: "r"(tm), "r"(512u) : "memory");
+  }
+  if (t == 0 && S.abort_) atomicOr(A.status, 1);
+}
+
 // A warp per (row, query, head): the pieces of the shared range and of the
 // row's own range, in piece order.
 __global__ void __launch_bounds__(PX_JOIN_THREADS) prefix_join_kernel(const PrefixParams P) {
@@ -566,14 +990,13 @@ __global__ void __launch_bounds__(PX_JOIN_THREADS) prefix_join_kernel(const Pref
     at1 = ((int64_t)P.g_item[g] + it + c0) * PX_ROWS + f % PX_ROWS;
   }
   const int tb = A.rowpre[b + 1] - A.rowpre[b];
-  const int RC = A.qc * A.group;
+  const int RC = P.qc * A.group;
   if (tb > 0) {
-    const int total = A.rowpre[A.B] * A.Hkv;
-    const int share = max(ATTN_MIN_SHARE, (total + A.ncta - 1) / A.ncta);
+    const int share = ow_share(A.rowpre[A.B] * A.Hkv);
     const int u = A.rowpre[b] * A.Hkv + h * tb;
-    const int c0 = (u + ATTN_SEG_OVH) / share, c1 = (u + tb - 1) / share;
+    const int c0 = (u + OW_OVH) / share, c1 = (u + tb - 1) / share;
     n2 = c1 - c0 + 1;
-    at2 = ((int64_t)(j / A.qc) * A.slots + b * A.Hkv + h + c0) * RC + (j % A.qc) * A.group + gq;
+    at2 = ((int64_t)(j / P.qc) * P.slots + b * A.Hkv + h + c0) * RC + (j % P.qc) * A.group + gq;
   }
   const int np = n1 + n2;
   auto row_of = [&](int i) -> int64_t {
@@ -634,18 +1057,19 @@ __global__ void __launch_bounds__(PX_JOIN_THREADS) prefix_join_kernel(const Pref
 // by itself (its kernels are bound by their arithmetic, not by the bytes that
 // sharing saves).
 static bool px_fast(int dtype, int D, int group) {
-  return dtype == SD_DTYPE_BF16 && D == PX_D && group <= 32;
+  return dtype == SD_DTYPE_BF16 && D == PX_D && group <= 128;
 }
 
 struct PxLayout {
   size_t ints, acc, ml, sacc, sml, bytes;
-  int max_items, qc, chunks, slots;
+  int max_items, qc, nq, chunks, slots;
 };
 static PxLayout px_layout(int B, int G, int Hq, int Hkv, int qlen) {
   PxLayout L;
   const int group = Hq / Hkv, R = qlen * group;
   L.max_items = (int)std::min<int64_t>((int64_t)Hkv * ((int64_t)B * R / PX_ROWS + G), 1 << 28);
-  L.qc = std::min(qlen, 32 / group);
+  L.qc = std::min(qlen, 128 / group);
+  L.nq = L.qc * group <= 32 ? 1 : L.qc * group <= 64 ? 2 : 4;
   L.chunks = (qlen + L.qc - 1) / L.qc;
   L.slots = B * Hkv + PX_CTAS;
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
@@ -703,7 +1127,7 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   if (rows >= (int64_t)1 << 31) return SD_ENOTSUP;
   // the schedules count units in 32 bits
   const int64_t R = (int64_t)qlen * group;
-  if (R * B > 0x7FFFFFFF || (int64_t)B * Hkv * (bt_stride + ATTN_SEG_OVH) > 0x7FFFFFFF ||
+  if (R * B > 0x7FFFFFFF || (int64_t)B * Hkv * (bt_stride + OW_OVH) > 0x7FFFFFFF ||
       (int64_t)Hkv * (B * R / PX_ROWS + G) * (bt_stride + PX_OVH) > 0x7FFFFFFF)
     return SD_ENOTSUP;
   const PxLayout L = px_layout(B, G, Hq, Hkv, qlen);
@@ -720,8 +1144,7 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   A.out_vec4 = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && obs % 4 == 0 && oqs % 4 == 0 &&
                ohs % 4 == 0;
   A.bt = block_table; A.bt_stride = bt_stride; A.npages = npages;
-  A.tile_keys = SD_KV_PAGE; A.seg_ovh = ATTN_SEG_OVH;
-  A.qc = L.qc; A.slots = L.slots; A.ncta = PX_CTAS;
+  P.qc = L.qc; P.nq = L.nq; P.slots = L.slots;
   P.starts = group_starts; P.pages = prefix_pages; P.G = G; P.max_items = L.max_items;
   int* in = reinterpret_cast<int*>(ws + L.ints);
   P.g_unit = in; in += G + 1;
@@ -730,7 +1153,7 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   P.g_rows = in; in += G;
   P.g_pages = in; in += G;
   P.rowgroup = in; in += B;
-  A.rowstart = in; in += B;
+  P.rowstart = in; in += B;
   A.rowkmax = in; in += B;
   A.rowpre = in; in += B + 1;
   A.status = in;
@@ -741,9 +1164,11 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   CUtensorMap mk, mv;
   if (!cache_map(&mk, kpool, rows) || !cache_map(&mv, vpool, rows)) return SD_ENOTSUP;
-  const int sm = (int)sizeof(PxSmem) + 1024;         // + room to align to 1024 B
+  const int sm = (int)sizeof(PxSmem) + 1024, smo = (int)sizeof(OwSmem) + 1024;   // room to align
   if (cudaFuncSetAttribute(prefix_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) !=
-      cudaSuccess)
+          cudaSuccess ||
+      cudaFuncSetAttribute(own_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smo) !=
+          cudaSuccess)
     return SD_ELAUNCH;
   prefix_plan_kernel<<<1, 1024, 0, st>>>(P);
   if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
@@ -751,7 +1176,8 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
     prefix_tc_kernel<<<PX_CTAS, PX_THREADS, sm, st>>>(P, mk, mv);
     if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
   }
-  if (int rc = launch_suffix(A, st)) return rc;
+  own_tc_kernel<<<dim3(PX_CTAS, L.chunks), OW_THREADS, smo, st>>>(P, mk, mv);
+  if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
   const int64_t warps = (int64_t)B * qlen * Hq, per = PX_JOIN_THREADS / 32;
   prefix_join_kernel<<<(unsigned)((warps + per - 1) / per), PX_JOIN_THREADS, 0, st>>>(P);
   return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;

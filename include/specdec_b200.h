@@ -387,7 +387,7 @@ int sd_verify_attn_paged(const void* q, int64_t qbs, int64_t qhs, int64_t qqs,
  * query does not see the whole shared range (a short length or cap) is
  * computed from its own table alone.  Both arrays are device memory, so a
  * captured call follows them.
- * bf16 with D = 128 and Hq / Hkv <= 32 shares (q, kpool and vpool 16-byte
+ * bf16 with D = 128 and Hq / Hkv <= 128 shares (q, kpool and vpool 16-byte
  * aligned, q strides multiples of 8); other shapes of sd_verify_attn_paged
  * are computed row by row.  scale > 0.  The workspace must be 256-byte aligned
  * and, as a call writes all it reads, needs no initialisation.  If a bounded
