@@ -51,7 +51,7 @@ __device__ __forceinline__ int row_limit(const AttnParams& P, int b, int j) {
 }
 
 // sd_attention.cu: a 2D tensor map over a cache viewed as [rows, 128] bf16
-// (boxes of 128 rows x 64 columns, 128-byte swizzle)
-bool cache_map(CUtensorMap* map, const void* base, int64_t rows);
+// (boxes of box_rows rows x 64 columns, 128-byte swizzle)
+bool cache_map(CUtensorMap* map, const void* base, int64_t rows, int box_rows = SD_KV_PAGE);
 
 }  // namespace sd

@@ -8,7 +8,9 @@
 //   unnormalised output over range i,
 // the shared range is computed for all query rows of a group at once and each
 // row's own range by itself:
-//   prefix_plan_kernel  lays out the work of both from the device lengths;
+//   prefix_plan_kernel  lays out the work of both from the device lengths, and
+//                       copies the queries kv head by kv head, so that TMA
+//                       brings any run of a group's query rows;
 //   prefix_tc_kernel    the shared pages, query rows of the whole group on
 //                       the M side of tcgen05.mma: K and V are read once per
 //                       256 query rows instead of once per row;
@@ -30,7 +32,11 @@ namespace sd {
 constexpr int PX_D = 128;
 constexpr int PX_ROWS = 256;                 // query rows per item: two tiles of 128
 constexpr int PX_SLOTS = 4;                  // 32 KB K / V tiles in flight
-constexpr int PX_THREADS = 320;              // warps 0-3, 4-7: softmax of tile 0, 1; 8 TMA; 9 MMA
+constexpr int PX_THREADS = 384;              // warps 0-3, 4-7: softmax of tile 0, 1; 8 TMA; 9, 10 MMA
+constexpr int PX_REGS_SOFTMAX = 208;         // registers per thread of the softmax warps and of
+constexpr int PX_REGS_REST = 88;             // the others, out of 168 each at launch
+static_assert(2 * PX_REGS_SOFTMAX + PX_REGS_REST <= 3 * 168, "the split fits the launch");
+constexpr int PX_PLAN_THREADS = 1024;
 constexpr int PX_CTAS = 148;                 // one CTA per SM
 constexpr int PX_OVH = 2;                    // schedule cost of an item beyond its pages, in pages
 constexpr int PX_MIN_SHARE = 4;              // fewest schedule units per CTA
@@ -56,6 +62,7 @@ struct PrefixParams {
   int* rowstart;                             // [B] first key of the row's own range, a page bound
   int qc, nq;                                // queries per chunk; lane quarters of a chunk's rows
   int slots;                                 // partial slots of a chunk of the own ranges
+  uint4* qp;                                 // queries [Hkv][B][qlen][group][D]
   float* pacc;                               // [slot][PX_ROWS][D]
   float* pml;                                // [slot][PX_ROWS][2]
 };
@@ -72,7 +79,20 @@ __device__ __forceinline__ int ow_share(int total) {
   return max(OW_MIN_SHARE, (total + PX_CTAS - 1) / PX_CTAS);
 }
 
-__global__ void __launch_bounds__(1024) prefix_plan_kernel(const PrefixParams P) {
+// CTA 0 plans, the others pack: 16 threads copy a query row.
+__global__ void __launch_bounds__(PX_PLAN_THREADS) prefix_plan_kernel(const PrefixParams P) {
+  if (blockIdx.x > 0) {
+    const AttnParams& A = P.A;
+    const int64_t i = ((int64_t)(blockIdx.x - 1) * PX_PLAN_THREADS + threadIdx.x) >> 4;
+    if (i >= (int64_t)A.B * A.Hq * A.qlen) return;
+    const int c = threadIdx.x & 15;
+    const int hb = (int)(i / A.R), f = (int)(i - (int64_t)hb * A.R), h = hb / A.B, b = hb - h * A.B;
+    const int j = f / A.group, hq = h * A.group + f - j * A.group;
+    P.qp[i * 16 + c] = __ldg(reinterpret_cast<const uint4*>(
+                                 reinterpret_cast<const __nv_bfloat16*>(A.q) + b * A.qbs + hq * A.qhs +
+                                 j * A.qqs) + c);
+    return;
+  }
   __shared__ long long red[33];
   __shared__ int redi[33];
   const AttnParams& A = P.A;
@@ -151,7 +171,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const PrefixParams P)
 // every role.
 struct PxSeg {
   int g, h, p, np, tb, off, tt, t1, ncost, j0, j1;   // pages [j0, j1) of the segment
-  bool dup;                                          // one tile of rows: both halves work on it
+  bool dup;                                          // one tile of rows: both tiles work on it
 };
 __device__ __forceinline__ void px_item(PxSeg& s, const PrefixParams& P) {
   s.dup = P.g_rows[s.g] * P.A.R - s.p * PX_ROWS <= PX_ROWS / 2;
@@ -191,78 +211,40 @@ __device__ __forceinline__ bool px_next(PxSeg& s, const PrefixParams& P) {
   px_bounds(s);
   return true;
 }
-// Pages of a segment that tile x works on: all, or every second one.
-__device__ __forceinline__ int px_tasks(const PxSeg& s, int x) {
-  const int n = s.j1 - s.j0;
-  return s.dup ? (n + 1 - x) / 2 : n;
-}
-// The current or next segment with work for tile x; false when none is left.
-__device__ __forceinline__ bool px_work(PxSeg& s, const PrefixParams& P, int x) {
-  while (px_tasks(s, x) == 0)
-    if (!px_next(s, P)) return false;
-  return true;
-}
+// Half pages (64 keys) of a segment that each tile works on: all, or, of an item
+// that fills one tile only, tile 0 the first and tile 1 the second half of every
+// page, on the same rows.
+__device__ __forceinline__ int px_tasks(const PxSeg& s) { return (s.j1 - s.j0) << (s.dup ? 0 : 1); }
 
 struct PxSmem {
   alignas(1024) unsigned char q[2][2][128 * 128];            // [tile][64-col box][128 rows x 128 B]
   alignas(1024) unsigned char kv[PX_SLOTS][2][128 * 128];    // [slot][64-col box][128 keys x 128 B]
   alignas(8) unsigned long long full[PX_SLOTS], empty[PX_SLOTS];
-  alignas(8) unsigned long long qfull[2], sfull[2], pfull[2], oready[2], fin;
+  // by tile and parity of the half page (at most two phases of each are open)
+  alignas(8) unsigned long long sfull[2][2], pfull[2][2], oready[2][2], qfull[2], fin[2];
   uint32_t tmem;
   int seg_g;
   int abort_;
 };
 static_assert(sizeof(PxSmem) + 1024 <= 227 * 1024, "prefix attention shared memory");
 
-// What one tile's issue state walks: its segments, the page of the segment,
-// and the page's number in the CTA's run (the ring position).
-struct PxIssue {
-  PxSeg s;
-  int i;                                             // page of the segment (0-based)
-  uint32_t q;                                        // ring number of the segment's first page
-  uint32_t n, segs;                                  // tasks issued, segments with work before
-  bool more;
-};
-__device__ __forceinline__ void px_issue_seg(PxIssue& c, const PrefixParams& P, int x) {
-  // skip segments without work for this tile, counting their pages
-  while (px_tasks(c.s, x) == 0) {
-    c.q += (uint32_t)(c.s.j1 - c.s.j0);
-    if (!px_next(c.s, P)) {
-      c.more = false;
-      return;
-    }
-  }
-  c.i = c.s.dup ? x : 0;
-}
-__device__ __forceinline__ void px_issue_next(PxIssue& c, const PrefixParams& P, int x) {
-  c.i += c.s.dup ? 2 : 1;
-  ++c.n;
-  if (c.i < c.s.j1 - c.s.j0) return;
-  c.q += (uint32_t)(c.s.j1 - c.s.j0);
-  ++c.segs;
-  if (!px_next(c.s, P)) {
-    c.more = false;
-    return;
-  }
-  px_issue_seg(c, P, x);
-}
-
 // Persistent, stream-K: the (item, page) units lie end to end and each CTA
-// takes one contiguous run.  Per page and tile of 128 query rows:
-//   S[128 rows, 128 keys] = Q . K^T      (tcgen05.mma, operands in shared memory)
+// takes one contiguous run.  Per half page of 64 keys and tile of 128 query rows:
+//   S[128 rows, 64 keys] = Q . K^T       (tcgen05.mma, operands in shared memory)
 //   thread t of the tile's four softmax warps owns row t (TMEM lane t): its
-//   128 scores in registers, a lazy reference maximum (moved when a score
+//   64 scores in registers, a lazy reference maximum (moved when a score
 //   passes it by PX_HEADROOM), p = 2^(s - m) as bf16 back into the TMEM columns
 //   of S
 //   O[128 rows, 128 d] += P . V          (tcgen05.mma, A in TMEM)
-// TMEM: S0, S1, O0, O1 (128 columns each: all 512).  While one tile's softmax
-// runs, the tensor core works on the other tile.  P overwrites S, so S of a
-// tile's next page is issued behind P . V of this one; both run in issue order.
-// Two waits bound a tile: its scores (sfull) and, before O is touched, its
-// last P . V (oready).
+// TMEM holds S (two halves of 64 columns) and O (128) of both tiles: all 512
+// columns, so P has to lie over S.  Half pages let a tile's tensor work on one
+// half run under its softmax of the other: with whole pages (S 128 columns) both
+// tiles fell into step, softmax then tensor cores, at 5400 cycles a page against
+// 2048 of either.  S of half page h + 2 is issued behind P . V of h, whose P it
+// overwrites; both run in issue order.
 __global__ void __launch_bounds__(PX_THREADS, 1)
 prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CUtensorMap tmk,
-                 const __grid_constant__ CUtensorMap tmv) {
+                 const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmq) {
   extern __shared__ __align__(1024) unsigned char px_raw[];
   const uint32_t pad = (1024u - (smem_addr(px_raw) & 1023u)) & 1023u;   // swizzle atoms: 1024 B
   PxSmem& S = *reinterpret_cast<PxSmem*>(px_raw + pad);
@@ -278,15 +260,17 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
   if (t == 0) {
     for (int i = 0; i < PX_SLOTS; ++i) {
       tc_bar_init(&S.full[i], 1);
-      tc_bar_init(&S.empty[i], 1);
+      tc_bar_init(&S.empty[i], 2);                   // both tiles are done with it
     }
     for (int x = 0; x < 2; ++x) {
-      tc_bar_init(&S.qfull[x], 128);
-      tc_bar_init(&S.sfull[x], 1);
-      tc_bar_init(&S.pfull[x], 128);
-      tc_bar_init(&S.oready[x], 1);
+      tc_bar_init(&S.qfull[x], 1);
+      tc_bar_init(&S.fin[x], 1);
+      for (int p = 0; p < 2; ++p) {
+        tc_bar_init(&S.sfull[x][p], 1);
+        tc_bar_init(&S.pfull[x][p], 128);
+        tc_bar_init(&S.oready[x][p], 1);
+      }
     }
-    tc_bar_init(&S.fin, 1);
     S.abort_ = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -302,9 +286,10 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
   PxSeg seg;
   px_init(seg, P, S.seg_g, t0, t1);
 
-  if (w == 8) {
-    // ---------------- TMA producer: K then V of each page, PX_SLOTS tiles ahead
-    if (lane == 0) {
+  if (w >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(PX_REGS_REST));
+    if (w == 8 && lane == 0) {
+      // ---------------- TMA producer: K then V of each page, PX_SLOTS tiles ahead
       uint32_t idx = 0;
       bool ok = true;
       do {
@@ -313,16 +298,16 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
           int pg = __ldg(bt + j);
           if ((unsigned)pg >= (unsigned)A.npages) pg = 0;    // a wrong table reads page 0
           const int y = (int)(((int64_t)pg * A.Hkv + seg.h) * SD_KV_PAGE);
-#pragma unroll
+#pragma unroll 1
           for (int kv = 0; kv < 2; ++kv, ++idx) {
             const int sl = (int)(idx % PX_SLOTS);
             if (idx >= (uint32_t)PX_SLOTS)
               ok = tc_wait(&S.empty[sl], ((idx / PX_SLOTS) - 1) & 1u, &S.abort_);
             if (!ok) break;
             tc_expect_tx(&S.full[sl], 2u * 128u * 128u);
-            const void* tm_ = kv ? (const void*)&tmv : (const void*)&tmk;
-            tc_tma_2d(S.kv[sl][0], tm_, 0, y, &S.full[sl]);
-            tc_tma_2d(S.kv[sl][1], tm_, 64, y, &S.full[sl]);
+            const void* map = kv ? (const void*)&tmv : (const void*)&tmk;
+            tc_tma_2d(S.kv[sl][0], map, 0, y, &S.full[sl]);
+            tc_tma_2d(S.kv[sl][1], map, 64, y, &S.full[sl]);
           }
         }
       } while (ok && px_next(seg, P));
@@ -333,140 +318,130 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
           tc_wait(&S.full[q % PX_SLOTS], (q / PX_SLOTS) & 1u, &dummy);
         }
       }
-    }
-  } else if (w == 9) {
-    // ---------------- MMA issuer: per tile an S queue and a P . V queue, polled
-    if (lane == 0) {
-      constexpr uint32_t ID1 = tc_idesc(128, 128, 0, 0);     // S = Q . K^T
+    } else if ((w == 9 || w == 10) && lane == 0) {
+      // ---------------- MMA issuers, one per tile: S(0) S(1) | PV(h) S(h + 2) | ...
+      // The tensor queue holds a few MMAs, and between two bursts an issuer
+      // spends some 500 cycles on its waits and commits: two issuers fill each
+      // other's gaps.
+      const int x = w - 9;
+      constexpr uint32_t ID1 = tc_idesc(128, 64, 0, 0);      // S = Q . K^T
       constexpr uint32_t ID2 = tc_idesc(128, 128, 0, 1);     // O += P . V (V [key][d]: N-major)
-      PxIssue cs[2], cp[2];
+      const uint32_t kv0 = smem_addr(S.kv[0][0]), scol = tm + 128u * (uint32_t)x;
+      const uint64_t dq = tc_desc(smem_addr(S.q[x][0]), 16, 1024, 2);
+      uint32_t page = 0, qn = 0, n = 0;              // ring pages before; Q tiles, half pages done
+      bool ok = true, dup = false;
+      // K of ring page g is in slot 2 g, its V in slot 2 g + 1; task h of a
+      // segment is half `hf` of its page
+      auto issue_s = [&](int h) {
+        const uint32_t g = page + (uint32_t)(dup ? h : h >> 1), idx = 2u * g, sl = idx % PX_SLOTS;
+        const uint32_t hf = dup ? (uint32_t)x : (uint32_t)h & 1u, p = (n + (uint32_t)h) & 1u;
+        ok = ok && tc_wait(&S.full[sl], (idx / PX_SLOTS) & 1u, &S.abort_);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t dk = tc_desc(kv0 + sl * 32768u + hf * 8192u, 16, 1024, 2);
+        const uint32_t d = scol + 64u * p;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        cs[x].s = seg;
-        cs[x].q = cs[x].n = cs[x].segs = 0;
-        cs[x].more = true;
-        px_issue_seg(cs[x], P, x);
-        cp[x] = cs[x];
-      }
-      uint32_t seen = 0;                             // tiles read by one of two users, by slot
-      long long idle0 = clock64();
-      while (cp[0].more || cp[1].more) {
-        bool progressed = false;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (cp[x].more && cp[x].n < cs[x].n) {
-            const uint32_t idx = 2u * (cp[x].q + (uint32_t)cp[x].i) + 1u, sl = idx % PX_SLOTS;
-            if (tc_test(&S.pfull[x], cp[x].n & 1u) && tc_test(&S.full[sl], (idx / PX_SLOTS) & 1u)) {
-              tc_fence_after();
-              const uint32_t va = smem_addr(S.kv[sl][0]);
-              const bool first = cp[x].i == (cp[x].s.dup ? x : 0);
-#pragma unroll
-              for (int ks = 0; ks < 8; ++ks)
-                tc_mma_ts(tm + 256u + 128u * x, tm + 128u * x + 8u * ks,
-                          tc_desc(va + ks * 2048, 16384, 1024, 2), ID2, (!first || ks > 0) ? 1 : 0);
-              tc_commit(&S.oready[x]);
-              if (cp[x].s.dup || (seen >> sl & 1u)) {
-                seen &= ~(1u << sl);
-                tc_commit(&S.empty[sl]);
-              } else {
-                seen |= 1u << sl;
-              }
-              px_issue_next(cp[x], P, x);
-              progressed = true;
-            }
-          }
-          if (cs[x].more && cs[x].n == cp[x].n) {
-            const uint32_t idx = 2u * (cs[x].q + (uint32_t)cs[x].i), sl = idx % PX_SLOTS;
-            const bool first = cs[x].i == (cs[x].s.dup ? x : 0);
-            if (tc_test(&S.full[sl], (idx / PX_SLOTS) & 1u) &&
-                (!first || tc_test(&S.qfull[x], cs[x].segs & 1u))) {
-              tc_fence_after();
-              const uint32_t k0 = smem_addr(S.kv[sl][0]), k1 = smem_addr(S.kv[sl][1]);
-              const uint32_t q0 = smem_addr(S.q[x][0]), q1 = smem_addr(S.q[x][1]);
-#pragma unroll
-              for (int ks = 0; ks < 8; ++ks) {
-                const uint32_t ko = (uint32_t)(ks & 3) * 32u;
-                tc_mma(tm + 128u * x, tc_desc((ks < 4 ? q0 : q1) + ko, 16, 1024, 2),
-                       tc_desc((ks < 4 ? k0 : k1) + ko, 16, 1024, 2), ID1, ks > 0 ? 1 : 0);
-              }
-              tc_commit(&S.sfull[x]);
-              if (cs[x].s.dup || (seen >> sl & 1u)) {
-                seen &= ~(1u << sl);
-                tc_commit(&S.empty[sl]);
-              } else {
-                seen |= 1u << sl;
-              }
-              px_issue_next(cs[x], P, x);
-              progressed = true;
-            }
-          }
+        for (int ks = 0; ks < 8; ++ks) {             // 16 of 128 d: 32 B, the second box 16 KB on
+          const uint64_t o = (uint64_t)((ks & 3) * 2 + (ks >> 2) * 1024);
+          tc_mma(d, dq + o, dk + o, ID1, ks > 0 ? 1 : 0);
         }
-        if (progressed) {
-          idle0 = clock64();
-        } else if (*reinterpret_cast<volatile int*>(&S.abort_) || clock64() - idle0 > TC_WAIT) {
-          *reinterpret_cast<volatile int*>(&S.abort_) = 1;
-          break;
+        tc_commit(&S.sfull[x][p]);
+        if (dup || (h & 1)) tc_commit(&S.empty[sl]);
+      };
+      auto issue_pv = [&](int h) {
+        const uint32_t g = page + (uint32_t)(dup ? h : h >> 1), idx = 2u * g + 1u, sl = idx % PX_SLOTS;
+        const uint32_t hf = dup ? (uint32_t)x : (uint32_t)h & 1u, k = n + (uint32_t)h, p = k & 1u;
+        ok = ok && tc_wait(&S.full[sl], (idx / PX_SLOTS) & 1u, &S.abort_);
+        ok = ok && tc_wait(&S.pfull[x][p], (k >> 1) & 1u, &S.abort_);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t dv = tc_desc(kv0 + sl * 32768u + hf * 8192u, 16384, 1024, 2);
+        const uint32_t a = scol + 64u * p;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)               // 16 of 64 keys: 2 KB
+          tc_mma_ts(scol + 256u, a + 8u * ks, dv + (uint64_t)(ks * 128), ID2,
+                    h > 0 || ks > 0 ? 1 : 0);
+        tc_commit(&S.oready[x][p]);
+        if (dup || (h & 1)) tc_commit(&S.empty[sl]);
+      };
+      do {
+        const int tasks = px_tasks(seg);
+        dup = seg.dup;
+        if (tasks > 0) {
+          ok = ok && tc_wait(&S.qfull[x], qn & 1u, &S.abort_);
+          ++qn;
+          if (ok) issue_s(0);
+          if (ok && tasks > 1) issue_s(1);
         }
-      }
+#pragma unroll 1
+        for (int h = 0; h < tasks && ok; ++h) {
+          issue_pv(h);
+          if (h + 2 < tasks && ok) issue_s(h + 2);
+        }
+        page += (uint32_t)(seg.j1 - seg.j0);
+        n += (uint32_t)tasks;
+      } while (ok && px_next(seg, P));
       // every MMA this thread issued has finished before the CTA leaves
-      tc_commit(&S.fin);
+      tc_commit(&S.fin[x]);
       int dummy = 0;
-      tc_wait(&S.fin, 0u, &dummy);
+      tc_wait(&S.fin[x], 0u, &dummy);
     }
   } else {
     // ---------------- softmax warps of tile x: thread r owns query row r
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(PX_REGS_SOFTMAX));
     const int x = w >> 2, r = t & 127;
     const uint32_t lrow = (uint32_t)(32 * (w & 3)) << 16;
     const uint32_t scol = tm + lrow + 128u * x, ocol = scol + 256u;
     const float sl2 = A.scale * 1.4426950408889634f;
-    const __nv_bfloat16* Qg = reinterpret_cast<const __nv_bfloat16*>(A.q);
-    uint32_t n = 0;                                  // tasks done
-    bool more = true;
-    while (more) {
-      const int tasks = px_tasks(seg, x);
-      const int rows = P.g_rows[seg.g] * A.R;
-      const int base = seg.p * PX_ROWS + (seg.dup ? 0 : 128 * x);
-      float m = -CUDART_INF_F, l = 0.f;
-      bool ok = true;
-      if (tasks > 0) {
-        // Q of the tile's rows (b, query, head of the group) into the swizzled
-        // K-major tile; rows past the group's are 0.  The last segment's S
-        // reads of this buffer ended before its last P . V was waited for.
-        // (all of a thread's loads go out before the first store)
-        const int c = r & 15, row0 = P.g_row0[seg.g];
-        uint4 v[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int f = base + (r >> 4) + 8 * i;
-          v[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (f < rows) {
-            const int bl = f / A.R, f2 = f - bl * A.R, j = f2 / A.group;
-            const int hq = seg.h * A.group + f2 - j * A.group;
-            v[i] = __ldg(reinterpret_cast<const uint4*>(Qg + (int64_t)(row0 + bl) * A.qbs +
-                                                        hq * A.qhs + j * A.qqs + 8 * c));
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int rr = (r >> 4) + 8 * i;
-          *reinterpret_cast<uint4*>(S.q[x][c >> 3] + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        tc_arrive(&S.qfull[x]);
+    auto first_row = [&](const PxSeg& g) { return g.p * PX_ROWS + (g.dup ? 0 : 128 * x); };
+    // slot (item + CTA) of the segment's partial, this thread's row
+    auto slot_row = [&](const PxSeg& g) {
+      return ((int64_t)P.g_item[g.g] + g.h * g.np + g.p + blockIdx.x) * PX_ROWS + 128 * x + r;
+    };
+    // on to the next segment with pages
+    auto find = [&](PxSeg& g) {
+      while (px_tasks(g) == 0)
+        if (!px_next(g, P)) return false;
+      return true;
+    };
+    // the tile's 128 query rows (rows past the group's end compute what nobody reads)
+    auto load_q = [&](const PxSeg& g) {
+      if (r == 0) {
+        const int y = (g.h * A.B + P.g_row0[g.g]) * A.R + first_row(g);
+        tc_expect_tx(&S.qfull[x], 2u * 128u * 128u);
+        tc_tma_2d(S.q[x][0], &tmq, 0, y, &S.qfull[x]);
+        tc_tma_2d(S.q[x][1], &tmq, 64, y, &S.qfull[x]);
       }
+    };
+    uint32_t n = 0, qn = 0;                          // half pages done, Q tiles asked for
+    bool ok = true, more = find(seg);
+    if (more) {
+      load_q(seg);
+      ++qn;
+    }
+    while (more) {
+      const PxSeg cur = seg;
+      more = px_next(seg, P) && find(seg);
+      const int tasks = px_tasks(cur);
+      float m = -CUDART_INF_F, l = 0.f;
+#pragma unroll 1
       for (int i = 0; i < tasks; ++i, ++n) {
-        ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[x], n & 1u, &S.abort_));
+        const uint32_t p = n & 1u, sc = scol + 64u * p;
+        ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[x][p], (n >> 1) & 1u, &S.abort_));
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[128];
-        TC_LD32((s + 0), scol);
-        TC_LD32((s + 32), scol + 32u);
-        TC_LD32((s + 64), scol + 64u);
-        TC_LD32((s + 96), scol + 96u);
+        uint32_t s[64];
+        TC_LD32((s + 0), sc);
+        TC_LD32((s + 32), sc + 32u);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        // the segment's S are all done with Q: the next segment's may come
+        if (i == tasks - 1 && more) {
+          load_q(seg);
+          ++qn;
+        }
         float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-        for (int e = 0; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
+        for (int e = 0; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
         const bool move = mt > m + PX_HEADROOM;
         if (__any_sync(0xffffffffu, move)) {
@@ -475,8 +450,9 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
           m = mn;
           l *= alpha;
           if (i > 0) {
-            // O holds this segment's earlier pages: the last P . V into it first
-            ok = __all_sync(0xffffffffu, tc_wait(&S.oready[x], (n - 1) & 1u, &S.abort_));
+            // O holds this segment's earlier keys: the last P . V into it first
+            ok = __all_sync(0xffffffffu,
+                            tc_wait(&S.oready[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, &S.abort_));
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -492,52 +468,52 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
         }
         const float mc = fmaxf(m, -1e30f);           // 2^(-inf - mc) = 0
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t pk[32];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float a = ex2f(fmaf(__uint_as_float(s[64 * hf + 2 * e]), sl2, -mc));
-            const float b = ex2f(fmaf(__uint_as_float(s[64 * hf + 2 * e + 1]), sl2, -mc));
-            ls[e & 3] += a + b;
-            pk[e] = pack_bf16(a, b);
-          }
-          TC_ST32(scol + 32u * hf, pk);
+        for (int e = 0; e < 32; ++e) {
+          const float a = ex2f(fmaf(__uint_as_float(s[2 * e]), sl2, -mc));
+          const float b = ex2f(fmaf(__uint_as_float(s[2 * e + 1]), sl2, -mc));
+          ls[e & 3] += a + b;
+          pk[e] = pack_bf16(a, b);
         }
+        TC_ST32(sc, pk);
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
-        tc_arrive(&S.pfull[x]);
+        tc_arrive(&S.pfull[x][p]);
       }
       if (!ok) break;
-      if (seg.j1 > seg.j0) {
-        // ---- the segment's partial: slot (item + CTA) of the workspace
-        const int64_t slot = (int64_t)P.g_item[seg.g] + seg.h * seg.np + seg.p + blockIdx.x;
-        const int64_t at = slot * PX_ROWS + 128 * x + r;
-        if (tasks > 0) {
-          ok = __all_sync(0xffffffffu, tc_wait(&S.oready[x], (n - 1) & 1u, &S.abort_));
-          if (!ok) break;
-          tc_fence_after();
-          float4* dst = reinterpret_cast<float4*>(P.pacc + at * PX_D);
+      // ---- the segment's partial
+      ok = __all_sync(0xffffffffu,
+                      tc_wait(&S.oready[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, &S.abort_));
+      if (!ok) break;
+      tc_fence_after();
+      const int64_t at = slot_row(cur);
+      const bool live = first_row(cur) + r < P.g_rows[cur.g] * A.R;
+      float4* dst = reinterpret_cast<float4*>(P.pacc + at * PX_D);
 #pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
-            uint32_t o[32];
-            TC_LD32(o, ocol + 32u * q);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            if (base + r < rows) {
+      for (int q = 0; q < 4; ++q) {
+        uint32_t o[32];
+        TC_LD32(o, ocol + 32u * q);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (live) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                dst[8 * q + e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                             __uint_as_float(o[4 * e + 2]),
-                                             __uint_as_float(o[4 * e + 3]));
-            }
-          }
-          tc_fence_before();
+          for (int e = 0; e < 8; ++e)
+            dst[8 * q + e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                         __uint_as_float(o[4 * e + 2]),
+                                         __uint_as_float(o[4 * e + 3]));
         }
-        P.pml[at * 2] = m;
-        P.pml[at * 2 + 1] = l;
       }
-      more = px_next(seg, P);
+      tc_fence_before();
+      P.pml[at * 2] = m;
+      P.pml[at * 2 + 1] = l;
+    }
+    if (!ok && r == 0) {
+      // let the Q tiles asked for land before the CTA leaves
+      for (uint32_t q = qn > 1 ? qn - 2 : 0u; q < qn; ++q) {
+        int dummy = 0;
+        tc_wait(&S.qfull[x], q & 1u, &dummy);
+      }
     }
   }
   // ---------------- teardown: TMEM back once every role is done with it
@@ -618,7 +594,7 @@ static_assert(sizeof(OwSmem) + 1024 <= 227 * 1024, "own-range attention shared m
 // brings in are zeroed in V before P . V reads them (they may hold NaN).
 __global__ void __launch_bounds__(OW_THREADS, 1)
 own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CUtensorMap tmk,
-              const __grid_constant__ CUtensorMap tmv) {
+              const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmq) {
   extern __shared__ __align__(1024) unsigned char px_raw[];
   const uint32_t pad = (1024u - (smem_addr(px_raw) & 1023u)) & 1023u;   // swizzle atoms: 1024 B
   OwSmem& S = *reinterpret_cast<OwSmem*>(px_raw + pad);
@@ -640,7 +616,7 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
       tc_bar_init(&S.empty[i], 1);
     }
     for (int i = 0; i < 4; ++i) {
-      tc_bar_init(&S.qfull[i], 32 * nq);
+      tc_bar_init(&S.qfull[i], nq);
       for (int p = 0; p < 2; ++p) {
         tc_bar_init(&S.sfull[i][p], 1);
         tc_bar_init(&S.pfull[i][p], 32 * nq);
@@ -795,29 +771,16 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
     const int s = w / nq, r = (w % nq) * 32 + lane;
     const uint32_t lcol = tm + ((uint32_t)(32 * w) << 16), ocol = lcol + 256u;
     const float sl2 = A.scale * 1.4426950408889634f;
-    const __nv_bfloat16* Qg = reinterpret_cast<const __nv_bfloat16*>(A.q);
-    // Q of the warp's 32 rows into the swizzled K-major tile; rows >= R are 0
-    auto write_q = [&](int b, int h) {
-      const int c = lane & 15;
-      uint4 v[16];                                   // all loads before the first store
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int f = (w % nq) * 32 + 2 * i + (lane >> 4);
-        v[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (f < R) {
-          const int j = j0 + f / A.group, hq = h * A.group + f % A.group;
-          v[i] = __ldg(reinterpret_cast<const uint4*>(Qg + (int64_t)b * A.qbs + hq * A.qhs +
-                                                      j * A.qqs + 8 * c));
-        }
+    // the warp's 32 query rows (rows past the segment's compute what nobody reads)
+    auto load_q = [&](int b, int h) {
+      if (lane == 0) {
+        const int y = (h * A.B + b) * A.R + j0 * A.group + (w % nq) * 32;
+        tc_expect_tx(&S.qfull[s], 2u * 32u * 128u);
+        tc_tma_2d(S.q[0] + 32 * w * 128, &tmq, 0, y, &S.qfull[s]);
+        tc_tma_2d(S.q[1] + 32 * w * 128, &tmq, 64, y, &S.qfull[s]);
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int rr = 32 * w + 2 * i + (lane >> 4);
-        *reinterpret_cast<uint4*>(S.q[c >> 3] + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tc_arrive(&S.qfull[s]);
     };
+    uint32_t qn = 0;                                 // Q tiles asked for
     uint32_t gi = 0, n = 0;                          // pages before; the stream's pages done
     int g = 0;                                       // segment
     // this stream's first segment
@@ -829,7 +792,10 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
       }
     };
     skip();
-    if (more) write_q(seg.b, seg.h);
+    if (more) {
+      load_q(seg.b, seg.h);
+      ++qn;
+    }
     bool ok = true;
     while (more) {
       const OwSeg cur = seg;
@@ -854,6 +820,11 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
         TC_LD32((sc + 64), scol + 64u);
         TC_LD32((sc + 96), scol + 96u);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        // the segment's S are all done with Q: the next segment's may come
+        if (i == cur.n - 1 && more) {
+          load_q(seg.b, seg.h);
+          ++qn;
+        }
         const int key0 = cur.s0 + i * SD_KV_PAGE;
         if (!__all_sync(0xffffffffu, key0 + SD_KV_PAGE <= lim)) {
 #pragma unroll
@@ -919,8 +890,6 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         tc_arrive(&S.pfull[s][n & 1u]);
-        // the segment's S are all done with Q: the next segment's may come
-        if (i == cur.n - 1 && more) write_q(seg.b, seg.h);
       }
       if (!ok) break;
       // ---- the segment's partial: slot (chunk, row * Hkv + head + CTA)
@@ -948,6 +917,13 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
       if (r < R) {
         A.part_ml[at * 2] = m;
         A.part_ml[at * 2 + 1] = l;
+      }
+    }
+    if (!ok && lane == 0) {
+      // let the Q tiles asked for land before the CTA leaves
+      for (uint32_t q = qn > 1 ? qn - 2 : 0u; q < qn; ++q) {
+        int dummy = 0;
+        tc_wait(&S.qfull[s], q & 1u, &dummy);
       }
     }
   }
@@ -1061,7 +1037,7 @@ static bool px_fast(int dtype, int D, int group) {
 }
 
 struct PxLayout {
-  size_t ints, acc, ml, sacc, sml, bytes;
+  size_t ints, qp, acc, ml, sacc, sml, bytes;
   int max_items, qc, nq, chunks, slots;
 };
 static PxLayout px_layout(int B, int G, int Hq, int Hkv, int qlen) {
@@ -1077,6 +1053,7 @@ static PxLayout px_layout(int B, int G, int Hq, int Hkv, int qlen) {
   const size_t n2 = (size_t)L.chunks * L.slots * L.qc * group;
   size_t o = up((5 * (size_t)G + 2 + 4 * (size_t)B + 2) * sizeof(int));
   L.ints = 0;
+  L.qp = o; o = up(o + (size_t)B * Hq * qlen * PX_D * 2);
   L.acc = o; o = up(o + n1 * PX_D * sizeof(float));
   L.ml = o; o = up(o + n1 * 2 * sizeof(float));
   L.sacc = o; o = up(o + n2 * PX_D * sizeof(float));
@@ -1127,7 +1104,7 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   if (rows >= (int64_t)1 << 31) return SD_ENOTSUP;
   // the schedules count units in 32 bits
   const int64_t R = (int64_t)qlen * group;
-  if (R * B > 0x7FFFFFFF || (int64_t)B * Hkv * (bt_stride + OW_OVH) > 0x7FFFFFFF ||
+  if (R * B * Hkv > 0x7FFFFFFF || (int64_t)B * Hkv * (bt_stride + OW_OVH) > 0x7FFFFFFF ||
       (int64_t)Hkv * (B * R / PX_ROWS + G) * (bt_stride + PX_OVH) > 0x7FFFFFFF)
     return SD_ENOTSUP;
   const PxLayout L = px_layout(B, G, Hq, Hkv, qlen);
@@ -1157,26 +1134,31 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   A.rowkmax = in; in += B;
   A.rowpre = in; in += B + 1;
   A.status = in;
+  P.qp = reinterpret_cast<uint4*>(ws + L.qp);
   P.pacc = reinterpret_cast<float*>(ws + L.acc);
   P.pml = reinterpret_cast<float*>(ws + L.ml);
   A.part_acc = reinterpret_cast<float*>(ws + L.sacc);
   A.part_ml = reinterpret_cast<float*>(ws + L.sml);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  CUtensorMap mk, mv;
-  if (!cache_map(&mk, kpool, rows) || !cache_map(&mv, vpool, rows)) return SD_ENOTSUP;
+  const int64_t qrows = (int64_t)B * Hq * qlen;
+  CUtensorMap mk, mv, mq, mq32;
+  if (!cache_map(&mk, kpool, rows) || !cache_map(&mv, vpool, rows) ||
+      !cache_map(&mq, P.qp, qrows) || !cache_map(&mq32, P.qp, qrows, 32))
+    return SD_ENOTSUP;
   const int sm = (int)sizeof(PxSmem) + 1024, smo = (int)sizeof(OwSmem) + 1024;   // room to align
   if (cudaFuncSetAttribute(prefix_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) !=
           cudaSuccess ||
       cudaFuncSetAttribute(own_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smo) !=
           cudaSuccess)
     return SD_ELAUNCH;
-  prefix_plan_kernel<<<1, 1024, 0, st>>>(P);
+  const int64_t pack = (qrows * 16 + PX_PLAN_THREADS - 1) / PX_PLAN_THREADS;
+  prefix_plan_kernel<<<(unsigned)(1 + pack), PX_PLAN_THREADS, 0, st>>>(P);
   if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
   if (G > 0) {
-    prefix_tc_kernel<<<PX_CTAS, PX_THREADS, sm, st>>>(P, mk, mv);
+    prefix_tc_kernel<<<PX_CTAS, PX_THREADS, sm, st>>>(P, mk, mv, mq);
     if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
   }
-  own_tc_kernel<<<dim3(PX_CTAS, L.chunks), OW_THREADS, smo, st>>>(P, mk, mv);
+  own_tc_kernel<<<dim3(PX_CTAS, L.chunks), OW_THREADS, smo, st>>>(P, mk, mv, mq32);
   if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
   const int64_t warps = (int64_t)B * qlen * Hq, per = PX_JOIN_THREADS / 32;
   prefix_join_kernel<<<(unsigned)((warps + per - 1) / per), PX_JOIN_THREADS, 0, st>>>(P);

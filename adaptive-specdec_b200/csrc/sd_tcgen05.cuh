@@ -93,13 +93,14 @@ __device__ __forceinline__ bool tc_test(unsigned long long* bar, uint32_t par) {
 // Bounded wait for the phase of parity `par`; false (and the CTA's abort
 // flag set) on expiry or when another thread already gave up.
 __device__ __forceinline__ bool tc_wait(unsigned long long* bar, uint32_t par, int* abort_) {
-  const long long t0 = clock64();
+  long long t0 = 0;
   while (true) {
     uint32_t done;
     asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
                  " selp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(smem_addr(bar)), "r"(par)
                  : "memory");
     if (done) return true;
+    if (t0 == 0) t0 = clock64();                       // (a phase already there costs no clock read)
     if (*reinterpret_cast<volatile int*>(abort_) || clock64() - t0 > TC_WAIT) {
       *reinterpret_cast<volatile int*>(abort_) = 1;
       return false;
