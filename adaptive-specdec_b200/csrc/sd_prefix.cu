@@ -32,7 +32,7 @@ namespace sd {
 constexpr int PX_D = 128;
 constexpr int PX_ROWS = 256;                 // query rows per item: two tiles of 128
 constexpr int PX_SLOTS = 4;                  // 32 KB K / V tiles in flight
-constexpr int PX_THREADS = 384;              // warps 0-3, 4-7: softmax of tile 0, 1; 8 TMA; 9, 10 MMA
+constexpr int PX_THREADS = 384;              // warps 0-3, 4-7: softmax of tile 0, 1; 8 TMA; 9 MMA
 constexpr int PX_REGS_SOFTMAX = 208;         // registers per thread of the softmax warps and of
 constexpr int PX_REGS_REST = 88;             // the others, out of 168 each at launch
 static_assert(2 * PX_REGS_SOFTMAX + PX_REGS_REST <= 3 * 168, "the split fits the launch");
@@ -211,17 +211,12 @@ __device__ __forceinline__ bool px_next(PxSeg& s, const PrefixParams& P) {
   px_bounds(s);
   return true;
 }
-// Half pages (64 keys) of a segment that each tile works on: all, or, of an item
-// that fills one tile only, tile 0 the first and tile 1 the second half of every
-// page, on the same rows.
-__device__ __forceinline__ int px_tasks(const PxSeg& s) { return (s.j1 - s.j0) << (s.dup ? 0 : 1); }
-
 struct PxSmem {
   alignas(1024) unsigned char q[2][2][128 * 128];            // [tile][64-col box][128 rows x 128 B]
   alignas(1024) unsigned char kv[PX_SLOTS][2][128 * 128];    // [slot][64-col box][128 keys x 128 B]
   alignas(8) unsigned long long full[PX_SLOTS], empty[PX_SLOTS];
-  // by tile and parity of the half page (at most two phases of each are open)
-  alignas(8) unsigned long long sfull[2][2], pfull[2][2], oready[2][2], qfull[2], fin[2];
+  // by tile, P and O also by half of the page's keys
+  alignas(8) unsigned long long sfull[2], pfull[2][2], oready[2][2], qfull[2], fin;
   uint32_t tmem;
   int seg_g;
   int abort_;
@@ -229,19 +224,23 @@ struct PxSmem {
 static_assert(sizeof(PxSmem) + 1024 <= 227 * 1024, "prefix attention shared memory");
 
 // Persistent, stream-K: the (item, page) units lie end to end and each CTA
-// takes one contiguous run.  Per half page of 64 keys and tile of 128 query rows:
-//   S[128 rows, 64 keys] = Q . K^T       (tcgen05.mma, operands in shared memory)
-//   thread t of the tile's four softmax warps owns row t (TMEM lane t): its
-//   64 scores in registers, a lazy reference maximum (moved when a score
-//   passes it by PX_HEADROOM), p = 2^(s - m) as bf16 back into the TMEM columns
-//   of S
-//   O[128 rows, 128 d] += P . V          (tcgen05.mma, A in TMEM)
-// TMEM holds S (two halves of 64 columns) and O (128) of both tiles: all 512
-// columns, so P has to lie over S.  Half pages let a tile's tensor work on one
-// half run under its softmax of the other: with whole pages (S 128 columns) both
-// tiles fell into step, softmax then tensor cores, at 5400 cycles a page against
-// 2048 of either.  S of half page h + 2 is issued behind P . V of h, whose P it
-// overwrites; both run in issue order.
+// takes one contiguous run.  Per page of 128 keys and tile of 128 query rows:
+//   S[128 rows, 128 keys] = Q . K^T      (tcgen05.mma, operands in shared memory)
+//   thread t of the tile's four softmax warps owns row t (TMEM lane t); for
+//   each half of the keys its 64 scores in registers, a lazy reference maximum
+//   (moved when a score passes it by PX_HEADROOM), p = 2^(s - m) as bf16 back
+//   into the first 64 columns of S
+//   O[128 rows, 128 d] += P . V          (tcgen05.mma, A in TMEM, half by half)
+// TMEM holds S and O of both tiles, all 512 columns, so P has to lie over S, and
+// S of a tile's next page is issued behind P . V of this one (MMAs run in issue
+// order).  One issuer takes the tiles in turns, so that one tile's softmax runs
+// under the other's tensor work.  Measured on the way, cycles per page with both
+// tiles (2072 of them MMAs): one issuer on a single thread 4950 (an issue gap of
+// 500 cycles at every wait); two such issuers, one per tile, 5400 (the tiles fall
+// into step: softmax, then tensor cores); half pages with S of N = 64, 4170 (an
+// MMA of N = 64 takes as long as one of N = 128); this form PX_CYCLES.
+// An item with rows for one tile only is worked on by both: tile 0 takes the
+// first, tile 1 the second half of every page's keys.
 __global__ void __launch_bounds__(PX_THREADS, 1)
 prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CUtensorMap tmk,
                  const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmq) {
@@ -260,17 +259,17 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
   if (t == 0) {
     for (int i = 0; i < PX_SLOTS; ++i) {
       tc_bar_init(&S.full[i], 1);
-      tc_bar_init(&S.empty[i], 2);                   // both tiles are done with it
+      tc_bar_init(&S.empty[i], 1);
     }
     for (int x = 0; x < 2; ++x) {
       tc_bar_init(&S.qfull[x], 1);
-      tc_bar_init(&S.fin[x], 1);
-      for (int p = 0; p < 2; ++p) {
-        tc_bar_init(&S.sfull[x][p], 1);
-        tc_bar_init(&S.pfull[x][p], 128);
-        tc_bar_init(&S.oready[x][p], 1);
+      tc_bar_init(&S.sfull[x], 1);
+      for (int hf = 0; hf < 2; ++hf) {
+        tc_bar_init(&S.pfull[x][hf], 128);
+        tc_bar_init(&S.oready[x][hf], 1);
       }
     }
+    tc_bar_init(&S.fin, 1);
     S.abort_ = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -318,73 +317,74 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
           tc_wait(&S.full[q % PX_SLOTS], (q / PX_SLOTS) & 1u, &dummy);
         }
       }
-    } else if ((w == 9 || w == 10) && lane == 0) {
-      // ---------------- MMA issuers, one per tile: S(0) S(1) | PV(h) S(h + 2) | ...
-      // The tensor queue holds a few MMAs, and between two bursts an issuer
-      // spends some 500 cycles on its waits and commits: two issuers fill each
-      // other's gaps.
-      const int x = w - 9;
-      constexpr uint32_t ID1 = tc_idesc(128, 64, 0, 0);      // S = Q . K^T
+    } else if (w == 9) {
+      // ---------------- MMA issuer (the whole warp): S0(0) S1(0) | PV0(i) S0(i + 1)
+      // PV1(i) S1(i + 1) | ...
+      constexpr uint32_t ID1 = tc_idesc(128, 128, 0, 0);     // S = Q . K^T
+      constexpr uint32_t ID1H = tc_idesc(128, 64, 0, 0);     // of half a page
       constexpr uint32_t ID2 = tc_idesc(128, 128, 0, 1);     // O += P . V (V [key][d]: N-major)
-      const uint32_t kv0 = smem_addr(S.kv[0][0]), scol = tm + 128u * (uint32_t)x;
-      const uint64_t dq = tc_desc(smem_addr(S.q[x][0]), 16, 1024, 2);
-      uint32_t page = 0, qn = 0, n = 0;              // ring pages before; Q tiles, half pages done
+      const uint32_t kv0 = smem_addr(S.kv[0][0]), q0 = smem_addr(S.q[0][0]);
+      uint32_t page = 0;                             // ring number of the segment's first page
+      uint32_t qn = 0, pn[2] = {0u, 0u};             // segments; P tiles seen, by half
       bool ok = true, dup = false;
-      // K of ring page g is in slot 2 g, its V in slot 2 g + 1; task h of a
-      // segment is half `hf` of its page
-      auto issue_s = [&](int h) {
-        const uint32_t g = page + (uint32_t)(dup ? h : h >> 1), idx = 2u * g, sl = idx % PX_SLOTS;
-        const uint32_t hf = dup ? (uint32_t)x : (uint32_t)h & 1u, p = (n + (uint32_t)h) & 1u;
-        ok = ok && tc_wait(&S.full[sl], (idx / PX_SLOTS) & 1u, &S.abort_);
+      // K of ring page g is in slot 2 g, its V in slot 2 g + 1
+      auto issue_s = [&](int x, uint32_t i) {
+        const uint32_t idx = 2u * (page + i), sl = idx % PX_SLOTS;
+        ok = ok && tc_wait2_warp(&S.full[sl], (idx / PX_SLOTS) & 1u, &S.qfull[x], qn & 1u, &S.abort_);
         if (!ok) return;
         tc_fence_after();
-        const uint64_t dk = tc_desc(kv0 + sl * 32768u + hf * 8192u, 16, 1024, 2);
-        const uint32_t d = scol + 64u * p;
+        const uint64_t dq = tc_desc(q0 + (uint32_t)x * 32768u, 16, 1024, 2);
+        const uint64_t dk = tc_desc(kv0 + sl * 32768u + (dup ? (uint32_t)x * 8192u : 0u), 16, 1024, 2);
+        const uint32_t d = tm + 128u * (uint32_t)x, id = dup ? ID1H : ID1;
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {             // 16 of 128 d: 32 B, the second box 16 KB on
           const uint64_t o = (uint64_t)((ks & 3) * 2 + (ks >> 2) * 1024);
-          tc_mma(d, dq + o, dk + o, ID1, ks > 0 ? 1 : 0);
+          tc_mma_warp(d, dq + o, dk + o, id, ks > 0 ? 1 : 0);
         }
-        tc_commit(&S.sfull[x][p]);
-        if (dup || (h & 1)) tc_commit(&S.empty[sl]);
+        tc_commit_warp(&S.sfull[x]);
+        if (x == 1) tc_commit_warp(&S.empty[sl]);
       };
-      auto issue_pv = [&](int h) {
-        const uint32_t g = page + (uint32_t)(dup ? h : h >> 1), idx = 2u * g + 1u, sl = idx % PX_SLOTS;
-        const uint32_t hf = dup ? (uint32_t)x : (uint32_t)h & 1u, k = n + (uint32_t)h, p = k & 1u;
-        ok = ok && tc_wait(&S.full[sl], (idx / PX_SLOTS) & 1u, &S.abort_);
-        ok = ok && tc_wait(&S.pfull[x][p], (k >> 1) & 1u, &S.abort_);
+      auto issue_pv = [&](int x, uint32_t i, int hf, bool last) {
+        const uint32_t idx = 2u * (page + i) + 1u, sl = idx % PX_SLOTS;
+        ok = ok && tc_wait2_warp(&S.full[sl], (idx / PX_SLOTS) & 1u, &S.pfull[x][hf], pn[hf] & 1u,
+                                 &S.abort_);
         if (!ok) return;
         tc_fence_after();
-        const uint64_t dv = tc_desc(kv0 + sl * 32768u + hf * 8192u, 16384, 1024, 2);
-        const uint32_t a = scol + 64u * p;
+        const uint32_t key = dup ? (uint32_t)x * 8192u : (uint32_t)hf * 8192u;
+        const uint64_t dv = tc_desc(kv0 + sl * 32768u + key, 16384, 1024, 2);
+        const uint32_t d = tm + 256u + 128u * (uint32_t)x, a = tm + 128u * (uint32_t)x + 32u * (uint32_t)hf;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)               // 16 of 64 keys: 2 KB
-          tc_mma_ts(scol + 256u, a + 8u * ks, dv + (uint64_t)(ks * 128), ID2,
-                    h > 0 || ks > 0 ? 1 : 0);
-        tc_commit(&S.oready[x][p]);
-        if (dup || (h & 1)) tc_commit(&S.empty[sl]);
+          tc_mma_ts_warp(d, a + 8u * ks, dv + (uint64_t)(ks * 128), ID2,
+                         i > 0u || hf > 0 || ks > 0 ? 1 : 0);
+        tc_commit_warp(&S.oready[x][hf]);
+        if (x == 1 && last) tc_commit_warp(&S.empty[sl]);
       };
       do {
-        const int tasks = px_tasks(seg);
+        const uint32_t pages = (uint32_t)(seg.j1 - seg.j0);
         dup = seg.dup;
-        if (tasks > 0) {
-          ok = ok && tc_wait(&S.qfull[x], qn & 1u, &S.abort_);
-          ++qn;
-          if (ok) issue_s(0);
-          if (ok && tasks > 1) issue_s(1);
-        }
+        if (pages > 0) {
+          issue_s(0, 0u);
+          if (ok) issue_s(1, 0u);
 #pragma unroll 1
-        for (int h = 0; h < tasks && ok; ++h) {
-          issue_pv(h);
-          if (h + 2 < tasks && ok) issue_s(h + 2);
+          for (uint32_t i = 0; i < pages && ok; ++i) {
+#pragma unroll 1
+            for (int x = 0; x < 2 && ok; ++x) {
+              issue_pv(x, i, 0, dup);
+              if (!dup && ok) issue_pv(x, i, 1, true);
+              if (i + 1u < pages && ok) issue_s(x, i + 1u);
+            }
+            ++pn[0];
+            if (!dup) ++pn[1];
+          }
+          ++qn;
         }
-        page += (uint32_t)(seg.j1 - seg.j0);
-        n += (uint32_t)tasks;
+        page += pages;
       } while (ok && px_next(seg, P));
-      // every MMA this thread issued has finished before the CTA leaves
-      tc_commit(&S.fin[x]);
+      // every MMA this warp issued has finished before the CTA leaves
+      tc_commit_warp(&S.fin);
       int dummy = 0;
-      tc_wait(&S.fin[x], 0u, &dummy);
+      tc_wait(&S.fin, 0u, &dummy);
     }
   } else {
     // ---------------- softmax warps of tile x: thread r owns query row r
@@ -400,7 +400,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
     };
     // on to the next segment with pages
     auto find = [&](PxSeg& g) {
-      while (px_tasks(g) == 0)
+      while (g.j1 == g.j0)
         if (!px_next(g, P)) return false;
       return true;
     };
@@ -413,7 +413,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
         tc_tma_2d(S.q[x][1], &tmq, 64, y, &S.qfull[x]);
       }
     };
-    uint32_t n = 0, qn = 0;                          // half pages done, Q tiles asked for
+    uint32_t n = 0, on[2] = {0u, 0u}, qn = 0;        // pages; halves given to P . V; Q tiles asked for
     bool ok = true, more = find(seg);
     if (more) {
       load_q(seg);
@@ -422,20 +422,23 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
     while (more) {
       const PxSeg cur = seg;
       more = px_next(seg, P) && find(seg);
-      const int tasks = px_tasks(cur);
+      const int pages = cur.j1 - cur.j0, halves = cur.dup ? 1 : 2, steps = pages * halves;
       float m = -CUDART_INF_F, l = 0.f;
+      int hf = 0;
 #pragma unroll 1
-      for (int i = 0; i < tasks; ++i, ++n) {
-        const uint32_t p = n & 1u, sc = scol + 64u * p;
-        ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[x][p], (n >> 1) & 1u, &S.abort_));
-        if (!ok) break;
-        tc_fence_after();
+      for (int i = 0; i < steps; ++i) {
+        if (hf == 0) {
+          ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[x], n & 1u, &S.abort_));
+          if (!ok) break;
+          ++n;
+          tc_fence_after();
+        }
         uint32_t s[64];
-        TC_LD32((s + 0), sc);
-        TC_LD32((s + 32), sc + 32u);
+        TC_LD32((s + 0), scol + 64u * hf);
+        TC_LD32((s + 32), scol + 64u * hf + 32u);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         // the segment's S are all done with Q: the next segment's may come
-        if (i == tasks - 1 && more) {
+        if (i == steps - halves && more) {
           load_q(seg);
           ++qn;
         }
@@ -451,8 +454,9 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
           l *= alpha;
           if (i > 0) {
             // O holds this segment's earlier keys: the last P . V into it first
+            const int lh = halves - 1 - hf;          // its half of the keys
             ok = __all_sync(0xffffffffu,
-                            tc_wait(&S.oready[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, &S.abort_));
+                            tc_wait(&S.oready[x][lh], ((lh ? on[1] : on[0]) - 1u) & 1u, &S.abort_));
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -476,16 +480,19 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
           ls[e & 3] += a + b;
           pk[e] = pack_bf16(a, b);
         }
-        TC_ST32(sc, pk);
+        TC_ST32(scol + 32u * hf, pk);
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
-        tc_arrive(&S.pfull[x][p]);
+        tc_arrive(&S.pfull[x][hf]);
+        if (hf) ++on[1]; else ++on[0];
+        hf = hf + 1 == halves ? 0 : hf + 1;
       }
       if (!ok) break;
       // ---- the segment's partial
       ok = __all_sync(0xffffffffu,
-                      tc_wait(&S.oready[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, &S.abort_));
+                      tc_wait(&S.oready[x][halves - 1], ((halves > 1 ? on[1] : on[0]) - 1u) & 1u,
+                              &S.abort_));
       if (!ok) break;
       tc_fence_after();
       const int64_t at = slot_row(cur);

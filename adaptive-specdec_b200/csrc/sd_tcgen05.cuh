@@ -107,6 +107,48 @@ __device__ __forceinline__ bool tc_wait(unsigned long long* bar, uint32_t par, i
     }
   }
 }
+// Warp-wide issue: every lane calls, one elected lane issues, and control flow
+// stays uniform.  (Under `if (lane == 0)` the operands' way to the uniform
+// registers is set up again after every wait: some 200 cycles each, while the
+// tensor queue runs dry.)
+__device__ __forceinline__ void tc_mma_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                            int acc) {
+  asm volatile("{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+               :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(acc) : "memory");
+}
+// A in tensor memory
+__device__ __forceinline__ void tc_mma_ts_warp(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
+                                               int acc) {
+  asm volatile("{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+               :: "r"(d), "r"(a), "l"(b), "r"(id), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void tc_commit_warp(unsigned long long* bar) {
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+               " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}"
+               :: "r"(smem_addr(bar)) : "memory");
+}
+// tc_wait on two phases at once, by a whole warp.
+__device__ __forceinline__ bool tc_wait2_warp(unsigned long long* b0, uint32_t p0,
+                                              unsigned long long* b1, uint32_t p1, int* abort_) {
+  long long t0 = 0;
+  while (true) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p, q;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+                 " mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n"
+                 " and.pred p, p, q;\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done) : "r"(smem_addr(b0)), "r"(p0), "r"(smem_addr(b1)), "r"(p1)
+                 : "memory");
+    if (__all_sync(0xffffffffu, done != 0u)) return true;
+    if (t0 == 0) t0 = clock64();
+    const bool stop = *reinterpret_cast<volatile int*>(abort_) || clock64() - t0 > TC_WAIT;
+    if (__any_sync(0xffffffffu, stop)) {
+      *reinterpret_cast<volatile int*>(abort_) = 1;
+      return false;
+    }
+  }
+}
 __device__ __forceinline__ void tc_tma_2d(void* dst, const void* tmap, int x, int y,
                                           unsigned long long* bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
