@@ -31,17 +31,17 @@ namespace sd {
 
 constexpr int PX_D = 128;
 constexpr int PX_ROWS = 256;                 // query rows per item: two tiles of 128
-constexpr int PX_SLOTS = 4;                  // 32 KB K / V tiles in flight
-constexpr int PX_THREADS = 384;              // warps 0-3, 4-7: softmax of tile 0, 1; 8 TMA; 9 MMA
-constexpr int PX_REGS_SOFTMAX = 208;         // registers per thread of the softmax warps and of
-constexpr int PX_REGS_REST = 88;             // the others, out of 168 each at launch
-static_assert(2 * PX_REGS_SOFTMAX + PX_REGS_REST <= 3 * 168, "the split fits the launch");
+constexpr int PX_SLOTS = 4;                  // 32 KB K / V tiles in flight (two pages)
+constexpr int PX_THREADS = 320;              // warps 0-3, 4-7: softmax of tile 0, 1; 8 TMA; 9 MMA
 constexpr int PX_PLAN_THREADS = 1024;
 constexpr int PX_CTAS = 148;                 // one CTA per SM
 constexpr int PX_OVH = 2;                    // schedule cost of an item beyond its pages, in pages
 constexpr int PX_MIN_SHARE = 4;              // fewest schedule units per CTA
 constexpr float PX_HEADROOM = 8.f;           // lazy-rescale headroom of the running max (base 2)
 constexpr int PX_JOIN_THREADS = 256;
+#ifndef PX_POLY
+#define PX_POLY(e) ((e) % 4 == 1)
+#endif
 constexpr int OW_STAGES = 3;                 // K + V tiles in flight (own ranges)
 constexpr int OW_THREADS = 192;              // warps 0-3 softmax, 4 TMA, 5 MMA
 constexpr int OW_OVH = 2;                    // schedule cost of a (row, kv head) beyond its pages
@@ -63,7 +63,7 @@ struct PrefixParams {
   int qc, nq;                                // queries per chunk; lane quarters of a chunk's rows
   int slots;                                 // partial slots of a chunk of the own ranges
   uint4* qp;                                 // queries [Hkv][B][qlen][group][D]
-  float* pacc;                               // [slot][PX_ROWS][D]
+  float* pacc;                               // [slot][2 tiles][4 chunks][128 rows][32]
   float* pml;                                // [slot][PX_ROWS][2]
 };
 
@@ -215,22 +215,48 @@ struct PxSmem {
   alignas(1024) unsigned char q[2][2][128 * 128];            // [tile][64-col box][128 rows x 128 B]
   alignas(1024) unsigned char kv[PX_SLOTS][2][128 * 128];    // [slot][64-col box][128 keys x 128 B]
   alignas(8) unsigned long long full[PX_SLOTS], empty[PX_SLOTS];
-  // by tile, P and O also by half of the page's keys
-  alignas(8) unsigned long long sfull[2], pfull[2][2], oready[2][2], qfull[2], fin;
+  alignas(128) unsigned char out[8][32 * 128];               // a warp's 32 rows x 32 floats of O
+  alignas(8) unsigned long long sfull[2], pfull[2], oready[2], qfull[2], fin;
   uint32_t tmem;
   int seg_g;
   int abort_;
 };
 static_assert(sizeof(PxSmem) + 1024 <= 227 * 1024, "prefix attention shared memory");
 
+__device__ __forceinline__ void px_max3(float& m, uint32_t a, uint32_t b) {
+  asm("max.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+}
+
+// (2^a, 2^b) on the FMA pipe, held at 2^-126: with a = i + f, i the nearest
+// integer, 2^f by a polynomial of degree 4 on [-1/2, 1/2] (least relative error,
+// 2.7e-6) times 2^i, whose bits the rounding constant leaves in place.  A NaN
+// stays one.
+__device__ __forceinline__ unsigned long long px_exp2(float a, float b) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  const float magic = 12582912.f + 127.f;            // 1.5 * 2^23: the sum's low byte is i + 127
+  const unsigned long long x2 = pair2(a, b), r2 = add2(x2, pair2(magic, magic));
+  const unsigned long long i2 = add2(r2, pair2(-magic, -magic));
+  const unsigned long long f2 = fma2(i2, pair2(-1.f, -1.f), x2);
+  unsigned long long p2 = pair2(0.009570100344717503f, 0.009570100344717503f);
+  p2 = fma2(p2, f2, pair2(0.05591785907745361f, 0.05591785907745361f));
+  p2 = fma2(p2, f2, pair2(0.240247443318367f, 0.240247443318367f));
+  p2 = fma2(p2, f2, pair2(0.6931217908859253f, 0.6931217908859253f));
+  p2 = fma2(p2, f2, pair2(0.9999992847442627f, 0.9999992847442627f));
+  float ra, rb;
+  unpair(r2, ra, rb);
+  return mul2(p2, pair2(__uint_as_float(__float_as_uint(ra) << 23),
+                        __uint_as_float(__float_as_uint(rb) << 23)));
+}
+
 // Persistent, stream-K: the (item, page) units lie end to end and each CTA
 // takes one contiguous run.  Per page of 128 keys and tile of 128 query rows:
 //   S[128 rows, 128 keys] = Q . K^T      (tcgen05.mma, operands in shared memory)
-//   thread t of the tile's four softmax warps owns row t (TMEM lane t); for
-//   each half of the keys its 64 scores in registers, a lazy reference maximum
-//   (moved when a score passes it by PX_HEADROOM), p = 2^(s - m) as bf16 back
-//   into the first 64 columns of S
-//   O[128 rows, 128 d] += P . V          (tcgen05.mma, A in TMEM, half by half)
+//   thread t of the tile's four softmax warps owns row t (TMEM lane t): its
+//   128 scores in registers, a lazy reference maximum (moved when a score
+//   passes it by PX_HEADROOM), p = 2^(s - m) as bf16 back into the first 64
+//   columns of S
+//   O[128 rows, 128 d] += P . V          (tcgen05.mma, A in TMEM)
 // TMEM holds S and O of both tiles, all 512 columns, so P has to lie over S, and
 // S of a tile's next page is issued behind P . V of this one (MMAs run in issue
 // order).  One issuer takes the tiles in turns, so that one tile's softmax runs
@@ -264,10 +290,8 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
     for (int x = 0; x < 2; ++x) {
       tc_bar_init(&S.qfull[x], 1);
       tc_bar_init(&S.sfull[x], 1);
-      for (int hf = 0; hf < 2; ++hf) {
-        tc_bar_init(&S.pfull[x][hf], 128);
-        tc_bar_init(&S.oready[x][hf], 1);
-      }
+      tc_bar_init(&S.pfull[x], 128);
+      tc_bar_init(&S.oready[x], 1);
     }
     tc_bar_init(&S.fin, 1);
     S.abort_ = 0;
@@ -286,7 +310,6 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
   px_init(seg, P, S.seg_g, t0, t1);
 
   if (w >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(PX_REGS_REST));
     if (w == 8 && lane == 0) {
       // ---------------- TMA producer: K then V of each page, PX_SLOTS tiles ahead
       uint32_t idx = 0;
@@ -323,63 +346,58 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
       constexpr uint32_t ID1 = tc_idesc(128, 128, 0, 0);     // S = Q . K^T
       constexpr uint32_t ID1H = tc_idesc(128, 64, 0, 0);     // of half a page
       constexpr uint32_t ID2 = tc_idesc(128, 128, 0, 1);     // O += P . V (V [key][d]: N-major)
+      // One burst of each kind in the code: a kernel starts with cold
+      // instruction caches, and each new burst (by tile, ring position) costs its
+      // first execution more than the constants in it save later.
       const uint32_t kv0 = smem_addr(S.kv[0][0]), q0 = smem_addr(S.q[0][0]);
-      uint32_t page = 0;                             // ring number of the segment's first page
-      uint32_t qn = 0, pn[2] = {0u, 0u};             // segments; P tiles seen, by half
+      uint32_t qn = 0, g = 0;                        // segments, pages done
       bool ok = true, dup = false;
-      // K of ring page g is in slot 2 g, its V in slot 2 g + 1
-      auto issue_s = [&](int x, uint32_t i) {
-        const uint32_t idx = 2u * (page + i), sl = idx % PX_SLOTS;
-        ok = ok && tc_wait2_warp(&S.full[sl], (idx / PX_SLOTS) & 1u, &S.qfull[x], qn & 1u, &S.abort_);
+      // K of ring page g is in slot 2 (g & 1), its V in slot 2 (g & 1) + 1
+      auto issue_s = [&](uint32_t x, uint32_t ring) {
+        const uint32_t sl = 2u * (ring & 1u), d = tm + 128u * x, id = dup ? ID1H : ID1;
+        const uint64_t dq = tc_desc(q0 + x * 32768u, 16, 1024, 2);
+        const uint64_t dk = tc_desc(kv0 + sl * 32768u + (dup ? x * 8192u : 0u), 16, 1024, 2);
+        ok = tc_wait2_warp(&S.full[sl], (ring >> 1) & 1u, &S.qfull[x], qn & 1u, &S.abort_);
         if (!ok) return;
         tc_fence_after();
-        const uint64_t dq = tc_desc(q0 + (uint32_t)x * 32768u, 16, 1024, 2);
-        const uint64_t dk = tc_desc(kv0 + sl * 32768u + (dup ? (uint32_t)x * 8192u : 0u), 16, 1024, 2);
-        const uint32_t d = tm + 128u * (uint32_t)x, id = dup ? ID1H : ID1;
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {             // 16 of 128 d: 32 B, the second box 16 KB on
           const uint64_t o = (uint64_t)((ks & 3) * 2 + (ks >> 2) * 1024);
           tc_mma_warp(d, dq + o, dk + o, id, ks > 0 ? 1 : 0);
         }
         tc_commit_warp(&S.sfull[x]);
-        if (x == 1) tc_commit_warp(&S.empty[sl]);
+        if (x == 1u) tc_commit_warp(&S.empty[sl]);
       };
-      auto issue_pv = [&](int x, uint32_t i, int hf, bool last) {
-        const uint32_t idx = 2u * (page + i) + 1u, sl = idx % PX_SLOTS;
-        ok = ok && tc_wait2_warp(&S.full[sl], (idx / PX_SLOTS) & 1u, &S.pfull[x][hf], pn[hf] & 1u,
-                                 &S.abort_);
+      auto issue_pv = [&](uint32_t x, bool first) {
+        const uint32_t sl = 2u * (g & 1u) + 1u, a = tm + 128u * x;
+        const uint64_t dv = tc_desc(kv0 + sl * 32768u + (dup ? x * 8192u : 0u), 16384, 1024, 2);
+        ok = tc_wait2_warp(&S.full[sl], (g >> 1) & 1u, &S.pfull[x], g & 1u, &S.abort_);
         if (!ok) return;
         tc_fence_after();
-        const uint32_t key = dup ? (uint32_t)x * 8192u : (uint32_t)hf * 8192u;
-        const uint64_t dv = tc_desc(kv0 + sl * 32768u + key, 16384, 1024, 2);
-        const uint32_t d = tm + 256u + 128u * (uint32_t)x, a = tm + 128u * (uint32_t)x + 32u * (uint32_t)hf;
+        for (int k4 = 0; k4 < 8; k4 += 4) {          // 16 keys: 2 KB
+          if (k4 > 0 && dup) break;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)               // 16 of 64 keys: 2 KB
-          tc_mma_ts_warp(d, a + 8u * ks, dv + (uint64_t)(ks * 128), ID2,
-                         i > 0u || hf > 0 || ks > 0 ? 1 : 0);
-        tc_commit_warp(&S.oready[x][hf]);
-        if (x == 1 && last) tc_commit_warp(&S.empty[sl]);
+          for (int ks = k4; ks < k4 + 4; ++ks)
+            tc_mma_ts_warp(a + 256u, a + 8u * ks, dv + (uint64_t)(ks * 128), ID2, ks || !first ? 1 : 0);
+        }
+        tc_commit_warp(&S.oready[x]);
+        if (x == 1u) tc_commit_warp(&S.empty[sl]);
       };
       do {
-        const uint32_t pages = (uint32_t)(seg.j1 - seg.j0);
+        const int pages = seg.j1 - seg.j0;
         dup = seg.dup;
-        if (pages > 0) {
-          issue_s(0, 0u);
-          if (ok) issue_s(1, 0u);
+        if (pages == 0) continue;
+        // page i: P . V of a tile, then its S of page i + 1; i = -1: the first S
 #pragma unroll 1
-          for (uint32_t i = 0; i < pages && ok; ++i) {
+        for (int i = -1; i < pages && ok; ++i) {
 #pragma unroll 1
-            for (int x = 0; x < 2 && ok; ++x) {
-              issue_pv(x, i, 0, dup);
-              if (!dup && ok) issue_pv(x, i, 1, true);
-              if (i + 1u < pages && ok) issue_s(x, i + 1u);
-            }
-            ++pn[0];
-            if (!dup) ++pn[1];
+          for (uint32_t x = 0; x < 2u && ok; ++x) {
+            if (i >= 0) issue_pv(x, i == 0);
+            if (ok && i + 1 < pages) issue_s(x, i < 0 ? g : g + 1u);
           }
-          ++qn;
+          if (i >= 0) ++g;
         }
-        page += pages;
+        ++qn;
       } while (ok && px_next(seg, P));
       // every MMA this warp issued has finished before the CTA leaves
       tc_commit_warp(&S.fin);
@@ -388,7 +406,6 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
     }
   } else {
     // ---------------- softmax warps of tile x: thread r owns query row r
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(PX_REGS_SOFTMAX));
     const int x = w >> 2, r = t & 127;
     const uint32_t lrow = (uint32_t)(32 * (w & 3)) << 16;
     const uint32_t scol = tm + lrow + 128u * x, ocol = scol + 256u;
@@ -413,7 +430,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
         tc_tma_2d(S.q[x][1], &tmq, 64, y, &S.qfull[x]);
       }
     };
-    uint32_t n = 0, on[2] = {0u, 0u}, qn = 0;        // pages; halves given to P . V; Q tiles asked for
+    uint32_t n = 0, qn = 0;                          // pages done, Q tiles asked for
     bool ok = true, more = find(seg);
     if (more) {
       load_q(seg);
@@ -422,29 +439,34 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
     while (more) {
       const PxSeg cur = seg;
       more = px_next(seg, P) && find(seg);
-      const int pages = cur.j1 - cur.j0, halves = cur.dup ? 1 : 2, steps = pages * halves;
+      const int pages = cur.j1 - cur.j0, halves = cur.dup ? 1 : 2;
       float m = -CUDART_INF_F, l = 0.f;
-      int hf = 0;
 #pragma unroll 1
-      for (int i = 0; i < steps; ++i) {
-        if (hf == 0) {
-          ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[x], n & 1u, &S.abort_));
-          if (!ok) break;
-          ++n;
-          tc_fence_after();
+      for (int i = 0; i < pages; ++i) {
+        ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[x], n & 1u, &S.abort_));
+        if (!ok) break;
+        tc_fence_after();
+        // the scores twice from TMEM, 64 columns at a time: for the maximum, then
+        // for the exponentials (all 128 in registers made the loop bodies so long
+        // that their first, cold pass cost 4 us)
+        uint32_t sa[32], sb[32];
+        float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll 1
+        for (int c = 0; c < halves; ++c) {
+          TC_LD32(sa, scol + 64u * c);
+          TC_LD32(sb, scol + 64u * c + 32u);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            px_max3(mx[e & 2], sa[e], sa[e + 1]);
+            px_max3(mx[(e & 2) + 1], sb[e], sb[e + 1]);
+          }
         }
-        uint32_t s[64];
-        TC_LD32((s + 0), scol + 64u * hf);
-        TC_LD32((s + 32), scol + 64u * hf + 32u);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         // the segment's S are all done with Q: the next segment's may come
-        if (i == steps - halves && more) {
+        if (i == pages - 1 && more) {
           load_q(seg);
           ++qn;
         }
-        float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-        for (int e = 0; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
         const bool move = mt > m + PX_HEADROOM;
         if (__any_sync(0xffffffffu, move)) {
@@ -453,10 +475,8 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
           m = mn;
           l *= alpha;
           if (i > 0) {
-            // O holds this segment's earlier keys: the last P . V into it first
-            const int lh = halves - 1 - hf;          // its half of the keys
-            ok = __all_sync(0xffffffffu,
-                            tc_wait(&S.oready[x][lh], ((lh ? on[1] : on[0]) - 1u) & 1u, &S.abort_));
+            // O holds this segment's earlier pages: the last P . V into it first
+            ok = __all_sync(0xffffffffu, tc_wait(&S.oready[x], (n - 1) & 1u, &S.abort_));
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -471,50 +491,74 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
           }
         }
         const float mc = fmaxf(m, -1e30f);           // 2^(-inf - mc) = 0
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        const unsigned long long sl22 = pair2(sl2, sl2), nm2 = pair2(-mc, -mc);
+        unsigned long long ls[2] = {0ULL, 0ULL};     // (0.f, 0.f)
         uint32_t pk[32];
+        auto weights = [&](const uint32_t (&s)[32], uint32_t* p) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float a = ex2f(fmaf(__uint_as_float(s[2 * e]), sl2, -mc));
-          const float b = ex2f(fmaf(__uint_as_float(s[2 * e + 1]), sl2, -mc));
-          ls[e & 3] += a + b;
-          pk[e] = pack_bf16(a, b);
+          for (int e = 0; e < 16; ++e) {
+            float a, b;
+            unpair(fma2(pair2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sl22, nm2), a, b);
+            // a part by the FMA pipe: the exponentials of a page take 2048
+            // cycles of the special-function units otherwise
+            const unsigned long long p2 = PX_POLY(e) ? px_exp2(a, b) : pair2(ex2f(a), ex2f(b));
+            ls[e & 1] = add2(ls[e & 1], p2);
+            unpair(p2, a, b);
+            p[e] = pack_bf16(a, b);
+          }
+        };
+#pragma unroll 1
+        for (int c = 0; c < halves; ++c) {
+          TC_LD32(sa, scol + 64u * c);
+          TC_LD32(sb, scol + 64u * c + 32u);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          weights(sa, pk);
+          weights(sb, pk + 16);
+          TC_ST32(scol + 32u * c, pk);               // over columns that have been read
         }
-        TC_ST32(scol + 32u * hf, pk);
-        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
-        tc_arrive(&S.pfull[x][hf]);
-        if (hf) ++on[1]; else ++on[0];
-        hf = hf + 1 == halves ? 0 : hf + 1;
+        tc_arrive(&S.pfull[x]);
+        float la, lb;
+        unpair(add2(ls[0], ls[1]), la, lb);
+        l += la + lb;
+        ++n;
       }
       if (!ok) break;
-      // ---- the segment's partial
-      ok = __all_sync(0xffffffffu,
-                      tc_wait(&S.oready[x][halves - 1], ((halves > 1 ? on[1] : on[0]) - 1u) & 1u,
-                              &S.abort_));
+      // ---- the segment's partial: 32 columns of the warp's rows at a time to
+      // shared memory, and from there as one 4 KB bulk copy; in a row's 128 B
+      // the 16-byte chunks are permuted by the row (no bank conflicts)
+      ok = __all_sync(0xffffffffu, tc_wait(&S.oready[x], (n - 1) & 1u, &S.abort_));
       if (!ok) break;
       tc_fence_after();
       const int64_t at = slot_row(cur);
-      const bool live = first_row(cur) + r < P.g_rows[cur.g] * A.R;
-      float4* dst = reinterpret_cast<float4*>(P.pacc + at * PX_D);
+      unsigned char* stage = S.out[w];
 #pragma unroll 1
       for (int q = 0; q < 4; ++q) {
         uint32_t o[32];
         TC_LD32(o, ocol + 32u * q);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (live) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();                                // the last copy has read the buffer
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dst[8 * q + e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                         __uint_as_float(o[4 * e + 2]),
-                                         __uint_as_float(o[4 * e + 3]));
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+              make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          // [slot][tile][32-column chunk][128 rows][32 floats]
+          float* dst = P.pacc + ((at - r) * PX_D + (q * 128 + 32 * (w & 3)) * 32);
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                       :: "l"(dst), "r"(smem_addr(stage)), "r"(32u * 128u) : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
       }
       tc_fence_before();
       P.pml[at * 2] = m;
       P.pml[at * 2 + 1] = l;
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     if (!ok && r == 0) {
       // let the Q tiles asked for land before the CTA leaves
       for (uint32_t q = qn > 1 ? qn - 2 : 0u; q < qn; ++q) {
@@ -986,6 +1030,15 @@ __global__ void __launch_bounds__(PX_JOIN_THREADS) prefix_join_kernel(const Pref
     return i < n1 ? at1 + (int64_t)(i >> dup) * PX_ROWS + (dup & i) * (PX_ROWS / 2)
                   : at2 + (int64_t)(i - n1) * RC;
   };
+  // this lane's 4 columns of a partial row: in the shared range's tiles column
+  // chunk lane / 8, row, and the 16-byte chunk permuted by the row
+  auto acc_of = [&](int i) {
+    const int64_t row = row_of(i);
+    if (i >= n1) return reinterpret_cast<const float4*>(A.part_acc + row * PX_D) + lane;
+    const int tr = (int)(row & 127);
+    return reinterpret_cast<const float4*>(P.pacc + (row - tr) * PX_D) +
+           ((lane >> 3) * 128 + tr) * 8 + ((lane & 7) ^ (tr & 7));
+  };
   float m = -CUDART_INF_F, l = 0.f;                  // per lane, then over the warp
   bool nan = false;                                  // a NaN score leaves no maximum, but its sum
   for (int i = lane; i < np; i += 32) {
@@ -1013,8 +1066,7 @@ __global__ void __launch_bounds__(PX_JOIN_THREADS) prefix_join_kernel(const Pref
       const float fq = __shfl_sync(0xffffffffu, f, q);
       if (fq == 0.f) continue;                       // nothing there (maybe never written)
       const int k = i0 + q;
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(
-                                  (k < n1 ? P.pacc : A.part_acc) + row_of(k) * PX_D) + lane);
+      const float4 v = __ldcg(acc_of(k));
       a.x = fmaf(fq, v.x, a.x); a.y = fmaf(fq, v.y, a.y);
       a.z = fmaf(fq, v.z, a.z); a.w = fmaf(fq, v.w, a.w);
     }
