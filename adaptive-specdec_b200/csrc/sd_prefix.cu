@@ -36,7 +36,7 @@ constexpr int PX_THREADS = 320;              // warps 0-3, 4-7: softmax of tile 
 constexpr int PX_PLAN_THREADS = 1024;
 constexpr int PX_CTAS = 148;                 // one CTA per SM
 constexpr int PX_OVH = 2;                    // schedule cost of an item beyond its pages, in pages
-constexpr int PX_MIN_SHARE = 4;              // fewest schedule units per CTA
+constexpr int PX_MIN_SHARE = PX_OVH + 1;     // fewest schedule units per CTA: a one-page item
 constexpr float PX_HEADROOM = 8.f;           // lazy-rescale headroom of the running max (base 2)
 constexpr int PX_JOIN_THREADS = 256;
 #ifndef PX_POLY
@@ -45,7 +45,7 @@ constexpr int PX_JOIN_THREADS = 256;
 constexpr int OW_STAGES = 3;                 // K + V tiles in flight (own ranges)
 constexpr int OW_THREADS = 192;              // warps 0-3 softmax, 4 TMA, 5 MMA
 constexpr int OW_OVH = 2;                    // schedule cost of a (row, kv head) beyond its pages
-constexpr int OW_MIN_SHARE = 4;
+constexpr int OW_MIN_SHARE = OW_OVH + 1;
 
 struct PrefixParams {
   AttnParams A;
@@ -865,6 +865,31 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
         if (!ok) break;
         tc_fence_after();
         const uint32_t scol = lcol + 128u * ((g0 + (uint32_t)i) & 1u);
+        const int key0 = cur.s0 + i * SD_KV_PAGE;
+        if (key0 + SD_KV_PAGE > cur.s1 || !__all_sync(0xffffffffu, key0 + SD_KV_PAGE <= lim)) {
+          // The last pages: keys past a row's limit to -inf, in TMEM, 32 columns at
+          // a time (a short loop: this code is cold whenever it runs).
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const int k0 = key0 + 32 * c;
+            if (__all_sync(0xffffffffu, k0 + 32 <= lim)) continue;
+            uint32_t x[32];
+            TC_LD32(x, scol + 32u * c);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = k0 + e < lim ? x[e] : 0xFF800000u;
+            TC_ST32(scol + 32u * c, x);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          // past the live window the page holds other slots, maybe NaN: their V to
+          // zero, four rows of a 128-byte box at a time
+          const int st = (int)((g0 + (uint32_t)i) % OW_STAGES);
+          for (int kr = cur.s1 - key0 + 4 * (w % nq) + (lane >> 3); kr < 128; kr += 4 * nq) {
+            *reinterpret_cast<uint4*>(S.v[st][0] + kr * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(S.v[st][1] + kr * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
         uint32_t sc[128];
         TC_LD32((sc + 0), scol);
         TC_LD32((sc + 32), scol + 32u);
@@ -875,12 +900,6 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
         if (i == cur.n - 1 && more) {
           load_q(seg.b, seg.h);
           ++qn;
-        }
-        const int key0 = cur.s0 + i * SD_KV_PAGE;
-        if (!__all_sync(0xffffffffu, key0 + SD_KV_PAGE <= lim)) {
-#pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (key0 + e >= lim) sc[e] = 0xFF800000u;          // -inf
         }
         float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
@@ -924,20 +943,6 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
           TC_ST32(scol + 32u * hf, pk);
         }
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-        if (key0 + SD_KV_PAGE > cur.s1) {
-          // past the live window the page holds other slots: zero their V
-          const int st = (int)((g0 + (uint32_t)i) % OW_STAGES);
-          for (int kr = cur.s1 - key0 + r; kr < 128; kr += 32 * nq) {
-            uint4* v0 = reinterpret_cast<uint4*>(S.v[st][0] + kr * 128);
-            uint4* v1 = reinterpret_cast<uint4*>(S.v[st][1] + kr * 128);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              v0[q] = make_uint4(0u, 0u, 0u, 0u);
-              v1[q] = make_uint4(0u, 0u, 0u, 0u);
-            }
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         tc_arrive(&S.pfull[s][n & 1u]);
