@@ -81,6 +81,7 @@ __device__ __forceinline__ int ow_share(int total) {
 
 // CTA 0 plans, the others pack: 16 threads copy a query row.
 __global__ void __launch_bounds__(PX_PLAN_THREADS) prefix_plan_kernel(const PrefixParams P) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x > 0) {
     const AttnParams& A = P.A;
     const int64_t i = ((int64_t)(blockIdx.x - 1) * PX_PLAN_THREADS + threadIdx.x) >> 4;
@@ -275,13 +276,6 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
   PxSmem& S = *reinterpret_cast<PxSmem*>(px_raw + pad);
   const AttnParams& A = P.A;
   const int t = threadIdx.x, w = t >> 5, lane = t & 31;
-  const int total = P.g_unit[P.G];
-  const int share = px_share(total);
-  const int t0 = (int)blockIdx.x * share;
-  if (t0 >= total) return;                           // no work for this CTA (uniform)
-  const int t1 = min(total, t0 + share);
-  for (int g = t; g < P.G; g += PX_THREADS)
-    if (P.g_unit[g] <= t0 && t0 < P.g_unit[g + 1]) S.seg_g = g;
   if (t == 0) {
     for (int i = 0; i < PX_SLOTS; ++i) {
       tc_bar_init(&S.full[i], 1);
@@ -302,10 +296,25 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
                  :: "r"(smem_addr(&S.tmem)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // the plan and the packed queries from here on; the next kernel, which needs
+  // the plan only, may come up on SMs that run out of work
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int total = P.g_unit[P.G];
+  const int share = px_share(total);
+  const int t0 = (int)blockIdx.x * share, t1 = min(total, t0 + share);
+  for (int g = t; g < P.G; g += PX_THREADS)
+    if (P.g_unit[g] <= t0 && t0 < P.g_unit[g + 1]) S.seg_g = g;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = S.tmem;
+  if (t0 >= total) {                                 // no work for this CTA (uniform)
+    if (w == 0)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
+                   :: "r"(tm), "r"(512u) : "memory");
+    return;
+  }
   PxSeg seg;
   px_init(seg, P, S.seg_g, t0, t1);
 
@@ -651,10 +660,18 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
   OwSmem& S = *reinterpret_cast<OwSmem*>(px_raw + pad);
   const AttnParams& A = P.A;
   const int t = threadIdx.x, w = t >> 5, lane = t & 31;
+  // This kernel reads the plan, which was complete before the shared ranges'
+  // kernel let it start; it waits for that kernel only before it ends, so that
+  // its own end stands for both.
+  if (P.G == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int total = A.rowpre[A.B] * A.Hkv;
   const int share = ow_share(total);
   const int t0 = (int)blockIdx.x * share;
-  if (t0 >= total) return;                           // no work for this CTA (uniform)
+  if (t0 >= total) {                                 // no work for this CTA (uniform)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const int t1 = min(total, t0 + share);
   const int j0 = (int)blockIdx.y * P.qc;             // the chunk's first query
   const int R = min(P.qc, A.qlen - j0) * A.group;    // its query rows per kv head
@@ -992,104 +1009,119 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
                  :: "r"(tm), "r"(512u) : "memory");
   }
   if (t == 0 && S.abort_) atomicOr(A.status, 1);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// A warp per (row, query, head): the pieces of the shared range and of the
-// row's own range, in piece order.
+// A CTA per (row, kv head), a warp per query row: the pieces of the shared
+// range and of the row's own range, in piece order.
 __global__ void __launch_bounds__(PX_JOIN_THREADS) prefix_join_kernel(const PrefixParams P) {
   const AttnParams& A = P.A;
-  const int lane = threadIdx.x & 31;
-  const int64_t wid = (int64_t)blockIdx.x * (PX_JOIN_THREADS / 32) + (threadIdx.x >> 5);
-  if (wid >= (int64_t)A.B * A.qlen * A.Hq) return;
-  const int hq = (int)(wid % A.Hq);
-  const int j = (int)(wid / A.Hq % A.qlen);
-  const int b = (int)(wid / A.Hq / A.qlen);
-  const int h = hq / A.group, gq = hq - h * A.group;
-  // pieces [0, n1): the shared range, two per CTA where both halves worked on
-  // the rows; [n1, n1 + n2): the row's own range
-  int n1 = 0, n2 = 0;
-  int64_t at1 = 0, at2 = 0;                          // row of the first piece's partial
-  int dup = 0;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int b = (int)(blockIdx.x / A.Hkv), h = (int)(blockIdx.x - b * A.Hkv);
+  // what the plan says (complete before the kernel in front of this one began)
   const int g = P.rowgroup[b];
+  const int tb = A.rowpre[b + 1] - A.rowpre[b], RC = P.qc * A.group;
+  const int oshare = ow_share(A.rowpre[A.B] * A.Hkv), ou = A.rowpre[b] * A.Hkv + h * tb;
+  const int oc0 = (ou + OW_OVH) / oshare;
+  const int n2 = tb > 0 ? (ou + tb - 1) / oshare - oc0 + 1 : 0;
+  int rows = 0, f0 = 0, gtb = 0, gu = 0, gi = 0, gshare = 1;
   if (g >= 0) {
-    const int rows = P.g_rows[g] * A.R, np = (rows + PX_ROWS - 1) / PX_ROWS;
-    const int f = ((b - P.g_row0[g]) * A.qlen + j) * A.group + gq, p = f / PX_ROWS;
-    const int tb = P.g_pages[g] + PX_OVH, it = h * np + p;
-    const int u = P.g_unit[g] + it * tb, share = px_share(P.g_unit[P.G]);
-    const int c0 = (u + PX_OVH) / share, c1 = (u + tb - 1) / share;
-    dup = rows - p * PX_ROWS <= PX_ROWS / 2;
-    n1 = (c1 - c0 + 1) << dup;
-    at1 = ((int64_t)P.g_item[g] + it + c0) * PX_ROWS + f % PX_ROWS;
+    rows = P.g_rows[g] * A.R;
+    f0 = (b - P.g_row0[g]) * A.R;
+    gtb = P.g_pages[g] + PX_OVH;
+    const int np = (rows + PX_ROWS - 1) / PX_ROWS;
+    gu = P.g_unit[g] + h * np * gtb;
+    gi = P.g_item[g] + h * np;
+    gshare = px_share(P.g_unit[P.G]);
   }
-  const int tb = A.rowpre[b + 1] - A.rowpre[b];
-  const int RC = P.qc * A.group;
-  if (tb > 0) {
-    const int share = ow_share(A.rowpre[A.B] * A.Hkv);
-    const int u = A.rowpre[b] * A.Hkv + h * tb;
-    const int c0 = (u + OW_OVH) / share, c1 = (u + tb - 1) / share;
-    n2 = c1 - c0 + 1;
-    at2 = ((int64_t)(j / P.qc) * P.slots + b * A.Hkv + h + c0) * RC + (j % P.qc) * A.group + gq;
-  }
-  const int np = n1 + n2;
-  auto row_of = [&](int i) -> int64_t {
-    return i < n1 ? at1 + (int64_t)(i >> dup) * PX_ROWS + (dup & i) * (PX_ROWS / 2)
-                  : at2 + (int64_t)(i - n1) * RC;
-  };
-  // this lane's 4 columns of a partial row: in the shared range's tiles column
-  // chunk lane / 8, row, and the 16-byte chunk permuted by the row
-  auto acc_of = [&](int i) {
-    const int64_t row = row_of(i);
-    if (i >= n1) return reinterpret_cast<const float4*>(A.part_acc + row * PX_D) + lane;
-    const int tr = (int)(row & 127);
-    return reinterpret_cast<const float4*>(P.pacc + (row - tr) * PX_D) +
-           ((lane >> 3) * 128 + tr) * 8 + ((lane & 7) ^ (tr & 7));
-  };
-  float m = -CUDART_INF_F, l = 0.f;                  // per lane, then over the warp
-  bool nan = false;                                  // a NaN score leaves no maximum, but its sum
-  for (int i = lane; i < np; i += 32) {
-    const float* ml = (i < n1 ? P.pml : A.part_ml) + row_of(i) * 2;
-    const float mi = __ldcg(ml), li = __ldcg(ml + 1);
-    nan |= li != li;
-    if (mi != -CUDART_INF_F) {
-      const float mn = fmaxf(m, mi);
-      l = (m == -CUDART_INF_F ? 0.f : l * ex2f(m - mn)) + li * ex2f(mi - mn);
-      m = mn;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int status = *A.status;
+  for (int r = w; r < A.R; r += PX_JOIN_THREADS / 32) {
+    const int j = r / A.group, hq = h * A.group + r - j * A.group;
+    // pieces [0, n1): the shared range, two per CTA where both tiles worked on
+    // the rows; [n1, n1 + n2): the row's own range
+    int n1 = 0, dup = 0;
+    int64_t at1 = 0;                                 // row of the first piece's partial
+    if (g >= 0) {
+      const int f = f0 + r, p = f / PX_ROWS, u = gu + p * gtb;
+      const int c0 = (u + PX_OVH) / gshare;
+      dup = rows - p * PX_ROWS <= PX_ROWS / 2;
+      n1 = ((u + gtb - 1) / gshare - c0 + 1) << dup;
+      at1 = ((int64_t)gi + p + c0) * PX_ROWS + f % PX_ROWS;
     }
-  }
-  const float gm = warp_max(m);
-  const float L = warp_sum(m == -CUDART_INF_F ? 0.f : l * ex2f(m - gm));
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < np; i0 += 32) {
-    const int i = i0 + lane;
-    float f = 0.f;
-    if (i < np) {
-      const float mi = __ldcg((i < n1 ? P.pml : A.part_ml) + row_of(i) * 2);
-      f = mi == -CUDART_INF_F ? 0.f : ex2f(mi - gm);
+    const int jc = j / P.qc;
+    const int64_t at2 = ((int64_t)jc * P.slots + b * A.Hkv + h + oc0) * RC + r - jc * RC;
+    const int np = n1 + n2;
+    auto row_of = [&](int i) -> int64_t {
+      return i < n1 ? at1 + (int64_t)(i >> dup) * PX_ROWS + (dup & i) * (PX_ROWS / 2)
+                    : at2 + (int64_t)(i - n1) * RC;
+    };
+    // this lane's 4 columns of a partial row: in the shared range's tiles column
+    // chunk lane / 8, row, and the 16-byte chunk permuted by the row
+    auto acc_of = [&](int i) {
+      const int64_t row = row_of(i);
+      if (i >= n1) return reinterpret_cast<const float4*>(A.part_acc + row * PX_D) + lane;
+      const int tr = (int)(row & 127);
+      return reinterpret_cast<const float4*>(P.pacc + (row - tr) * PX_D) +
+             ((lane >> 3) * 128 + tr) * 8 + ((lane & 7) ^ (tr & 7));
+    };
+    // the first pieces' columns on their way before their weights are known
+    float4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = i < np ? __ldcg(acc_of(i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -CUDART_INF_F, l = 0.f, m0 = -CUDART_INF_F;      // per lane, then over the warp
+    bool nan = false;                                // a NaN score leaves no maximum, but its sum
+    for (int i = lane; i < np; i += 32) {
+      const float* ml = (i < n1 ? P.pml : A.part_ml) + row_of(i) * 2;
+      const float mi = __ldcg(ml), li = __ldcg(ml + 1);
+      if (i == lane) m0 = mi;
+      nan |= li != li;
+      if (mi != -CUDART_INF_F) {
+        const float mn = fmaxf(m, mi);
+        l = (m == -CUDART_INF_F ? 0.f : l * ex2f(m - mn)) + li * ex2f(mi - mn);
+        m = mn;
+      }
     }
-    const int cnt = min(32, np - i0);
-    for (int q = 0; q < cnt; ++q) {
-      const float fq = __shfl_sync(0xffffffffu, f, q);
-      if (fq == 0.f) continue;                       // nothing there (maybe never written)
-      const int k = i0 + q;
-      const float4 v = __ldcg(acc_of(k));
-      a.x = fmaf(fq, v.x, a.x); a.y = fmaf(fq, v.y, a.y);
-      a.z = fmaf(fq, v.z, a.z); a.w = fmaf(fq, v.w, a.w);
+    const float gm = warp_max(m);
+    const float L = warp_sum(m == -CUDART_INF_F ? 0.f : l * ex2f(m - gm));
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float f, const float4& x) {
+      if (f == 0.f) return;                          // nothing there (maybe never written)
+      a.x = fmaf(f, x.x, a.x); a.y = fmaf(f, x.y, a.y);
+      a.z = fmaf(f, x.z, a.z); a.w = fmaf(f, x.w, a.w);
+    };
+    const float w0 = m0 == -CUDART_INF_F ? 0.f : ex2f(m0 - gm);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) add(__shfl_sync(0xffffffffu, w0, i), v[i]);
+    for (int i0 = 4; i0 < np; i0 += 4) {
+      // four more at a time; lane q of the group holds piece i0 + q's weight
+      float fw = 0.f;
+      if (lane < 4 && i0 + lane < np) {
+        const float mi = __ldcg((i0 + lane < n1 ? P.pml : A.part_ml) + row_of(i0 + lane) * 2);
+        fw = mi == -CUDART_INF_F ? 0.f : ex2f(mi - gm);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = i0 + i < np ? __ldcg(acc_of(i0 + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) add(__shfl_sync(0xffffffffu, fw, i), v[i]);
     }
-  }
-  // a wait that gave up somewhere leaves partials unwritten: say so in the output
-  nan = __any_sync(0xffffffffu, nan);
-  const float il = nan || *A.status ? CUDART_NAN_F : L == 0.f ? 0.f : 1.f / L;
-  const __nv_bfloat162 y0 = __floats2bfloat162_rn(a.x * il, a.y * il);
-  const __nv_bfloat162 y1 = __floats2bfloat162_rn(a.z * il, a.w * il);
-  __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(A.out) + b * A.obs + j * A.oqs + hq * A.ohs +
-                       4 * lane;
-  if (A.out_vec4) {
-    uint2 pk;
-    pk.x = *reinterpret_cast<const uint32_t*>(&y0);
-    pk.y = *reinterpret_cast<const uint32_t*>(&y1);
-    *reinterpret_cast<uint2*>(dst) = pk;
-  } else {
-    dst[0] = y0.x; dst[1] = y0.y; dst[2] = y1.x; dst[3] = y1.y;
+    // a wait that gave up somewhere leaves partials unwritten: say so in the output
+    nan = __any_sync(0xffffffffu, nan);
+    const float il = nan || status ? CUDART_NAN_F : L == 0.f ? 0.f : 1.f / L;
+    const __nv_bfloat162 y0 = __floats2bfloat162_rn(a.x * il, a.y * il);
+    const __nv_bfloat162 y1 = __floats2bfloat162_rn(a.z * il, a.w * il);
+    __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(A.out) + b * A.obs + j * A.oqs +
+                         hq * A.ohs + 4 * lane;
+    if (A.out_vec4) {
+      uint2 pk;
+      pk.x = *reinterpret_cast<const uint32_t*>(&y0);
+      pk.y = *reinterpret_cast<const uint32_t*>(&y1);
+      *reinterpret_cast<uint2*>(dst) = pk;
+    } else {
+      dst[0] = y0.x; dst[1] = y0.y; dst[2] = y1.x; dst[3] = y1.y;
+    }
   }
 }
 
@@ -1218,14 +1250,28 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   const int64_t pack = (qrows * 16 + PX_PLAN_THREADS - 1) / PX_PLAN_THREADS;
   prefix_plan_kernel<<<(unsigned)(1 + pack), PX_PLAN_THREADS, 0, st>>>(P);
   if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
+  // the others as programmatic dependents: launched while the one before runs
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = st;
   if (G > 0) {
-    prefix_tc_kernel<<<PX_CTAS, PX_THREADS, sm, st>>>(P, mk, mv, mq);
-    if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
+    cfg.gridDim = dim3(PX_CTAS);
+    cfg.blockDim = dim3(PX_THREADS);
+    cfg.dynamicSmemBytes = sm;
+    if (cudaLaunchKernelEx(&cfg, prefix_tc_kernel, P, mk, mv, mq) != cudaSuccess) return SD_ELAUNCH;
   }
-  own_tc_kernel<<<dim3(PX_CTAS, L.chunks), OW_THREADS, smo, st>>>(P, mk, mv, mq32);
-  if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
-  const int64_t warps = (int64_t)B * qlen * Hq, per = PX_JOIN_THREADS / 32;
-  prefix_join_kernel<<<(unsigned)((warps + per - 1) / per), PX_JOIN_THREADS, 0, st>>>(P);
+  cfg.gridDim = dim3(PX_CTAS, L.chunks);
+  cfg.blockDim = dim3(OW_THREADS);
+  cfg.dynamicSmemBytes = smo;
+  if (cudaLaunchKernelEx(&cfg, own_tc_kernel, P, mk, mv, mq32) != cudaSuccess) return SD_ELAUNCH;
+  cfg.gridDim = dim3((unsigned)(B * Hkv));
+  cfg.blockDim = dim3(PX_JOIN_THREADS);
+  cfg.dynamicSmemBytes = 0;
+  if (cudaLaunchKernelEx(&cfg, prefix_join_kernel, P) != cudaSuccess) return SD_ELAUNCH;
   return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
 }
 
