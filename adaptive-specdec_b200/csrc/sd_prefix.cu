@@ -39,6 +39,7 @@ constexpr int PX_OVH = 2;                    // schedule cost of an item beyond 
 constexpr int PX_MIN_SHARE = PX_OVH + 1;     // fewest schedule units per CTA: a one-page item
 constexpr float PX_HEADROOM = 8.f;           // lazy-rescale headroom of the running max (base 2)
 constexpr int PX_JOIN_THREADS = 256;
+constexpr int PX_JOIN_CTAS = 4;              // per SM
 #ifndef PX_POLY
 #define PX_POLY(e) ((e) % 4 == 1)
 #endif
@@ -1012,12 +1013,13 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// A CTA per (row, kv head), a warp per query row: the pieces of the shared
-// range and of the row's own range, in piece order.
-__global__ void __launch_bounds__(PX_JOIN_THREADS) prefix_join_kernel(const PrefixParams P) {
+// A CTA per (row, kv head, 8 query rows), a warp per query row: the pieces of the
+// shared range and of the row's own range, in piece order.
+__global__ void __launch_bounds__(PX_JOIN_THREADS, PX_JOIN_CTAS) prefix_join_kernel(const PrefixParams P) {
   const AttnParams& A = P.A;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int b = (int)(blockIdx.x / A.Hkv), h = (int)(blockIdx.x - b * A.Hkv);
+  const int chunks = (A.R + PX_JOIN_THREADS / 32 - 1) / (PX_JOIN_THREADS / 32);
+  const int bh = (int)(blockIdx.x / chunks), b = bh / A.Hkv, h = bh - b * A.Hkv;
   // what the plan says (complete before the kernel in front of this one began)
   const int g = P.rowgroup[b];
   const int tb = A.rowpre[b + 1] - A.rowpre[b], RC = P.qc * A.group;
@@ -1036,7 +1038,8 @@ __global__ void __launch_bounds__(PX_JOIN_THREADS) prefix_join_kernel(const Pref
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int status = *A.status;
-  for (int r = w; r < A.R; r += PX_JOIN_THREADS / 32) {
+  const int r = (int)(blockIdx.x - bh * chunks) * (PX_JOIN_THREADS / 32) + w;
+  if (r < A.R) {
     const int j = r / A.group, hq = h * A.group + r - j * A.group;
     // pieces [0, n1): the shared range, two per CTA where both tiles worked on
     // the rows; [n1, n1 + n2): the row's own range
@@ -1268,7 +1271,8 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   cfg.blockDim = dim3(OW_THREADS);
   cfg.dynamicSmemBytes = smo;
   if (cudaLaunchKernelEx(&cfg, own_tc_kernel, P, mk, mv, mq32) != cudaSuccess) return SD_ELAUNCH;
-  cfg.gridDim = dim3((unsigned)(B * Hkv));
+  const int64_t per = PX_JOIN_THREADS / 32;
+  cfg.gridDim = dim3((unsigned)((int64_t)B * Hkv * ((R + per - 1) / per)));
   cfg.blockDim = dim3(PX_JOIN_THREADS);
   cfg.dynamicSmemBytes = 0;
   if (cudaLaunchKernelEx(&cfg, prefix_join_kernel, P) != cudaSuccess) return SD_ELAUNCH;
