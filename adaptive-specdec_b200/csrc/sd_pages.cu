@@ -13,12 +13,16 @@
 //            past the rows' keeps (of F) goes to free[n_free + F - 1 - o], so
 //            a trim undoes a reserve to the entry
 // A call that cannot be done for every row (a row past its table, too few
-// free pages, too small a slot array) changes nothing but *err.
+// free pages, too small a slot array, a new token in one of a row's first
+// floor[b] pages) changes nothing but *err.
 //
 // Bytes are few; what bounds these calls is launches and the scan over the
-// rows.  One CTA scans (pages and tokens packed in one 64-bit sum); the slots
-// and table entries of a reserve are filled by a second launch (programmatic
-// dependent) with a warp per (row, run of tokens).
+// rows (pages and tokens packed in one 64-bit sum).  A reserve is a scan by one
+// CTA and a second launch (programmatic dependent) with a warp per (row, run of
+// tokens); for few tokens the scanning CTA does the second part too.  A trim is
+// one cluster of CTAs: every CTA scans all rows, and behind a cluster barrier
+// (all have read the state that is about to change) moves the pages of its
+// share of the rows, a warp each.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -28,6 +32,14 @@
 namespace sd {
 
 constexpr int PT_THREADS = 1024;
+constexpr int PT_CLUSTER = 8;
+// (row, run) pairs up to which the scanning CTA fills the slots itself: a launch
+// less for the host, and on the device, in a CUDA graph, 3.9 us against 4.6 for
+// 8 rows of 5 tokens, 5.4 against 5.0 for 64, 7.0 against 5.0 for 128.  Rows from
+// which a trim takes a cluster: 3.0 us by one CTA against 3.8 by eight for 16
+// rows; a trim and a reserve of 128 rows 10.3 against 9.6, of 512 rows 22 against
+// 10.1 (512 rows that give back and take 32 pages each: 15 us, 2 M slots).
+constexpr int PT_FUSED_WARPS = 64;
 constexpr int PF_THREADS = 256;
 
 struct PagesParams {
@@ -41,12 +53,14 @@ struct PagesParams {
   const int64_t* lengths;
   const int64_t* add;                           // new tokens per row, or nullptr: add_all each
   int64_t add_all;
+  const int32_t* floor;                         // pages per row that take no new tokens, or nullptr
   int64_t* slots;
   int64_t max_tokens;
   int32_t* starts;                              // [B + 1]
   int* err;
-  int* plan;                                    // workspace: pre [B], had [B], n_free, ok
+  int* plan;                                    // workspace: pages before row b [B], had [B], n_free, ok
   int run, runs;                                // tokens per warp of the fill, warps per row
+  bool fused;                                   // the scanning CTA fills
 };
 
 // Exclusive block scan of packed (tokens, pages << 32) sums over PT_THREADS.
@@ -54,9 +68,48 @@ __device__ __forceinline__ long long scan_pair(long long v, long long* red, long
   return block_excl_scan<long long>(v, red, total);
 }
 
+// Warp w of warps: the slots of a row's tokens [run * P.run, ...) and, for run 0,
+// its new table entries; the warps past the rows fill the slots behind the last
+// token with -1.
+__device__ __forceinline__ void reserve_fill(const PagesParams& P, const int* plan,
+                                             const int32_t* starts, int64_t w, int64_t warps) {
+  const int lane = threadIdx.x & 31;
+  const bool ok = plan[2 * P.B + 1] != 0;
+  const int top = plan[2 * P.B] - 1;
+  const int64_t rows = (int64_t)P.B * P.runs;
+  if (w >= rows) {
+    const int64_t first = ok ? starts[P.B] : 0;
+    for (int64_t i = first + (w - rows) * 32 + lane; i < P.max_tokens; i += (warps - rows) * 32)
+      P.slots[i] = -1;
+    return;
+  }
+  if (!ok) return;
+  const int b = (int)(w / P.runs), run = (int)(w % P.runs);
+  const int64_t len = P.lengths[b];
+  const int s0 = starts[b], n = starts[b + 1] - s0;
+  const int pre = plan[b], had = plan[P.B + b];
+  int32_t* row = P.bt + b * P.bt_stride;
+  if (run == 0) {
+    const int need = (int)((len + n + SD_KV_PAGE - 1) / SD_KV_PAGE);
+    for (int p = had + lane; p < need; p += 32) row[p] = P.free_stack[top - (pre + p - had)];
+  }
+  if (!P.slots) return;
+  const int i1 = (int)min((int64_t)n, (int64_t)(run + 1) * P.run);
+  for (int i = run * P.run + lane; i < i1; i += 32) {
+    const int64_t pos = len + i;
+    const int p = (int)(pos / SD_KV_PAGE);
+    const int page = p < had ? row[p] : P.free_stack[top - (pre + p - had)];
+    P.slots[(int64_t)s0 + i] =
+        page < 0 ? -1 : (int64_t)page * SD_KV_PAGE + (pos & (SD_KV_PAGE - 1));
+  }
+}
+
 __global__ void __launch_bounds__(PT_THREADS) pages_reserve_plan_kernel(const PagesParams P) {
   __shared__ long long red[33];
   __shared__ int bad;
+  __shared__ int own_plan[2 * PT_FUSED_WARPS + 2], own_starts[PT_FUSED_WARPS + 1];
+  int* plan = P.fused ? own_plan : P.plan;
+  int32_t* starts = P.fused ? own_starts : P.starts;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int t = threadIdx.x;
   if (t == 0) bad = 0;
@@ -70,34 +123,37 @@ __global__ void __launch_bounds__(PT_THREADS) pages_reserve_plan_kernel(const Pa
       const int had = P.owned[b];
       const int64_t cap = (int64_t)P.W * SD_KV_PAGE;
       int why = 0;
-      if (len < 0 || add < 0 || len > cap || add > cap - len) {
+      if (len < 0 || add < 0 || len > cap || add > cap - len || had < 0) {
         why = SD_PAGES_ERR_CAPACITY;
       } else {
         const int64_t need = (len + add + SD_KV_PAGE - 1) / SD_KV_PAGE;
         v = (add & 0xFFFFFFFFLL) | ((need > had ? need - had : 0) << 32);
       }
+      if (!why && P.floor && add > 0 && len < (int64_t)P.floor[b] * SD_KV_PAGE)
+        why = SD_PAGES_ERR_SHARED;
       if (why) atomicOr(&bad, why);
-      P.plan[P.B + b] = had;
+      plan[P.B + b] = had;
     }
     long long sum;
     const long long ex = carry + scan_pair(v, red, &sum);
     carry += sum;
     if (b < P.B) {
-      P.starts[b] = (int32_t)(ex & 0xFFFFFFFFLL);
-      P.plan[b] = (int32_t)(ex >> 32);
+      starts[b] = (int32_t)(ex & 0xFFFFFFFFLL);
+      plan[b] = (int32_t)(ex >> 32);
     }
     __syncthreads();
   }
   const long long tokens = carry & 0xFFFFFFFFLL, pages = carry >> 32;
   const int had_free = *P.n_free;
-  if (t == 0) P.starts[P.B] = (int32_t)tokens;
+  if (t == 0) starts[P.B] = (int32_t)tokens;
   int why = bad;
+  if (had_free < 0 || had_free > P.n_pages) why |= SD_PAGES_ERR_CAPACITY;   // a broken table
   if (!why && pages > had_free) why = SD_PAGES_ERR_EXHAUSTED;
   if (!why && P.slots && tokens > P.max_tokens) why = SD_PAGES_ERR_SLOTS;
   __syncthreads();                                   // everybody has read n_free
   if (t == 0) {
-    P.plan[2 * P.B] = had_free;
-    P.plan[2 * P.B + 1] = why == 0;
+    plan[2 * P.B] = had_free;
+    plan[2 * P.B + 1] = why == 0;
     if (why)
       atomicOr(P.err, why);
     else
@@ -107,65 +163,54 @@ __global__ void __launch_bounds__(PT_THREADS) pages_reserve_plan_kernel(const Pa
     for (int b = t; b < P.B; b += PT_THREADS) {
       const int64_t add = P.add ? P.add[b] : P.add_all;
       const int need = (int)((P.lengths[b] + add + SD_KV_PAGE - 1) / SD_KV_PAGE);
-      if (need > P.plan[P.B + b]) P.owned[b] = need;
+      if (need > plan[P.B + b]) P.owned[b] = need;
     }
   }
+  if (!P.fused) return;
+  __syncthreads();                                   // plan and starts, for the CTA's other warps
+  for (int b = t; b <= P.B; b += PT_THREADS) P.starts[b] = starts[b];
+  const int64_t n = (int64_t)P.B * P.runs + PT_THREADS / 32;     // the last 32: slots behind
+  for (int64_t w = t >> 5; w < n; w += PT_THREADS / 32) reserve_fill(P, plan, starts, w, n);
 }
 
-// Warp (row, run): the slots of the row's tokens [run * P.run, ...) and, for
-// run 0, its new table entries.  The warps past the rows fill the slots
-// behind the last token with -1.
 __global__ void __launch_bounds__(PF_THREADS) pages_reserve_fill_kernel(const PagesParams P) {
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * (PF_THREADS / 32) + (threadIdx.x >> 5);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const bool ok = P.plan[2 * P.B + 1] != 0;
-  const int top = P.plan[2 * P.B] - 1;
-  const int64_t rows = (int64_t)P.B * P.runs;
-  if (w >= rows) {
-    const int64_t n = (int64_t)gridDim.x * (PF_THREADS / 32) - rows;
-    const int64_t first = ok ? P.starts[P.B] : 0;
-    for (int64_t i = first + (w - rows) * 32 + lane; i < P.max_tokens; i += n * 32) P.slots[i] = -1;
-    return;
-  }
-  if (!ok) return;
-  const int b = (int)(w / P.runs), run = (int)(w % P.runs);
-  const int64_t len = P.lengths[b];
-  const int s0 = P.starts[b], n = P.starts[b + 1] - s0;
-  const int pre = P.plan[b], had = P.plan[P.B + b];
-  int32_t* row = P.bt + b * P.bt_stride;
-  if (run == 0) {
-    const int need = (int)((len + n + SD_KV_PAGE - 1) / SD_KV_PAGE);
-    for (int p = had + lane; p < need; p += 32) row[p] = P.free_stack[top - (pre + p - had)];
-  }
-  if (!P.slots) return;
-  const int i1 = min(n, (run + 1) * P.run);
-  for (int i = run * P.run + lane; i < i1; i += 32) {
-    const int64_t pos = len + i;
-    const int p = (int)(pos / SD_KV_PAGE);
-    const int page = p < had ? row[p] : P.free_stack[top - (pre + p - had)];
-    P.slots[(int64_t)s0 + i] =
-        page < 0 ? -1 : (int64_t)page * SD_KV_PAGE + (pos & (SD_KV_PAGE - 1));
+  reserve_fill(P, P.plan, P.starts, (int64_t)blockIdx.x * (PF_THREADS / 32) + (threadIdx.x >> 5),
+               (int64_t)gridDim.x * (PF_THREADS / 32));
+}
+
+// The barrier of the launch's only cluster (or CTA).
+__device__ __forceinline__ void grid_barrier() {
+  if (gridDim.x > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    __syncthreads();
   }
 }
 
-// One CTA: the rows' keeps and their scan, then a warp per row moves its pages.
+// Every CTA of the cluster: the rows' keeps and their scan, PT_THREADS rows at a
+// time; then its warps move the pages of their share of those rows.
 __global__ void __launch_bounds__(PT_THREADS) pages_trim_kernel(const PagesParams P) {
   __shared__ int red[33];
   __shared__ int pre[PT_THREADS], keep[PT_THREADS], had[PT_THREADS];
-  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+  const int t = threadIdx.x, lane = t & 31;
+  const int gw = (int)blockIdx.x * (PT_THREADS / 32) + (t >> 5);       // warp of the cluster
+  const int nw = (int)gridDim.x * (PT_THREADS / 32);
   const int had_free = *P.n_free;
+  auto keep_of = [&](int b) {
+    const int64_t len = max(P.lengths[b], (int64_t)0);
+    return max((len + SD_KV_PAGE - 1) / SD_KV_PAGE, (int64_t)P.shared[b]);
+  };
   // all pages first: where the stack will end decides where each page goes
   int mine = 0;
-  for (int b = t; b < P.B; b += PT_THREADS) {
-    const int64_t len = max(P.lengths[b], (int64_t)0);
-    const int64_t k = max((len + SD_KV_PAGE - 1) / SD_KV_PAGE, (int64_t)P.shared[b]);
-    mine += (int)max((int64_t)P.owned[b] - k, (int64_t)0);
-  }
+  for (int b = t; b < P.B; b += PT_THREADS)
+    mine += (int)max(min(P.owned[b], P.W) - keep_of(b), (int64_t)0);
   const int all = block_sum<int>(mine, red);
-  __syncthreads();
-  if (all > P.n_pages - had_free) {                  // more pages than there are: a broken table
-    if (t == 0) atomicOr(P.err, SD_PAGES_ERR_CAPACITY);
+  grid_barrier();                                    // everybody has read owned and n_free
+  // more pages than there are: a broken table
+  if (had_free < 0 || all < 0 || all > P.n_pages - had_free) {
+    if (gw == 0 && lane == 0) atomicOr(P.err, SD_PAGES_ERR_CAPACITY);
     return;
   }
   int carry = 0;
@@ -173,10 +218,8 @@ __global__ void __launch_bounds__(PT_THREADS) pages_trim_kernel(const PagesParam
     const int b = b0 + t;
     int gone = 0, o = 0, k32 = 0;
     if (b < P.B) {
-      o = P.owned[b];
-      const int64_t len = max(P.lengths[b], (int64_t)0);
-      const int64_t k = max((len + SD_KV_PAGE - 1) / SD_KV_PAGE, (int64_t)P.shared[b]);
-      k32 = (int)min(k, (int64_t)o);
+      o = min(P.owned[b], P.W);
+      k32 = (int)min(keep_of(b), (int64_t)o);
       gone = o - k32;
     }
     int sum;
@@ -185,20 +228,20 @@ __global__ void __launch_bounds__(PT_THREADS) pages_trim_kernel(const PagesParam
     keep[t] = k32;
     had[t] = o;
     carry += sum;
-    __syncthreads();
+    grid_barrier();                                  // these rows' state has been read by all
     const int nb = min(PT_THREADS, P.B - b0);
-    for (int q = w; q < nb; q += PT_THREADS / 32) {
-      const int k = keep[q], h = min(had[q], P.W);
+    for (int q = gw; q < nb; q += nw) {
+      const int k = keep[q], h = had[q];
       int32_t* row = P.bt + (int64_t)(b0 + q) * P.bt_stride;
       for (int p = k + lane; p < h; p += 32) {
         P.free_stack[had_free + all - 1 - (pre[q] + p - k)] = row[p];
         row[p] = -1;
       }
-      if (lane == 0 && k < had[q]) P.owned[b0 + q] = k;
+      if (lane == 0 && k < h) P.owned[b0 + q] = k;
     }
-    __syncthreads();
+    __syncthreads();                                 // pre, keep and had are rewritten next
   }
-  if (t == 0) *P.n_free = had_free + all;
+  if (gw == 0 && lane == 0) *P.n_free = had_free + all;
 }
 
 static int pages_check(const PagesParams& P) {
@@ -222,13 +265,14 @@ size_t sd_pages_workspace_bytes(int B) {
 
 int sd_pages_reserve(int32_t* block_table, int bt_stride, int W, int32_t* owned,
                      const int32_t* free_stack, int n_pages, int32_t* n_free,
-                     const int64_t* lengths, const int64_t* new_tokens, int64_t new_each, int B,
-                     int64_t* slots, int64_t max_tokens, int32_t* starts, int* err,
-                     void* workspace, size_t workspace_bytes, void* stream) {
+                     const int64_t* lengths, const int64_t* new_tokens, int64_t new_each,
+                     const int32_t* floor_pages, int B, int64_t* slots, int64_t max_tokens, int32_t* starts,
+                     int* err, void* workspace, size_t workspace_bytes, void* stream) {
   PagesParams P = {};
   P.bt = block_table; P.bt_stride = bt_stride; P.W = W; P.n_pages = n_pages; P.B = B;
   P.owned = owned; P.free_stack = const_cast<int32_t*>(free_stack); P.n_free = n_free;
   P.lengths = lengths; P.add = new_tokens; P.add_all = new_each;
+  P.floor = floor_pages;
   P.slots = slots; P.max_tokens = slots ? max_tokens : 0; P.starts = starts; P.err = err;
   P.plan = reinterpret_cast<int*>(workspace);
   if (int rc = pages_check(P)) return rc;
@@ -247,11 +291,13 @@ int sd_pages_reserve(int32_t* block_table, int bt_stride, int W, int32_t* owned,
   P.run = 512;
   while ((most + P.run - 1) / P.run * B > 65536) P.run *= 2;
   P.runs = (int)std::max<int64_t>(1, (most + P.run - 1) / P.run);
+  P.fused = (int64_t)B * P.runs <= PT_FUSED_WARPS && P.max_tokens <= PT_FUSED_WARPS * 32;
   // some warps for the slots behind the last token
   const int64_t tail = (P.max_tokens + 4095) / 4096;
   const int64_t warps = (int64_t)B * P.runs + std::min<int64_t>(std::max<int64_t>(tail, 1), 1024);
   pages_reserve_plan_kernel<<<1, PT_THREADS, 0, st>>>(P);
   if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;
+  if (P.fused) return SD_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((warps + PF_THREADS / 32 - 1) / (PF_THREADS / 32)));
   cfg.blockDim = dim3(PF_THREADS);
@@ -275,7 +321,17 @@ int sd_pages_trim(int32_t* block_table, int bt_stride, int W, int32_t* owned,
   if (int rc = pages_check(P)) return rc;
   if (B == 0) return SD_OK;
   if (!shared) return SD_EINVAL;
-  pages_trim_kernel<<<1, PT_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(P);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(B > 2 * PT_THREADS / 32 ? PT_CLUSTER : 1);
+  cfg.blockDim = dim3(PT_THREADS);
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cfg.gridDim.x;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, pages_trim_kernel, P) != cudaSuccess) return SD_ELAUNCH;
   return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
 }
 

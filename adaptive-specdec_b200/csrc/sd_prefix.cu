@@ -22,6 +22,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "sd_attn.cuh"
 #include "sd_common.cuh"
@@ -40,9 +41,6 @@ constexpr int PX_MIN_SHARE = PX_OVH + 1;     // fewest schedule units per CTA: a
 constexpr float PX_HEADROOM = 8.f;           // lazy-rescale headroom of the running max (base 2)
 constexpr int PX_JOIN_THREADS = 256;
 constexpr int PX_JOIN_CTAS = 4;              // per SM
-#ifndef PX_POLY
-#define PX_POLY(e) ((e) % 4 == 1)
-#endif
 constexpr int OW_STAGES = 3;                 // K + V tiles in flight (own ranges)
 constexpr int OW_THREADS = 192;              // warps 0-3 softmax, 4 TMA, 5 MMA
 constexpr int OW_OVH = 2;                    // schedule cost of a (row, kv head) beyond its pages
@@ -511,7 +509,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
             unpair(fma2(pair2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sl22, nm2), a, b);
             // a part by the FMA pipe: the exponentials of a page take 2048
             // cycles of the special-function units otherwise
-            const unsigned long long p2 = PX_POLY(e) ? px_exp2(a, b) : pair2(ex2f(a), ex2f(b));
+            const unsigned long long p2 = e % 4 == 1 ? px_exp2(a, b) : pair2(ex2f(a), ex2f(b));
             ls[e & 1] = add2(ls[e & 1], p2);
             unpair(p2, a, b);
             p[e] = pack_bf16(a, b);
@@ -1245,11 +1243,18 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
       !cache_map(&mq, P.qp, qrows) || !cache_map(&mq32, P.qp, qrows, 32))
     return SD_ENOTSUP;
   const int sm = (int)sizeof(PxSmem) + 1024, smo = (int)sizeof(OwSmem) + 1024;   // room to align
-  if (cudaFuncSetAttribute(prefix_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) !=
-          cudaSuccess ||
-      cudaFuncSetAttribute(own_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smo) !=
-          cudaSuccess)
-    return SD_ELAUNCH;
+  static std::atomic<uint64_t> ready{0};             // devices whose kernels may use that much
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return SD_ELAUNCH;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!(ready.load() & bit) || !bit) {
+    if (cudaFuncSetAttribute(prefix_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) !=
+            cudaSuccess ||
+        cudaFuncSetAttribute(own_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smo) !=
+            cudaSuccess)
+      return SD_ELAUNCH;
+    ready.fetch_or(bit);
+  }
   const int64_t pack = (qrows * 16 + PX_PLAN_THREADS - 1) / PX_PLAN_THREADS;
   prefix_plan_kernel<<<(unsigned)(1 + pack), PX_PLAN_THREADS, 0, st>>>(P);
   if (cudaGetLastError() != cudaSuccess) return SD_ELAUNCH;

@@ -41,8 +41,8 @@ _SIGNATURES = {
     "sd_token_logprobs": ([_vp, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _f32, _i32, _vp,
                            _vp, _vp, _vp, _vp, _vp], _i32),
     "sd_pages_workspace_bytes": ([_i32], _sz),
-    "sd_pages_reserve": ([_vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _i64,
-                          _vp, _vp, _vp, _sz, _vp], _i32),
+    "sd_pages_reserve": ([_vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _i32,
+                          _vp, _i64, _vp, _vp, _vp, _sz, _vp], _i32),
     "sd_pages_trim": ([_vp, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp], _i32),
     "sd_kv_lengths_update": ([_vp, _vp, _i64, _i32, _i32, _i64, _vp, _vp], _i32),
     "sd_qkv_norm_rope_append": ([_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _f32, _vp, _vp, _i64,
@@ -151,7 +151,7 @@ _SAME_DEVICE = contextlib.nullcontext()
 def on_device(device):
     """Context in which ``device`` is the current one (nothing to do when it is:
     torch.cuda.device costs more than a small kernel's launch)."""
-    if torch.cuda.current_device() == device.index:
+    if torch._C._cuda_getDevice() == device.index:
         return _SAME_DEVICE
     return torch.cuda.device(device)
 

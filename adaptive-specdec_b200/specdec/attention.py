@@ -120,16 +120,21 @@ def prefix_attention(q, k_pool, v_pool, lengths, block_table, group_starts, pref
     Both group arrays live on the device, so a captured call follows them.
     bf16 heads of 128 share; other shapes are computed row by row.
     """
-    dev = q.device
-    if dev.type != "cuda":
+    dev, dt = q.device, q.dtype
+    if not q.is_cuda:
         L.require_cuda(q)
-    for t in (k_pool, v_pool, lengths, block_table, group_starts, prefix_pages, valid, out):
-        if t is not None and t.device != dev:
-            raise L.SpecdecError("prefix_attention needs every tensor on one CUDA device")
+    if k_pool.device != dev or v_pool.device != dev or lengths.device != dev \
+            or block_table.device != dev or group_starts.device != dev \
+            or prefix_pages.device != dev or (valid is not None and valid.device != dev) \
+            or (out is not None and out.device != dev):
+        raise L.SpecdecError("prefix_attention needs every tensor on one CUDA device")
+    if torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return prefix_attention(q, k_pool, v_pool, lengths, block_table, group_starts,
+                                    prefix_pages, valid, scale, out)
     if q.dim() != 4 or k_pool.dim() != 4:
         raise L.SpecdecError("prefix_attention needs q [B, Hq, qlen, D] and pools "
                              "[n_pages, Hkv, PAGE, D]")
-    dt = q.dtype
     if dt not in _ATTN_DTYPES or k_pool.dtype != dt or v_pool.dtype != dt:
         raise L.SpecdecError(f"prefix_attention supports bf16 / fp32, got {dt}")
     B, Hq, qlen, D = q.shape
@@ -147,12 +152,9 @@ def prefix_attention(q, k_pool, v_pool, lengths, block_table, group_starts, pref
         raise L.SpecdecError("group_starts [G + 1] and prefix_pages [G] must be contiguous int32")
     if lengths.numel() != B or (valid is not None and valid.numel() != B):
         raise L.SpecdecError(f"lengths and valid need one entry per row ({B})")
-    sc = float(scale) if scale is not None else D ** -0.5
+    sc = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < sc < 3e38:
         raise L.SpecdecError(f"scale must be positive and finite, got {scale}")
-    if out is not None and (out.shape != (B, qlen, Hq, D) or out.dtype != dt
-                            or (D > 1 and out.stride(3) != 1)):
-        raise L.SpecdecError(f"out must be {(B, qlen, Hq, D)} of {dt}, contiguous along D")
     qb, qh, ql, qd = q.stride()
     if qd != 1 or (dt == torch.bfloat16 and D == 128 and (
             q.data_ptr() % 16 or qb % 8 or qh % 8 or ql % 8)):
@@ -164,22 +166,25 @@ def prefix_attention(q, k_pool, v_pool, lengths, block_table, group_starts, pref
         lengths = lengths.long().contiguous()
     if valid is not None and (valid.dtype != torch.long or not valid.is_contiguous()):
         valid = valid.long().contiguous()
-    W, code = block_table.shape[1], _ATTN_DTYPES[dt]
-    with L.on_device(dev):
-        if out is None:
-            out = torch.empty((B, qlen, Hq, D), dtype=dt, device=dev)
-        if B == 0 or qlen == 0:
-            return out
-        # a fresh buffer per call: calls on several streams and calls captured
-        # into different graphs never share one
-        nws = L.workspace_bytes("sd_prefix_attn_workspace_bytes", B, G, Hq, Hkv, D, W, qlen, code)
-        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+    if out is None:
+        out = torch.empty((B, qlen, Hq, D), dtype=dt, device=dev)
+        ob, ol, oh = qlen * Hq * D, Hq * D, D
+    else:
+        if out.shape != (B, qlen, Hq, D) or out.dtype != dt or (D > 1 and out.stride(3) != 1):
+            raise L.SpecdecError(f"out must be {(B, qlen, Hq, D)} of {dt}, contiguous along D")
         ob, ol, oh, _ = out.stride()
-        L.check(L.lib().sd_prefix_attn(
-            q.data_ptr(), qb, qh, ql, k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
-            W, npages, lengths.data_ptr(), L.address(valid), group_starts.data_ptr(),
-            prefix_pages.data_ptr(), G, B, Hq, Hkv, D, qlen, sc, out.data_ptr(), ob, ol, oh, code,
-            ws.data_ptr(), nws, L.stream_of(dev)), "prefix_attn")
+    if B == 0 or qlen == 0:
+        return out
+    W, code = block_table.shape[1], _ATTN_DTYPES[dt]
+    # a fresh buffer per call: calls on several streams and calls captured into
+    # different graphs never share one
+    nws = L.workspace_bytes("sd_prefix_attn_workspace_bytes", B, G, Hq, Hkv, D, W, qlen, code)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+    L.check(L.lib().sd_prefix_attn(
+        q.data_ptr(), qb, qh, ql, k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
+        W, npages, lengths.data_ptr(), L.address(valid), group_starts.data_ptr(),
+        prefix_pages.data_ptr(), G, B, Hq, Hkv, D, qlen, sc, out.data_ptr(), ob, ol, oh, code,
+        ws.data_ptr(), nws, L.stream_of(dev)), "prefix_attn")
     return out
 
 

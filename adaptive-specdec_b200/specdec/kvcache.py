@@ -441,7 +441,8 @@ class DevicePageTable:
     """
 
     ERRORS = {1: "a row's length left [0, capacity]", 2: "a slot was written without a page",
-              4: "page pool exhausted", 8: "more new tokens than max_tokens"}
+              4: "page pool exhausted", 8: "more new tokens than max_tokens",
+              16: "a new token below a row's floor of shared pages"}
 
     def __init__(self, batch_size, pages_per_row, n_pages, device, err=None, stack=None):
         B, W, n = int(batch_size), int(pages_per_row), int(n_pages)
@@ -473,13 +474,15 @@ class DevicePageTable:
     @classmethod
     def over(cls, block_table, owned, shared, free, n_free, err):
         """A table over state that the caller holds (no copies)."""
-        dev = block_table.device
-        if dev.type != "cuda":
+        dev, i32 = block_table.device, torch.int32
+        if not block_table.is_cuda:
             raise L.SpecdecError("DevicePageTable keeps its state on the GPU (no CPU fallback)")
-        for t in (block_table, owned, shared, free, n_free, err):
-            if t.dtype != torch.int32 or t.device != dev:
+        if block_table.dtype != i32:
+            raise L.SpecdecError("a page table's state is int32 on one CUDA device")
+        for t in (owned, shared, free, n_free, err):
+            if t.dtype != i32 or t.device != dev:
                 raise L.SpecdecError("a page table's state is int32 on one CUDA device")
-            if t is not block_table and not t.is_contiguous():
+            if not t.is_contiguous():
                 raise L.SpecdecError("owned, shared, free, n_free and err must be contiguous")
         if block_table.dim() != 2 or block_table.stride(1) != 1:
             raise L.SpecdecError("block_table must be [B, W] with contiguous rows")
@@ -497,7 +500,7 @@ class DevicePageTable:
             raise L.SpecdecError(f"{name} must be an integer [B] tensor on {self.device}")
         return t if t.dtype == torch.long and t.is_contiguous() else t.long().contiguous()
 
-    def reserve(self, lengths, new, max_tokens=None, slot_map=True):
+    def reserve(self, lengths, new, max_tokens=None, slot_map=True, floor=None):
         """Pages for ``new`` more tokens of every row past ``lengths`` [B].
 
         ``new`` is one int for all rows or an integer [B] tensor; with a tensor
@@ -505,7 +508,9 @@ class DevicePageTable:
         (slots [max_tokens] int64, starts [B + 1] int32): token i of row b goes
         to pool slot slots[starts[b] + i] = page * PAGE + offset; slots behind
         the last token are -1.  ``slot_map=False`` leaves the map out: (None,
-        starts).
+        starts).  With ``floor`` [B] int32 (``shared``, for rows that must not
+        write what others read) a new token of row b in its first floor[b]
+        pages is an error.
         """
         lens = self._rows(lengths, "lengths")
         if not slot_map:
@@ -516,24 +521,26 @@ class DevicePageTable:
             add, each, total = self._rows(new, "new"), 0, int(max_tokens)
         else:
             add, each = None, int(new)
-            if each < 0:
-                raise L.SpecdecError(f"new tokens must not be negative, got {each}")
+            if not 0 <= each < 1 << 31:
+                raise L.SpecdecError(f"new tokens must be in [0, 2^31), got {each}")
             total = self.B * each if max_tokens is None else int(max_tokens)
-        if total < 0:
-            raise L.SpecdecError(f"max_tokens must not be negative, got {total}")
+        if floor is not None and (floor.dtype != torch.int32 or floor.device != self.device
+                                  or floor.numel() != self.B or not floor.is_contiguous()):
+            raise L.SpecdecError(f"floor must be a contiguous int32 [B] tensor on {self.device}")
+        if not 0 <= total < 1 << 31:
+            raise L.SpecdecError(f"max_tokens must be in [0, 2^31), got {total}")
         dev = self.device
+        # (an empty map still has an address: NULL means no map)
+        slots = torch.empty(max(total, 1), dtype=torch.long, device=dev) if slot_map else None
+        starts = torch.empty(self.B + 1, dtype=torch.int32, device=dev)
+        nws = L.workspace_bytes("sd_pages_workspace_bytes", self.B)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
         with L.on_device(dev):
-            # (an empty map still has an address: NULL means no map)
-            slots = torch.empty(max(total, 1), dtype=torch.long, device=dev) \
-                if slot_map else None
-            starts = torch.empty(self.B + 1, dtype=torch.int32, device=dev)
-            nws = L.workspace_bytes("sd_pages_workspace_bytes", self.B)
-            ws = torch.empty(nws, dtype=torch.uint8, device=dev)
             L.check(L.lib().sd_pages_reserve(
                 self.block_table.data_ptr(), self.block_table.stride(0), self.W,
                 self.owned.data_ptr(), self.free.data_ptr(), self.n_pages, self.n_free.data_ptr(),
-                lens.data_ptr(), L.address(add), each, self.B, L.address(slots), total,
-                starts.data_ptr(), self.err.data_ptr(), ws.data_ptr(), nws, L.stream_of(dev)),
+                lens.data_ptr(), L.address(add), each, L.address(floor), self.B, L.address(slots),
+                total, starts.data_ptr(), self.err.data_ptr(), ws.data_ptr(), nws, L.stream_of(dev)),
                 "pages_reserve")
         return (slots[:total] if slot_map and total == 0 else slots), starts
 
@@ -585,7 +592,9 @@ class PagedRaggedCache(RaggedCache):
     follows the device lengths with no host copy of them, a pool that runs out
     sets the error flag instead of raising, and ``fork`` makes several rows
     of each prompt that share its pages.  ``prefix`` (group starts, shared
-    pages) then tells the attention which rows share what.
+    pages) then tells the attention which rows share what.  A forked row may
+    not be rolled back into its shared pages and then grow: ``reserve`` sets
+    the error flag (bit 16) and hands out nothing.
 
     Only the kernel attention path (attn_impl "specdec_b200") reads paged
     layers.
@@ -627,7 +636,9 @@ class PagedRaggedCache(RaggedCache):
     def reserve(self, q):
         """Pages for the next q tokens of every row (call before the forward)."""
         if self.device_pages:
-            self.pages.reserve(self.lengths, int(q), slot_map=False)
+            # (rows of a fork must not write the pages that they share)
+            self.pages.reserve(self.lengths, int(q), slot_map=False,
+                               floor=None if self.prefix is None else self.pages.shared)
             return
         self._push(self.pages.reserve(self._mirror().numpy(), q))
 
@@ -636,7 +647,8 @@ class PagedRaggedCache(RaggedCache):
         plen (real pages for each row's prompt, the sink for its padding)."""
         if self.device_pages:
             pl = torch.as_tensor(plen).to(self.device, torch.long).reshape(-1).clamp(max=int(P))
-            self.pages.reserve(self.lengths, pl, slot_map=False)
+            self.pages.reserve(self.lengths, pl, slot_map=False,
+                               floor=None if self.prefix is None else self.pages.shared)
             top = (self.lengths + int(P) + PAGE - 1) // PAGE
             pad = (self._columns() < top.view(-1, 1)) & (self.block_table < 0)
             self.block_table.masked_fill_(pad, self.pages.sink)
@@ -646,7 +658,8 @@ class PagedRaggedCache(RaggedCache):
 
     def release(self, rows):
         """Return the pages of the given rows to the pool (their lengths go to 0).
-        Shared pages of a forked row stay with the rows that still read them."""
+        Shared pages of a forked row stay with the rows that still read them; the
+        row itself leaves its group."""
         rows = [int(r) for r in rows]
         if self.device_pages:
             at = torch.tensor(rows, dtype=torch.long, device=self.device)
@@ -657,6 +670,12 @@ class PagedRaggedCache(RaggedCache):
             self.block_table[at] = -1
             self.pages.owned[at] = 0
             self.pages.shared[at] = 0
+            if self.prefix is not None:
+                gone = set(rows)
+                self._set_groups([
+                    (a, b, 0 if a in gone else p)
+                    for first, end, p in self._groups
+                    for a, b in self._runs(first, end, gone)])
             if self._host_valid:
                 self._host[rows] = 0
             return
@@ -665,6 +684,30 @@ class PagedRaggedCache(RaggedCache):
         self.pages.release(rows)
         self.set_lengths(h)
         self._push()
+
+    @staticmethod
+    def _runs(first, end, gone):
+        """[first, end) as runs without the rows of `gone` and these rows one by one."""
+        out, a = [], first
+        for r in range(first, end):
+            if r in gone:
+                out += ([(a, r)] if a < r else []) + [(r, r + 1)]
+                a = r + 1
+        return out + ([(a, end)] if a < end else [])
+
+    def _set_groups(self, groups):
+        """The groups (first row, end, shared pages) behind ``prefix``, whose
+        tensors have room for a group per row (groups behind the last are
+        empty) and keep their addresses: captured graphs follow a release."""
+        B, n = self.batch_size, len(groups)
+        self._groups = groups
+        starts = [g[0] for g in groups] + [B] * (B + 1 - n)
+        pages = [g[2] for g in groups] + [0] * (B - n)
+        if self.prefix is None:
+            self.prefix = (torch.empty(B + 1, dtype=torch.int32, device=self.device),
+                           torch.empty(B, dtype=torch.int32, device=self.device))
+        for t, v in zip(self.prefix, (starts, pages)):
+            t.copy_(torch.tensor(v, dtype=torch.int32))
 
     def fork(self, counts):
         """counts[b] rows for each row b, which share the full pages of row b;
@@ -709,9 +752,8 @@ class PagedRaggedCache(RaggedCache):
         self.pages.owned.zero_()
         self.pages.shared.zero_()
         self.set_lengths(torch.zeros(self.batch_size, dtype=torch.long))
-        starts = torch.tensor([0] + counts).cumsum(0)
-        new.prefix = (starts.to(self.device, torch.int32),
-                      (host // PAGE).to(self.device, torch.int32))
+        ends = torch.tensor(counts).cumsum(0).tolist()
+        new._set_groups(list(zip([0] + ends[:-1], ends, (host // PAGE).tolist())))
         return new
 
     def set_lengths(self, lengths):
@@ -735,6 +777,9 @@ class PagedRaggedCache(RaggedCache):
             self._err.zero_()
             if e & 4:
                 raise L.SpecdecError("KV page pool exhausted")
+            if e & 16:
+                raise RuntimeError("PagedRaggedCache: a forked row was rolled back into the pages "
+                                   "it shares and would write them")
             if e & 2:
                 raise RuntimeError("PagedRaggedCache: a slot was written without a page "
                                    "(reserve() before the forward)")

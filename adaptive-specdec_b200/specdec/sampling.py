@@ -272,19 +272,21 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
     a +inf, or with nothing above -inf, has NaN log-probabilities and entropy.
     One pass over the logits (sd_token_logprobs), no host synchronisation.
     """
-    dev, shape, V = logits.device, ids.shape, logits.shape[-1] if logits.dim() else 0
-    if dev.type != "cuda" or ids.device != dev:
+    dev, shape, dims = logits.device, ids.shape, logits.dim()
+    if not logits.is_cuda or ids.device != dev:
         L.require_cuda(logits, ids)
         raise L.SpecdecError("logits and ids must be on one device")
-    if logits.dim() < 1 or shape != logits.shape[:-1]:
+    if dims < 1 or shape != logits.shape[:-1]:
         raise L.SpecdecError(f"token_logprobs needs one id per row: logits {tuple(logits.shape)}, "
                              f"ids {tuple(shape)}")
     if ids.dtype != torch.long:
         if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
             raise L.SpecdecError(f"ids must be integers, got {ids.dtype}")
         ids = ids.long()
-    code = L.dtype_code(logits.dtype)
-    n, T = int(top_n), float(temperature)
+    if torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return token_logprobs(logits, ids, temperature, top_n)
+    code, V, n, T = L.dtype_code(logits.dtype), logits.shape[-1], int(top_n), float(temperature)
     if not 1 <= V <= LOGPROBS_MAX_V:
         raise L.SpecdecError(f"the vocabulary must have 1 to {LOGPROBS_MAX_V} entries, got {V}")
     if not 0 <= n <= min(V, TOP_N_MAX):
@@ -292,16 +294,14 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
     if not 1e-6 <= T <= 1e6:
         raise L.SpecdecError(f"temperature must be between 1e-6 and 1e6, got {temperature}")
     # rows (b, l) with strides (bs, ps), their ids with stride ids_bs over b
-    dims = logits.dim()
     if V == 1:
         logits = logits.contiguous()
     x = _vocab_rows(logits, "logits")
     if dims == 2:
-        B, Lr, bs, ps = shape[0], 1, x.stride(0), 0
-        ids_bs = ids.stride(0)
+        B, Lr, bs, ps, ids_bs = shape[0], 1, x.stride(0), 0, ids.stride(0)
     elif dims == 3:
-        B, Lr, bs, ps = shape[0], shape[1], x.stride(0), x.stride(1)
-        if ids.stride(1) != 1 and Lr > 1:
+        (B, Lr), (bs, ps, _) = shape, x.stride()
+        if Lr > 1 and ids.stride(1) != 1:
             ids = ids.contiguous()
         ids_bs = ids.stride(0)
     else:
@@ -310,14 +310,20 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
             x = x.contiguous()
         ids = ids.reshape(-1)
         B, Lr, bs, ps, ids_bs = x.shape[0], 1, x.stride(0), 0, ids.stride(0)
-    with L.on_device(dev):
+    if dims in (2, 3) and ids.is_contiguous():
+        # (empty_like costs half of an empty with a torch.Size)
+        logprob = torch.empty_like(ids, dtype=torch.float32)
+        rank, entropy = torch.empty_like(ids), torch.empty_like(logprob)
+    else:
         logprob = torch.empty(shape, dtype=torch.float32, device=dev)
         rank = torch.empty(shape, dtype=torch.long, device=dev)
         entropy = torch.empty(shape, dtype=torch.float32, device=dev)
-        top_ids = torch.empty(shape + (n,), dtype=torch.long, device=dev) if n else None
-        top_lp = torch.empty(shape + (n,), dtype=torch.float32, device=dev) if n else None
-        L.check(L.lib().sd_token_logprobs(
-            x.data_ptr(), bs, ps, code, ids.data_ptr(), ids_bs, B, Lr, V, T, n, logprob.data_ptr(),
-            rank.data_ptr(), entropy.data_ptr(), L.address(top_ids), L.address(top_lp),
-            L.stream_of(dev)), "token_logprobs")
+    top_ids = top_lp = None
+    if n:
+        top_ids = torch.empty([*shape, n], dtype=torch.long, device=dev)
+        top_lp = torch.empty_like(top_ids, dtype=torch.float32)
+    L.check(L.lib().sd_token_logprobs(
+        x.data_ptr(), bs, ps, code, ids.data_ptr(), ids_bs, B, Lr, V, T, n, logprob.data_ptr(),
+        rank.data_ptr(), entropy.data_ptr(), L.address(top_ids), L.address(top_lp),
+        L.stream_of(dev)), "token_logprobs")
     return TokenLogprobs(logprob, rank, entropy, top_ids, top_lp)

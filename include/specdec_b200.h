@@ -257,25 +257,29 @@ int sd_kv_append_paged(void* kpool, void* vpool, const void* new_k, const void* 
  *   slots[starts[b] + i] = page * SD_KV_PAGE + offset
  * of cache position lengths[b] + i; slots behind the last token are -1.
  * With slots NULL there is no slot map and max_tokens does not count.
- * Rows keep the pages they have: nothing is given back.
+ * Rows keep the pages they have: nothing is given back.  With floor_pages
+ * (may be NULL) row b takes no new token in its first floor_pages[b] pages: a
+ * row of a forked cache must not write what its neighbours read.
  *
  * sd_pages_trim gives back every row's pages past max(ceil(lengths[b] /
  * SD_KV_PAGE), shared[b]), so that a trim after a reserve restores the stack.
  *
  * A call that cannot serve every row changes nothing and sets bits of *err:
  * CAPACITY (a row past W pages, a negative length or count), EXHAUSTED (too
- * few free pages), SLOTS (more new tokens than max_tokens); starts is still
- * written and every slot is -1.  Calls on one table are stream ordered.
+ * few free pages), SLOTS (more new tokens than max_tokens), SHARED (a new
+ * token below floor_pages); starts is still written and every slot is -1.  Calls on one table are stream ordered.
  */
 #define SD_PAGES_ERR_CAPACITY 1
 #define SD_PAGES_ERR_EXHAUSTED 4
 #define SD_PAGES_ERR_SLOTS 8
+#define SD_PAGES_ERR_SHARED 16
 size_t sd_pages_workspace_bytes(int B);
 int sd_pages_reserve(int32_t* block_table, int bt_stride, int W, int32_t* owned,
                      const int32_t* free_stack, int n_pages, int32_t* n_free,
-                     const int64_t* lengths, const int64_t* new_tokens, int64_t new_each, int B,
-                     int64_t* slots, int64_t max_tokens, int32_t* starts, int* err,
-                     void* workspace, size_t workspace_bytes, void* stream);
+                     const int64_t* lengths, const int64_t* new_tokens, int64_t new_each,
+                     const int32_t* floor_pages, int B, int64_t* slots, int64_t max_tokens,
+                     int32_t* starts, int* err, void* workspace, size_t workspace_bytes,
+                     void* stream);
 int sd_pages_trim(int32_t* block_table, int bt_stride, int W, int32_t* owned,
                   const int32_t* shared, int32_t* free_stack, int n_pages, int32_t* n_free,
                   const int64_t* lengths, int B, int* err, void* stream);

@@ -187,6 +187,45 @@ def test_a_trim_of_more_pages_than_the_pool_has_changes_nothing():
 
 
 @gpu
+@pytest.mark.parametrize("field,value", [("n_free", 9), ("n_free", -1), ("owned", -1)])
+def test_a_broken_table_hands_out_nothing(field, value):
+    t = DevicePageTable(2, 3, 8, DEV)
+    getattr(t, field).fill_(value)
+    before = [x.clone() for x in (t.block_table, t.owned, t.free, t.n_free)]
+    slots, _ = t.reserve(_lens([0, 0]), 5)
+    assert int(t.err) == 1 and bool((slots == -1).all())
+    if field == "n_free":
+        t.trim(_lens([0, 0]))
+    assert all(torch.equal(a, b) for a, b in zip(before, (t.block_table, t.owned, t.free, t.n_free)))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 100])                   # one launch, two launches
+def test_a_floor_of_pages_takes_no_new_tokens(rows):
+    t = DevicePageTable(rows, 3, 3 * rows + 1, DEV)
+    lens, floor = [PAGE] * rows, torch.zeros(rows, dtype=torch.int32, device=DEV)
+    t.reserve(_lens(lens), 0, slot_map=False)
+    floor[rows - 1] = 2
+    lens[rows - 1] = 2 * PAGE - 1
+    before = [x.clone() for x in (t.block_table, t.owned, t.n_free)]
+    slots, _ = t.reserve(_lens(lens), 2, floor=floor)
+    assert int(t.err) == 16 and bool((slots == -1).all())
+    assert all(torch.equal(a, b) for a, b in zip(before, (t.block_table, t.owned, t.n_free)))
+    with pytest.raises(RuntimeError, match="floor"):
+        t.check_errors()
+    new = [2] * (rows - 1) + [0]                             # nothing new in the row: no error
+    t.reserve(_lens(lens), _lens(new), max_tokens=2 * rows, floor=floor)
+    lens[rows - 1] = 2 * PAGE
+    slots, _ = t.reserve(_lens(lens), 2, floor=floor)
+    t.check_errors()
+    assert bool((slots >= 0).all())
+    with pytest.raises(L.SpecdecError):
+        t.reserve(_lens(lens), 2, floor=floor.long())
+    with pytest.raises(L.SpecdecError):
+        t.reserve(_lens(lens), 2, floor=floor[:1])
+
+
+@gpu
 def test_captured_rounds_follow_the_device_lengths():
     """trim and reserve in a graph, replayed while the lengths move."""
     B, W, n = 16, 10, 200
@@ -247,6 +286,8 @@ def test_refusals():
     with pytest.raises(L.SpecdecError):
         t.reserve(_lens([0, 0, 0]), -1)
     with pytest.raises(L.SpecdecError):
+        t.reserve(_lens([0, 0, 0]), 1 << 64, slot_map=False)
+    with pytest.raises(L.SpecdecError):
         t.reserve(torch.zeros(3, dtype=torch.long), 1)
     with pytest.raises(L.SpecdecError):
         DevicePageTable(3, 4, 1, DEV)
@@ -271,8 +312,8 @@ def test_arguments_are_checked_before_any_launch():
 
     def reserve(bt=d, stride=4, W=4, owned=d, pages=20, lens=d, each=1, B=3, slots=d, room=3, ws=d,
                 nws=1 << 16):
-        return lib.sd_pages_reserve(bt, stride, W, owned, d, pages, d, lens, n, each, B, slots, room,
-                                    d, d, ws, nws, n)
+        return lib.sd_pages_reserve(bt, stride, W, owned, d, pages, d, lens, n, each, n, B, slots,
+                                    room, d, d, ws, nws, n)
     assert reserve(B=0) == 0
     assert reserve(B=-1) == -22 and reserve(bt=n) == -22 and reserve(lens=n) == -22
     assert reserve(W=0) == -22 and reserve(stride=3) == -22 and reserve(pages=0) == -22

@@ -75,7 +75,8 @@ def test_fork_shares_full_pages_and_copies_the_last():
     f = c.fork([3, 1, 2, 4])
     src = [0] * 3 + [1] + [2] * 2 + [3] * 4
     assert f.lengths.tolist() == [lens[s] for s in src]
-    assert f.prefix[0].tolist() == [0, 3, 4, 6, 10] and f.prefix[1].tolist() == [0, 2, 1, 2]
+    assert f.prefix[0].tolist() == [0, 3, 4, 6, 10] + [10] * 6
+    assert f.prefix[1].tolist() == [0, 2, 1, 2] + [0] * 6
     for l, w in zip(f.layers, want):
         for pool, ww in zip((l.keys, l.values), w):
             got = A.gather_pages(pool, f.block_table, 512)
@@ -112,15 +113,59 @@ def test_forked_rows_attend_like_unforked_ones():
     f.reserve(4)
     k = torch.randn(17, 2, 4, 128, device=DEV).bfloat16()
     f.layers[0].update(k, k)
-    q = torch.randn(17, 8, 4, 128, device=DEV).bfloat16()
-    got = A.prefix_attention(q, f.layers[0].keys, f.layers[0].values, f.lengths, f.block_table,
-                             *f.prefix).float()
-    want = A.verify_attention(q, f.layers[0].keys, f.layers[0].values, f.lengths,
-                              block_table=f.block_table).float()
-    mag = A.verify_attention(q, f.layers[0].keys, f.layers[0].values.abs(), f.lengths,
-                             block_table=f.block_table).float()
+    _same_attention(f, 4, 1)
+
+
+def _same_attention(f, qlen, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    B = f.batch_size
+    q = torch.randn(B, 8, qlen, 128, generator=g, device=DEV).bfloat16()
+    k, v = f.layers[0].keys, f.layers[0].values
+    got = A.prefix_attention(q, k, v, f.lengths, f.block_table, *f.prefix).float()
+    want = A.verify_attention(q, k, v, f.lengths, block_table=f.block_table).float()
+    mag = A.verify_attention(q, k, v.abs(), f.lengths, block_table=f.block_table).float()
     # weights and results are rounded to bf16 on both sides: 4 * 2^-8 of sum w |v|
     assert bool(((got - want).abs() <= 2.0 ** -6 * mag * 1.02).all())
+
+
+def test_released_rows_of_a_fork_leave_their_group():
+    """A released row (the group's first too) that grows again holds other
+    pages and other keys than the group it was in."""
+    c, _ = _filled([260, 300], 80, H=2)
+    f = c.fork([6, 4])
+    held = f.prefix[0].data_ptr(), f.prefix[1].data_ptr()
+    f.release([0, 3, 9])
+    assert f.prefix[0].tolist() == [0, 1, 3, 4, 6, 9, 10, 10, 10, 10, 10]
+    assert f.prefix[1].tolist() == [0, 2, 0, 2, 2, 0, 0, 0, 0, 0]
+    assert held == (f.prefix[0].data_ptr(), f.prefix[1].data_ptr())
+    g = torch.Generator(device=DEV).manual_seed(3)
+    for _ in range(3):                                 # past the 256 tokens that the others share
+        f.reserve(100)
+        k = torch.randn(10, 2, 100, 128, generator=g, device=DEV).bfloat16()
+        f.layers[0].update(k, k)
+        f.advance(100)
+    f.reserve(4)
+    k = torch.randn(10, 2, 4, 128, generator=g, device=DEV).bfloat16()
+    f.layers[0].update(k, k)
+    f.check_errors()
+    _same_attention(f, 4, 5)
+    f.release(range(10))
+    assert f.prefix[1].tolist() == [0] * 10 and f.pages.owned.tolist() == [0] * 10
+
+
+def test_a_forked_row_does_not_grow_inside_its_shared_pages():
+    c, _ = _filled([260, 300], 80, H=2)
+    f = c.fork([2, 2])
+    f.rollback([0, 5, 0, 44])                          # rows of 260, 255, 300 and 256 tokens
+    owned, free = f.pages.owned.clone(), f.free_pages
+    f.reserve(200)
+    assert torch.equal(f.pages.owned, owned) and f.free_pages == free
+    with pytest.raises(RuntimeError, match="shares"):
+        f.check_errors()
+    f.reserve(0)                                       # nothing is written
+    f.set_lengths(torch.tensor([260, 256, 300, 256]))
+    f.reserve(200)
+    f.check_errors()
 
 
 def test_fork_refusals():
