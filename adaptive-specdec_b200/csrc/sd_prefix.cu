@@ -41,6 +41,7 @@ constexpr int PX_MIN_SHARE = PX_OVH + 1;     // fewest schedule units per CTA: a
 constexpr float PX_HEADROOM = 8.f;           // lazy-rescale headroom of the running max (base 2)
 constexpr int PX_JOIN_THREADS = 256;
 constexpr int PX_JOIN_CTAS = 4;              // per SM
+constexpr int PX_JOIN_LOADS = 4;             // pieces of a row on their way at once
 constexpr int OW_STAGES = 3;                 // K + V tiles in flight (own ranges)
 constexpr int OW_THREADS = 192;              // warps 0-3 softmax, 4 TMA, 5 MMA
 constexpr int OW_OVH = 2;                    // schedule cost of a (row, kv head) beyond its pages
@@ -716,6 +717,9 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
   if (w == 4) {
     // ---------------- TMA producer: pages in segment order
     if (lane == 0) {
+      // a row's own pages are read by nobody else: they go first from L2, so that
+      // the shared ranges' partials stay in it for the join
+      const uint64_t once = tc_evict_first();
       uint32_t gi = 0;
       bool ok = true;
       while (more && ok) {
@@ -726,10 +730,10 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
           if (!ok) break;
           const int y = (int)kv_row(A, seg.b, seg.h, seg.s0 + i * SD_KV_PAGE);
           tc_expect_tx(&S.full[st], 4u * 128u * 128u);
-          tc_tma_2d(S.k[st][0], &tmk, 0, y, &S.full[st]);
-          tc_tma_2d(S.k[st][1], &tmk, 64, y, &S.full[st]);
-          tc_tma_2d(S.v[st][0], &tmv, 0, y, &S.full[st]);
-          tc_tma_2d(S.v[st][1], &tmv, 64, y, &S.full[st]);
+          tc_tma_2d(S.k[st][0], &tmk, 0, y, &S.full[st], once);
+          tc_tma_2d(S.k[st][1], &tmk, 64, y, &S.full[st], once);
+          tc_tma_2d(S.v[st][0], &tmv, 0, y, &S.full[st], once);
+          tc_tma_2d(S.v[st][1], &tmv, 64, y, &S.full[st], once);
         }
         if (ok) more = ow_next(seg, P) && ow_real(seg, P);
       }
@@ -1011,118 +1015,106 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// A CTA per (row, kv head, 8 query rows), a warp per query row: the pieces of the
-// shared range and of the row's own range, in piece order.
+// A warp per query row: the pieces of the shared range and of the row's own range,
+// in piece order.
 __global__ void __launch_bounds__(PX_JOIN_THREADS, PX_JOIN_CTAS) prefix_join_kernel(const PrefixParams P) {
   const AttnParams& A = P.A;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int chunks = (A.R + PX_JOIN_THREADS / 32 - 1) / (PX_JOIN_THREADS / 32);
-  const int bh = (int)(blockIdx.x / chunks), b = bh / A.Hkv, h = bh - b * A.Hkv;
-  // what the plan says (complete before the kernel in front of this one began)
-  const int g = P.rowgroup[b];
-  const int tb = A.rowpre[b + 1] - A.rowpre[b], RC = P.qc * A.group;
-  const int oshare = ow_share(A.rowpre[A.B] * A.Hkv), ou = A.rowpre[b] * A.Hkv + h * tb;
-  const int oc0 = (ou + OW_OVH) / oshare;
-  const int n2 = tb > 0 ? (ou + tb - 1) / oshare - oc0 + 1 : 0;
-  int rows = 0, f0 = 0, gtb = 0, gu = 0, gi = 0, gshare = 1;
+  const int lane = threadIdx.x & 31;
+  const int64_t q = (int64_t)blockIdx.x * (PX_JOIN_THREADS / 32) + (threadIdx.x >> 5);
+  if (q >= (int64_t)A.B * A.Hkv * A.R) return;
+  const int bh = (int)q / A.R, r = (int)q - bh * A.R, b = bh / A.Hkv, h = bh - b * A.Hkv;
+  // what the plan says (complete before the kernel in front of this one began):
+  // pieces [0, n1) are of the shared range, two per CTA where both tiles worked on
+  // the rows; [n1, np) of the row's own range.  Rows of partials in 32 bits: each
+  // is 512 bytes of memory.
+  const int g = P.rowgroup[b], pre = A.rowpre[b], tb = A.rowpre[b + 1] - pre;
+  const int RC = P.qc * A.group, oshare = ow_share(A.rowpre[A.B] * A.Hkv);
+  const int ou = pre * A.Hkv + h * tb, oc0 = (ou + OW_OVH) / oshare, jc = r / RC;
+  const int at2 = (jc * P.slots + bh + oc0) * RC + r - jc * RC;
+  int n1 = 0, dup = 0, at1 = 0;
   if (g >= 0) {
-    rows = P.g_rows[g] * A.R;
-    f0 = (b - P.g_row0[g]) * A.R;
-    gtb = P.g_pages[g] + PX_OVH;
-    const int np = (rows + PX_ROWS - 1) / PX_ROWS;
-    gu = P.g_unit[g] + h * np * gtb;
-    gi = P.g_item[g] + h * np;
-    gshare = px_share(P.g_unit[P.G]);
+    const int rows = P.g_rows[g] * A.R, gtb = P.g_pages[g] + PX_OVH;
+    const int gshare = px_share(P.g_unit[P.G]);
+    const int f = (b - P.g_row0[g]) * A.R + r, p = f / PX_ROWS;
+    const int it = h * ((rows + PX_ROWS - 1) / PX_ROWS) + p, u = P.g_unit[g] + it * gtb;
+    const int c0 = (u + PX_OVH) / gshare;
+    dup = rows - p * PX_ROWS <= PX_ROWS / 2;
+    n1 = ((u + gtb - 1) / gshare - c0 + 1) << dup;
+    at1 = (P.g_item[g] + it + c0) * PX_ROWS + f % PX_ROWS;
   }
+  const int np = n1 + (tb > 0 ? (ou + tb - 1) / oshare - oc0 + 1 : 0);
+  auto row_of = [&](int i) {
+    return i < n1 ? at1 + (i >> dup) * PX_ROWS + (dup & i) * (PX_ROWS / 2) : at2 + (i - n1) * RC;
+  };
+  // this lane's 4 columns of a partial row: in the shared range's tiles column
+  // chunk lane / 8, row, and the 16-byte chunk permuted by the row
+  float4 v[PX_JOIN_LOADS];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < PX_JOIN_LOADS; ++i) {
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i0 + i >= np) continue;
+      const int row = row_of(i0 + i), tr = row & 127;
+      const bool own = i0 + i >= n1;
+      const int64_t at = (int64_t)(own ? row : row - tr) * 32 +
+                         (own ? lane : ((lane >> 3) * 128 + tr) * 8 + ((lane & 7) ^ (tr & 7)));
+      v[i] = __ldcg(reinterpret_cast<const float4*>(own ? A.part_acc : P.pacc) + at);
+    }
+  };
+  auto ml_of = [&](int i) {
+    return __ldcg(reinterpret_cast<const float2*>(i < n1 ? P.pml : A.part_ml) + row_of(i));
+  };
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int status = *A.status;
-  const int r = (int)(blockIdx.x - bh * chunks) * (PX_JOIN_THREADS / 32) + w;
-  if (r < A.R) {
-    const int j = r / A.group, hq = h * A.group + r - j * A.group;
-    // pieces [0, n1): the shared range, two per CTA where both tiles worked on
-    // the rows; [n1, n1 + n2): the row's own range
-    int n1 = 0, dup = 0;
-    int64_t at1 = 0;                                 // row of the first piece's partial
-    if (g >= 0) {
-      const int f = f0 + r, p = f / PX_ROWS, u = gu + p * gtb;
-      const int c0 = (u + PX_OVH) / gshare;
-      dup = rows - p * PX_ROWS <= PX_ROWS / 2;
-      n1 = ((u + gtb - 1) / gshare - c0 + 1) << dup;
-      at1 = ((int64_t)gi + p + c0) * PX_ROWS + f % PX_ROWS;
+  load(0);                                           // on their way before their weights are known
+  float m = -CUDART_INF_F, l = 0.f, m0 = -CUDART_INF_F;        // per lane, then over the warp
+  bool nan = false;                                  // a NaN score leaves no maximum, but its sum
+  for (int i = lane; i < np; i += 32) {
+    const float2 ml = ml_of(i);
+    if (i == lane) m0 = ml.x;
+    nan |= ml.y != ml.y;
+    if (ml.x != -CUDART_INF_F) {
+      const float mn = fmaxf(m, ml.x);
+      l = (m == -CUDART_INF_F ? 0.f : l * ex2f(m - mn)) + ml.y * ex2f(ml.x - mn);
+      m = mn;
     }
-    const int jc = j / P.qc;
-    const int64_t at2 = ((int64_t)jc * P.slots + b * A.Hkv + h + oc0) * RC + r - jc * RC;
-    const int np = n1 + n2;
-    auto row_of = [&](int i) -> int64_t {
-      return i < n1 ? at1 + (int64_t)(i >> dup) * PX_ROWS + (dup & i) * (PX_ROWS / 2)
-                    : at2 + (int64_t)(i - n1) * RC;
-    };
-    // this lane's 4 columns of a partial row: in the shared range's tiles column
-    // chunk lane / 8, row, and the 16-byte chunk permuted by the row
-    auto acc_of = [&](int i) {
-      const int64_t row = row_of(i);
-      if (i >= n1) return reinterpret_cast<const float4*>(A.part_acc + row * PX_D) + lane;
-      const int tr = (int)(row & 127);
-      return reinterpret_cast<const float4*>(P.pacc + (row - tr) * PX_D) +
-             ((lane >> 3) * 128 + tr) * 8 + ((lane & 7) ^ (tr & 7));
-    };
-    // the first pieces' columns on their way before their weights are known
-    float4 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = i < np ? __ldcg(acc_of(i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-    float m = -CUDART_INF_F, l = 0.f, m0 = -CUDART_INF_F;      // per lane, then over the warp
-    bool nan = false;                                // a NaN score leaves no maximum, but its sum
-    for (int i = lane; i < np; i += 32) {
-      const float* ml = (i < n1 ? P.pml : A.part_ml) + row_of(i) * 2;
-      const float mi = __ldcg(ml), li = __ldcg(ml + 1);
-      if (i == lane) m0 = mi;
-      nan |= li != li;
-      if (mi != -CUDART_INF_F) {
-        const float mn = fmaxf(m, mi);
-        l = (m == -CUDART_INF_F ? 0.f : l * ex2f(m - mn)) + li * ex2f(mi - mn);
-        m = mn;
-      }
-    }
-    const float gm = warp_max(m);
-    const float L = warp_sum(m == -CUDART_INF_F ? 0.f : l * ex2f(m - gm));
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float f, const float4& x) {
-      if (f == 0.f) return;                          // nothing there (maybe never written)
-      a.x = fmaf(f, x.x, a.x); a.y = fmaf(f, x.y, a.y);
-      a.z = fmaf(f, x.z, a.z); a.w = fmaf(f, x.w, a.w);
-    };
-    const float w0 = m0 == -CUDART_INF_F ? 0.f : ex2f(m0 - gm);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) add(__shfl_sync(0xffffffffu, w0, i), v[i]);
-    for (int i0 = 4; i0 < np; i0 += 4) {
-      // four more at a time; lane q of the group holds piece i0 + q's weight
-      float fw = 0.f;
-      if (lane < 4 && i0 + lane < np) {
-        const float mi = __ldcg((i0 + lane < n1 ? P.pml : A.part_ml) + row_of(i0 + lane) * 2);
+  }
+  const float gm = warp_max(m);
+  const float L = warp_sum(m == -CUDART_INF_F ? 0.f : l * ex2f(m - gm));
+  float fw = m0 == -CUDART_INF_F ? 0.f : ex2f(m0 - gm);        // piece lane's weight
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int i0 = 0; i0 < np; i0 += PX_JOIN_LOADS) {
+    if (i0 > 0) {
+      load(i0);
+      if (i0 % 32 == 0) {
+        const float mi = i0 + lane < np ? ml_of(i0 + lane).x : -CUDART_INF_F;
         fw = mi == -CUDART_INF_F ? 0.f : ex2f(mi - gm);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = i0 + i < np ? __ldcg(acc_of(i0 + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) add(__shfl_sync(0xffffffffu, fw, i), v[i]);
     }
-    // a wait that gave up somewhere leaves partials unwritten: say so in the output
-    nan = __any_sync(0xffffffffu, nan);
-    const float il = nan || status ? CUDART_NAN_F : L == 0.f ? 0.f : 1.f / L;
-    const __nv_bfloat162 y0 = __floats2bfloat162_rn(a.x * il, a.y * il);
-    const __nv_bfloat162 y1 = __floats2bfloat162_rn(a.z * il, a.w * il);
-    __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(A.out) + b * A.obs + j * A.oqs +
-                         hq * A.ohs + 4 * lane;
-    if (A.out_vec4) {
-      uint2 pk;
-      pk.x = *reinterpret_cast<const uint32_t*>(&y0);
-      pk.y = *reinterpret_cast<const uint32_t*>(&y1);
-      *reinterpret_cast<uint2*>(dst) = pk;
-    } else {
-      dst[0] = y0.x; dst[1] = y0.y; dst[2] = y1.x; dst[3] = y1.y;
+#pragma unroll
+    for (int i = 0; i < PX_JOIN_LOADS; ++i) {
+      const float f = __shfl_sync(0xffffffffu, fw, (i0 & 31) + i);
+      if (f == 0.f) continue;                        // nothing there (maybe never written)
+      a.x = fmaf(f, v[i].x, a.x); a.y = fmaf(f, v[i].y, a.y);
+      a.z = fmaf(f, v[i].z, a.z); a.w = fmaf(f, v[i].w, a.w);
     }
+  }
+  // a wait that gave up somewhere leaves partials unwritten: say so in the output
+  nan = __any_sync(0xffffffffu, nan);
+  const float il = nan || status ? CUDART_NAN_F : L == 0.f ? 0.f : 1.f / L;
+  const int j = r / A.group, hq = h * A.group + r - j * A.group;
+  const __nv_bfloat162 y0 = __floats2bfloat162_rn(a.x * il, a.y * il);
+  const __nv_bfloat162 y1 = __floats2bfloat162_rn(a.z * il, a.w * il);
+  __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(A.out) + b * A.obs + j * A.oqs +
+                       hq * A.ohs + 4 * lane;
+  if (A.out_vec4) {
+    uint2 pk;
+    pk.x = *reinterpret_cast<const uint32_t*>(&y0);
+    pk.y = *reinterpret_cast<const uint32_t*>(&y1);
+    *reinterpret_cast<uint2*>(dst) = pk;
+  } else {
+    dst[0] = y0.x; dst[1] = y0.y; dst[2] = y1.x; dst[3] = y1.y;
   }
 }
 
@@ -1276,8 +1268,8 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   cfg.blockDim = dim3(OW_THREADS);
   cfg.dynamicSmemBytes = smo;
   if (cudaLaunchKernelEx(&cfg, own_tc_kernel, P, mk, mv, mq32) != cudaSuccess) return SD_ELAUNCH;
-  const int64_t per = PX_JOIN_THREADS / 32;
-  cfg.gridDim = dim3((unsigned)((int64_t)B * Hkv * ((R + per - 1) / per)));
+  const int64_t per = PX_JOIN_THREADS / 32;          // query rows of a CTA
+  cfg.gridDim = dim3((unsigned)((R * B * Hkv + per - 1) / per));
   cfg.blockDim = dim3(PX_JOIN_THREADS);
   cfg.dynamicSmemBytes = 0;
   if (cudaLaunchKernelEx(&cfg, prefix_join_kernel, P) != cudaSuccess) return SD_ELAUNCH;

@@ -156,6 +156,19 @@ __device__ __forceinline__ void tc_tma_2d(void* dst, const void* tmap, int x, in
                :: "r"(smem_addr(dst)), "l"(tmap), "r"(x), "r"(y), "r"(smem_addr(bar))
                : "memory");
 }
+// A cache policy for data that is read once, and a load under a policy
+__device__ __forceinline__ uint64_t tc_evict_first() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void tc_tma_2d(void* dst, const void* tmap, int x, int y,
+                                          unsigned long long* bar, uint64_t policy) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+               ".L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;"
+               :: "r"(smem_addr(dst)), "l"(tmap), "r"(x), "r"(y), "r"(smem_addr(bar)), "l"(policy)
+               : "memory");
+}
 #define TC_LD32(r, addr)                                                                        \
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,"    \
                "%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"  \
