@@ -628,7 +628,7 @@ struct OwSmem {
   alignas(1024) unsigned char k[OW_STAGES][2][128 * 128];    // [stage][64-col box][128 keys x 128 B]
   alignas(1024) unsigned char v[OW_STAGES][2][128 * 128];
   alignas(1024) unsigned char q[2][128 * 128];               // [64-col box][128 rows x 128 B]
-  alignas(8) unsigned long long full[OW_STAGES], empty[OW_STAGES];
+  alignas(8) unsigned long long full[OW_STAGES][2], empty[OW_STAGES][2];   // K, V
   // by stream and the stream's page parity (at most two phases of each are open)
   alignas(8) unsigned long long sfull[4][2], pfull[4][2], oready[4][2], qfull[4], fin;
   uint32_t tmem;
@@ -650,7 +650,7 @@ static_assert(sizeof(OwSmem) + 1024 <= 227 * 1024, "own-range attention shared m
 // pages of the next one, no reduction crosses a thread, and K and V are read
 // once whatever the number of query rows.  The idle lanes cost tensor time that
 // is not the bound: 1024 cycles a page against about 2800 for its 64 KB from HBM.
-// K and V of a page share a stage; slots behind a row's live keys that TMA
+// K leaves its slot when S is done, V when P . V is; slots behind a row's live keys that TMA
 // brings in are zeroed in V before P . V reads them (they may hold NaN).
 __global__ void __launch_bounds__(OW_THREADS, 1)
 own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CUtensorMap tmk,
@@ -679,10 +679,11 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
   for (int b = t; b < A.B; b += OW_THREADS)
     if (A.rowpre[b] * A.Hkv <= t0 && t0 < A.rowpre[b + 1] * A.Hkv) S.seg_b = b;
   if (t == 0) {
-    for (int i = 0; i < OW_STAGES; ++i) {
-      tc_bar_init(&S.full[i], 1);
-      tc_bar_init(&S.empty[i], 1);
-    }
+    for (int i = 0; i < OW_STAGES; ++i)
+      for (int kv = 0; kv < 2; ++kv) {
+        tc_bar_init(&S.full[i][kv], 1);
+        tc_bar_init(&S.empty[i][kv], 1);
+      }
     for (int i = 0; i < 4; ++i) {
       tc_bar_init(&S.qfull[i], nq);
       for (int p = 0; p < 2; ++p) {
@@ -720,123 +721,128 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
       // a row's own pages are read by nobody else: they go first from L2, so that
       // the shared ranges' partials stay in it for the join
       const uint64_t once = tc_evict_first();
-      uint32_t gi = 0;
+      uint32_t gi = 0, tiles = 0;                    // pages, K and V tiles asked for
       bool ok = true;
       while (more && ok) {
         for (int i = 0; i < seg.n && ok; ++i, ++gi) {
           const int st = (int)(gi % OW_STAGES);
-          if (gi >= (uint32_t)OW_STAGES)
-            ok = tc_wait(&S.empty[st], ((gi / OW_STAGES) - 1) & 1u, &S.abort_);
-          if (!ok) break;
           const int y = (int)kv_row(A, seg.b, seg.h, seg.s0 + i * SD_KV_PAGE);
-          tc_expect_tx(&S.full[st], 4u * 128u * 128u);
-          tc_tma_2d(S.k[st][0], &tmk, 0, y, &S.full[st], once);
-          tc_tma_2d(S.k[st][1], &tmk, 64, y, &S.full[st], once);
-          tc_tma_2d(S.v[st][0], &tmv, 0, y, &S.full[st], once);
-          tc_tma_2d(S.v[st][1], &tmv, 64, y, &S.full[st], once);
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv, ++tiles) {
+            if (gi >= (uint32_t)OW_STAGES)
+              ok = tc_wait(&S.empty[st][kv], ((gi / OW_STAGES) - 1) & 1u, &S.abort_);
+            if (!ok) break;
+            tc_expect_tx(&S.full[st][kv], 2u * 128u * 128u);
+            const void* map = kv ? (const void*)&tmv : (const void*)&tmk;
+            unsigned char* dst = kv ? S.v[st][0] : S.k[st][0];
+            tc_tma_2d(dst, map, 0, y, &S.full[st][kv], once);
+            tc_tma_2d(dst + 128 * 128, map, 64, y, &S.full[st][kv], once);
+          }
         }
         if (ok) more = ow_next(seg, P) && ow_real(seg, P);
       }
       if (!ok) {
         // let the copies already issued land before the CTA leaves
-        for (uint32_t q = gi > (uint32_t)OW_STAGES ? gi - OW_STAGES : 0u; q < gi; ++q) {
+        constexpr uint32_t RING = 2 * OW_STAGES;
+        for (uint32_t q = tiles > RING ? tiles - RING : 0u; q < tiles; ++q) {
           int dummy = 0;
-          tc_wait(&S.full[q % OW_STAGES], (q / OW_STAGES) & 1u, &dummy);
+          tc_wait(&S.full[q / 2 % OW_STAGES][q & 1], (q / RING) & 1u, &dummy);
         }
       }
     }
   } else if (w == 5) {
-    // ---------------- MMA issuer: S of page a and P . V of page c, each in page
-    // order, polled together; S(a) behind P . V(a - 2), whose P it overwrites
-    if (lane == 0) {
-      constexpr uint32_t ID1 = tc_idesc(128, 128, 0, 0);     // S = Q . K^T
-      constexpr uint32_t ID2 = tc_idesc(128, 128, 0, 1);     // O += P . V (V [key][d]: N-major)
-      OwSeg sa = seg, sc = seg;
-      bool ma = more, mc = more;
-      int ia = 0, ic = 0;                            // page of the segment
-      uint32_t a = 0, c = 0, ga = 0, gc = 0;         // pages and segments issued
-      uint32_t na[4] = {0u, 0u, 0u, 0u}, nc[4] = {0u, 0u, 0u, 0u};   // pages by stream
-      auto lanes = [&](uint32_t (&off)[4], uint32_t g) {
-        const int q0 = (int)(g % ns) * nq;
+    // ---------------- MMA issuer (the whole warp): S of page a and P . V of page c,
+    // each in page order, polled together; S(a) behind P . V(a - 2), whose P it
+    // overwrites
+    constexpr uint32_t ID1 = tc_idesc(128, 128, 0, 0);     // S = Q . K^T
+    constexpr uint32_t ID2 = tc_idesc(128, 128, 0, 1);     // O += P . V (V [key][d]: N-major)
+    const uint64_t dq = tc_desc(smem_addr(S.q[0]), 16, 1024, 2);
+    OwSeg sa = seg, sc = seg;
+    bool ma = more, mc = more;
+    int ia = 0, ic = 0;                            // page of the segment
+    uint32_t a = 0, c = 0, ga = 0, gc = 0;         // pages and segments issued
+    uint32_t na[4] = {0u, 0u, 0u, 0u}, nc[4] = {0u, 0u, 0u, 0u};   // pages by stream
+    auto lanes = [&](uint32_t (&off)[4], uint32_t g) {
+      const int q0 = (int)(g % ns) * nq;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) off[i] = i >= q0 && i < q0 + nq ? 0u : 0xFFFFFFFFu;
-      };
-      auto count = [&](uint32_t (&n)[4], int s, bool step) -> uint32_t {
-        uint32_t v = 0;
+      for (int i = 0; i < 4; ++i) off[i] = i >= q0 && i < q0 + nq ? 0u : 0xFFFFFFFFu;
+    };
+    auto count = [&](uint32_t (&n)[4], int s, bool step) -> uint32_t {
+      uint32_t v = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i == s) {
-            v = n[i];
-            if (step) ++n[i];
-          }
-        return v;
-      };
-      long long idle0 = clock64();
-      while (mc) {
-        bool progressed = false;
-        if (ma && a < c + 2) {
-          const int st = (int)(a % OW_STAGES), s = (int)(ga % ns);
-          if (tc_test(&S.full[st], (a / OW_STAGES) & 1u) &&
-              (ia != 0 || tc_test(&S.qfull[s], (ga / ns) & 1u))) {
-            tc_fence_after();
-            uint32_t off[4];
-            lanes(off, ga);
-            const uint32_t n = count(na, s, true);
-            const uint32_t k0 = smem_addr(S.k[st][0]), k1 = smem_addr(S.k[st][1]);
-            const uint32_t q0 = smem_addr(S.q[0]), q1 = smem_addr(S.q[1]);
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-              const uint32_t ko = (uint32_t)(ks & 3) * 32u;
-              tc_mma_lanes(tm + 128u * (a & 1u), tc_desc((ks < 4 ? q0 : q1) + ko, 16, 1024, 2),
-                           tc_desc((ks < 4 ? k0 : k1) + ko, 16, 1024, 2), ID1, off, ks > 0 ? 1 : 0);
-            }
-            tc_commit(&S.sfull[s][n & 1u]);
-            ++a;
-            if (++ia == sa.n) {
-              ia = 0;
-              ++ga;
-              ma = ow_next(sa, P) && ow_real(sa, P);
-            }
-            progressed = true;
-          }
+      for (int i = 0; i < 4; ++i)
+        if (i == s) {
+          v = n[i];
+          if (step) ++n[i];
         }
-        if (c < a) {
-          const int st = (int)(c % OW_STAGES), s = (int)(gc % ns);
-          const uint32_t n = count(nc, s, false);
-          if (tc_test(&S.pfull[s][n & 1u], (n >> 1) & 1u)) {
-            tc_fence_after();
-            uint32_t off[4];
-            lanes(off, gc);
-            count(nc, s, true);
-            const uint32_t va = smem_addr(S.v[st][0]);
+      return v;
+    };
+    long long idle0 = clock64();
+    while (mc) {
+      bool progressed = false;
+      if (ma && a < c + 2) {
+        const int st = (int)(a % OW_STAGES), s = (int)(ga % ns);
+        if (__all_sync(0xffffffffu, tc_test(&S.full[st][0], (a / OW_STAGES) & 1u) &&
+                                        (ia != 0 || tc_test(&S.qfull[s], (ga / ns) & 1u)))) {
+          tc_fence_after();
+          uint32_t off[4];
+          lanes(off, ga);
+          const uint32_t n = count(na, s, true);
+          const uint64_t dk = tc_desc(smem_addr(S.k[st][0]), 16, 1024, 2);
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-              tc_mma_ts_lanes(tm + 256u, tm + 128u * (c & 1u) + 8u * ks,
-                              tc_desc(va + ks * 2048, 16384, 1024, 2), ID2, off,
-                              (ic > 0 || ks > 0) ? 1 : 0);
-            tc_commit(&S.empty[st]);
-            tc_commit(&S.oready[s][n & 1u]);
-            ++c;
-            if (++ic == sc.n) {
-              ic = 0;
-              ++gc;
-              mc = ow_next(sc, P) && ow_real(sc, P);
-            }
-            progressed = true;
+          for (int ks = 0; ks < 8; ++ks) {           // 16 of 128 d: 32 B, the second box 16 KB on
+            const uint64_t o = (uint64_t)((ks & 3) * 2 + (ks >> 2) * 1024);
+            tc_mma_lanes_warp(tm + 128u * (a & 1u), dq + o, dk + o, ID1, off, ks > 0 ? 1 : 0);
           }
-        }
-        if (progressed) {
-          idle0 = clock64();
-        } else if (*reinterpret_cast<volatile int*>(&S.abort_) || clock64() - idle0 > TC_WAIT) {
-          *reinterpret_cast<volatile int*>(&S.abort_) = 1;
-          break;
+          tc_commit_warp(&S.sfull[s][n & 1u]);
+          tc_commit_warp(&S.empty[st][0]);
+          ++a;
+          if (++ia == sa.n) {
+            ia = 0;
+            ++ga;
+            ma = ow_next(sa, P) && ow_real(sa, P);
+          }
+          progressed = true;
         }
       }
-      // every MMA this thread issued has finished before the CTA leaves
-      tc_commit(&S.fin);
-      int dummy = 0;
-      tc_wait(&S.fin, 0u, &dummy);
+      if (c < a) {
+        const int st = (int)(c % OW_STAGES), s = (int)(gc % ns);
+        const uint32_t n = count(nc, s, false);
+        if (__all_sync(0xffffffffu, tc_test(&S.pfull[s][n & 1u], (n >> 1) & 1u) &&
+                                        tc_test(&S.full[st][1], (c / OW_STAGES) & 1u))) {
+          tc_fence_after();
+          uint32_t off[4];
+          lanes(off, gc);
+          count(nc, s, true);
+          const uint64_t dv = tc_desc(smem_addr(S.v[st][0]), 16384, 1024, 2);
+          const uint32_t pa = tm + 128u * (c & 1u);
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)             // 16 keys: 2 KB
+            tc_mma_ts_lanes_warp(tm + 256u, pa + 8u * ks, dv + (uint64_t)(ks * 128), ID2, off,
+                                 ic > 0 || ks > 0 ? 1 : 0);
+          tc_commit_warp(&S.empty[st][1]);
+          tc_commit_warp(&S.oready[s][n & 1u]);
+          ++c;
+          if (++ic == sc.n) {
+            ic = 0;
+            ++gc;
+            mc = ow_next(sc, P) && ow_real(sc, P);
+          }
+          progressed = true;
+        }
+      }
+      if (progressed) {
+        idle0 = clock64();
+      } else if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&S.abort_) ||
+                                             clock64() - idle0 > TC_WAIT)) {
+        *reinterpret_cast<volatile int*>(&S.abort_) = 1;
+        break;
+      }
     }
+    // every MMA this warp issued has finished before the CTA leaves
+    tc_commit_warp(&S.fin);
+    int dummy = 0;
+    tc_wait(&S.fin, 0u, &dummy);
   } else {
     // ---------------- softmax warps: lane quarter w, query row r of the chunk
     const int s = w / nq, r = (w % nq) * 32 + lane;
@@ -903,7 +909,9 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           // past the live window the page holds other slots, maybe NaN: their V to
           // zero, four rows of a 128-byte box at a time
-          const int st = (int)((g0 + (uint32_t)i) % OW_STAGES);
+          const uint32_t pg = g0 + (uint32_t)i, st = pg % OW_STAGES;
+          ok = __all_sync(0xffffffffu, tc_wait(&S.full[st][1], (pg / OW_STAGES) & 1u, &S.abort_));
+          if (!ok) break;
           for (int kr = cur.s1 - key0 + 4 * (w % nq) + (lane >> 3); kr < 128; kr += 4 * nq) {
             *reinterpret_cast<uint4*>(S.v[st][0] + kr * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
             *reinterpret_cast<uint4*>(S.v[st][1] + kr * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);

@@ -43,29 +43,6 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint3
                " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
                :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(acc) : "memory");
 }
-// D[lanes that `off` leaves on] (+)= A[shared] B[shared]: a set bit of off keeps
-// its accumulator lane (quarter i: bits of off[i]) as it is
-__device__ __forceinline__ void tc_mma_lanes(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
-                                             const uint32_t (&off)[4], int acc) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}"
-               :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(acc), "r"(off[0]), "r"(off[1]), "r"(off[2]),
-                  "r"(off[3]) : "memory");
-}
-// The same with A in tensor memory
-__device__ __forceinline__ void tc_mma_ts_lanes(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
-                                                const uint32_t (&off)[4], int acc) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}"
-               :: "r"(d), "r"(a), "l"(b), "r"(id), "r"(acc), "r"(off[0]), "r"(off[1]), "r"(off[2]),
-                  "r"(off[3]) : "memory");
-}
-// D (+)= A[tensor memory] B[shared]
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, int acc) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-               :: "r"(d), "r"(a), "l"(b), "r"(id), "r"(acc) : "memory");
-}
 __device__ __forceinline__ void tc_commit(unsigned long long* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
                :: "r"(smem_addr(bar)) : "memory");
@@ -123,6 +100,23 @@ __device__ __forceinline__ void tc_mma_ts_warp(uint32_t d, uint32_t a, uint64_t 
   asm volatile("{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
                " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
                :: "r"(d), "r"(a), "l"(b), "r"(id), "r"(acc) : "memory");
+}
+// D[lanes that `off` leaves on] (+)= A[shared] B[shared]: a set bit of off keeps
+// its accumulator lane (quarter i: bits of off[i]) as it is
+__device__ __forceinline__ void tc_mma_lanes_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                                  const uint32_t (&off)[4], int acc) {
+  asm volatile("{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}"
+               :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(acc), "r"(off[0]), "r"(off[1]), "r"(off[2]),
+                  "r"(off[3]) : "memory");
+}
+// The same with A in tensor memory
+__device__ __forceinline__ void tc_mma_ts_lanes_warp(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
+                                                     const uint32_t (&off)[4], int acc) {
+  asm volatile("{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}"
+               :: "r"(d), "r"(a), "l"(b), "r"(id), "r"(acc), "r"(off[0]), "r"(off[1]), "r"(off[2]),
+                  "r"(off[3]) : "memory");
 }
 __device__ __forceinline__ void tc_commit_warp(unsigned long long* bar) {
   asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
