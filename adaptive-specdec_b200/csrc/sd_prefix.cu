@@ -68,8 +68,8 @@ struct PrefixParams {
 };
 
 // The items of a group: (kv head, 256 query rows), kv head outer.
-__device__ __forceinline__ int px_pairs(const PrefixParams& P, int g) {
-  return (P.g_rows[g] * P.A.R + PX_ROWS - 1) / PX_ROWS;
+__device__ __forceinline__ int px_pairs(const PrefixParams& P, int rows) {
+  return (rows * P.A.R + PX_ROWS - 1) / PX_ROWS;
 }
 __device__ __forceinline__ int px_share(int total) {
   return max(PX_MIN_SHARE, (total + PX_CTAS - 1) / PX_CTAS);
@@ -171,22 +171,25 @@ __global__ void __launch_bounds__(PX_PLAN_THREADS) prefix_plan_kernel(const Pref
 // A CTA's run of schedule units as segments of items, walked identically by
 // every role.
 struct PxSeg {
-  int g, h, p, np, tb, off, tt, t1, ncost, j0, j1;   // pages [j0, j1) of the segment
+  int g, rows, h, p, np, tb, off, tt, t1, ncost, j0, j1;     // pages [j0, j1) of the segment
   bool dup;                                          // one tile of rows: both tiles work on it
 };
 __device__ __forceinline__ void px_item(PxSeg& s, const PrefixParams& P) {
-  s.dup = P.g_rows[s.g] * P.A.R - s.p * PX_ROWS <= PX_ROWS / 2;
+  s.dup = s.rows * P.A.R - s.p * PX_ROWS <= PX_ROWS / 2;
 }
 __device__ __forceinline__ void px_bounds(PxSeg& s) {
   s.ncost = min(s.tb - s.off, s.t1 - s.tt);
   s.j0 = max(s.off, PX_OVH) - PX_OVH;
   s.j1 = max(s.off + s.ncost - PX_OVH, s.j0);
 }
-__device__ __forceinline__ void px_init(PxSeg& s, const PrefixParams& P, int g, int t0, int t1) {
-  s.g = g;
-  s.np = px_pairs(P, g);
-  s.tb = P.g_pages[g] + PX_OVH;
-  const int u = t0 - P.g_unit[g], it = u / s.tb;
+// first: the group's index, its first unit, its rows and pages
+__device__ __forceinline__ void px_init(PxSeg& s, const PrefixParams& P, const int (&first)[4], int t0,
+                                        int t1) {
+  s.g = first[0];
+  s.rows = first[2];
+  s.np = px_pairs(P, s.rows);
+  s.tb = first[3] + PX_OVH;
+  const int u = t0 - first[1], it = u / s.tb;
   s.off = u % s.tb;
   s.h = it / s.np;
   s.p = it % s.np;
@@ -204,7 +207,8 @@ __device__ __forceinline__ bool px_next(PxSeg& s, const PrefixParams& P) {
     if (++s.h == P.A.Hkv) {
       s.h = 0;
       do { ++s.g; } while (P.g_pages[s.g] == 0);     // units remain, so a sharing group follows
-      s.np = px_pairs(P, s.g);
+      s.rows = P.g_rows[s.g];
+      s.np = px_pairs(P, s.rows);
       s.tb = P.g_pages[s.g] + PX_OVH;
     }
   }
@@ -219,7 +223,7 @@ struct PxSmem {
   alignas(128) unsigned char out[8][32 * 128];               // a warp's 32 rows x 32 floats of O
   alignas(8) unsigned long long sfull[2], pfull[2], oready[2], qfull[2], fin;
   uint32_t tmem;
-  int seg_g;
+  int first[4];                                              // the CTA's first group: g, unit, rows, pages
   int abort_;
 };
 static_assert(sizeof(PxSmem) + 1024 <= 227 * 1024, "prefix attention shared memory");
@@ -303,8 +307,15 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
   const int total = P.g_unit[P.G];
   const int share = px_share(total);
   const int t0 = (int)blockIdx.x * share, t1 = min(total, t0 + share);
-  for (int g = t; g < P.G; g += PX_THREADS)
-    if (P.g_unit[g] <= t0 && t0 < P.g_unit[g + 1]) S.seg_g = g;
+  for (int g = t; g < P.G; g += PX_THREADS) {
+    const int u0 = P.g_unit[g], u1 = P.g_unit[g + 1], rows = P.g_rows[g], pages = P.g_pages[g];
+    if (u0 <= t0 && t0 < u1) {
+      S.first[0] = g;
+      S.first[1] = u0;
+      S.first[2] = rows;
+      S.first[3] = pages;
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -316,7 +327,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
     return;
   }
   PxSeg seg;
-  px_init(seg, P, S.seg_g, t0, t1);
+  px_init(seg, P, S.first, t0, t1);
 
   if (w >= 8) {
     if (w == 8 && lane == 0) {
@@ -595,14 +606,14 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
 // each (row, kv head)'s pages).
 struct OwSeg {
   int b, h, tb, off, tt, t1, ncost, n, s0, s1;       // n pages; keys [s0, s1)
+  int k0, kmax;                                      // the row's own range
 };
-__device__ __forceinline__ void ow_bounds(OwSeg& g, const PrefixParams& P) {
+__device__ __forceinline__ void ow_bounds(OwSeg& g) {
   g.ncost = min(g.tb - g.off, g.t1 - g.tt);
   const int r0 = max(g.off, OW_OVH) - OW_OVH, r1 = g.off + g.ncost - OW_OVH;
   g.n = max(r1 - r0, 0);
-  const int k0 = P.rowstart[g.b];
-  g.s0 = k0 + r0 * SD_KV_PAGE;
-  g.s1 = min(P.A.rowkmax[g.b], k0 + r1 * SD_KV_PAGE);
+  g.s0 = g.k0 + r0 * SD_KV_PAGE;
+  g.s1 = min(g.kmax, g.k0 + r1 * SD_KV_PAGE);
 }
 __device__ __forceinline__ bool ow_next(OwSeg& g, const PrefixParams& P) {
   const AttnParams& A = P.A;
@@ -613,8 +624,10 @@ __device__ __forceinline__ bool ow_next(OwSeg& g, const PrefixParams& P) {
     g.h = 0;
     do { ++g.b; } while (A.rowpre[g.b + 1] == A.rowpre[g.b]);   // units remain, so a row follows
     g.tb = A.rowpre[g.b + 1] - A.rowpre[g.b];
+    g.k0 = P.rowstart[g.b];
+    g.kmax = A.rowkmax[g.b];
   }
-  ow_bounds(g, P);
+  ow_bounds(g);
   return true;
 }
 // The current or next segment with pages; false when none is left.
@@ -632,7 +645,7 @@ struct OwSmem {
   // by stream and the stream's page parity (at most two phases of each are open)
   alignas(8) unsigned long long sfull[4][2], pfull[4][2], oready[4][2], qfull[4], fin;
   uint32_t tmem;
-  int seg_b;
+  int first[5];                                      // the CTA's first row: OwSeg's b, unit, tb, k0, kmax
   int abort_;
 };
 static_assert(sizeof(OwSmem) + 1024 <= 227 * 1024, "own-range attention shared memory");
@@ -665,6 +678,17 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
   // its own end stands for both.
   if (P.G == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // one round trip for all that the start needs: what the rows say is on its way
+  // with the total
+  int b = t, first[4] = {0, 0, 0, 0};                // rowpre, its next, k0, kmax
+  auto fetch = [&]() {
+    if (b >= A.B) return;
+    first[0] = A.rowpre[b];
+    first[1] = A.rowpre[b + 1];
+    first[2] = P.rowstart[b];
+    first[3] = A.rowkmax[b];
+  };
+  fetch();
   const int total = A.rowpre[A.B] * A.Hkv;
   const int share = ow_share(total);
   const int t0 = (int)blockIdx.x * share;
@@ -676,8 +700,14 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
   const int j0 = (int)blockIdx.y * P.qc;             // the chunk's first query
   const int R = min(P.qc, A.qlen - j0) * A.group;    // its query rows per kv head
   const int nq = P.nq, ns = 4 / nq;                  // quarters per segment, streams
-  for (int b = t; b < A.B; b += OW_THREADS)
-    if (A.rowpre[b] * A.Hkv <= t0 && t0 < A.rowpre[b + 1] * A.Hkv) S.seg_b = b;
+  for (; b < A.B; b += OW_THREADS, fetch())
+    if (first[0] * A.Hkv <= t0 && t0 < first[1] * A.Hkv) {
+      S.first[0] = b;
+      S.first[1] = first[0] * A.Hkv;
+      S.first[2] = first[1] - first[0];
+      S.first[3] = first[2];
+      S.first[4] = first[3];
+    }
   if (t == 0) {
     for (int i = 0; i < OW_STAGES; ++i)
       for (int kv = 0; kv < 2; ++kv) {
@@ -706,13 +736,15 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
   tc_fence_after();
   const uint32_t tm = S.tmem;                        // S0, S1 (128 columns each), O (128)
   OwSeg seg;
-  seg.b = S.seg_b;
-  seg.tb = A.rowpre[seg.b + 1] - A.rowpre[seg.b];
-  seg.h = (t0 - A.rowpre[seg.b] * A.Hkv) / seg.tb;
-  seg.off = (t0 - A.rowpre[seg.b] * A.Hkv) % seg.tb;
+  seg.b = S.first[0];
+  seg.tb = S.first[2];
+  seg.k0 = S.first[3];
+  seg.kmax = S.first[4];
+  seg.h = (t0 - S.first[1]) / seg.tb;
+  seg.off = (t0 - S.first[1]) % seg.tb;
   seg.tt = t0;
   seg.t1 = t1;
-  ow_bounds(seg, P);
+  ow_bounds(seg);
   bool more = ow_real(seg, P);
 
   if (w == 4) {
