@@ -18,7 +18,7 @@ INCLUDE = ROOT / "include"
 LIB = HERE / "libspecdec_b200.so"
 
 SOURCES = ["sd_sampling.cu", "sd_kvcache.cu", "sd_attention.cu", "sd_shard.cu", "sd_layers.cu",
-           "sd_logprobs.cu", "sd_pages.cu", "sd_prefix.cu"]
+           "sd_logprobs.cu", "sd_pages.cu", "sd_prefix.cu", "sd_prefix_rows.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-Xptxas", "-warn-spills"]

@@ -54,4 +54,7 @@ __device__ __forceinline__ int row_limit(const AttnParams& P, int b, int j) {
 // (boxes of box_rows rows x 64 columns, 128-byte swizzle)
 bool cache_map(CUtensorMap* map, const void* base, int64_t rows, int box_rows = SD_KV_PAGE);
 
+// sd_prefix_rows.cu: attention over a paged cache row by row, D <= 128
+int prefix_rows(const AttnParams& P, int dtype, cudaStream_t st);
+
 }  // namespace sd

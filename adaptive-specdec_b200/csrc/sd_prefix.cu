@@ -1159,8 +1159,7 @@ __global__ void __launch_bounds__(PX_JOIN_THREADS, PX_JOIN_CTAS) prefix_join_ker
 }
 
 // The shapes of the tensor-core path; every other shape reads each row's pages
-// by itself (its kernels are bound by their arithmetic, not by the bytes that
-// sharing saves).
+// by itself (bound by its arithmetic, not by the bytes that sharing saves).
 static bool px_fast(int dtype, int D, int group) {
   return dtype == SD_DTYPE_BF16 && D == PX_D && group <= 128;
 }
@@ -1201,8 +1200,7 @@ size_t sd_prefix_attn_workspace_bytes(int B, int G, int Hq, int Hkv, int D, int 
                                       int dtype) {
   if (B <= 0 || G < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || W <= 0 || qlen <= 0) return 0;
   if ((int64_t)W * SD_KV_PAGE > 0x7FFFFFFF) return 0;
-  if (!px_fast(dtype, D, Hq / Hkv))
-    return sd_verify_attn_workspace_bytes(B, Hq, Hkv, D, W * SD_KV_PAGE, qlen);
+  if (!px_fast(dtype, D, Hq / Hkv)) return 0;
   return px_layout(B, G, Hq, Hkv, qlen).bytes;
 }
 
@@ -1221,25 +1219,8 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   if (dtype != SD_DTYPE_BF16 && dtype != SD_DTYPE_F32) return SD_ENOTSUP;
   if ((int64_t)bt_stride * SD_KV_PAGE > 0x7FFFFFFF) return SD_ENOTSUP;
   const int group = Hq / Hkv;
-  if (!px_fast(dtype, D, group))
-    return sd_verify_attn_paged(q, qbs, qhs, qqs, kpool, vpool, block_table, bt_stride, npages,
-                                lengths, valid, B, Hq, Hkv, D, qlen, scale, out, obs, oqs, ohs,
-                                dtype, workspace, workspace_bytes, stream);
-  // 16-byte loads of q rows and TMA boxes of the pools
-  if ((reinterpret_cast<uintptr_t>(q) & 15) || qbs % 8 || qhs % 8 || qqs % 8 ||
-      (reinterpret_cast<uintptr_t>(kpool) & 15) || (reinterpret_cast<uintptr_t>(vpool) & 15))
-    return SD_EINVAL;
-  const int64_t rows = (int64_t)npages * Hkv * SD_KV_PAGE;
-  if (rows >= (int64_t)1 << 31) return SD_ENOTSUP;
-  // the schedules count units in 32 bits
   const int64_t R = (int64_t)qlen * group;
-  if (R * B * Hkv > 0x7FFFFFFF || (int64_t)B * Hkv * (bt_stride + OW_OVH) > 0x7FFFFFFF ||
-      (int64_t)Hkv * (B * R / PX_ROWS + G) * (bt_stride + PX_OVH) > 0x7FFFFFFF)
-    return SD_ENOTSUP;
-  const PxLayout L = px_layout(B, G, Hq, Hkv, qlen);
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < L.bytes)
-    return SD_ENOSPC;
-  char* ws = reinterpret_cast<char*>(workspace);
+  if (R > 0x7FFFFFFF) return SD_ENOTSUP;
   PrefixParams P = {};
   AttnParams& A = P.A;
   A.q = q; A.qbs = qbs; A.qhs = qhs; A.qqs = qqs;
@@ -1250,6 +1231,22 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   A.out_vec4 = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && obs % 4 == 0 && oqs % 4 == 0 &&
                ohs % 4 == 0;
   A.bt = block_table; A.bt_stride = bt_stride; A.npages = npages;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (!px_fast(dtype, D, group)) return prefix_rows(A, dtype, st);
+  // 16-byte loads of q rows and TMA boxes of the pools
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || qbs % 8 || qhs % 8 || qqs % 8 ||
+      (reinterpret_cast<uintptr_t>(kpool) & 15) || (reinterpret_cast<uintptr_t>(vpool) & 15))
+    return SD_EINVAL;
+  const int64_t rows = (int64_t)npages * Hkv * SD_KV_PAGE;
+  if (rows >= (int64_t)1 << 31) return SD_ENOTSUP;
+  // the schedules count units in 32 bits
+  if (R * B * Hkv > 0x7FFFFFFF || (int64_t)B * Hkv * (bt_stride + OW_OVH) > 0x7FFFFFFF ||
+      (int64_t)Hkv * (B * R / PX_ROWS + G) * (bt_stride + PX_OVH) > 0x7FFFFFFF)
+    return SD_ENOTSUP;
+  const PxLayout L = px_layout(B, G, Hq, Hkv, qlen);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < L.bytes)
+    return SD_ENOSPC;
+  char* ws = reinterpret_cast<char*>(workspace);
   P.qc = L.qc; P.nq = L.nq; P.slots = L.slots;
   P.starts = group_starts; P.pages = prefix_pages; P.G = G; P.max_items = L.max_items;
   int* in = reinterpret_cast<int*>(ws + L.ints);
@@ -1268,7 +1265,6 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   P.pml = reinterpret_cast<float*>(ws + L.ml);
   A.part_acc = reinterpret_cast<float*>(ws + L.sacc);
   A.part_ml = reinterpret_cast<float*>(ws + L.sml);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int64_t qrows = (int64_t)B * Hq * qlen;
   CUtensorMap mk, mv, mq, mq32;
   if (!cache_map(&mk, kpool, rows) || !cache_map(&mv, vpool, rows) ||

@@ -118,7 +118,10 @@ def prefix_attention(q, k_pool, v_pool, lengths, block_table, group_starts, pref
     prompt.  Their keys are read once for the group instead of once per row.
     The result is ``verify_attention``'s but for the order of the float32 sums.
     Both group arrays live on the device, so a captured call follows them.
-    bf16 heads of 128 share; other shapes are computed row by row.
+    bf16 heads of 128 share; other shapes (D <= 128) are computed row by row.
+    Slots that no query of a row sees may hold anything.  In the slots of this
+    step's own queries V has to be finite: a NaN there reaches the row's earlier
+    queries, too.
     """
     dev, dt = q.device, q.dtype
     if not q.is_cuda:

@@ -392,9 +392,9 @@ int sd_verify_attn_paged(const void* q, int64_t qbs, int64_t qhs, int64_t qqs,
  * computed from its own table alone.  Both arrays are device memory, so a
  * captured call follows them.
  * bf16 with D = 128 and Hq / Hkv <= 128 shares (q, kpool and vpool 16-byte
- * aligned, q strides multiples of 8); other shapes of sd_verify_attn_paged
- * are computed row by row.  scale > 0.  The workspace must be 256-byte aligned
- * and, as a call writes all it reads, needs no initialisation.  If a bounded
+ * aligned, q strides multiples of 8); fp32 and other shapes with D <= 128 are
+ * computed row by row, without a workspace.  scale > 0.  The workspace must be
+ * 256-byte aligned and, as a call writes all it reads, needs no initialisation.  If a bounded
  * wait inside the kernels gives up, the output is NaN.
  */
 size_t sd_prefix_attn_workspace_bytes(int B, int G, int Hq, int Hkv, int D, int W, int qlen,

@@ -10,7 +10,9 @@ Scores are float32 sums of 128 exact products, so a weight is off by at most
 (2^-22) and the float32 accumulation are far below.  So
 |out - exact| <= 2^-8 |exact| + (2^-8 + 2^-10) A.
 fp32 (CUDA-core path): the same 2^-10 for the scores bounds it; 2^-9 A leaves
-the exponential and the sums their part.
+the exponential and the sums their part.  bf16 of other head sizes takes that
+path too, with float32 weights: 2^-9 A and 2^-8 of the result's own rounding,
+within the bf16 bound above.
 """
 import ctypes
 import math
@@ -175,16 +177,57 @@ def test_matches_verify_attention():
     assert bool(((got - want).abs().cpu() <= 2 * (2.0 ** -7 + 2.0 ** -10) * mag).all())
 
 
+F32, BF16 = torch.float32, torch.bfloat16
+
+
 @gpu
-@pytest.mark.parametrize("D,dt", [(64, torch.float32), (128, torch.float32), (64, torch.bfloat16),
-                                  (8, torch.float32)])
+@pytest.mark.parametrize("D,dt", [(64, F32), (128, F32), (64, BF16), (8, F32), (1, F32), (33, F32),
+                                  (100, F32), (72, BF16), (30, BF16)])
 def test_other_shapes_row_by_row(D, dt):
-    _check(_case([3, 2], [1, 2], [5, 0, 130, 44, 17], 3, 8, 2, D=D, dt=dt, stale=0.0))
+    _check(_case([3, 2], [1, 2], [5, 0, 130, 44, 17], 3, 8, 2, D=D, dt=dt))
 
 
 @gpu
-def test_wide_head_groups_row_by_row():
-    _check(_case([2], [1], [5, 9], 1, 64, 1, stale=0.0))
+@pytest.mark.parametrize("hq,hkv,qlen,dt", [(8, 8, 1, F32), (6, 2, 7, F32), (4, 1, 40, F32),
+                                            (256, 1, 1, BF16), (64, 1, 1, BF16)])
+def test_rows_of_a_head_over_several_blocks(hq, hkv, qlen, dt):
+    _check(_case([2], [1], [5, 9], qlen, hq, hkv, dt=dt))
+
+
+@gpu
+@pytest.mark.parametrize("rows,suffix", [(1, 2500), (2, 31), (2, 2049), (40, 300), (1, 0)])
+def test_row_by_row_clusters(rows, suffix):
+    """One to eight CTAs on a row, more groups of keys than they have warps."""
+    _check(_case([], [], [suffix + 3 * b for b in range(rows)], 2, 4, 2, D=64, dt=F32, lone=rows,
+                 width=24))
+
+
+@gpu
+def test_row_by_row_masks_nan_and_repeats():
+    c = _case([3], [1], [100, 3, 250], 4, 4, 2, D=64, dt=F32)
+    _check(c, valid=[0, 5, 300])
+    _check(c, valid=[1, 128, 129], scale=0.5)
+    want = _run(c)
+    assert torch.equal(want, _run(c))
+    q = c["q"].clone()
+    q[1, 2, 3] = math.nan
+    got = _run(dict(c, q=q))
+    assert bool(got[1, 3, 2].isnan().all())
+    got[1, 3, 2] = want[1, 3, 2]
+    assert torch.equal(got, want)
+    q = torch.empty(3, 4, 4, 65, device=DEV)[..., 1:]        # rows off the 16-byte bounds
+    q.copy_(c["q"])
+    assert torch.equal(_run(dict(c, q=q)), want)
+    k = torch.empty(c["k"].numel() + 1, device=DEV)[1:].view(c["k"].shape)
+    k.copy_(c["k"])
+    _check(dict(c, k=k))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = _run(c)
+    c["lens"].add_(-3)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, _run(c)) and not torch.equal(out, want)
 
 
 @gpu
@@ -348,3 +391,4 @@ def test_arguments_are_checked_before_any_launch():
     assert call(ws=n) == -28 and call(nws=100) == -28 and call(ws=ctypes.c_void_p(4112)) == -28
     size = lib.sd_prefix_attn_workspace_bytes
     assert size(64, 1, 32, 8, 128, 66, 5, 2) > 0 and size(64, 1, 32, 7, 128, 66, 5, 2) == 0
+    assert size(64, 1, 32, 8, 64, 66, 5, 2) == 0 and call(D=136) == -95 and call(D=256, dtype=0) == -95

@@ -1,8 +1,9 @@
 """Several samples per prompt: the device page table, the forked cache, the
 shared-prefix attention and the token log-probabilities together.
 
-Cache comparisons are exact.  fp32 tiny models attend row by row on the CUDA
-cores whether rows share or not, so their greedy tokens are equal, too.  The
+Cache comparisons are exact.  fp32 tiny models attend row by row whether rows
+share or not, with the same float32 sums in another order (some 1e-6 of scale), so
+their greedy tokens are equal, too, unless two logits are that close.  The
 log-probability comparisons are between two fp32 forwards of the same 2-layer
 model (other batch sizes, or the engine's and a plain teacher-forced one): float32 rounding through
 about 10 dependent matrix products of widths up to 64 and logits of order 1 is
