@@ -16,6 +16,9 @@
 //                       256 query rows instead of once per row;
 //   own_tc_kernel       the rows' own pages, four rows at a time;
 //   prefix_join_kernel  merges the partials, in piece order, into the output.
+// Each is launched as a programmatic dependent of the one before.  64 rows of 5
+// queries, 32 / 8 heads, 64 shared pages and up to 1 K own keys: 91 us for the
+// call; kernel by kernel, with cold caches, 6 + 45 + 34 + 14.
 // A row whose first query does not see the whole shared range (an empty or a
 // padding row, a short cap) takes no part in it: its own range starts at 0, so
 // the shared range needs no mask and no row meets another row's masked keys.
@@ -269,7 +272,12 @@ __device__ __forceinline__ unsigned long long px_exp2(float a, float b) {
 // tiles (2072 of them MMAs): one issuer on a single thread 4950 (an issue gap of
 // 500 cycles at every wait); two such issuers, one per tile, 5400 (the tiles fall
 // into step: softmax, then tensor cores); half pages with S of N = 64, 4170 (an
-// MMA of N = 64 takes as long as one of N = 128); this form PX_CYCLES.
+// MMA of N = 64 takes as long as one of N = 128); this form 3550.  A tile's own
+// chain is what bounds it: 1900 cycles of softmax, then P . V and the next S with
+// their latencies.  Two warps per 32 rows, each with half of the keys, left the
+// softmax as long (1850: the pipes of the SM quarter are shared); weights and
+// maximum in one pass over S, 3600.  128 rows of 5 queries over 128 pages, 32 / 8
+// heads: 150 us, 1.15 PFLOP/s.
 // An item with rows for one tile only is worked on by both: tile 0 takes the
 // first, tile 1 the second half of every page's keys.
 __global__ void __launch_bounds__(PX_THREADS, 1)
@@ -519,8 +527,9 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
           for (int e = 0; e < 16; ++e) {
             float a, b;
             unpair(fma2(pair2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sl22, nm2), a, b);
-            // a part by the FMA pipe: the exponentials of a page take 2048
-            // cycles of the special-function units otherwise
+            // a quarter by the FMA pipe: the exponentials of a page take 2048
+            // cycles of the special-function units otherwise (a call of 101.3 us
+            // took 102.5 without, 103 with half of them there)
             const unsigned long long p2 = e % 4 == 1 ? px_exp2(a, b) : pair2(ex2f(a), ex2f(b));
             ls[e & 1] = add2(ls[e & 1], p2);
             unpair(p2, a, b);
@@ -662,9 +671,12 @@ static_assert(sizeof(OwSmem) + 1024 <= 227 * 1024, "own-range attention shared m
 // So a segment's start and end (Q, first maximum, partial out) overlap the
 // pages of the next one, no reduction crosses a thread, and K and V are read
 // once whatever the number of query rows.  The idle lanes cost tensor time that
-// is not the bound: 1024 cycles a page against about 2800 for its 64 KB from HBM.
-// K leaves its slot when S is done, V when P . V is; slots behind a row's live keys that TMA
-// brings in are zeroed in V before P . V reads them (they may hold NaN).
+// is not the bound: 1024 cycles a page against about 2600 for its 64 KB from HBM.
+// K leaves its slot when S is done, V when P . V is; slots behind a row's live
+// keys that TMA brings in are zeroed in V before P . V reads them (they may hold
+// NaN).  64 rows of 520 own keys, 8 heads (136 MB): 34 us, 4 TB/s; in its middle
+// a page takes 2130 cycles, the bandwidth of HBM, but the first three pages of a
+// CTA take 10 us (cold code and first loads), which so short a run does not hide.
 __global__ void __launch_bounds__(OW_THREADS, 1)
 own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CUtensorMap tmk,
               const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmq) {
@@ -1056,7 +1068,10 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
 }
 
 // A warp per query row: the pieces of the shared range and of the row's own range,
-// in piece order.
+// in piece order.  Bound by latency (plan, then the partials): 10240 rows of some 6
+// pieces (31 MB) in 6 us behind the own ranges, 14 from HBM.  Two rows per warp and
+// eight pieces on their way were slower (more code, cold, and spills), as were 6 or
+// 8 CTAs per SM.
 __global__ void __launch_bounds__(PX_JOIN_THREADS, PX_JOIN_CTAS) prefix_join_kernel(const PrefixParams P) {
   const AttnParams& A = P.A;
   const int lane = threadIdx.x & 31;
