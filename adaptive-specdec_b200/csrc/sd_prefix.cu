@@ -1186,7 +1186,9 @@ struct PxLayout {
 static PxLayout px_layout(int B, int G, int Hq, int Hkv, int qlen) {
   PxLayout L;
   const int group = Hq / Hkv, R = qlen * group;
-  L.max_items = (int)std::min<int64_t>((int64_t)Hkv * ((int64_t)B * R / PX_ROWS + G), 1 << 28);
+  // a group of two rows or more shares: no more than B / 2 of them
+  L.max_items = (int)std::min<int64_t>(
+      (int64_t)Hkv * ((int64_t)B * R / PX_ROWS + std::min(G, B / 2)), 1 << 28);
   L.qc = std::min(qlen, 128 / group);
   L.nq = L.qc * group <= 32 ? 1 : L.qc * group <= 64 ? 2 : 4;
   L.chunks = (qlen + L.qc - 1) / L.qc;
@@ -1259,6 +1261,7 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
       (int64_t)Hkv * (B * R / PX_ROWS + G) * (bt_stride + PX_OVH) > 0x7FFFFFFF)
     return SD_ENOTSUP;
   const PxLayout L = px_layout(B, G, Hq, Hkv, qlen);
+  if (L.chunks > 65535) return SD_ENOTSUP;           // a grid dimension
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < L.bytes)
     return SD_ENOSPC;
   char* ws = reinterpret_cast<char*>(workspace);

@@ -662,6 +662,8 @@ class PagedRaggedCache(RaggedCache):
         row itself leaves its group."""
         rows = [int(r) for r in rows]
         if self.device_pages:
+            if rows and not 0 <= min(rows) <= max(rows) < self.batch_size:
+                raise L.SpecdecError(f"rows must be in [0, {self.batch_size}), got {rows}")
             at = torch.tensor(rows, dtype=torch.long, device=self.device)
             keep = self.pages.owned.long() * PAGE
             keep[at] = 0
@@ -696,16 +698,32 @@ class PagedRaggedCache(RaggedCache):
         return out + ([(a, end)] if a < end else [])
 
     def _set_groups(self, groups):
-        """The groups (first row, end, shared pages) behind ``prefix``, whose
-        tensors have room for a group per row (groups behind the last are
-        empty) and keep their addresses: captured graphs follow a release."""
-        B, n = self.batch_size, len(groups)
-        self._groups = groups
-        starts = [g[0] for g in groups] + [B] * (B + 1 - n)
-        pages = [g[2] for g in groups] + [0] * (B - n)
+        """The groups (first row, end, shared pages) behind ``prefix``.  Its
+        tensors keep their size and addresses, so that captured graphs follow a
+        release: twice the first groups and one (groups behind the last are
+        empty).  Runs that share nothing are one group; past the room, the
+        groups that save least stop sharing."""
+        B = self.batch_size
         if self.prefix is None:
-            self.prefix = (torch.empty(B + 1, dtype=torch.int32, device=self.device),
-                           torch.empty(B, dtype=torch.int32, device=self.device))
+            room = min(B, 2 * len(groups) + 1)
+            self.prefix = (torch.empty(room + 1, dtype=torch.int32, device=self.device),
+                           torch.empty(room, dtype=torch.int32, device=self.device))
+        room = self.prefix[1].numel()
+        while True:
+            runs = []
+            for a, b, p in groups:
+                p = p if b - a > 1 else 0
+                if runs and p == 0 and runs[-1][2] == 0:
+                    runs[-1] = (runs[-1][0], b, 0)
+                else:
+                    runs.append((a, b, p))
+            if len(runs) <= room:
+                break
+            least = min((r for r in runs if r[2]), key=lambda r: (r[1] - r[0] - 1) * r[2])
+            groups = [(a, b, 0 if (a, b, p) == least else p) for a, b, p in runs]
+        self._groups, n = runs, len(runs)
+        starts = [r[0] for r in runs] + [B] * (room + 1 - n)
+        pages = [r[2] for r in runs] + [0] * (room - n)
         for t, v in zip(self.prefix, (starts, pages)):
             t.copy_(torch.tensor(v, dtype=torch.int32))
 
@@ -752,6 +770,7 @@ class PagedRaggedCache(RaggedCache):
         self.pages.owned.zero_()
         self.pages.shared.zero_()
         self.set_lengths(torch.zeros(self.batch_size, dtype=torch.long))
+        self.prefix = None
         ends = torch.tensor(counts).cumsum(0).tolist()
         new._set_groups(list(zip([0] + ends[:-1], ends, (host // PAGE).tolist())))
         return new
