@@ -12,7 +12,8 @@
 // the verify round give a token and its probability after top-k / top-p; a
 // caller that ranks samples needs the untruncated log-probabilities.
 //
-// One pass over the logits, one launch.  Clusters of 1, 2, 4 or 8 CTAs take
+// One pass over the logits, one launch.  (Small vocabularies: a warp per row, see
+// logp_warp_kernel.)  Clusters of 1, 2, 4 or 8 CTAs take
 // either a whole row per CTA or one row together, a part each: whole rows while
 // there is one for every SM, then parts, so that the SMs end together.  A CTA
 // streams its part's 16-byte
@@ -25,7 +26,7 @@
 // CTA, which joins them in part order.  No atomics reach a result: the list
 // below is filled in any order and then ranked by unique keys.
 //
-// Top n of a part without comparing every element: of the 32 maxima of 8
+// Top n of a part without comparing every element: of 32 to 64 maxima of up to 8
 // threads each, the n-th largest has at least n elements at or above it, and
 // few more; only threads whose maximum reaches it look through their units
 // again (from L2), a warp together.
@@ -53,9 +54,13 @@ constexpr int LP_SMS = 148;
 constexpr int LP_STEP = LP_THREADS * LP_UNITS;  // units per step of a CTA
 constexpr float LP_HEADROOM = 8.f;              // base 2
 constexpr int LP_LIST = 2048;                   // a part's flagged elements
+constexpr int LP_GROUPS = 64;                   // groups of threads behind the top n's threshold
 constexpr int LP_MAX_PARTS = 8;                 // CTAs of a cluster
+constexpr int LP_WARP_V = 1024;                 // largest vocabulary of a warp per row
+constexpr int LP_WLIST = 256;                   // its flagged elements
 static_assert(LP_MAX_PARTS * SD_TOPN_MAX <= LP_THREADS, "a thread per key of the join");
-static_assert(SD_TOPN_MAX <= 4 * LP_WARPS, "the n-th largest of the group maxima");
+static_assert(SD_TOPN_MAX <= LP_GROUPS / 2 && LP_THREADS / 8 >= LP_GROUPS / 2,
+              "the n-th largest of the group maxima");
 
 struct LpPart {
   float m, s, e;                                // max (base-2 units), sum 2^d, sum d 2^d
@@ -295,7 +300,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   unsigned long long* list = reinterpret_cast<unsigned long long*>(lp_smem);   // TOP only
   __shared__ float red_m[LP_WARPS], red_s[LP_WARPS], red_e[LP_WARPS];
   __shared__ int red_c[LP_WARPS];
-  __shared__ uint32_t group_k[4 * LP_WARPS];
+  __shared__ uint32_t group_k[LP_GROUPS];
   __shared__ unsigned long long red_k[LP_WARPS];
   __shared__ int n_list, counter;
   // of the cluster's first CTA: what every part found
@@ -415,12 +420,20 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   float bm = warp_max(nan ? -CUDART_INF_F : ms);
   if (lane == 0) red_m[w] = bm;
   const bool any = u0 + t < u1 || lone;              // this thread holds an element
+  int size = 8;
   if (TOP) {
-    // the maximum of 8 threads each
+    // the maximum of 8 threads each, of fewer when few hold a unit: at least 32
+    // groups that hold something, at most 64
+    while (size > 1 && u1 - u0 < 32 * size) size /= 2;
     uint32_t k = any ? lp_key(m) : 0u;
+    if (size == 8) {
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
-    if ((lane & 7) == 0) group_k[4 * w + (lane >> 3)] = k;
+      for (int o = 4; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+    } else {
+#pragma unroll 1
+      for (int o = size / 2; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+    }
+    if (t % size == 0 && t / size < LP_GROUPS) group_k[t / size] = k;
   }
   __syncthreads();
   bm = red_m[0];
@@ -441,10 +454,23 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   if (TOP) {
     // the largest group maximum with n group maxima at or above it
     const uint32_t mine = group_k[lane];
-    int above = 0;
+    uint32_t at_or_above = 0u;                       // a group maximum with n at or above it
+    if (size == 8) {
+      int above = 0;
 #pragma unroll
-    for (int q = 0; q < 4 * LP_WARPS; ++q) above += group_k[q] >= mine;
-    const uint32_t thr = max(__reduce_max_sync(0xffffffffu, above >= P.top ? mine : 0u), 1u);
+      for (int q = 0; q < LP_THREADS / 8; ++q) above += group_k[q] >= mine;
+      if (above >= P.top) at_or_above = mine;
+    } else {
+      const uint32_t mine2 = group_k[lane + 32];
+      int above = 0, above2 = 0;
+#pragma unroll 1
+      for (int q = 0; q < LP_GROUPS; ++q) {
+        above += group_k[q] >= mine;
+        above2 += group_k[q] >= mine2;
+      }
+      at_or_above = max(above >= P.top ? mine : 0u, above2 >= P.top ? mine2 : 0u);
+    }
+    const uint32_t thr = max(__reduce_max_sync(0xffffffffu, at_or_above), 1u);
     auto put = [&](uint32_t k, int idx) {
       const int at = atomicAdd(&n_list, 1);
       if (at < LP_LIST) list[at] = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)idx;
@@ -581,6 +607,124 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   }
 }
 
+__device__ __forceinline__ float lp_f(float x) { return x; }
+__device__ __forceinline__ float lp_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float lp_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ unsigned long long lp_entry(float x, int idx) {
+  return ((unsigned long long)lp_key(x) << 32) | (uint32_t)~(uint32_t)idx;
+}
+
+// Small vocabularies, up to 32 NE entries: a warp per row, the row in its
+// registers (entry 32 i + lane in x[i]).  Of 64 maxima, of the lanes' even and odd
+// entries, the n-th largest has at least n entries at or above it (some 45 for n =
+// 32): those go to the warp's list and are ranked there; when it is too short (flat
+// logits), the n largest one after the other.
+// Bound by the loads' latency and the list.
+template <typename T, int NE>
+__global__ void __launch_bounds__(LP_THREADS) logp_warp_kernel(const LpParams P, int64_t rows) {
+  __shared__ unsigned long long lists[LP_WARPS][LP_WLIST];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, V = P.V;
+  const int64_t r = (int64_t)blockIdx.x * LP_WARPS + w;
+  if (r >= rows) return;
+  const int64_t rb = r / P.L, rl = r - rb * P.L;
+  const T* row = reinterpret_cast<const T*>(P.x) + rb * P.bs + rl * P.ps;
+  const int64_t tok = P.ids[rb * P.ids_bs + rl];
+  float x[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int idx = 32 * i + lane;
+    x[i] = idx < V ? lp_f(row[idx]) : -CUDART_INF_F;
+  }
+  const bool have = tok >= 0 && tok < V;
+  const float xt = have ? lp_f(row[tok]) : CUDART_INF_F;
+  const uint32_t kt = lp_key(xt);
+  uint32_t mk[2] = {0u, 0u};                         // the largest keys of the even and odd i
+  int ahead = 0;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int idx = 32 * i + lane;
+    if (idx >= V) break;
+    const uint32_t k = lp_key(x[i]);
+    mk[i & 1] = max(mk[i & 1], k);
+    ahead += k > kt || (k == kt && idx <= tok);
+  }
+  ahead = warp_sum(ahead);
+  const uint32_t wk = __reduce_max_sync(0xffffffffu, max(mk[0], mk[1]));
+  const float m = lp_value(wk);                      // (a NaN's key: NaN)
+  const float rm = m * P.c;                          // the row's maximum, base-2 units
+  const bool finite = rm > -CUDART_INF_F && rm < CUDART_INF_F;
+  const float m0 = finite ? rm : 0.f;
+  float s0 = 0.f, s1 = 0.f, e0 = 0.f, e1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < NE; i += 2) {
+    const float a = fmaxf(fmaf(x[i], P.c, -m0), -256.f), b = fmaxf(fmaf(x[i + 1], P.c, -m0), -256.f);
+    const float pa = lp_ex2(a), pb = lp_ex2(b);
+    s0 += pa;
+    s1 += pb;
+    e0 = fmaf(a, pa, e0);
+    e1 = fmaf(b, pb, e1);
+  }
+  const float rs = warp_sum(s0 + s1), re = warp_sum(e0 + e1);
+  const float lz = log2f(rs);
+  // all -inf, +inf or NaN among them: as the formula, NaN
+  const double lse = finite ? (double)rm + (double)lz : CUDART_NAN;
+  if (lane == 0) {
+    const float h = 0.69314718055994531f * (lz - re / rs);
+    P.entropy[r] = !finite ? CUDART_NAN_F : h < 0.f ? 0.f : h;
+    P.rank[r] = have ? (int64_t)ahead : 0;
+    P.logprob[r] = have ? lp_final(xt, P.c, lse) : CUDART_NAN_F;
+  }
+  const int n = P.top;
+  if (n == 0) return;
+  unsigned long long* list = lists[w];
+  int above[2] = {0, 0};
+#pragma unroll 4
+  for (int q = 0; q < 32; ++q) {
+    const uint32_t a = __shfl_sync(0xffffffffu, mk[0], q), b = __shfl_sync(0xffffffffu, mk[1], q);
+    above[0] += (a >= mk[0]) + (b >= mk[0]);
+    above[1] += (a >= mk[1]) + (b >= mk[1]);
+  }
+  // (a group without an entry has the key 0; n <= V groups or 32 hold one)
+  const uint32_t thr = max(__reduce_max_sync(0xffffffffu, max(above[0] >= n ? mk[0] : 0u,
+                                                             above[1] >= n ? mk[1] : 0u)), 1u);
+  int cnt = 0;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    if (32 * i >= V) break;
+    const bool hit = 32 * i + lane < V && lp_key(x[i]) >= thr;
+    const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+    const int at = cnt + __popc(hits & ((1u << lane) - 1u));
+    if (hit && at < LP_WLIST) list[at] = lp_entry(x[i], 32 * i + lane);
+    cnt += __popc(hits);
+  }
+  auto put = [&](int rank, unsigned long long key) {
+    P.top_ids[r * n + rank] = (int64_t)(uint32_t)~(uint32_t)key;
+    P.top_lp[r * n + rank] = lp_final(lp_value((uint32_t)(key >> 32)), P.c, lse);
+  };
+  __syncwarp();
+  if (cnt <= LP_WLIST) {
+    for (int i = lane; i < cnt; i += 32) {
+      const unsigned long long key = list[i];
+      int rank = 0;
+      for (int j = 0; j < cnt; ++j) rank += list[j] > key;
+      if (rank < n) put(rank, key);
+    }
+    return;
+  }
+  unsigned long long last = ~0ULL;
+  for (int k = 0; k < n; ++k) {
+    unsigned long long best = 0ULL;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      if (32 * i + lane >= V) break;
+      const unsigned long long key = lp_entry(x[i], 32 * i + lane);
+      if (key < last && key > best) best = key;
+    }
+    last = warp_max(best);
+    if (lane == 0) put(k, last);
+  }
+}
+
 // How the rows are cut.  Up to one row per SM, every row is split, over as many
 // CTAs as fit the machine at once; beyond, whole rows while there is one for
 // every SM and the rest in halves, so that the SMs end together.  Measured
@@ -603,8 +747,24 @@ static LpPlan lp_plan(int64_t rows, int V, int dtype) {
   return p;
 }
 
+// Up to LP_WARP_V entries a warp takes a row: 4000 rows of 300 bf16 in 5.3 us (a CTA
+// each: 27.5), 4000 x 1000 with five alternatives 19 (58), 1000 x 1000 8.6 (18.8), one
+// row of 1000 7.6 (6.1).  Beyond, 64 entries in a thread's registers leave one CTA per
+// SM: 4000 x 2000 in 48 us against 45.
+template <typename T>
+static int launch_warps(const LpParams& P, cudaStream_t st) {
+  const int64_t rows = (int64_t)P.B * P.L, ctas = (rows + LP_WARPS - 1) / LP_WARPS;
+  if (ctas > 0x7FFFFFFF) return SD_ENOTSUP;
+  if (P.V <= 512)
+    logp_warp_kernel<T, 16><<<(unsigned)ctas, LP_THREADS, 0, st>>>(P, rows);
+  else
+    logp_warp_kernel<T, 32><<<(unsigned)ctas, LP_THREADS, 0, st>>>(P, rows);
+  return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
+}
+
 template <typename T>
 static int launch_logprobs(const LpParams& P, int64_t ctas, cudaStream_t st) {
+  if (P.V <= LP_WARP_V) return launch_warps<T>(P, st);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(LP_THREADS);

@@ -122,6 +122,26 @@ def test_against_the_definition(dt, V, n):
 
 
 @gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V,n", [(3, 0), (31, 31), (40, 32), (300, 32), (512, 20), (513, 32),
+                                 (1000, 5), (1024, 32), (1025, 32), (1500, 32), (2047, 20)])
+def test_small_vocabularies(dt, V, n):
+    """A warp per row, and rows with fewer units than threads."""
+    x, ids = _logits((37,), V, dt, 7 * V + n)
+    x[0] = 0.0                                               # every entry on the list
+    x[1] = -math.inf
+    x[2, V // 2:] = -math.inf
+    x[3, V - 1] = math.nan
+    x[4, 0] = math.inf
+    x[5] = -1.0
+    x[5, V // 3:] = 1.0
+    x[6, :-1] = torch.finfo(dt).min
+    _check(x, ids, 1.0, n)
+    _check(x[:, 1:], ids.clamp(max=V - 2), 0.3, min(n, V - 1))
+    _check(x[:5].view(5, 1, V).expand(5, 3, V), ids[:15].view(5, 3), 2.0, n)
+
+
+@gpu
 @pytest.mark.parametrize("rows", [(1,), (150,), (700,), (5, 3), (2, 2, 3)])
 def test_batches_and_shapes(rows):
     x, ids = _logits(rows, 5001, torch.bfloat16, 1)
