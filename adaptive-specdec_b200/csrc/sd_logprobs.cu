@@ -31,7 +31,7 @@
 // few more; only threads whose maximum reaches it look through their units
 // again (from L2), a warp together.
 //
-// Bound by HBM with many rows: 2048 rows of 151936 bf16 in 113 us, 5.5 TB/s (the
+// Bound by HBM with many rows: 2048 rows of 151936 bf16 in 114 us, 5.4 TB/s (the
 // copy rate here is 6.57); by latency with few: one row in 7 us, 320 rows with five
 // alternatives in 27 (3.6 TB/s: 2.2 rows per SM, whose tails show).
 #include <cuda_runtime.h>

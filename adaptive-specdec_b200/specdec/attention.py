@@ -170,7 +170,7 @@ def prefix_attention(q, k_pool, v_pool, lengths, block_table, group_starts, pref
     if valid is not None and (valid.dtype != torch.long or not valid.is_contiguous()):
         valid = valid.long().contiguous()
     if out is None:
-        out = torch.empty((B, qlen, Hq, D), dtype=dt, device=dev)
+        out = q.new_empty(B, qlen, Hq, D)
         ob, ol, oh = qlen * Hq * D, Hq * D, D
     else:
         if out.shape != (B, qlen, Hq, D) or out.dtype != dt or (D > 1 and out.stride(3) != 1):

@@ -320,7 +320,7 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
         entropy = torch.empty(shape, dtype=torch.float32, device=dev)
     top_ids = top_lp = None
     if n:
-        top_ids = torch.empty([*shape, n], dtype=torch.long, device=dev)
+        top_ids = ids.new_empty(*shape, n)
         top_lp = torch.empty_like(top_ids, dtype=torch.float32)
     L.check(L.lib().sd_token_logprobs(
         x.data_ptr(), bs, ps, code, ids.data_ptr(), ids_bs, B, Lr, V, T, n, logprob.data_ptr(),
