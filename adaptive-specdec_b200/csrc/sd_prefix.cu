@@ -78,8 +78,23 @@ __device__ __forceinline__ int px_share(int total) {
   return max(PX_MIN_SHARE, (total + PX_CTAS - 1) / PX_CTAS);
 }
 
-__device__ __forceinline__ int ow_share(int total) {
-  return max(OW_MIN_SHARE, (total + PX_CTAS - 1) / PX_CTAS);
+// Units per CTA of the own ranges.  Where the shared ranges leave SMs idle, only
+// the CTAs that come up on those get work, if it then ends before the ones that
+// have to wait for a busy SM would (a shared page takes about 1.5 own ones).  32 / 8
+// heads, 1 query: 8 rows, 16 shared pages, up to 1000 own keys 21.4 us for the call
+// (27.1 with the work over all SMs); 64 rows, 8 pages, up to 300 keys 31.6 (36.3); 16
+// rows the same 19.5 (19.4).
+__device__ __forceinline__ int ow_share(const PrefixParams& P, int total) {
+  int share = max(OW_MIN_SHARE, (total + PX_CTAS - 1) / PX_CTAS);
+  const int units = P.g_unit[P.G];
+  if (units > 0 && P.qc >= P.A.qlen) {
+    const int ps = px_share(units), idle = PX_CTAS - (units + ps - 1) / ps;
+    if (idle > 0) {
+      const int apart = max(share, (total + idle - 1) / idle);
+      if (apart - share < ps + ps / 2) share = apart;
+    }
+  }
+  return share;
 }
 
 // CTA 0 plans, the others pack: 16 threads copy a query row.
@@ -702,13 +717,12 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
   };
   fetch();
   const int total = A.rowpre[A.B] * A.Hkv;
-  const int share = ow_share(total);
-  const int t0 = (int)blockIdx.x * share;
-  if (t0 >= total) {                                 // no work for this CTA (uniform)
+  const int share = ow_share(P, total);
+  if ((int64_t)blockIdx.x * share >= total) {                                 // no work for this CTA (uniform)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
-  const int t1 = min(total, t0 + share);
+  const int t0 = (int)blockIdx.x * share, t1 = t0 + min(total - t0, share);
   const int j0 = (int)blockIdx.y * P.qc;             // the chunk's first query
   const int R = min(P.qc, A.qlen - j0) * A.group;    // its query rows per kv head
   const int nq = P.nq, ns = 4 / nq;                  // quarters per segment, streams
@@ -1083,7 +1097,7 @@ __global__ void __launch_bounds__(PX_JOIN_THREADS, PX_JOIN_CTAS) prefix_join_ker
   // the rows; [n1, np) of the row's own range.  Rows of partials in 32 bits: each
   // is 512 bytes of memory.
   const int g = P.rowgroup[b], pre = A.rowpre[b], tb = A.rowpre[b + 1] - pre;
-  const int RC = P.qc * A.group, oshare = ow_share(A.rowpre[A.B] * A.Hkv);
+  const int RC = P.qc * A.group, oshare = ow_share(P, A.rowpre[A.B] * A.Hkv);
   const int ou = pre * A.Hkv + h * tb, oc0 = (ou + OW_OVH) / oshare, jc = r / RC;
   const int at2 = (jc * P.slots + bh + oc0) * RC + r - jc * RC;
   int n1 = 0, dup = 0, at1 = 0;
