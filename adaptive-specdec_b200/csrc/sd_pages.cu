@@ -63,11 +63,6 @@ struct PagesParams {
   bool fused;                                   // the scanning CTA fills
 };
 
-// Exclusive block scan of packed (tokens, pages << 32) sums over PT_THREADS.
-__device__ __forceinline__ long long scan_pair(long long v, long long* red, long long* total) {
-  return block_excl_scan<long long>(v, red, total);
-}
-
 // Warp w of warps: the slots of a row's tokens [run * P.run, ...) and, for run 0,
 // its new table entries; the warps past the rows fill the slots behind the last
 // token with -1.
@@ -135,7 +130,8 @@ __global__ void __launch_bounds__(PT_THREADS) pages_reserve_plan_kernel(const Pa
       plan[P.B + b] = had;
     }
     long long sum;
-    const long long ex = carry + scan_pair(v, red, &sum);
+    // (tokens in the low 32 bits, pages above)
+    const long long ex = carry + block_excl_scan<long long>(v, red, &sum);
     carry += sum;
     if (b < P.B) {
       starts[b] = (int32_t)(ex & 0xFFFFFFFFLL);

@@ -107,9 +107,9 @@ __global__ void __launch_bounds__(PX_PLAN_THREADS) prefix_plan_kernel(const Pref
     const int c = threadIdx.x & 15;
     const int hb = (int)(i / A.R), f = (int)(i - (int64_t)hb * A.R), h = hb / A.B, b = hb - h * A.B;
     const int j = f / A.group, hq = h * A.group + f - j * A.group;
-    P.qp[i * 16 + c] = __ldg(reinterpret_cast<const uint4*>(
-                                 reinterpret_cast<const __nv_bfloat16*>(A.q) + b * A.qbs + hq * A.qhs +
-                                 j * A.qqs) + c);
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(A.q);
+    P.qp[i * 16 + c] =
+        __ldg(reinterpret_cast<const uint4*>(q + b * A.qbs + hq * A.qhs + j * A.qqs) + c);
     return;
   }
   __shared__ long long red[33];
@@ -201,8 +201,8 @@ __device__ __forceinline__ void px_bounds(PxSeg& s) {
   s.j1 = max(s.off + s.ncost - PX_OVH, s.j0);
 }
 // first: the group's index, its first unit, its rows and pages
-__device__ __forceinline__ void px_init(PxSeg& s, const PrefixParams& P, const int (&first)[4], int t0,
-                                        int t1) {
+__device__ __forceinline__ void px_init(PxSeg& s, const PrefixParams& P, const int (&first)[4],
+                                        int t0, int t1) {
   s.g = first[0];
   s.rows = first[2];
   s.np = px_pairs(P, s.rows);
@@ -241,7 +241,7 @@ struct PxSmem {
   alignas(128) unsigned char out[8][32 * 128];               // a warp's 32 rows x 32 floats of O
   alignas(8) unsigned long long sfull[2], pfull[2], oready[2], qfull[2], fin;
   uint32_t tmem;
-  int first[4];                                              // the CTA's first group: g, unit, rows, pages
+  int first[4];                                      // the CTA's first group: g, unit, rows, pages
   int abort_;
 };
 static_assert(sizeof(PxSmem) + 1024 <= 227 * 1024, "prefix attention shared memory");
@@ -421,7 +421,8 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
           if (k4 > 0 && dup) break;
 #pragma unroll
           for (int ks = k4; ks < k4 + 4; ++ks)
-            tc_mma_ts_warp(a + 256u, a + 8u * ks, dv + (uint64_t)(ks * 128), ID2, ks || !first ? 1 : 0);
+            tc_mma_ts_warp(a + 256u, a + 8u * ks, dv + (uint64_t)(ks * 128), ID2,
+                           ks || !first ? 1 : 0);
         }
         tc_commit_warp(&S.oready[x]);
         if (x == 1u) tc_commit_warp(&S.empty[sl]);
@@ -541,7 +542,8 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float a, b;
-            unpair(fma2(pair2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sl22, nm2), a, b);
+            const unsigned long long s2 = pair2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+            unpair(fma2(s2, sl22, nm2), a, b);
             // a quarter by the FMA pipe: the exponentials of a page take 2048
             // cycles of the special-function units otherwise (a call of 101.3 us
             // took 102.5 without, 103 with half of them there)
@@ -669,7 +671,7 @@ struct OwSmem {
   // by stream and the stream's page parity (at most two phases of each are open)
   alignas(8) unsigned long long sfull[4][2], pfull[4][2], oready[4][2], qfull[4], fin;
   uint32_t tmem;
-  int first[5];                                      // the CTA's first row: OwSeg's b, unit, tb, k0, kmax
+  int first[5];                                      // the CTA's first row: b, unit, tb, k0, kmax
   int abort_;
 };
 static_assert(sizeof(OwSmem) + 1024 <= 227 * 1024, "own-range attention shared memory");
@@ -718,7 +720,7 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
   fetch();
   const int total = A.rowpre[A.B] * A.Hkv;
   const int share = ow_share(P, total);
-  if ((int64_t)blockIdx.x * share >= total) {                                 // no work for this CTA (uniform)
+  if ((int64_t)blockIdx.x * share >= total) {        // no work for this CTA (uniform)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
@@ -971,8 +973,9 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
           ok = __all_sync(0xffffffffu, tc_wait(&S.full[st][1], (pg / OW_STAGES) & 1u, &S.abort_));
           if (!ok) break;
           for (int kr = cur.s1 - key0 + 4 * (w % nq) + (lane >> 3); kr < 128; kr += 4 * nq) {
-            *reinterpret_cast<uint4*>(S.v[st][0] + kr * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(S.v[st][1] + kr * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            const int at = kr * 128 + (lane & 7) * 16;
+            *reinterpret_cast<uint4*>(S.v[st][0] + at) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(S.v[st][1] + at) = make_uint4(0u, 0u, 0u, 0u);
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
