@@ -14,7 +14,7 @@ import torch
 
 own = False
 
-PACKAGE = str(pathlib.Path(__file__).resolve().parent.parent / "adaptive-specdec_b200")
+ROOT = pathlib.Path(__file__).resolve().parent.parent
 PAGE = 128                       # tokens per page of the paged cache
 VOCAB = 151936
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
@@ -22,8 +22,9 @@ TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 def _package():
     """This repository's package on the path (it lives in a folder that is no module name)."""
-    if PACKAGE not in sys.path:
-        sys.path.insert(0, PACKAGE)
+    p = str(ROOT / "adaptive-specdec_b200")
+    if p not in sys.path:
+        sys.path.insert(0, p)
 
 
 # ---- cases --------------------------------------------------------------------------------------
