@@ -649,8 +649,12 @@ class PagedRaggedCache(RaggedCache):
             pl = torch.as_tensor(plen).to(self.device, torch.long).reshape(-1).clamp(max=int(P))
             self.pages.reserve(self.lengths, pl, slot_map=False,
                                floor=None if self.prefix is None else self.pages.shared)
+            # only the padding goes to the sink: where the pool ran out, the prompt's
+            # columns stay -1, so that writes there are flagged
+            need = (self.lengths + pl + PAGE - 1) // PAGE
             top = (self.lengths + int(P) + PAGE - 1) // PAGE
-            pad = (self._columns() < top.view(-1, 1)) & (self.block_table < 0)
+            col = self._columns()
+            pad = (col >= need.view(-1, 1)) & (col < top.view(-1, 1)) & (self.block_table < 0)
             self.block_table.masked_fill_(pad, self.pages.sink)
             return
         pl = torch.as_tensor(plen).to("cpu", torch.long).reshape(-1).numpy()
@@ -732,12 +736,18 @@ class PagedRaggedCache(RaggedCache):
         its last, partly filled page is copied to each.  Returns the new cache
         (rows of one source row side by side) over the same pools; this cache
         is left empty and must not be used further.  The shared pages go back
-        with the new cache's ``reset``.  Synchronises once (error check)."""
+        with the new cache's ``reset``.  Raises what this cache's error flag holds
+        (a prefill that found no pages), or when a row holds tokens without
+        a page.  Synchronises (error checks)."""
         if not self.device_pages:
             raise L.SpecdecError("fork needs device_pages=True")
         counts = [int(c) for c in counts]
         if len(counts) != self.batch_size or min(counts) < 1:
             raise L.SpecdecError(f"fork needs one positive count per row ({self.batch_size})")
+        self.check_errors()
+        need = (self.lengths.view(-1, 1) + PAGE - 1) // PAGE
+        if bool(((self._columns() < need) & (self.block_table < 0)).any()):
+            raise L.SpecdecError("fork: a row holds tokens without a page")
         host = self._mirror().clone()
         src = torch.repeat_interleave(torch.arange(self.batch_size), torch.tensor(counts))
         new = PagedRaggedCache(len(self.layers), len(src), self.capacity, self.device,

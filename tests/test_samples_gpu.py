@@ -310,3 +310,30 @@ def test_bad_arguments(engine):
     for bad in (dict(n=0), dict(logprobs=-1), dict(logprobs=VOCAB + 1)):
         with pytest.raises(ValueError):
             engine.generate(ids, plen, 4, **bad)
+
+
+def test_rows_without_their_pages_do_not_fork(engine):
+    """A prefill that found too few pages: nothing went to the sink for it, and the
+    fork raises, also when somebody has read the flag in between."""
+    lens = [700, 5]
+    c = PagedRaggedCache(1, 2, 1024, DEV, n_pages=6, device_pages=True)
+    c.reserve_prefill(700, torch.tensor(lens))                 # seven pages wanted, five free
+    assert c.block_table[0, :6].tolist() == [-1] * 6 and c.block_table[1, 0] == -1
+    assert c.block_table[1, 1:6].tolist() == [c.pages.sink] * 5
+    k = torch.randn(2, 2, 700, 128, device=DEV).bfloat16()
+    c.layers[0].update(k, k)
+    c.set_lengths(torch.tensor(lens))
+    assert int(c._err) & 6 == 6                                # no pages, slots without one
+    with pytest.raises(L.SpecdecError, match="exhausted"):
+        c.fork([2, 1])
+    with pytest.raises(L.SpecdecError, match="without a page"):
+        c.fork([2, 1])
+    assert c.free_pages == 5 and bool((c.block_table == -1).all())
+    # the same from the engine: two pages are enough for the samples' own tokens,
+    # not for the prompt's 384
+    small = SpecDecodeEngine(engine.target, engine.draft, TinyTok(), device=DEV, capacity=512,
+                             kv_pages=3)
+    torch.manual_seed(0)
+    ids = torch.randint(0, VOCAB, (1, 384))
+    with pytest.raises(L.SpecdecError, match="exhausted"):
+        small.generate(ids, torch.tensor([384]), 8, sampling=SamplingConfig(), k_fixed=3, n=2)
