@@ -284,8 +284,9 @@ int sd_pages_reserve(int32_t* block_table, int bt_stride, int W, int32_t* owned,
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int64_t most = std::min<int64_t>(
       std::min<int64_t>(P.max_tokens, (int64_t)W * SD_KV_PAGE), new_tokens ? P.max_tokens : new_each);
-  P.run = 512;
-  while ((most + P.run - 1) / P.run * B > 65536) P.run *= 2;
+  // tokens per warp: 512, or as many as leave 65536 warps (at least one per row)
+  const int64_t cuts = std::max<int64_t>(1, 65536 / B);
+  P.run = (int)std::max<int64_t>(512, (most + cuts - 1) / cuts);
   P.runs = (int)std::max<int64_t>(1, (most + P.run - 1) / P.run);
   P.fused = (int64_t)B * P.runs <= PT_FUSED_WARPS && P.max_tokens <= PT_FUSED_WARPS * 32;
   // some warps for the slots behind the last token

@@ -323,3 +323,24 @@ def test_arguments_are_checked_before_any_launch():
     assert reserve(ws=n) == -28 and reserve(nws=16) == -28
     assert lib.sd_pages_trim(d, 4, 4, d, n, d, 20, d, d, 3, d, n) == -22
     assert lib.sd_pages_trim(d, 4, 4, d, d, d, 20, d, d, 0, d, n) == 0
+
+
+@gpu
+@pytest.mark.parametrize("B", [65536, 65537, 70000])
+@pytest.mark.parametrize("each", [1, 2, 5])
+def test_more_rows_than_a_launch_cuts_into_runs(B, each):
+    """Page b goes to row b: every slot is known."""
+    want = torch.arange(B, device=DEV).view(-1, 1) * PAGE + torch.arange(each, device=DEV)
+    zero = torch.zeros(B, dtype=torch.long, device=DEV)
+    t = DevicePageTable(B, 1, B + 1, DEV)
+    slots, starts = t.reserve(zero, each)
+    assert torch.equal(slots.view(B, each), want)
+    assert torch.equal(starts, torch.arange(B + 1, dtype=torch.int32, device=DEV) * each)
+    assert torch.equal(t.block_table.view(-1), torch.arange(B, dtype=torch.int32, device=DEV))
+    t.check_errors()
+    t.trim(zero)
+    assert int(t.n_free) == B
+    slots, _ = t.reserve(zero, zero + each, max_tokens=B * each + 7)
+    assert torch.equal(slots[:-7].view(B, each), want) and bool((slots[-7:] == -1).all())
+    t.reserve(zero, each, slot_map=False)
+    t.check_errors()
