@@ -246,6 +246,8 @@ static int pages_check(const PagesParams& P) {
   if (!P.bt || !P.owned || !P.free_stack || !P.n_free || !P.lengths || !P.err) return SD_EINVAL;
   if (P.W <= 0 || P.bt_stride < P.W || P.n_pages <= 0) return SD_EINVAL;
   if ((int64_t)P.W * SD_KV_PAGE > 0x7FFFFFFF) return SD_ENOTSUP;
+  // a trim counts the rows' pages in 32 bits before it compares them with the pool
+  if ((int64_t)P.B * P.W > 0x7FFFFFFF) return SD_ENOTSUP;
   return SD_OK;
 }
 

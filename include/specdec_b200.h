@@ -267,7 +267,9 @@ int sd_kv_append_paged(void* kpool, void* vpool, const void* new_k, const void* 
  * A call that cannot serve every row changes nothing and sets bits of *err:
  * CAPACITY (a row past W pages, a negative length or count), EXHAUSTED (too
  * few free pages), SLOTS (more new tokens than max_tokens), SHARED (a new
- * token below floor_pages); starts is still written and every slot is -1.  Calls on one table are stream ordered.
+ * token below floor_pages); starts is still written and every slot is -1.  Calls
+ * on one table are stream ordered.  SD_ENOTSUP: B * W past 2^31 - 1, for a
+ * reserve B * W * SD_KV_PAGE.
  */
 #define SD_PAGES_ERR_CAPACITY 1
 #define SD_PAGES_ERR_EXHAUSTED 4

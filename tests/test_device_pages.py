@@ -344,3 +344,13 @@ def test_more_rows_than_a_launch_cuts_into_runs(B, each):
     assert torch.equal(slots[:-7].view(B, each), want) and bool((slots[-7:] == -1).all())
     t.reserve(zero, each, slot_map=False)
     t.check_errors()
+
+
+def test_tables_of_more_pages_than_are_counted_are_refused():
+    lib = L.lib()
+    n, d = ctypes.c_void_p(0), ctypes.c_void_p(4096)
+
+    def trim(W, B):
+        return lib.sd_pages_trim(d, W, W, d, d, d, 20, d, d, B, d, n)
+    assert trim((1 << 24) - 1, 129) == -95 and trim(1 << 23, 1 << 20) == -95
+    assert trim(1 << 24, 1) == -95
