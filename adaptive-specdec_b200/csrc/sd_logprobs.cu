@@ -19,7 +19,8 @@
 // streams its part's 16-byte
 // units, LP_UNITS per thread and step with the next step's loads in flight,
 // each thread keeping its maximum, sums in base 2 against a reference that
-// moves only when a step's maximum passes it by LP_HEADROOM, and the count of
+// moves only when a step's maximum passes it by LP_HEADROOM (rows whose largest
+// logit is beyond LP_TAME in base-2 units take a second pass), and the count of
 // elements ahead of the token (packed compares and adds).  Each CTA leaves its
 // sums at the part's maximum, its count and its top n as sorted 64-bit keys
 // (value key, complement of the id) in the shared memory of the cluster's first
@@ -53,6 +54,11 @@ constexpr int LP_CTAS = 4;                      // per SM
 constexpr int LP_SMS = 148;
 constexpr int LP_STEP = LP_THREADS * LP_UNITS;  // units per step of a CTA
 constexpr float LP_HEADROOM = 8.f;              // base 2
+// The largest reference, in base-2 units.  A reference is the float next to m c;
+// from 2^31 on it may be more than 128 away from it, so that the maximum's own
+// exponent d = fma(m, c, -R) is no longer near 0 and 2^d leaves the float range.
+// Up to 2^20 they are within 1/32.
+constexpr float LP_TAME = 1048576.f;
 constexpr int LP_LIST = 2048;                   // a part's flagged elements
 constexpr int LP_GROUPS = 64;                   // groups of threads behind the top n's threshold
 constexpr int LP_MAX_PARTS = 8;                 // CTAs of a cluster
@@ -63,7 +69,8 @@ static_assert(SD_TOPN_MAX <= LP_GROUPS / 2 && LP_THREADS / 8 >= LP_GROUPS / 2,
               "the n-th largest of the group maxima");
 
 struct LpPart {
-  float m, s, e;                                // max (base-2 units), sum 2^d, sum d 2^d
+  double ref;                                   // reference of the sums (base-2 units)
+  float s, e;                                   // sum 2^d, sum d 2^d
   int ahead;                                    // elements at or ahead of the token
 };
 
@@ -96,11 +103,11 @@ __device__ __forceinline__ uint32_t lp_key(float f) {
 // maximum (-inf, or a mask of the type's lowest value) then adds 0 * -256 to
 // the entropy sum, not 0 * -inf.  A NaN stays.
 __device__ __forceinline__ float lp_hold(float x) { return x < -256.f ? -256.f : x; }
-// ln2 (x c - lse): a log-probability from a logit and the base-2 log of the sum.
-// In 64 bits, where x c is exact and the difference loses nothing; the rounding
-// of the sum alone may not make a probability above 1.
-__device__ __forceinline__ float lp_final(float x, float c, double lse) {
-  const double v = 0.69314718055994530942 * ((double)x * (double)c - lse);
+// ln2 (x c - ref - lz): a log-probability from a logit, the reference and the base-2
+// log of the sum.  In 64 bits, where x c is exact and the difference loses
+// nothing; the rounding of the sum alone may not make a probability above 1.
+__device__ __forceinline__ float lp_final(float x, float c, double ref, float lz) {
+  const double v = 0.69314718055994530942 * ((double)x * (double)c - ref - (double)lz);
   return v > 0.0 ? 0.f : (float)v;
 }
 __device__ __forceinline__ float lp_value(uint32_t k) {
@@ -218,8 +225,10 @@ __device__ void sort_top(unsigned long long* list, int cnt, int n, unsigned long
 }
 
 // A thread's running state over its units.  Exponents are d = fma(x, c, -R) with
-// the reference R a float in base-2 units: one rounding of d, whatever the size
-// of x c, as long as everything is measured against the same R.
+// the reference R a float in base-2 units, |R| <= LP_TAME: one rounding of d, as
+// long as everything is measured against the same R.  A thread whose maximum is
+// below that range has sums of 0, which is what they are worth beside a maximum
+// within it; one above it has no valid sums (the block notices).
 template <typename T>
 struct LpRun {
   using Wd = Word<T>;
@@ -240,9 +249,9 @@ struct LpRun {
       g = Wd::vmax(g, Wd::vmax(Wd::vmax(d[i].x, d[i].y), Wd::vmax(d[i].z, d[i].w)));
     wm = Wd::vmax(wm, g);
     const float gs = fmaxf(Wd::get(g, 0), Wd::get(g, Wd::N - 1)) * c;
-    // nothing summed yet: any finite maximum is the reference
+    // nothing summed yet: any maximum is the reference
     const bool first = s2 == 0ULL;
-    if (gs < CUDART_INF_F && (first ? gs > -CUDART_INF_F : gs - R > LP_HEADROOM)) {
+    if (fabsf(gs) <= LP_TAME && (first || gs - R > LP_HEADROOM)) {
       // the sums so far move to the new reference (2^-256 is 0)
       const float dm = fmaxf(R - gs, -256.f), f = lp_ex2(dm);
       const unsigned long long f2 = pair2(f, f);
@@ -265,7 +274,7 @@ struct LpRun {
                                                  : pair2(Wd::get(w[q], 0), Wd::get(w[q | 1], 0));
         float a, b;
         unpair(fma2(x2, c2, nR2), a, b);
-        // -inf elements add 0 * -256, not 0 * -inf
+        // elements far below (-inf, masks) add 0 * -256, not 0 * -inf
         a = fmaxf(a, -256.f);
         b = fmaxf(b, -256.f);
         const unsigned long long p2 = pair2(lp_ex2(a), lp_ex2(b));
@@ -306,7 +315,9 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   // of the cluster's first CTA: what every part found
   __shared__ LpPart parts[LP_MAX_PARTS];
   __shared__ unsigned long long part_keys[LP_MAX_PARTS * SD_TOPN_MAX];
-  __shared__ double sh_lse;                          // log2 of the sum of all exponentials
+  // log2 of the sum of all exponentials: the reference and the rest
+  __shared__ double sh_ref;
+  __shared__ float sh_lz;
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   const cg::cluster_group cluster = cg::this_cluster();
   const int cid = (int)(blockIdx.x / P.csize), crank = (int)(blockIdx.x % P.csize);
@@ -377,7 +388,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   const bool nan = m != m;
   // the thread's sums at its own maximum (base-2 units), with its extra element
   const float ms = m * P.c;
-  const float m0 = ms > -CUDART_INF_F && ms < CUDART_INF_F ? ms : 0.f;
+  const float m0 = fabsf(ms) <= LP_TAME ? ms : 0.f;
   float s, es;
   {
     float a, b;
@@ -417,8 +428,8 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   }
   if (split) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   // join over the block: the maxima first, then the sums at the block's maximum
-  float bm = warp_max(nan ? -CUDART_INF_F : ms);
-  if (lane == 0) red_m[w] = bm;
+  float bx = warp_max(nan ? -CUDART_INF_F : m);
+  if (lane == 0) red_m[w] = bx;
   const bool any = u0 + t < u1 || lone;              // this thread holds an element
   int size = 8;
   if (TOP) {
@@ -436,13 +447,38 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
     if (t % size == 0 && t / size < LP_GROUPS) group_k[t / size] = k;
   }
   __syncthreads();
-  bm = red_m[0];
+  bx = red_m[0];
 #pragma unroll
-  for (int q = 1; q < LP_WARPS; ++q) bm = fmaxf(bm, red_m[q]);
-  const float dm = lp_hold(ms - bm), f = lp_ex2(dm);
-  float sj = f * s, ej = f * fmaf(dm, s, es);
-  if (ms == -CUDART_INF_F) sj = ej = 0.f;            // nothing above -inf
-  if (nan || ms == CUDART_INF_F) sj = CUDART_NAN_F;  // as the formula: inf - inf
+  for (int q = 1; q < LP_WARPS; ++q) bx = fmaxf(bx, red_m[q]);
+  const float bm = bx * P.c;
+  const bool wild = !(fabsf(bm) <= LP_TAME) && fabsf(bx) < CUDART_INF_F;
+  float sj, ej;
+  if (wild) {
+    // No float is near enough to the maximum's x c: once more over the part (from
+    // L2, or HBM), with d = (x - bx) c, which is 0 at the maximum.
+    sj = ej = 0.f;
+    auto add = [&](float x) {
+      const float d = fmaxf((x - bx) * P.c, -256.f), p = lp_ex2(d);
+      sj += p;
+      ej = fmaf(d, p, ej);
+    };
+#pragma unroll 1
+    for (int v = u0 + t; v < u1; v += LP_THREADS) {
+      const uint4 d = __ldg(body + v);
+      const uint32_t x[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < Wd::N; ++e) add(Wd::get(x[q], e));
+    }
+    if (lone) add(xe);
+  } else {
+    const float dm = lp_hold(ms - bm), f = lp_ex2(dm);
+    sj = f * s;
+    ej = f * fmaf(dm, s, es);
+    if (ms == -CUDART_INF_F) sj = ej = 0.f;          // nothing above -inf
+  }
+  if (nan || m == CUDART_INF_F) sj = CUDART_NAN_F;   // as the formula: inf - inf
   sj = warp_sum(sj);
   ej = warp_sum(ej);
   ahead = warp_sum(ahead);
@@ -554,7 +590,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   }
   if (t == 0) {
     LpPart o;
-    o.m = bm;
+    o.ref = wild ? (double)bx * (double)P.c : (double)bm;
     o.s = 0.f;
     o.e = 0.f;
     o.ahead = 0;
@@ -570,24 +606,27 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
   if (split) cluster.sync(); else __syncthreads();
   if (part != 0) return;
   if (t == 0) {
-    float rm = -CUDART_INF_F, rs = 0.f, re = 0.f;
+    double rm = -CUDART_INF;
+    float rs = 0.f, re = 0.f;
     int ra = 0;
-    for (int i = 0; i < nparts; ++i) rm = fmaxf(rm, parts[i].m);
+    for (int i = 0; i < nparts; ++i) rm = fmax(rm, parts[i].ref);
     for (int i = 0; i < nparts; ++i) {
       const LpPart q = parts[i];
       ra += q.ahead;
-      if (q.m == -CUDART_INF_F && q.s == q.s) continue;          // nothing above -inf, no NaN
-      const float dj = lp_hold(q.m - rm), fj = lp_ex2(dj);
+      if (q.ref == -CUDART_INF && q.s == q.s) continue;          // nothing above -inf, no NaN
+      const float dj = (float)fmax(q.ref - rm, -256.0), fj = lp_ex2(dj);
       rs = fmaf(fj, q.s, rs);
       re = fmaf(fj, fmaf(dj, q.s, q.e), re);
     }
-    const float lz = log2f(rs);
-    const bool none = !(rm > -CUDART_INF_F);                     // every entry is -inf
-    sh_lse = none ? CUDART_NAN : (double)rm + (double)lz;
+    // every entry is -inf, or one +inf: NaN, as the formula
+    const bool none = !(fabs(rm) < CUDART_INF);
+    const float lz = none ? CUDART_NAN_F : log2f(rs);
+    sh_ref = rm;
+    sh_lz = lz;
     const float h = 0.69314718055994531f * (lz - re / rs);
-    P.entropy[r] = none || rm == CUDART_INF_F ? CUDART_NAN_F : h < 0.f ? 0.f : h;
+    P.entropy[r] = h < 0.f ? 0.f : h;
     P.rank[r] = have ? (int64_t)ra : 0;
-    P.logprob[r] = have ? lp_final(xt, P.c, sh_lse) : CUDART_NAN_F;
+    P.logprob[r] = have ? lp_final(xt, P.c, rm, lz) : CUDART_NAN_F;
   }
   if (!TOP) return;
   __syncthreads();
@@ -602,7 +641,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logp_kernel(const LpParam
     if (rank < P.top) {                              // absent keys (0) rank behind the V >= n real ones
       P.top_ids[r * P.top + rank] = (int64_t)(uint32_t)~(uint32_t)key;
       P.top_lp[r * P.top + rank] =
-          lp_final(lp_value((uint32_t)(key >> 32)), P.c, sh_lse);
+          lp_final(lp_value((uint32_t)(key >> 32)), P.c, sh_ref, sh_lz);
     }
   }
 }
@@ -651,13 +690,12 @@ __global__ void __launch_bounds__(LP_THREADS) logp_warp_kernel(const LpParams P,
   ahead = warp_sum(ahead);
   const uint32_t wk = __reduce_max_sync(0xffffffffu, max(mk[0], mk[1]));
   const float m = lp_value(wk);                      // (a NaN's key: NaN)
-  const float rm = m * P.c;                          // the row's maximum, base-2 units
-  const bool finite = rm > -CUDART_INF_F && rm < CUDART_INF_F;
-  const float m0 = finite ? rm : 0.f;
+  const bool finite = fabsf(m) < CUDART_INF_F;
+  const float m0 = finite ? m : 0.f;
   float s0 = 0.f, s1 = 0.f, e0 = 0.f, e1 = 0.f;
 #pragma unroll
   for (int i = 0; i < NE; i += 2) {
-    const float a = fmaxf(fmaf(x[i], P.c, -m0), -256.f), b = fmaxf(fmaf(x[i + 1], P.c, -m0), -256.f);
+    const float a = fmaxf((x[i] - m0) * P.c, -256.f), b = fmaxf((x[i + 1] - m0) * P.c, -256.f);
     const float pa = lp_ex2(a), pb = lp_ex2(b);
     s0 += pa;
     s1 += pb;
@@ -665,14 +703,14 @@ __global__ void __launch_bounds__(LP_THREADS) logp_warp_kernel(const LpParams P,
     e1 = fmaf(b, pb, e1);
   }
   const float rs = warp_sum(s0 + s1), re = warp_sum(e0 + e1);
-  const float lz = log2f(rs);
   // all -inf, +inf or NaN among them: as the formula, NaN
-  const double lse = finite ? (double)rm + (double)lz : CUDART_NAN;
+  const float lz = finite ? log2f(rs) : CUDART_NAN_F;
+  const double ref = (double)m * (double)P.c;
   if (lane == 0) {
     const float h = 0.69314718055994531f * (lz - re / rs);
-    P.entropy[r] = !finite ? CUDART_NAN_F : h < 0.f ? 0.f : h;
+    P.entropy[r] = h < 0.f ? 0.f : h;
     P.rank[r] = have ? (int64_t)ahead : 0;
-    P.logprob[r] = have ? lp_final(xt, P.c, lse) : CUDART_NAN_F;
+    P.logprob[r] = have ? lp_final(xt, P.c, ref, lz) : CUDART_NAN_F;
   }
   const int n = P.top;
   if (n == 0) return;
@@ -699,7 +737,7 @@ __global__ void __launch_bounds__(LP_THREADS) logp_warp_kernel(const LpParams P,
   }
   auto put = [&](int rank, unsigned long long key) {
     P.top_ids[r * n + rank] = (int64_t)(uint32_t)~(uint32_t)key;
-    P.top_lp[r * n + rank] = lp_final(lp_value((uint32_t)(key >> 32)), P.c, lse);
+    P.top_lp[r * n + rank] = lp_final(lp_value((uint32_t)(key >> 32)), P.c, ref, lz);
   };
   __syncwarp();
   if (cnt <= LP_WLIST) {

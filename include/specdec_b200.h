@@ -186,8 +186,10 @@ int sd_gather_prob(const float* probs, int n_rows, int V, const int64_t* ids, fl
  * logits [B, L, V] of `dtype` (element strides (bs, ps, 1)), ids [B, L] int64
  * (row stride ids_bs); outputs contiguous.  An id outside [0, V) (a padding
  * position) gets logprob NaN and rank 0; its row's other outputs are as for
- * any id.  temperature in [1e-6, 1e6].  -inf entries have probability 0; an
- * x * log2(e) / T past the float range counts as infinite.  A row with a NaN or a +inf, or
+ * any id.  temperature in [1e-6, 1e6].  -inf entries have probability 0.  Every
+ * finite logit counts by its difference to the row's largest one, whatever its
+ * size (a row of nothing but the type's lowest value is uniform); a
+ * log-probability past the float range is -inf.  A row with a NaN or a +inf, or
  * with nothing above -inf, has NaN log-probabilities and entropy (as the
  * formula); its rank and top_ids still follow the logits, NaN first.  Needs
  * no workspace.

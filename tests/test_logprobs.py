@@ -342,3 +342,59 @@ def test_arguments_are_checked_before_any_launch():
     assert call(top=33, tops=d) == -95
     assert call(V=(1 << 20) + 1) == -95
     assert call(x=ctypes.c_void_p(4097)) == -22                # not aligned to its type
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [40, 700, 1024, 1500, 20000, 151936])
+@pytest.mark.parametrize("T", [1e-6, 1e-5, 0.01, 1e6])
+def test_large_logits_at_any_temperature(dt, V, T):
+    """Products x log2(e) / T far beyond what a float32 resolves: only differences
+    of logits count.  Few distinct values, so that rows have ties at the maximum."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.randint(-3, 4, (7, V), generator=g, device=DEV).float()
+    x[1] += 5000.0
+    x[2] -= 5000.0
+    x[3] += 65504.0 - 3.0
+    x[4] = (x[4] * 16.0 - 40000.0)
+    x[5] = 65504.0
+    x[6, V // 2:] = -65504.0
+    ids = torch.randint(0, V, (7,), generator=g, device=DEV)
+    x = x.to(dt)
+    _check(x, ids, T, 5)
+    _check(x, x.argmax(-1), T, 0)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [40, 700, 1500, 20000, 151936])
+@pytest.mark.parametrize("T", [0.7, 1.0, 1.5])
+def test_finite_masks(dt, V, T):
+    """Masks of every size down to the type's lowest value, over most of a row and
+    over all of it; entries at both ends of the type."""
+    x, ids = _logits((9,), V, dt, V)
+    lo, hi = torch.finfo(dt).min, torch.finfo(dt).max
+    for r, mask in enumerate((-1e4, -1e9, -1e10, -3e20, -1e30, lo)):
+        x[r, 7:] = max(mask, lo)
+    x[6] = lo                                                  # nothing but masks: uniform
+    x[7] = hi
+    x[7, ::2] = lo
+    x[8, V // 3:] = max(-1e30, lo)
+    x[8, V // 2:] = lo
+    x[8, :V // 3] = -math.inf
+    ids[:6] = 3
+    got = _check(x, ids, T, 6)
+    assert abs(float(got.logprob[6]) + math.log(V)) < 1e-4
+    _check(x, x.argmax(-1), T, 0)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 30, 100, 150, 500])
+def test_large_rows_among_others_in_parts_and_whole(rows):
+    """Rows of one and of several CTAs: a part's maximum may be far above the others'."""
+    V = 40000
+    x, ids = _logits((rows,), V, torch.float32, rows)
+    x[::3] *= 1e6
+    x[0, V - 5:] = 3e38
+    x[0, :V // 2] = -3e38
+    _check(x, ids, 0.5, 3)
