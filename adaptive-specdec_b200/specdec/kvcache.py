@@ -737,8 +737,9 @@ class PagedRaggedCache(RaggedCache):
         (rows of one source row side by side) over the same pools; this cache
         is left empty and must not be used further.  The shared pages go back
         with the new cache's ``reset``.  Raises what this cache's error flag holds
-        (a prefill that found no pages), or when a row holds tokens without
-        a page.  Synchronises (error checks)."""
+        (a prefill that found no pages), when a row holds tokens without a
+        page, and when a forked row was rolled back into the pages it shares
+        (its neighbours read them).  Synchronises (error checks)."""
         if not self.device_pages:
             raise L.SpecdecError("fork needs device_pages=True")
         counts = [int(c) for c in counts]
@@ -748,6 +749,8 @@ class PagedRaggedCache(RaggedCache):
         need = (self.lengths.view(-1, 1) + PAGE - 1) // PAGE
         if bool(((self._columns() < need) & (self.block_table < 0)).any()):
             raise L.SpecdecError("fork: a row holds tokens without a page")
+        if bool((self.lengths < self.pages.shared * PAGE).any()):
+            raise L.SpecdecError("fork: a row was rolled back into the pages it shares")
         host = self._mirror().clone()
         src = torch.repeat_interleave(torch.arange(self.batch_size), torch.tensor(counts))
         new = PagedRaggedCache(len(self.layers), len(src), self.capacity, self.device,

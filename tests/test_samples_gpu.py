@@ -337,3 +337,19 @@ def test_rows_without_their_pages_do_not_fork(engine):
     ids = torch.randint(0, VOCAB, (1, 384))
     with pytest.raises(L.SpecdecError, match="exhausted"):
         small.generate(ids, torch.tensor([384]), 8, sampling=SamplingConfig(), k_fixed=3, n=2)
+
+
+def test_a_row_rolled_back_into_its_shared_pages_does_not_fork():
+    """Its neighbours still read those pages: they are not its to give or to split."""
+    c, _ = _filled([300, 5], 40, H=2)
+    f = c.fork([2, 1])
+    f.rollback([170, 0, 0])                                    # rows of 130, 300 and 5 tokens
+    bt, free, owned = f.block_table.clone(), f.free_pages, f.pages.owned.clone()
+    with pytest.raises(L.SpecdecError, match="shares"):
+        f.fork([1, 1, 1])
+    assert torch.equal(f.block_table, bt) and f.free_pages == free
+    assert torch.equal(f.pages.owned, owned) and f.lengths.tolist() == [130, 300, 5]
+    f.release([0])                                             # a row without tokens may
+    h = f.fork([1, 2, 1])
+    used = [p for p in h.block_table.flatten().tolist() if p >= 0]
+    assert len(set(used)) == 2 + 2 + 1 and h.free_pages == 39 - 5
