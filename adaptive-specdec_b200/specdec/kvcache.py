@@ -612,6 +612,10 @@ class PagedRaggedCache(RaggedCache):
             self.batch_size * self.pages_per_row + 1
         self.device_pages = bool(device_pages)
         self.prefix = None
+        # (rows that read them, first column, end) of the table columns whose pages
+        # several rows of a fork share.  A row's runs follow one another from
+        # column 0, and the readers of a later one read the earlier ones too.
+        self._shared_runs = []
         if self.device_pages:
             self.pages = DevicePageTable(self.batch_size, self.pages_per_row, self.n_pages,
                                          self.device, err=self._err, stack=_stack)
@@ -662,13 +666,17 @@ class PagedRaggedCache(RaggedCache):
 
     def release(self, rows):
         """Return the pages of the given rows to the pool (their lengths go to 0).
-        Shared pages of a forked row stay with the rows that still read them; the
-        row itself leaves its group."""
+        Shared pages of a forked row stay with the rows that still read them and
+        go back with the last of these; the row itself leaves its group."""
         rows = [int(r) for r in rows]
         if self.device_pages:
             if rows and not 0 <= min(rows) <= max(rows) < self.batch_size:
                 raise L.SpecdecError(f"rows must be in [0, {self.batch_size}), got {rows}")
             at = torch.tensor(rows, dtype=torch.long, device=self.device)
+            own = self._last_readers(rows)             # shared pages that are the row's now
+            if own:
+                self.pages.shared[list(own)] = torch.tensor(list(own.values()), dtype=torch.int32,
+                                                            device=self.device)
             keep = self.pages.owned.long() * PAGE
             keep[at] = 0
             self.pages.trim(keep)
@@ -690,6 +698,18 @@ class PagedRaggedCache(RaggedCache):
         self.pages.release(rows)
         self.set_lengths(h)
         self._push()
+
+    def _last_readers(self, rows):
+        """Take `rows` out of the shared runs: {row: first column that nobody else reads}."""
+        own = {}
+        for r in rows:
+            for readers, first, _ in self._shared_runs:
+                if r in readers:
+                    readers.remove(r)
+                    if not readers:
+                        own[r] = min(own.get(r, first), first)
+        self._shared_runs = [run for run in self._shared_runs if run[0]]
+        return own
 
     @staticmethod
     def _runs(first, end, gone):
@@ -736,10 +756,11 @@ class PagedRaggedCache(RaggedCache):
         its last, partly filled page is copied to each.  Returns the new cache
         (rows of one source row side by side) over the same pools; this cache
         is left empty and must not be used further.  The shared pages go back
-        with the new cache's ``reset``.  Raises what this cache's error flag holds
-        (a prefill that found no pages), when a row holds tokens without a
-        page, and when a forked row was rolled back into the pages it shares
-        (its neighbours read them).  Synchronises (error checks)."""
+        with the last of their rows that the new cache releases, or its ``reset``.
+        Raises what this cache's error flag holds (a prefill that found no
+        pages), when a row holds tokens without a page, and when a forked row was
+        rolled back into the pages it shares (its neighbours read them).
+        Synchronises (error checks)."""
         if not self.device_pages:
             raise L.SpecdecError("fork needs device_pages=True")
         counts = [int(c) for c in counts]
@@ -776,6 +797,14 @@ class PagedRaggedCache(RaggedCache):
             b.dtype, b.device, b.is_initialized = a.dtype, a.device, True
             b.keys, b.values = a.keys[:], a.values[:]
             b.keys._sd_cache = b.values._sd_cache = new
+        ends = torch.tensor(counts).cumsum(0).tolist()
+        rows = [set(range(e - n, e)) for n, e in zip(counts, ends)]
+        new._shared_runs = [(set().union(*(rows[r] for r in readers)), first, end)
+                            for readers, first, end in self._shared_runs]
+        for b, n in enumerate((host // PAGE).tolist()):
+            first = max((end for readers, _, end in self._shared_runs if b in readers), default=0)
+            if first < n:
+                new._shared_runs.append((rows[b], first, n))
         # the copies are taken: the partly filled source pages go back
         self.pages.shared.copy_(host // PAGE)
         self.pages.trim(self.lengths // PAGE * PAGE)
@@ -784,7 +813,7 @@ class PagedRaggedCache(RaggedCache):
         self.pages.shared.zero_()
         self.set_lengths(torch.zeros(self.batch_size, dtype=torch.long))
         self.prefix = None
-        ends = torch.tensor(counts).cumsum(0).tolist()
+        self._shared_runs = []
         new._set_groups(list(zip([0] + ends[:-1], ends, (host // PAGE).tolist())))
         return new
 
@@ -798,6 +827,7 @@ class PagedRaggedCache(RaggedCache):
     def reset(self):
         super().reset()
         self.prefix = None
+        self._shared_runs = []
         if self.device_pages:
             self.pages.reset()
             return

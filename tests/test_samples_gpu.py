@@ -353,3 +353,60 @@ def test_a_row_rolled_back_into_its_shared_pages_does_not_fork():
     h = f.fork([1, 2, 1])
     used = [p for p in h.block_table.flatten().tolist() if p >= 0]
     assert len(set(used)) == 2 + 2 + 1 and h.free_pages == 39 - 5
+
+
+@pytest.mark.parametrize("order", [[range(7)], [[0], [1, 2], [3], [4, 5, 6]], [[6], [5, 0, 2], [4, 1], [3]],
+                                   [[3, 3], [0, 1, 2, 0], [5, 4], [6, 6, 6]]])
+def test_the_last_row_of_a_prompt_gives_its_pages_back(order):
+    c, _ = _filled([260, 5, 700], 30, H=2)                     # 2, 0 and 5 shared pages
+    f = c.fork([3, 1, 3])
+    f.reserve(200)
+    f.check_errors()
+    left = set(range(7))
+    for rows in order:
+        held = set(f.block_table[sorted(left)].flatten().tolist()) - {-1}
+        f.release(rows)
+        left -= set(rows)
+        now = set(f.block_table[sorted(left)].flatten().tolist()) - {-1}
+        assert now <= held and f.free_pages == 29 - len(now)
+        assert not now & set(f.pages.free[:f.free_pages].tolist())
+        f.release(rows)                                        # a second time: nothing to give
+        assert f.free_pages == 29 - len(now)
+    assert f.free_pages == 29 and sorted(f.pages.free[:29].tolist()) == list(range(29))
+    # every page is handed out once again
+    f.reserve(4 * PAGE)
+    f.check_errors()
+    got = f.block_table[:, :4].flatten().tolist()
+    assert len(set(got)) == 28 and -1 not in got
+
+
+def test_pages_of_a_fork_of_a_fork_come_back_once():
+    c, _ = _filled([260, 300], 60, H=2)
+    f = c.fork([2, 1])
+    f.reserve(300)
+    k = torch.randn(3, 2, 300, 128, device=DEV).bfloat16()
+    f.layers[0].update(k, k)
+    f.advance(300)                                             # rows of 560, 560 and 600 tokens
+    h = f.fork([2, 3, 1])                                      # rows 0 to 4 hold the first two pages
+    h.check_errors()
+    h.reserve(100)
+    free = [h.free_pages]
+    for rows in ([1], [0], [2, 4], [3], [5]):
+        h.release(rows)
+        free.append(h.free_pages)
+        used = set(h.block_table.flatten().tolist()) - {-1}
+        assert free[-1] == 59 - len(used) and not used & set(h.pages.free[:free[-1]].tolist())
+    # own page(s) of 560 + 100 tokens past four shared ones: 2; a source row's own two
+    # full pages leave with its last reader, the prompt's two with the last of all
+    assert [b - a for a, b in zip(free, free[1:])] == [2, 4, 4, 6, 6]
+
+
+def test_rows_released_before_a_fork_leave_their_pages_to_the_others():
+    c, _ = _filled([300, 5], 40, H=2)
+    f = c.fork([2, 1])
+    f.release([0])
+    h = f.fork([1, 2, 1])
+    h.release([0, 3, 1])
+    assert h.free_pages == 39 - 3                              # row 2 still reads the prompt
+    h.release([2])
+    assert h.free_pages == 39
