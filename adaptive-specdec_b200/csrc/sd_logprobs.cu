@@ -32,9 +32,14 @@
 // few more; only threads whose maximum reaches it look through their units
 // again (from L2), a warp together.
 //
-// Bound by HBM with many rows: 2048 rows of 151936 bf16 in 114 us, 5.4 TB/s (the
-// copy rate here is 6.57); by latency with few: one row in 7 us, 320 rows with five
-// alternatives in 27 (3.6 TB/s: 2.2 rows per SM, whose tails show).
+// The list holds 2048 elements; where more reach the threshold (flat logits; fewer
+// than n of the groups with anything above -inf, as under a mask that leaves a few
+// neighbouring ids), the part is read once per alternative: 320 rows with 15 live
+// entries take 408 us with five alternatives, 1127 with twenty.
+//
+// Bound by HBM with many rows: 2048 rows of 151936 bf16 in 117 us, 5.3 TB/s (the
+// copy rate here is 6.57); by latency with few: one row in 6 us, 320 rows with five
+// alternatives in 29 (3.4 TB/s: 2.2 rows per SM, whose tails show).
 #include <cuda_runtime.h>
 #include <cooperative_groups.h>
 #include <math_constants.h>
@@ -765,18 +770,23 @@ __global__ void __launch_bounds__(LP_THREADS) logp_warp_kernel(const LpParams P,
 
 // How the rows are cut.  Up to one row per SM, every row is split, over as many
 // CTAs as fit the machine at once; beyond, whole rows while there is one for
-// every SM and the rest in halves, so that the SMs end together.  Measured
-// (bf16, V = 151936, five alternatives; us): 8 rows in 8 parts 8.0, in 4 9.8, in
-// 1 16.2; 100 rows in 4 parts 13.4, in 2 15.5, in 8 21.5; 148 rows in 2 parts
-// 15.9, in 4 21.8, in 1 18.4; 320 rows, 296 of them whole and 24 in halves 26.2,
-// all whole 31.2, all in halves 33.0.  A part has at least a unit per thread.
+// every SM and the rest in halves, so that the SMs end together.  Clusters of four
+// do not fill all of the machine's 592 places (four CTAs per SM): 142 of them run
+// at once, so four parts end at 15/16 of the places, 138 rows.  Measured (bf16, V =
+// 151936, five alternatives; us): 8 rows in 8 parts 8.5, in 4 8.8, in 2 11.4, in 1
+// 15.5; 18 rows in 8 9.5, in 4 9.7; 30 rows in 4 10.9, in 2 13.7; 100 rows in 4
+// 14.5, in 2 17.0, in 1 21.0; 138 rows in 4 17.3, in 2 17.8; 142 in 4 17.4, 143 in 4
+// 21.5, in 2 18.1; 148 rows in 4 22.2, in 2 18.1, in 1 21.9; 320 rows, 296 of
+// them whole and 24 in halves 29.2, all whole 33.5, all in halves 37.1 (700 rows:
+// 51, 55.5, 60.7).  Shorter rows gain less: 111 rows of 32003 fp32 take 12.7 in 4
+// parts and 12.1 in 2, 37 rows 9.6 and 9.9.  A part has at least a unit per thread.
 struct LpPlan { int csize, whole; int64_t ctas; };
 static LpPlan lp_plan(int64_t rows, int V, int dtype) {
   const int units = V / (dtype == SD_DTYPE_F32 ? 4 : 8);
   LpPlan p = {2, 0, 0};
   if (rows * 8 <= LP_SMS)
     p.csize = 8;
-  else if (rows * 4 <= LP_SMS * LP_CTAS)
+  else if (rows * 4 <= LP_SMS * LP_CTAS * 15 / 16)
     p.csize = 4;
   while (p.csize > 1 && units / p.csize < LP_THREADS) p.csize /= 2;
   const int64_t full = p.csize == 1 ? rows : rows <= LP_SMS ? 0 : rows / LP_SMS * LP_SMS;
@@ -785,10 +795,12 @@ static LpPlan lp_plan(int64_t rows, int V, int dtype) {
   return p;
 }
 
-// Up to LP_WARP_V entries a warp takes a row: 4000 rows of 300 bf16 in 5.3 us (a CTA
-// each: 27.5), 4000 x 1000 with five alternatives 19 (58), 1000 x 1000 8.6 (18.8), one
-// row of 1000 7.6 (6.1).  Beyond, 64 entries in a thread's registers leave one CTA per
-// SM: 4000 x 2000 in 48 us against 45.
+// Up to LP_WARP_V entries a warp takes a row: 4000 rows of 300 bf16 in 5.1 us (a CTA
+// each: 27.8), 4000 x 1000 9.3 (28.0), with five alternatives 18.9 (70.6), 1000 x 1000
+// with five 8.6 (20.7), one row of 1000 with five 7.3 (8.1), without 3.7 (3.5).  Beyond,
+// 64 entries in a thread's registers leave one CTA per SM: 4000 x 2000 bf16 in 25 us
+// against 28, with five alternatives 52 against 70, but fp32 25 and 52 against 25 and
+// 43.
 template <typename T>
 static int launch_warps(const LpParams& P, cudaStream_t st) {
   const int64_t rows = (int64_t)P.B * P.L, ctas = (rows + LP_WARPS - 1) / LP_WARPS;

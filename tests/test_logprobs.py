@@ -398,3 +398,11 @@ def test_large_rows_among_others_in_parts_and_whole(rows):
     x[0, V - 5:] = 3e38
     x[0, :V // 2] = -3e38
     _check(x, ids, 0.5, 3)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [18, 19, 137, 138, 139, 142, 148, 149, 296, 297])
+def test_rows_around_the_bounds_of_the_split(rows):
+    """Eight, four and two parts, whole rows with a rest in halves."""
+    x, ids = _logits((rows,), 17001, torch.bfloat16, rows)
+    _check(x, ids, 0.8, 3)
