@@ -392,3 +392,25 @@ def test_arguments_are_checked_before_any_launch():
     size = lib.sd_prefix_attn_workspace_bytes
     assert size(64, 1, 32, 8, 128, 66, 5, 2) > 0 and size(64, 1, 32, 7, 128, 66, 5, 2) == 0
     assert size(64, 1, 32, 8, 64, 66, 5, 2) == 0 and call(D=136) == -95 and call(D=256, dtype=0) == -95
+
+
+@gpu
+@pytest.mark.parametrize("hq,hkv,qlen", [(4, 1, 40), (8, 2, 33), (32, 1, 5), (128, 1, 2), (8, 8, 129),
+                                         (6, 2, 100)])
+def test_more_query_rows_than_a_chunk(hq, hkv, qlen):
+    """More than 128 query rows of a kv head: the own ranges take them in chunks, the
+    last one shorter."""
+    _check(_case([2, 1], [2, 1], [5, 126, 300], qlen, hq, hkv, seed=qlen))
+    _check(_case([3], [1], [0, 60, 200], qlen, hq, hkv, seed=qlen), valid=[0, PAGE + 70, 10 ** 6])
+
+
+@gpu
+@pytest.mark.parametrize("sizes,pages", [([200], [2]), ([3] * 70, [1, 0, 2, 1, 3] * 14),
+                                         ([2] * 330, [1] * 330), ([1100], [1]),
+                                         ([2] * 520 + [40], [1, 0] * 260 + [2]),
+                                         ([1] * 1030 + [5], [1] * 1030 + [1])])
+def test_many_rows_and_groups(sizes, pages):
+    """Past the plan's 1024 rows or groups at a time, past the threads of the kernels
+    that look for a CTA's first row or group."""
+    n = sum(sizes)
+    _check(_case(sizes, pages, [(7 * b) % 130 for b in range(n)], 1, 2, 1, seed=n, stale=0.0))
