@@ -11,14 +11,15 @@
 //   prefix_plan_kernel  lays out the work of both from the device lengths, and
 //                       copies the queries kv head by kv head, so that TMA
 //                       brings any run of a group's query rows;
-//   prefix_tc_kernel    the shared pages, query rows of the whole group on
-//                       the M side of tcgen05.mma: K and V are read once per
-//                       256 query rows instead of once per row;
-//   own_tc_kernel       the rows' own pages, four rows at a time;
+//   prefix_tc_kernel    some CTAs: the shared pages, query rows of the whole group
+//                       on the M side of tcgen05.mma: K and V are read once per
+//                       256 query rows instead of once per row; the others: the
+//                       rows' own pages, four rows at a time;
 //   prefix_join_kernel  merges the partials, in piece order, into the output.
-// Each is launched as a programmatic dependent of the one before.  64 rows of 5
-// queries, 32 / 8 heads, 64 shared pages and up to 1 K own keys: 91 us for the
-// call; kernel by kernel, with cold caches, 6 + 45 + 34 + 14.
+// Each is launched as a programmatic dependent of the one before and reads what
+// that one wrote (and what it had waited for) behind its own wait.  64 rows of 5
+// queries, 32 / 8 heads, 64 shared pages and up to 1 K own keys: 96 us for the
+// call; kernel by kernel, with cold caches, 7 + 82 + 14.
 // A row whose first query does not see the whole shared range (an empty or a
 // padding row, a short cap) takes no part in it: its own range starts at 0, so
 // the shared range needs no mask and no row meets another row's masked keys.
@@ -45,8 +46,8 @@ constexpr float PX_HEADROOM = 8.f;           // lazy-rescale headroom of the run
 constexpr int PX_JOIN_THREADS = 256;
 constexpr int PX_JOIN_CTAS = 4;              // per SM
 constexpr int PX_JOIN_LOADS = 4;             // pieces of a row on their way at once
-constexpr int OW_STAGES = 3;                 // K + V tiles in flight (own ranges)
-constexpr int OW_THREADS = 192;              // warps 0-3 softmax, 4 TMA, 5 MMA
+constexpr int OW_STAGES = 3;                 // K + V tiles in flight (own ranges: of the
+                                             // PX_THREADS warps 0-3 softmax, 4 TMA, 5 MMA)
 constexpr int OW_OVH = 2;                    // schedule cost of a (row, kv head) beyond its pages
 constexpr int OW_MIN_SHARE = OW_OVH + 1;
 
@@ -61,14 +62,23 @@ struct PrefixParams {
   int* g_row0;                               // [G]
   int* g_rows;                               // [G]
   int* g_pages;                              // [G] 0: the group shares nothing
-  int* rowgroup;                             // [B] the row's group, -1: it takes no part
+  int4* rowjoin;                             // [B][2] what the join needs of the row, see PxRow
+  int4* totals;                              // own and shared ranges: schedule units, units per CTA
   int* rowstart;                             // [B] first key of the row's own range, a page bound
-  int qc, nq;                                // queries per chunk; lane quarters of a chunk's rows
+  int qc, nq, chunks;                        // queries per chunk; lane quarters of a chunk's rows
   int slots;                                 // partial slots of a chunk of the own ranges
   uint4* qp;                                 // queries [Hkv][B][qlen][group][D]
   float* pacc;                               // [slot][2 tiles][4 chunks][128 rows][32]
   float* pml;                                // [slot][PX_ROWS][2]
 };
+
+// What the join needs of a row, in one load: its units of the own ranges and the
+// ones before them; its group's units and items before, rows (0: it takes no
+// part) and pages, and the row's place in it.
+struct __align__(16) PxRow {
+  int pre, tb, unit, item, rows, pages, place, unused;
+};
+static_assert(sizeof(PxRow) == 2 * sizeof(int4), "two loads");
 
 // The items of a group: (kv head, 256 query rows), kv head outer.
 __device__ __forceinline__ int px_pairs(const PrefixParams& P, int rows) {
@@ -81,14 +91,13 @@ __device__ __forceinline__ int px_share(int total) {
 // Units per CTA of the own ranges.  Where the shared ranges leave SMs idle, only
 // the CTAs that come up on those get work, if it then ends before the ones that
 // have to wait for a busy SM would (a shared page takes about 1.5 own ones).  32 / 8
-// heads, 1 query: 8 rows, 16 shared pages, up to 1000 own keys 21.4 us for the call
-// (27.1 with the work over all SMs); 64 rows, 8 pages, up to 300 keys 31.6 (36.3); 16
-// rows the same 19.5 (19.4).
-__device__ __forceinline__ int ow_share(const PrefixParams& P, int total) {
+// heads, 1 query: 8 rows, 16 shared pages, up to 1000 own keys 23.1 us for the call
+// (27.2 with the work over all SMs); 64 rows, 8 pages, up to 300 keys 35.0 (39.7); 16
+// rows the same 21.3 (21.0), 4 rows, 4 pages, up to 100 keys 20.4 (19.8).
+__device__ __forceinline__ int ow_share(const PrefixParams& P, int total, int units, int ps) {
   int share = max(OW_MIN_SHARE, (total + PX_CTAS - 1) / PX_CTAS);
-  const int units = P.g_unit[P.G];
   if (units > 0 && P.qc >= P.A.qlen) {
-    const int ps = px_share(units), idle = PX_CTAS - (units + ps - 1) / ps;
+    const int idle = PX_CTAS - (units + ps - 1) / ps;
     if (idle > 0) {
       const int apart = max(share, (total + idle - 1) / idle);
       if (apart - share < ps + ps / 2) share = apart;
@@ -158,6 +167,7 @@ __global__ void __launch_bounds__(PX_PLAN_THREADS) prefix_plan_kernel(const Pref
   for (int b0 = 0; b0 < A.B; b0 += 1024) {
     const int b = b0 + t;
     int tiles = 0;
+    PxRow row = {};
     if (b < A.B) {
       int lo = 0, hi = P.G;                          // the last group that starts at or before b
       while (lo < hi) {
@@ -170,7 +180,13 @@ __global__ void __launch_bounds__(PX_PLAN_THREADS) prefix_plan_kernel(const Pref
         const int keys = P.g_pages[g] * SD_KV_PAGE;
         if (row_limit(A, b, 0) >= keys) start = keys;
       }
-      P.rowgroup[b] = start > 0 ? g : -1;
+      if (start > 0) {
+        row.unit = P.g_unit[g];
+        row.item = P.g_item[g];
+        row.rows = P.g_rows[g];
+        row.pages = P.g_pages[g];
+        row.place = b - P.g_row0[g];
+      }
       const int km = row_limit(A, b, A.qlen - 1);
       P.rowstart[b] = start;
       A.rowkmax[b] = km;
@@ -179,11 +195,20 @@ __global__ void __launch_bounds__(PX_PLAN_THREADS) prefix_plan_kernel(const Pref
     }
     int sum;
     const int ex = block_excl_scan<int>(tiles, redi, &sum);
-    if (b < A.B) A.rowpre[b] = carry + ex;
+    if (b < A.B) {
+      A.rowpre[b] = row.pre = carry + ex;
+      row.tb = tiles;
+      P.rowjoin[2 * b] = make_int4(row.pre, row.tb, row.unit, row.item);
+      P.rowjoin[2 * b + 1] = make_int4(row.rows, row.pages, row.place, 0);
+    }
     carry += sum;
     __syncthreads();
   }
-  if (t == 0) A.rowpre[A.B] = carry;
+  if (t == 0) {
+    A.rowpre[A.B] = carry;
+    const int own = carry * A.Hkv, shared = share ? (int)units0 : 0, ps = px_share(shared);
+    *P.totals = make_int4(own, shared, ow_share(P, own, shared, ps), ps);
+  }
 }
 
 // A CTA's run of schedule units as segments of items, walked identically by
@@ -240,23 +265,22 @@ struct PxSmem {
   alignas(8) unsigned long long full[PX_SLOTS], empty[PX_SLOTS];
   alignas(128) unsigned char out[8][32 * 128];               // a warp's 32 rows x 32 floats of O
   alignas(8) unsigned long long sfull[2], pfull[2], oready[2], qfull[2], fin;
-  uint32_t tmem;
   int first[4];                                      // the CTA's first group: g, unit, rows, pages
   int abort_;
 };
-static_assert(sizeof(PxSmem) + 1024 <= 227 * 1024, "prefix attention shared memory");
+static_assert(sizeof(PxSmem) + 2048 <= 227 * 1024, "shared memory, with room to align");
 
 __device__ __forceinline__ void px_max3(float& m, uint32_t a, uint32_t b) {
   asm("max.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
 }
 
-// (2^a, 2^b) on the FMA pipe, held at 2^-126: with a = i + f, i the nearest
-// integer, 2^f by a polynomial of degree 4 on [-1/2, 1/2] (least relative error,
-// 2.7e-6) times 2^i, whose bits the rounding constant leaves in place.  A NaN
-// stays one.
+// (2^a, 2^b) on the FMA pipe: with a = i + f, i the nearest integer, 2^f by a
+// polynomial of degree 4 on [-1/2, 1/2] (least relative error, 2.7e-6) times
+// 2^i, whose bits the rounding constant leaves in place.  Held at i = -127, whose
+// bits are those of 0: a masked score (-inf) weighs nothing.  A NaN stays one.
 __device__ __forceinline__ unsigned long long px_exp2(float a, float b) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
   const float magic = 12582912.f + 127.f;            // 1.5 * 2^23: the sum's low byte is i + 127
   const unsigned long long x2 = pair2(a, b), r2 = add2(x2, pair2(magic, magic));
   const unsigned long long i2 = add2(r2, pair2(-magic, -magic));
@@ -270,6 +294,30 @@ __device__ __forceinline__ unsigned long long px_exp2(float a, float b) {
   unpair(r2, ra, rb);
   return mul2(p2, pair2(__uint_as_float(__float_as_uint(ra) << 23),
                         __uint_as_float(__float_as_uint(rb) << 23)));
+}
+
+// The weights p = 2^(s sl2 - m) of 32 scores as bf16 pairs, and their sums.  A
+// quarter by the FMA pipe: the exponentials of a page take 2048 cycles of the
+// special-function units otherwise (shared ranges: a call of 101.3 us took 102.5
+// without, 103 with half of them there).
+__device__ __forceinline__ void px_weights(const uint32_t (&s)[32], uint32_t* p,
+                                           unsigned long long (&sum)[2], unsigned long long sl22,
+                                           unsigned long long nm2) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    float a, b;
+    const unsigned long long s2 = pair2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+    unpair(fma2(s2, sl22, nm2), a, b);
+    const unsigned long long p2 = e % 4 == 1 ? px_exp2(a, b) : pair2(ex2f(a), ex2f(b));
+    sum[e & 1] = add2(sum[e & 1], p2);
+    unpair(p2, a, b);
+    p[e] = pack_bf16(a, b);
+  }
+}
+
+// A group's first unit, the next one's, rows and pages
+__device__ __forceinline__ int4 px_group(const PrefixParams& P, int g) {
+  return make_int4(P.g_unit[g], P.g_unit[g + 1], P.g_rows[g], P.g_pages[g]);
 }
 
 // Persistent, stream-K: the (item, page) units lie end to end and each CTA
@@ -292,12 +340,12 @@ __device__ __forceinline__ unsigned long long px_exp2(float a, float b) {
 // their latencies.  Two warps per 32 rows, each with half of the keys, left the
 // softmax as long (1850: the pipes of the SM quarter are shared); weights and
 // maximum in one pass over S, 3600.  128 rows of 5 queries over 128 pages, 32 / 8
-// heads: 150 us, 1.15 PFLOP/s.
+// heads: 150 us as a launch of its own, 1.15 PFLOP/s.
 // An item with rows for one tile only is worked on by both: tile 0 takes the
 // first, tile 1 the second half of every page's keys.
-__global__ void __launch_bounds__(PX_THREADS, 1)
-prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CUtensorMap tmk,
-                 const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmq) {
+__device__ __forceinline__ void shared_ranges(const PrefixParams& P, const CUtensorMap& tmk,
+                                              const CUtensorMap& tmv, const CUtensorMap& tmq,
+                                              int4 totals, int4 group, const uint32_t* tmem) {
   extern __shared__ __align__(1024) unsigned char px_raw[];
   const uint32_t pad = (1024u - (smem_addr(px_raw) & 1023u)) & 1023u;   // swizzle atoms: 1024 B
   PxSmem& S = *reinterpret_cast<PxSmem*>(px_raw + pad);
@@ -318,37 +366,20 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
     S.abort_ = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (w == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                 :: "r"(smem_addr(&S.tmem)), "r"(512u) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  // the plan and the packed queries from here on; the next kernel, which needs
-  // the plan only, may come up on SMs that run out of work
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int total = P.g_unit[P.G];
-  const int share = px_share(total);
-  const int t0 = (int)blockIdx.x * share, t1 = min(total, t0 + share);
+  const int t0 = (int)blockIdx.x * totals.w, t1 = min(totals.y, t0 + totals.w);
   for (int g = t; g < P.G; g += PX_THREADS) {
-    const int u0 = P.g_unit[g], u1 = P.g_unit[g + 1], rows = P.g_rows[g], pages = P.g_pages[g];
-    if (u0 <= t0 && t0 < u1) {
+    if (g != t) group = px_group(P, g);
+    if (group.x <= t0 && t0 < group.y) {
       S.first[0] = g;
-      S.first[1] = u0;
-      S.first[2] = rows;
-      S.first[3] = pages;
+      S.first[1] = group.x;
+      S.first[2] = group.z;
+      S.first[3] = group.w;
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tm = S.tmem;
-  if (t0 >= total) {                                 // no work for this CTA (uniform)
-    if (w == 0)
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
-                   :: "r"(tm), "r"(512u) : "memory");
-    return;
-  }
+  const uint32_t tm = *tmem;
   PxSeg seg;
   px_init(seg, P, S.first, t0, t1);
 
@@ -538,28 +569,13 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
         const unsigned long long sl22 = pair2(sl2, sl2), nm2 = pair2(-mc, -mc);
         unsigned long long ls[2] = {0ULL, 0ULL};     // (0.f, 0.f)
         uint32_t pk[32];
-        auto weights = [&](const uint32_t (&s)[32], uint32_t* p) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float a, b;
-            const unsigned long long s2 = pair2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
-            unpair(fma2(s2, sl22, nm2), a, b);
-            // a quarter by the FMA pipe: the exponentials of a page take 2048
-            // cycles of the special-function units otherwise (a call of 101.3 us
-            // took 102.5 without, 103 with half of them there)
-            const unsigned long long p2 = e % 4 == 1 ? px_exp2(a, b) : pair2(ex2f(a), ex2f(b));
-            ls[e & 1] = add2(ls[e & 1], p2);
-            unpair(p2, a, b);
-            p[e] = pack_bf16(a, b);
-          }
-        };
 #pragma unroll 1
         for (int c = 0; c < halves; ++c) {
           TC_LD32(sa, scol + 64u * c);
           TC_LD32(sb, scol + 64u * c + 32u);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          weights(sa, pk);
-          weights(sb, pk + 16);
+          px_weights(sa, pk, ls, sl22, nm2);
+          px_weights(sb, pk + 16, ls, sl22, nm2);
           TC_ST32(scol + 32u * c, pk);               // over columns that have been read
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -613,14 +629,8 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__
       }
     }
   }
-  // ---------------- teardown: TMEM back once every role is done with it
   tc_fence_before();
-  __syncthreads();
-  if (w == 0) {
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
-                 :: "r"(tm), "r"(512u) : "memory");
-  }
+  __syncthreads();                                   // every role is done
   if (t == 0 && S.abort_) atomicOr(A.status, 1);
 }
 
@@ -670,11 +680,15 @@ struct OwSmem {
   alignas(8) unsigned long long full[OW_STAGES][2], empty[OW_STAGES][2];   // K, V
   // by stream and the stream's page parity (at most two phases of each are open)
   alignas(8) unsigned long long sfull[4][2], pfull[4][2], oready[4][2], qfull[4], fin;
-  uint32_t tmem;
   int first[5];                                      // the CTA's first row: b, unit, tb, k0, kmax
   int abort_;
 };
-static_assert(sizeof(OwSmem) + 1024 <= 227 * 1024, "own-range attention shared memory");
+static_assert(sizeof(OwSmem) + 2048 <= 227 * 1024, "shared memory, with room to align");
+
+// A row's first unit per kv head, the next one's, first key and end of its own range
+__device__ __forceinline__ int4 ow_row(const PrefixParams& P, int b) {
+  return make_int4(P.A.rowpre[b], P.A.rowpre[b + 1], P.rowstart[b], P.A.rowkmax[b]);
+}
 
 // Stream-K over the pages of all (row, kv head) segments.  A segment has at
 // most 128 query rows and needs 1, 2 or 4 quarters of the 128 accumulator lanes
@@ -691,51 +705,35 @@ static_assert(sizeof(OwSmem) + 1024 <= 227 * 1024, "own-range attention shared m
 // is not the bound: 1024 cycles a page against about 2600 for its 64 KB from HBM.
 // K leaves its slot when S is done, V when P . V is; slots behind a row's live
 // keys that TMA brings in are zeroed in V before P . V reads them (they may hold
-// NaN).  64 rows of 520 own keys, 8 heads (136 MB): 34 us, 4 TB/s; in its middle
-// a page takes 2130 cycles, the bandwidth of HBM, but the first three pages of a
-// CTA take 10 us (cold code and first loads), which so short a run does not hide.
-__global__ void __launch_bounds__(OW_THREADS, 1)
-own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CUtensorMap tmk,
-              const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmq) {
+// NaN).  64 rows of 5 queries and 520 own keys, 32 / 8 heads (136 MB): 45 us for the
+// call, 34 as a launch of its own (4 TB/s); in its middle a page takes 2130 cycles,
+// the bandwidth of HBM, but the first three pages of a CTA take 10 us (cold code and
+// first loads), which so short a run does not hide.
+__device__ __forceinline__ void own_ranges(const PrefixParams& P, const CUtensorMap& tmk,
+                                           const CUtensorMap& tmv, const CUtensorMap& tmq,
+                                           int4 totals, int4 row, int cta, int chunk,
+                                           const uint32_t* tmem) {
   extern __shared__ __align__(1024) unsigned char px_raw[];
   const uint32_t pad = (1024u - (smem_addr(px_raw) & 1023u)) & 1023u;   // swizzle atoms: 1024 B
   OwSmem& S = *reinterpret_cast<OwSmem*>(px_raw + pad);
   const AttnParams& A = P.A;
   const int t = threadIdx.x, w = t >> 5, lane = t & 31;
-  // This kernel reads the plan, which was complete before the shared ranges'
-  // kernel let it start; it waits for that kernel only before it ends, so that
-  // its own end stands for both.
-  if (P.G == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // one round trip for all that the start needs: what the rows say is on its way
-  // with the total
-  int b = t, first[4] = {0, 0, 0, 0};                // rowpre, its next, k0, kmax
-  auto fetch = [&]() {
-    if (b >= A.B) return;
-    first[0] = A.rowpre[b];
-    first[1] = A.rowpre[b + 1];
-    first[2] = P.rowstart[b];
-    first[3] = A.rowkmax[b];
-  };
-  fetch();
-  const int total = A.rowpre[A.B] * A.Hkv;
-  const int share = ow_share(P, total);
-  if ((int64_t)blockIdx.x * share >= total) {        // no work for this CTA (uniform)
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    return;
-  }
-  const int t0 = (int)blockIdx.x * share, t1 = t0 + min(total - t0, share);
-  const int j0 = (int)blockIdx.y * P.qc;             // the chunk's first query
+  const int total = totals.x, share = totals.z;
+  if ((int64_t)cta * share >= total) return;         // no work for this CTA (uniform)
+  const int t0 = cta * share, t1 = t0 + min(total - t0, share);
+  const int j0 = chunk * P.qc;                       // the chunk's first query
   const int R = min(P.qc, A.qlen - j0) * A.group;    // its query rows per kv head
   const int nq = P.nq, ns = 4 / nq;                  // quarters per segment, streams
-  for (; b < A.B; b += OW_THREADS, fetch())
-    if (first[0] * A.Hkv <= t0 && t0 < first[1] * A.Hkv) {
+  for (int b = t; b < A.B; b += PX_THREADS) {
+    if (b != t) row = ow_row(P, b);
+    if (row.x * A.Hkv <= t0 && t0 < row.y * A.Hkv) {
       S.first[0] = b;
-      S.first[1] = first[0] * A.Hkv;
-      S.first[2] = first[1] - first[0];
-      S.first[3] = first[2];
-      S.first[4] = first[3];
+      S.first[1] = row.x * A.Hkv;
+      S.first[2] = row.y - row.x;
+      S.first[3] = row.z;
+      S.first[4] = row.w;
     }
+  }
   if (t == 0) {
     for (int i = 0; i < OW_STAGES; ++i)
       for (int kv = 0; kv < 2; ++kv) {
@@ -754,15 +752,10 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
     S.abort_ = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (w == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                 :: "r"(smem_addr(&S.tmem)), "r"(512u) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tm = S.tmem;                        // S0, S1 (128 columns each), O (128)
+  const uint32_t tm = *tmem;                         // S0, S1 (128 columns each), O (128)
   OwSeg seg;
   seg.b = S.first[0];
   seg.tb = S.first[2];
@@ -903,7 +896,7 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
     tc_commit_warp(&S.fin);
     int dummy = 0;
     tc_wait(&S.fin, 0u, &dummy);
-  } else {
+  } else if (w < 4) {
     // ---------------- softmax warps: lane quarter w, query row r of the chunk
     const int s = w / nq, r = (w % nq) * 32 + lane;
     const uint32_t lcol = tm + ((uint32_t)(32 * w) << 16), ocol = lcol + 256u;
@@ -979,20 +972,26 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        uint32_t sc[128];
-        TC_LD32((sc + 0), scol);
-        TC_LD32((sc + 32), scol + 32u);
-        TC_LD32((sc + 64), scol + 64u);
-        TC_LD32((sc + 96), scol + 96u);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        // the scores twice from TMEM, 64 columns at a time: for the maximum, then for
+        // the exponentials (all 128 in registers are too many beside 320 threads)
+        uint32_t sa[32], sb[32];
+        float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          TC_LD32(sa, scol + 64u * c);
+          TC_LD32(sb, scol + 64u * c + 32u);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            px_max3(mx[e & 2], sa[e], sa[e + 1]);
+            px_max3(mx[(e & 2) + 1], sb[e], sb[e + 1]);
+          }
+        }
         // the segment's S are all done with Q: the next segment's may come
         if (i == cur.n - 1 && more) {
           load_q(seg.b, seg.h);
           ++qn;
         }
-        float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-        for (int e = 0; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(sc[e]));
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
         const bool move = mt > m + PX_HEADROOM;
         if (__any_sync(0xffffffffu, move)) {
@@ -1018,23 +1017,24 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
           }
         }
         const float mc = fmaxf(m, -1e30f);           // 2^(-inf - mc) = 0
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float x = ex2f(fmaf(__uint_as_float(sc[64 * hf + 2 * e]), sl2, -mc));
-            const float y = ex2f(fmaf(__uint_as_float(sc[64 * hf + 2 * e + 1]), sl2, -mc));
-            ls[e & 3] += x + y;
-            pk[e] = pack_bf16(x, y);
-          }
-          TC_ST32(scol + 32u * hf, pk);
+        const unsigned long long sl22 = pair2(sl2, sl2), nm2 = pair2(-mc, -mc);
+        unsigned long long ls[2] = {0ULL, 0ULL};     // (0.f, 0.f)
+        uint32_t pk[32];
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          TC_LD32(sa, scol + 64u * c);
+          TC_LD32(sb, scol + 64u * c + 32u);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          px_weights(sa, pk, ls, sl22, nm2);
+          px_weights(sb, pk + 16, ls, sl22, nm2);
+          TC_ST32(scol + 32u * c, pk);               // over columns that have been read
         }
-        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         tc_arrive(&S.pfull[s][n & 1u]);
+        float la, lb;
+        unpair(add2(ls[0], ls[1]), la, lb);
+        l += la + lb;
       }
       if (!ok) break;
       // ---- the segment's partial: slot (chunk, row * Hkv + head + CTA)
@@ -1042,7 +1042,7 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
                       tc_wait(&S.oready[s][(n - 1) & 1u], ((n - 1) >> 1) & 1u, &S.abort_));
       if (!ok) break;
       tc_fence_after();
-      const int64_t at = ((int64_t)blockIdx.y * P.slots + cur.b * A.Hkv + cur.h + blockIdx.x) *
+      const int64_t at = ((int64_t)chunk * P.slots + cur.b * A.Hkv + cur.h + cta) *
                              (P.qc * A.group) + r;
       float4* dst = reinterpret_cast<float4*>(A.part_acc + at * PX_D);
 #pragma unroll 1
@@ -1072,16 +1072,49 @@ own_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CU
       }
     }
   }
-  // ---------------- teardown: TMEM back once every role is done with it
   tc_fence_before();
-  __syncthreads();
+  __syncthreads();                                   // every role is done
+  if (t == 0 && S.abort_) atomicOr(A.status, 1);
+}
+
+// Both ranges in one launch, of which every CTA waits for the plan by itself: as
+// many CTAs as the shared ranges need take those, the next ones the own ranges, at
+// once on the SMs that the shared ones leave idle, else as SMs run out of shared
+// work (a CTA's shared memory fills an SM).  As two launches, whose second would have
+// to wait for the first to see the plan, 2 rows and one shared page took 24.5 us
+// instead of 16.4, a step of 32 rows, 16 / 8 heads, four shared pages and up to 300
+// own keys 36.7 instead of 26.0.
+__global__ void __launch_bounds__(PX_THREADS, 1)
+prefix_tc_kernel(const __grid_constant__ PrefixParams P, const __grid_constant__ CUtensorMap tmk,
+                 const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmq,
+                 const __grid_constant__ CUtensorMap tmq32) {
+  __shared__ uint32_t tmem;
+  const int t = threadIdx.x, w = t >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (w == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_addr(&tmem)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the plan and the packed queries
+  // one round trip for all that the start needs: what groups and rows say is on
+  // its way with the totals
+  const int4 totals = *P.totals;
+  int4 group = make_int4(0, 0, 0, 0), row = group;
+  if (t < P.G) group = px_group(P, t);
+  if (t < P.A.B) row = ow_row(P, t);
+  const int i = (int)blockIdx.x - (totals.y + totals.w - 1) / totals.w;
+  if (i < 0)
+    shared_ranges(P, tmk, tmv, tmq, totals, group, &tmem);
+  else if (i < PX_CTAS * P.chunks)
+    own_ranges(P, tmk, tmv, tmq32, totals, row, i % PX_CTAS, i / PX_CTAS, &tmem);
+  tc_fence_before();
+  __syncthreads();                                   // nobody uses TMEM any more
   if (w == 0) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
-                 :: "r"(tm), "r"(512u) : "memory");
+                 :: "r"(tmem), "r"(512u) : "memory");
   }
-  if (t == 0 && S.abort_) atomicOr(A.status, 1);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // A warp per query row: the pieces of the shared range and of the row's own range,
@@ -1095,24 +1128,26 @@ __global__ void __launch_bounds__(PX_JOIN_THREADS, PX_JOIN_CTAS) prefix_join_ker
   const int64_t q = (int64_t)blockIdx.x * (PX_JOIN_THREADS / 32) + (threadIdx.x >> 5);
   if (q >= (int64_t)A.B * A.Hkv * A.R) return;
   const int bh = (int)q / A.R, r = (int)q - bh * A.R, b = bh / A.Hkv, h = bh - b * A.Hkv;
-  // what the plan says (complete before the kernel in front of this one began):
-  // pieces [0, n1) are of the shared range, two per CTA where both tiles worked on
-  // the rows; [n1, np) of the row's own range.  Rows of partials in 32 bits: each
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // what the plan says: pieces [0, n1) are of the shared range, two per CTA where
+  // both tiles worked on the rows; [n1, np) of the row's own range.  Rows of partials in 32 bits: each
   // is 512 bytes of memory.
-  const int g = P.rowgroup[b], pre = A.rowpre[b], tb = A.rowpre[b + 1] - pre;
-  const int RC = P.qc * A.group, oshare = ow_share(P, A.rowpre[A.B] * A.Hkv);
-  const int ou = pre * A.Hkv + h * tb, oc0 = (ou + OW_OVH) / oshare, jc = r / RC;
+  const int status = *A.status;
+  const int4 totals = *P.totals;
+  const int4 j0 = P.rowjoin[2 * b], j1 = P.rowjoin[2 * b + 1];
+  const PxRow row = {j0.x, j0.y, j0.z, j0.w, j1.x, j1.y, j1.z, 0};
+  const int tb = row.tb, RC = P.qc * A.group, oshare = totals.z, gshare = totals.w;
+  const int ou = row.pre * A.Hkv + h * tb, oc0 = (ou + OW_OVH) / oshare, jc = r / RC;
   const int at2 = (jc * P.slots + bh + oc0) * RC + r - jc * RC;
   int n1 = 0, dup = 0, at1 = 0;
-  if (g >= 0) {
-    const int rows = P.g_rows[g] * A.R, gtb = P.g_pages[g] + PX_OVH;
-    const int gshare = px_share(P.g_unit[P.G]);
-    const int f = (b - P.g_row0[g]) * A.R + r, p = f / PX_ROWS;
-    const int it = h * ((rows + PX_ROWS - 1) / PX_ROWS) + p, u = P.g_unit[g] + it * gtb;
+  if (row.rows > 0) {
+    const int rows = row.rows * A.R, gtb = row.pages + PX_OVH;
+    const int f = row.place * A.R + r, p = f / PX_ROWS;
+    const int it = h * ((rows + PX_ROWS - 1) / PX_ROWS) + p, u = row.unit + it * gtb;
     const int c0 = (u + PX_OVH) / gshare;
     dup = rows - p * PX_ROWS <= PX_ROWS / 2;
     n1 = ((u + gtb - 1) / gshare - c0 + 1) << dup;
-    at1 = (P.g_item[g] + it + c0) * PX_ROWS + f % PX_ROWS;
+    at1 = (row.item + it + c0) * PX_ROWS + f % PX_ROWS;
   }
   const int np = n1 + (tb > 0 ? (ou + tb - 1) / oshare - oc0 + 1 : 0);
   auto row_of = [&](int i) {
@@ -1136,8 +1171,6 @@ __global__ void __launch_bounds__(PX_JOIN_THREADS, PX_JOIN_CTAS) prefix_join_ker
   auto ml_of = [&](int i) {
     return __ldcg(reinterpret_cast<const float2*>(i < n1 ? P.pml : A.part_ml) + row_of(i));
   };
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int status = *A.status;
   load(0);                                           // on their way before their weights are known
   float m = -CUDART_INF_F, l = 0.f, m0 = -CUDART_INF_F;        // per lane, then over the warp
   bool nan = false;                                  // a NaN score leaves no maximum, but its sum
@@ -1213,7 +1246,7 @@ static PxLayout px_layout(int B, int G, int Hq, int Hkv, int qlen) {
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   const size_t n1 = (size_t)(L.max_items + PX_CTAS) * PX_ROWS;
   const size_t n2 = (size_t)L.chunks * L.slots * L.qc * group;
-  size_t o = up((5 * (size_t)G + 2 + 4 * (size_t)B + 2) * sizeof(int));
+  size_t o = up((8 * (size_t)B + 4 + 5 * (size_t)G + 2 + 3 * (size_t)B + 2) * sizeof(int));
   L.ints = 0;
   L.qp = o; o = up(o + (size_t)B * Hq * qlen * PX_D * 2);
   L.acc = o; o = up(o + n1 * PX_D * sizeof(float));
@@ -1282,15 +1315,16 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < L.bytes)
     return SD_ENOSPC;
   char* ws = reinterpret_cast<char*>(workspace);
-  P.qc = L.qc; P.nq = L.nq; P.slots = L.slots;
+  P.qc = L.qc; P.nq = L.nq; P.chunks = L.chunks; P.slots = L.slots;
   P.starts = group_starts; P.pages = prefix_pages; P.G = G; P.max_items = L.max_items;
   int* in = reinterpret_cast<int*>(ws + L.ints);
+  P.rowjoin = reinterpret_cast<int4*>(in); in += 8 * (size_t)B;
+  P.totals = reinterpret_cast<int4*>(in); in += 4;
   P.g_unit = in; in += G + 1;
   P.g_item = in; in += G + 1;
   P.g_row0 = in; in += G;
   P.g_rows = in; in += G;
   P.g_pages = in; in += G;
-  P.rowgroup = in; in += B;
   P.rowstart = in; in += B;
   A.rowkmax = in; in += B;
   A.rowpre = in; in += B + 1;
@@ -1305,16 +1339,14 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   if (!cache_map(&mk, kpool, rows) || !cache_map(&mv, vpool, rows) ||
       !cache_map(&mq, P.qp, qrows) || !cache_map(&mq32, P.qp, qrows, 32))
     return SD_ENOTSUP;
-  const int sm = (int)sizeof(PxSmem) + 1024, smo = (int)sizeof(OwSmem) + 1024;   // room to align
+  const int sm = (int)std::max(sizeof(PxSmem), sizeof(OwSmem)) + 1024;           // room to align
   static std::atomic<uint64_t> ready{0};             // devices whose kernels may use that much
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return SD_ELAUNCH;
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (!(ready.load() & bit) || !bit) {
     if (cudaFuncSetAttribute(prefix_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) !=
-            cudaSuccess ||
-        cudaFuncSetAttribute(own_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smo) !=
-            cudaSuccess)
+        cudaSuccess)
       return SD_ELAUNCH;
     ready.fetch_or(bit);
   }
@@ -1329,16 +1361,11 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.stream = st;
-  if (G > 0) {
-    cfg.gridDim = dim3(PX_CTAS);
-    cfg.blockDim = dim3(PX_THREADS);
-    cfg.dynamicSmemBytes = sm;
-    if (cudaLaunchKernelEx(&cfg, prefix_tc_kernel, P, mk, mv, mq) != cudaSuccess) return SD_ELAUNCH;
-  }
-  cfg.gridDim = dim3(PX_CTAS, L.chunks);
-  cfg.blockDim = dim3(OW_THREADS);
-  cfg.dynamicSmemBytes = smo;
-  if (cudaLaunchKernelEx(&cfg, own_tc_kernel, P, mk, mv, mq32) != cudaSuccess) return SD_ELAUNCH;
+  cfg.gridDim = dim3(PX_CTAS * ((unsigned)L.chunks + (G > 0 ? 1 : 0)));
+  cfg.blockDim = dim3(PX_THREADS);
+  cfg.dynamicSmemBytes = sm;
+  if (cudaLaunchKernelEx(&cfg, prefix_tc_kernel, P, mk, mv, mq, mq32) != cudaSuccess)
+    return SD_ELAUNCH;
   const int64_t per = PX_JOIN_THREADS / 32;          // query rows of a CTA
   cfg.gridDim = dim3((unsigned)((R * B * Hkv + per - 1) / per));
   cfg.blockDim = dim3(PX_JOIN_THREADS);
