@@ -43,6 +43,10 @@ constexpr int PX_CTAS = 148;                 // one CTA per SM
 constexpr int PX_OVH = 2;                    // schedule cost of an item beyond its pages, in pages
 constexpr int PX_MIN_SHARE = PX_OVH + 1;     // fewest schedule units per CTA: a one-page item
 constexpr float PX_HEADROOM = 8.f;           // lazy-rescale headroom of the running max (base 2)
+// Largest maximum (base 2) whose scores go through fma(s, sl2, -m).  m is the float
+// next to s sl2 of the largest score: from 2^31 on it may be more than 128 away
+// from it, and 2^(s sl2 - m) leaves the float range; up to 2^20, 1/32.
+constexpr float PX_TAME = 1048576.f;
 constexpr int PX_JOIN_THREADS = 256;
 constexpr int PX_JOIN_CTAS = 4;              // per SM
 constexpr int PX_JOIN_LOADS = 4;             // pieces of a row on their way at once
@@ -315,6 +319,16 @@ __device__ __forceinline__ void px_weights(const uint32_t (&s)[32], uint32_t* p,
   }
 }
 
+// Beyond PX_TAME the scores are scaled first, with a rounding of their own: the
+// largest one's exponent is 0 again.  (Rare; px_weights then gets a factor of 1.)
+__device__ __forceinline__ bool px_wild(float m) {
+  return __any_sync(0xffffffffu, fabsf(m) > PX_TAME && m != -CUDART_INF_F);
+}
+__device__ __forceinline__ void px_scale(uint32_t (&s)[32], float sl2) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__fmul_rn(__uint_as_float(s[e]), sl2));
+}
+
 // A group's first unit, the next one's, rows and pages
 __device__ __forceinline__ int4 px_group(const PrefixParams& P, int g) {
   return make_int4(P.g_unit[g], P.g_unit[g + 1], P.g_rows[g], P.g_pages[g]);
@@ -516,6 +530,7 @@ __device__ __forceinline__ void shared_ranges(const PrefixParams& P, const CUten
       more = px_next(seg, P) && find(seg);
       const int pages = cur.j1 - cur.j0, halves = cur.dup ? 1 : 2;
       float m = -CUDART_INF_F, l = 0.f;
+      bool wild = false;
 #pragma unroll 1
       for (int i = 0; i < pages; ++i) {
         ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[x], n & 1u, &S.abort_));
@@ -549,6 +564,7 @@ __device__ __forceinline__ void shared_ranges(const PrefixParams& P, const CUten
           const float alpha = move ? (m == -CUDART_INF_F ? 0.f : ex2f(m - mn)) : 1.f;
           m = mn;
           l *= alpha;
+          wild = px_wild(m);
           if (i > 0) {
             // O holds this segment's earlier pages: the last P . V into it first
             ok = __all_sync(0xffffffffu, tc_wait(&S.oready[x], (n - 1) & 1u, &S.abort_));
@@ -565,8 +581,8 @@ __device__ __forceinline__ void shared_ranges(const PrefixParams& P, const CUten
             }
           }
         }
-        const float mc = fmaxf(m, -1e30f);           // 2^(-inf - mc) = 0
-        const unsigned long long sl22 = pair2(sl2, sl2), nm2 = pair2(-mc, -mc);
+        const float mc = m == -CUDART_INF_F ? 0.f : m, sf = wild ? 1.f : sl2;
+        const unsigned long long sl22 = pair2(sf, sf), nm2 = pair2(-mc, -mc);
         unsigned long long ls[2] = {0ULL, 0ULL};     // (0.f, 0.f)
         uint32_t pk[32];
 #pragma unroll 1
@@ -574,6 +590,10 @@ __device__ __forceinline__ void shared_ranges(const PrefixParams& P, const CUten
           TC_LD32(sa, scol + 64u * c);
           TC_LD32(sb, scol + 64u * c + 32u);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          if (wild) {
+            px_scale(sa, sl2);
+            px_scale(sb, sl2);
+          }
           px_weights(sa, pk, ls, sl22, nm2);
           px_weights(sb, pk + 16, ls, sl22, nm2);
           TC_ST32(scol + 32u * c, pk);               // over columns that have been read
@@ -939,6 +959,7 @@ __device__ __forceinline__ void own_ranges(const PrefixParams& P, const CUtensor
       int lim = 0x7FFFFFFF;
       if (r < R) lim = row_limit(A, cur.b, j0 + r / A.group);
       float m = -CUDART_INF_F, l = 0.f;
+      bool wild = false;
       for (int i = 0; i < cur.n; ++i, ++n) {
         ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[s][n & 1u], (n >> 1) & 1u, &S.abort_));
         if (!ok) break;
@@ -999,6 +1020,7 @@ __device__ __forceinline__ void own_ranges(const PrefixParams& P, const CUtensor
           const float alpha = move ? (m == -CUDART_INF_F ? 0.f : ex2f(m - mn)) : 1.f;
           m = mn;
           l *= alpha;
+          wild = px_wild(m);
           if (i > 0) {
             // O holds this segment's earlier pages: the last P . V into it first
             ok = __all_sync(0xffffffffu,
@@ -1016,8 +1038,8 @@ __device__ __forceinline__ void own_ranges(const PrefixParams& P, const CUtensor
             }
           }
         }
-        const float mc = fmaxf(m, -1e30f);           // 2^(-inf - mc) = 0
-        const unsigned long long sl22 = pair2(sl2, sl2), nm2 = pair2(-mc, -mc);
+        const float mc = m == -CUDART_INF_F ? 0.f : m, sf = wild ? 1.f : sl2;
+        const unsigned long long sl22 = pair2(sf, sf), nm2 = pair2(-mc, -mc);
         unsigned long long ls[2] = {0ULL, 0ULL};     // (0.f, 0.f)
         uint32_t pk[32];
 #pragma unroll 1
@@ -1025,6 +1047,10 @@ __device__ __forceinline__ void own_ranges(const PrefixParams& P, const CUtensor
           TC_LD32(sa, scol + 64u * c);
           TC_LD32(sb, scol + 64u * c + 32u);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          if (wild) {
+            px_scale(sa, sl2);
+            px_scale(sb, sl2);
+          }
           px_weights(sa, pk, ls, sl22, nm2);
           px_weights(sb, pk + 16, ls, sl22, nm2);
           TC_ST32(scol + 32u * c, pk);               // over columns that have been read

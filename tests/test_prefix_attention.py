@@ -414,3 +414,35 @@ def test_many_rows_and_groups(sizes, pages):
     that look for a CTA's first row or group."""
     n = sum(sizes)
     _check(_case(sizes, pages, [(7 * b) % 130 for b in range(n)], 1, 2, 1, seed=n, stale=0.0))
+
+
+@gpu
+@pytest.mark.parametrize("scale", [1e4, 1e7, 3e8, 1e10, 1e20, 1e30])
+@pytest.mark.parametrize("shift", [0.0, -60.0])
+def test_scores_beyond_what_a_float_resolves(scale, shift):
+    """Scores of 1e5 to 1e31, all of one sign in the second form: the largest takes
+    the whole weight.  A float32 score of 128 products is off by at most 128 *
+    2^-24 of their magnitudes' sum (1.5e-3 of scale here, with |q k| sums of 200): rows
+    whose two largest scores are nearer than 4e-3 may give either and are left out."""
+    c = _case([7, 3], [2, 1], [5, 130, 0, 44, 300, 9, 77, 12, 1, 200], 2, 8, 2, seed=3)
+    c["k"][..., 0] = torch.where(c["k"][..., 0].isnan(), c["k"][..., 0], shift / 8.0)
+    c["q"][..., 0] = 8.0
+    got = _run(c, scale=scale).cpu().double()
+    q, k, v = c["q"].cpu().double(), c["k"].cpu().double(), c["v"].cpu().double()
+    seen = 0
+    for b, n in enumerate(c["lens"].tolist()):
+        for j in range(2):
+            pg = c["bt"][b, :-(-(n + j + 1) // PAGE)].long().cpu()
+            kb = k[pg].permute(1, 0, 2, 3).reshape(2, -1, 128)[:, :n + j + 1]
+            vb = v[pg].permute(1, 0, 2, 3).reshape(2, -1, 128)[:, :n + j + 1]
+            s = torch.einsum("hgd,hsd->hgs", q[b, :, j].view(2, 4, 128), kb)
+            top, at = s.topk(2, -1)
+            for h in range(2):
+                for g in range(4):
+                    if float(top[h, g, 0] - top[h, g, 1]) < 4e-3 + 20.0 / scale:
+                        continue
+                    want = vb[h, at[h, g, 0]]
+                    tol = (2.0 ** -7 + 2.0 ** -10) * want.abs()
+                    assert bool(((got[b, j, 4 * h + g] - want).abs() <= tol).all()), (b, j, h, g)
+                    seen += 1
+    assert seen > 120
