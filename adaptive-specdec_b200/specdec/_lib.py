@@ -67,6 +67,20 @@ _SIGNATURES = {
     "sd_prefix_attn": ([_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32,
                         _i32, _i32, _i32, _i32, _i32, _f32, _vp, _i64, _i64, _i64, _i32, _vp, _sz,
                         _vp], _i32),
+    "sd_tree_masks": ([_vp, _i64, _i32, _i32, _vp, _vp, _vp], _i32),
+    "sd_tree_accept": ([_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp],
+                       _i32),
+    "sd_kv_commit_tree": ([_vp, _i32, _vp, _i32, _i32, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _i32,
+                           _i32, _i32, _i32, _vp, _vp], _i32),
+    "sd_tree_attn_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32], _sz),
+    "sd_tree_attn": ([_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _i64, _i32, _i32,
+                      _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _i64, _i64, _i64, _i32, _vp,
+                      _sz, _vp], _i32),
+    "sd_process_logits": ([_vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _i32,
+                           _i32, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i64,
+                           _vp, _i64, _i64, _vp], _i32),
+    "sd_history_add": ([_vp, _i64, _i32, _vp, _i64, _i32, _vp, _i64, _vp, _i32, _i32, _i32, _vp],
+                       _i32),
     "sd_shard_workspace_bytes": ([_i32, _i32, _i32], _sz),
     "sd_shard_send_bytes": ([_i32, _i32, _i32, _i32, _i32], _sz),
     "sd_shard_phase": ([_vp, _i32, _vp, _vp, _vp], _i32),

@@ -6,7 +6,8 @@ s < valid[b] in a right-padded prefill).  It replaces the reference's HF SDPA
 over ``_RaggedLayer.update``'s max-width view plus the additive mask
 (specdec/kvcache.py:61-74 and :138-162, called at specdec/engine.py:274): each
 row reads only its own live keys.  ``prefix_attention`` is the same over a paged
-cache whose rows share their first pages (sd_prefix_attn).
+cache whose rows share their first pages (sd_prefix_attn), ``tree_attention`` that
+of a drafted tree's nodes (sd_tree_attn).
 
 ``register()`` installs it as the transformers attention implementation
 "specdec_b200" (with a mask function that builds no mask); a model loaded with
@@ -16,6 +17,7 @@ cache whose rows share their first pages (sd_prefix_attn).
 import torch
 
 from specdec import _lib as L
+from specdec.tree import check_masks
 
 IMPL = "specdec_b200"
 PREFILL_SDPA_MIN = 64          # prefills longer than this (fresh cache) use torch SDPA
@@ -191,6 +193,91 @@ def prefix_attention(q, k_pool, v_pool, lengths, block_table, group_starts, pref
     return out
 
 
+def tree_attention(q, k_cache, v_cache, lengths, masks, first=0, scale=None, out=None,
+                   block_table=None):
+    """Attention of the nodes of a drafted tree over the cache (``specdec.tree``).
+
+    q [B, Hq, qlen, D], caches [B, Hkv, C, D] (or, with ``block_table`` [B, W]
+    int32, page pools [n_pages, Hkv, PAGE, D]) -> out [B, qlen, Hq, D].  Query j is
+    node ``first`` + j of the row's tree; ``lengths`` [B] are the lengths before this
+    forward's advance (so with ``first`` = 0 the row's tokens, and ``first`` more when
+    the tree is fed level by level).  It reads the slots s < lengths[b] - first and
+    those of its ancestors and itself, lengths[b] - first + a for every bit a of
+    ``masks`` [N, W] or [B, N, W] (``tree_masks``).  A node without a bit gives 0.
+    Slots that no node sees may hold anything; V has to be finite in the slots that
+    some of the row's nodes see and others do not.  bf16 and fp32.
+    """
+    dev, dt = q.device, q.dtype
+    if not q.is_cuda:
+        L.require_cuda(q)
+    if k_cache.device != dev or v_cache.device != dev or lengths.device != dev \
+            or masks.device != dev or (block_table is not None and block_table.device != dev) \
+            or (out is not None and out.device != dev):
+        raise L.SpecdecError("tree_attention needs every tensor on one CUDA device")
+    if torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return tree_attention(q, k_cache, v_cache, lengths, masks, first, scale, out,
+                                  block_table)
+    if q.dim() != 4 or k_cache.dim() != 4:
+        raise L.SpecdecError("tree_attention needs q [B, Hq, qlen, D] and caches [B, Hkv, C, D] "
+                             "or pools [n_pages, Hkv, PAGE, D]")
+    if dt not in _ATTN_DTYPES or k_cache.dtype != dt or v_cache.dtype != dt:
+        raise L.SpecdecError(f"tree_attention supports bf16 / fp32, got {dt}")
+    B, Hq, qlen, D = q.shape
+    n0, Hkv, C, Dk = k_cache.shape
+    if Dk != D or v_cache.shape != k_cache.shape or not (k_cache.is_contiguous()
+                                                         and v_cache.is_contiguous()):
+        raise L.SpecdecError("K and V caches must be contiguous, of one shape, with q's head size")
+    W = npages = 0
+    if block_table is not None:
+        if C != SD_PAGE:
+            raise L.SpecdecError("paged caches must be [n_pages, Hkv, PAGE, D] pools")
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
+                block_table.shape[0] != B or not block_table.is_contiguous():
+            raise L.SpecdecError("block_table must be a contiguous [B, W] int32 tensor")
+        W, npages = block_table.shape[1], n0
+        C = W * SD_PAGE
+    elif n0 != B:
+        raise L.SpecdecError(f"a cache of {n0} rows for {B} rows of queries")
+    mask_bs, N = check_masks(masks, B, "tree_attention")
+    first = int(first)
+    if not 0 <= first <= N - qlen:
+        raise L.SpecdecError(f"nodes {first} to {first + qlen - 1} of a tree of {N}")
+    if lengths.numel() != B:
+        raise L.SpecdecError(f"lengths needs one entry per row ({B})")
+    sc = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < sc < 3e38:
+        raise L.SpecdecError(f"scale must be positive and finite, got {scale}")
+    qb, qh, ql, qd = q.stride()
+    if qd != 1 or (dt == torch.bfloat16 and D == 128 and (
+            q.data_ptr() % 16 or qb % 8 or qh % 8 or ql % 8)):
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+        qb, qh, ql, qd = q.stride()
+    if lengths.dtype != torch.long or not lengths.is_contiguous():
+        lengths = lengths.long().contiguous()
+    if out is None:
+        out = q.new_empty(B, qlen, Hq, D)
+        ob, ol, oh = qlen * Hq * D, Hq * D, D
+    else:
+        if out.shape != (B, qlen, Hq, D) or out.dtype != dt or (D > 1 and out.stride(3) != 1):
+            raise L.SpecdecError(f"out must be {(B, qlen, Hq, D)} of {dt}, contiguous along D")
+        ob, ol, oh, _ = out.stride()
+    if B == 0 or qlen == 0:
+        return out
+    code = _ATTN_DTYPES[dt]
+    # a fresh buffer per call: calls on several streams and calls captured into
+    # different graphs never share one
+    nws = L.workspace_bytes("sd_tree_attn_workspace_bytes", B, Hq, Hkv, D, C, qlen, code)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    L.check(L.lib().sd_tree_attn(
+        q.data_ptr(), qb, qh, ql, k_cache.data_ptr(), v_cache.data_ptr(), L.address(block_table),
+        W, npages, lengths.data_ptr(), masks.data_ptr(), mask_bs, N, first, B, Hq, Hkv, D, C, qlen,
+        sc, out.data_ptr(), ob, ol, oh, code, L.address(ws), nws, L.stream_of(dev)), "tree_attn")
+    return out
+
+
 def gather_pages(pool, block_table, n):
     """The first n slots of every row of a page pool as [B, Hkv, n, D]."""
     from specdec.kvcache import PAGE
@@ -221,6 +308,10 @@ def hf_attention(module, query, key, value, attention_mask, dropout=0.0, scaling
                 query, ks, vs, is_causal=True, scale=scaling, enable_gqa=True)
             return out.transpose(1, 2), None
         bt, prefix = getattr(cache, "block_table", None), getattr(cache, "prefix", None)
+        if cache.tree is not None:                  # a drafted tree: nodes see their ancestors
+            masks, _, first = cache.tree
+            return tree_attention(query, key, value, cache.lengths, masks, first, scaling,
+                                  block_table=bt), None
         if prefix is not None:                      # a forked cache: rows share their prompt's pages
             return prefix_attention(query, key, value, cache.lengths, bt, *prefix,
                                     valid=cache.valid, scale=scaling), None

@@ -33,15 +33,83 @@ kvcache.py:98-116).  Its page bookkeeping runs on the host (``PageTable``) or, w
 device lengths without a host copy of them, and ``fork`` makes several rows of
 one prompt that share its pages.
 """
+import ctypes
+
 import numpy as np
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
 from specdec import _lib as L
+from specdec.tree import TREE_MAX
 
-__all__ = ["RaggedCache", "PagedRaggedCache", "DevicePageTable", "PAGE"]
+__all__ = ["RaggedCache", "PagedRaggedCache", "DevicePageTable", "commit_tree", "PAGE"]
+
+_BAD_PATH = "RaggedCache: a committed path was not a rising list of the tree's nodes"
 
 PAGE = 128            # tokens per page (SD_KV_PAGE): one K/V tile of the verify attention
+
+
+def commit_tree(keys, values, lengths, path, n_acc, nodes, block_table=None, err=None):
+    """Commit a tree round in every layer: the accepted path's K and V move to the
+    slots behind the row's tokens, ``lengths`` follow.
+
+    keys / values: the layers' caches, lists of [B, Hkv, C, D] or, with
+    ``block_table`` [B, W] int32, of pools [n_pages, Hkv, PAGE, D]; 2- or 4-byte
+    types.  ``lengths`` [B] int64 are those after the forward over ``nodes`` tree
+    nodes (base + nodes) and become base + 1 + n_acc; ``path`` [B, P] int32 and
+    ``n_acc`` [B] are ``specdec.tree.tree_accept``'s.  A row whose slots would leave
+    the cache, or whose path is not strictly rising below ``nodes``, stays as it
+    was and sets bit 0 or 5 of ``err`` ([1] int32); a slot without a page is not
+    moved (bit 1).  No host synchronisation.
+    """
+    keys, values = list(keys), list(values)
+    dev = lengths.device
+    if not lengths.is_cuda:
+        L.require_cuda(lengths)
+    B = lengths.numel()
+    if lengths.dtype != torch.long or not lengths.is_contiguous():
+        raise L.SpecdecError("lengths must be contiguous int64 (they are updated in place)")
+    if path.device != dev or path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != B \
+            or path.shape[1] < 1 or (path.shape[1] > 1 and path.stride(1) != 1):
+        raise L.SpecdecError(f"path must be int32 [{B}, P] on {dev}")
+    if n_acc.device != dev or n_acc.numel() != B or n_acc.is_floating_point():
+        raise L.SpecdecError(f"n_acc must be integers [{B}] on {dev}")
+    if n_acc.dtype != torch.long or not n_acc.is_contiguous():
+        n_acc = n_acc.long().contiguous()
+    N = int(nodes)
+    if not 1 <= N <= TREE_MAX:
+        raise L.SpecdecError(f"a tree has 1 to {TREE_MAX} nodes, got {nodes}")
+    if err is not None and (err.device != dev or err.dtype != torch.int32 or err.numel() != 1):
+        raise L.SpecdecError(f"err must be int32 [1] on {dev}")
+    bufs = keys + values
+    if not bufs or len(keys) != len(values):
+        raise L.SpecdecError(f"commit_tree needs K and V of every layer, got {len(keys)} and "
+                             f"{len(values)}")
+    shape, dt, e = bufs[0].shape, bufs[0].dtype, bufs[0].element_size()
+    if len(shape) != 4 or e not in (2, 4):
+        raise L.SpecdecError("caches must be [B, Hkv, C, D] or [n_pages, Hkv, PAGE, D] of a 2- or "
+                             "4-byte type")
+    for t in bufs:
+        if t.dtype != dt or t.shape != shape or t.device != dev or not t.is_contiguous():
+            raise L.SpecdecError("every layer's K and V must be contiguous, of one shape, type and "
+                                 f"device ({dev})")
+    n0, H, C, D = shape
+    W = npages = 0
+    if block_table is not None:
+        if block_table.device != dev or block_table.dtype != torch.int32 or block_table.dim() != 2 \
+                or block_table.shape[0] != B or not block_table.is_contiguous():
+            raise L.SpecdecError(f"block_table must be contiguous int32 [{B}, W] on {dev}")
+        W, npages = block_table.shape[1], n0
+        if C != PAGE:
+            raise L.SpecdecError("paged caches must be [n_pages, Hkv, PAGE, D] pools")
+    elif n0 != B:
+        raise L.SpecdecError(f"caches of {n0} rows for {B} lengths")
+    ptrs = (ctypes.c_void_p * len(bufs))(*[t.data_ptr() for t in bufs])
+    with L.on_device(dev):
+        L.check(L.lib().sd_kv_commit_tree(
+            ptrs, len(bufs), L.address(block_table), W, npages, lengths.data_ptr(),
+            path.data_ptr(), path.stride(0), path.shape[1], n_acc.data_ptr(), N, B, H, C, D, e,
+            L.address(err), L.stream_of(dev)), "kv_commit_tree")
 
 
 class _RaggedLayer(CacheLayerMixin):
@@ -128,6 +196,7 @@ class RaggedCache(Cache):
         self._host = torch.zeros(self.batch_size, dtype=torch.long)
         self._host_valid = True
         self.valid = None           # optional [B] cap for right-padded prefill
+        self.tree = None            # (masks, depths, first node) of a drafted tree's forward
         self._last_q = 0
         super().__init__(layers=[self._layer_cls(self) for _ in range(n_layers)])
 
@@ -162,7 +231,11 @@ class RaggedCache(Cache):
         return self.max_len + q
 
     def positions(self, q):
-        """RoPE positions [B, q]: each row continues from its own length."""
+        """RoPE positions [B, q]: each row continues from its own length (a tree's
+        nodes by their depth)."""
+        if self.tree is not None:
+            _, depths, first = self.tree
+            return (self.lengths.view(-1, 1) - first) + depths[..., first:first + q]
         ar = torch.arange(q, device=self.device).view(1, q)
         return self.lengths.view(-1, 1) + ar
 
@@ -266,10 +339,36 @@ class RaggedCache(Cache):
                                          L.stream_ptr(self.device)), "kv commit")
         self._host_valid = False
 
+    # ---- trees of drafted tokens ---------------------------------------------
+    def set_tree(self, masks=None, depths=None, first=0):
+        """The next forwards are over nodes first, first + 1, ... of a drafted tree
+        (``specdec.tree.tree_masks``) whose earlier nodes the cache already holds;
+        without arguments they are over chains again.  Only the kernel attention
+        path (attn_impl "specdec_b200") knows trees."""
+        if masks is None:
+            self.tree = None
+            return
+        if self.attn_impl != "specdec_b200":
+            raise L.SpecdecError("trees of drafted tokens need the specdec_b200 attention")
+        self.tree = (masks, depths, int(first))
+
+    def commit_tree(self, path, n_acc, nodes):
+        """Tree-round commit, after a forward over ``nodes`` tree nodes and its
+        advance: every layer keeps the accepted path behind the row's tokens,
+        lengths go from base + nodes to base + 1 + n_acc (``commit_tree``)."""
+        live = [layer for layer in self.layers if layer.is_initialized]
+        commit_tree([x.keys for x in live], [x.values for x in live], self.lengths, path, n_acc,
+                    nodes, block_table=getattr(self, "block_table", None), err=self._err)
+        self._host_valid = False
+        self.tree = None
+
     def check_errors(self):
         """Raise if any device-side update was refused (syncs once)."""
-        if int(self._err.item()):
+        e = int(self._err.item())
+        if e:
             self._err.zero_()
+            if e & 32:
+                raise RuntimeError(_BAD_PATH)
             raise RuntimeError("RaggedCache: a length update left [0, capacity]")
 
     # ---- Cache interface ---------------------------------------------------
@@ -442,7 +541,8 @@ class DevicePageTable:
 
     ERRORS = {1: "a row's length left [0, capacity]", 2: "a slot was written without a page",
               4: "page pool exhausted", 8: "more new tokens than max_tokens",
-              16: "a new token below a row's floor of shared pages"}
+              16: "a new token below a row's floor of shared pages",
+              32: "a committed path was not a rising list of the tree's nodes"}
 
     def __init__(self, batch_size, pages_per_row, n_pages, device, err=None, stack=None):
         B, W, n = int(batch_size), int(pages_per_row), int(n_pages)
@@ -839,6 +939,8 @@ class PagedRaggedCache(RaggedCache):
             self._err.zero_()
             if e & 4:
                 raise L.SpecdecError("KV page pool exhausted")
+            if e & 32:
+                raise RuntimeError(_BAD_PATH)
             if e & 16:
                 raise RuntimeError("PagedRaggedCache: a forked row was rolled back into the pages "
                                    "it shares and would write them")

@@ -11,7 +11,9 @@ meaning and output dtypes, plus the two fused entry points the engine uses:
 
 and ``token_logprobs`` (no counterpart in the reference): log-probability, rank
 and entropy for given tokens, with the largest alternatives, for callers that
-rank several samples of one prompt.
+rank several samples of one prompt; and ``process_logits`` with ``TokenHistory``:
+penalties for repeated tokens, biases and grammar masks on the logits of a draft or
+verify forward, the drafted tokens before each position counted in.
 
 Draws are inverse-CDF with uniforms: either passed in (``u=...``) or drawn
 from ``generator`` on the device.  Given the same uniforms, results match the
@@ -26,13 +28,15 @@ from typing import NamedTuple, Optional
 import torch
 
 from specdec import _lib as L
+from specdec.tree import TREE_MAX, check_masks
 
 __all__ = ["to_probs", "sample_from_probs", "residual_probs", "gather_prob",
            "verify_sample", "verify_sample_probs", "draft_sample", "TokenLogprobs",
-           "token_logprobs"]
+           "token_logprobs", "TokenHistory", "process_logits"]
 
 TOP_N_MAX = 32             # SD_TOPN_MAX
 LOGPROBS_MAX_V = 1 << 20   # SD_LOGPROBS_MAX_V
+BIAS_MAX = 1024            # SD_BIAS_MAX
 
 
 def _knobs(temperature, top_p, top_k):
@@ -327,3 +331,206 @@ def token_logprobs(logits, ids, temperature=1.0, top_n=0):
         rank.data_ptr(), entropy.data_ptr(), L.address(top_ids), L.address(top_lp),
         L.stream_of(dev)), "token_logprobs")
     return TokenLogprobs(logprob, rank, entropy, top_ids, top_lp)
+
+
+class TokenHistory:
+    """Which tokens each row's prompt holds and how often it has written each.
+
+    ``counts`` [B, V] int16 on the device: the low 15 bits count the written
+    tokens (up to 32767), the sign bit marks the prompt's.  ``process_logits`` reads
+    it; ``add_prompt`` and ``append`` add to it.  Both are stream ordered, never
+    synchronise and can be captured into CUDA graphs.
+    """
+
+    def __init__(self, batch_size, vocab_size, device):
+        B, V = int(batch_size), int(vocab_size)
+        dev = torch.device(device)
+        if B < 0 or V < 1:
+            raise L.SpecdecError(f"a history needs rows and a vocabulary, got {B} x {V}")
+        if dev.type != "cuda":
+            raise L.SpecdecError("TokenHistory keeps its counts on the GPU (no CPU fallback)")
+        # (rows of whole 16-byte units)
+        self._bind(torch.zeros(B, -(-V // 8) * 8, dtype=torch.int16, device=dev)[:, :V])
+
+    def _bind(self, counts):
+        self.counts, self.device = counts, counts.device
+        self.B, self.V = counts.shape
+
+    @classmethod
+    def over(cls, counts):
+        """A history over counts [B, V] int16 that the caller holds (no copy)."""
+        if not counts.is_cuda:
+            raise L.SpecdecError("TokenHistory keeps its counts on the GPU (no CPU fallback)")
+        if counts.dtype != torch.int16 or counts.dim() != 2 or counts.shape[1] < 1 \
+                or (counts.stride(1) != 1 and counts.shape[1] > 1) \
+                or (counts.shape[0] > 1 and counts.stride(0) < counts.shape[1]):
+            raise L.SpecdecError("counts must be int16 [B, V] with contiguous rows")
+        self = cls.__new__(cls)
+        self._bind(counts)
+        return self
+
+    def _add(self, ids, counts, path, prompt):
+        dev = self.device
+        if ids.device != dev or ids.dim() != 2 or ids.shape[0] != self.B:
+            raise L.SpecdecError(f"ids must be [{self.B}, n] on {dev}")
+        if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+            raise L.SpecdecError(f"ids must be integers, got {ids.dtype}")
+        n = ids.shape[1]
+        ids = ids.long() if ids.dtype != torch.long else ids
+        if ids.stride(1) != 1 and n > 1:
+            ids = ids.contiguous()
+        if counts is not None:
+            if counts.device != dev or counts.numel() != self.B or counts.is_floating_point():
+                raise L.SpecdecError(f"counts must be integers [{self.B}] on {dev}")
+            counts = counts.reshape(-1).long().contiguous()
+        path_bs = 0
+        if path is not None:
+            if path.device != dev or path.dtype != torch.int32 or path.dim() != 2 \
+                    or path.shape[0] != self.B or (path.stride(1) != 1 and path.shape[1] > 1):
+                raise L.SpecdecError(f"path must be int32 [{self.B}, P] on {dev}")
+            path_bs = path.stride(0)
+        with L.on_device(dev):
+            L.check(L.lib().sd_history_add(
+                self.counts.data_ptr(), self.counts.stride(0), self.V, ids.data_ptr(),
+                ids.stride(0), n, L.address(path), path_bs, L.address(counts),
+                n if path is None else path.shape[1], self.B, int(prompt), L.stream_of(dev)),
+                "history_add")
+
+    def add_prompt(self, ids, lengths=None):
+        """Marks the first lengths[b] (default: all) of ids [B, n] as prompt tokens."""
+        self._add(ids, lengths, None, True)
+
+    def append(self, ids, counts=None, path=None):
+        """Counts the first counts[b] (default: all) of ids [B, n] as written; with
+        ``path`` [B, P] int32 (``tree_accept``'s) the tokens ids[b, path[b, i]], i <
+        counts[b], instead.  Ids outside [0, V) are padding."""
+        self._add(ids, counts, path, False)
+
+    def repeat_interleave(self, n):
+        """A history with n copies of every row, side by side."""
+        return TokenHistory.over(self.counts.repeat_interleave(int(n), 0))
+
+    def reset(self, rows=None):
+        """Forgets every row, or the given ones."""
+        if rows is None:
+            self.counts.zero_()
+        else:
+            self.counts[rows] = 0
+
+
+def _per_row(x, B, dev, name):
+    """A float32 [B] tensor of a number or a tensor; None stays None."""
+    if x is None:
+        return None
+    if not torch.is_tensor(x):
+        return torch.full((B,), float(x), dtype=torch.float32, device=dev)
+    if x.device != dev or x.numel() != B:
+        raise L.SpecdecError(f"{name} must be a number or [{B}] on {dev}")
+    return x if x.dtype == torch.float32 and x.is_contiguous() else x.reshape(-1).float().contiguous()
+
+
+def process_logits(logits, tokens=None, masks=None, history=None, repetition=None, presence=None,
+                   frequency=None, bias=None, allowed=None, out=None):
+    """Penalties, biases and a grammar mask on the logits of a draft or verify forward.
+
+    logits [B, L, V] (bf16 / fp16 / fp32, vocabulary contiguous) are those of the
+    last L of N drafted tokens ``tokens`` [B, N] (N >= L): a chain, or with ``masks``
+    (``tree_masks``) a tree.  Position l is node N - L + l; what stands before it is
+    the row's ``history`` (a TokenHistory or its counts; without this forward's
+    tokens) and the tokens of its path, itself included.  Per entry, in float32 and
+    rounded once:
+
+      c = times written + times on the path;  s = c > 0 or in the prompt
+      s:      x = x / repetition if x > 0 else x * repetition
+              x = x - frequency * c
+      c > 0:  x = x - presence
+              x = x + bias            bias = (ids [B or 1, M], values [B or 1, M])
+      bit t % 32 of allowed[b, l, t // 32] is 0:  x = -inf
+
+    ``repetition``, ``presence`` and ``frequency`` are numbers or float [B] tensors and
+    need ``history``; ``allowed`` int32 [B or 1, L or 1, ceil(V / 32)].  Ids outside
+    [0, V) are padding, biases of one id add up; at most BIAS_MAX per row and
+    TREE_MAX tokens.  repetition > 0.  Returns a new tensor, or ``out`` ([B, L, V], which may be
+    ``logits`` itself).  One launch, no synchronisation.
+    """
+    dev = logits.device
+    if not logits.is_cuda:
+        L.require_cuda(logits)
+    if torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return process_logits(logits, tokens, masks, history, repetition, presence, frequency,
+                                  bias, allowed, out)
+    if logits.dim() != 3:
+        raise L.SpecdecError(f"process_logits expects [B, L, V] logits, got {tuple(logits.shape)}")
+    code = L.dtype_code(logits.dtype)
+    B, Lq, V = logits.shape
+    if V < 1:
+        raise L.SpecdecError("the vocabulary must have at least one entry")
+    if V > 1:
+        _vocab_rows(logits, "logits")
+    N = first = tokens_bs = mask_bs = 0
+    hist = None
+    if history is not None:
+        hist = history.counts if isinstance(history, TokenHistory) else \
+            TokenHistory.over(history).counts
+        if hist.shape != (B, V) or hist.device != dev:
+            raise L.SpecdecError(f"history is {tuple(hist.shape)} on {hist.device}, the logits "
+                                 f"{tuple(logits.shape)} on {dev}")
+        repetition = _per_row(repetition, B, dev, "repetition")
+        presence = _per_row(presence, B, dev, "presence")
+        frequency = _per_row(frequency, B, dev, "frequency")
+    elif repetition is not None or presence is not None or frequency is not None:
+        raise L.SpecdecError("repetition, presence and frequency need a history")
+    if tokens is not None:
+        if tokens.device != dev or tokens.dim() != 2 or tokens.shape[0] != B or \
+                tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:
+            raise L.SpecdecError(f"tokens must be integers [{B}, N] on {dev}")
+        N = tokens.shape[1]
+        if not Lq <= N <= TREE_MAX:
+            raise L.SpecdecError(f"{Lq} positions of {N} drafted tokens (at most {TREE_MAX})")
+        if tokens.dtype != torch.long:
+            tokens = tokens.long()
+        if N > 1 and tokens.stride(1) != 1:
+            tokens = tokens.contiguous()
+        tokens_bs, first = tokens.stride(0), N - Lq
+    if masks is not None:
+        if tokens is None or masks.device != dev:
+            raise L.SpecdecError(f"masks need tokens, and to be on {dev}")
+        mask_bs, n = check_masks(masks, B, "process_logits")
+        if n != N:
+            raise L.SpecdecError(f"process_logits: {N} tokens per row, but masks of {n} nodes")
+    ids = values = None
+    M = bias_bs = 0
+    if bias is not None:
+        ids, values = bias
+        if ids.device != dev or values.device != dev or ids.dim() != 2 or ids.shape != values.shape \
+                or ids.shape[0] not in (1, B) or ids.is_floating_point():
+            raise L.SpecdecError(f"bias must be (integer ids, values), both [{B} or 1, M] on {dev}")
+        M = ids.shape[1]
+        if M > BIAS_MAX:
+            raise L.SpecdecError(f"at most {BIAS_MAX} biases per row, got {M}")
+        ids, values = ids.long().contiguous(), values.float().contiguous()
+        bias_bs = M if ids.shape[0] == B else 0
+    allowed_bs = allowed_ps = 0
+    if allowed is not None:
+        words = -(-V // 32)
+        if allowed.device != dev or allowed.dtype != torch.int32 or allowed.dim() != 3 \
+                or allowed.shape[0] not in (1, B) or allowed.shape[1] not in (1, Lq) \
+                or allowed.shape[2] != words or (words > 1 and allowed.stride(2) != 1):
+            raise L.SpecdecError(f"allowed must be int32 [{B} or 1, {Lq} or 1, {words}] on {dev}")
+        allowed_bs = allowed.stride(0) if allowed.shape[0] == B else 0
+        allowed_ps = allowed.stride(1) if allowed.shape[1] == Lq else 0
+    if out is None:
+        out = torch.empty(B, Lq, V, dtype=logits.dtype, device=dev)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev \
+            or (V > 1 and out.stride(2) != 1):
+        raise L.SpecdecError(f"out must be {tuple(logits.shape)} of {logits.dtype} on {dev}, "
+                             "contiguous along the vocabulary")
+    L.check(L.lib().sd_process_logits(
+        logits.data_ptr(), logits.stride(0), logits.stride(1), code, B, Lq, V, L.address(tokens),
+        tokens_bs, L.address(masks), mask_bs, N, first, L.address(hist),
+        0 if hist is None else hist.stride(0), L.address(repetition), L.address(presence),
+        L.address(frequency), L.address(ids), L.address(values), bias_bs, M, L.address(allowed),
+        allowed_bs, allowed_ps, out.data_ptr(), out.stride(0), out.stride(1), L.stream_of(dev)),
+        "process_logits")
+    return out

@@ -201,6 +201,48 @@ int sd_token_logprobs(const void* logits, int64_t bs, int64_t ps, int dtype, con
                       float* logprob, int64_t* rank, float* entropy, int64_t* top_ids,
                       float* top_logprobs, void* stream);
 
+/*
+ * Constraints on logits (no counterpart in the reference): penalties for
+ * repeated tokens, biases and grammar masks, at every position of a verify or
+ * draft forward.  Position l of row b is node first + l of a tree of N drafted
+ * tokens (masks as in sd_tree_masks; masks NULL: a chain, node i behind the nodes
+ * before it); its path is the node itself and its ancestors.
+ *   h = history[b, t]: the low 15 bits count how often token t was written, the
+ *       sign bit is set when t stands in the prompt (both without this
+ *       forward's tokens);  c = (h & 0x7FFF) + times t stands on the path
+ *   x = logits[b, l, t]
+ *   if c > 0 or the sign bit:  x = x > 0 ? x / repetition[b] : x * repetition[b]
+ *   x = x - frequency[b] * c;  if c > 0: x = x - presence[b]
+ *   x = x + sum of bias_values[b, m] over bias_ids[b, m] == t
+ *   if bit t % 32 of allowed[b, l, t / 32] is 0: x = -inf
+ * in float32, rounded once to out[b, l, t] (which may be the same memory as
+ * logits).  history NULL: no penalties (the three [B] arrays are then unused; each
+ * may be NULL by itself: neutral); bias_ids NULL: no bias (an id outside [0, V) is
+ * padding); allowed NULL: no mask.  bias_bs / allowed_bs / allowed_ps may be 0
+ * (one list / mask for all rows / positions).  A drafted token outside [0, V) is
+ * padding.  M <= SD_BIAS_MAX.
+ */
+#define SD_BIAS_MAX 1024
+int sd_process_logits(const void* logits, int64_t bs, int64_t ps, int dtype, int B, int L, int V,
+                      const int64_t* tokens, int64_t tokens_bs, const int32_t* masks,
+                      int64_t mask_bs, int N, int first, const int16_t* history,
+                      int64_t history_bs, const float* repetition, const float* presence,
+                      const float* frequency, const int64_t* bias_ids, const float* bias_values,
+                      int64_t bias_bs, int M, const int32_t* allowed, int64_t allowed_bs,
+                      int64_t allowed_ps, void* out, int64_t out_bs, int64_t out_ps, void* stream);
+
+/*
+ * Tokens into a history [B, V] (rows history_bs apart): the first counts[b]
+ * (NULL: all n) of ids[b, 0..n) (int64, rows ids_bs apart).  With path non-NULL
+ * token i is ids[b, path[b, i]] for i < counts[b] (an accepted path of a tree;
+ * path rows path_bs apart, n entries, an entry outside [0, n_ids) adds nothing).
+ * prompt != 0 marks them as prompt tokens, else they are counted (up to 32767).
+ * Ids outside [0, V) are padding.
+ */
+int sd_history_add(int16_t* history, int64_t history_bs, int V, const int64_t* ids,
+                   int64_t ids_bs, int n_ids, const int32_t* path, int64_t path_bs,
+                   const int64_t* counts, int n, int B, int prompt, void* stream);
+
 /* ---- ragged KV cache (reference specdec/kvcache.py) --------------------- */
 
 /*
@@ -409,6 +451,82 @@ int sd_prefix_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const v
                    const int32_t* prefix_pages, int G, int B, int Hq, int Hkv, int D, int qlen,
                    float scale, void* out, int64_t obs, int64_t oqs, int64_t ohs, int dtype,
                    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Trees of drafted tokens (no counterpart in the reference, whose drafts are
+ * chains).  A forward over a tree of N nodes writes node i's key and value to
+ * cache slot base[b] + i, base[b] being the row's tokens before it.  Trees are
+ * given as ancestor bits: masks [T, N, W] int32 words, W = ceil(N / 32), T = 1
+ * (one tree for every row) or B (mask_bs = 0 or the words between rows' trees):
+ * bit a of node i's words is set when a is i itself or one of its ancestors.  A
+ * node without any bit is absent.  Bits from N on are ignored.  N <= SD_TREE_MAX.
+ *
+ * sd_tree_masks: parents [T, N] int32 (rows parents_bs apart) -> masks
+ * (contiguous) and depths [T, N] (may be NULL).  A parent comes before its
+ * child; -1 is a root (depth 0); any other value that is not an earlier node
+ * makes the node absent, and so does an absent parent (no bits, depth 0).
+ */
+#define SD_TREE_MAX 256
+int sd_tree_masks(const int32_t* parents, int64_t parents_bs, int T, int N, int32_t* masks,
+                  int32_t* depths, void* stream);
+
+/*
+ * The accepted path of each row: from node 0, the first child (lowest index;
+ * a node's parent is the highest other bit of its mask) whose token is the
+ * choice of the node it hangs on, until none is, or max_path nodes are reached.
+ *   tokens, choices [B, N] int64 (rows tokens_bs / choices_bs apart): the token
+ *          of each node, and what the target model draws behind it
+ *   alive  [B] uint8 or NULL: a row that is 0 stays at node 0
+ *   path   [B, max_path] int32 out: path[b, 0] = 0, then the nodes, -1 behind
+ *   n_acc  [B] int64 out: accepted drafts (nodes of the path without node 0)
+ *   y      [B] int64 out: the choice of the path's last node
+ * With choices drawn from the target's own distribution at each node, the
+ * emitted tokens (the path's, then y) follow the target's distribution.
+ */
+int sd_tree_accept(const int64_t* tokens, int64_t tokens_bs, const int64_t* choices,
+                   int64_t choices_bs, const int32_t* masks, int64_t mask_bs,
+                   const uint8_t* alive, int B, int N, int max_path, int32_t* path,
+                   int64_t* n_acc, int64_t* y, void* stream);
+
+/*
+ * Commit a tree round: lengths[b] (base + N after the forward's advance)
+ * becomes base + 1 + n_acc[b], and in each of n_bufs cache buffers (the layers'
+ * K and V; `bufs` is a host array of device pointers) the slots base + path[b, j],
+ * 0 <= j <= n_acc[b], move to base + j.  Buffers are [B, H, C, D] or, with a
+ * block table, pools [npages, H, SD_KV_PAGE, D] (C is then bt_stride *
+ * SD_KV_PAGE); elem_bytes is 2 or 4.  path rows are path_bs apart, strictly
+ * rising, and hold n_acc[b] + 1 <= path_len nodes; n_acc[b] < N.  A row whose
+ * slots leave [0, C] (bit 0 of *err) or whose path breaks these rules (bit 5)
+ * is left as it was, length included; a slot without a page is not moved (bit 1).
+ */
+int sd_kv_commit_tree(void* const* bufs, int n_bufs, const int32_t* block_table, int bt_stride,
+                      int npages, int64_t* lengths, const int32_t* path, int64_t path_bs,
+                      int path_len, const int64_t* n_acc, int N, int B, int H, int C, int D,
+                      int elem_bytes, int* err, void* stream);
+
+/*
+ * Attention of a tree's nodes over the cache (after the append of this
+ * forward): query j is node first + j, base[b] = lengths[b] - first, and it
+ * attends to the slots s < base[b] and to base[b] + a for every bit a of its
+ * mask; an absent node gives 0.  `lengths` are the lengths BEFORE this
+ * forward's advance, so that a tree can be fed level by level.  qlen <= N - first.
+ * Other arguments as sd_verify_attn / sd_verify_attn_paged (block_table NULL: the
+ * contiguous cache, C its capacity; else pools, C is bt_stride * SD_KV_PAGE).
+ * Slots that no node sees may hold anything; V in a slot that some node of the
+ * tree sees has to be finite where other nodes of the row do not see it.
+ * bf16 with D = 128 and Hq / Hkv <= 128 runs on the tensor cores (q, caches
+ * 16-byte aligned, q strides multiples of 8); fp32 and other shapes with D <= 128
+ * on the CUDA cores, without a workspace.  scale > 0.  The workspace must be
+ * 256-byte aligned and needs no initialisation.  If a bounded wait inside the
+ * kernels gives up, the output is NaN.
+ */
+size_t sd_tree_attn_workspace_bytes(int B, int Hq, int Hkv, int D, int C, int qlen, int dtype);
+int sd_tree_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const void* kcache,
+                 const void* vcache, const int32_t* block_table, int bt_stride, int npages,
+                 const int64_t* lengths, const int32_t* masks, int64_t mask_bs, int N, int first,
+                 int B, int Hq, int Hkv, int D, int C, int qlen, float scale, void* out,
+                 int64_t obs, int64_t oqs, int64_t ohs, int dtype, void* workspace,
+                 size_t workspace_bytes, void* stream);
 
 /*
  * Vocabulary-sharded verify round: the SPMD form of sd_verify_sample for a
