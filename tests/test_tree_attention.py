@@ -6,12 +6,13 @@ o = sum p v / l, and A = sum p |v| / l (per output element):
     sum |q k| (u = 2^-24; products of bf16 values are exact), which moves a weight by
     that much relative: at most e_s = (D + 4) u max_s(scale sum |q k|) for every key;
     beyond 2^20 (base 2) the scaled score is rounded by itself, u |score| more;
-    ex2 is good to 2^-21 (approximation or polynomial), and its argument s - m to
-    2 u (|s| + |m|): with |s| <= max |score| that is 6 u max|score| in all;
+    a power of two is good to 2^-18 (the approximation to 2^-21, the polynomial of
+    degree 4 to 2.7e-6), and its argument s - m to 2 u (|s| + |m|): with |s| <= max
+    |score| that is 6 u max|score| in all;
   sums: at most 3 + (keys / 32 + 128) additions deep in any order the kernels use,
     (keys / 32 + 200) u relative, for l and for o;
   bf16: each weight is rounded once, 2^-8 relative of p, and the output 2^-8 of o.
-So |error| <= A (2 (e_s + 6 u max|s| + 2^-21) + 2 (keys / 32 + 200) u [+ 2^-8]) [+ 2^-8 |o|].
+So |error| <= A (2 (e_s + 6 u max|s| + 2^-18) + 2 (keys / 32 + 200) u [+ 2^-8]) [+ 2^-8 |o|].
 """
 import math
 
@@ -125,7 +126,7 @@ def _compare(got, q, ref, first, scale=None):
             o = torch.einsum("hgjs,hsd->jhgd", p, vb)
             av = torch.einsum("hgjs,hsd->jhgd", p, vb.abs())
             big, e_s = float(s.abs().max()), float(sab.max()) * (d + 4) * U
-        rel = 2 * (e_s + 6 * U * big + 2.0 ** -21) + 2 * ((n + N) / 32 + 200) * U
+        rel = 2 * (e_s + 6 * U * big + 2.0 ** -18) + 2 * ((n + N) / 32 + 200) * U
         tol = av * (rel + (2.0 ** -8 if q.dtype == torch.bfloat16 else 0))
         tol = tol + o.abs() * (2.0 ** -8 if q.dtype == torch.bfloat16 else U) + 1e-37
         diff = (got[b].double().view(qlen, hkv, hq // hkv, d) - o).abs()
