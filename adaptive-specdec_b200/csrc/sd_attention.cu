@@ -1222,6 +1222,24 @@ bool cache_map(CUtensorMap* map, const void* base, int64_t rows, int box_rows) {
          CUDA_SUCCESS;
 }
 
+bool tile_map(CUtensorMap* map, const void* base, const int64_t (&sizes)[4],
+              const int64_t (&strides)[3], const int (&box)[4]) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  cuuint64_t dims[4], bytes[3];
+  cuuint32_t tile[4];
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  for (int i = 0; i < 4; ++i) {
+    dims[i] = (cuuint64_t)sizes[i];
+    tile[i] = (cuuint32_t)box[i];
+  }
+  for (int i = 0; i < 3; ++i)                        // (the stride of a dimension of one is any)
+    bytes[i] = sizes[i + 1] > 1 ? (cuuint64_t)strides[i] * 2 : (cuuint64_t)sizes[0] * 2;
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, bytes, tile,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int NTG>
 static int launch_tc_ntg(const AttnParams& P, const CUtensorMap& mk, const CUtensorMap& mv,
                          int nsm, cudaStream_t st) {

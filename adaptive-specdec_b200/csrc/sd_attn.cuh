@@ -53,6 +53,10 @@ __device__ __forceinline__ int row_limit(const AttnParams& P, int b, int j) {
 // sd_attention.cu: a 2D tensor map over a cache viewed as [rows, 128] bf16
 // (boxes of box_rows rows x 64 columns, 128-byte swizzle)
 bool cache_map(CUtensorMap* map, const void* base, int64_t rows, int box_rows = SD_KV_PAGE);
+// A 4D tensor map over bf16 [sizes[3], sizes[2], sizes[1], sizes[0]] with element
+// strides (strides[2], strides[1], strides[0], 1), multiples of 8; 128-byte swizzle
+bool tile_map(CUtensorMap* map, const void* base, const int64_t (&sizes)[4],
+              const int64_t (&strides)[3], const int (&box)[4]);
 
 // sd_prefix_rows.cu: attention over a paged cache row by row, D <= 128
 int prefix_rows(const AttnParams& P, int dtype, cudaStream_t st);

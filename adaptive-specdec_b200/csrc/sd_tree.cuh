@@ -15,12 +15,14 @@ struct TreeParams {
   int N, W, first;                           // nodes, words per node, node of query 0
 };
 
-// Words of a node's mask without the bits from N on.
+// Word w of a node's mask without the bits from N on.
+__device__ __forceinline__ uint32_t tree_valid(int N, int w) {
+  const int left = N - 32 * w;
+  return left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u;
+}
 __device__ __forceinline__ uint32_t tree_word(const int32_t* m, int W, int N, int w) {
   if ((unsigned)w >= (unsigned)W) return 0u;
-  const uint32_t x = (uint32_t)__ldg(m + w);
-  const int left = N - 32 * w;
-  return left >= 32 ? x : x & ((1u << left) - 1u);
+  return (uint32_t)__ldg(m + w) & tree_valid(N, w);
 }
 
 // The tokens of row b before the tree, held in the cache's capacity (a wrong
