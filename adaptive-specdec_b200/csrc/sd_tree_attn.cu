@@ -43,7 +43,8 @@ struct TreeTcParams {
   int rs;                                    // rows of a piece: ni * group, rounded up to 32
   int out_vec;                               // 16-byte stores of the output are aligned
   // workspace
-  int* rowpre;                               // [B + 1] exclusive prefix of a row's units per item
+  int4* cut;                                 // [TT_CTAS] the item that is cut at a CTA's end, if it is the
+                                             // first to work on it: row, kv head, item, pieces (0: none)
   int* status;                               // [TT_CTAS] a bounded wait gave up
   float4* pacc;                              // [2 TT_CTAS][32 column groups][rs] pieces
   float2* pml;                               // [2 TT_CTAS][rs]
@@ -61,9 +62,10 @@ struct TtSmem {
   alignas(1024) unsigned char q[NT][2][128 * 128];           // [tile][64-col box][128 rows x 128 B]
   alignas(1024) unsigned char kv[SLOTS][2][128 * 128];       // [slot][64-col box][128 keys x 128 B]
   alignas(16) unsigned char out[8][32 * 64];         // a warp's 32 rows x 32 outputs
-  // sfull, pfull by step parity; oready by tile and page parity; xch by lane quarter
-  alignas(8) unsigned long long full[SLOTS], empty[SLOTS], sfull[2], pfull[2], oready[NT][2], qfull[NT],
-      qempty[NT], fin;
+  // one tile: sfull, pfull and oready by page parity; two: by tile, of the two halves of S (slo,
+  // shi), of S's second half in registers (sread)
+  alignas(8) unsigned long long full[SLOTS], empty[SLOTS], sfull[2], pfull[2], oready[2], qfull[NT],
+      qempty[NT], slo[2], shi[2], sread[2], fin;
   uint32_t mask[NT][128][TT_WORDS];          // the query rows: their nodes' bits
   // what the threads of a row tell one another: [exchange parity][warpgroup][row], (value, number)
   unsigned long long peer[2][2][128];
@@ -152,14 +154,12 @@ __device__ __forceinline__ void tt_plan(TtSmem<NT>& S, const TreeTcParams& P, in
       carry += sum;
     }
     if (b < B) {
-      if (cta == 0) P.rowpre[b] = ex;
       if ((int64_t)ex * per <= t0 && t0 < (int64_t)(ex + mine) * per) {
         S.first[0] = b;
         S.first[1] = ex * per;
       }
     }
   }
-  if (cta == 0 && t == 0) P.rowpre[B] = all;
 }
 
 // A whole warp's arrival, as one.
@@ -268,48 +268,589 @@ __device__ __forceinline__ void tt_write(unsigned char* stage, const float (&o)[
   __syncwarp();
 }
 
-#ifndef TTV
-#define TTV 0
-#endif
-__device__ __forceinline__ void tt_weights(const uint32_t (&s)[32], uint32_t* p,
-                                           unsigned long long (&sum)[2], unsigned long long sl22,
-                                           unsigned long long nm2) {
-#if TTV == 0
-  px_weights(s, p, sum, sl22, nm2);
-#elif TTV == 1
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    float a, b;
-    const unsigned long long s2 = pair2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
-    unpair(fma2(s2, sl22, nm2), a, b);
-    const unsigned long long p2 = pair2(ex2f(a), ex2f(b));
-    sum[e & 1] = add2(sum[e & 1], p2);
-    unpair(p2, a, b);
-    p[e] = pack_bf16(a, b);
+// ---- the roles of a CTA's warps ---------------------------------------------------------------
+// Q of a tile of a segment's item: its nodes x heads.
+template <int NT>
+__device__ __forceinline__ void tt_ask_q(TtSmem<NT>& S, const TreeTcParams& P, const CUtensorMap& tmq,
+                                         const TtSeg& g, int ti) {
+  const int group = P.T.A.group, j = g.p * P.ni + P.nt * ti;
+  tc_expect_tx(&S.qfull[ti], 2u * 128u * (uint32_t)(P.nt * group));
+  tt_tma_4d(S.q[ti][0], &tmq, 0, g.h * group, j, g.b, &S.qfull[ti]);
+  tt_tma_4d(S.q[ti][1], &tmq, 64, g.h * group, j, g.b, &S.qfull[ti]);
+}
+
+// TMA producer (one thread): K then V of each page, SLOTS tiles ahead; the first segment's Q
+// in front, before all SMs' K and V are on their way.
+template <int NT>
+__device__ __forceinline__ void tt_load_kv(TtSmem<NT>& S, const TreeTcParams& P, const CUtensorMap& tmk,
+                                           const CUtensorMap& tmv, const CUtensorMap& tmq, TtSeg seg,
+                                           bool more, int share) {
+  constexpr int SLOTS = TtSmem<NT>::SLOTS;
+  int4 cut = make_int4(0, 0, 0, 0);
+  for (int ti = 0; ti < NT && more; ++ti) tt_ask_q(S, P, tmq, seg, ti);
+  uint32_t idx = 0;
+  bool ok = true;
+  while (more && ok) {
+    for (int j = seg.j0; j < seg.j1 && ok; ++j) {
+      const int y = (int)kv_row(P.T.A, seg.b, seg.h, j * SD_KV_PAGE);
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv, ++idx) {
+        const int sl = (int)(idx % SLOTS);
+        if (idx >= (uint32_t)SLOTS) ok = tc_wait(&S.empty[sl], ((idx / SLOTS) - 1) & 1u, &S.abort_);
+        if (!ok) break;
+        tc_expect_tx(&S.full[sl], 2u * 128u * 128u);
+        const void* map = kv ? (const void*)&tmv : (const void*)&tmk;
+        tc_tma_2d(S.kv[sl][0], map, 0, y, &S.full[sl]);
+        tc_tma_2d(S.kv[sl][1], map, 64, y, &S.full[sl]);
+      }
+    }
+    if (seg.j0 == 0 && seg.j1 + TT_OVH < seg.tb)     // (the last segment)
+      cut = make_int4(seg.b, seg.h, seg.p, (seg.tt - seg.off + seg.tb - 1) / share - (int)blockIdx.x + 1);
+    if (ok) more = tt_next(seg, S, P) && tt_real(seg, S, P);
   }
-#elif TTV == 2
-  float sl, nm, d, t0, t1, t2, t3;
-  unpair(sl22, sl, d); unpair(nm2, nm, d); unpair(sum[0], t0, t1); unpair(sum[1], t2, t3);
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const float a = ex2f(fmaf(__uint_as_float(s[2 * e]), sl, nm)), b = ex2f(fmaf(__uint_as_float(s[2 * e + 1]), sl, nm));
-    if (e & 1) { t0 += a; t1 += b; } else { t2 += a; t3 += b; }
-    p[e] = pack_bf16(a, b);
+  P.cut[blockIdx.x] = cut;
+  if (!ok) {
+    // let the copies already issued land before the CTA leaves
+    for (uint32_t q = idx > (uint32_t)SLOTS ? idx - SLOTS : 0u; q < idx; ++q) {
+      int dummy = 0;
+      tc_wait(&S.full[q % SLOTS], (q / SLOTS) & 1u, &dummy);
+    }
   }
-  sum[0] = pair2(t0, t1); sum[1] = pair2(t2, t3);
-#elif TTV == 3
-  float sl, nm, d, t0, t1, t2, t3;
-  unpair(sl22, sl, d); unpair(nm2, nm, d); unpair(sum[0], t0, t1); unpair(sum[1], t2, t3);
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    float a, b;
-    if (e % 8 == 1) unpair(px_exp2(fmaf(__uint_as_float(s[2 * e]), sl, nm), fmaf(__uint_as_float(s[2 * e + 1]), sl, nm)), a, b);
-    else { a = ex2f(fmaf(__uint_as_float(s[2 * e]), sl, nm)); b = ex2f(fmaf(__uint_as_float(s[2 * e + 1]), sl, nm)); }
-    if (e & 1) { t0 += a; t1 += b; } else { t2 += a; t3 += b; }
-    p[e] = pack_bf16(a, b);
+}
+
+// TMA producer (one thread) of the later segments' Q, once a tile's last S is done.
+template <int NT>
+__device__ __forceinline__ void tt_load_q(TtSmem<NT>& S, const TreeTcParams& P, const CUtensorMap& tmq,
+                                          TtSeg seg, bool more) {
+  uint32_t sent = more ? NT : 0u;                    // tiles asked for, tile inner
+  bool ok = true;
+  while (ok && more && tt_next(seg, S, P) && tt_real(seg, S, P)) {
+    for (int ti = 0; ti < NT; ++ti, ++sent) {
+      ok = tc_wait(&S.qempty[ti], (sent / NT - 1) & 1u, &S.abort_);
+      if (!ok) break;
+      tt_ask_q(S, P, tmq, seg, ti);
+    }
   }
-  sum[0] = pair2(t0, t1); sum[1] = pair2(t2, t3);
-#endif
+  if (!ok) {
+    // let the copies already issued land before the CTA leaves
+    for (uint32_t q = sent > (uint32_t)NT ? sent - NT : 0u; q < sent; ++q) {
+      int dummy = 0;
+      tc_wait(&S.qfull[q % NT], (q / NT) & 1u, &dummy);
+    }
+  }
+}
+
+constexpr uint32_t TT_ID_S = tc_idesc(128, 128, 0, 0);       // S = Q . K^T of 128 keys
+constexpr uint32_t TT_ID_H = tc_idesc(128, 64, 0, 0);        // of 64 keys
+constexpr uint32_t TT_ID_O = tc_idesc(128, 128, 0, 1);       // O += P . V (V [key][d]: N-major)
+
+// S = Q . K^T by a warp: 16 of 128 d an MMA: 32 B, the second box 16 KB on.
+__device__ __forceinline__ void tt_mma_s(uint32_t d, uint32_t q, uint32_t k, uint32_t id) {
+  const uint64_t dq = tc_desc(q, 16, 1024, 2), dk = tc_desc(k, 16, 1024, 2);
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+    const uint64_t o = (uint64_t)((ks & 3) * 2 + (ks >> 2) * 1024);
+    tc_mma_warp(d, dq + o, dk + o, id, ks > 0 ? 1 : 0);
+  }
+}
+// O (+)= P . V by a warp: 16 keys an MMA: 2 KB of V, 8 columns of P, whose second 64 keys start
+// at column `half`.
+__device__ __forceinline__ void tt_mma_o(uint32_t o, uint32_t p, uint32_t half, uint32_t v, bool acc) {
+  const uint64_t dv = tc_desc(v, 16384, 1024, 2);
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks)
+    tc_mma_ts_warp(o, p + half * (ks >> 2) + 8u * (ks & 3), dv + (uint64_t)(ks * 128), TT_ID_O,
+                   ks || acc ? 1 : 0);
+}
+// An issuer that has found nothing to do since `idle` (0: it has just begun): whether it goes on.
+__device__ __forceinline__ bool tt_idle(long long& idle, int* abort_) {
+  const long long now = clock64();
+  if (idle == 0) idle = now;
+  if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(abort_) || now - idle > TC_WAIT)) {
+    *reinterpret_cast<volatile int*>(abort_) = 1;
+    return false;
+  }
+  return true;
+}
+// Every MMA that this warp issued has finished before the CTA leaves.
+__device__ __forceinline__ void tt_finish(unsigned long long* bar) {
+  tc_commit_warp(bar);
+  int dummy = 0;
+  tc_wait(bar, 0u, &dummy);
+}
+
+// MMA issuer of one tile: S(0) S(1) P.V(0) S(2) P.V(1) ...; S of page i in buffer i & 1 (128
+// columns each), P over it; where S's tiles are late, P . V does not wait for it.
+__device__ __forceinline__ void tt_issue_one(TtSmem<1>& S, const TreeTcParams& P, TtSeg seg, bool more) {
+  constexpr int SLOTS = TtSmem<1>::SLOTS;
+  const uint32_t kv0 = smem_addr(S.kv[0][0]), q0 = smem_addr(S.q[0][0]), tm = S.tmem;
+  TtSeg back = seg;
+  int ahead = seg.j1 - seg.j0, behind = ahead;       // pages left of the segments of S and of P . V
+  uint32_t a = 0, c = 0, qn = 0;                     // pages issued; segments begun by S
+  bool ok = true, acc = false;
+  long long idle = 0;
+  while (ok) {
+    const uint32_t ki = 2u * a, vi = 2u * c + 1u;
+    unsigned long long* vfull = &S.full[vi % SLOTS];
+    bool s_go = false, p_go = false;
+    if (more && a < c + 2u)
+      s_go = __all_sync(0xffffffffu, tc_test(&S.full[ki % SLOTS], (ki / SLOTS) & 1u) &&
+                                         tc_test(&S.qfull[0], qn & 1u));
+    if (!s_go && c < a) {
+      if (more && a < c + 2u)
+        p_go = __all_sync(0xffffffffu, tc_test(vfull, (vi / SLOTS) & 1u) &&
+                                           tc_test(&S.pfull[c & 1u], (c >> 1) & 1u));
+      else
+        p_go = ok = tc_wait2_warp(vfull, (vi / SLOTS) & 1u, &S.pfull[c & 1u], (c >> 1) & 1u, &S.abort_);
+    }
+    if (!s_go && !p_go) {
+      if (!ok || (c == a && !more) || !tt_idle(idle, &S.abort_)) break;
+      continue;
+    }
+    idle = 0;
+    tc_fence_after();
+    if (s_go) {
+      tt_mma_s(tm + 128u * (a & 1u), q0, kv0 + (ki % SLOTS) * 32768u, TT_ID_S);
+      tc_commit_warp(&S.sfull[a & 1u]);
+      tc_commit_warp(&S.empty[ki % SLOTS]);
+      ++a;
+      if (--ahead == 0) {                            // the segment's last S: Q may be replaced
+        tc_commit_warp(&S.qempty[0]);
+        more = tt_next(seg, S, P) && tt_real(seg, S, P);
+        ahead = seg.j1 - seg.j0;
+        ++qn;
+      }
+      continue;
+    }
+    tt_mma_o(tm + 256u, tm + 128u * (c & 1u), 64u, kv0 + (vi % SLOTS) * 32768u, acc);
+    tc_commit_warp(&S.oready[c & 1u]);
+    tc_commit_warp(&S.empty[vi % SLOTS]);
+    ++c;
+    acc = true;
+    if (--behind == 0) {
+      if (!(tt_next(back, S, P) && tt_real(back, S, P))) break;
+      behind = back.j1 - back.j0;
+      acc = false;
+    }
+  }
+  tt_finish(&S.fin);
+}
+
+// MMA issuer of two tiles.  S comes in halves of 64 keys: with H0, H1 the two 64-column halves
+// of a tile's S, page i has its first half in H(i & 1) and its second in the other one; P of the
+// whole page lies over the first, so the second is free as soon as it is in registers, and the
+// next page's first half goes there before this page's P is made.  The tiles take turns in a fixed
+// order, half a page apart: left to themselves they fall into step, and softmax and tensor cores
+// wait for one another (8 rows of 64 nodes over 16384 keys: 171 us instead of 167).
+__device__ __forceinline__ void tt_issue_pair(TtSmem<2>& S, const TreeTcParams& P, TtSeg seg, bool more) {
+  constexpr int SLOTS = TtSmem<2>::SLOTS;
+  const uint32_t kv0 = smem_addr(S.kv[0][0]), q0 = smem_addr(S.q[0][0]), tm = S.tmem;
+  uint32_t g = 0, qn = 0;                            // page of the next P . V; segments done
+  bool ok = true;
+  // the first or second half of S of page i of tile x
+  auto issue_s = [&](uint32_t x, uint32_t i, uint32_t half) {
+    tt_mma_s(tm + 128u * x + 64u * ((i + half) & 1u), q0 + x * 32768u,
+             kv0 + (2u * i % SLOTS) * 32768u + half * 8192u, TT_ID_H);
+    tc_commit_warp(half ? &S.shi[x] : &S.slo[x]);
+    if (half && x == 1u) tc_commit_warp(&S.empty[2u * i % SLOTS]);
+  };
+  while (more && ok) {
+    int pages = seg.j1 - seg.j0;
+    // the segment's first S, of both tiles
+#pragma unroll 1
+    for (uint32_t x = 0; x < 2u && ok; ++x) {
+      ok = tc_wait2_warp(&S.full[2u * g % SLOTS], (2u * g / SLOTS) & 1u, &S.qfull[x], qn & 1u, &S.abort_);
+      if (!ok) break;
+      tc_fence_after();
+      issue_s(x, g, 0u);
+      issue_s(x, g, 1u);
+      if (pages == 1) tc_commit_warp(&S.qempty[x]);
+    }
+#pragma unroll 1
+    for (; pages > 0 && ok; --pages, ++g) {
+      const uint32_t ki = 2u * (g + 1u), vi = 2u * g + 1u;
+#pragma unroll 1
+      for (uint32_t x = 0; x < 2u; ++x) {
+        if (pages > 1) {
+          ok = tc_wait2_warp(&S.full[ki % SLOTS], (ki / SLOTS) & 1u, &S.sread[x], g & 1u, &S.abort_);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(x, g + 1u, 0u);
+        }
+        ok = tc_wait2_warp(&S.full[vi % SLOTS], (vi / SLOTS) & 1u, &S.pfull[x], g & 1u, &S.abort_);
+        if (!ok) break;
+        tc_fence_after();
+        tt_mma_o(tm + 256u + 128u * x, tm + 128u * x + 64u * (g & 1u), 32u, kv0 + (vi % SLOTS) * 32768u,
+                 pages < seg.j1 - seg.j0);
+        tc_commit_warp(&S.oready[x]);
+        if (x == 1u) tc_commit_warp(&S.empty[vi % SLOTS]);
+        if (pages > 1) issue_s(x, g + 1u, 1u);
+        if (pages == 2) tc_commit_warp(&S.qempty[x]);        // the segment's last S: Q may be replaced
+      }
+    }
+    ++qn;
+    if (ok) more = tt_next(seg, S, P) && tt_real(seg, S, P);
+  }
+  tt_finish(&S.fin);
+}
+
+// What the softmax warps know of a segment's nodes.
+struct TtNodes {
+  int b = -1, p = -1;                                // the row and item that these are of
+  uint32_t uni = 0;                                  // lane i: word i of what any query of the row sees
+  bool settled = false, there = false;               // the bits are in; the thread's node is present
+};
+// A thread's row r of tile ti: its node's bits to shared memory (asked for now, used in the
+// tree's pages), unless they are there.
+template <int NT>
+__device__ __forceinline__ void tt_ask_nodes(TtNodes& N, TtSmem<NT>& S, const TreeTcParams& P,
+                                             const TtSeg& g, int ti, int r, bool live) {
+  const TreeParams& T = P.T;
+  if (N.p == g.p && (N.b == g.b || (N.b >= 0 && T.mask_bs == 0))) return;
+  if (!N.settled) asm volatile("cp.async.wait_all;" ::: "memory");       // an older copy first
+  const int32_t* m = T.masks + (int64_t)g.b * T.mask_bs +
+                     (int64_t)(T.first + g.p * P.ni + P.nt * ti + r / T.A.group) * T.W;
+  for (int i = 0; i < T.W; ++i) {
+    if (live)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
+                   :: "r"(smem_addr(&S.mask[ti][r][i])), "l"(m + i) : "memory");
+    else
+      S.mask[ti][r][i] = 0u;
+  }
+  N.settled = false;
+  N.b = g.b;
+  N.p = g.p;
+}
+template <int NT>
+__device__ __forceinline__ void tt_settle(TtNodes& N, const TtSmem<NT>& S, const TreeTcParams& P,
+                                          const TtSeg& g, int ti, int r) {
+  const TreeParams& T = P.T;
+  const int lane = threadIdx.x & 31;
+  const int32_t* m = T.masks + (int64_t)g.b * T.mask_bs + (int64_t)T.first * T.W;
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  uint32_t some = 0, uni = 0;
+  for (int i = 0; i < T.W; ++i) {
+    some |= S.mask[ti][r][i] & tree_valid(T.N, i);
+    uint32_t word = 0;
+#pragma unroll 4
+    for (int q = lane; q < T.A.qlen; q += 32) word |= tree_word(m + (int64_t)q * T.W, T.W, T.N, i);
+    word = __reduce_or_sync(0xffffffffu, word);
+    if (lane == i) uni = word;
+  }
+  N.uni = uni;
+  N.there = some != 0u;
+  N.settled = true;
+}
+
+// The largest of 64 scores.
+__device__ __forceinline__ float tt_largest(const uint32_t (&s0)[32], const uint32_t (&s1)[32]) {
+  float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) {
+    px_max3(mx[e & 2], s0[e], s0[e + 1]);
+    px_max3(mx[(e & 2) + 1], s1[e], s1[e + 1]);
+  }
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+// The weights of 64 scores as bf16 pairs under the reference m, and their sum.
+__device__ __forceinline__ float tt_weights(uint32_t (&s0)[32], uint32_t (&s1)[32], uint32_t (&pk)[32],
+                                            float m, float sl2, bool wild) {
+  if (wild) {
+    px_scale(s0, sl2);
+    px_scale(s1, sl2);
+  }
+  const float mc = m == -CUDART_INF_F ? 0.f : m, sf = wild ? 1.f : sl2;
+  const unsigned long long sl22 = pair2(sf, sf), nm2 = pair2(-mc, -mc);
+  unsigned long long ls[2] = {0ULL, 0ULL};           // (0.f, 0.f)
+  px_weights(s0, pk, ls, sl22, nm2);
+  px_weights(s1, pk + 16, ls, sl22, nm2);
+  float a, b;
+  unpair(add2(ls[0], ls[1]), a, b);
+  return a + b;
+}
+// Columns [col, col + n) of O times alpha.
+__device__ __forceinline__ void tt_rescale(uint32_t col, int n, float alpha) {
+#pragma unroll 1
+  for (int q = 0; q < n; q += 16) {
+    uint32_t o[16];
+    TC_LD16(o, col + (uint32_t)q);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+    TC_ST16(col + (uint32_t)q, o);
+  }
+}
+// Columns [32 q0, 32 q1) of a thread's row of O: divided by the row's sum and written out, or as
+// a piece.  oc: TMEM column of O (with the warp's lanes).
+template <int NT>
+__device__ __forceinline__ void tt_emit(TtSmem<NT>& S, const TreeTcParams& P, const TtSeg& g, int ti, int r,
+                                        bool live, bool there, float m, float l, uint32_t oc, int q0, int q1) {
+  const AttnParams& A = P.T.A;
+  const bool whole = g.j0 == 0 && g.j1 + TT_OVH == g.tb;
+  const float il = !whole ? 1.f : l == 0.f || !there ? 0.f : 1.f / l;    // (a NaN sum: NaN)
+  const int jt = r / A.group, j = g.p * P.ni + P.nt * ti + jt, hq = g.h * A.group + r - jt * A.group;
+  __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(A.out) + g.b * A.obs + j * A.oqs + hq * A.ohs;
+  const int slot = 2 * (int)blockIdx.x + (g.j0 == 0), pr = P.nt * A.group * ti + r;
+  float4* part = P.pacc + (int64_t)slot * (TT_D / 4) * P.rs + pr;
+#pragma unroll 1
+  for (int q = q0; q < q1; ++q) {
+    uint32_t u[32];
+    TC_LD32(u, oc + 32u * q);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    float o[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = il == 0.f ? 0.f : il * __uint_as_float(u[e]);
+    if (whole) {
+      tt_write(S.out[threadIdx.x >> 5], o, out + 32 * q, live, P.out_vec != 0);
+    } else if (live) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        part[(int64_t)(8 * q + e) * P.rs] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+    }
+    __syncwarp();
+  }
+  if (!whole && live && q0 == 0) P.pml[(int64_t)slot * P.rs + pr] = make_float2(m, l);
+}
+// Query rows of tile ti of a segment's item.
+__device__ __forceinline__ int tt_rows(const TreeTcParams& P, const TtSeg& g, int ti) {
+  const AttnParams& A = P.T.A;
+  return A.group * min(min(P.nt, P.ni - P.nt * ti), A.qlen - g.p * P.ni - P.nt * ti);
+}
+// What moves from reference m to mn: 2^(m - mn) of the sums and of O.
+__device__ __forceinline__ float tt_alpha(float m, float mn) {
+  return m == -CUDART_INF_F ? 0.f : ex2f(m - mn);
+}
+
+// Softmax of one tile: the threads of warpgroups 0 and 1 with the same lane own the same query
+// row, x takes the keys [64 x, 64 x + 64) of a page and half of the columns of O.
+__device__ __forceinline__ void tt_softmax_one(TtSmem<1>& S, const TreeTcParams& P, TtSeg seg, bool more) {
+  constexpr int SLOTS = TtSmem<1>::SLOTS;
+  const TreeParams& T = P.T;
+  const int t = threadIdx.x, w = t >> 5, x = w >> 2, wq = w & 3, r = t & 127;
+  const uint32_t lcol = S.tmem + ((uint32_t)(32 * wq) << 16), ocol = lcol + 256u;
+  const float sl2 = T.A.scale * 1.4426950408889634f;
+  uint32_t n = 0, xn = 0;                            // pages done; exchanges with the peer
+  bool ok = true;
+  // A value to the thread with the row's other keys, and that thread's (a word of shared memory
+  // holds the value and the exchange's number; two of them by parity, as the peer may be one
+  // exchange ahead).  `ok` is false when a bounded wait gives up.
+  auto tell = [&](float v) {
+    ++xn;
+    *reinterpret_cast<volatile unsigned long long*>(&S.peer[xn & 1u][x][r]) =
+        ((unsigned long long)xn << 32) | __float_as_uint(v);
+  };
+  auto told = [&]() {
+    const volatile unsigned long long* from = &S.peer[xn & 1u][x ^ 1][r];
+    unsigned long long v = *from;
+    long long since = 0;
+    while ((uint32_t)(v >> 32) != xn) {
+      const long long now = clock64();
+      if (since == 0) since = now;
+      if (*reinterpret_cast<volatile int*>(&S.abort_) || now - since > TC_WAIT) {
+        *reinterpret_cast<volatile int*>(&S.abort_) = 1;
+        ok = false;
+        break;
+      }
+      v = *from;
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    return __uint_as_float((uint32_t)v);
+  };
+  // P . V of page n - 1 is in O (that of page n - 2 may be under way, too: two barriers)
+  auto o_ready = [&]() {
+    return __all_sync(0xffffffffu,
+                      tc_wait(&S.oready[(n - 1) & 1u], ((n - 1) >> 1) & 1u, &S.abort_));
+  };
+  TtNodes nodes;
+  while (more) {
+    const TtSeg cur = seg;
+    more = tt_next(seg, S, P) && tt_real(seg, S, P);
+    const int pages = cur.j1 - cur.j0, end = tree_end(T, cur.base);
+    const bool live = r < tt_rows(P, cur, 0), dead = __all_sync(0xffffffffu, !live);
+    tt_ask_nodes(nodes, S, P, cur, 0, r, live);
+    float m = -CUDART_INF_F, l = 0.f;
+    bool wild = false;
+#pragma unroll 1
+    for (int i = 0; i < pages; ++i, ++n) {
+      ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[n & 1u], (n >> 1) & 1u, &S.abort_));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t scol = lcol + 128u * (n & 1u) + 64u * x;
+      const int key0 = (cur.j0 + i) * SD_KV_PAGE;
+      if (key0 + SD_KV_PAGE > cur.base) {
+        // the tree's pages, and what lies behind it
+        if (!nodes.settled) tt_settle(nodes, S, P, cur, 0, r);
+        if (!dead) tt_hide(S.mask[0][r], T, cur.base, end, key0 + 64 * x, 64, scol);
+        // V: each warpgroup its half of the keys, two warps 32 of them
+        const uint32_t vi = 2u * n + 1u;
+        const int grp = 2 * x + (wq & 1);
+        ok = tt_blank(S.kv[vi % SLOTS], T, nodes.uni, cur.base, end, key0 + 32 * grp, 32 * grp, wq >> 1,
+                      (wq >> 1) + 1, &S.full[vi % SLOTS], (vi / SLOTS) & 1u, &S.abort_);
+        if (!ok) break;
+      }
+      if (!dead) {
+        uint32_t s0[32], s1[32], pk[32];
+        if (i == 0) {                                // a reference for the segment, for both halves
+          TC_LD32(s0, scol);
+          TC_LD32(s1, scol + 32u);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          const float mine = tt_largest(s0, s1) * sl2;
+          tell(mine);
+          m = fmaxf(mine, told());
+          if (!ok) break;
+          wild = px_wild(m);
+        }
+        // weights under the reference as it is, and the largest score beside them: where that is
+        // too far above it (rare), the reference moves and the weights are made again
+        float sum;
+        while (true) {
+          TC_LD32(s0, scol);
+          TC_LD32(s1, scol + 32u);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          const float mine = tt_largest(s0, s1) * sl2;
+          tell(mine);
+          sum = tt_weights(s0, s1, pk, m, sl2, wild);
+          const float mt = fmaxf(mine, told());
+          if (!ok) break;
+          const bool move = mt > m + PX_HEADROOM;
+          if (!__any_sync(0xffffffffu, move)) break;
+          const float mn = move ? mt : m, alpha = move ? tt_alpha(m, mn) : 1.f;
+          m = mn;
+          l *= alpha;
+          wild = px_wild(m);
+          if (i > 0) {
+            // O holds this segment's earlier pages: the last P . V into it first
+            ok = o_ready();
+            if (!ok) break;
+            tc_fence_after();
+            tt_rescale(ocol + 64u * x, 64, alpha);
+          }
+        }
+        if (!ok) break;
+        l += sum;
+        TC_ST32(scol, pk);                           // over columns that have been read
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      }
+      tc_fence_before();
+      tt_arrive(&S.pfull[n & 1u]);
+    }
+    if (!ok) break;
+    if (!dead) {
+      tell(l);
+      const float lp = told();
+      ok = ok && o_ready();
+      if (!ok) break;
+      tc_fence_after();
+      l = x ? lp + l : l + lp;                       // (the first warpgroup's half first, in both)
+      tt_emit(S, P, cur, 0, r, live, nodes.there, m, l, ocol, 2 * x, 2 * x + 2);
+    }
+    tc_fence_before();
+  }
+}
+
+// Softmax of two tiles: a thread owns its query row of tile x, warpgroup x.
+__device__ __forceinline__ void tt_softmax_pair(TtSmem<2>& S, const TreeTcParams& P, TtSeg seg, bool more) {
+  constexpr int SLOTS = TtSmem<2>::SLOTS;
+  const TreeParams& T = P.T;
+  const int t = threadIdx.x, w = t >> 5, x = w >> 2, wq = w & 3, r = t & 127;
+  const uint32_t lcol = S.tmem + ((uint32_t)(32 * wq) << 16) + 128u * x, ocol = lcol + 256u;
+  const float sl2 = T.A.scale * 1.4426950408889634f;
+  uint32_t n = 0;                                    // pages done
+  bool ok = true;
+  // P . V of page n - 1 is in O
+  auto o_ready = [&]() {
+    return __all_sync(0xffffffffu, tc_wait(&S.oready[x], (n - 1) & 1u, &S.abort_));
+  };
+  TtNodes nodes;
+  while (more) {
+    const TtSeg cur = seg;
+    more = tt_next(seg, S, P) && tt_real(seg, S, P);
+    const int pages = cur.j1 - cur.j0, end = tree_end(T, cur.base);
+    const bool live = r < tt_rows(P, cur, x), dead = __all_sync(0xffffffffu, !live);
+    tt_ask_nodes(nodes, S, P, cur, x, r, live);
+    float m = -CUDART_INF_F, l = 0.f;
+    bool wild = false;
+#pragma unroll 1
+    for (int i = 0; i < pages; ++i, ++n) {
+      const uint32_t pcol = lcol + 64u * (n & 1u);   // P, over the page's first half of S
+      const int key0 = (cur.j0 + i) * SD_KV_PAGE;
+      const bool tree = key0 + SD_KV_PAGE > cur.base;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        ok = __all_sync(0xffffffffu, tc_wait(half ? &S.shi[x] : &S.slo[x], n & 1u, &S.abort_));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t scol = lcol + 64u * ((n + (uint32_t)half) & 1u);
+        if (tree) {
+          // the tree's pages, and what lies behind it (V: both tiles the same)
+          if (!nodes.settled) tt_settle(nodes, S, P, cur, x, r);
+          if (!dead) tt_hide(S.mask[x][r], T, cur.base, end, key0 + 64 * half, 64, scol);
+          if (half) {
+            const uint32_t vi = 2u * n + 1u;
+            ok = tt_blank(S.kv[vi % SLOTS], T, nodes.uni, cur.base, end, key0 + 32 * wq, 32 * wq, 0, 2,
+                          &S.full[vi % SLOTS], (vi / SLOTS) & 1u, &S.abort_);
+            if (!ok) break;
+          }
+        }
+        if (dead) {
+          if (half) tt_arrive(&S.sread[x]);
+          continue;
+        }
+        uint32_t s0[32], s1[32], pk[32];
+        TC_LD32(s0, scol);
+        TC_LD32(s1, scol + 32u);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (half) {
+          tc_fence_before();
+          tt_arrive(&S.sread[x]);
+        }
+        const float mt = tt_largest(s0, s1) * sl2;
+        const bool move = mt > m + PX_HEADROOM;
+        if (__any_sync(0xffffffffu, move)) {
+          // (between the halves by a whole number, or next to one: the weights already made are
+          // scaled by a power of two, which rounds nothing)
+          const float up = half && m != -CUDART_INF_F ? m + ceilf(mt - m) : mt;
+          const float mn = move ? up : m, alpha = move ? tt_alpha(m, mn) : 1.f;
+          m = mn;
+          l *= alpha;
+          wild = px_wild(m);
+          if (half) {
+            // the page's first weights, already made
+            TC_LD32(pk, pcol);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            const __nv_bfloat162 a2 = __float2bfloat162_rn(alpha);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              __nv_bfloat162 v = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&pk[e]), a2);
+              pk[e] = *reinterpret_cast<uint32_t*>(&v);
+            }
+            TC_ST32(pcol, pk);
+          }
+          if (i > 0) {
+            // O holds this segment's earlier pages: the last P . V into it first
+            ok = o_ready();
+            if (!ok) break;
+            tc_fence_after();
+            tt_rescale(ocol, 128, alpha);
+          }
+        }
+        l += tt_weights(s0, s1, pk, m, sl2, wild);
+        TC_ST32(pcol + 32u * half, pk);              // over columns that have been read
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      }
+      if (!ok) break;
+      tc_fence_before();
+      tt_arrive(&S.pfull[x]);
+    }
+    if (!ok) break;
+    if (!dead) {
+      ok = o_ready();
+      if (!ok) break;
+      tc_fence_after();
+      tt_emit(S, P, cur, x, r, live, nodes.there, m, l, ocol, 0, 4);
+    }
+    tc_fence_before();
+  }
 }
 
 template <int NT>
@@ -319,9 +860,7 @@ tree_tc_kernel(const __grid_constant__ TreeTcParams P, const __grid_constant__ C
   extern __shared__ __align__(1024) unsigned char tt_raw[];
   const uint32_t pad = (1024u - (smem_addr(tt_raw) & 1023u)) & 1023u;   // swizzle atoms: 1024 B
   TtSmem<NT>& S = *reinterpret_cast<TtSmem<NT>*>(tt_raw + pad);
-  constexpr int SLOTS = TtSmem<NT>::SLOTS;
   const TreeParams& T = P.T;
-  const AttnParams& A = T.A;
   const int t = threadIdx.x, w = t >> 5, lane = t & 31, cta = (int)blockIdx.x;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (w == 9) {
@@ -330,39 +869,39 @@ tree_tc_kernel(const __grid_constant__ TreeTcParams P, const __grid_constant__ C
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (t == 256) {
-    for (int i = 0; i < SLOTS; ++i) {
+    for (int i = 0; i < TtSmem<NT>::SLOTS; ++i) {
       tc_bar_init(&S.full[i], 1);
       tc_bar_init(&S.empty[i], 1);
     }
     for (int x = 0; x < 2; ++x) {
       tc_bar_init(&S.sfull[x], 1);
-      tc_bar_init(&S.pfull[x], 8);
+      tc_bar_init(&S.slo[x], 1);
+      tc_bar_init(&S.shi[x], 1);
+      tc_bar_init(&S.sread[x], 4);
+      tc_bar_init(&S.pfull[x], NT == 2 ? 4 : 8);     // warps
+      tc_bar_init(&S.oready[x], 1);
     }
+    tc_bar_init(&S.fin, 1);
     for (int x = 0; x < NT; ++x) {
       tc_bar_init(&S.qfull[x], 1);
       tc_bar_init(&S.qempty[x], 1);
-      tc_bar_init(&S.oready[x][0], 1);
-      tc_bar_init(&S.oready[x][1], 1);
     }
-    tc_bar_init(&S.fin, 1);
     S.abort_ = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int i = t; i < 2 * 2 * 128; i += TT_THREADS) S.peer[0][0][i] = 0ULL;     // (numbers start at 1)
   // the rows of a tile that no query fills stay 0
-  for (int i = P.nt * A.group * 8 + t; i < NT * 2 * 128 * 8; i += TT_THREADS)
-    if (i % 1024 >= P.nt * A.group * 8)
-      reinterpret_cast<uint4*>(S.q[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
+  const int filled = P.nt * T.A.group * 8;
+  for (int i = t; i < NT * 2 * 128 * 8; i += TT_THREADS)
+    if (i % 1024 >= filled) reinterpret_cast<uint4*>(S.q[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   int total, share;
   tt_plan(S, P, &total, &share);
-  const bool work = (int64_t)cta * share < total;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tm = S.tmem;
-  if (work) {
-    const int t0 = cta * share, t1 = t0 + min(total - t0, share);
+  if ((int64_t)cta * share < total) {
+    const int t0 = cta * share;
     TtSeg seg;
     seg.b = S.first[0];
     seg.base = tt_base(S, T, seg.b);
@@ -372,423 +911,34 @@ tree_tc_kernel(const __grid_constant__ TreeTcParams P, const __grid_constant__ C
     seg.h = it / P.np;
     seg.p = it % P.np;
     seg.tt = t0;
-    seg.t1 = t1;
+    seg.t1 = t0 + min(total - t0, share);
     tt_bounds(seg);
-    bool more = tt_real(seg, S, P);
-
-    // Q of a tile of a segment's item: its nodes x heads
-    auto ask_q = [&](const TtSeg& g, int ti) {
-      const int j = g.p * P.ni + P.nt * ti;
-      tc_expect_tx(&S.qfull[ti], 2u * 128u * (uint32_t)(P.nt * A.group));
-      tt_tma_4d(S.q[ti][0], &tmq, 0, g.h * A.group, j, g.b, &S.qfull[ti]);
-      tt_tma_4d(S.q[ti][1], &tmq, 64, g.h * A.group, j, g.b, &S.qfull[ti]);
-    };
+    const bool more = tt_real(seg, S, P);
     if (w == 8) {
-      if (lane == 0) {
-        // ---------------- TMA producer: K then V of each page, SLOTS tiles ahead; the first
-        // segment's Q in front, before all SMs' K and V are on their way
-        for (int ti = 0; ti < NT && more; ++ti) ask_q(seg, ti);
-        uint32_t idx = 0;
-        bool ok = true;
-        while (more && ok) {
-          for (int j = seg.j0; j < seg.j1 && ok; ++j) {
-            const int y = (int)kv_row(A, seg.b, seg.h, j * SD_KV_PAGE);
-#pragma unroll 1
-            for (int kv = 0; kv < 2; ++kv, ++idx) {
-              const int sl = (int)(idx % SLOTS);
-              if (idx >= (uint32_t)SLOTS)
-                ok = tc_wait(&S.empty[sl], ((idx / SLOTS) - 1) & 1u, &S.abort_);
-              if (!ok) break;
-              tc_expect_tx(&S.full[sl], 2u * 128u * 128u);
-              const void* map = kv ? (const void*)&tmv : (const void*)&tmk;
-              tc_tma_2d(S.kv[sl][0], map, 0, y, &S.full[sl]);
-              tc_tma_2d(S.kv[sl][1], map, 64, y, &S.full[sl]);
-            }
-          }
-          if (ok) more = tt_next(seg, S, P) && tt_real(seg, S, P);
-        }
-        if (!ok) {
-          // let the copies already issued land before the CTA leaves
-          for (uint32_t q = idx > (uint32_t)SLOTS ? idx - SLOTS : 0u; q < idx; ++q) {
-            int dummy = 0;
-            tc_wait(&S.full[q % SLOTS], (q / SLOTS) & 1u, &dummy);
-          }
-        }
-      }
-    } else if (w == 9) {
-      // ---------------- MMA issuer (the whole warp): S(0) S(1) P.V(0) S(2) P.V(1) ... in steps
-      // of (page, tile), tile inner; S of a step lies in buffer step & 1, P over it
-      constexpr uint32_t ID1 = tc_idesc(128, 128, 0, 0);     // S = Q . K^T
-      constexpr uint32_t ID2 = tc_idesc(128, 128, 0, 1);     // O += P . V (V [key][d]: N-major)
-      const uint32_t kv0 = smem_addr(S.kv[0][0]), q0 = smem_addr(S.q[0][0]);
-      TtSeg back = seg;
-      int ahead = seg.j1 - seg.j0, behind = ahead;   // pages left of the segments of S and of P . V
-      uint32_t ga = 0, gc = 0, xa = 0, xc = 0;       // pages and tiles of the next S, the next P . V
-      uint32_t a = 0, c = 0, qn = 0;                 // steps issued; segments begun by S
-      bool ok = true, acc = false;
-      long long idle = 0;
-      while (ok) {
-        const uint32_t ki = 2u * ga, vi = 2u * gc + 1u;
-        unsigned long long* kfull = &S.full[ki % SLOTS];
-        // S comes first, up to two ahead; where its tiles are late, P . V does not wait for it
-        bool s_go = false, p_go = false;
-        if (more && a < c + 2u)
-          s_go = __all_sync(0xffffffffu, tc_test(kfull, (ki / SLOTS) & 1u) && tc_test(&S.qfull[xa], qn & 1u));
-        if (!s_go && c < a) {
-          unsigned long long* vfull = &S.full[vi % SLOTS];
-          if (more && a < c + 2u)
-            p_go = __all_sync(0xffffffffu, tc_test(vfull, (vi / SLOTS) & 1u) &&
-                                               tc_test(&S.pfull[c & 1u], (c >> 1) & 1u));
-          else
-            p_go = ok = tc_wait2_warp(vfull, (vi / SLOTS) & 1u, &S.pfull[c & 1u], (c >> 1) & 1u, &S.abort_);
-          if (!ok) break;
-        }
-        if (!s_go && !p_go) {
-          if (c == a && !more) break;
-          const long long now = clock64();
-          if (idle == 0) idle = now;
-          if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&S.abort_) || now - idle > TC_WAIT)) {
-            *reinterpret_cast<volatile int*>(&S.abort_) = 1;
-            break;
-          }
-          continue;
-        }
-        idle = 0;
-        tc_fence_after();
-        if (s_go) {
-          const uint32_t sl = ki % SLOTS, d = tm + 128u * (a & 1u);
-          const uint64_t dq = tc_desc(q0 + xa * 32768u, 16, 1024, 2);
-          const uint64_t dk = tc_desc(kv0 + sl * 32768u, 16, 1024, 2);
-#pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {           // 16 of 128 d: 32 B, the second box 16 KB on
-            const uint64_t o = (uint64_t)((ks & 3) * 2 + (ks >> 2) * 1024);
-            tc_mma_warp(d, dq + o, dk + o, ID1, ks > 0 ? 1 : 0);
-          }
-          tc_commit_warp(&S.sfull[a & 1u]);
-          if (ahead == 1) tc_commit_warp(&S.qempty[xa]);     // the segment's last S of the tile
-          ++a;
-          if (++xa == (uint32_t)NT) {
-            xa = 0;
-            tc_commit_warp(&S.empty[sl]);
-            ++ga;
-            if (--ahead == 0) {
-              more = tt_next(seg, S, P) && tt_real(seg, S, P);
-              ahead = seg.j1 - seg.j0;
-              ++qn;
-            }
-          }
-          continue;
-        }
-        const uint32_t sl = vi % SLOTS, pa = tm + 128u * (c & 1u);
-        const uint64_t dv = tc_desc(kv0 + sl * 32768u, 16384, 1024, 2);
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks)               // 16 keys: 2 KB; P of 64 keys every 64 columns
-          tc_mma_ts_warp(tm + 256u + 128u * xc, pa + 64u * (ks >> 2) + 8u * (ks & 3),
-                         dv + (uint64_t)(ks * 128), ID2, ks || acc ? 1 : 0);
-        tc_commit_warp(&S.oready[xc][gc & 1u]);
-        ++c;
-        if (++xc == (uint32_t)NT) {
-          xc = 0;
-          tc_commit_warp(&S.empty[sl]);
-          ++gc;
-          acc = true;
-          if (--behind == 0) {
-            if (!(tt_next(back, S, P) && tt_real(back, S, P))) break;
-            behind = back.j1 - back.j0;
-            acc = false;
-          }
-        }
-      }
-      // every MMA this warp issued has finished before the CTA leaves
-      tc_commit_warp(&S.fin);
-      int dummy = 0;
-      tc_wait(&S.fin, 0u, &dummy);
+      if (lane == 0) tt_load_kv(S, P, tmk, tmv, tmq, seg, more, share);
     } else if (w == 10) {
-      if (lane == 0) {
-        // ---------------- TMA producer of the later segments' Q, once a tile's last S is done
-        uint32_t sent = more ? NT : 0u;              // tiles asked for, tile inner
-        bool ok = true;
-        while (ok && more && tt_next(seg, S, P) && tt_real(seg, S, P)) {
-          for (int ti = 0; ti < NT; ++ti, ++sent) {
-            ok = tc_wait(&S.qempty[ti], (sent / NT - 1) & 1u, &S.abort_);
-            if (!ok) break;
-            ask_q(seg, ti);
-          }
-        }
-        if (!ok) {
-          // let the copies already issued land before the CTA leaves
-          for (uint32_t q = sent > (uint32_t)NT ? sent - NT : 0u; q < sent; ++q) {
-            int dummy = 0;
-            tc_wait(&S.qfull[q % NT], (q / NT) & 1u, &dummy);
-          }
-        }
-      }
+      if (lane == 0) tt_load_q(S, P, tmq, seg, more);
+    } else if constexpr (NT == 2) {
+      if (w == 9) tt_issue_pair(S, P, seg, more);
+      else if (w < 8) tt_softmax_pair(S, P, seg, more);
     } else {
-      // ---------------- softmax warps: the threads of warpgroups 0 and 1 with the same lane own
-      // the same query row of every tile; warpgroup x takes the keys [64 x, 64 x + 64) of a page
-      const int x = w >> 2, wq = w & 3, r = t & 127;
-      const uint32_t lcol = tm + ((uint32_t)(32 * wq) << 16);
-      const float sl2 = A.scale * 1.4426950408889634f;
-      unsigned char* stage = S.out[w];
-      // rows of tile ti of a segment's item
-      auto rows_of = [&](const TtSeg& g, int ti) {
-        return A.group * min(min(P.nt, P.ni - P.nt * ti), A.qlen - g.p * P.ni - P.nt * ti);
-      };
-      uint32_t k = 0, n = 0, xn = 0;                 // steps and pages done; exchanges with the peer
-      bool ok = true;
-      // A value to the thread with the row's other keys, and that thread's (a word of shared memory
-      // holds the value and the exchange's number; two of them by parity, as the peer may be one
-      // exchange ahead).  `ok` is false when a bounded wait gives up.
-      auto tell = [&](float v) {
-        ++xn;
-        *reinterpret_cast<volatile unsigned long long*>(&S.peer[xn & 1u][x][r]) =
-            ((unsigned long long)xn << 32) | __float_as_uint(v);
-      };
-      auto told = [&]() {
-        const volatile unsigned long long* from = &S.peer[xn & 1u][x ^ 1][r];
-        unsigned long long v = *from;
-        long long since = 0;
-        while ((uint32_t)(v >> 32) != xn) {
-          const long long now = clock64();
-          if (since == 0) since = now;
-          if (*reinterpret_cast<volatile int*>(&S.abort_) || now - since > TC_WAIT) {
-            *reinterpret_cast<volatile int*>(&S.abort_) = 1;
-            ok = false;
-            break;
-          }
-          v = *from;
-        }
-        ok = __all_sync(0xffffffffu, ok);
-        return __uint_as_float((uint32_t)v);
-      };
-      // P . V of page n - 1 is in O (that of page n - 2 may be under way, too: two barriers)
-      auto o_ready = [&](int ti) {
-        return tc_wait(&S.oready[ti][(n - 1) & 1u], ((n - 1) >> 1) & 1u, &S.abort_);
-      };
-      int seen_b = -1, seen_p = -1;                  // the segment that these are of:
-      uint32_t uni = 0;
-      bool settled = false;
-      uint32_t there = 0, dead = 0;                  // bit ti: the row's node is present; no row in the warp
-      while (more) {
-        const TtSeg cur = seg;
-        more = tt_next(seg, S, P) && tt_real(seg, S, P);
-        const int pages = cur.j1 - cur.j0, end = tree_end(T, cur.base);
-        const int32_t* mask0 = T.masks + (int64_t)cur.b * T.mask_bs + (int64_t)T.first * T.W;
-        // the rows' bits to shared memory (both warpgroups write the same), unless they are there:
-        // asked for now, used in the tree's pages
-        if (seen_p != cur.p || (seen_b != cur.b && (T.mask_bs != 0 || seen_b < 0))) {
-          if (!settled) asm volatile("cp.async.wait_all;" ::: "memory");   // an older copy first
-          dead = 0;
-#pragma unroll
-          for (int ti = 0; ti < NT; ++ti) {
-            const bool live = r < rows_of(cur, ti);
-            dead |= __all_sync(0xffffffffu, !live) ? 1u << ti : 0u;
-            const int32_t* m = mask0 + (int64_t)(cur.p * P.ni + P.nt * ti + r / A.group) * T.W;
-            for (int i = 0; i < T.W; ++i) {
-              if (live)
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
-                             :: "r"(smem_addr(&S.mask[ti][r][i])), "l"(m + i) : "memory");
-              else
-                S.mask[ti][r][i] = 0u;
-            }
-          }
-          settled = false;
-          seen_b = cur.b;
-          seen_p = cur.p;
-        }
-        auto settle = [&]() {
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          there = 0;
-#pragma unroll
-          for (int ti = 0; ti < NT; ++ti) {
-            uint32_t some = 0;
-            for (int i = 0; i < T.W; ++i) some |= S.mask[ti][r][i] & tree_valid(T.N, i);
-            there |= some != 0u ? 1u << ti : 0u;
-          }
-          // lane i: word i of what any query of the row sees
-          uni = 0u;
-          for (int i = 0; i < T.W; ++i) {
-            uint32_t word = 0;
-#pragma unroll 4
-            for (int q = lane; q < A.qlen; q += 32) word |= tree_word(mask0 + (int64_t)q * T.W, T.W, T.N, i);
-            word = __reduce_or_sync(0xffffffffu, word);
-            if (lane == i) uni = word;
-          }
-          settled = true;
-        };
-        // of the tile in turn, and of the other one
-        float m = -CUDART_INF_F, l = 0.f, m2 = -CUDART_INF_F, l2 = 0.f;
-        bool wild = false, wild2 = false;
-#pragma unroll 1
-        for (int i = 0; i < pages && ok; ++i, ++n) {
-#pragma unroll 1
-          for (int ti = 0; ti < NT; ++ti, ++k) {
-            ok = __all_sync(0xffffffffu, tc_wait(&S.sfull[k & 1u], (k >> 1) & 1u, &S.abort_));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t scol = lcol + 128u * (k & 1u) + 64u * x;
-            const int key0 = (cur.j0 + i) * SD_KV_PAGE;
-            const bool idle = (dead >> ti) & 1u;
-            if (key0 + SD_KV_PAGE > cur.base) {
-              // the tree's pages, and what lies behind it
-              if (!settled) settle();
-              if (!idle) tt_hide(S.mask[ti][r], T, cur.base, end, key0 + 64 * x, 64, scol);
-              if (ti == 0) {
-                // each warpgroup its half of the keys, two warps 32 of them
-                const uint32_t vi = 2u * n + 1u;
-                const int grp = 2 * x + (wq & 1);
-                ok = tt_blank(S.kv[vi % SLOTS], T, uni, cur.base, end, key0 + 32 * grp, 32 * grp,
-                              wq >> 1, (wq >> 1) + 1, &S.full[vi % SLOTS], (vi / SLOTS) & 1u,
-                              &S.abort_);
-                if (!ok) break;
-              }
-            }
-            if (!idle) {
-              uint32_t s0[32], s1[32], pk[32];
-              unsigned long long ls[2];
-              auto largest = [&]() {
-                float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                  px_max3(mx[e & 2], s0[e], s0[e + 1]);
-                  px_max3(mx[(e & 2) + 1], s1[e], s1[e + 1]);
-                }
-                return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-              };
-              if (i == 0) {                            // a reference for the segment
-                TC_LD32(s0, scol);
-                TC_LD32(s1, scol + 32u);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                const float mine = largest();
-                tell(mine);
-                m = fmaxf(mine, told());
-                if (!ok) break;
-                wild = px_wild(m);
-              }
-              // weights under the reference as it is, and the largest score beside them: where
-              // that is too far above it (rare), the reference moves and the weights are made again
-              while (true) {
-                TC_LD32(s0, scol);
-                TC_LD32(s1, scol + 32u);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                const float mine = largest();
-                if (wild) {
-                  px_scale(s0, sl2);
-                  px_scale(s1, sl2);
-                }
-                const float mc = m == -CUDART_INF_F ? 0.f : m, sf = wild ? 1.f : sl2;
-                const unsigned long long sl22 = pair2(sf, sf), nm2 = pair2(-mc, -mc);
-                ls[0] = ls[1] = 0ULL;                  // (0.f, 0.f)
-                tell(mine);
-                tt_weights(s0, pk, ls, sl22, nm2);
-                tt_weights(s1, pk + 16, ls, sl22, nm2);
-                const float mt = fmaxf(mine, told());
-                if (!ok) break;
-                const bool move = mt > m + PX_HEADROOM;
-                if (!__any_sync(0xffffffffu, move)) break;
-                const float mn = move ? mt : m;
-                const float alpha = move ? (m == -CUDART_INF_F ? 0.f : ex2f(m - mn)) : 1.f;
-                m = mn;
-                l *= alpha;
-                wild = px_wild(m);
-                if (i > 0) {
-                  // O holds this segment's earlier pages: the last P . V into it first; each
-                  // warpgroup half of the columns
-                  ok = __all_sync(0xffffffffu, o_ready(ti));
-                  if (!ok) break;
-                  tc_fence_after();
-#pragma unroll 1
-                  for (int q = 0; q < 4; ++q) {
-                    const uint32_t oc = lcol + 256u + 128u * ti + 64u * x + 16u * q;
-                    uint32_t o[16];
-                    TC_LD16(o, oc);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                    TC_ST16(oc, o);
-                  }
-                }
-              }
-              if (!ok) break;
-              TC_ST32(scol, pk);                       // over columns that have been read
-              asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-              float la, lb;
-              unpair(add2(ls[0], ls[1]), la, lb);
-              l += la + lb;
-            }
-            tc_fence_before();
-            tt_arrive(&S.pfull[k & 1u]);
-            if constexpr (NT == 2) {                   // the other tile's turn
-              const float tm0 = m, tl0 = l;
-              const bool tw0 = wild;
-              m = m2; l = l2; wild = wild2;
-              m2 = tm0; l2 = tl0; wild2 = tw0;
-            }
-          }
-        }
-        if (!ok) break;
-        // ---- the segment's end: O divided by the row's sum and written out, or as a piece; each
-        // warpgroup half of the columns
-        const bool whole = cur.j0 == 0 && cur.j1 + TT_OVH == cur.tb;
-        const int slot = 2 * cta + (cur.j0 == 0);
-#pragma unroll 1
-        for (int ti = 0; ti < NT; ++ti) {
-          if (!((dead >> ti) & 1u)) {
-            tell(l);
-            const float lp = told();
-            ok = ok && __all_sync(0xffffffffu, o_ready(ti));
-            if (!ok) break;
-            tc_fence_after();
-            l = x ? lp + l : l + lp;                 // (the first warpgroup's half first, in both)
-            const int pr = P.nt * A.group * ti + r;
-            const bool live = r < rows_of(cur, ti);
-            const float il = !whole ? 1.f : l == 0.f || !((there >> ti) & 1u) ? 0.f : 1.f / l;
-            const int jt = r / A.group, j = cur.p * P.ni + P.nt * ti + jt;
-            const int hq = cur.h * A.group + r - jt * A.group;
-            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(A.out) + cur.b * A.obs + j * A.oqs +
-                                 hq * A.ohs;
-            float4* part = P.pacc + (int64_t)slot * (TT_D / 4) * P.rs + pr;
-#pragma unroll 1
-            for (int q = 2 * x; q < 2 * x + 2; ++q) {
-              uint32_t u[32];
-              TC_LD32(u, lcol + 256u + 128u * ti + 32u * q);
-              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-              float o[32];
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = il == 0.f ? 0.f : il * __uint_as_float(u[e]);
-              if (whole) {
-                tt_write(stage, o, out + 32 * q, live, P.out_vec != 0);
-              } else if (live) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  part[(int64_t)(8 * q + e) * P.rs] =
-                      make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-              }
-              __syncwarp();
-            }
-            if (!whole && live && x == 0) P.pml[(int64_t)slot * P.rs + pr] = make_float2(m, l);
-          }
-          m = m2;
-          l = l2;
-        }
-        if (!ok) break;
-        tc_fence_before();
-      }
+      if (w == 9) tt_issue_one(S, P, seg, more);
+      else if (w < 8) tt_softmax_one(S, P, seg, more);
     }
   }
+  if ((int64_t)cta * share >= total && t == 0) P.cut[cta] = make_int4(0, 0, 0, 0);
   tc_fence_before();
   __syncthreads();                                   // every role is done
   if (t == 0) P.status[cta] = S.abort_;
   if (w == 9) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
-                 :: "r"(tm), "r"(512u) : "memory");
+                 :: "r"(S.tmem), "r"(512u) : "memory");
   }
 }
 
-// CTA (boundary c, rows): where CTA c's run ends inside an item that it is the first to
-// work on, the item's pieces are merged, in order; a lane takes a query row, a warp
-// 16 columns.
+// CTA (c, rows): the item that the run of CTA c of the main kernel cuts, if any: its pieces are
+// merged, in order; a lane takes a query row, a warp 16 columns.
 __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_constant__ TreeTcParams P) {
   const TreeParams& T = P.T;
   const AttnParams& A = T.A;
@@ -796,7 +946,7 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
   const int c = (int)blockIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int stop = t < TT_CTAS ? P.status[t] : 0;
-  const int per = A.Hkv * P.np, total = P.rowpre[A.B] * per, share = tt_share(total);
+  const int4 cut = P.cut[c];
   if (__syncthreads_or(stop)) {
     // a wait gave up somewhere: say so in the output
     const int64_t n = (int64_t)A.B * A.qlen * A.Hq * TT_D, nt = (int64_t)gridDim.x * gridDim.y * TJ_THREADS;
@@ -808,21 +958,13 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
     }
     return;
   }
-  const int64_t U = (int64_t)(c + 1) * share;
-  if (U >= total) return;
-  int lo = 0, hi = A.B;                              // the last row that starts at or before U
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if ((int64_t)P.rowpre[mid] * per <= U) lo = mid + 1; else hi = mid;
-  }
-  const int b = lo - 1, u0 = P.rowpre[b] * per, tb = P.rowpre[b + 1] - P.rowpre[b];
-  const int it = ((int)U - u0) / tb, h = it / P.np, p = it % P.np;
-  const int start = u0 + it * tb + TT_OVH;           // the unit of the item's first page
-  const int c0 = start / share, c1 = (u0 + it * tb + tb - 1) / share;
-  if (c0 != c || c1 == c) return;
-  const int rows = A.group * min(P.ni, A.qlen - p * P.ni), np = c1 - c0 + 1;
+  const int b = cut.x, h = cut.y, p = cut.z, np = cut.w;
+  if (np == 0) return;
+  const int rows = A.group * min(P.ni, A.qlen - p * P.ni);
   const int r = (int)blockIdx.y * TJ_ROWS + lane;
   if (r >= rows) return;
+  const int ji = r / A.group, j = p * P.ni + ji, hq = h * A.group + r - ji * A.group;
+  const bool there = tree_present(T.masks + (int64_t)b * T.mask_bs + (int64_t)(T.first + j) * T.W, T.W, T.N);
   // piece i: the item's start in its first CTA, then a CTA's start each
   auto slot_of = [&](int i) { return (int64_t)(2 * (c + i) + (i == 0)); };
   float gm = -CUDART_INF_F;
@@ -849,9 +991,7 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
       }
     }
   }
-  const int ji = r / A.group, j = p * P.ni + ji, hq = h * A.group + r - ji * A.group;
-  const int32_t* mask = T.masks + (int64_t)b * T.mask_bs + (int64_t)(T.first + j) * T.W;
-  const bool none = L == 0.f || !tree_present(mask, T.W, T.N);
+  const bool none = L == 0.f || !there;
   const float il = none ? 0.f : 1.f / L;
   __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(A.out) + b * A.obs + j * A.oqs + hq * A.ohs + 16 * w;
 #pragma unroll
@@ -882,7 +1022,7 @@ struct TtLayout {
   size_t status, acc, ml, bytes;
   int np, ni, nt, rs;
 };
-static TtLayout tt_layout(int qlen, int group, int B) {
+static TtLayout tt_layout(int qlen, int group) {
   TtLayout L;
   // items of up to two tiles of whole nodes, of about the same size, and so their tiles
   const int most = TT_TILE / group;
@@ -891,7 +1031,7 @@ static TtLayout tt_layout(int qlen, int group, int B) {
   L.nt = qlen <= most ? qlen : (L.ni + 1) / 2;
   L.rs = (L.ni * group + 31) / 32 * 32;
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  size_t o = up(((size_t)B + 1) * sizeof(int));
+  size_t o = up(TT_CTAS * sizeof(int4));
   L.status = o; o = up(o + TT_CTAS * sizeof(int));
   L.acc = o; o = up(o + (size_t)2 * TT_CTAS * L.rs * TT_D * sizeof(float));
   L.ml = o; o = up(o + (size_t)2 * TT_CTAS * L.rs * 2 * sizeof(float));
@@ -926,7 +1066,7 @@ static int tree_tc(TreeTcParams& P, void* workspace, size_t workspace_bytes, cud
   if ((A.B > 1 && A.qbs <= 0) || (A.Hq > 1 && A.qhs <= 0) || (A.qlen > 1 && A.qqs <= 0)) return SD_EINVAL;
   const int64_t rows = A.bt ? (int64_t)A.npages * A.Hkv * SD_KV_PAGE : (int64_t)A.B * A.Hkv * A.C;
   if (rows >= (int64_t)1 << 31) return SD_ENOTSUP;   // a TMA coordinate
-  const TtLayout L = tt_layout(A.qlen, A.group, A.B);
+  const TtLayout L = tt_layout(A.qlen, A.group);
   // the schedule counts units in 32 bits
   const int64_t tiles = ((int64_t)A.C + SD_KV_PAGE - 1) / SD_KV_PAGE + TT_OVH;
   if (tiles * A.B > 0x7FFFFFFF / ((int64_t)A.Hkv * L.np)) return SD_ENOTSUP;
@@ -934,7 +1074,7 @@ static int tree_tc(TreeTcParams& P, void* workspace, size_t workspace_bytes, cud
     return SD_ENOSPC;
   char* ws = reinterpret_cast<char*>(workspace);
   P.np = L.np; P.ni = L.ni; P.nt = L.nt; P.rs = L.rs;
-  P.rowpre = reinterpret_cast<int*>(ws);
+  P.cut = reinterpret_cast<int4*>(ws);
   P.status = reinterpret_cast<int*>(ws + L.status);
   P.pacc = reinterpret_cast<float4*>(ws + L.acc);
   P.pml = reinterpret_cast<float2*>(ws + L.ml);
@@ -954,7 +1094,7 @@ static int tree_tc(TreeTcParams& P, void* workspace, size_t workspace_bytes, cud
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.stream = st;
-  cfg.gridDim = dim3(TT_CTAS - 1, (unsigned)((L.rs + TJ_ROWS - 1) / TJ_ROWS));
+  cfg.gridDim = dim3(TT_CTAS, (unsigned)((L.rs + TJ_ROWS - 1) / TJ_ROWS));
   cfg.blockDim = dim3(TJ_THREADS);
   if (cudaLaunchKernelEx(&cfg, tree_join_kernel, P) != cudaSuccess) return SD_ELAUNCH;
   return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
@@ -969,7 +1109,7 @@ extern "C" {
 size_t sd_tree_attn_workspace_bytes(int B, int Hq, int Hkv, int D, int C, int qlen, int dtype) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || C <= 0 || qlen <= 0) return 0;
   if (!tt_fast(dtype, D, Hq / Hkv) || (int64_t)qlen * (Hq / Hkv) > 0x7FFFFFFF) return 0;
-  return tt_layout(qlen, Hq / Hkv, B).bytes;
+  return tt_layout(qlen, Hq / Hkv).bytes;
 }
 
 int sd_tree_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const void* kcache,
