@@ -5,14 +5,20 @@
 //   x = logit;  seen (in the prompt, written, or on the node's path):
 //   x = x > 0 ? x / r : x r;  x -= f c;  x -= p [c > 0];  x += bias;  x = -inf where not allowed
 //
-// One pass: what it has to move is a logit in and out (and, per row, 16 bits of
-// history per token; per position, one bit of mask), so HBM bounds it.  A CTA
-// takes a chunk of one position's vocabulary.  Nearly every 16-byte unit of the
-// history is zero (a row has written some thousand of 151936 tokens), so a unit is
-// tested whole.  A unit that the mask bans whole is written without being read.
-// What is sparse (the tokens of the path, the biases) is not looked up element by
-// element: the CTA computes those of its chunk first, from the logits as they
-// came, and writes them over what the pass left, so out may be the logits.
+// What it has to move is a logit in and out (and, per row, 16 bits of history per
+// token; per position, one bit of mask), so HBM bounds it.  A CTA takes a chunk of
+// a row's vocabulary for up to LG_POS positions and passes over it once: 16-byte units
+// of the input, wherever they start in the row (rows of an odd vocabulary are aligned
+// differently), with -inf for what the mask bans; a unit that it bans whole is written
+// without being read.  What is sparse is then written over what the pass left: the
+// tokens that have a history (some thousand of 151936: the CTA reads the row's history
+// once and lists them), then those of the position's path and the biases, which, where
+// out is the logits themselves, have been computed before the pass.
+// 320 positions of 151936 bf16 logits, 64 rows of history, masks, biases (220 MB): 47.4 us,
+// 832 positions (531 MB): 110 us.  Copy and mask alone take 35 and 79 (98 % of the copy
+// rate), the list 5 and 7, the tokens on it the rest: two memory sectors each.  Looking
+// every unit up in the history during the pass took 59.8 and 127.5 (the history is then
+// read from L2 once per position), a position's chunk by way of shared memory 89 and 202.
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
@@ -24,8 +30,11 @@
 namespace sd {
 
 constexpr int LG_THREADS = 256;
-constexpr int LG_UNITS = 8;                  // most 16-byte units per thread
+constexpr int LG_UNITS = 4;                  // most 16-byte units per thread and position
 constexpr int LG_AHEAD = 4;                  // units whose loads are on their way at once
+constexpr int LG_POS = 8;                    // most positions of a CTA
+constexpr int LG_CTAS = 4 * 148;             // enough CTAs: four per SM
+constexpr int LG_CHUNK = LG_UNITS * LG_THREADS * 8;          // most tokens of a chunk: 32 a thread
 
 struct LogitsParams {
   const void* logits; int64_t bs, ps;
@@ -39,6 +48,7 @@ struct LogitsParams {
   const int32_t* allowed; int64_t allowed_bs, allowed_ps;
   void* out; int64_t out_bs, out_ps;
   int chunk, chunks;                         // elements of a CTA's chunk, chunks of a position
+  int lg, groups;                            // positions of a CTA, CTAs along the positions
 };
 
 template <int DT> struct LgType;
@@ -51,6 +61,23 @@ __device__ __forceinline__ float lg_in(__nv_bfloat16 x) { return __bfloat162floa
 __device__ __forceinline__ void lg_out(float* p, float x) { *p = x; }
 __device__ __forceinline__ void lg_out(__half* p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void lg_out(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+
+// A unit with -inf for the elements whose bit of `on` is 0: 16-bit ones by a byte permutation of
+// a word and a pair of -inf, whose selector is 0x3210 where both stay and 0x7654 where none does.
+template <int DT>
+__device__ __forceinline__ uint4 lg_ban(uint4 v, uint32_t on) {
+  if constexpr (DT == SD_DTYPE_F32) {
+    const uint32_t none = 0xFF800000u;
+    return make_uint4(on & 1u ? v.x : none, on & 2u ? v.y : none, on & 4u ? v.z : none, on & 8u ? v.w : none);
+  } else {
+    const uint32_t none = DT == SD_DTYPE_BF16 ? 0xFF80FF80u : 0xFC00FC00u;
+    auto pick = [&](uint32_t word, uint32_t two) {
+      return __byte_perm(word, none, 0x7654u - 0x44u * ((two | two << 7) & 0x101u));
+    };
+    return make_uint4(pick(v.x, on & 3u), pick(v.y, (on >> 2) & 3u), pick(v.z, (on >> 4) & 3u),
+                      pick(v.w, (on >> 6) & 3u));
+  }
+}
 
 struct LgPenalty {
   float r, p, f;
@@ -65,152 +92,224 @@ struct LgPenalty {
   }
 };
 
-template <int DT>
-__global__ void __launch_bounds__(LG_THREADS) process_logits_kernel(const __grid_constant__ LogitsParams P) {
+// Eight bits from bit `at` on of a bit string whose last word is `last`.
+__device__ __forceinline__ uint32_t lg_bits(const uint32_t* p, int at, int last) {
+  const int w = at >> 5;
+  return __funnelshift_r(p[w], p[min(w + 1, last)], at & 31);
+}
+
+// What a CTA knows of a position: its node's path and how its tokens become logits.
+struct LgPosition {
+  const int32_t* mask;                               // the node's ancestor bits; null: a chain
+  int node;
+};
+__device__ __forceinline__ bool lg_on_path(const LogitsParams& P, const LgPosition& q, int i) {
+  return q.mask ? (tree_word(q.mask, P.W, P.N, i >> 5) >> (i & 31)) & 1u : i <= q.node;
+}
+// Entry id of a position, in full: its history, its path, its biases, its mask.
+template <typename T>
+__device__ __forceinline__ float lg_entry(const LogitsParams& P, const LgPosition& q, const LgPenalty& pen,
+                                       const T* x, const int16_t* hist, const uint32_t* allow, int b,
+                                       int id) {
+  float z = lg_in(x[id]);
+  if (hist) {
+    int c = 0;
+    for (int i = 0; i < P.N; ++i)
+      c += P.tokens[b * P.tokens_bs + i] == id && lg_on_path(P, q, i);
+    z = pen(z, hist[id], c);
+  }
+  float bias = 0.f;                                  // (in the list's order: the same sum every time)
+  for (int k = 0; k < P.M; ++k)
+    if (P.bias_ids[b * P.bias_bs + k] == id) bias += P.bias_values[b * P.bias_bs + k];
+  z += bias;
+  return !allow || ((allow[id >> 5] >> (id & 31)) & 1u) ? z : -CUDART_INF_F;
+}
+
+// INPLACE: out is the logits (one position per CTA; what is sparse is computed before the pass)
+template <int DT, bool INPLACE>
+__global__ void __launch_bounds__(LG_THREADS, 5) process_logits_kernel(const __grid_constant__ LogitsParams P) {
   using T = typename LgType<DT>::T;
   constexpr int E = 16 / sizeof(T);                  // elements of a unit
-  // the path's tokens, the biases, and the entries of this chunk that they touch
-  __shared__ int path_tok[SD_TREE_MAX], bias_id[SD_BIAS_MAX];
-  __shared__ float bias_val[SD_BIAS_MAX];
-  __shared__ int at[SD_TREE_MAX + SD_BIAS_MAX];
-  __shared__ float val[SD_TREE_MAX + SD_BIAS_MAX];
-  __shared__ int n_path, n_at;
+  constexpr uint32_t ALL = (1u << E) - 1u;
+  constexpr int SPARSE = INPLACE ? SD_TREE_MAX + SD_BIAS_MAX : 1;
+  // the chunk's tokens that have a history: place in the chunk, history above
+  __shared__ uint32_t seen[LG_CHUNK];
+  __shared__ int red[33];
+  __shared__ int at[SPARSE];
+  __shared__ float val[SPARSE];
+  __shared__ int n_at;
   const int t = threadIdx.x;
-  const int chunk = (int)(blockIdx.x % P.chunks);
-  const int64_t pos = blockIdx.x / P.chunks;
-  const int b = (int)(pos / P.L), l = (int)(pos - (int64_t)b * P.L);
+  const int chunk = (int)(blockIdx.x % P.chunks), bg = (int)(blockIdx.x / P.chunks);
+  const int b = bg / P.groups, l0 = (bg - b * P.groups) * P.lg, nl = min(P.lg, P.L - l0);
   const int c0 = chunk * P.chunk, c1 = min(P.V, c0 + P.chunk);
-  const T* x = reinterpret_cast<const T*>(P.logits) + b * P.bs + l * P.ps;
-  T* y = reinterpret_cast<T*>(P.out) + b * P.out_bs + l * P.out_ps;
   const int16_t* hist = P.history ? P.history + b * P.history_bs : nullptr;
-  const uint32_t* allow = P.allowed ? reinterpret_cast<const uint32_t*>(P.allowed) +
-                                          b * P.allowed_bs + l * P.allowed_ps : nullptr;
   LgPenalty pen = {1.f, 0.f, 0.f};
   if (hist) {
     if (P.repetition) pen.r = P.repetition[b];
     if (P.presence) pen.p = P.presence[b];
     if (P.frequency) pen.f = P.frequency[b];
   }
-  const bool sparse = (hist && P.N > 0) || P.M > 0;
-  if (sparse) {
-    if (t == 0) n_path = n_at = 0;
-    __syncthreads();
+  auto logits = [&](int l) { return reinterpret_cast<const T*>(P.logits) + b * P.bs + (int64_t)l * P.ps; };
+  auto output = [&](int l) { return reinterpret_cast<T*>(P.out) + b * P.out_bs + (int64_t)l * P.out_ps; };
+  auto mask = [&](int l) {
+    return P.allowed ? reinterpret_cast<const uint32_t*>(P.allowed) + b * P.allowed_bs +
+                           (int64_t)l * P.allowed_ps : nullptr;
+  };
+  auto position = [&](int l) {
     const int node = P.first + l;
-    if (hist) {
-      const int32_t* m = P.masks ? P.masks + b * P.mask_bs + (int64_t)node * P.W : nullptr;
-      for (int i = t; i < P.N; i += LG_THREADS) {
-        const bool on = m ? (tree_word(m, P.W, P.N, i >> 5) >> (i & 31)) & 1u : i <= node;
-        if (!on) continue;
-        const int64_t id = P.tokens[b * P.tokens_bs + i];
-        if (id >= 0 && id < P.V) path_tok[atomicAdd(&n_path, 1)] = (int)id;
+    return LgPosition{P.masks ? P.masks + b * P.mask_bs + (int64_t)node * P.W : nullptr, node};
+  };
+  int n_seen = 0;
+  if (hist) {
+    // 32 tokens a thread
+    const int e = c0 + 32 * t, n = 32 * t < P.chunk ? min(32, c1 - e) : 0;
+    uint32_t h[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) h[k] = 0u;
+    if ((reinterpret_cast<uintptr_t>(hist) & 15) == 0 && n == 32) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(hist + e) + k);
+        h[4 * k] = v.x; h[4 * k + 1] = v.y; h[4 * k + 2] = v.z; h[4 * k + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 32; ++k)
+        if (k < n) h[k >> 1] |= (uint32_t)(unsigned short)hist[e + k] << (16 * (k & 1));
+    }
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) mine += ((h[k] & 0xFFFFu) != 0u) + (h[k] >> 16 != 0u);
+    int to = block_excl_scan<int>(mine, red, &n_seen);
+    if (mine) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const uint32_t v = (h[k >> 1] >> (16 * (k & 1))) & 0xFFFFu;
+        if (v) seen[to++] = v << 16 | (uint32_t)(32 * t + k);
       }
     }
-    for (int i = t; i < P.M; i += LG_THREADS) {
-      const int64_t id = P.bias_ids[b * P.bias_bs + i];
-      bias_id[i] = id >= 0 && id < P.V ? (int)id : -1;
-      bias_val[i] = P.bias_values[b * P.bias_bs + i];
+  }
+  if (INPLACE && t == 0) n_at = 0;
+  __syncthreads();
+  // the entries that a position's path or the biases touch
+  const int np = hist ? P.N : 0;
+  auto sparse_id = [&](const LgPosition& q, int i) -> int {
+    int64_t id = -1;
+    if (i < np) {
+      if (lg_on_path(P, q, i)) id = P.tokens[b * P.tokens_bs + i];
+    } else {
+      id = P.bias_ids[b * P.bias_bs + i - np];
     }
-    __syncthreads();
-    const int np = n_path;
+    return id >= c0 && id < c1 ? (int)id : -1;
+  };
+  if (INPLACE) {
+    const LgPosition q = position(l0);
     for (int i = t; i < np + P.M; i += LG_THREADS) {
-      const int id = i < np ? path_tok[i] : bias_id[i - np];
-      if (id < c0 || id >= c1) continue;
-      int c = 0;
-      for (int k = 0; k < np; ++k) c += path_tok[k] == id;
-      float z = lg_in(x[id]);
-      if (hist) z = pen(z, hist[id], c);
-      float bias = 0.f;
-      for (int k = 0; k < P.M; ++k)
-        if (bias_id[k] == id) bias += bias_val[k];   // (in the list's order: the same sum every time)
-      z += bias;
-      if (allow && !((allow[id >> 5] >> (id & 31)) & 1u)) z = -CUDART_INF_F;
+      const int id = sparse_id(q, i);
+      if (id < 0) continue;
       const int k = atomicAdd(&n_at, 1);
       at[k] = id;
-      val[k] = z;                                    // (an id that is there twice: the same value)
+      val[k] = lg_entry(P, q, pen, logits(l0), hist, mask(l0), b, id);   // (twice: the same value)
     }
     __syncthreads();
   }
-  // units of 16 bytes where everything is aligned to them, else element by element
-  const bool wide = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0 &&
-                    (!hist || (reinterpret_cast<uintptr_t>(hist) & (2 * E - 1)) == 0);
-  int e0 = c0;                                       // what the units leave
-  if (wide) {
-    const int nu = (c1 - c0) / E;
+  // ---- the pass, position by position: 16-byte units of the input, wherever they start in the row
+  const int words = (P.V + 31) / 32 - 1;
+#pragma unroll 1
+  for (int l = l0; l < l0 + nl; ++l) {
+    const T* x = logits(l) + c0;
+    T* y = output(l) + c0;
+    const int head = (int)((16u - (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15)) & 15u) / (int)sizeof(T);
+    const int nu = c0 + head <= c1 ? (c1 - c0 - head) / E : 0;
+    const uint32_t* allow = mask(l);
+    x += head;
+    y += head;
+    const bool wide = (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+#pragma unroll 1
     for (int u0 = t; u0 < nu; u0 += LG_THREADS * LG_AHEAD) {
-      uint32_t on[LG_AHEAD];
       uint4 v[LG_AHEAD];
-      uint4 h[LG_AHEAD];
+      uint32_t on[LG_AHEAD];
 #pragma unroll
       for (int k = 0; k < LG_AHEAD; ++k) {
-        const int u = u0 + k * LG_THREADS, e = c0 + u * E;
-        on[k] = u < nu ? (1u << E) - 1u : 0u;
-        if (allow && u < nu) on[k] &= __ldg(allow + (e >> 5)) >> (e & 31);
+        const int u = u0 + k * LG_THREADS;
+        on[k] = u < nu ? ALL : 0u;
+        if (allow && u < nu) on[k] = lg_bits(allow, c0 + head + u * E, words) & ALL;
       }
 #pragma unroll
       for (int k = 0; k < LG_AHEAD; ++k) {
-        const int64_t e = c0 + (int64_t)(u0 + k * LG_THREADS) * E;
-        v[k] = h[k] = make_uint4(0u, 0u, 0u, 0u);
-        if (on[k]) {
-          v[k] = __ldcs(reinterpret_cast<const uint4*>(x + e));
-          if (hist) {
-            if constexpr (E == 8) {
-              h[k] = __ldg(reinterpret_cast<const uint4*>(hist + e));
-            } else {
-              const uint2 z = __ldg(reinterpret_cast<const uint2*>(hist + e));
-              h[k].x = z.x;
-              h[k].y = z.y;
-            }
-          }
-        }
+        v[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (on[k]) v[k] = (reinterpret_cast<const uint4*>(x))[u0 + k * LG_THREADS];
       }
 #pragma unroll
       for (int k = 0; k < LG_AHEAD; ++k) {
         const int u = u0 + k * LG_THREADS;
         if (u >= nu) continue;
-        T* xe = reinterpret_cast<T*>(&v[k]);
-        if ((h[k].x | h[k].y | h[k].z | h[k].w) != 0u) {
-          const int16_t* he = reinterpret_cast<const int16_t*>(&h[k]);
+        if (on[k] != ALL) v[k] = lg_ban<DT>(v[k], on[k]);
+        if (wide) {
+          reinterpret_cast<uint4*>(y)[u] = v[k];
+        } else {
+          const uint32_t word[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (he[e] != 0) lg_out(&xe[e], pen(lg_in(xe[e]), he[e], 0));
+          for (int j = 0; j < E; ++j) {
+            if constexpr (E == 4) reinterpret_cast<uint32_t*>(y)[u * E + j] = word[j];
+            else reinterpret_cast<unsigned short*>(y)[u * E + j] = (unsigned short)(word[j / 2] >> (16 * (j & 1)));
+          }
         }
-        if (on[k] != (1u << E) - 1u) {
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (!((on[k] >> e) & 1u)) lg_out(&xe[e], -CUDART_INF_F);
-        }
-        __stcs(reinterpret_cast<uint4*>(y + c0 + (int64_t)u * E), v[k]);
       }
     }
-    e0 = c0 + nu * E;
   }
-  for (int i0 = e0 + t; i0 < c1; i0 += LG_THREADS * LG_UNITS) {
-    T v[LG_UNITS];
-    int h[LG_UNITS];
-    uint32_t on[LG_UNITS];
-#pragma unroll
-    for (int k = 0; k < LG_UNITS; ++k) {
-      const int i = i0 + k * LG_THREADS;
-      on[k] = 0u;
-      h[k] = 0;
-      if (i < c1) {
-        v[k] = x[i];
-        if (hist) h[k] = hist[i];
-        on[k] = allow ? (__ldg(allow + (i >> 5)) >> (i & 31)) & 1u : 1u;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < LG_UNITS; ++k) {
-      const int i = i0 + k * LG_THREADS;
-      if (i >= c1) continue;
-      if (!on[k]) lg_out(&y[i], -CUDART_INF_F);
-      else if (h[k] != 0) lg_out(&y[i], pen(lg_in(v[k]), h[k], 0));
-      else y[i] = v[k];
-    }
+  // the elements before the first and behind the last unit, at most 2 E - 2 of a position
+  for (int i = t; i < nl * 2 * E; i += LG_THREADS) {
+    const int l = l0 + i / (2 * E), k = i % (2 * E);
+    const T* x = logits(l);
+    const int head = (int)((16u - (uint32_t)(reinterpret_cast<uintptr_t>(x + c0) & 15)) & 15u) / (int)sizeof(T);
+    const int body = c0 + head <= c1 ? (c1 - c0 - head) / E * E : 0;
+    int e;
+    if (k < E) e = k < head ? c0 + k : -1;
+    else e = c0 + head + body + k - E;
+    if (e < 0 || e >= c1) continue;
+    const uint32_t* allow = mask(l);
+    T* y = output(l) + e;
+    if (allow && !((allow[e >> 5] >> (e & 31)) & 1u)) lg_out(y, -CUDART_INF_F);
+    else *y = x[e];
   }
-  if (sparse) {
+  if (n_seen > 0) {
+    // the tokens that have a history, over what the pass left
     __syncthreads();
-    for (int k = t; k < n_at; k += LG_THREADS) lg_out(&y[at[k]], val[k]);
+    const int pairs = n_seen * nl;                   // (token, position)
+    for (int i0 = t; i0 < pairs; i0 += LG_THREADS * LG_AHEAD) {
+      T z[LG_AHEAD];
+      T* y[LG_AHEAD];
+      uint32_t on[LG_AHEAD], what[LG_AHEAD];
+#pragma unroll
+      for (int k = 0; k < LG_AHEAD; ++k) {
+        const int i = i0 + k * LG_THREADS, p = i / n_seen, l = l0 + p;
+        on[k] = i < pairs;
+        what[k] = on[k] ? seen[i - p * n_seen] : 0u;
+        const int e = c0 + (int)(what[k] & 0xFFFFu);
+        if (on[k]) {
+          const uint32_t* allow = mask(l);
+          if (allow) on[k] = (__ldg(allow + (e >> 5)) >> (e & 31)) & 1u;
+          y[k] = output(l) + e;
+          z[k] = logits(l)[e];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < LG_AHEAD; ++k)
+        if (on[k]) lg_out(y[k], pen(lg_in(z[k]), (int)what[k] >> 16, 0));
+    }
+  }
+  if (np + P.M == 0) return;
+  __syncthreads();
+  if (INPLACE) {
+    for (int k = t; k < n_at; k += LG_THREADS) lg_out(&output(l0)[at[k]], val[k]);
+  } else {
+    for (int i = t; i < nl * (np + P.M); i += LG_THREADS) {
+      const int l = l0 + i / (np + P.M);
+      const LgPosition q = position(l);
+      const int id = sparse_id(q, i % (np + P.M));
+      if (id >= 0) lg_out(&output(l)[id], lg_entry(P, q, pen, logits(l), hist, mask(l), b, id));
+    }
   }
 }
 
@@ -270,23 +369,42 @@ int sd_process_logits(const void* logits, int64_t bs, int64_t ps, int dtype, int
   P.bias_ids = bias_ids; P.bias_values = bias_values; P.bias_bs = bias_bs; P.M = M;
   P.allowed = allowed; P.allowed_bs = allowed_bs; P.allowed_ps = allowed_ps;
   P.out = out; P.out_bs = out_bs; P.out_ps = out_ps;
-  const int E = dtype == SD_DTYPE_F32 ? 4 : 8;
-  // a chunk is 8 units per thread, less where that would leave SMs without a CTA
+  const int E = dtype == SD_DTYPE_F32 ? 4 : 8, size = 16 / E;
+  // the memory of one may overlap the other's: a CTA has to read its sparse entries first
+  auto span = [&](const void* p, int64_t s0, int64_t s1, uintptr_t* lo, uintptr_t* hi) {
+    const int64_t d0 = (B - 1) * s0 * size, d1 = (L - 1) * s1 * size, base = (int64_t)(uintptr_t)p;
+    *lo = (uintptr_t)(base + std::min<int64_t>(d0, 0) + std::min<int64_t>(d1, 0));
+    *hi = (uintptr_t)(base + std::max<int64_t>(d0, 0) + std::max<int64_t>(d1, 0) + (int64_t)V * size);
+  };
+  uintptr_t a0, a1, b0, b1;
+  span(logits, bs, ps, &a0, &a1);
+  span(out, out_bs, out_ps, &b0, &b1);
+  const bool inplace = a0 < b1 && b0 < a1;
+  // the same elements, or memory that a position may be read from after it was written
+  if (inplace && (logits != out || (B > 1 && bs != out_bs) || (L > 1 && ps != out_ps))) return SD_EINVAL;
+  if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & (size - 1)) return SD_EINVAL;
+  // a chunk is 8 units per thread, and a CTA takes up to 8 positions, less where that would
+  // leave SMs without a CTA: first the positions, then the chunk
   int units = LG_UNITS;
-  while (units > 1 && (int64_t)B * L * ((V + units * LG_THREADS * E - 1) / (units * LG_THREADS * E)) <
-                          4 * 148)
-    units /= 2;
-  P.chunk = units * LG_THREADS * E;
-  P.chunks = (V + P.chunk - 1) / P.chunk;
-  const int64_t grid = (int64_t)B * L * P.chunks;
-  if (grid > 0x7FFFFFFF) return SD_ENOTSUP;
+  P.lg = inplace ? 1 : std::min(L, LG_POS);
+  auto ctas = [&]() {
+    P.chunk = units * LG_THREADS * E;
+    P.chunks = (V + P.chunk - 1) / P.chunk;
+    P.groups = (L + P.lg - 1) / P.lg;
+    return (int64_t)B * P.groups * P.chunks;
+  };
+  while (P.lg > 1 && ctas() < 2 * LG_CTAS) P.lg = (P.lg + 1) / 2;
+  while (units > 1 && ctas() < LG_CTAS) units /= 2;
+  const int64_t grid = ctas();
+  if (grid > 0x7FFFFFFF || (int64_t)L * P.chunk > 0x7FFFFFFF) return SD_ENOTSUP;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  auto go = [&](auto kernel) { kernel<<<(unsigned)grid, LG_THREADS, 0, st>>>(P); };
   if (dtype == SD_DTYPE_F32)
-    process_logits_kernel<SD_DTYPE_F32><<<(unsigned)grid, LG_THREADS, 0, st>>>(P);
+    inplace ? go(process_logits_kernel<SD_DTYPE_F32, true>) : go(process_logits_kernel<SD_DTYPE_F32, false>);
   else if (dtype == SD_DTYPE_F16)
-    process_logits_kernel<SD_DTYPE_F16><<<(unsigned)grid, LG_THREADS, 0, st>>>(P);
+    inplace ? go(process_logits_kernel<SD_DTYPE_F16, true>) : go(process_logits_kernel<SD_DTYPE_F16, false>);
   else
-    process_logits_kernel<SD_DTYPE_BF16><<<(unsigned)grid, LG_THREADS, 0, st>>>(P);
+    inplace ? go(process_logits_kernel<SD_DTYPE_BF16, true>) : go(process_logits_kernel<SD_DTYPE_BF16, false>);
   return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
 }
 

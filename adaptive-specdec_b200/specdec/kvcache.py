@@ -89,8 +89,9 @@ def commit_tree(keys, values, lengths, path, n_acc, nodes, block_table=None, err
     if len(shape) != 4 or e not in (2, 4):
         raise L.SpecdecError("caches must be [B, Hkv, C, D] or [n_pages, Hkv, PAGE, D] of a 2- or "
                              "4-byte type")
-    for t in bufs:
-        if t.dtype != dt or t.shape != shape or t.device != dev or not t.is_contiguous():
+    index = dev.index
+    for t in bufs:                                   # (two per layer: what a call costs most)
+        if t.dtype is not dt or t.get_device() != index or not t.is_contiguous() or t.shape != shape:
             raise L.SpecdecError("every layer's K and V must be contiguous, of one shape, type and "
                                  f"device ({dev})")
     n0, H, C, D = shape
