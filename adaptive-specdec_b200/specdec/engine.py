@@ -38,7 +38,13 @@ prompt is prefilled once, its full cache pages are shared by its n rows (a
 forked PagedRaggedCache with its page table on the device) and read once per
 group by the verify attention; ``logprobs=...`` reports the target model's
 log-probability of every emitted token (and alternatives), which is what ranks
-the samples.
+the samples.  ``generate(tree=...)`` drafts a tree of continuations per round instead of
+a chain (specdec.tree): the draft model's likeliest children of every node, level by
+level, one target forward over all nodes, and the longest path that the target's own
+draws follow.  SamplingConfig's penalties, biases and allowed tokens
+(specdec.sampling.process_logits) apply to the draft's and the target's logits at
+every position, the drafted tokens before it counted in, so speculation changes
+nothing about them.
 """
 import time
 from dataclasses import dataclass, field
@@ -47,7 +53,9 @@ import torch
 
 from specdec import attention as A
 from specdec.kvcache import PAGE, PagedRaggedCache, RaggedCache
-from specdec.sampling import TOP_N_MAX, draft_sample, to_probs, token_logprobs, verify_sample
+from specdec.sampling import (BIAS_MAX, TOP_N_MAX, TokenHistory, draft_sample, process_logits,
+                              to_probs, token_logprobs, verify_sample)
+from specdec.tree import tree_accept, tree_masks, tree_of_widths
 
 __all__ = ["SamplingConfig", "RunStats", "SpecDecodeEngine"]
 
@@ -57,6 +65,12 @@ class SamplingConfig:
     temperature: float = 0.0     # 0 => greedy, and the generic path still applies
     top_p: float = 1.0
     top_k: int = 0
+    # beyond the reference (specdec.sampling.process_logits), before all of the above
+    repetition_penalty: float = 1.0     # of tokens in the prompt or written: / if > 0, else *
+    presence_penalty: float = 0.0       # off once for a written token
+    frequency_penalty: float = 0.0      # off once per time that it was written
+    logit_bias: dict = None             # {token: added to its logit}
+    allowed_tokens: list = None         # no other token is ever drawn
 
     def probs(self, logits):
         return to_probs(logits, self.temperature, self.top_p, self.top_k)
@@ -129,6 +143,63 @@ class RunStats:
         }
 
 
+class _Constraints:
+    """A generate call's penalties, biases and allowed tokens, with the rows' token
+    history.  ``history`` holds what the caches hold: the prompt and the committed
+    tokens, not those of the round under way."""
+
+    def __init__(self, sp, input_ids, plen, vocab, device):
+        r = float(sp.repetition_penalty)
+        if not 0.0 < r < float("inf"):
+            raise ValueError(f"repetition_penalty must be positive, got {sp.repetition_penalty}")
+        self.history = None
+        self.kw = {}
+        if r != 1.0 or sp.presence_penalty or sp.frequency_penalty:
+            self.history = TokenHistory(input_ids.shape[0], vocab, device)
+            self.history.add_prompt(input_ids, plen)
+            self.scales = [("repetition", r), ("presence", float(sp.presence_penalty)),
+                           ("frequency", float(sp.frequency_penalty))]
+            self._rows(input_ids.shape[0], device)
+        if sp.logit_bias:
+            if len(sp.logit_bias) > BIAS_MAX:
+                raise ValueError(f"logit_bias has {len(sp.logit_bias)} tokens, at most {BIAS_MAX}")
+            self.kw["bias"] = (torch.tensor([list(sp.logit_bias)], dtype=torch.long, device=device),
+                               torch.tensor([list(sp.logit_bias.values())], dtype=torch.float32,
+                                            device=device))
+        if sp.allowed_tokens is not None:
+            ids = torch.as_tensor(list(sp.allowed_tokens), dtype=torch.long)
+            if ids.numel() == 0 or int(ids.min()) < 0 or int(ids.max()) >= vocab:
+                raise ValueError(f"allowed_tokens must be tokens in [0, {vocab}), at least one")
+            on = torch.zeros(-(-vocab // 32) * 32, dtype=torch.long)
+            on[ids] = 1
+            word = (on.view(-1, 32) << torch.arange(32)).sum(-1)
+            word = torch.where(word >= 1 << 31, word - (1 << 32), word).to(torch.int32)
+            self.kw["allowed"] = word.view(1, 1, -1).to(device)
+
+    def _rows(self, B, device):
+        self.kw["history"] = self.history
+        for name, x in self.scales:
+            self.kw[name] = torch.full((B,), x, dtype=torch.float32, device=device)
+
+    @classmethod
+    def of(cls, sp, input_ids, plen, vocab, device):
+        """None where the sampling has no constraints."""
+        c = cls(sp, input_ids, plen, vocab, device)
+        return c if c.kw else None
+
+    def fork(self, n):
+        if self.history is not None:
+            self.history = self.history.repeat_interleave(n)
+            self._rows(self.history.B, self.history.device)
+
+    def __call__(self, logits, tokens=None, masks=None, out=None):
+        return process_logits(logits, tokens, masks, out=out, **self.kw)
+
+    def commit(self, tokens, counts=None, path=None):
+        if self.history is not None:
+            self.history.append(tokens, counts, path)
+
+
 class _RoundGraphs:
     """CUDA graphs of one generate call's fixed-shape round steps.
 
@@ -141,9 +212,9 @@ class _RoundGraphs:
     mirrors are invalidated so that no step touches host state.
     """
 
-    def __init__(self, eng, B, k_max, dcache, tcache, drf_buf, T, tp, tk):
+    def __init__(self, eng, B, k_max, dcache, tcache, drf_buf, T, tp, tk, con=None):
         dev = eng.device
-        self.eng, self.B = eng, B
+        self.eng, self.B, self.con = eng, B, con
         self.dcache, self.tcache, self.drf_buf = dcache, tcache, drf_buf
         self.T, self.tp, self.tk = T, tp, tk
         self.pool = torch.cuda.graph_pool_handle()
@@ -151,6 +222,8 @@ class _RoundGraphs:
         self.u = torch.zeros(k_max, B, dtype=torch.float32, device=dev)
         self.xs = torch.zeros(B, k_max, dtype=torch.long, device=dev)
         self.qx = torch.ones(k_max, B, dtype=torch.float32, device=dev)
+        # what stands before each draft position: pending, then the drafts
+        self.path = torch.zeros(B, k_max + 1, dtype=torch.long, device=dev)
         self.rows0 = torch.zeros(B, dtype=torch.long, device=dev)
         self.vin, self.vlog, self.graphs = {}, {}, {}
         self.stream = torch.cuda.Stream(device=dev)
@@ -174,7 +247,11 @@ class _RoundGraphs:
         def body():
             logits = e._forward(e.draft, self.dcache, self.feed)[:, -1]
             self.dcache.advance(1)
-            self.drf_buf[:, i].copy_(logits)
+            if self.con is None:
+                self.drf_buf[:, i].copy_(logits)
+            else:
+                self.path[:, i].copy_(self.feed.view(B))
+                self.con(logits.unsqueeze(1), self.path[:, :i + 1], out=self.drf_buf[:, i:i + 1])
             x, q = draft_sample(self.drf_buf[:, i], self.u[i], self.T, self.tp, self.tk)
             self.xs[:, i].copy_(x)
             self.qx[i].copy_(q)
@@ -199,6 +276,76 @@ class _RoundGraphs:
             self.tcache.advance(k + 1)
         self._run(("target", k), body)
         return self.vlog[k]
+
+
+class _TreeRound:
+    """One round's forwards over a tree of drafted tokens (specdec.tree): the draft
+    model's children of every node level by level, then the target's forward over all
+    nodes.  From the second round on every step replays a CUDA graph of its own."""
+
+    def __init__(self, eng, B, widths, dcache, tcache, con, cuda_graphs):
+        dev = eng.device
+        self.eng, self.dcache, self.tcache, self.con = eng, dcache, tcache, con
+        self.widths = [int(w) for w in widths]
+        if max(self.widths, default=1) > min(TOP_N_MAX, eng.vocab_size):
+            raise ValueError(f"a node has at most {min(TOP_N_MAX, eng.vocab_size)} children, got "
+                             f"{list(widths)}")
+        parents, self.starts = tree_of_widths(self.widths)
+        self.nodes, self.depth = len(parents), len(self.widths)
+        self.masks, self.depths = tree_masks(parents, device=dev)
+        # the tree as far as each level, for the logits of its last nodes
+        self.upto = [self.masks[:n, :-(-n // 32)].contiguous() for n in self.starts[1:]]
+        self.tokens = torch.zeros(B, self.nodes, dtype=torch.long, device=dev)
+        self.vlog = None
+        self.rows0 = torch.zeros(B, dtype=torch.long, device=dev)
+        self.graphs = {} if cuda_graphs else None
+        self.pool = torch.cuda.graph_pool_handle() if cuda_graphs else None
+        self.stream = torch.cuda.Stream(device=dev) if cuda_graphs else None
+
+    def _level(self, d):
+        """Level d's nodes through the draft model, their children into ``tokens``."""
+        a, b = self.starts[d], self.starts[d + 1]
+        self.dcache.set_tree(self.masks, self.depths, a)
+        feed = self.tokens[:, a:b]
+        if d == self.depth:                          # only their keys and values are wanted
+            self.eng._forward(self.eng.draft, self.dcache, feed, rows_last=self.rows0)
+        else:
+            logits = self.eng._forward(self.eng.draft, self.dcache, feed)
+            if self.con is not None:
+                logits = self.con(logits, self.tokens[:, :b], self.upto[d])
+            top = token_logprobs(logits, feed, top_n=self.widths[d]).top_ids
+            self.tokens[:, b:self.starts[d + 2]].copy_(top.flatten(1))
+        self.dcache.advance(b - a)
+
+    def _verify(self):
+        self.tcache.set_tree(self.masks, self.depths)
+        self.vlog = self.eng._forward(self.eng.target, self.tcache, self.tokens)
+        self.tcache.advance(self.nodes)
+
+    def _run(self, key, body, first):
+        if self.graphs is None or first:             # (the first round warms every workspace)
+            return body()
+        self.dcache.invalidate_host()
+        self.tcache.invalidate_host()
+        g = self.graphs.get(key)
+        cur = torch.cuda.current_stream(self.eng.device)
+        if g is None:
+            g = torch.cuda.CUDAGraph()
+            self.stream.wait_stream(cur)
+            with torch.cuda.graph(g, pool=self.pool, stream=self.stream):
+                body()
+            cur.wait_stream(self.stream)
+            self.graphs[key] = g
+        g.replay()
+
+    def draft(self, pending, first):
+        self.tokens[:, 0].copy_(pending)
+        for d in range(self.depth + 1):
+            self._run(d, lambda: self._level(d), first)
+
+    def verify(self, first):
+        self._run("target", self._verify, first)
+        return self.vlog
 
 
 class _NullCtx:
@@ -348,10 +495,12 @@ class SpecDecodeEngine:
     # ---- main loop ---------------------------------------------------------
     @torch.inference_mode()
     def generate(self, input_ids, plen, max_new_tokens, sampling=None, controller=None,
-                 seed=None, k_fixed=None, n=1, logprobs=None):
+                 seed=None, k_fixed=None, n=1, logprobs=None, tree=None):
         """input_ids [B, P] right-padded, plen [B] real prompt lengths.
 
-        ``n`` samples per prompt (rows of one prompt side by side: B * n lists);
+        ``tree`` (number of children per node, level by level: (4, 2, 1)) drafts a tree
+        per round instead of a chain of k (``controller`` and ``k_fixed`` are then not
+        given); ``n`` samples per prompt (rows of one prompt side by side: B * n lists);
         ``logprobs`` (0 or more alternatives, None: off) fills the stats'
         ``logprobs`` and ``top_logprobs`` per row and emitted token.
 
@@ -362,6 +511,8 @@ class SpecDecodeEngine:
             raise ValueError(f"n must be at least 1, got {n}")
         if logprobs is not None and not 0 <= int(logprobs) <= min(TOP_N_MAX, self.vocab_size):
             raise ValueError(f"logprobs must be None or between 0 and {TOP_N_MAX}, got {logprobs}")
+        if tree is not None and (controller is not None or k_fixed is not None):
+            raise ValueError("a tree takes the place of controller and k_fixed")
         sp = sampling or SamplingConfig()
         T, tp, tk = sp.temperature, sp.top_p, sp.top_k
         dev = self.device
@@ -370,7 +521,8 @@ class SpecDecodeEngine:
         B = input_ids.shape[0]
         input_ids = input_ids.to(dev)
         plen = plen.to(dev)
-        k_cap = int(k_fixed) if k_fixed is not None else int(getattr(controller, "k_max", 16))
+        con = _Constraints.of(sp, input_ids, plen, self.vocab_size, dev)
+        k_cap = len(tree_of_widths(tree)[0]) if tree is not None else int(k_fixed) if k_fixed is not None else int(getattr(controller, "k_max", 16))
         tcache = self._mk_cache(self.target, B, plen, max_new_tokens, k_cap, n)
         dcache = self._mk_cache(self.draft, B, plen, max_new_tokens, k_cap, n)
         paged = self.paged_kv and n == 1
@@ -387,8 +539,11 @@ class SpecDecodeEngine:
                 tcache, dcache = tcache.fork([n] * B), dcache.fork([n] * B)
                 tlog = tlog.repeat_interleave(n, 0)
                 B = B * n
+                if con is not None:
+                    con.fork(n)
 
-        pending, _ = draft_sample(tlog, torch.rand(B, generator=gen, device=dev), T, tp, tk)
+        first = tlog if con is None else con(tlog.unsqueeze(1)).squeeze(1)
+        pending, _ = draft_sample(first, torch.rand(B, generator=gen, device=dev), T, tp, tk)
         pend_l = pending.tolist()
         out = [[int(pend_l[b])] for b in range(B)]
         done_l = [int(pend_l[b]) in self.eos_ids for b in range(B)]
@@ -400,6 +555,78 @@ class SpecDecodeEngine:
         drf_buf = None
         graphs = None
         K_BUF = 8
+        rnd = None if tree is None else _TreeRound(self, B, tree, dcache, tcache, con,
+                                                   self.cuda_graphs)
+
+        while tree is not None and not all(done_l):
+            if paged or device_pages:
+                dcache.reserve(rnd.nodes)
+                tcache.reserve(rnd.nodes)
+            d0 = time.perf_counter()
+            with self._range("draft_loop"):
+                rnd.draft(pending, st.rounds == 0)
+                st.draft_forwards += rnd.depth + 1
+            self._sync_phase()
+            v0 = time.perf_counter()
+            st.t_draft += v0 - d0
+            with self._range("verify"):
+                vlog = rnd.verify(st.rounds == 0)
+                st.target_forwards += 1
+            self._sync_phase()
+            st.t_target += time.perf_counter() - v0
+            with self._range("accept"):
+                u = torch.rand(B * rnd.nodes, generator=gen, device=dev)
+                alive = torch.tensor([not d for d in done_l], device=dev)
+                seen = vlog if con is None else con(vlog, rnd.tokens, rnd.masks)
+                # what the target draws behind every node: a child that holds it is accepted
+                choices, _ = draft_sample(seen.flatten(0, 1), u, T, tp, tk)
+                n_acc, y, path = tree_accept(rnd.tokens, choices.view(B, rnd.nodes), rnd.masks,
+                                             alive=alive, max_path=rnd.depth + 1)
+                if con is not None:
+                    con.commit(rnd.tokens, n_acc + 1, path)
+                tcache.commit_tree(path, n_acc, rnd.nodes)
+                dcache.commit_tree(path, n_acc, rnd.nodes)
+                nodes = path.long().clamp_min(0)
+                # the path's drafts, then y; -1 past that
+                at = torch.arange(rnd.depth + 1, device=dev).view(1, -1)
+                emitted = torch.cat([rnd.tokens.gather(1, nodes)[:, 1:], y.view(B, 1)], dim=1)
+                emitted = torch.where(at < n_acc.view(B, 1), emitted,
+                                      torch.where(at == n_acc.view(B, 1), y.view(B, 1), -1))
+                cols = [n_acc.view(B, 1), emitted]
+                if paged:
+                    cols += [tcache.lengths.view(B, 1), dcache.lengths.view(B, 1)]
+                if device_pages:
+                    cols += [(tcache._err | dcache._err).long().expand(B).view(B, 1)]
+                host = torch.cat(cols, dim=1).tolist()
+                if device_pages and host[0][-1]:
+                    tcache.check_errors()
+                    dcache.check_errors()
+                if logprobs is not None:
+                    rows = torch.arange(B, device=dev).view(-1, 1)
+                    lp, top = self._logprob_lists(vlog[rows, nodes], emitted, logprobs)
+                if paged:
+                    tcache.set_host_lengths([r[-2] for r in host])
+                    dcache.set_host_lengths([r[-1] for r in host])
+            n_acc_l = [r[0] for r in host]
+            st.rounds += 1
+            st.proposed += (rnd.nodes - 1) * B
+            st.accepted += sum(n_acc_l)
+            st.observe(rnd.depth, n_acc_l)
+            st.k_history.append(rnd.depth)
+            st.accept_history.append(n_acc_l)
+            for b in range(B):
+                for j in range(n_acc_l[b] + 1):
+                    if done_l[b]:
+                        break
+                    tok = host[b][1 + j]
+                    out[b].append(tok)
+                    st.emitted += 1
+                    if logprobs is not None:
+                        st.logprobs[b].append(lp[b][j])
+                        if logprobs:
+                            st.top_logprobs[b].append(top[b][j])
+                    done_l[b] = tok in self.eos_ids or len(out[b]) >= max_new_tokens
+            pending = y
 
         while not all(done_l):
             k = int(k_fixed) if k_fixed is not None else controller.propose_k()
@@ -414,7 +641,7 @@ class SpecDecodeEngine:
             use_g = self.cuda_graphs and st.rounds > 0 and graphs is not None
             if self.cuda_graphs and graphs is None and st.rounds > 0:
                 graphs = _RoundGraphs(self, B, drf_buf.shape[1], dcache, tcache, drf_buf,
-                                      T, tp, tk)
+                                      T, tp, tk, con)
                 use_g = True
             if paged:
                 # pages for this round's k + 1 tokens per cache, from the
@@ -452,7 +679,11 @@ class SpecDecodeEngine:
                         logits = self._forward(self.draft, dcache, feed)[:, -1]
                         dcache.advance(1)
                         st.draft_forwards += 1
-                        drf_buf[:, i].copy_(logits)
+                        if con is None:
+                            drf_buf[:, i].copy_(logits)
+                        else:
+                            before = torch.cat([pending.view(B, 1), xs[:, :i]], dim=1)
+                            con(logits.unsqueeze(1), before, out=drf_buf[:, i:i + 1])
                         x, qx = draft_sample(drf_buf[:, i], u_draft[i], T, tp, tk)
                         xs[:, i] = x
                         feed = x.view(B, 1)
@@ -492,8 +723,14 @@ class SpecDecodeEngine:
                 u_acc = torch.rand(B, k_eff, generator=gen, device=dev)
                 u_res = torch.rand(B, generator=gen, device=dev)
                 alive = torch.tensor([not d for d in done_l], device=dev)
-                n_acc, y = verify_sample(vlog, drf_buf[:, :k_eff], xs, u_acc, u_res, T, tp, tk,
+                seen = vlog
+                if con is not None:
+                    drafted = torch.cat([pending.view(B, 1), xs], dim=1)
+                    seen = con(vlog, drafted)
+                n_acc, y = verify_sample(seen, drf_buf[:, :k_eff], xs, u_acc, u_res, T, tp, tk,
                                          alive=alive)
+                if con is not None:
+                    con.commit(drafted, n_acc + 1)
                 tcache.commit(n_acc, k_eff)
                 dcache.commit(n_acc, k_eff)
                 # the one designed host sync of the round (with the paged
@@ -576,12 +813,14 @@ class SpecDecodeEngine:
         gen.manual_seed(int(seed) if seed is not None else int(torch.seed() % (2 ** 63)))
         B = input_ids.shape[0]
         input_ids, plen = input_ids.to(dev), plen.to(dev)
+        con = _Constraints.of(sp, input_ids, plen, self.vocab_size, dev)
         cache = self._mk_cache(self.target, B, plen, max_new_tokens, 1)
         st = RunStats(batch=B)
         t0 = time.perf_counter()
         logits = self._prefill(self.target, cache, input_ids, plen)
         st.target_forwards += 1
-        nxt, _ = draft_sample(logits, torch.rand(B, generator=gen, device=dev), T, tp, tk)
+        seen = logits if con is None else con(logits.unsqueeze(1)).squeeze(1)
+        nxt, _ = draft_sample(seen, torch.rand(B, generator=gen, device=dev), T, tp, tk)
         nl = nxt.tolist()
         out = [[int(nl[b])] for b in range(B)]
         done_l = [int(nl[b]) in self.eos_ids for b in range(B)]
@@ -597,7 +836,11 @@ class SpecDecodeEngine:
                                    rows_last=torch.zeros(B, dtype=torch.long, device=dev))
             cache.advance(1)
             st.target_forwards += 1
-            nxt, _ = draft_sample(logits, torch.rand(B, generator=gen, device=dev), T, tp, tk)
+            seen = logits
+            if con is not None:
+                con.commit(nxt.view(B, 1))
+                seen = con(logits.unsqueeze(1)).squeeze(1)
+            nxt, _ = draft_sample(seen, torch.rand(B, generator=gen, device=dev), T, tp, tk)
             nl = nxt.tolist()
             if logprobs is not None:
                 lp, top = self._logprob_lists(logits.unsqueeze(1), nxt.view(B, 1), logprobs)
