@@ -10,15 +10,19 @@
 // a row's vocabulary for up to LG_POS positions and passes over it once: 16-byte units
 // of the input, wherever they start in the row (rows of an odd vocabulary are aligned
 // differently), with -inf for what the mask bans; a unit that it bans whole is written
-// without being read.  What is sparse is then written over what the pass left: the
-// tokens that have a history (some thousand of 151936: the CTA reads the row's history
-// once and lists them), then those of the position's path and the biases, which, where
-// out is the logits themselves, have been computed before the pass.
-// 320 positions of 151936 bf16 logits, 64 rows of history, masks, biases (220 MB): 47.4 us,
-// 832 positions (531 MB): 110 us.  Copy and mask alone take 35 and 79 (98 % of the copy
-// rate), the list 5 and 7, the tokens on it the rest: two memory sectors each.  Looking
-// every unit up in the history during the pass took 59.8 and 127.5 (the history is then
-// read from L2 once per position), a position's chunk by way of shared memory 89 and 202.
+// without being read.  Tokens that have a history (some thousand of 151936) get their
+// penalties on the way: the CTA takes the chunk's history to shared memory once for all
+// its positions, with a bit per token, and a thread loops over the bits of its unit.  The
+// tokens of the position's path and the biases are written over what the pass left; where
+// out is the logits themselves, they have been computed before the pass.
+// 320 positions of 151936 bf16 logits, 64 rows of history, masks, biases (220 MB): 47.0 us,
+// 832 positions (531 MB): 101 us; without history and biases 32 and 79, a copy's rate.  What is
+// left is the penalties' arithmetic (3 and 5 us), the history's way to shared memory ahead
+// of the pass, and the sparse entries behind it.  Measured and left: the tokens with a
+// history listed and written over the pass's output (47.3 and 111; 33 instead of 23 for fp32 rows
+// of 32003), units asked for a position ahead (51, 108: fewer CTAs fit), one run of positions
+// per resident CTA (60, 121), the history looked up in global memory for every unit
+// (60, 127) or for the units whose bits are set (53, 110).
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
@@ -34,7 +38,7 @@ constexpr int LG_UNITS = 4;                  // most 16-byte units per thread an
 constexpr int LG_AHEAD = 4;                  // units whose loads are on their way at once
 constexpr int LG_POS = 8;                    // most positions of a CTA
 constexpr int LG_CTAS = 4 * 148;             // enough CTAs: four per SM
-constexpr int LG_CHUNK = LG_UNITS * LG_THREADS * 8;          // most tokens of a chunk: 32 a thread
+constexpr int LG_CHUNK = LG_UNITS * LG_THREADS * 8;          // most tokens of a chunk
 
 struct LogitsParams {
   const void* logits; int64_t bs, ps;
@@ -125,16 +129,41 @@ __device__ __forceinline__ float lg_entry(const LogitsParams& P, const LgPositio
   return !allow || ((allow[id >> 5] >> (id & 31)) & 1u) ? z : -CUDART_INF_F;
 }
 
+// Element j of a unit with its penalties.
+template <int DT>
+__device__ __forceinline__ void lg_penalize(uint4& v, int j, const LgPenalty& pen, int h) {
+  if constexpr (DT == SD_DTYPE_F32) {
+    const uint32_t z = __float_as_uint(pen(__uint_as_float(j & 2 ? (j & 1 ? v.w : v.z) : (j & 1 ? v.y : v.x)), h, 0));
+    if (j == 0) v.x = z;
+    if (j == 1) v.y = z;
+    if (j == 2) v.z = z;
+    if (j == 3) v.w = z;
+  } else {
+    using T = typename LgType<DT>::T;
+    const uint32_t word = j & 4 ? (j & 2 ? v.w : v.z) : (j & 2 ? v.y : v.x);
+    const unsigned short in = (unsigned short)(word >> (16 * (j & 1)));
+    T out;
+    lg_out(&out, pen(lg_in(*reinterpret_cast<const T*>(&in)), h, 0));
+    const uint32_t z =
+        __byte_perm(word, *reinterpret_cast<const unsigned short*>(&out), j & 1 ? 0x5410 : 0x3254);
+    const int w = j >> 1;
+    if (w == 0) v.x = z;
+    if (w == 1) v.y = z;
+    if (w == 2) v.z = z;
+    if (w == 3) v.w = z;
+  }
+}
+
 // INPLACE: out is the logits (one position per CTA; what is sparse is computed before the pass)
 template <int DT, bool INPLACE>
-__global__ void __launch_bounds__(LG_THREADS, 5) process_logits_kernel(const __grid_constant__ LogitsParams P) {
+__global__ void __launch_bounds__(LG_THREADS, INPLACE ? 5 : 6) process_logits_kernel(const __grid_constant__ LogitsParams P) {
   using T = typename LgType<DT>::T;
   constexpr int E = 16 / sizeof(T);                  // elements of a unit
   constexpr uint32_t ALL = (1u << E) - 1u;
   constexpr int SPARSE = INPLACE ? SD_TREE_MAX + SD_BIAS_MAX : 1;
-  // the chunk's tokens that have a history: place in the chunk, history above
-  __shared__ uint32_t seen[LG_CHUNK];
-  __shared__ int red[33];
+  // the chunk's history, and which of its tokens have one
+  __shared__ __align__(16) int16_t past[LG_CHUNK];
+  __shared__ uint32_t some[LG_CHUNK / 32 + 1];
   __shared__ int at[SPARSE];
   __shared__ float val[SPARSE];
   __shared__ int n_at;
@@ -159,34 +188,27 @@ __global__ void __launch_bounds__(LG_THREADS, 5) process_logits_kernel(const __g
     const int node = P.first + l;
     return LgPosition{P.masks ? P.masks + b * P.mask_bs + (int64_t)node * P.W : nullptr, node};
   };
-  int n_seen = 0;
   if (hist) {
-    // 32 tokens a thread
-    const int e = c0 + 32 * t, n = 32 * t < P.chunk ? min(32, c1 - e) : 0;
-    uint32_t h[16];
+    // eight tokens a thread; behind the chunk's end 0
+    const bool vec = (reinterpret_cast<uintptr_t>(hist) & 15) == 0;
+    unsigned char* bits = reinterpret_cast<unsigned char*>(some);
+#pragma unroll 1
+    for (int i = t; i < P.chunk / 8 + 4; i += LG_THREADS) {
+      const int e = c0 + 8 * i, n = min(8, c1 - e);
+      uint32_t h[4] = {0u, 0u, 0u, 0u};
+      if (vec && n == 8) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(hist + e));
+        h[0] = v.x; h[1] = v.y; h[2] = v.z; h[3] = v.w;
+      } else {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) h[k] = 0u;
-    if ((reinterpret_cast<uintptr_t>(hist) & 15) == 0 && n == 32) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(hist + e) + k);
-        h[4 * k] = v.x; h[4 * k + 1] = v.y; h[4 * k + 2] = v.z; h[4 * k + 3] = v.w;
+        for (int k = 0; k < 8; ++k)
+          if (k < n) h[k >> 1] |= (uint32_t)(unsigned short)hist[e + k] << (16 * (k & 1));
       }
-    } else {
+      uint32_t on = 0;
 #pragma unroll
-      for (int k = 0; k < 32; ++k)
-        if (k < n) h[k >> 1] |= (uint32_t)(unsigned short)hist[e + k] << (16 * (k & 1));
-    }
-    int mine = 0;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) mine += ((h[k] & 0xFFFFu) != 0u) + (h[k] >> 16 != 0u);
-    int to = block_excl_scan<int>(mine, red, &n_seen);
-    if (mine) {
-#pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const uint32_t v = (h[k >> 1] >> (16 * (k & 1))) & 0xFFFFu;
-        if (v) seen[to++] = v << 16 | (uint32_t)(32 * t + k);
-      }
+      for (int k = 0; k < 8; ++k) on |= (uint32_t)(((h[k >> 1] >> (16 * (k & 1))) & 0xFFFFu) != 0u) << k;
+      bits[i] = (unsigned char)on;
+      if (8 * i < P.chunk) *reinterpret_cast<uint4*>(&past[8 * i]) = make_uint4(h[0], h[1], h[2], h[3]);
     }
   }
   if (INPLACE && t == 0) n_at = 0;
@@ -244,6 +266,13 @@ __global__ void __launch_bounds__(LG_THREADS, 5) process_logits_kernel(const __g
       for (int k = 0; k < LG_AHEAD; ++k) {
         const int u = u0 + k * LG_THREADS;
         if (u >= nu) continue;
+        if (hist) {
+          const int e = head + u * E;
+          for (uint32_t which = lg_bits(some, e, LG_CHUNK / 32) & on[k]; which; which &= which - 1) {
+            const int j = __ffs((int)which) - 1;
+            lg_penalize<DT>(v[k], j, pen, past[e + j]);
+          }
+        }
         if (on[k] != ALL) v[k] = lg_ban<DT>(v[k], on[k]);
         if (wide) {
           reinterpret_cast<uint4*>(y)[u] = v[k];
@@ -271,33 +300,8 @@ __global__ void __launch_bounds__(LG_THREADS, 5) process_logits_kernel(const __g
     const uint32_t* allow = mask(l);
     T* y = output(l) + e;
     if (allow && !((allow[e >> 5] >> (e & 31)) & 1u)) lg_out(y, -CUDART_INF_F);
+    else if (hist) lg_out(y, pen(lg_in(x[e]), past[e - c0], 0));
     else *y = x[e];
-  }
-  if (n_seen > 0) {
-    // the tokens that have a history, over what the pass left
-    __syncthreads();
-    const int pairs = n_seen * nl;                   // (token, position)
-    for (int i0 = t; i0 < pairs; i0 += LG_THREADS * LG_AHEAD) {
-      T z[LG_AHEAD];
-      T* y[LG_AHEAD];
-      uint32_t on[LG_AHEAD], what[LG_AHEAD];
-#pragma unroll
-      for (int k = 0; k < LG_AHEAD; ++k) {
-        const int i = i0 + k * LG_THREADS, p = i / n_seen, l = l0 + p;
-        on[k] = i < pairs;
-        what[k] = on[k] ? seen[i - p * n_seen] : 0u;
-        const int e = c0 + (int)(what[k] & 0xFFFFu);
-        if (on[k]) {
-          const uint32_t* allow = mask(l);
-          if (allow) on[k] = (__ldg(allow + (e >> 5)) >> (e & 31)) & 1u;
-          y[k] = output(l) + e;
-          z[k] = logits(l)[e];
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < LG_AHEAD; ++k)
-        if (on[k]) lg_out(y[k], pen(lg_in(z[k]), (int)what[k] >> 16, 0));
-    }
   }
   if (np + P.M == 0) return;
   __syncthreads();
@@ -383,7 +387,7 @@ int sd_process_logits(const void* logits, int64_t bs, int64_t ps, int dtype, int
   // the same elements, or memory that a position may be read from after it was written
   if (inplace && (logits != out || (B > 1 && bs != out_bs) || (L > 1 && ps != out_ps))) return SD_EINVAL;
   if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & (size - 1)) return SD_EINVAL;
-  // a chunk is 8 units per thread, and a CTA takes up to 8 positions, less where that would
+  // a chunk is up to 4 units per thread, and a CTA takes up to 8 positions, less where that would
   // leave SMs without a CTA: first the positions, then the chunk
   int units = LG_UNITS;
   P.lg = inplace ? 1 : std::min(L, LG_POS);
@@ -396,7 +400,7 @@ int sd_process_logits(const void* logits, int64_t bs, int64_t ps, int dtype, int
   while (P.lg > 1 && ctas() < 2 * LG_CTAS) P.lg = (P.lg + 1) / 2;
   while (units > 1 && ctas() < LG_CTAS) units /= 2;
   const int64_t grid = ctas();
-  if (grid > 0x7FFFFFFF || (int64_t)L * P.chunk > 0x7FFFFFFF) return SD_ENOTSUP;
+  if ((double)B * P.groups * P.chunks > 0x7FFFFFFF) return SD_ENOTSUP;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto go = [&](auto kernel) { kernel<<<(unsigned)grid, LG_THREADS, 0, st>>>(P); };
   if (dtype == SD_DTYPE_F32)
