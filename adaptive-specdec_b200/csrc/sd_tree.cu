@@ -6,8 +6,9 @@
 // takes one 16-byte column of a (row, buffer, kv head) along the whole path, in
 // order, so source p_j is read before any later step writes slot p_j, and no two
 // threads touch the same bytes: the move is done in place, in one pass.  What it
-// has to move is tiny (32 rows, 36 layers, 3 nodes: 28 MB with the stores), so it
-// is bound by the latency of its chain: path, page, K / V, store.
+// has to move is tiny, so it is bound by the latency of its chain: path, page,
+// K / V, store.  Accept, move and lengths take 9.2 us in a graph for 32 rows and 36 layers
+// (19 MB read and written), 13.1 us for 64 rows and up to 8 nodes (76 MB).
 #include <cuda_runtime.h>
 #include <stdint.h>
 

@@ -522,7 +522,10 @@ class SpecDecodeEngine:
         input_ids = input_ids.to(dev)
         plen = plen.to(dev)
         con = _Constraints.of(sp, input_ids, plen, self.vocab_size, dev)
-        k_cap = len(tree_of_widths(tree)[0]) if tree is not None else int(k_fixed) if k_fixed is not None else int(getattr(controller, "k_max", 16))
+        if tree is not None:
+            k_cap = len(tree_of_widths(tree)[0])
+        else:
+            k_cap = int(k_fixed) if k_fixed is not None else int(getattr(controller, "k_max", 16))
         tcache = self._mk_cache(self.target, B, plen, max_new_tokens, k_cap, n)
         dcache = self._mk_cache(self.draft, B, plen, max_new_tokens, k_cap, n)
         paged = self.paged_kv and n == 1

@@ -33,7 +33,7 @@ kvcache.py:98-116).  Its page bookkeeping runs on the host (``PageTable``) or, w
 device lengths without a host copy of them, and ``fork`` makes several rows of
 one prompt that share its pages.
 """
-import ctypes
+from array import array
 
 import numpy as np
 import torch
@@ -105,10 +105,10 @@ def commit_tree(keys, values, lengths, path, n_acc, nodes, block_table=None, err
             raise L.SpecdecError("paged caches must be [n_pages, Hkv, PAGE, D] pools")
     elif n0 != B:
         raise L.SpecdecError(f"caches of {n0} rows for {B} lengths")
-    ptrs = (ctypes.c_void_p * len(bufs))(*[t.data_ptr() for t in bufs])
+    ptrs = array("Q", map(torch.Tensor.data_ptr, bufs))
     with L.on_device(dev):
         L.check(L.lib().sd_kv_commit_tree(
-            ptrs, len(bufs), L.address(block_table), W, npages, lengths.data_ptr(),
+            ptrs.buffer_info()[0], len(bufs), L.address(block_table), W, npages, lengths.data_ptr(),
             path.data_ptr(), path.stride(0), path.shape[1], n_acc.data_ptr(), N, B, H, C, D, e,
             L.address(err), L.stream_of(dev)), "kv_commit_tree")
 

@@ -215,8 +215,9 @@ int sd_token_logprobs(const void* logits, int64_t bs, int64_t ps, int dtype, con
  *   x = x - frequency[b] * c;  if c > 0: x = x - presence[b]
  *   x = x + sum of bias_values[b, m] over bias_ids[b, m] == t
  *   if bit t % 32 of allowed[b, l, t / 32] is 0: x = -inf
- * in float32, rounded once to out[b, l, t] (which may be the same memory as
- * logits).  history NULL: no penalties (the three [B] arrays are then unused; each
+ * in float32, rounded once to out[b, l, t]: the logits themselves (same address and
+ * strides), or memory outside the span from their first to their last entry, else
+ * SD_EINVAL.  history NULL: no penalties (the three [B] arrays are then unused; each
  * may be NULL by itself: neutral); bias_ids NULL: no bias (an id outside [0, V) is
  * padding); allowed NULL: no mask.  bias_bs / allowed_bs / allowed_ps may be 0
  * (one list / mask for all rows / positions).  A drafted token outside [0, V) is
@@ -515,9 +516,10 @@ int sd_kv_commit_tree(void* const* bufs, int n_bufs, const int32_t* block_table,
  * Slots that no node sees may hold anything; V in a slot that some node of the
  * tree sees has to be finite where other nodes of the row do not see it.
  * bf16 with D = 128 and Hq / Hkv <= 128 runs on the tensor cores (q, caches
- * 16-byte aligned, q strides multiples of 8); fp32 and other shapes with D <= 128
- * on the CUDA cores, without a workspace.  scale > 0.  The workspace must be
- * 256-byte aligned and needs no initialisation.  If a bounded wait inside the
+ * 16-byte aligned, q strides positive multiples of 8); fp32 and other shapes with
+ * D <= 128 on the CUDA cores, without a workspace.  scale > 0.  The workspace must be
+ * 256-byte aligned and needs no initialisation; calls on two streams, or captured
+ * into two graphs that may run at once, need one each.  If a bounded wait inside the
  * kernels gives up, the output is NaN.
  */
 size_t sd_tree_attn_workspace_bytes(int B, int Hq, int Hkv, int D, int C, int qlen, int dtype);
