@@ -106,6 +106,8 @@ def commit_tree(keys, values, lengths, path, n_acc, nodes, block_table=None, err
     elif n0 != B:
         raise L.SpecdecError(f"caches of {n0} rows for {B} lengths")
     ptrs = array("Q", map(torch.Tensor.data_ptr, bufs))
+    if len(set(ptrs)) != len(ptrs) and bufs[0].numel():
+        raise L.SpecdecError("a buffer stands twice among the layers' K and V")
     with L.on_device(dev):
         L.check(L.lib().sd_kv_commit_tree(
             ptrs.buffer_info()[0], len(bufs), L.address(block_table), W, npages, lengths.data_ptr(),

@@ -90,9 +90,12 @@ def tree_of_widths(widths):
 
 def check_masks(masks, rows, name):
     """(words between rows' trees, N) of masks [N, W], [1, N, W] or [rows, N, W]."""
-    if masks.dtype != torch.int32 or masks.dim() not in (2, 3) or not masks.is_contiguous():
-        raise L.SpecdecError(f"{name}: masks must be contiguous int32 [N, W] or [B, N, W]")
+    if masks.dtype != torch.int32 or masks.dim() not in (2, 3):
+        raise L.SpecdecError(f"{name}: masks must be int32 [N, W] or [B, N, W]")
     N, W = masks.shape[-2:]
+    if not masks.is_contiguous() and ((W > 1 and masks.stride(-1) != 1)
+                                      or (N > 1 and masks.stride(-2) != W)):
+        raise L.SpecdecError(f"{name}: the words of a tree's masks must lie together")
     if not 1 <= N <= TREE_MAX or W != -(-N // 32):
         raise L.SpecdecError(f"{name}: a tree of N nodes (1 to {TREE_MAX}) has ceil(N / 32) words "
                              f"per node, got {tuple(masks.shape)}")
@@ -100,7 +103,7 @@ def check_masks(masks, rows, name):
         return 0, N
     if masks.shape[0] != rows:
         raise L.SpecdecError(f"{name}: masks for {masks.shape[0]} trees, but {rows} rows")
-    return N * W, N
+    return masks.stride(0), N
 
 
 class TreePath(NamedTuple):

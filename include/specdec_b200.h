@@ -499,6 +499,7 @@ int sd_tree_accept(const int64_t* tokens, int64_t tokens_bs, const int64_t* choi
  * rising, and hold n_acc[b] + 1 <= path_len nodes; n_acc[b] < N.  A row whose
  * slots leave [0, C] (bit 0 of *err) or whose path breaks these rules (bit 5)
  * is left as it was, length included; a slot without a page is not moved (bit 1).
+ * The buffers do not overlap.
  */
 int sd_kv_commit_tree(void* const* bufs, int n_bufs, const int32_t* block_table, int bt_stride,
                       int npages, int64_t* lengths, const int32_t* path, int64_t path_bs,

@@ -152,6 +152,40 @@ def test_against_the_definition(dtype, B, Lq, V, N, tree, M, pad, hist_pad):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [40, 2049, 20001])
+def test_every_alignment_of_input_output_and_history(dtype, V):
+    x, tokens, parents, sees, hist, par, bias, allowed = _inputs(2, 3, V, 4, dtype, V, M=5)
+    gb, allowed_d = tuple(t.to(DEV) for t in bias), allowed.to(DEV)
+    gp = dict(zip(("repetition", "presence", "frequency"), (t.to(DEV) for t in par)))
+    z, tol = _plain(x, tokens, sees, hist, *par, bias, allowed)
+    for a, c, h in ((0, 1, 1), (1, 0, 2), (3, 3, 8), (5, 2, 0), (8, 7, 5)):
+        room = torch.full((2, 3, V + 16), 3.0, dtype=dtype, device=DEV)
+        room_h = torch.full((2, V + 16), 77, dtype=torch.int16, device=DEV)
+        room[..., a:a + V], room_h[:, h:h + V] = x.to(DEV), hist.to(DEV)
+        out = torch.full((2, 3, V + 16), 3.0, dtype=dtype, device=DEV)
+        kw = dict(history=room_h[:, h:h + V], bias=gb, allowed=allowed_d, **gp)
+        _check(process_logits(room[..., a:a + V], tokens.to(DEV), out=out[..., c:c + V], **kw), z, tol, dtype)
+        assert bool((out[..., :c] == 3).all()) and bool((out[..., c + V:] == 3).all())
+        view = room[..., a:a + V]
+        _check(process_logits(view, tokens.to(DEV), out=view, **kw), z, tol, dtype)
+        assert bool((room[..., :a] == 3).all()) and bool((room[..., a + V:] == 3).all())
+
+
+@gpu
+def test_outputs_over_other_logits_are_refused():
+    wide = torch.randn(4, 3, 64, device=DEV)
+    for logits, out in ((wide[:2], wide[1:3]), (wide[::2], wide[1::2])):
+        before = wide.clone()
+        with pytest.raises(L.SpecdecError):
+            process_logits(logits, out=out)
+        assert torch.equal(wide, before)
+    flat = torch.randn(2 * 3 * 64 + 8, device=DEV)
+    with pytest.raises(L.SpecdecError):
+        process_logits(flat[:384].view(2, 3, 64), out=flat[4:388].view(2, 3, 64))
+
+
+@gpu
 def test_shared_masks_numbers_and_missing_tokens():
     """One mask for all rows or positions, numbers for the penalties, no drafted tokens."""
     x, tokens, _, _, hist, par, _, allowed = _inputs(3, 4, 515, 4, torch.float32, 0)

@@ -359,6 +359,18 @@ def test_refusals():
         RaggedCache(1, 1, 10, DEV).set_tree(masks, masks)
 
 
+@gpu
+def test_a_buffer_that_is_there_twice_is_refused():
+    """Two threads would move the same bytes."""
+    k, v = torch.zeros(2, 1, 20, 8, device=DEV), torch.zeros(2, 1, 20, 8, device=DEV)
+    lens, n = torch.tensor([5, 5], device=DEV), torch.zeros(2, dtype=torch.long, device=DEV)
+    path = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    for keys, values in (([k], [k]), ([k, k], [v, torch.zeros_like(v)])):
+        with pytest.raises(L.SpecdecError):
+            commit_tree(keys, values, lens, path, n, 3)
+    assert lens.tolist() == [5, 5]
+
+
 def test_refused_on_the_host():
     lib = L.lib()
     assert lib.sd_tree_masks(None, 0, 1, 4, 16, 16, None) == -22

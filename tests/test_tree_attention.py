@@ -258,6 +258,43 @@ def test_strides_scale_and_given_output(dtype, d):
 
 
 @gpu
+@pytest.mark.parametrize("bases", [[70, 300], [2000, 5000]])
+def test_outputs_that_no_wide_store_reaches(bases):
+    """Rows of an output that start 2 bytes past aligned addresses: whole and joined items."""
+    g = torch.Generator().manual_seed(16)
+    call, kw, ref = _case(bases, [_parents(7, g)], 8, 2, 128, torch.bfloat16)
+    room = torch.full((2, 7, 8, 131), 7.0, dtype=torch.bfloat16, device=DEV)
+    _check(call, kw, ref, out=room[..., 1:129])
+    assert bool((room[..., 0] == 7).all()) and bool((room[..., 129:] == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float32, 64)])
+def test_broadcast_queries_and_masks(dtype, d):
+    """One query for all heads, nodes or rows, one row of masks for all rows."""
+    g = torch.Generator().manual_seed(17)
+    call, kw, ref = _case([9, 150], [_parents(5, g)], 8, 2, d, dtype)
+    q, k, v, lengths, masks = call
+    for x in (q[:1].expand(2, -1, -1, -1), q[:, :1].expand(-1, 8, -1, -1), q[:, :, :1].expand(-1, -1, 5, -1)):
+        _check((x, k, v, lengths, masks.expand(2, -1, -1)), kw, ref)
+
+
+@gpu
+@pytest.mark.parametrize("hq,hkv", [(5, 1), (71, 1), (128, 1), (129, 1), (40, 8), (192, 3)])
+@pytest.mark.parametrize("n", [1, 3, 20])
+def test_head_groups_of_every_size(hq, hkv, n):
+    g = torch.Generator().manual_seed(n)
+    _check(*_case([0, 60, 900], [_parents(n, g)], hq, hkv, 128, torch.bfloat16, paged=n == 3, seed=n))
+
+
+@gpu
+def test_caches_smaller_than_a_tile():
+    g = torch.Generator().manual_seed(18)
+    for n, base in ((1, 0), (2, 3), (9, 1)):
+        _check(*_case([base], [_parents(n, g)], 2, 1, 128, torch.bfloat16, slack=0))
+
+
+@gpu
 def test_masks_that_are_no_tree_and_bits_past_the_nodes():
     """Any bits are followed; the ones from N on are ignored."""
     call, kw, ref = _case([140], [[-1, 0, 1, 0, 3]], 4, 2, 128, torch.bfloat16)
