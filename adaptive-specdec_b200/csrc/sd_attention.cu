@@ -1207,13 +1207,13 @@ static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
 }
 
-// 2D map over a [B, Hkv, C, 128] bf16 cache viewed as [B * Hkv * C, 128]:
+// 2D map over a [B, Hkv, C, D] bf16 cache viewed as [B * Hkv * C, D]:
 // boxes of 128 rows x 64 columns (128 B), 128-byte swizzle, zero fill
-bool cache_map(CUtensorMap* map, const void* base, int64_t rows, int box_rows) {
+bool cache_map(CUtensorMap* map, const void* base, int64_t rows, int box_rows, int D) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
   if (enc == nullptr) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)MT_D, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)MT_D * 2};
+  const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
   const cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1u, 1u};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides,

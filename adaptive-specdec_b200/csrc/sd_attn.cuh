@@ -50,9 +50,10 @@ __device__ __forceinline__ int row_limit(const AttnParams& P, int b, int j) {
   return lim > 0 ? (int)lim : 0;
 }
 
-// sd_attention.cu: a 2D tensor map over a cache viewed as [rows, 128] bf16
+// sd_attention.cu: a 2D tensor map over a cache viewed as [rows, D] bf16
 // (boxes of box_rows rows x 64 columns, 128-byte swizzle)
-bool cache_map(CUtensorMap* map, const void* base, int64_t rows, int box_rows = SD_KV_PAGE);
+bool cache_map(CUtensorMap* map, const void* base, int64_t rows, int box_rows = SD_KV_PAGE,
+               int D = 128);
 // A 4D tensor map over bf16 [sizes[3], sizes[2], sizes[1], sizes[0]] with element
 // strides (strides[2], strides[1], strides[0], 1), multiples of 8; 128-byte swizzle
 bool tile_map(CUtensorMap* map, const void* base, const int64_t (&sizes)[4],

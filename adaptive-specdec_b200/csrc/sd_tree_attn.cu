@@ -1,5 +1,5 @@
 // Attention of a tree's nodes over the cache (sm_100a): host entry, and the tensor-core
-// kernels for bf16 heads of 128.
+// kernels for bf16 heads of 64 and 128.
 //
 // The query rows of a (row, kv head) are its nodes times the heads of the group:
 // 64 nodes under 32 / 8 heads are 256 rows that read the same keys.  An item is one
@@ -22,6 +22,8 @@
 // One tile: S of the next page stands ready in TMEM's second buffer, and its 128 columns go
 // to two warpgroups, so that a page's softmax takes half as long.  Two tiles: S and O of both
 // fill TMEM, so S comes in halves of 64 keys (tt_issue_pair); whole pages of S took 422 us.
+// Heads of 64 halve the tiles and so put twice as many on their way: 32 rows of 26 nodes over
+// 2048 keys take 55 us (CUDA cores: 1.17 ms).
 // Queries come by TMA (the softmax threads' own loads waited 8000 cycles behind K and V),
 // the nodes' bits late and by asynchronous copies, as only the tree's pages look at them.
 #include <cuda_bf16.h>
@@ -38,7 +40,6 @@
 
 namespace sd {
 
-constexpr int TT_D = 128;
 constexpr int TT_TILE = 128;                 // query rows of a tile
 constexpr int TT_THREADS = 352;              // warps 0-7: softmax; 8: TMA of K, V; 9: MMA; 10: TMA of Q
 constexpr int TT_CTAS = 148;                 // one CTA per SM
@@ -69,12 +70,14 @@ __device__ __forceinline__ int tt_share(int total) {
   return max(TT_MIN_SHARE, (total + TT_CTAS - 1) / TT_CTAS);
 }
 
-// NT: tiles of query rows of an item
-template <int NT>
+// NT: tiles of query rows of an item; D: head size, 64 or 128
+template <int NT, int D>
 struct TtSmem {
-  static constexpr int SLOTS = NT == 2 ? 4 : 5;      // 32 KB K / V tiles in flight
-  alignas(1024) unsigned char q[NT][2][128 * 128];           // [tile][64-col box][128 rows x 128 B]
-  alignas(1024) unsigned char kv[SLOTS][2][128 * 128];       // [slot][64-col box][128 keys x 128 B]
+  static constexpr int BOXES = D / 64;               // of 64 columns
+  static constexpr uint32_t TILE = BOXES * 16384u;   // bytes of a tile of 128 rows
+  static constexpr int SLOTS = (NT == 2 ? 4 : 5) * 2 / BOXES;          // K / V tiles in flight
+  alignas(1024) unsigned char q[NT][BOXES][128 * 128];       // [tile][64-col box][128 rows x 128 B]
+  alignas(1024) unsigned char kv[SLOTS][BOXES][128 * 128];   // [slot][64-col box][128 keys x 128 B]
   alignas(16) unsigned char out[8][32 * 64];         // a warp's 32 rows x 32 outputs
   // one tile: sfull, pfull and oready by page parity; two: by tile, of the two halves of S (slo,
   // shi), of S's second half in registers (sread)
@@ -89,8 +92,10 @@ struct TtSmem {
   int abort_;
   uint32_t tmem;
 };
-static_assert(sizeof(TtSmem<2>) + 1024 <= 227 * 1024, "shared memory, with room to align");
-static_assert(sizeof(TtSmem<1>) + 1024 <= 227 * 1024, "shared memory, with room to align");
+static_assert(sizeof(TtSmem<2, 128>) + 1024 <= 227 * 1024, "shared memory, with room to align");
+static_assert(sizeof(TtSmem<1, 128>) + 1024 <= 227 * 1024, "shared memory, with room to align");
+static_assert(sizeof(TtSmem<2, 64>) + 1024 <= 227 * 1024, "shared memory, with room to align");
+static_assert(sizeof(TtSmem<1, 64>) + 1024 <= 227 * 1024, "shared memory, with room to align");
 
 // A CTA's run of schedule units as segments of items, walked identically by
 // every role: row-major, kv head and then the item inner; TT_OVH virtual units in
@@ -98,8 +103,8 @@ static_assert(sizeof(TtSmem<1>) + 1024 <= 227 * 1024, "shared memory, with room 
 struct TtSeg {
   int b, h, p, base, tb, off, tt, t1, ncost, j0, j1;         // pages [j0, j1) of the segment
 };
-template <int NT>
-__device__ __forceinline__ int tt_base(const TtSmem<NT>& S, const TreeParams& T, int b) {
+template <int NT, int D>
+__device__ __forceinline__ int tt_base(const TtSmem<NT, D>& S, const TreeParams& T, int b) {
   return b < TT_BASES ? S.base[b] : tree_base(T, b);
 }
 __device__ __forceinline__ void tt_bounds(TtSeg& s) {
@@ -107,8 +112,8 @@ __device__ __forceinline__ void tt_bounds(TtSeg& s) {
   s.j0 = max(s.off, TT_OVH) - TT_OVH;
   s.j1 = max(s.off + s.ncost - TT_OVH, s.j0);
 }
-template <int NT>
-__device__ __forceinline__ bool tt_next(TtSeg& s, const TtSmem<NT>& S, const TreeTcParams& P) {
+template <int NT, int D>
+__device__ __forceinline__ bool tt_next(TtSeg& s, const TtSmem<NT, D>& S, const TreeTcParams& P) {
   s.tt += s.ncost;
   if (s.tt >= s.t1) return false;
   s.off = 0;
@@ -125,8 +130,8 @@ __device__ __forceinline__ bool tt_next(TtSeg& s, const TtSmem<NT>& S, const Tre
   return true;
 }
 // On to the current or next segment with pages; false when none is left.
-template <int NT>
-__device__ __forceinline__ bool tt_real(TtSeg& s, const TtSmem<NT>& S, const TreeTcParams& P) {
+template <int NT, int D>
+__device__ __forceinline__ bool tt_real(TtSeg& s, const TtSmem<NT, D>& S, const TreeTcParams& P) {
   while (s.j1 == s.j0)
     if (!tt_next(s, S, P)) return false;
   return true;
@@ -134,8 +139,8 @@ __device__ __forceinline__ bool tt_real(TtSeg& s, const TtSmem<NT>& S, const Tre
 
 // The schedule: every CTA sums the rows' units and finds its own first row.  The
 // units per CTA and, in S.first, where the run of this one starts.
-template <int NT>
-__device__ __forceinline__ void tt_plan(TtSmem<NT>& S, const TreeTcParams& P, int* total, int* share) {
+template <int NT, int D>
+__device__ __forceinline__ void tt_plan(TtSmem<NT, D>& S, const TreeTcParams& P, int* total, int* share) {
   const TreeParams& T = P.T;
   const int t = threadIdx.x, cta = (int)blockIdx.x, B = T.A.B, per = T.A.Hkv * P.np;
   int mine = 0, ex = 0, all = 0;
@@ -284,22 +289,22 @@ __device__ __forceinline__ void tt_write(unsigned char* stage, const float (&o)[
 
 // ---- the roles of a CTA's warps ---------------------------------------------------------------
 // Q of a tile of a segment's item: its nodes x heads.
-template <int NT>
-__device__ __forceinline__ void tt_ask_q(TtSmem<NT>& S, const TreeTcParams& P, const CUtensorMap& tmq,
+template <int NT, int D>
+__device__ __forceinline__ void tt_ask_q(TtSmem<NT, D>& S, const TreeTcParams& P, const CUtensorMap& tmq,
                                          const TtSeg& g, int ti) {
   const int group = P.T.A.group, j = g.p * P.ni + P.nt * ti;
-  tc_expect_tx(&S.qfull[ti], 2u * 128u * (uint32_t)(P.nt * group));
-  tt_tma_4d(S.q[ti][0], &tmq, 0, g.h * group, j, g.b, &S.qfull[ti]);
-  tt_tma_4d(S.q[ti][1], &tmq, 64, g.h * group, j, g.b, &S.qfull[ti]);
+  tc_expect_tx(&S.qfull[ti], 2u * D * (uint32_t)(P.nt * group));
+#pragma unroll
+  for (int x = 0; x < D / 64; ++x) tt_tma_4d(S.q[ti][x], &tmq, 64 * x, g.h * group, j, g.b, &S.qfull[ti]);
 }
 
 // TMA producer (one thread): K then V of each page, SLOTS tiles ahead; the first segment's Q
 // in front, before all SMs' K and V are on their way.
-template <int NT>
-__device__ __forceinline__ void tt_load_kv(TtSmem<NT>& S, const TreeTcParams& P, const CUtensorMap& tmk,
+template <int NT, int D>
+__device__ __forceinline__ void tt_load_kv(TtSmem<NT, D>& S, const TreeTcParams& P, const CUtensorMap& tmk,
                                            const CUtensorMap& tmv, const CUtensorMap& tmq, TtSeg seg,
                                            bool more, int share) {
-  constexpr int SLOTS = TtSmem<NT>::SLOTS;
+  constexpr int SLOTS = TtSmem<NT, D>::SLOTS;
   int4 cut = make_int4(0, 0, 0, 0);
   for (int ti = 0; ti < NT && more; ++ti) tt_ask_q(S, P, tmq, seg, ti);
   uint32_t idx = 0;
@@ -312,10 +317,10 @@ __device__ __forceinline__ void tt_load_kv(TtSmem<NT>& S, const TreeTcParams& P,
         const int sl = (int)(idx % SLOTS);
         if (idx >= (uint32_t)SLOTS) ok = tc_wait(&S.empty[sl], ((idx / SLOTS) - 1) & 1u, &S.abort_);
         if (!ok) break;
-        tc_expect_tx(&S.full[sl], 2u * 128u * 128u);
+        tc_expect_tx(&S.full[sl], TtSmem<NT, D>::TILE);
         const void* map = kv ? (const void*)&tmv : (const void*)&tmk;
-        tc_tma_2d(S.kv[sl][0], map, 0, y, &S.full[sl]);
-        tc_tma_2d(S.kv[sl][1], map, 64, y, &S.full[sl]);
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) tc_tma_2d(S.kv[sl][x], map, 64 * x, y, &S.full[sl]);
       }
     }
     if (seg.j0 == 0 && seg.j1 + TT_OVH < seg.tb)     // (the last segment)
@@ -333,8 +338,8 @@ __device__ __forceinline__ void tt_load_kv(TtSmem<NT>& S, const TreeTcParams& P,
 }
 
 // TMA producer (one thread) of the later segments' Q, once a tile's last S is done.
-template <int NT>
-__device__ __forceinline__ void tt_load_q(TtSmem<NT>& S, const TreeTcParams& P, const CUtensorMap& tmq,
+template <int NT, int D>
+__device__ __forceinline__ void tt_load_q(TtSmem<NT, D>& S, const TreeTcParams& P, const CUtensorMap& tmq,
                                           TtSeg seg, bool more) {
   uint32_t sent = more ? NT : 0u;                    // tiles asked for, tile inner
   bool ok = true;
@@ -356,24 +361,26 @@ __device__ __forceinline__ void tt_load_q(TtSmem<NT>& S, const TreeTcParams& P, 
 
 constexpr uint32_t TT_ID_S = tc_idesc(128, 128, 0, 0);       // S = Q . K^T of 128 keys
 constexpr uint32_t TT_ID_H = tc_idesc(128, 64, 0, 0);        // of 64 keys
-constexpr uint32_t TT_ID_O = tc_idesc(128, 128, 0, 1);       // O += P . V (V [key][d]: N-major)
+template <int D> constexpr uint32_t TT_ID_O = tc_idesc(128, D, 0, 1);           // O += P . V (V [key][d]: N-major)
 
-// S = Q . K^T by a warp: 16 of 128 d an MMA: 32 B, the second box 16 KB on.
+// S = Q . K^T by a warp: 16 of D columns an MMA: 32 B, the second box 16 KB on.
+template <int D>
 __device__ __forceinline__ void tt_mma_s(uint32_t d, uint32_t q, uint32_t k, uint32_t id) {
   const uint64_t dq = tc_desc(q, 16, 1024, 2), dk = tc_desc(k, 16, 1024, 2);
 #pragma unroll
-  for (int ks = 0; ks < 8; ++ks) {
+  for (int ks = 0; ks < D / 16; ++ks) {
     const uint64_t o = (uint64_t)((ks & 3) * 2 + (ks >> 2) * 1024);
     tc_mma_warp(d, dq + o, dk + o, id, ks > 0 ? 1 : 0);
   }
 }
 // O (+)= P . V by a warp: 16 keys an MMA: 2 KB of V, 8 columns of P, whose second 64 keys start
 // at column `half`.
+template <int D>
 __device__ __forceinline__ void tt_mma_o(uint32_t o, uint32_t p, uint32_t half, uint32_t v, bool acc) {
   const uint64_t dv = tc_desc(v, 16384, 1024, 2);
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks)
-    tc_mma_ts_warp(o, p + half * (ks >> 2) + 8u * (ks & 3), dv + (uint64_t)(ks * 128), TT_ID_O,
+    tc_mma_ts_warp(o, p + half * (ks >> 2) + 8u * (ks & 3), dv + (uint64_t)(ks * 128), TT_ID_O<D>,
                    ks || acc ? 1 : 0);
 }
 // An issuer that has found nothing to do since `idle` (0: it has just begun): whether it goes on.
@@ -395,8 +402,9 @@ __device__ __forceinline__ void tt_finish(unsigned long long* bar) {
 
 // MMA issuer of one tile: S(0) S(1) P.V(0) S(2) P.V(1) ...; S of page i in buffer i & 1 (128
 // columns each), P over it; where S's tiles are late, P . V does not wait for it.
-__device__ __forceinline__ void tt_issue_one(TtSmem<1>& S, const TreeTcParams& P, TtSeg seg, bool more) {
-  constexpr int SLOTS = TtSmem<1>::SLOTS;
+template <int D>
+__device__ __forceinline__ void tt_issue_one(TtSmem<1, D>& S, const TreeTcParams& P, TtSeg seg, bool more) {
+  constexpr int SLOTS = TtSmem<1, D>::SLOTS;
   const uint32_t kv0 = smem_addr(S.kv[0][0]), q0 = smem_addr(S.q[0][0]), tm = S.tmem;
   TtSeg back = seg;
   int ahead = seg.j1 - seg.j0, behind = ahead;       // pages left of the segments of S and of P . V
@@ -424,7 +432,7 @@ __device__ __forceinline__ void tt_issue_one(TtSmem<1>& S, const TreeTcParams& P
     idle = 0;
     tc_fence_after();
     if (s_go) {
-      tt_mma_s(tm + 128u * (a & 1u), q0, kv0 + (ki % SLOTS) * 32768u, TT_ID_S);
+      tt_mma_s<D>(tm + 128u * (a & 1u), q0, kv0 + (ki % SLOTS) * TtSmem<1, D>::TILE, TT_ID_S);
       tc_commit_warp(&S.sfull[a & 1u]);
       tc_commit_warp(&S.empty[ki % SLOTS]);
       ++a;
@@ -436,7 +444,7 @@ __device__ __forceinline__ void tt_issue_one(TtSmem<1>& S, const TreeTcParams& P
       }
       continue;
     }
-    tt_mma_o(tm + 256u, tm + 128u * (c & 1u), 64u, kv0 + (vi % SLOTS) * 32768u, acc);
+    tt_mma_o<D>(tm + 256u, tm + 128u * (c & 1u), 64u, kv0 + (vi % SLOTS) * TtSmem<1, D>::TILE, acc);
     tc_commit_warp(&S.oready[c & 1u]);
     tc_commit_warp(&S.empty[vi % SLOTS]);
     ++c;
@@ -456,15 +464,16 @@ __device__ __forceinline__ void tt_issue_one(TtSmem<1>& S, const TreeTcParams& P
 // next page's first half goes there before this page's P is made.  The tiles take turns in a fixed
 // order, half a page apart: left to themselves they fall into step, and softmax and tensor cores
 // wait for one another (8 rows of 64 nodes over 16384 keys: 171 us instead of 167).
-__device__ __forceinline__ void tt_issue_pair(TtSmem<2>& S, const TreeTcParams& P, TtSeg seg, bool more) {
-  constexpr int SLOTS = TtSmem<2>::SLOTS;
+template <int D>
+__device__ __forceinline__ void tt_issue_pair(TtSmem<2, D>& S, const TreeTcParams& P, TtSeg seg, bool more) {
+  constexpr int SLOTS = TtSmem<2, D>::SLOTS;
   const uint32_t kv0 = smem_addr(S.kv[0][0]), q0 = smem_addr(S.q[0][0]), tm = S.tmem;
   uint32_t g = 0, qn = 0;                            // page of the next P . V; segments done
   bool ok = true;
   // the first or second half of S of page i of tile x
   auto issue_s = [&](uint32_t x, uint32_t i, uint32_t half) {
-    tt_mma_s(tm + 128u * x + 64u * ((i + half) & 1u), q0 + x * 32768u,
-             kv0 + (2u * i % SLOTS) * 32768u + half * 8192u, TT_ID_H);
+    tt_mma_s<D>(tm + 128u * x + 64u * ((i + half) & 1u), q0 + x * TtSmem<1, D>::TILE,
+             kv0 + (2u * i % SLOTS) * TtSmem<1, D>::TILE + half * 8192u, TT_ID_H);
     tc_commit_warp(half ? &S.shi[x] : &S.slo[x]);
     if (half && x == 1u) tc_commit_warp(&S.empty[2u * i % SLOTS]);
   };
@@ -494,7 +503,7 @@ __device__ __forceinline__ void tt_issue_pair(TtSmem<2>& S, const TreeTcParams& 
         ok = tc_wait2_warp(&S.full[vi % SLOTS], (vi / SLOTS) & 1u, &S.pfull[x], g & 1u, &S.abort_);
         if (!ok) break;
         tc_fence_after();
-        tt_mma_o(tm + 256u + 128u * x, tm + 128u * x + 64u * (g & 1u), 32u, kv0 + (vi % SLOTS) * 32768u,
+        tt_mma_o<D>(tm + 256u + 128u * x, tm + 128u * x + 64u * (g & 1u), 32u, kv0 + (vi % SLOTS) * TtSmem<1, D>::TILE,
                  pages < seg.j1 - seg.j0);
         tc_commit_warp(&S.oready[x]);
         if (x == 1u) tc_commit_warp(&S.empty[vi % SLOTS]);
@@ -516,8 +525,8 @@ struct TtNodes {
 };
 // A thread's row r of tile ti: its node's bits to shared memory (asked for now, used in the
 // tree's pages), unless they are there.
-template <int NT>
-__device__ __forceinline__ void tt_ask_nodes(TtNodes& N, TtSmem<NT>& S, const TreeTcParams& P,
+template <int NT, int D>
+__device__ __forceinline__ void tt_ask_nodes(TtNodes& N, TtSmem<NT, D>& S, const TreeTcParams& P,
                                              const TtSeg& g, int ti, int r, bool live) {
   const TreeParams& T = P.T;
   if (N.p == g.p && (N.b == g.b || (N.b >= 0 && T.mask_bs == 0))) return;
@@ -535,8 +544,8 @@ __device__ __forceinline__ void tt_ask_nodes(TtNodes& N, TtSmem<NT>& S, const Tr
   N.b = g.b;
   N.p = g.p;
 }
-template <int NT>
-__device__ __forceinline__ void tt_settle(TtNodes& N, const TtSmem<NT>& S, const TreeTcParams& P,
+template <int NT, int D>
+__device__ __forceinline__ void tt_settle(TtNodes& N, const TtSmem<NT, D>& S, const TreeTcParams& P,
                                           const TtSeg& g, int ti, int r) {
   const TreeParams& T = P.T;
   const int lane = threadIdx.x & 31;
@@ -596,8 +605,8 @@ __device__ __forceinline__ void tt_rescale(uint32_t col, int n, float alpha) {
 }
 // Columns [32 q0, 32 q1) of a thread's row of O: divided by the row's sum and written out, or as
 // a piece.  oc: TMEM column of O (with the warp's lanes).
-template <int NT>
-__device__ __forceinline__ void tt_emit(TtSmem<NT>& S, const TreeTcParams& P, const TtSeg& g, int ti, int r,
+template <int NT, int D>
+__device__ __forceinline__ void tt_emit(TtSmem<NT, D>& S, const TreeTcParams& P, const TtSeg& g, int ti, int r,
                                         bool live, bool there, float m, float l, uint32_t oc, int q0, int q1) {
   const AttnParams& A = P.T.A;
   const bool whole = g.j0 == 0 && g.j1 + TT_OVH == g.tb;
@@ -605,7 +614,7 @@ __device__ __forceinline__ void tt_emit(TtSmem<NT>& S, const TreeTcParams& P, co
   const int jt = r / A.group, j = g.p * P.ni + P.nt * ti + jt, hq = g.h * A.group + r - jt * A.group;
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(A.out) + g.b * A.obs + j * A.oqs + hq * A.ohs;
   const int slot = 2 * (int)blockIdx.x + (g.j0 == 0), pr = P.nt * A.group * ti + r;
-  float4* part = P.pacc + (int64_t)slot * (TT_D / 4) * P.rs + pr;
+  float4* part = P.pacc + (int64_t)slot * (D / 4) * P.rs + pr;
 #pragma unroll 1
   for (int q = q0; q < q1; ++q) {
     uint32_t u[32];
@@ -637,8 +646,9 @@ __device__ __forceinline__ float tt_alpha(float m, float mn) {
 
 // Softmax of one tile: the threads of warpgroups 0 and 1 with the same lane own the same query
 // row, x takes the keys [64 x, 64 x + 64) of a page and half of the columns of O.
-__device__ __forceinline__ void tt_softmax_one(TtSmem<1>& S, const TreeTcParams& P, TtSeg seg, bool more) {
-  constexpr int SLOTS = TtSmem<1>::SLOTS;
+template <int D>
+__device__ __forceinline__ void tt_softmax_one(TtSmem<1, D>& S, const TreeTcParams& P, TtSeg seg, bool more) {
+  constexpr int SLOTS = TtSmem<1, D>::SLOTS;
   const TreeParams& T = P.T;
   const int t = threadIdx.x, w = t >> 5, x = w >> 2, wq = w & 3, r = t & 127;
   const uint32_t lcol = S.tmem + ((uint32_t)(32 * wq) << 16), ocol = lcol + 256u;
@@ -699,7 +709,7 @@ __device__ __forceinline__ void tt_softmax_one(TtSmem<1>& S, const TreeTcParams&
         const uint32_t vi = 2u * n + 1u;
         const int grp = 2 * x + (wq & 1);
         ok = tt_blank(S.kv[vi % SLOTS], T, nodes.uni, cur.base, end, key0 + 32 * grp, 32 * grp, wq >> 1,
-                      (wq >> 1) + 1, &S.full[vi % SLOTS], (vi / SLOTS) & 1u, &S.abort_);
+                      D == 128 ? (wq >> 1) + 1 : 1, &S.full[vi % SLOTS], (vi / SLOTS) & 1u, &S.abort_);
         if (!ok) break;
       }
       if (!dead) {
@@ -737,7 +747,7 @@ __device__ __forceinline__ void tt_softmax_one(TtSmem<1>& S, const TreeTcParams&
             ok = o_ready();
             if (!ok) break;
             tc_fence_after();
-            tt_rescale(ocol + 64u * x, 64, alpha);
+            tt_rescale(ocol + (D / 2) * x, D / 2, alpha);
           }
         }
         if (!ok) break;
@@ -756,15 +766,16 @@ __device__ __forceinline__ void tt_softmax_one(TtSmem<1>& S, const TreeTcParams&
       if (!ok) break;
       tc_fence_after();
       l = x ? lp + l : l + lp;                       // (the first warpgroup's half first, in both)
-      tt_emit(S, P, cur, 0, r, live, nodes.there, m, l, ocol, 2 * x, 2 * x + 2);
+      tt_emit(S, P, cur, 0, r, live, nodes.there, m, l, ocol, D / 64 * x, D / 64 * (x + 1));
     }
     tc_fence_before();
   }
 }
 
 // Softmax of two tiles: a thread owns its query row of tile x, warpgroup x.
-__device__ __forceinline__ void tt_softmax_pair(TtSmem<2>& S, const TreeTcParams& P, TtSeg seg, bool more) {
-  constexpr int SLOTS = TtSmem<2>::SLOTS;
+template <int D>
+__device__ __forceinline__ void tt_softmax_pair(TtSmem<2, D>& S, const TreeTcParams& P, TtSeg seg, bool more) {
+  constexpr int SLOTS = TtSmem<2, D>::SLOTS;
   const TreeParams& T = P.T;
   const int t = threadIdx.x, w = t >> 5, x = w >> 2, wq = w & 3, r = t & 127;
   const uint32_t lcol = S.tmem + ((uint32_t)(32 * wq) << 16) + 128u * x, ocol = lcol + 256u;
@@ -801,7 +812,7 @@ __device__ __forceinline__ void tt_softmax_pair(TtSmem<2>& S, const TreeTcParams
           if (!dead) tt_hide(S.mask[x][r], T, cur.base, end, key0 + 64 * half, 64, scol);
           if (half) {
             const uint32_t vi = 2u * n + 1u;
-            ok = tt_blank(S.kv[vi % SLOTS], T, nodes.uni, cur.base, end, key0 + 32 * wq, 32 * wq, 0, 2,
+            ok = tt_blank(S.kv[vi % SLOTS], T, nodes.uni, cur.base, end, key0 + 32 * wq, 32 * wq, 0, D / 64,
                           &S.full[vi % SLOTS], (vi / SLOTS) & 1u, &S.abort_);
             if (!ok) break;
           }
@@ -845,7 +856,7 @@ __device__ __forceinline__ void tt_softmax_pair(TtSmem<2>& S, const TreeTcParams
             ok = o_ready();
             if (!ok) break;
             tc_fence_after();
-            tt_rescale(ocol, 128, alpha);
+            tt_rescale(ocol, D, alpha);
           }
         }
         l += tt_weights(s0, s1, pk, m, sl2, wild);
@@ -861,19 +872,19 @@ __device__ __forceinline__ void tt_softmax_pair(TtSmem<2>& S, const TreeTcParams
       ok = o_ready();
       if (!ok) break;
       tc_fence_after();
-      tt_emit(S, P, cur, x, r, live, nodes.there, m, l, ocol, 0, 4);
+      tt_emit(S, P, cur, x, r, live, nodes.there, m, l, ocol, 0, D / 32);
     }
     tc_fence_before();
   }
 }
 
-template <int NT>
+template <int NT, int D>
 __global__ void __launch_bounds__(TT_THREADS, 1)
 tree_tc_kernel(const __grid_constant__ TreeTcParams P, const __grid_constant__ CUtensorMap tmk,
                const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmq) {
   extern __shared__ __align__(1024) unsigned char tt_raw[];
   const uint32_t pad = (1024u - (smem_addr(tt_raw) & 1023u)) & 1023u;   // swizzle atoms: 1024 B
-  TtSmem<NT>& S = *reinterpret_cast<TtSmem<NT>*>(tt_raw + pad);
+  TtSmem<NT, D>& S = *reinterpret_cast<TtSmem<NT, D>*>(tt_raw + pad);
   const TreeParams& T = P.T;
   const int t = threadIdx.x, w = t >> 5, lane = t & 31, cta = (int)blockIdx.x;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -883,7 +894,7 @@ tree_tc_kernel(const __grid_constant__ TreeTcParams P, const __grid_constant__ C
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (t == 256) {
-    for (int i = 0; i < TtSmem<NT>::SLOTS; ++i) {
+    for (int i = 0; i < TtSmem<NT, D>::SLOTS; ++i) {
       tc_bar_init(&S.full[i], 1);
       tc_bar_init(&S.empty[i], 1);
     }
@@ -906,7 +917,7 @@ tree_tc_kernel(const __grid_constant__ TreeTcParams P, const __grid_constant__ C
   for (int i = t; i < 2 * 2 * 128; i += TT_THREADS) S.peer[0][0][i] = 0ULL;     // (numbers start at 1)
   // the rows of a tile that no query fills stay 0
   const int filled = P.nt * T.A.group * 8;
-  for (int i = t; i < NT * 2 * 128 * 8; i += TT_THREADS)
+  for (int i = t; i < NT * (D / 64) * 128 * 8; i += TT_THREADS)
     if (i % 1024 >= filled) reinterpret_cast<uint4*>(S.q[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   int total, share;
@@ -969,13 +980,13 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
   const int4 cut = P.cut[c];
   if (__syncthreads_or(stop)) {
     // a wait gave up somewhere: say so in the output
-    const int64_t n = (int64_t)A.B * A.qlen * A.Hq * TT_D;
+    const int64_t n = (int64_t)A.B * A.qlen * A.Hq * A.D;
     const int64_t nt = (int64_t)gridDim.x * gridDim.y * gridDim.z * TJ_THREADS;
     const int64_t cta = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + c;
     for (int64_t i = cta * TJ_THREADS + t; i < n; i += nt) {
-      const int64_t v = i / TT_D, bj = v / A.Hq;
+      const int64_t v = i / A.D, bj = v / A.Hq;
       reinterpret_cast<__nv_bfloat16*>(A.out)[(bj / A.qlen) * A.obs + (bj % A.qlen) * A.oqs +
-                                              (v % A.Hq) * A.ohs + i % TT_D] =
+                                              (v % A.Hq) * A.ohs + i % A.D] =
           __float2bfloat16(CUDART_NAN_F);
     }
     return;
@@ -1004,7 +1015,7 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
       ml[i] = is ? __ldcg(&P.pml[slot * P.rs + r]) : make_float2(-CUDART_INF_F, 0.f);
 #pragma unroll
       for (int k = 0; k < NC; ++k)
-        v[i][k] = is ? __ldcg(P.pacc + (slot * (TT_D / 4) + col + k * (TJ_COLS / 4)) * P.rs + r)
+        v[i][k] = is ? __ldcg(P.pacc + (slot * (A.D / 4) + col + k * (TJ_COLS / 4)) * P.rs + r)
                      : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     float mx = gm;
@@ -1064,14 +1075,14 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
 
 // The shapes of the tensor-core path.
 static bool tt_fast(int dtype, int D, int group) {
-  return dtype == SD_DTYPE_BF16 && D == TT_D && group <= 128;
+  return dtype == SD_DTYPE_BF16 && (D == 64 || D == 128) && group <= 128;
 }
 
 struct TtLayout {
   size_t status, acc, ml, bytes;
   int np, ni, nt, rs;
 };
-static TtLayout tt_layout(int qlen, int group) {
+static TtLayout tt_layout(int qlen, int group, int D) {
   TtLayout L;
   // items of up to two tiles of whole nodes, of about the same size, and so their tiles
   const int most = TT_TILE / group;
@@ -1082,27 +1093,27 @@ static TtLayout tt_layout(int qlen, int group) {
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   size_t o = up(TT_CTAS * sizeof(int4));
   L.status = o; o = up(o + TT_CTAS * sizeof(int));
-  L.acc = o; o = up(o + (size_t)2 * TT_CTAS * L.rs * TT_D * sizeof(float));
+  L.acc = o; o = up(o + (size_t)2 * TT_CTAS * L.rs * D * sizeof(float));
   L.ml = o; o = up(o + (size_t)2 * TT_CTAS * L.rs * 2 * sizeof(float));
   L.bytes = o;
   return L;
 }
 
-template <int NT>
+template <int NT, int D>
 static int launch_tc(const TreeTcParams& P, const CUtensorMap& mk, const CUtensorMap& mv,
                      const CUtensorMap& mq, cudaStream_t st) {
-  const int sm = (int)sizeof(TtSmem<NT>) + 1024;   // room to align
+  const int sm = (int)sizeof(TtSmem<NT, D>) + 1024;   // room to align
   static std::atomic<uint64_t> ready{0};             // devices whose kernel may use that much
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return SD_ELAUNCH;
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (!(ready.load() & bit) || !bit) {
-    if (cudaFuncSetAttribute(tree_tc_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) !=
+    if (cudaFuncSetAttribute(tree_tc_kernel<NT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) !=
         cudaSuccess)
       return SD_ELAUNCH;
     ready.fetch_or(bit);
   }
-  tree_tc_kernel<NT><<<TT_CTAS, TT_THREADS, sm, st>>>(P, mk, mv, mq);
+  tree_tc_kernel<NT, D><<<TT_CTAS, TT_THREADS, sm, st>>>(P, mk, mv, mq);
   return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
 }
 
@@ -1115,7 +1126,7 @@ static int tree_tc(TreeTcParams& P, void* workspace, size_t workspace_bytes, cud
   if ((A.B > 1 && A.qbs <= 0) || (A.Hq > 1 && A.qhs <= 0) || (A.qlen > 1 && A.qqs <= 0)) return SD_EINVAL;
   const int64_t rows = A.bt ? (int64_t)A.npages * A.Hkv * SD_KV_PAGE : (int64_t)A.B * A.Hkv * A.C;
   if (rows >= (int64_t)1 << 31) return SD_ENOTSUP;   // a TMA coordinate
-  const TtLayout L = tt_layout(A.qlen, A.group);
+  const TtLayout L = tt_layout(A.qlen, A.group, A.D);
   // the schedule counts units in 32 bits
   const int64_t tiles = ((int64_t)A.C + SD_KV_PAGE - 1) / SD_KV_PAGE + TT_OVH;
   if (tiles * A.B > (0x7FFFFFFF - TT_CTAS) / ((int64_t)A.Hkv * L.np)) return SD_ENOTSUP;
@@ -1130,12 +1141,16 @@ static int tree_tc(TreeTcParams& P, void* workspace, size_t workspace_bytes, cud
   P.out_vec = (reinterpret_cast<uintptr_t>(A.out) & 15) == 0 && A.obs % 8 == 0 && A.oqs % 8 == 0 &&
               A.ohs % 8 == 0;
   CUtensorMap mk, mv, mq;
-  if (!cache_map(&mk, A.k, rows) || !cache_map(&mv, A.v, rows)) return SD_ENOTSUP;
+  if (!cache_map(&mk, A.k, rows, SD_KV_PAGE, A.D) || !cache_map(&mv, A.v, rows, SD_KV_PAGE, A.D)) return SD_ENOTSUP;
   // the queries of a tile: 64 columns of `group` heads of L.nt nodes of a row
-  const int64_t sizes[4] = {TT_D, A.Hq, A.qlen, A.B}, strides[3] = {A.qhs, A.qqs, A.qbs};
+  const int64_t sizes[4] = {A.D, A.Hq, A.qlen, A.B}, strides[3] = {A.qhs, A.qqs, A.qbs};
   const int box[4] = {64, A.group, L.nt, 1};
   if (!tile_map(&mq, A.q, sizes, strides, box)) return SD_ENOTSUP;
-  if (int rc = L.nt < L.ni ? launch_tc<2>(P, mk, mv, mq, st) : launch_tc<1>(P, mk, mv, mq, st)) return rc;
+  const int rc = A.D == 64 ? L.nt < L.ni ? launch_tc<2, 64>(P, mk, mv, mq, st)
+                                         : launch_tc<1, 64>(P, mk, mv, mq, st)
+                           : L.nt < L.ni ? launch_tc<2, 128>(P, mk, mv, mq, st)
+                                         : launch_tc<1, 128>(P, mk, mv, mq, st);
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1145,13 +1160,12 @@ static int tree_tc(TreeTcParams& P, void* workspace, size_t workspace_bytes, cud
   cfg.stream = st;
   cfg.blockDim = dim3(TJ_THREADS);
   // (at most as many items are cut as there are)
-  constexpr int blocks = TT_D / TJ_COLS;
+  const int blocks = A.D / TJ_COLS;
   const int64_t cut = std::min<int64_t>(TT_CTAS, (int64_t)A.B * A.Hkv * L.np) * (L.rs / TJ_ROWS) * blocks;
   const bool few = cut <= TT_CTAS * 4;
   cfg.gridDim = dim3(TT_CTAS, (unsigned)(L.rs / TJ_ROWS), few ? blocks : 1);
-  if ((few ? cudaLaunchKernelEx(&cfg, tree_join_kernel<1>, P)
-           : cudaLaunchKernelEx(&cfg, tree_join_kernel<blocks>, P)) != cudaSuccess)
-    return SD_ELAUNCH;
+  const auto join = few ? tree_join_kernel<1> : blocks == 2 ? tree_join_kernel<2> : tree_join_kernel<4>;
+  if (cudaLaunchKernelEx(&cfg, join, P) != cudaSuccess) return SD_ELAUNCH;
   return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
 }
 
@@ -1164,7 +1178,7 @@ extern "C" {
 size_t sd_tree_attn_workspace_bytes(int B, int Hq, int Hkv, int D, int C, int qlen, int dtype) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || C <= 0 || qlen <= 0) return 0;
   if (!tt_fast(dtype, D, Hq / Hkv) || (int64_t)qlen * (Hq / Hkv) > 0x7FFFFFFF) return 0;
-  return tt_layout(qlen, Hq / Hkv).bytes;
+  return tt_layout(qlen, Hq / Hkv, D).bytes;
 }
 
 int sd_tree_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const void* kcache,

@@ -1,5 +1,5 @@
 // Tree attention on the CUDA cores (sm_100a): the shapes that the tensor-core
-// kernel does not take (fp32, head sizes other than 128, very wide head groups).
+// kernel does not take (fp32, head sizes other than 64 and 128, very wide head groups).
 //
 // A cluster of S CTAs holds TR_ROWS query rows (node, head) of one (row, kv head).
 // The keys go out in groups of 32 to the cluster's 8 S warps in turn.  Per group
@@ -14,8 +14,8 @@
 // Bound by latency for few rows (so S grows while the machine has room), else by
 // the products: each K and V element meets TR_ROWS query rows.  8 rows of 9 nodes over up
 // to 460 fp32 keys of 64: 13.1 us, about eight dependent trips to memory; 32 rows of 26 nodes
-// over 2048 keys: 1.01 ms with fp32 heads of 64, 1.84 with 128, 1.17 with bf16 heads of 64
-// (14 to 15 TFLOP/s).  Two CTAs per SM, at 128 registers a thread, beat one with more of K
+// over 2048 keys: 1.01 ms with fp32 heads of 64, 1.84 with 128, 1.17 with bf16 in heads of 64
+// or a little less (12 to 15 TFLOP/s).  Two CTAs per SM, at 128 registers a thread, beat one with more of K
 // and V on the way (1.03, 2.36, 1.33 ms) and three (1.10, 2.02, 1.46).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

@@ -249,7 +249,7 @@ def tree_attention(q, k_cache, v_cache, lengths, masks, first=0, scale=None, out
     if not 0.0 < sc < 3e38:
         raise L.SpecdecError(f"scale must be positive and finite, got {scale}")
     qb, qh, ql, qd = q.stride()
-    if qd != 1 or (dt == torch.bfloat16 and D == 128 and (
+    if qd != 1 or (dt == torch.bfloat16 and D in (64, 128) and (
             q.data_ptr() % 16 or qb % 8 or qh % 8 or ql % 8 or not (qb and qh and ql))):
         q = q.contiguous()
         if q.data_ptr() % 16:

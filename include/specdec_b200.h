@@ -516,7 +516,7 @@ int sd_kv_commit_tree(void* const* bufs, int n_bufs, const int32_t* block_table,
  * contiguous cache, C its capacity; else pools, C is bt_stride * SD_KV_PAGE).
  * Slots that no node sees may hold anything; V in a slot that some node of the
  * tree sees has to be finite where other nodes of the row do not see it.
- * bf16 with D = 128 and Hq / Hkv <= 128 runs on the tensor cores (q, caches
+ * bf16 with D = 64 or 128 and Hq / Hkv <= 128 runs on the tensor cores (q, caches
  * 16-byte aligned, q strides positive multiples of 8); fp32 and other shapes with
  * D <= 128 on the CUDA cores, without a workspace.  scale > 0.  The workspace must be
  * 256-byte aligned and needs no initialisation; calls on two streams, or captured

@@ -258,6 +258,24 @@ def test_strides_scale_and_given_output(dtype, d):
 
 
 @gpu
+@pytest.mark.parametrize("hq,hkv", [(32, 8), (4, 4), (16, 2)])
+@pytest.mark.parametrize("n,first", [(1, 0), (9, 4), (33, 0), (64, 0), (65, 2), (TREE_MAX, 0)])
+@pytest.mark.parametrize("bases", [[0, 90, 129, 1037], [3000, 9000]])
+def test_heads_of_64(hq, hkv, n, first, bases):
+    g = torch.Generator().manual_seed(n)
+    parents = [_parents(n, g, missing=min(n - 1, b % 3)) for b in range(len(bases))]
+    _check(*_case(bases, parents, hq, hkv, 64, torch.bfloat16, first=first, paged=n % 2 == 0, seed=n))
+
+
+@gpu
+@pytest.mark.parametrize("scale_q", [1e3, 1e7, 1e12])
+def test_scores_of_every_size_with_heads_of_64(scale_q):
+    g = torch.Generator().manual_seed(19)
+    for n, hq in ((12, 8), (70, 16)):
+        _check(*_case([40, 700], [_parents(n, g)], hq, 2, 64, torch.bfloat16, scale_q=scale_q))
+
+
+@gpu
 @pytest.mark.parametrize("bases", [[70, 300], [2000, 5000]])
 def test_outputs_that_no_wide_store_reaches(bases):
     """Rows of an output that start 2 bytes past aligned addresses: whole and joined items."""
