@@ -163,6 +163,8 @@ class _Constraints:
         if sp.logit_bias:
             if len(sp.logit_bias) > BIAS_MAX:
                 raise ValueError(f"logit_bias has {len(sp.logit_bias)} tokens, at most {BIAS_MAX}")
+            if min(sp.logit_bias) < 0 or max(sp.logit_bias) >= vocab:
+                raise ValueError(f"logit_bias must name tokens in [0, {vocab})")
             self.kw["bias"] = (torch.tensor([list(sp.logit_bias)], dtype=torch.long, device=device),
                                torch.tensor([list(sp.logit_bias.values())], dtype=torch.float32,
                                             device=device))
@@ -524,6 +526,11 @@ class SpecDecodeEngine:
         con = _Constraints.of(sp, input_ids, plen, self.vocab_size, dev)
         if tree is not None:
             k_cap = len(tree_of_widths(tree)[0])
+            # a row ends with its last round's whole path, and a round holds all nodes
+            most = int(plen.max()) + int(max_new_tokens) + len(tree) + k_cap if B else 0
+            if most > self.capacity:
+                raise ValueError(f"trees of {k_cap} nodes need a capacity of {most} tokens per row "
+                                 f"here, got {self.capacity}")
         else:
             k_cap = int(k_fixed) if k_fixed is not None else int(getattr(controller, "k_max", 16))
         tcache = self._mk_cache(self.target, B, plen, max_new_tokens, k_cap, n)
@@ -589,6 +596,9 @@ class SpecDecodeEngine:
                     con.commit(rnd.tokens, n_acc + 1, path)
                 tcache.commit_tree(path, n_acc, rnd.nodes)
                 dcache.commit_tree(path, n_acc, rnd.nodes)
+                if any(done_l):                      # a row that is done does not grow
+                    for cache in (tcache, dcache):
+                        cache.lengths.sub_((~alive).long())
                 nodes = path.long().clamp_min(0)
                 # the path's drafts, then y; -1 past that
                 at = torch.arange(rnd.depth + 1, device=dev).view(1, -1)

@@ -245,6 +245,32 @@ def test_several_samples_with_penalties(pair):
         assert all(out[b][:16] == ar[b // 2][:16] for b in range(8)), how
 
 
+@pytest.mark.parametrize("paged", [False, True])
+def test_rows_that_are_done_do_not_grow_and_the_capacity_is_enough(pair, paged):
+    """A row that ends after a few tokens waits for the others with the length it has, and the
+    smallest capacity that is not refused gives the same tokens."""
+    ids, plen = _prompts()
+    sp, tree, new = SamplingConfig(temperature=0.0), (3, 2), 40
+    nodes = len(tree_of_widths(tree)[0])
+    need = int(plen.max()) + new + len(tree) + nodes
+    eng = SpecDecodeEngine(*pair, TinyTok(), device=DEV, capacity=need, paged_kv=paged)
+    free, _ = eng.generate(ids, plen, new, sampling=sp, tree=tree)
+    caches = []
+    make = eng._mk_cache
+    eng._mk_cache = lambda *a, **k: caches.append(make(*a, **k)) or caches[-1]
+    eng.eos_ids = {free[0][3]}
+    out, st = eng.generate(ids, plen, new, sampling=sp, tree=tree)
+    for b in range(4):
+        cut = next((i + 1 for i, t in enumerate(free[b][:new]) if t in eng.eos_ids), new)
+        assert out[b][:cut] == free[b][:cut] and len(out[b]) == cut
+        for c in caches:
+            assert int(c.lengths[b]) <= int(plen[b]) + cut + len(tree)
+    assert len(out[0]) <= 4 and st.rounds > 4
+    small = SpecDecodeEngine(*pair, TinyTok(), device=DEV, capacity=need - 1, paged_kv=paged)
+    with pytest.raises(ValueError, match="capacity"):
+        small.generate(ids, plen, new, sampling=sp, tree=tree)
+
+
 def test_refusals(pair):
     eng = SpecDecodeEngine(*pair, TinyTok(), device=DEV, capacity=160)
     ids, plen = _prompts()
@@ -254,7 +280,8 @@ def test_refusals(pair):
             eng.generate(ids, plen, 8, **kw)
     for bad in (dict(repetition_penalty=0.0), dict(repetition_penalty=-1.0),
                 dict(repetition_penalty=math.inf), dict(allowed_tokens=[]),
-                dict(allowed_tokens=[VOCAB]), dict(logit_bias={i: 1.0 for i in range(2000)})):
+                dict(allowed_tokens=[VOCAB]), dict(logit_bias={i: 1.0 for i in range(2000)}),
+                dict(logit_bias={VOCAB: 1.0}), dict(logit_bias={-1: 1.0})):
         with pytest.raises(ValueError):
             eng.generate(ids, plen, 8, sampling=SamplingConfig(**bad), k_fixed=2)
     with pytest.raises(Exception):
