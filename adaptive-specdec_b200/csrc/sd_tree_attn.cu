@@ -1119,11 +1119,11 @@ static int launch_tc(const TreeTcParams& P, const CUtensorMap& mk, const CUtenso
 
 static int tree_tc(TreeTcParams& P, void* workspace, size_t workspace_bytes, cudaStream_t st) {
   AttnParams& A = P.T.A;
-  // TMA boxes of the queries and the caches
-  if ((reinterpret_cast<uintptr_t>(A.q) & 15) || A.qbs % 8 || A.qhs % 8 || A.qqs % 8 ||
+  // TMA boxes of the queries (the stride of a dimension of one is any) and the caches
+  auto odd = [](int n, int64_t stride) { return n > 1 && (stride <= 0 || stride % 8); };
+  if ((reinterpret_cast<uintptr_t>(A.q) & 15) || odd(A.B, A.qbs) || odd(A.Hq, A.qhs) || odd(A.qlen, A.qqs) ||
       (reinterpret_cast<uintptr_t>(A.k) & 15) || (reinterpret_cast<uintptr_t>(A.v) & 15))
     return SD_EINVAL;
-  if ((A.B > 1 && A.qbs <= 0) || (A.Hq > 1 && A.qhs <= 0) || (A.qlen > 1 && A.qqs <= 0)) return SD_EINVAL;
   const int64_t rows = A.bt ? (int64_t)A.npages * A.Hkv * SD_KV_PAGE : (int64_t)A.B * A.Hkv * A.C;
   if (rows >= (int64_t)1 << 31) return SD_ENOTSUP;   // a TMA coordinate
   const TtLayout L = tt_layout(A.qlen, A.group, A.D);

@@ -250,7 +250,7 @@ def tree_attention(q, k_cache, v_cache, lengths, masks, first=0, scale=None, out
         raise L.SpecdecError(f"scale must be positive and finite, got {scale}")
     qb, qh, ql, qd = q.stride()
     if qd != 1 or (dt == torch.bfloat16 and D in (64, 128) and (
-            q.data_ptr() % 16 or qb % 8 or qh % 8 or ql % 8 or not (qb and qh and ql))):
+            q.data_ptr() % 16 or any(n > 1 and (x % 8 or not x) for n, x in zip(q.shape, (qb, qh, ql))))):
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()

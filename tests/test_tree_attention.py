@@ -298,6 +298,20 @@ def test_broadcast_queries_and_masks(dtype, d):
 
 
 @gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_any_stride_of_dimensions_of_one(d):
+    g = torch.Generator().manual_seed(20)
+    call, kw, ref = _case([33], [_parents(6, g)], 1, 1, d, torch.bfloat16)
+    q = call[0]
+    assert q.shape == (1, 1, 6, d)
+    rows = q[0, 0].contiguous()
+    _check((rows.as_strided((1, 1, 6, d), (3, 5, d, 1)),) + call[1:], kw, ref)
+    call, kw, ref = _case([33, 200], [[-1]], 4, 2, d, torch.bfloat16)
+    q = call[0].contiguous()
+    _check((q.as_strided((2, 4, 1, d), (4 * d, d, 7, 1)),) + call[1:], kw, ref)
+
+
+@gpu
 @pytest.mark.parametrize("hq,hkv", [(5, 1), (71, 1), (128, 1), (129, 1), (40, 8), (192, 3)])
 @pytest.mark.parametrize("n", [1, 3, 20])
 def test_head_groups_of_every_size(hq, hkv, n):
