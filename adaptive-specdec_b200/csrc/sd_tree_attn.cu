@@ -920,6 +920,7 @@ tree_tc_kernel(const __grid_constant__ TreeTcParams P, const __grid_constant__ C
   for (int i = t; i < NT * (D / 64) * 128 * 8; i += TT_THREADS)
     if (i % 1024 >= filled) reinterpret_cast<uint4*>(S.q[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");         // what the kernel before this one wrote
   int total, share;
   tt_plan(S, P, &total, &share);
   tc_fence_before();
@@ -975,6 +976,7 @@ __global__ void __launch_bounds__(TJ_THREADS) tree_join_kernel(const __grid_cons
   const AttnParams& A = T.A;
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   const int c = (int)blockIdx.x;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int stop = t < TT_CTAS ? P.status[t] : 0;
   const int4 cut = P.cut[c];
@@ -1113,7 +1115,18 @@ static int launch_tc(const TreeTcParams& P, const CUtensorMap& mk, const CUtenso
       return SD_ELAUNCH;
     ready.fetch_or(bit);
   }
-  tree_tc_kernel<NT, D><<<TT_CTAS, TT_THREADS, sm, st>>>(P, mk, mv, mq);
+  // (its start, up to the first read of memory, beside the end of the kernel before it)
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = st;
+  cfg.gridDim = dim3(TT_CTAS);
+  cfg.blockDim = dim3(TT_THREADS);
+  cfg.dynamicSmemBytes = sm;
+  if (cudaLaunchKernelEx(&cfg, tree_tc_kernel<NT, D>, P, mk, mv, mq) != cudaSuccess) return SD_ELAUNCH;
   return cudaGetLastError() == cudaSuccess ? SD_OK : SD_ELAUNCH;
 }
 
