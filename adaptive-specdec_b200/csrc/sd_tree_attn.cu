@@ -15,9 +15,9 @@
 //
 // What bounds it.  K and V are read once for all nodes and heads, so up to 128 query
 // rows it is HBM: 32 rows of 26 nodes over 128 to 4096 keys (294 MB) take 64 us in a graph,
-// 5.1 TB/s in the main kernel, and a start (plan, first loads) and join of 3 and 7 us;
-// 2 rows of 33 nodes over 30011 keys (246 MB) 58 us.  With two tiles it is the chain of S,
-// softmax and P V of a tile: 64 rows of 64 nodes over 512 to 8192 keys take 341 us, the
+// 5.1 TB/s in the main kernel, and a start (plan, first loads) and join of 3 and 6 us;
+// 2 rows of 33 nodes over 30011 keys (246 MB) 50 to 59 us.  With two tiles it is the chain of S,
+// softmax and P V of a tile: 64 rows of 64 nodes over 512 to 8192 keys take 330 us, the
 // tensor pipe is busy 47 % of the time.  (The CUDA-core kernel: 20.2 ms.)
 // One tile: S of the next page stands ready in TMEM's second buffer, and its 128 columns go
 // to two warpgroups, so that a page's softmax takes half as long.  Two tiles: S and O of both

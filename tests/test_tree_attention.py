@@ -395,6 +395,60 @@ def test_the_same_result_on_every_run_stream_and_replay():
 
 
 @gpu
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("bases", [[40, 7], [3000, 9000]])
+def test_inputs_that_kernels_before_it_or_another_stream_still_write(bases, captured):
+    """The kernel starts beside the end of the one before it, and reads nothing until that and
+    whatever its stream waits for are done."""
+    g = torch.Generator().manual_seed(21)
+    call, kw, ref = _case(bases, [_parents(9, g)], 8, 2, 128, torch.bfloat16)
+    q, k, v, lengths, masks = call
+    src = [t.clone() for t in (q, k, v, lengths, masks)]
+    live = [torch.zeros_like(t) for t in src]
+    side = torch.cuda.Stream()
+    main = torch.cuda.Stream()
+
+    def body():
+        cur = torch.cuda.current_stream()
+        side.wait_stream(cur)
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(400000)
+            live[1].copy_(src[1])
+            live[4].copy_(src[4])
+        live[2].copy_(src[2])
+        cur.wait_stream(side)
+        first = A.tree_attention(src[0], live[1], live[2], src[3], live[4], **kw)
+        torch.cuda._sleep(400000)
+        live[0].copy_(src[0])
+        live[3].copy_(src[3])
+        second = A.tree_attention(live[0], live[1], live[2], live[3], live[4], **kw)
+        third = A.tree_attention(second.transpose(1, 2), live[1], live[2], live[3], live[4], **kw)
+        for t in live:
+            t.zero_()                                  # the calls have read them
+        return first, second, third
+
+    main.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(main):
+        if captured:
+            body()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=main):
+                outs = body()
+            for _ in range(3):
+                for t in live:
+                    t.zero_()
+                graph.replay()
+        else:
+            outs = body()
+    torch.cuda.synchronize()
+    for got in outs[:2]:
+        _compare(got, q, ref, kw["first"])
+    assert torch.equal(outs[0], outs[1])
+    _compare(outs[2], outs[1].transpose(1, 2), ref, kw["first"])
+
+
+@gpu
 def test_chains_match_verify_attention():
     """A chain of drafts is the tree that verify_attention computes."""
     n = 5
