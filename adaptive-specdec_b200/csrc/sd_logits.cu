@@ -386,6 +386,8 @@ int sd_process_logits(const void* logits, int64_t bs, int64_t ps, int dtype, int
   const bool inplace = a0 < b1 && b0 < a1;
   // the same elements, or memory that a position may be read from after it was written
   if (inplace && (logits != out || (B > 1 && bs != out_bs) || (L > 1 && ps != out_ps))) return SD_EINVAL;
+  // one CTA per entry of the output
+  if (!rows_apart<2>(V, {B, L}, {out_bs, out_ps})) return SD_EINVAL;
   if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & (size - 1)) return SD_EINVAL;
   // a chunk is up to 4 units per thread, and a CTA takes up to 8 positions, less where that would
   // leave SMs without a CTA: first the positions, then the chunk

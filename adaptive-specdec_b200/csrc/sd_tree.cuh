@@ -51,6 +51,24 @@ __device__ __forceinline__ bool tree_present(const int32_t* m, int W, int N) {
   return any != 0;
 }
 
+// Whether rows of `row` elements, sizes[i] of them at strides[i] (elements), share none: in
+// order of the strides, each steps over all that the smaller ones reach.  (So are all views
+// of a dense tensor that do not expand or unfold it; the stride of a dimension of one is any.)
+template <int N>
+bool rows_apart(int64_t row, const int64_t (&sizes)[N], const int64_t (&strides)[N]) {
+  int order[N];
+  for (int i = 0; i < N; ++i) order[i] = i;
+  auto step = [&](int i) { return (__int128)(strides[i] < 0 ? -(__int128)strides[i] : strides[i]); };
+  std::sort(order, order + N, [&](int a, int b) { return step(a) < step(b); });
+  __int128 reach = row;
+  for (int i : order) {
+    if (sizes[i] <= 1) continue;
+    if (step(i) < reach) return false;
+    reach += (sizes[i] - 1) * step(i);
+  }
+  return true;
+}
+
 // sd_tree_rows.cu: tree attention on the CUDA cores, D <= 128
 int tree_rows(const TreeParams& P, int dtype, cudaStream_t st);
 

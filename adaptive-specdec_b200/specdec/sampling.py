@@ -452,7 +452,8 @@ def process_logits(logits, tokens=None, masks=None, history=None, repetition=Non
     [0, V) are padding, biases of one id add up; at most BIAS_MAX per row and
     TREE_MAX tokens.  repetition > 0.  Returns a new tensor, or ``out`` ([B, L, V]): the
     logits themselves, or memory outside the span from their first to their last
-    entry (anything else is refused).  One launch, no synchronisation.
+    entry; anything else is refused, and so is an ``out`` whose rows share entries
+    (an expanded tensor).  One launch, no synchronisation.
     """
     dev = logits.device
     if not logits.is_cuda:

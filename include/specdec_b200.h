@@ -217,11 +217,12 @@ int sd_token_logprobs(const void* logits, int64_t bs, int64_t ps, int dtype, con
  *   if bit t % 32 of allowed[b, l, t / 32] is 0: x = -inf
  * in float32, rounded once to out[b, l, t]: the logits themselves (same address and
  * strides), or memory outside the span from their first to their last entry, else
- * SD_EINVAL.  history NULL: no penalties (the three [B] arrays are then unused; each
- * may be NULL by itself: neutral); bias_ids NULL: no bias (an id outside [0, V) is
- * padding); allowed NULL: no mask.  bias_bs / allowed_bs / allowed_ps may be 0
- * (one list / mask for all rows / positions).  A drafted token outside [0, V) is
- * padding.  M <= SD_BIAS_MAX.
+ * SD_EINVAL; so are rows of out that share entries (strides in order of size, each
+ * must step over all that the smaller ones reach).  history NULL: no penalties (the
+ * three [B] arrays are then unused; each may be NULL by itself: neutral); bias_ids
+ * NULL: no bias (an id outside [0, V) is padding); allowed NULL: no mask.  bias_bs /
+ * allowed_bs / allowed_ps may be 0 (one list / mask for all rows / positions).  A
+ * drafted token outside [0, V) is padding.  M <= SD_BIAS_MAX.
  */
 #define SD_BIAS_MAX 1024
 int sd_process_logits(const void* logits, int64_t bs, int64_t ps, int dtype, int B, int L, int V,

@@ -375,3 +375,42 @@ def test_refused_on_the_host():
               lambda: TokenHistory.over(torch.zeros(1, 4, dtype=torch.int16))):
         with pytest.raises(L.SpecdecError):
             f()
+
+
+def _out_strides(**kw):
+    """rc of a call whose output has these sizes and strides (refused before any launch)."""
+    a = dict(x=1 << 20, xbs=64, xps=8, B=1, L=1, V=8, out=1 << 24, bs=8, ps=8)
+    a.update(kw)
+    return L.lib().sd_process_logits(a["x"], a["xbs"], a["xps"], 0, a["B"], a["L"], a["V"], None, 0,
+                                     None, 0, 0, 0, None, 0, None, None, None, None, None, 0, 0, None,
+                                     0, 0, a["out"], a["bs"], a["ps"], None)
+
+
+def test_outputs_that_overlap_themselves_are_refused_on_the_host():
+    """Rows or positions of the output that share entries: several CTAs would write them."""
+    same = dict(x=1 << 24)                               # in place
+    for kw in (dict(B=2, bs=0), dict(L=2, ps=0), dict(B=2, bs=7), dict(L=2, ps=7), dict(B=2, bs=-7),
+               dict(B=2, L=3, bs=16, ps=8), dict(B=3, L=2, bs=8, ps=16), dict(B=2, L=2, bs=12, ps=8),
+               dict(B=2, bs=0, xbs=0, **same), dict(L=4, ps=0, xps=0, **same),
+               dict(B=2, L=2, bs=8, ps=8, xbs=8, xps=8, **same)):
+        assert _out_strides(**kw) == -22, kw
+
+
+@gpu
+def test_outputs_that_overlap_themselves_are_refused():
+    x = torch.randn(3, 2, 40, device=DEV)
+    room = torch.zeros(400, device=DEV)
+    for out in (room[:80].view(1, 2, 40).expand(3, -1, -1), room[:120].view(3, 1, 40).expand(-1, 2, -1),
+                room.as_strided((3, 2, 40), (60, 40, 1)), room.as_strided((3, 2, 40), (40, 39, 1))):
+        with pytest.raises(L.SpecdecError):
+            process_logits(x, out=out)
+    for same in (x[:1].expand(3, -1, -1), x[:, :1].expand(-1, 2, -1)):
+        before = x.clone()
+        with pytest.raises(L.SpecdecError):
+            process_logits(same, out=same)
+        assert torch.equal(x, before)
+        assert torch.equal(process_logits(same), same)   # (as an input they are good)
+    turned = torch.zeros(2, 3, 40, device=DEV).transpose(0, 1)
+    assert torch.equal(process_logits(x, out=turned), x)
+    one = room.as_strided((1, 2, 40), (0, 50, 1))        # the stride of a single row is any
+    assert torch.equal(process_logits(x[:1], out=one), x[:1])
