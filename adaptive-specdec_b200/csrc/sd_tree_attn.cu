@@ -1206,7 +1206,7 @@ int sd_tree_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const voi
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || first + qlen > N) return SD_EINVAL;
   if (!(scale > 0.f) || scale > 3e38f) return SD_EINVAL;
   if (dtype != SD_DTYPE_BF16 && dtype != SD_DTYPE_F32) return SD_ENOTSUP;
-  if (N > SD_TREE_MAX) return SD_ENOTSUP;
+  if (N > SD_TREE_MAX || D > 128) return SD_ENOTSUP;
   if (block_table) {
     if (bt_stride <= 0 || npages <= 0) return SD_EINVAL;
     if ((int64_t)bt_stride * SD_KV_PAGE > 0x7FFFFFFF) return SD_ENOTSUP;
@@ -1218,6 +1218,8 @@ int sd_tree_attn(const void* q, int64_t qbs, int64_t qhs, int64_t qqs, const voi
   const int group = Hq / Hkv;
   const int64_t R = (int64_t)qlen * group;
   if (R > 0x7FFFFFFF) return SD_ENOTSUP;
+  // one CTA per entry of the output
+  if (!rows_apart<3>(D, {B, qlen, Hq}, {obs, oqs, ohs})) return SD_EINVAL;
   TreeTcParams P = {};
   AttnParams& A = P.T.A;
   A.q = q; A.qbs = qbs; A.qhs = qhs; A.qqs = qqs;

@@ -254,7 +254,6 @@ static int tree_rows_of(const TreeParams& P, int blocks, int S, cudaStream_t st)
 }
 
 int tree_rows(const TreeParams& P, int dtype, cudaStream_t st) {
-  if (P.A.D > 128) return SD_ENOTSUP;
   const int64_t blocks = ((int64_t)P.A.R + TR_ROWS - 1) / TR_ROWS, units = blocks * P.A.B * P.A.Hkv;
   // CTAs up to two per SM, and no more than the cache has groups of keys for
   int S = 1;

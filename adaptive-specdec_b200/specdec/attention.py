@@ -205,7 +205,9 @@ def tree_attention(q, k_cache, v_cache, lengths, masks, first=0, scale=None, out
     those of its ancestors and itself, lengths[b] - first + a for every bit a of
     ``masks`` [N, W] or [B, N, W] (``tree_masks``).  A node without a bit gives 0.
     Slots that no node sees may hold anything; V has to be finite in the slots that
-    some of the row's nodes see and others do not.  bf16 and fp32.
+    some of the row's nodes see and others do not.  bf16 and fp32.  ``out`` lies in
+    memory of its own, contiguous along D; one whose heads share entries (an
+    expanded tensor) is refused.
     """
     dev, dt = q.device, q.dtype
     if not q.is_cuda:

@@ -519,7 +519,9 @@ int sd_kv_commit_tree(void* const* bufs, int n_bufs, const int32_t* block_table,
  * tree sees has to be finite where other nodes of the row do not see it.
  * bf16 with D = 64 or 128 and Hq / Hkv <= 128 runs on the tensor cores (q, caches
  * 16-byte aligned, q strides positive multiples of 8); fp32 and other shapes with
- * D <= 128 on the CUDA cores, without a workspace.  scale > 0.  The workspace must be
+ * D <= 128 on the CUDA cores, without a workspace.  scale > 0.  Heads of out that share
+ * entries are SD_EINVAL (strides in order of size, each must step over all that the
+ * smaller ones reach); out does not overlap what the call reads.  The workspace must be
  * 256-byte aligned and needs no initialisation; calls on two streams, or captured
  * into two graphs that may run at once, need one each.  If a bounded wait inside the
  * kernels gives up, the output is NaN.

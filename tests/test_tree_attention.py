@@ -537,3 +537,32 @@ def test_refused_on_the_host():
     with pytest.raises(L.SpecdecError):
         A.tree_attention(*[torch.zeros(1, 1, 1, 8)] * 3, torch.zeros(1).long(),
                          torch.ones(1, 1, dtype=torch.int32))
+
+
+def test_outputs_that_overlap_themselves_are_refused_on_the_host():
+    """Rows, nodes or heads of the output that share entries (refused before any launch)."""
+    lib = L.lib()
+
+    def call(obs, oqs, ohs, B=2, qlen=3, Hq=4, dtype=0):
+        return lib.sd_tree_attn(1 << 20, 96, 8, 32, 1 << 21, 1 << 22, None, 0, 0, 1 << 23, 1 << 24, 0, 4, 0,
+                                B, Hq, 2, 8, 64, qlen, 0.1, 1 << 25, obs, oqs, ohs, dtype, None, 0, None)
+    for strides in ((0, 32, 8), (96, 0, 8), (96, 32, 0), (96, 32, 7), (96, 24, 8), (88, 32, 8), (-88, 32, 8)):
+        assert call(*strides) == -22, strides
+    assert call(0, 8, 8, B=1, qlen=2, Hq=2) == -22
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float32, 64)])
+def test_outputs_that_overlap_themselves_are_refused(dtype, d):
+    g = torch.Generator().manual_seed(22)
+    call, kw, ref = _case([70, 300], [_parents(6, g)], 8, 2, d, dtype)
+    for i, shape in enumerate(((1, 6, 8, d), (2, 1, 8, d), (2, 6, 1, d))):
+        with pytest.raises(L.SpecdecError):
+            A.tree_attention(*call, out=torch.empty(shape, dtype=dtype, device=DEV).expand(2, 6, 8, d), **kw)
+    room = torch.empty(2 * 6 * 8 * d, dtype=dtype, device=DEV)
+    with pytest.raises(L.SpecdecError):
+        A.tree_attention(*call, out=room.as_strided((2, 6, 8, d), (5 * 8 * d, 8 * d, d, 1)), **kw)
+    for order in ((0, 1, 2, 3), (2, 1, 0, 3), (1, 2, 0, 3)):     # any order of the dimensions
+        out = torch.empty([(2, 6, 8, d)[i] for i in order], dtype=dtype, device=DEV)
+        back = [order.index(i) for i in range(4)]
+        _check(call, kw, ref, out=out.permute(back))
