@@ -292,7 +292,7 @@ class RaggedCache(Cache):
         self.valid = None
 
     def set_lengths(self, lengths):
-        self.valid = None
+        self.valid = self.tree = None
         t = torch.as_tensor(lengths, dtype=torch.long)
         if t.is_cuda:
             self.lengths.copy_(t)
@@ -321,6 +321,7 @@ class RaggedCache(Cache):
             d = n.to(torch.long).reshape(-1).contiguous()
             self._update(d, 0, -1)
             self._host_valid = False
+            self.tree = None
             return
         if isinstance(n, int):
             n_cpu = torch.full((self.batch_size,), n, dtype=torch.long)
@@ -333,6 +334,7 @@ class RaggedCache(Cache):
             raise RuntimeError("RaggedCache.rollback below zero")
         self._update(n_cpu.to(self.device, non_blocking=True), 0, -1)
         self._host = h - n_cpu
+        self.tree = None
 
     def commit(self, n_acc, k):
         """Verify-round commit: lengths -= k - n_acc (device n_acc, no sync)."""
@@ -341,13 +343,15 @@ class RaggedCache(Cache):
                                          self.batch_size, L.ptr(self._err),
                                          L.stream_ptr(self.device)), "kv commit")
         self._host_valid = False
+        self.tree = None
 
     # ---- trees of drafted tokens ---------------------------------------------
     def set_tree(self, masks=None, depths=None, first=0):
         """The next forwards are over nodes first, first + 1, ... of a drafted tree
-        (``specdec.tree.tree_masks``) whose earlier nodes the cache already holds;
-        without arguments they are over chains again.  Only the kernel attention
-        path (attn_impl "specdec_b200") knows trees."""
+        (``specdec.tree.tree_masks``) whose earlier nodes the cache already holds.
+        They are over chains again once the round ends, in commit_tree, commit,
+        rollback, set_lengths or reset, or by a call without arguments.  Only the
+        kernel attention path (attn_impl "specdec_b200") knows trees."""
         if masks is None:
             self.tree = None
             return
@@ -395,6 +399,7 @@ class RaggedCache(Cache):
 
     def reset(self):
         self.lengths.zero_()
+        self.tree = None
         self._host = torch.zeros(self.batch_size, dtype=torch.long)
         self._host_valid = True
         self._err.zero_()

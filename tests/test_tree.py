@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from specdec import _lib as L
+from specdec import attention as A
 from specdec.kvcache import PAGE, PagedRaggedCache, RaggedCache, commit_tree
 from specdec.tree import TREE_MAX, tree_accept, tree_masks, tree_of_widths
 
@@ -407,3 +408,51 @@ def test_refused_on_the_host():
                                   torch.zeros(1).long(), 1)):
         with pytest.raises(L.SpecdecError):
             f()
+
+
+@gpu
+@pytest.mark.parametrize("make", ["contiguous", "paged", "device pages"])
+@pytest.mark.parametrize("end", ["reset", "rollback", "rollback on the device", "set_lengths", "commit"])
+def test_a_tree_ends_with_its_round(make, end):
+    """A tree's forward that is not committed: what follows is a chain again, its positions by
+    place and every query behind the keys before it."""
+    g = torch.Generator().manual_seed(7)
+    masks, depths = tree_masks([-1, 0, 0, 1], device=DEV)
+    c = RaggedCache(1, 2, 256, DEV, attn_impl="specdec_b200") if make == "contiguous" else \
+        PagedRaggedCache(1, 2, 256, DEV, device_pages=make == "device pages")
+    x = [torch.randn(2, 2, 20, 16, generator=g).to(DEV) for _ in range(3)]
+
+    def forward(part):
+        n = part.stop - part.start
+        if make != "contiguous":
+            c.reserve(n)
+        assert c.attn_mask(n, torch.float32) is None
+        pos = c.positions(n)
+        keys, values = c.layers[0].update(x[1][:, :, part], x[2][:, :, part])
+        out, _ = A.hf_attention(None, x[0][:, :, part], keys, values, None, scaling=0.25)
+        c.advance(n)
+        return pos, out
+    forward(slice(0, 6))
+    c.set_tree(masks, depths)
+    forward(slice(6, 10))
+    base = 6
+    if end == "reset":
+        c.reset()
+        base = 0
+    elif end == "rollback":
+        c.rollback(4)
+    elif end == "rollback on the device":
+        c.rollback(torch.tensor([4, 4], device=DEV))
+    elif end == "commit":
+        c.commit(torch.tensor([0, 0], device=DEV), 4)
+    else:
+        c.set_lengths([6, 6])
+    assert c.tree is None
+    pos, out = forward(slice(12, 15))
+    assert pos.tolist() == [[base, base + 1, base + 2]] * 2
+    k, v = (torch.cat([t[:, :, :base], t[:, :, 12:15]], 2).double() for t in x[1:])
+    s = torch.einsum("bhqd,bhkd->bhqk", x[0][:, :, 12:15].double(), k) * 0.25
+    s.masked_fill_(torch.ones(3, base + 3, dtype=torch.bool, device=DEV).triu(base + 1), -torch.inf)
+    want = torch.einsum("bhqk,bhkd->bqhd", s.softmax(-1), v)
+    # fp32: at most 9 keys of |v| < 5, scores of 16 terms; 2^-18 for the powers of two
+    assert float((out.double() - want).abs().max()) <= 5 * 2.0 ** -16
