@@ -197,6 +197,14 @@ class _Constraints:
     def __call__(self, logits, tokens=None, masks=None, out=None):
         return process_logits(logits, tokens, masks, out=out, **self.kw)
 
+    def write(self, buf, logits, tokens):
+        """The processed logits into buf, whose type may be another one (a draft head's
+        logits need not be of the model's type)."""
+        if logits.dtype == buf.dtype:
+            self(logits, tokens, out=buf)
+        else:
+            buf.copy_(self(logits, tokens))
+
     def commit(self, tokens, counts=None, path=None):
         if self.history is not None:
             self.history.append(tokens, counts, path)
@@ -253,7 +261,7 @@ class _RoundGraphs:
                 self.drf_buf[:, i].copy_(logits)
             else:
                 self.path[:, i].copy_(self.feed.view(B))
-                self.con(logits.unsqueeze(1), self.path[:, :i + 1], out=self.drf_buf[:, i:i + 1])
+                self.con.write(self.drf_buf[:, i:i + 1], logits.unsqueeze(1), self.path[:, :i + 1])
             x, q = draft_sample(self.drf_buf[:, i], self.u[i], self.T, self.tp, self.tk)
             self.xs[:, i].copy_(x)
             self.qx[i].copy_(q)
@@ -696,7 +704,7 @@ class SpecDecodeEngine:
                             drf_buf[:, i].copy_(logits)
                         else:
                             before = torch.cat([pending.view(B, 1), xs[:, :i]], dim=1)
-                            con(logits.unsqueeze(1), before, out=drf_buf[:, i:i + 1])
+                            con.write(drf_buf[:, i:i + 1], logits.unsqueeze(1), before)
                         x, qx = draft_sample(drf_buf[:, i], u_draft[i], T, tp, tk)
                         xs[:, i] = x
                         feed = x.view(B, 1)

@@ -286,3 +286,22 @@ def test_refusals(pair):
             eng.generate(ids, plen, 8, sampling=SamplingConfig(**bad), k_fixed=2)
     with pytest.raises(Exception):
         process_logits(torch.zeros(1, 1, 4, device=DEV), repetition=1.0)
+
+
+@pytest.mark.parametrize("cuda_graphs", [True, False])
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_constraints_with_a_draft_head_of_another_type(cuda_graphs, temperature):
+    """A draft head that gives float32 logits of a bf16 model: the draft's logits end in bf16,
+    rounded once from the same float32 values, so the tokens are those of its own head."""
+    target, draft = _bf16_pair()
+    g = torch.Generator().manual_seed(6)
+    ids, plen = torch.randint(0, 300, (3, 40), generator=g), torch.tensor([40, 12, 33])
+    for kw in ({}, dict(repetition_penalty=1.2, frequency_penalty=0.1, logit_bias={5: 1.0})):
+        sp = SamplingConfig(temperature=temperature, **kw)
+        runs = []
+        for head in (None, lambda hidden, tokens: draft.lm_head(hidden).float()):
+            draft.specdec_head = head
+            eng = SpecDecodeEngine(target, draft, TinyTok(), device=DEV, capacity=256,
+                                   cuda_graphs=cuda_graphs)
+            runs.append(eng.generate(ids, plen, 12, sampling=sp, k_fixed=3, seed=1)[0])
+        assert runs[0] == runs[1]
