@@ -59,7 +59,7 @@ def tree_masks(parents, device=None):
         raise L.SpecdecError("tree_masks needs a CUDA device (no CPU fallback)")
     p = parents if parents.dim() == 2 else parents.unsqueeze(0)
     if p.dtype != torch.int32:
-        p = p.clamp(-2, TREE_MAX).to(torch.int32)
+        p = p.long().clamp(-2, TREE_MAX).to(torch.int32)     # (8 bits do not hold the limits)
     if p.stride(1) != 1:
         p = p.contiguous()
     T, N = p.shape

@@ -456,3 +456,14 @@ def test_a_tree_ends_with_its_round(make, end):
     want = torch.einsum("bhqk,bhkd->bqhd", s.softmax(-1), v)
     # fp32: at most 9 keys of |v| < 5, scores of 16 terms; 2^-18 for the powers of two
     assert float((out.double() - want).abs().max()) <= 5 * 2.0 ** -16
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64])
+def test_masks_of_parents_of_every_integer_type(dtype):
+    """(In an unsigned type no node is a root: 255 and 254 are no earlier nodes, so all are absent.)"""
+    trees = [[-1, 0, 0, 1, -2, 4, 2, 100, 3], [-1, -1, -2, 1, 0, 3, 5, 5, 8]]
+    parents = torch.tensor(trees).to(dtype)
+    want = [_masks_plain(t) for t in parents.tolist()]
+    got = tree_masks(parents, device=DEV)
+    assert _sets(got.masks) == [w[0] for w in want] and got.depths.tolist() == [w[1] for w in want]
