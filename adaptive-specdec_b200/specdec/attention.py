@@ -294,6 +294,11 @@ def hf_attention(module, query, key, value, attention_mask, dropout=0.0, scaling
     """transformers AttentionInterface function for RaggedCache buffers."""
     cache = getattr(key, "_sd_cache", None)
     if cache is not None:
+        bt, prefix = getattr(cache, "block_table", None), getattr(cache, "prefix", None)
+        if cache.tree is not None:                  # a drafted tree: nodes see their ancestors
+            masks, _, first = cache.tree
+            return tree_attention(query, key, value, cache.lengths, masks, first, scaling,
+                                  block_table=bt), None
         q_len = query.shape[2]
         if (cache.valid is not None and q_len > PREFILL_SDPA_MIN and cache._host_valid
                 and int(cache._host.max()) == 0):
@@ -301,7 +306,6 @@ def hf_attention(module, query, key, value, attention_mask, dropout=0.0, scaling
             # plain causal attention over the q new keys; a real token i < valid[b]
             # only sees keys s <= i, so the padding never reaches it.  Prefill is
             # outside the verify round; torch's SDPA (flash / cuDNN) runs it.
-            bt = getattr(cache, "block_table", None)
             if bt is not None:
                 ks, vs = gather_pages(key, bt, q_len), gather_pages(value, bt, q_len)
             else:
@@ -309,11 +313,6 @@ def hf_attention(module, query, key, value, attention_mask, dropout=0.0, scaling
             out = torch.nn.functional.scaled_dot_product_attention(
                 query, ks, vs, is_causal=True, scale=scaling, enable_gqa=True)
             return out.transpose(1, 2), None
-        bt, prefix = getattr(cache, "block_table", None), getattr(cache, "prefix", None)
-        if cache.tree is not None:                  # a drafted tree: nodes see their ancestors
-            masks, _, first = cache.tree
-            return tree_attention(query, key, value, cache.lengths, masks, first, scaling,
-                                  block_table=bt), None
         if prefix is not None:                      # a forked cache: rows share their prompt's pages
             return prefix_attention(query, key, value, cache.lengths, bt, *prefix,
                                     valid=cache.valid, scale=scaling), None

@@ -566,3 +566,24 @@ def test_outputs_that_overlap_themselves_are_refused(dtype, d):
         out = torch.empty([(2, 6, 8, d)[i] for i in order], dtype=dtype, device=DEV)
         back = [order.index(i) for i in range(4)]
         _check(call, kw, ref, out=out.permute(back))
+
+
+@gpu
+@pytest.mark.parametrize("n", [40, 70])
+@pytest.mark.parametrize("paged", [False, True])
+def test_a_tree_on_an_empty_cache_is_a_tree(n, paged):
+    """Through the caches, with a cap on the padding given, too: no causal shortcut."""
+    from specdec.kvcache import PagedRaggedCache, RaggedCache
+    g = torch.Generator().manual_seed(n)
+    masks, depths = tree_masks(_parents(n, g), device=DEV)
+    c = PagedRaggedCache(1, 2, 128, DEV) if paged else RaggedCache(1, 2, 128, DEV, attn_impl="specdec_b200")
+    if paged:
+        c.reserve(n)
+    c.set_tree(masks, depths)
+    q, k, v = (torch.randn(2, h, n, 128, generator=g).to(torch.bfloat16).to(DEV) for h in (4, 2, 2))
+    c.attn_mask(n, torch.bfloat16, valid=torch.tensor([n, n], device=DEV))
+    keys, values = c.layers[0].update(k, v)
+    out, _ = A.hf_attention(None, q, keys, values, None, scaling=0.125)
+    want = A.tree_attention(q, keys, values, c.lengths, masks, scale=0.125,
+                            block_table=c.block_table if paged else None)
+    assert torch.equal(out, want)
