@@ -8,7 +8,7 @@
 // threads touch the same bytes: the move is done in place, in one pass.  What it
 // has to move is tiny, so it is bound by the latency of its chain: path, page,
 // K / V, store.  Accept, move and lengths take 9.2 us in a graph for 32 rows and 36 layers
-// (19 MB read and written), 13.1 us for 64 rows and up to 8 nodes (76 MB).
+// (19 MB read and written), 13.4 us for 64 rows and up to 8 nodes (76 MB).
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -116,7 +116,6 @@ struct CommitParams {
   int path_len;
   const int64_t* n_acc;
   int N, B, H, C, cols;                      // cols: units of a (slot, head)
-  int n_bufs;
   int* err;
   void* bufs[COMMIT_BUFS];
 };
@@ -277,9 +276,9 @@ int sd_kv_commit_tree(void* const* bufs, int n_bufs, const int32_t* block_table,
   P.cols = row / unit;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   for (int i0 = 0; i0 < n_bufs; i0 += COMMIT_BUFS) {
-    P.n_bufs = std::min(n_bufs - i0, COMMIT_BUFS);
-    std::copy(bufs + i0, bufs + i0 + P.n_bufs, P.bufs);
-    const dim3 grid((unsigned)B, (unsigned)P.n_bufs);
+    const int here = std::min(n_bufs - i0, COMMIT_BUFS);
+    std::copy(bufs + i0, bufs + i0 + here, P.bufs);
+    const dim3 grid((unsigned)B, (unsigned)here);
     if (unit == 16) tree_move_kernel<uint4><<<grid, COMMIT_THREADS, 0, st>>>(P);
     else if (unit == 4) tree_move_kernel<uint32_t><<<grid, COMMIT_THREADS, 0, st>>>(P);
     else tree_move_kernel<uint16_t><<<grid, COMMIT_THREADS, 0, st>>>(P);
