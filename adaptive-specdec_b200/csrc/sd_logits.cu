@@ -6,23 +6,29 @@
 //   x = x > 0 ? x / r : x r;  x -= f c;  x -= p [c > 0];  x += bias;  x = -inf where not allowed
 //
 // What it has to move is a logit in and out (and, per row, 16 bits of history per
-// token; per position, one bit of mask), so HBM bounds it.  A CTA takes a chunk of
-// a row's vocabulary for up to LG_POS positions and passes over it once: 16-byte units
-// of the input, wherever they start in the row (rows of an odd vocabulary are aligned
-// differently), with -inf for what the mask bans; a unit that it bans whole is written
-// without being read.  Tokens that have a history (some thousand of 151936) get their
-// penalties on the way: the CTA takes the chunk's history to shared memory once for all
-// its positions, with a bit per token, and a thread loops over the bits of its unit.  The
+// token; per position, one bit of mask), so HBM bounds it while paths and biases touch few
+// entries.  A CTA takes a chunk of a row's vocabulary for up to LG_POS positions and passes
+// over it once: 16-byte units of the input, wherever they start in the row (rows of an odd
+// vocabulary are aligned differently), with -inf for what the mask bans; a unit that it bans
+// whole is written without being read.  Tokens that have a history (some thousand of 151936)
+// get their penalties on the way: the CTA takes the chunk's history to shared memory once for
+// all its positions, with a bit per token, and a thread loops over the bits of its unit.  The
 // tokens of the position's path and the biases are written over what the pass left; where
 // out is the logits themselves, they have been computed before the pass.
-// 320 positions of 151936 bf16 logits, 64 rows of history, masks, biases (220 MB): 47.0 us,
-// 832 positions (531 MB): 101 us; without history and biases 32 and 79, a copy's rate.  What is
-// left is the penalties' arithmetic (3 and 5 us), the history's way to shared memory ahead
-// of the pass, and the sparse entries behind it.  Measured and left: the tokens with a
-// history listed and written over the pass's output (47.3 and 111; 33 instead of 23 for fp32 rows
-// of 32003), units asked for a position ahead (51, 108: fewer CTAs fit), one run of positions
-// per resident CTA (60, 121), the history looked up in global memory for every unit
-// (60, 127) or for the units whose bits are set (53, 110).
+// 320 positions of 151936 bf16 logits, 64 rows of history, masks, 16 biases (220 MB): 46.9 us
+// (fp16 47.2, fp32 68.0), 832 positions (531 MB): 101 us; without history and biases 32 and
+// 79, a copy's rate.  What is left is the penalties' arithmetic (3 and 5 us), the history's way
+// to shared memory ahead of the pass, and the sparse entries behind it.  In place a CTA takes
+// one position, and so the history to shared memory for each: 73.8 and 162 us.
+// A touched entry costs a walk over its row's N tokens and M biases, so a position's cost
+// grows by (N + M)^2: 320 positions with 300 biases take 261 us, with 1024 2.5 ms, 832 positions
+// 703 us and 6.2 ms; 256 rows of 64 nodes over a vocabulary of 1000 (65 MB) 107 us without
+// biases, 909 us with 300.
+// Measured and left: the tokens with a history listed and written over the pass's output
+// (47.3 and 111; 33 instead of 23 for fp32 rows of 32003), units asked for a position ahead
+// (51, 108: fewer CTAs fit), one run of positions per resident CTA (60, 121), the history
+// looked up in global memory for every unit (60, 127) or for the units whose bits are set
+// (53, 110).
 #include <cuda_runtime.h>
 #include <math_constants.h>
 

@@ -7,7 +7,11 @@
 // keys in tiles of 128 ("pages", whether the cache is paged or not):
 //   S = Q K^T,  p = 2^(s - m) under a lazy running maximum m,  O += P V
 // Every page but the last few is seen whole by every node; in those that hold
-// the tree a row keeps the scores whose bit its node's mask has.
+// the tree a row keeps the scores whose bit its node's mask has.  The weights are
+// rounded to bf16 for P V (both operands of an MMA have one type, V's), each off by up to
+// 2^-8 of itself like the output: over 40 keys the error against 64 bits is 1.75e-3
+// (rms, relative) where 32-bit weights leave 1.65e-3, over 500 keys and more 1 % above
+// theirs or less.  Scores, maxima, sums, O and the pieces are 32 bits.
 // tree_tc_kernel    persistent, stream-K: the pages of all items lie end to end
 //                   and a CTA takes one contiguous run; an item that lies within a
 //                   run is written out, a cut one leaves (m, l, O) per piece
@@ -15,15 +19,17 @@
 //
 // What bounds it.  K and V are read once for all nodes and heads, so up to 128 query
 // rows it is HBM: 32 rows of 26 nodes over 128 to 4096 keys (294 MB) take 64 us in a graph,
-// 5.1 TB/s in the main kernel, and a start (plan, first loads) and join of 3 and 6 us;
-// 2 rows of 33 nodes over 30011 keys (246 MB) 50 to 59 us.  With two tiles it is the chain of S,
-// softmax and P V of a tile: 64 rows of 64 nodes over 512 to 8192 keys take 330 us, the
-// tensor pipe is busy 47 % of the time.  (The CUDA-core kernel: 20.2 ms.)
+// 5.0 TB/s in the main kernel, and a start (plan, first loads) and join of 3 and 6 us;
+// 2 rows of 33 nodes over 30011 keys (246 MB) 53 to 58 us.  With two tiles it is the chain of S,
+// softmax and P V of a tile: 64 rows of 64 nodes over 512 to 8192 keys take 337 us, the
+// tensor pipe is busy 47 % of the time.  (The CUDA-core kernel: 20.2 ms.)  These are bursts at
+// 1965 MHz.  Back to back for 0.4 s the power cap lowers the clock: 64 rows of 64 nodes then take
+// 404 us near 1500 MHz, 32 rows of 26 nodes 71 us at 1635 MHz.
 // One tile: S of the next page stands ready in TMEM's second buffer, and its 128 columns go
 // to two warpgroups, so that a page's softmax takes half as long.  Two tiles: S and O of both
 // fill TMEM, so S comes in halves of 64 keys (tt_issue_pair); whole pages of S took 422 us.
 // Heads of 64 halve the tiles and so put twice as many on their way: 32 rows of 26 nodes over
-// 2048 keys take 55 us (CUDA cores: 1.17 ms).
+// 2048 keys take 52 us (CUDA cores: 1.17 ms).
 // Queries come by TMA (the softmax threads' own loads waited 8000 cycles behind K and V),
 // the nodes' bits late and by asynchronous copies, as only the tree's pages look at them.
 #include <cuda_bf16.h>

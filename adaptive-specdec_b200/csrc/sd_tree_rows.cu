@@ -13,10 +13,13 @@
 // A key that a node does not see adds nothing to it whatever K and V hold there.
 // Bound by latency for few rows (so S grows while the machine has room), else by
 // the products: each K and V element meets TR_ROWS query rows.  8 rows of 9 nodes over up
-// to 460 fp32 keys of 64: 13.1 us, about eight dependent trips to memory; 32 rows of 26 nodes
-// over 2048 keys: 1.01 ms with fp32 heads of 64, 1.84 with 128, 1.17 with bf16 in heads of 64
-// or a little less (12 to 15 TFLOP/s).  Two CTAs per SM, at 128 registers a thread, beat one with more of K
-// and V on the way (1.03, 2.36, 1.33 ms) and three (1.10, 2.02, 1.46).
+// to 460 fp32 keys of 64: 12.4 to 14.1 us, about eight dependent trips to memory; 32 rows of 26
+// nodes over 2048 keys: 1.01 ms with fp32 heads of 64, 1.84 with 128, 1.17 with bf16 in heads of
+// 64 or a little less, 1.90, 2.04 and 2.15 with 80, 96 and 112 (9 to 15 TFLOP/s of the 74 that
+// the FMA pipes have).  P V is what holds it there: a (key, row) costs a shuffle and a test of its
+// weight for D / 32 multiply-adds of a lane, and in Q K a 16-byte load of q feeds four.  Two CTAs
+// per SM, at 128 registers a thread, beat one with more of K and V on the way (1.03, 2.36,
+// 1.33 ms) and three (1.10, 2.02, 1.46).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>

@@ -510,7 +510,8 @@ class SpecDecodeEngine:
 
         ``tree`` (number of children per node, level by level: (4, 2, 1)) drafts a tree
         per round instead of a chain of k (``controller`` and ``k_fixed`` are then not
-        given); ``n`` samples per prompt (rows of one prompt side by side: B * n lists);
+        given); ``n`` samples per prompt (rows of one prompt side by side: B * n lists;
+        a tree's attention reads their shared pages once per row, a chain's once);
         ``logprobs`` (0 or more alternatives, None: off) fills the stats'
         ``logprobs`` and ``top_logprobs`` per row and emitted token.
 

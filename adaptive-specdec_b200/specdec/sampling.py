@@ -450,10 +450,11 @@ def process_logits(logits, tokens=None, masks=None, history=None, repetition=Non
     ``repetition``, ``presence`` and ``frequency`` are numbers or float [B] tensors and
     need ``history``; ``allowed`` int32 [B or 1, L or 1, ceil(V / 32)].  Ids outside
     [0, V) are padding, biases of one id add up; at most BIAS_MAX per row and
-    TREE_MAX tokens.  repetition > 0.  Returns a new tensor, or ``out`` ([B, L, V]): the
-    logits themselves, or memory outside the span from their first to their last
-    entry; anything else is refused, and so is an ``out`` whose rows share entries
-    (an expanded tensor).  One launch, no synchronisation.
+    TREE_MAX tokens (made for some dozens of biases: with M of them and N tokens a
+    position's time grows by (M + N)^2).  repetition > 0.  Returns a new tensor, or
+    ``out`` ([B, L, V]): the logits themselves, or memory outside the span from their
+    first to their last entry; anything else is refused, and so is an ``out`` whose
+    rows share entries (an expanded tensor).  One launch, no synchronisation.
     """
     dev = logits.device
     if not logits.is_cuda:
