@@ -804,7 +804,9 @@ class PagedRaggedCache(RaggedCache):
         h = self._mirror().clone()
         h[rows] = 0
         self.pages.release(rows)
+        tree = self.tree
         self.set_lengths(h)
+        self.tree = tree                             # (the other rows' round goes on)
         self._push()
 
     def _last_readers(self, rows):

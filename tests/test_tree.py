@@ -467,3 +467,16 @@ def test_masks_of_parents_of_every_integer_type(dtype):
     want = [_masks_plain(t) for t in parents.tolist()]
     got = tree_masks(parents, device=DEV)
     assert _sets(got.masks) == [w[0] for w in want] and got.depths.tolist() == [w[1] for w in want]
+
+
+@gpu
+@pytest.mark.parametrize("device_pages", [False, True])
+def test_a_released_row_leaves_the_others_their_tree(device_pages):
+    masks, depths = tree_masks([-1, 0, 0, 1], device=DEV)
+    c = PagedRaggedCache(1, 2, 256, DEV, device_pages=device_pages)
+    c.reserve(6)
+    c.advance(6)
+    c.set_tree(masks, depths)
+    c.release([1])
+    assert c.tree is not None
+    assert c.positions(4).tolist() == [[6, 7, 7, 8], [0, 1, 1, 2]]
